@@ -6,6 +6,7 @@ sm_100 device.  There is no fallback: if the library is missing, `lib()` raises.
 """
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -118,6 +119,29 @@ SIGNATURES.update({
     "w8_lm_head_peer_argmax": (_i, [_p, _p, _p, _f, _i64, _i64, _i64, _i64, _i, _i, ctypes.POINTER(ctypes.c_void_p), _p,
                                  _p]),
 })
+
+SIGNATURES.update({
+    "w8_attention_tree": (_i, [ctypes.c_char_p, _p, _i64, _p]),
+    "w8_attention_tree_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i]),
+    "w8_cache_append": (_i, [ctypes.c_char_p, _p]),
+    "w8_cache_evict": (_i, [ctypes.c_char_p, _p, _i64, _p]),
+    "w8_cache_evict_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "w8_beam_select": (_i, [_p, _i, _i64, _i64, _p, _p, _i64, _f, _i64, _i64, _i64, _i64, _i, _p, _p, _p, _p, _i64,
+                            _p]),
+    "w8_beam_select_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "w8_cache_reorder": (_i, [_p, _i64, _p, _p, _i, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+})
+
+# The argument structs of w8a8_b200.h: 8-byte fields in the header's order, packed as bytes
+# (ctypes passes a bytes object by its address, which is cheaper than filling a Structure).
+ATTENTION_TREE_ARGS = struct.Struct("12Q33qd")
+CACHE_APPEND_ARGS = struct.Struct("11Q25q")
+CACHE_EVICT_ARGS = struct.Struct("8Q21q")
+
+# Element type codes.
+W8_BF16 = 0
+W8_FP16 = 1
+W8_FP32 = 2
 
 _lock = threading.Lock()
 _lib = None

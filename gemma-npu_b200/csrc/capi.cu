@@ -68,6 +68,8 @@ int num_sms(int* out) {
 int gemm_device_status(int clear, int* out);
 int attention_device_status(int clear, int* out);
 int peer_device_status(int clear, int* out);
+int tree_device_status(int clear, int* out);
+int cache_device_status(int clear, int* out);
 
 }  // namespace w8host
 
@@ -100,6 +102,18 @@ extern "C" int w8_device_status(int clear) {
   int vp = W8_OK;
   st = w8host::peer_device_status(clear, &vp);
   if (st != W8_OK) return st;
-  if (v != W8_OK) return v;
-  return va != W8_OK ? va : vp;
+  int vt = W8_OK, vc = W8_OK;
+  st = w8host::tree_device_status(clear, &vt);
+  if (st != W8_OK) return st;
+  st = w8host::cache_device_status(clear, &vc);
+  if (st != W8_OK) return st;
+  // A wait that gave up says more than an index that was skipped.
+  for (const int s : {v, va, vp, vt, vc})
+    if (s == W8_ERR_DEVICE_TIMEOUT) return s;
+  if (vt != W8_OK || vc != W8_OK)
+    w8host::set_error("a length or index in device memory lay outside its range (%s)",
+                      vt != W8_OK ? "attention over a cache" : "cache operation");
+  for (const int s : {v, va, vp, vt, vc})
+    if (s != W8_OK) return s;
+  return W8_OK;
 }

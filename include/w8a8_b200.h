@@ -34,6 +34,10 @@
  *   w8_gemm_qkv_norm_rope_tiled  the same, cos / sin in an 8-column tiled layout
  *   w8_attention_prefill_bf16 pipeline.py:139-180 (full_attention / sliding_attention)
  *   w8_attention_prefill_quant the same followed by pipeline.py:88-92 (k_attn_out)
+ *   w8_attention_tree       pipeline.py:133-180 behind cached keys, local_attn.py:44-83 (decode)
+ *   w8_cache_append         the DynamicCache update of pipeline.py:318-339
+ *   w8_cache_evict, w8_beam_select, w8_cache_reorder  no counterpart (the reference never
+ *                           evicts and decodes greedily, gemma_npu.py:291)
  */
 #ifndef W8A8_B200_H
 #define W8A8_B200_H
@@ -59,12 +63,19 @@ typedef struct CUstream_st* w8_stream_t;
 #define W8_B_KN 0 /* B is [K, N] row-major: the reference's mm_i8 layout (npu_kernels.py:59-60) */
 #define W8_B_NK 1 /* B is [N, K] row-major (K-major): the resident weight layout, shared with the GEMV */
 
+/* Element types of the decoding operators. */
+#define W8_BF16 0
+#define W8_FP16 1
+#define W8_FP32 2
+
 /* ---- diagnostics ------------------------------------------------------- */
 const char* w8_status_string(int status);
 /* Text of the last host-side error on this thread ("" if none). */
 const char* w8_last_error(void);
-/* Sticky device-side status (W8_OK or W8_ERR_DEVICE_TIMEOUT) of the current device;
- * synchronises the device first.  clear != 0 resets it to W8_OK. */
+/* Sticky device-side status of the current device: W8_OK, W8_ERR_DEVICE_TIMEOUT, or
+ * W8_ERR_INVALID_ARG when a length or index that a kernel read from device memory lay
+ * outside its range (it was skipped, not followed).  Synchronises the device first;
+ * clear != 0 resets it to W8_OK. */
 int w8_device_status(int clear);
 /* ABI version: (major << 16) | minor. */
 int w8_abi_version(void);
@@ -274,6 +285,120 @@ int w8_attention_prefill_mma_bf16(const uint16_t* q, int64_t q_head, int64_t q_t
                                   int64_t v_tok, uint16_t* o, int64_t o_head, int64_t o_tok, int64_t t,
                                   int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window,
                                   w8_stream_t stream);
+
+/* ---- decoding: attention over a cache, the cache, beam search -------------
+ * Caches are [batch, kv_heads, slots, head_dim] with unit stride along head_dim and any
+ * other strides; `lens` (int32 on the device) counts each sequence's committed slots, and
+ * what lies behind them is neither read nor written.  Lengths and indexes are device
+ * memory, so they are checked there: one outside its range is clamped or skipped and
+ * reported by w8_device_status.  Workspaces are the caller's, need no initialisation, and
+ * must not be shared by calls that may run at the same time. */
+
+typedef struct w8_attention_tree_args {
+  /* q [batch, heads, n, D], k / v the caches, k_new / v_new [batch, kv_heads, n, D], out like
+   * q: 16-byte aligned, strides (batch, head, token; elements) multiples of 8. */
+  const void *q, *k, *v, *k_new, *v_new;
+  void* out;
+  const int32_t* lens;   /* [batch] */
+  const uint8_t* tree;   /* [batch, n, n], nonzero at (i, j): new token i sees new token j; NULL: j <= i */
+  const int32_t* depth;  /* [batch, n]: the token's distance behind the cache; NULL: its index */
+  const float* weights;  /* [batch, kv_heads, slots] accumulated weights, or NULL with the two below */
+  float* weights_out;    /* the same shape; may be `weights` */
+  float* draft_weights;  /* [batch, kv_heads, n] contiguous: the new tokens' own */
+  int64_t q_stride[3], k_stride[3], v_stride[3], k_new_stride[3], v_new_stride[3], out_stride[3];
+  int64_t tree_stride[2], depth_stride, weights_stride[2], weights_out_stride[2]; /* batch 0 pitch: shared */
+  int64_t batch, heads, kv_heads, head_dim, slots, n_new, window, dtype; /* dtype: W8_BF16 or W8_FP16 */
+  double scale;
+} w8_attention_tree_args;
+
+/* Attention of n new tokens per sequence over its cache and over one another.  Token i of
+ * sequence b sees the committed slots j < lens[b] and the new tokens j with tree[b, i, j]
+ * (a drafted tree's ancestors and itself; NULL: a causal chunk, n = 1 a decode step), all
+ * cut to the last `window` positions when window > 0, where slot j stands at position j and
+ * new token i at lens[b] + depth[b, i]:
+ *   out = softmax(scale q . k) v over what it sees; zeros where it sees nothing.
+ * Grouped-query heads, head_dim 64, 128, 256 or 512, fp32 softmax and sums.  With weights:
+ * weights_out[b, c, j] = weights[b, c, j] + the probabilities of slot j summed over the
+ * group's heads and the n tokens (slots behind lens[b] are left alone), and draft_weights
+ * the same sums for the new tokens.  Values of a new token that some token must not see may
+ * be infinite or NaN; those of a committed slot that any token sees must be finite.
+ * Replaces full_attention / sliding_attention behind cached keys (pipeline.py:133-180) and
+ * the decode attention (local_attn.py:44-83). */
+int w8_attention_tree(const w8_attention_tree_args* args, void* workspace, int64_t workspace_bytes,
+                      w8_stream_t stream);
+/* Workspace of w8_attention_tree in bytes (16-byte aligned; -1 on a bad shape). */
+int64_t w8_attention_tree_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                          int64_t slots, int64_t n_new, int64_t window, int weights);
+
+typedef struct w8_cache_append_args {
+  void *k, *v;                 /* caches, rows of row_bytes (a multiple of 16), 16-byte aligned */
+  const void *k_new, *v_new;   /* [batch, kv_heads, n_new] rows */
+  const int32_t* lens;         /* [batch] */
+  const int32_t* path;         /* [batch, steps] indexes of new tokens, ended by a negative one; NULL: all */
+  float* weights;              /* [batch, kv_heads, slots] or NULL */
+  const float* draft_weights;  /* [batch, kv_heads, n_new] or NULL (new slots then start at 0) */
+  int32_t* positions;          /* [batch, kv_heads, slots] or NULL */
+  const int32_t* seen;         /* [batch]: position of the first appended token (with positions) */
+  int32_t* lens_out;           /* [batch], not lens itself */
+  int64_t k_stride[3], v_stride[3], k_new_stride[3], v_new_stride[3]; /* batch, head, row; bytes */
+  int64_t path_stride, weights_stride[2], draft_weights_stride[2], positions_stride[2]; /* elements */
+  int64_t batch, kv_heads, slots, n_new, steps, row_bytes;
+} w8_cache_append_args;
+
+/* Rows path[b, 0], path[b, 1], ... of the new keys and values go to the slots lens[b],
+ * lens[b] + 1, ... (a drafted tree's accepted path, or the new token itself), with their
+ * weights and positions; lens_out[b] = lens[b] + their number. */
+int w8_cache_append(const w8_cache_append_args* args, w8_stream_t stream);
+
+typedef struct w8_cache_evict_args {
+  void *k, *v;             /* caches, rows of row_bytes (a multiple of 16), 16-byte aligned */
+  const float* weights;    /* [batch, kv_heads, slots] */
+  const int32_t* positions; /* [batch, kv_heads, slots]: distinct and not negative within a head */
+  const int32_t* lens;     /* [batch] */
+  float* weights_out;      /* like weights; may be `weights` */
+  int32_t* positions_out;  /* like positions; may be `positions` */
+  int32_t* lens_out;       /* [batch], not lens itself */
+  int64_t k_stride[3], v_stride[3]; /* batch, head, slot; bytes */
+  int64_t weights_stride[2], positions_stride[2], weights_out_stride[2], positions_out_stride[2]; /* elements */
+  int64_t batch, kv_heads, slots, row_bytes, budget, sink, recent;
+} w8_cache_evict_args;
+
+/* Cuts every cache head of the sequences longer than `budget` to `budget` slots: those at
+ * positions below `sink`, the `recent` last positions, and of the others the ones with the
+ * largest accumulated weight (ties to the lower slot; NaN counts as -inf).  The i-th kept
+ * slot at or behind `budget` moves into the i-th evicted slot below it, in place: nothing
+ * else moves, and attention does not depend on the slots' order.  weights_out and
+ * positions_out describe the slots after the cut (0 and -1 behind the last), lens_out[b] =
+ * min(lens[b], budget).  sink + recent <= budget. */
+int w8_cache_evict(const w8_cache_evict_args* args, void* workspace, int64_t workspace_bytes, w8_stream_t stream);
+int64_t w8_cache_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t slots, int64_t budget);
+
+/* Beam search's selection: of all (beam, token) of a sequence the n with the largest
+ *   total = scores[beam] + y - log sum e^y,  y = cap tanh(logit / cap) (cap <= 0: the logit),
+ * best first, equal totals to the lower beam, then the lower token.  logits [batch, beams,
+ * vocab] of `dtype` with strides stride_b, stride_k (elements); a logit of -inf is an
+ * impossible token.  A finished beam's only continuation is `pad`, at an unchanged score; a
+ * beam whose score or log sum is not finite has none: impossible continuations have total
+ * -inf and come last, in their own order.  slot_order != 0 (n = beams): the best
+ * continuation of a surviving beam stands in that beam's slot and the others fill the free
+ * slots, best first, so that w8_cache_reorder moves as little as can be.  At most 32 beams
+ * and 64 continuations. */
+int w8_beam_select(const void* logits, int dtype, int64_t stride_b, int64_t stride_k, const float* scores,
+                   const uint8_t* finished, int64_t pad, float cap, int64_t batch, int64_t beams, int64_t vocab,
+                   int64_t n, int slot_order, float* out_scores, int64_t* out_beam, int64_t* out_token,
+                   void* workspace, int64_t workspace_bytes, w8_stream_t stream);
+int64_t w8_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t n);
+
+/* The beams' states follow their parents, in place: in each of the `count` tensors
+ * [groups * beams, heads, slots] of rows of row_bytes (strides row, head, slot in bytes, the
+ * same for all; 16-byte aligned) state i of a group takes the first lens[parent] slots
+ * (NULL: all) of state beam[i] of its group.  Any map of beams is right, the same parent
+ * twice and swaps included.  beam is int64 (beam_i64 != 0) or int32 [groups, beams], lens
+ * [groups * beams].  `tensors` and `strides` are host arrays, read before the call returns;
+ * at most 32 beams. */
+int w8_cache_reorder(void* const* tensors, int64_t count, const int64_t* strides, const void* beam, int beam_i64,
+                     const int32_t* lens, int64_t groups, int64_t beams, int64_t heads, int64_t slots,
+                     int64_t row_bytes, w8_stream_t stream);
 
 /* ---- quantisation ------------------------------------------------------ */
 

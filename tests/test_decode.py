@@ -1,0 +1,87 @@
+"""Host-side checks of the decoding operators, without a GPU: the wrappers refuse host
+tensors, and the C ABI answers bad arguments with status codes before any CUDA call."""
+import pytest
+import torch
+
+import gemma_npu_b200 as w8
+from gemma_npu_b200 import _lib
+
+
+def tree_args(**change):
+    """The packed arguments of a small valid-looking attention_tree call (pointers 256 apart)."""
+    p = {name: 4096 + 256 * i for i, name in enumerate(
+        ["q", "k", "v", "k_new", "v_new", "out", "lens", "tree", "depth", "weights", "weights_out", "draft_weights"])}
+    p.update(tree=0, depth=0, weights=0, weights_out=0, draft_weights=0)
+    s = {name: (64, 64, 64) for name in ["qs", "ks", "vs", "kns", "vns", "os"]}
+    n = dict(B=1, H=4, KV=2, D=64, S=16, N=2, window=0, dtype=_lib.W8_BF16, scale=1.0)
+    for name, v in change.items():
+        next(d for d in (p, s, n) if name in d)[name] = v
+    return _lib.ATTENTION_TREE_ARGS.pack(*p.values(), *(x for v in s.values() for x in v), 4, 2, 0, 0, 0, 0, 0,
+                                         *n.values())
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(H=5), _lib.W8_ERR_INVALID_ARG), (dict(B=-1), _lib.W8_ERR_INVALID_ARG), (dict(window=-1), _lib.W8_ERR_INVALID_ARG),
+    (dict(D=96), _lib.W8_ERR_UNSUPPORTED), (dict(dtype=_lib.W8_FP32), _lib.W8_ERR_INVALID_ARG), (dict(q=0), _lib.W8_ERR_INVALID_ARG),
+    (dict(lens=0), _lib.W8_ERR_INVALID_ARG), (dict(k=0), _lib.W8_ERR_INVALID_ARG), (dict(tree=4096, window=3), _lib.W8_ERR_INVALID_ARG),
+    (dict(weights=4096), _lib.W8_ERR_INVALID_ARG), (dict(k=4104), _lib.W8_ERR_ALIGNMENT), (dict(ks=(64, 64, 60)), _lib.W8_ERR_ALIGNMENT),
+    (dict(N=65537), _lib.W8_ERR_INVALID_ARG)])
+def test_attention_tree_refuses(change, status):
+    assert _lib.lib().w8_attention_tree(tree_args(**change), None, 0, None) == status
+
+
+def test_empty_attention_is_a_no_op():
+    assert _lib.lib().w8_attention_tree(tree_args(B=0), None, 0, None) == _lib.W8_OK
+    assert _lib.lib().w8_attention_tree(tree_args(N=0), None, 0, None) == _lib.W8_OK
+
+
+def test_struct_sizes_match_the_header():
+    """8-byte fields, in number as the header declares them."""
+    import re
+
+    text = re.sub(r"/\*.*?\*/", "", open(_lib.HEADER_PATH).read(), flags=re.S)
+    for name, packed in (("w8_attention_tree_args", _lib.ATTENTION_TREE_ARGS), ("w8_cache_append_args", _lib.CACHE_APPEND_ARGS),
+                         ("w8_cache_evict_args", _lib.CACHE_EVICT_ARGS)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1)
+        fields = 0
+        for decl in body.split(";"):
+            for item in decl.split(","):
+                if item.strip():
+                    m = re.search(r"\[(\d+)\]", item)
+                    fields += int(m.group(1)) if m else 1
+        assert packed.size == 8 * fields, name
+
+
+def test_evict_refuses():
+    def args(budget=4, sink=0, recent=0, lens=4096, lens_out=8192, row=128):
+        return _lib.CACHE_EVICT_ARGS.pack(4096, 4096, 4096, 4096, lens, 4096, 4096, lens_out, *[128] * 6, *[16] * 8, 1, 1, 16,
+                                          row, budget, sink, recent)
+
+    run = _lib.lib().w8_cache_evict
+    for a in (args(budget=0), args(sink=-1), args(sink=2, recent=3), args(lens=0), args(lens_out=4096)):
+        assert run(a, 4096, 1 << 20, None) == _lib.W8_ERR_INVALID_ARG
+    assert run(args(row=24), 4096, 1 << 20, None) == _lib.W8_ERR_ALIGNMENT
+    assert run(args(), 4096, 8, None) == _lib.W8_ERR_INVALID_ARG
+    assert b"workspace" in _lib.lib().w8_last_error()
+
+
+def test_select_refuses():
+    def run(beams=2, vocab=10, n=2, pad=0, dtype=_lib.W8_FP32, slot=0, logits=4096):
+        return _lib.lib().w8_beam_select(logits, dtype, vocab * beams, vocab, 4096, None, pad, 0.0, 1, beams, vocab, n, slot,
+                                         4096, 4096, 4096, 4096, 1 << 20, None)
+
+    for kw in (dict(n=21), dict(n=0), dict(pad=10), dict(pad=-1), dict(dtype=3), dict(slot=1, n=3), dict(logits=None)):
+        assert run(**kw) == _lib.W8_ERR_INVALID_ARG, kw
+    assert run(beams=33) == _lib.W8_ERR_UNSUPPORTED and run(n=65, vocab=100) == _lib.W8_ERR_UNSUPPORTED
+    assert run(logits=4098) == _lib.W8_ERR_ALIGNMENT
+
+
+def test_wrappers_refuse_host_tensors():
+    x = torch.zeros((1, 1, 4, 64), dtype=torch.bfloat16)
+    ln = torch.zeros(1, dtype=torch.int32)
+    w = torch.zeros((1, 1, 4))
+    for call in (lambda: w8.attention_tree(x, x, x, ln, x, x), lambda: w8.cache_append(x, x, x, x, ln),
+                 lambda: w8.cache_evict(x, x, w, w.int(), ln, 2), lambda: w8.beam_select(w, w[0]),
+                 lambda: w8.cache_reorder(x, torch.zeros((1, 1), dtype=torch.int64))):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
