@@ -133,10 +133,14 @@ SIGNATURES.update({
 })
 
 # The argument structs of w8a8_b200.h: 8-byte fields in the header's order, packed as bytes
-# (ctypes passes a bytes object by its address, which is cheaper than filling a Structure).
-ATTENTION_TREE_ARGS = struct.Struct("12Q33qd")
-CACHE_APPEND_ARGS = struct.Struct("11Q25q")
-CACHE_EVICT_ARGS = struct.Struct("8Q21q")
+# (ctypes passes a bytes object by its address, which is cheaper than filling a Structure):
+# the pointers, which change from call to call, then strides and sizes, which seldom do.
+ATTENTION_TREE_POINTERS = struct.Struct("12Q")
+ATTENTION_TREE_TAIL = struct.Struct("33qd")
+CACHE_APPEND_POINTERS = struct.Struct("11Q")
+CACHE_APPEND_TAIL = struct.Struct("25q")
+CACHE_EVICT_POINTERS = struct.Struct("8Q")
+CACHE_EVICT_TAIL = struct.Struct("21q")
 
 # Element type codes.
 W8_BF16 = 0

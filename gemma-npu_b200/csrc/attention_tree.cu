@@ -19,95 +19,16 @@
 // columns, so both K and V fragments are read from shared memory once per row tile, and P
 // and the row maxima cross warps through shared memory.  The key axis is split over CTAs
 // until the GPU is full; partial (m, l, O) are joined by attn_tree_combine_kernel.
-#include "common.cuh"
-
-#include <cuda_fp16.h>
+#include "attention_tree.cuh"
 
 #include <algorithm>
 
 namespace w8 {
 
-__device__ int g_tree_status = 0;
-
 constexpr int kTreeThreads = 256;
 constexpr int kTreeWarps = 8;
 constexpr int kTreeBN = 64;          // keys per tile
 constexpr int kTreePPitch = 72;      // P row pitch (elements): 144 bytes, conflict-free ldmatrix
-constexpr int kTreeMaxSplits = 256;
-
-struct TreeArgs {
-  const uint16_t *q, *k, *v, *kn, *vn;
-  uint16_t* o;
-  const int* lens;
-  const uint8_t* tree;   // [B, N, N] or null: causal
-  const int* depth;      // [B, N] or null: the token's index
-  int64_t q_b, q_h, q_t, k_b, k_h, k_s, v_b, v_h, v_s, kn_b, kn_h, kn_t, vn_b, vn_h, vn_t, o_b, o_h, o_t;
-  int64_t tree_b, tree_i, depth_b;
-  int batch, kv_heads, group, n, slots, window;
-  float scale_log2;      // scale * log2(e): scores in log2 units
-  int row_tiles, splits;
-  float* part_o;         // [item][split][BM][D] fp32, item = (b * kv_heads + c) * row_tiles + rt
-  float2* part_ml;       // [item][split][BM]
-  float* lse;            // [b * kv_heads + c][R] (log2 units) when the weights are wanted
-  float* scores;         // [b * kv_heads + c][R][score_pitch] (log2 units), slots then drafts
-  int64_t score_pitch;
-  const float* w_in;
-  float* w_out;
-  float* w_new;          // [B, KV, N]
-  int64_t wi_b, wi_h, wo_b, wo_h;
-};
-
-__device__ __forceinline__ float ex2_tree(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// The committed length of sequence b, kept inside the cache whatever the memory holds.
-__device__ __forceinline__ int tree_len(const TreeArgs& a, int b) {
-  const int n = a.lens[b];
-  if (n < 0 || n > a.slots) {
-    atomicExch(&g_tree_status, W8_ERR_INVALID_ARG);
-    return n < 0 ? 0 : a.slots;
-  }
-  return n;
-}
-
-// First committed slot that token i at `depth` sees under the window (0: all of them).
-__device__ __forceinline__ int tree_first(const TreeArgs& a, int len, int depth) {
-  if (a.window <= 0) return 0;
-  const int64_t f = static_cast<int64_t>(len) + depth - a.window + 1;
-  return f <= 0 ? 0 : (f >= len ? len : static_cast<int>(f));
-}
-
-__device__ __forceinline__ int tree_depth(const TreeArgs& a, int b, int i) {
-  return a.depth != nullptr ? a.depth[b * a.depth_b + i] : i;
-}
-
-// Whether token i sees new token j (both < n).
-__device__ __forceinline__ bool tree_sees(const TreeArgs& a, int b, int i, int j, int depth_i) {
-  const bool on = a.tree != nullptr ? a.tree[b * a.tree_b + i * a.tree_i + j] != 0 : j <= i;
-  if (!on || a.window <= 0) return on;
-  return static_cast<int64_t>(tree_depth(a, b, j)) > static_cast<int64_t>(depth_i) - a.window;
-}
-
-// Tiles of one row tile: committed tiles [c0, c1), then draft tiles [0, nd).
-struct TreeSpan {
-  int c0, c1, nd;
-};
-__device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int len, int rt, int bm) {
-  TreeSpan s;
-  const int rows = a.group * a.n;
-  const int i0 = rt * bm / a.group, i1 = min((rt + 1) * bm, rows) - 1;
-  // Without given depths the first row's token is the shallowest; with them, 0 is a bound.
-  s.c0 = tree_first(a, len, a.depth != nullptr ? 0 : i0) / kTreeBN;
-  s.c1 = (len + kTreeBN - 1) / kTreeBN;
-  // A causal chunk's row tile needs the new keys up to its last token only.
-  const int last = a.tree != nullptr ? a.n - 1 : i1 / a.group;
-  s.nd = last / kTreeBN + 1;
-  if (s.c0 > s.c1) s.c0 = s.c1;
-  return s;
-}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;
@@ -150,35 +71,6 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&p);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  __half2 p = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&p);
-}
-template <typename T>
-__device__ __forceinline__ float tree_f32(uint16_t bits);
-template <>
-__device__ __forceinline__ float tree_f32<__nv_bfloat16>(uint16_t bits) {
-  return __uint_as_float(static_cast<uint32_t>(bits) << 16);
-}
-template <>
-__device__ __forceinline__ float tree_f32<__half>(uint16_t bits) {
-  return __half2float(__ushort_as_half(bits));
-}
-// Infinity or NaN: every exponent bit set.
-template <typename T>
-__device__ __forceinline__ bool tree_nonfinite(uint32_t bits) {
-  constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, __half) ? 0x7C00u : 0x7F80u;
-  return (bits & e) == e;
-}
-
 template <int D, int MT>
 struct TreeCfg {
   static constexpr int kBM = 16 * MT;
@@ -209,7 +101,7 @@ __global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs 
   pdl_launch_dependents();
   pdl_wait();
   const int len = tree_len(a, b);
-  const TreeSpan span = tree_span(a, len, rt, BM);
+  const TreeSpan span = tree_span(a, len, rt, BM, kTreeBN);
   const int nc = span.c1 - span.c0, nt = nc + span.nd;
   const int t0 = static_cast<int>(static_cast<int64_t>(nt) * split / a.splits);
   const int t1 = static_cast<int>(static_cast<int64_t>(nt) * (split + 1) / a.splits);
@@ -609,22 +501,31 @@ namespace w8host {
 
 int require_sm100(int* device);
 
+int tree_tc(const w8::TreeArgs& a, bool half, int64_t d, int64_t items, int device, cudaStream_t stream);
+int tree_tc_device_status(int clear, int* out);
+
 // How a call is cut: rows per tile, row tiles and key splits.
 struct TreePlan {
+  bool tc;  // the tcgen05 schedule (attention_tree_tc.cu)
   int bm, row_tiles, splits;
   int64_t items;
 };
 
+// More than 32 rows a cache head at head_dim >= 128 go to the tcgen05 schedule (`tma`: its
+// maps can describe the tensors), whose tiles take 256 rows; fewer to mma.sync tiles of 16
+// or 32, which a split key axis spreads over more SMs.
 static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t n, int64_t d, int64_t slots,
-                          int64_t window, int sms) {
+                          int64_t window, int sms, bool tma) {
   TreePlan p;
   const int64_t rows = group * n;
-  p.bm = rows > 16 && d <= 256 ? 32 : 16;
+  p.tc = tma && rows > 32 && d >= 128;
+  p.bm = p.tc ? 256 : rows > 16 && d <= 256 ? 32 : 16;
   p.row_tiles = static_cast<int>((rows + p.bm - 1) / p.bm);
   p.items = batch * kv_heads * p.row_tiles;
-  const int64_t keys = window > 0 ? std::min(slots, window + n + w8::kTreeBN) : slots;
-  const int64_t tiles = (keys + w8::kTreeBN - 1) / w8::kTreeBN + (n + w8::kTreeBN - 1) / w8::kTreeBN;
-  const int64_t want = static_cast<int64_t>(sms) * (d == 512 ? 1 : 2);
+  const int64_t bn = p.tc ? 128 : w8::kTreeBN;
+  const int64_t keys = window > 0 ? std::min(slots, window + n + bn) : slots;
+  const int64_t tiles = (keys + bn - 1) / bn + (n + bn - 1) / bn;
+  const int64_t want = p.tc ? (d == 512 ? sms / 4 : sms / 2) : static_cast<int64_t>(sms) * (d == 512 ? 1 : 2);
   p.splits = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>({want / std::max<int64_t>(p.items, 1), tiles, w8::kTreeMaxSplits})));
   return p;
@@ -700,7 +601,9 @@ static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStr
   const int64_t blocks = p.items * p.splits;
   W8_CHECK_ARG(blocks < (1ll << 31), "too many row tiles");
   int st;
-  if constexpr (D <= 256)
+  if (p.tc)
+    st = tree_tc(a, __is_same(T, __half), D, p.items, device, stream);
+  else if constexpr (D <= 256)
     st = p.bm == 32 ? tree_main<T, D, 2>(a, blocks, device, stream) : tree_main<T, D, 1>(a, blocks, device, stream);
   else
     st = tree_main<T, D, 1>(a, blocks, device, stream);
@@ -729,7 +632,10 @@ int tree_device_status(int clear, int* out) {
     const int zero = 0;
     W8_CUDA_TRY(cudaMemcpyToSymbol(w8::g_tree_status, &zero, sizeof(int)));
   }
-  *out = v;
+  int vt = W8_OK;
+  const int st = tree_tc_device_status(clear, &vt);
+  if (st != W8_OK) return st;
+  *out = v == W8_OK || vt == W8_ERR_DEVICE_TIMEOUT ? vt : v;
   return W8_OK;
 }
 
@@ -741,8 +647,13 @@ extern "C" int64_t w8_attention_tree_workspace_bytes(int64_t batch, int64_t head
   if (tree_shape(batch, heads, kv_heads, head_dim, slots, n_new, window) != W8_OK) return -1;
   int sms = 148;
   if (num_sms(&sms) != W8_OK) sms = 148;
-  const TreePlan p = tree_plan(batch, kv_heads, heads / kv_heads, n_new, head_dim, slots, window, sms);
-  return tree_ws(p, batch, kv_heads, heads / kv_heads, n_new, head_dim, slots, weights != 0).total;
+  // The larger of the two schedules' needs: which one runs depends on the strides too.
+  int64_t most = 0;
+  for (const bool tma : {false, true}) {
+    const TreePlan p = tree_plan(batch, kv_heads, heads / kv_heads, n_new, head_dim, slots, window, sms, tma);
+    most = std::max(most, tree_ws(p, batch, kv_heads, heads / kv_heads, n_new, head_dim, slots, weights != 0).total);
+  }
+  return most;
 }
 
 extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspace, int64_t workspace_bytes,
@@ -754,6 +665,9 @@ extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspa
   if (st != W8_OK) return st;
   W8_CHECK_ARG(x.dtype == W8_BF16 || x.dtype == W8_FP16, "dtype must be W8_BF16 or W8_FP16");
   if (x.batch == 0 || x.n_new == 0) return W8_OK;
+  // (positive in the kernels' fp32 log2 units too: a masked score is -inf times it)
+  const float scale_log2 = static_cast<float>(x.scale * 1.4426950408889634);
+  W8_CHECK_ARG(scale_log2 > 0.f && scale_log2 < 3e38f, "scale must be positive and finite");
   W8_CHECK_ARG(x.q && x.k_new && x.v_new && x.out && x.lens, "null pointer");
   W8_CHECK_ARG(x.slots == 0 || (x.k && x.v), "null cache");
   W8_CHECK_ARG(x.tree == nullptr || x.window == 0 || x.depth != nullptr,
@@ -774,7 +688,14 @@ extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspa
   st = num_sms(&sms);
   if (st != W8_OK) return st;
   const int64_t group = x.heads / x.kv_heads;
-  const TreePlan p = tree_plan(x.batch, x.kv_heads, group, x.n_new, x.head_dim, x.slots, x.window, sms);
+  // TMA maps take no stride of 0 (an expanded view: beams that share one prompt's cache).
+  const int64_t sizes[4][3] = {{x.batch, x.kv_heads, x.slots}, {x.batch, x.kv_heads, x.slots},
+                               {x.batch, x.kv_heads, x.n_new}, {x.batch, x.kv_heads, x.n_new}};
+  bool tma = true;
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 3; ++j)
+      if (sizes[i][j] > 1 && (strides[i + 1][j] <= 0 || strides[i + 1][j] >= (1ll << 38))) tma = false;
+  const TreePlan p = tree_plan(x.batch, x.kv_heads, group, x.n_new, x.head_dim, x.slots, x.window, sms, tma);
   const TreeWs w = tree_ws(p, x.batch, x.kv_heads, group, x.n_new, x.head_dim, x.slots, weights);
   W8_CHECK_ARG(w.total == 0 || (workspace != nullptr && workspace_bytes >= w.total),
                "workspace of %lld bytes needed (got %lld)", (long long)w.total, (long long)workspace_bytes);
@@ -805,7 +726,7 @@ extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspa
   a.n = static_cast<int>(x.n_new);
   a.slots = static_cast<int>(x.slots);
   a.window = static_cast<int>(x.window);
-  a.scale_log2 = static_cast<float>(x.scale * 1.4426950408889634);
+  a.scale_log2 = scale_log2;
   a.row_tiles = p.row_tiles;
   a.splits = p.splits;
   uint8_t* ws = static_cast<uint8_t*>(workspace);

@@ -35,25 +35,60 @@ from .kernels import _need
 _DTYPES = {torch.bfloat16: _lib.W8_BF16, torch.float16: _lib.W8_FP16, torch.float32: _lib.W8_FP32}
 _ORDERS = ("score", "slot")
 
+# Checked layouts.  A decode step makes the same few calls over and over, and checking a dozen
+# tensors in Python costs more than a short kernel runs: what the checks depend on (shapes,
+# strides, dtypes, devices, the plain arguments) is looked up here, and only a layout that was
+# never seen is checked in full.  Addresses and values are no part of it: pointers and their
+# alignment go to the C ABI with every call.
+_CHECKED = {}
+_MOST_CHECKED = 4096
+
+
+def _layout(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _known(check, key, *args):
+    """check(*args) for a layout key, remembered; a key that is None is never remembered."""
+    plan = _CHECKED.get(key) if key is not None else None
+    if plan is None:
+        plan = check(*args)
+        if key is not None:
+            if len(_CHECKED) >= _MOST_CHECKED:
+                _CHECKED.clear()
+            _CHECKED[key] = plan
+    return plan
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
 
 def _shape(t, name, shape, dtype, device):
-    """A CUDA tensor of this dtype and shape on `device`; returns its data pointer."""
+    """A tensor of this dtype and shape on `device`."""
     _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
     _need(t.dtype == dtype, f"{name} must be {dtype} (got {t.dtype})")
     _need(t.shape == shape, f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
     _need(t.device == device, f"{name} must be on {device} (got {t.device})")
-    return t.data_ptr()
+
+
+def _vector(t, name, shape, dtype, device):
+    _shape(t, name, shape, dtype, device)
+    _need(t.is_contiguous(), f"{name} must be contiguous")
+
+
+def _per_slot(t, name, shape, dtype, device):
+    """[batch, kv_heads, n] with unit stride along n: its other strides."""
+    _shape(t, name, shape, dtype, device)
+    _need(t.stride(2) == 1 or shape[2] <= 1, f"{name} must have unit stride along its last dimension")
+    return t.stride()[:2]
 
 
 def _rows4(t, name, dtype, device):
-    """A 4-D tensor of rows with unit stride along the last dimension: (pointer, strides)."""
+    """A 4-D tensor of rows with unit stride along the last dimension: its other strides."""
     _need(isinstance(t, torch.Tensor) and t.dim() == 4, f"{name} must be a 4-D tensor")
     _need(t.dtype == dtype, f"{name} must be {dtype} (got {t.dtype})")
     _need(t.device == device, f"{name} must be on {device} (got {t.device})")
-    return t.data_ptr(), _strides4(t, name)
-
-
-def _strides4(t, name):
     s0, s1, s2, s3 = t.stride()
     n0, n1, n2, n3 = t.shape
     _need(s3 == 1 or n3 <= 1, f"{name} must have unit stride along its last dimension")
@@ -67,24 +102,73 @@ def _cuda(t, name):
     return t.device
 
 
-def _call(device, fn, *args):
+def _run(device, fn, *args):
     """One C-ABI call on `device`'s current stream, with that device current."""
-    if torch.cuda.current_device() == device.index:
-        _lib.call(fn, *args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            _lib.call(fn, *args, torch.cuda.current_stream(device).cuda_stream)
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, fn.__name__)
 
 
-def _workspace(device, nbytes, what):
-    _need(nbytes >= 0, what)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+def _integer(v, name):
+    _need(isinstance(v, int), f"{name} must be an integer (got {v!r})")
 
 
 def _disjoint_rows(t, name, n):
     """The first n dimensions of a tensor that is written must not overlap themselves."""
     for size, stride in zip(t.shape[:n], t.stride()[:n]):
         _need(size <= 1 or stride != 0, f"{name} is written and must not be an expanded view")
+
+
+def _check_tree(q, k, v, lens, k_new, v_new, tree, depth, window, scale, out, weights, weights_out, draft_weights):
+    dev = _cuda(q, "q")
+    dt = q.dtype
+    _need(dt in (torch.bfloat16, torch.float16), f"q must be bfloat16 or float16 (got {dt})")
+    strides = [x for t, name in ((q, "q"), (k, "k"), (v, "v"), (k_new, "k_new"), (v_new, "v_new"))
+               for x in _rows4(t, name, dt, dev)]
+    B, H, N, D = q.shape
+    KV, S = k.shape[1], k.shape[2]
+    _need(k.shape == (B, KV, S, D) and v.shape == k.shape, "k and v must be [B, KV, S, D] with q's B and D")
+    _need(k_new.shape == (B, KV, N, D) and v_new.shape == k_new.shape, "k_new and v_new must be [B, KV, N, D]")
+    _need(KV >= 1 and H % KV == 0, f"H = {H} must be a multiple of KV = {KV}")
+    _vector(lens, "lens", (B,), torch.int32, dev)
+    ts, ds = (0, 0), 0
+    if tree is not None:
+        _need(isinstance(tree, torch.Tensor) and tree.dim() in (2, 3), "tree must be [N, N] or [B, N, N]")
+        _shape(tree, "tree", (N, N) if tree.dim() == 2 else (B, N, N), torch.bool, dev)
+        _need(tree.stride(-1) == 1 or N <= 1, "tree must have unit stride along its last dimension")
+        ts = (tree.stride(0) if tree.dim() == 3 else 0, tree.stride(-2))
+    if depth is not None:
+        _need(isinstance(depth, torch.Tensor) and depth.dim() in (1, 2), "depth must be [N] or [B, N]")
+        _shape(depth, "depth", (N,) if depth.dim() == 1 else (B, N), torch.int32, dev)
+        _need(depth.stride(-1) == 1 or N <= 1, "depth must have unit stride along its last dimension")
+        ds = depth.stride(0) if depth.dim() == 2 else 0
+    _integer(window, "window")
+    _need(tree is None or window == 0 or depth is not None, "a tree with a window needs the tokens' depths")
+    if out is not None:
+        _need(out.shape == q.shape, f"out must be {tuple(q.shape)}")
+        _disjoint_rows(out, "out", 3)
+        strides += _rows4(out, "out", dt, dev)
+    else:
+        strides += (H * N * D, N * D, D)
+    ws, wos = (0, 0), (0, 0)
+    if weights is not None:
+        ws = _per_slot(weights, "weights", (B, KV, S), torch.float32, dev)
+        to = weights if weights_out is None else weights_out
+        wos = _per_slot(to, "weights_out", (B, KV, S), torch.float32, dev)
+        _disjoint_rows(to, "weights_out", 2)
+        if draft_weights is not None:
+            _vector(draft_weights, "draft_weights", (B, KV, N), torch.float32, dev)
+    else:
+        _need(weights_out is None and draft_weights is None, "weights_out and draft_weights go with weights")
+    # (a negative size is a shape that the call itself refuses, with its reason)
+    nbytes = max(0, _lib.lib().w8_attention_tree_workspace_bytes(B, H, KV, D, S, N, window, weights is not None))
+    tail = _lib.ATTENTION_TREE_TAIL.pack(*strides, *ts, ds, *ws, *wos, B, H, KV, D, S, N, window, _DTYPES[dt], scale)
+    return dev, (B, H, N, D), (B, KV, N), nbytes, tail, _lib.lib().w8_attention_tree
 
 
 def attention_tree(q, k, v, lens, k_new, v_new, tree=None, depth=None, window=0, scale=1.0, out=None, weights=None,
@@ -102,70 +186,69 @@ def attention_tree(q, k, v, lens, k_new, v_new, tree=None, depth=None, window=0,
     at position j, new token i at lens + depth[i], depth int32 [N] or [B, N] (its number of
     ancestors; needed with a tree, i without one).
 
-    Returns out [B, H, N, D] = softmax(scale * q k^T) v, zeros where a token sees nothing.
+    Returns out [B, H, N, D] = softmax(scale * q k^T) v (scale > 0), zeros where a token sees nothing.
     With `weights` fp32 [B, KV, S] returns (out, weights_out, draft_weights): weights_out =
     weights plus the probabilities of each committed slot summed over the group's heads and
     the N tokens (in place unless weights_out is given; slots behind lens are left alone),
     draft_weights fp32 [B, KV, N] the same sums of the new tokens."""
-    dev = _cuda(q, "q")
-    dt = q.dtype
-    _need(dt in (torch.bfloat16, torch.float16), f"q must be bfloat16 or float16 (got {dt})")
-    qp, qs = _rows4(q, "q", dt, dev)
-    kp, ks = _rows4(k, "k", dt, dev)
-    vp, vs = _rows4(v, "v", dt, dev)
-    knp, kns = _rows4(k_new, "k_new", dt, dev)
-    vnp, vns = _rows4(v_new, "v_new", dt, dev)
-    B, H, N, D = q.shape
-    KV, S = k.shape[1], k.shape[2]
-    _need(k.shape == (B, KV, S, D) and v.shape == k.shape, "k and v must be [B, KV, S, D] with q's B and D")
-    _need(k_new.shape == (B, KV, N, D) and v_new.shape == k_new.shape, "k_new and v_new must be [B, KV, N, D]")
-    _need(KV >= 1 and H % KV == 0, f"H = {H} must be a multiple of KV = {KV}")
-    lp = _shape(lens, "lens", (B,), torch.int32, dev)
-    _need(lens.is_contiguous(), "lens must be contiguous")
-    tp, ts, dp, ds = 0, (0, 0), 0, 0
-    if tree is not None:
-        _need(isinstance(tree, torch.Tensor) and tree.dim() in (2, 3), "tree must be [N, N] or [B, N, N]")
-        tp = _shape(tree, "tree", (N, N) if tree.dim() == 2 else (B, N, N), torch.bool, dev)
-        _need(tree.stride(-1) == 1 or N <= 1, "tree must have unit stride along its last dimension")
-        ts = (tree.stride(0) if tree.dim() == 3 else 0, tree.stride(-2))
-    if depth is not None:
-        _need(isinstance(depth, torch.Tensor) and depth.dim() in (1, 2), "depth must be [N] or [B, N]")
-        dp = _shape(depth, "depth", (N,) if depth.dim() == 1 else (B, N), torch.int32, dev)
-        _need(depth.stride(-1) == 1 or N <= 1, "depth must have unit stride along its last dimension")
-        ds = depth.stride(0) if depth.dim() == 2 else 0
-    _need(tree is None or window == 0 or depth is not None, "a tree with a window needs the tokens' depths")
+    try:
+        key = ("attention_tree", _layout(q), _layout(k), _layout(v), _layout(lens), _layout(k_new), _layout(v_new),
+               _layout(tree), _layout(depth), window, scale, _layout(out), _layout(weights), _layout(weights_out),
+               _layout(draft_weights))
+    except (AttributeError, TypeError):
+        key = None
+    dev, shape, per_new, nbytes, tail, fn = _known(_check_tree, key, q, k, v, lens, k_new, v_new, tree, depth, window,
+                                                   scale, out, weights, weights_out, draft_weights)
     if out is None:
-        out = torch.empty((B, H, N, D), dtype=dt, device=dev)
-    else:
-        _need(out.shape == q.shape, f"out must be {tuple(q.shape)}")
-        _disjoint_rows(out, "out", 3)
-    op, os_ = _rows4(out, "out", dt, dev)
-    wp = wop = dwp = 0
-    ws_, wos = (0, 0), (0, 0)
+        out = q.new_empty(shape)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     if weights is not None:
-        wp = _shape(weights, "weights", (B, KV, S), torch.float32, dev)
         weights_out = weights if weights_out is None else weights_out
-        wop = _shape(weights_out, "weights_out", (B, KV, S), torch.float32, dev)
-        _need((weights.stride(2) == 1 and weights_out.stride(2) == 1) or S <= 1,
-              "weights and weights_out must have unit stride along S")
-        _disjoint_rows(weights_out, "weights_out", 2)
-        ws_, wos = weights.stride()[:2], weights_out.stride()[:2]
-        if draft_weights is None:
-            draft_weights = torch.empty((B, KV, N), dtype=torch.float32, device=dev)
-        dwp = _shape(draft_weights, "draft_weights", (B, KV, N), torch.float32, dev)
-        _need(draft_weights.is_contiguous(), "draft_weights must be contiguous")
-    else:
-        _need(weights_out is None and draft_weights is None, "weights_out and draft_weights go with weights")
-    if B and N:
-        nbytes = _lib.lib().w8_attention_tree_workspace_bytes(B, H, KV, D, S, N, window, weights is not None)
-        if nbytes < 0:
-            nbytes = 0  # a shape the call itself refuses, with its reason
-        ws = _workspace(dev, nbytes, "bad shape")
-        args = _lib.ATTENTION_TREE_ARGS.pack(qp, kp, vp, knp, vnp, op, lp, tp, dp, wp, wop, dwp, *qs, *ks, *vs, *kns,
-                                             *vns, *os_, *ts, ds, *ws_, *wos, B, H, KV, D, S, N, window, _DTYPES[dt],
-                                             scale)
-        _call(dev, "w8_attention_tree", args, ws.data_ptr(), nbytes)
+        draft_weights = weights.new_empty(per_new) if draft_weights is None else draft_weights
+    args = _lib.ATTENTION_TREE_POINTERS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_new.data_ptr(),
+                                             v_new.data_ptr(), out.data_ptr(), lens.data_ptr(), _ptr(tree), _ptr(depth),
+                                             _ptr(weights), _ptr(weights_out), _ptr(draft_weights)) + tail
+    _run(dev, fn, args, _ptr(ws), nbytes)
     return out if weights is None else (out, weights_out, draft_weights)
+
+
+def _check_append(k, v, k_new, v_new, lens, path, weights, draft_weights, positions, seen, lens_out):
+    dev = _cuda(k, "k")
+    dt = k.dtype
+    e = k.element_size()
+    strides = [x * e for t, name in ((k, "k"), (v, "v"), (k_new, "k_new"), (v_new, "v_new"))
+               for x in _rows4(t, name, dt, dev)]
+    B, KV, S, D = k.shape
+    N = k_new.shape[2]
+    _need(v.shape == k.shape, "v must have the shape of k")
+    _need(k_new.shape == (B, KV, N, D) and v_new.shape == k_new.shape, "k_new and v_new must be [B, KV, N, D]")
+    _disjoint_rows(k, "k", 3)
+    _disjoint_rows(v, "v", 3)
+    _vector(lens, "lens", (B,), torch.int32, dev)
+    ps, P = 0, N
+    if path is not None:
+        _need(isinstance(path, torch.Tensor) and path.dim() == 2, "path must be [B, P]")
+        P = path.shape[1]
+        _shape(path, "path", (B, P), torch.int32, dev)
+        _need(path.stride(1) == 1 or P <= 1, "path must have unit stride along P")
+        ps = path.stride(0)
+    ws, dws, pos = (0, 0), (0, 0), (0, 0)
+    if weights is not None:
+        ws = _per_slot(weights, "weights", (B, KV, S), torch.float32, dev)
+        _disjoint_rows(weights, "weights", 2)
+        if draft_weights is not None:
+            dws = _per_slot(draft_weights, "draft_weights", (B, KV, N), torch.float32, dev)
+    else:
+        _need(draft_weights is None, "draft_weights go with weights")
+    if positions is not None:
+        _need(seen is not None, "positions go with seen")
+        pos = _per_slot(positions, "positions", (B, KV, S), torch.int32, dev)
+        _disjoint_rows(positions, "positions", 2)
+        _vector(seen, "seen", (B,), torch.int32, dev)
+    if lens_out is not None:
+        _vector(lens_out, "lens_out", (B,), torch.int32, dev)
+    tail = _lib.CACHE_APPEND_TAIL.pack(*strides, ps, *ws, *dws, *pos, B, KV, S, N, P, D * e)
+    return dev, B, P, tail, _lib.lib().w8_cache_append
 
 
 def cache_append(k, v, k_new, v_new, lens, path=None, weights=None, draft_weights=None, positions=None, seen=None,
@@ -179,58 +262,50 @@ def cache_append(k, v, k_new, v_new, lens, path=None, weights=None, draft_weight
     weight from draft_weights [B, KV, N] (None: 0), with `positions` int32 [B, KV, S] the
     positions seen[b], seen[b] + 1, ... (seen int32 [B]: the tokens so far, evicted ones
     included).  Returns lens_out int32 [B] (not `lens` itself)."""
+    try:
+        key = ("cache_append", _layout(k), _layout(v), _layout(k_new), _layout(v_new), _layout(lens), _layout(path),
+               _layout(weights), _layout(draft_weights), _layout(positions), _layout(seen), _layout(lens_out))
+    except (AttributeError, TypeError):
+        key = None
+    dev, B, P, tail, fn = _known(_check_append, key, k, v, k_new, v_new, lens, path, weights, draft_weights, positions,
+                                 seen, lens_out)
+    if lens_out is None:
+        lens_out = lens.new_empty((B,))
+    lp = lens.data_ptr()
+    # An empty path is a path: nothing is appended and nothing of it is read.
+    pp = 0 if path is None else path.data_ptr() if P else lp
+    args = _lib.CACHE_APPEND_POINTERS.pack(k.data_ptr(), v.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), lp, pp,
+                                           _ptr(weights), _ptr(draft_weights), _ptr(positions),
+                                           _ptr(seen) if positions is not None else 0, lens_out.data_ptr()) + tail
+    _run(dev, fn, args)
+    return lens_out
+
+
+def _check_evict(k, v, weights, positions, lens, budget, sink, recent, weights_out, positions_out, lens_out):
     dev = _cuda(k, "k")
     dt = k.dtype
-    kp, ks = _rows4(k, "k", dt, dev)
-    vp, vs = _rows4(v, "v", dt, dev)
-    knp, kns = _rows4(k_new, "k_new", dt, dev)
-    vnp, vns = _rows4(v_new, "v_new", dt, dev)
+    e = k.element_size()
+    strides = [x * e for t, name in ((k, "k"), (v, "v")) for x in _rows4(t, name, dt, dev)]
     B, KV, S, D = k.shape
-    N = k_new.shape[2]
     _need(v.shape == k.shape, "v must have the shape of k")
-    _need(k_new.shape == (B, KV, N, D) and v_new.shape == k_new.shape, "k_new and v_new must be [B, KV, N, D]")
     _disjoint_rows(k, "k", 3)
     _disjoint_rows(v, "v", 3)
-    lp = _shape(lens, "lens", (B,), torch.int32, dev)
-    _need(lens.is_contiguous(), "lens must be contiguous")
-    pp, ps, P = 0, 0, N
-    if path is not None:
-        _need(isinstance(path, torch.Tensor) and path.dim() == 2, "path must be [B, P]")
-        P = path.shape[1]
-        pp = _shape(path, "path", (B, P), torch.int32, dev)
-        _need(path.stride(1) == 1 or P <= 1, "path must have unit stride along P")
-        ps = path.stride(0)
-        pp = pp if P else lp  # an empty path is a path: nothing is appended, nothing is read
-    wp, wst, dwp, dws = 0, (0, 0), 0, (0, 0)
-    if weights is not None:
-        wp, wst = _shape(weights, "weights", (B, KV, S), torch.float32, dev), weights.stride()[:2]
-        _need(weights.stride(2) == 1 or S <= 1, "weights must have unit stride along S")
-        _disjoint_rows(weights, "weights", 2)
-        if draft_weights is not None:
-            dwp = _shape(draft_weights, "draft_weights", (B, KV, N), torch.float32, dev)
-            dws = draft_weights.stride()[:2]
-            _need(draft_weights.stride(2) == 1 or N <= 1, "draft_weights must have unit stride along N")
-    else:
-        _need(draft_weights is None, "draft_weights go with weights")
-    pop, pos, sp = 0, (0, 0), 0
-    if positions is not None:
-        _need(seen is not None, "positions go with seen")
-        pop, pos = _shape(positions, "positions", (B, KV, S), torch.int32, dev), positions.stride()[:2]
-        _need(positions.stride(2) == 1 or S <= 1, "positions must have unit stride along S")
-        _disjoint_rows(positions, "positions", 2)
-        sp = _shape(seen, "seen", (B,), torch.int32, dev)
-        _need(seen.is_contiguous(), "seen must be contiguous")
-    if lens_out is None:
-        lens_out = torch.empty((B,), dtype=torch.int32, device=dev)
-    lop = _shape(lens_out, "lens_out", (B,), torch.int32, dev)
-    _need(lens_out.is_contiguous(), "lens_out must be contiguous")
-    if B:
-        e = k.element_size()
-        args = _lib.CACHE_APPEND_ARGS.pack(kp, vp, knp, vnp, lp, pp, wp, dwp, pop, sp, lop, *(s * e for s in ks),
-                                           *(s * e for s in vs), *(s * e for s in kns), *(s * e for s in vns), ps, *wst,
-                                           *dws, *pos, B, KV, S, N, P, D * e)
-        _call(dev, "w8_cache_append", args)
-    return lens_out
+    _vector(lens, "lens", (B,), torch.int32, dev)
+    for t, name, d in ((weights, "weights", torch.float32), (positions, "positions", torch.int32),
+                       (weights_out, "weights_out", torch.float32), (positions_out, "positions_out", torch.int32)):
+        if t is None and name.endswith("out"):
+            strides += (KV * S, S)
+            continue
+        strides += _per_slot(t, name, (B, KV, S), d, dev)
+        if name.endswith("out"):
+            _disjoint_rows(t, name, 2)
+    if lens_out is not None:
+        _vector(lens_out, "lens_out", (B,), torch.int32, dev)
+    for x, name in ((budget, "budget"), (sink, "sink"), (recent, "recent")):
+        _integer(x, name)
+    nbytes = max(0, _lib.lib().w8_cache_evict_workspace_bytes(B, KV, S, budget))
+    tail = _lib.CACHE_EVICT_TAIL.pack(*strides, B, KV, S, D * e, budget, sink, recent)
+    return dev, (B, KV, S), nbytes, tail, _lib.lib().w8_cache_evict
 
 
 def cache_evict(k, v, weights, positions, lens, budget, sink=0, recent=0, weights_out=None, positions_out=None,
@@ -248,37 +323,41 @@ def cache_evict(k, v, weights, positions, lens, budget, sink=0, recent=0, weight
     says which token stands where.  weights_out and positions_out (new tensors unless given;
     the inputs themselves are allowed) hold 0 and -1 behind the last slot; lens_out =
     min(lens, budget) is not `lens` itself."""
-    dev = _cuda(k, "k")
-    dt = k.dtype
-    kp, ks = _rows4(k, "k", dt, dev)
-    vp, vs = _rows4(v, "v", dt, dev)
-    B, KV, S, D = k.shape
-    _need(v.shape == k.shape, "v must have the shape of k")
-    _disjoint_rows(k, "k", 3)
-    _disjoint_rows(v, "v", 3)
-    lp = _shape(lens, "lens", (B,), torch.int32, dev)
-    _need(lens.is_contiguous(), "lens must be contiguous")
-    weights_out = torch.empty((B, KV, S), dtype=torch.float32, device=dev) if weights_out is None else weights_out
-    positions_out = torch.empty((B, KV, S), dtype=torch.int32, device=dev) if positions_out is None else positions_out
-    lens_out = torch.empty((B,), dtype=torch.int32, device=dev) if lens_out is None else lens_out
-    ptrs, strides = [], []
-    for t, name, d in ((weights, "weights", torch.float32), (positions, "positions", torch.int32),
-                       (weights_out, "weights_out", torch.float32), (positions_out, "positions_out", torch.int32)):
-        ptrs.append(_shape(t, name, (B, KV, S), d, dev))
-        _need(t.stride(2) == 1 or S <= 1, f"{name} must have unit stride along S")
-        strides += t.stride()[:2]
-    _disjoint_rows(weights_out, "weights_out", 2)
-    _disjoint_rows(positions_out, "positions_out", 2)
-    lop = _shape(lens_out, "lens_out", (B,), torch.int32, dev)
-    _need(lens_out.is_contiguous(), "lens_out must be contiguous")
-    if B:
-        e = k.element_size()
-        nbytes = max(0, _lib.lib().w8_cache_evict_workspace_bytes(B, KV, S, budget))
-        ws = _workspace(dev, nbytes, "bad shape")
-        args = _lib.CACHE_EVICT_ARGS.pack(kp, vp, ptrs[0], ptrs[1], lp, ptrs[2], ptrs[3], lop, *(s * e for s in ks),
-                                          *(s * e for s in vs), *strides, B, KV, S, D * e, budget, sink, recent)
-        _call(dev, "w8_cache_evict", args, ws.data_ptr(), nbytes)
+    try:
+        key = ("cache_evict", _layout(k), _layout(v), _layout(weights), _layout(positions), _layout(lens), budget, sink,
+               recent, _layout(weights_out), _layout(positions_out), _layout(lens_out))
+    except (AttributeError, TypeError):
+        key = None
+    dev, shape, nbytes, tail, fn = _known(_check_evict, key, k, v, weights, positions, lens, budget, sink, recent,
+                                          weights_out, positions_out, lens_out)
+    weights_out = weights.new_empty(shape) if weights_out is None else weights_out
+    positions_out = positions.new_empty(shape) if positions_out is None else positions_out
+    lens_out = lens.new_empty(shape[:1]) if lens_out is None else lens_out
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    args = _lib.CACHE_EVICT_POINTERS.pack(k.data_ptr(), v.data_ptr(), weights.data_ptr(), positions.data_ptr(),
+                                          lens.data_ptr(), weights_out.data_ptr(), positions_out.data_ptr(),
+                                          lens_out.data_ptr()) + tail
+    _run(dev, fn, args, ws.data_ptr(), nbytes)
     return weights_out, positions_out, lens_out
+
+
+def _check_select(logits, scores, finished, pad, n, cap, order):
+    dev = _cuda(logits, "logits")
+    _need(logits.dtype in _DTYPES, f"logits must be float32, bfloat16 or float16 (got {logits.dtype})")
+    _need(logits.dim() == 3, "logits must be [B, K, V]")
+    B, K, V = logits.shape
+    _need(logits.stride(2) == 1 or V <= 1, "logits must have unit stride along V")
+    _vector(scores, "scores", (B, K), torch.float32, dev)
+    if finished is not None:
+        _vector(finished, "finished", (B, K), torch.bool, dev)
+    n = K if n is None else n
+    _integer(n, "n")
+    _integer(pad, "pad")
+    _need(n >= 1, f"n = {n} must be positive")
+    _need(order in _ORDERS, f"order must be one of {_ORDERS}")
+    nbytes = max(0, _lib.lib().w8_beam_select_workspace_bytes(B, K, V, n))
+    mid = (pad, cap, B, K, V, n, order == "slot")
+    return dev, (B, n), nbytes, _DTYPES[logits.dtype], logits.stride(0), logits.stride(1), mid, _lib.lib().w8_beam_select
 
 
 def beam_select(logits, scores, finished=None, pad=0, n=None, cap=0.0, order="score"):
@@ -297,30 +376,35 @@ def beam_select(logits, scores, finished=None, pad=0, n=None, cap=0.0, order="sc
     order="slot" (n = K): the best continuation of a surviving beam stands in that beam's own
     slot, the others fill the free slots, best first: the same continuations, arranged so
     that `cache_reorder` moves as little as can be."""
-    dev = _cuda(logits, "logits")
-    _need(logits.dtype in _DTYPES, f"logits must be float32, bfloat16 or float16 (got {logits.dtype})")
-    _need(logits.dim() == 3, "logits must be [B, K, V]")
-    B, K, V = logits.shape
-    _need(logits.stride(2) == 1 or V <= 1, "logits must have unit stride along V")
-    sp = _shape(scores, "scores", (B, K), torch.float32, dev)
-    _need(scores.is_contiguous(), "scores must be contiguous")
-    fp = None
-    if finished is not None:
-        fp = _shape(finished, "finished", (B, K), torch.bool, dev)
-        _need(finished.is_contiguous(), "finished must be contiguous")
-    n = K if n is None else n
-    _need(n >= 1, f"n = {n} must be positive")
-    _need(order in _ORDERS, f"order must be one of {_ORDERS}")
-    out = torch.empty((B, n), dtype=torch.float32, device=dev)
-    beam = torch.empty((B, n), dtype=torch.int64, device=dev)
-    token = torch.empty((B, n), dtype=torch.int64, device=dev)
-    if B:
-        nbytes = max(0, _lib.lib().w8_beam_select_workspace_bytes(B, K, V, n))
-        ws = _workspace(dev, nbytes, "bad shape")
-        _call(dev, "w8_beam_select", logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), logits.stride(1), sp,
-              fp, pad, cap, B, K, V, n, order == "slot", out.data_ptr(), beam.data_ptr(), token.data_ptr(),
-              ws.data_ptr(), nbytes)
+    try:
+        key = ("beam_select", _layout(logits), _layout(scores), _layout(finished), pad, n, cap, order)
+    except (AttributeError, TypeError):
+        key = None
+    dev, shape, nbytes, dt, s0, s1, mid, fn = _known(_check_select, key, logits, scores, finished, pad, n, cap, order)
+    out = scores.new_empty(shape)
+    beam = torch.empty(shape, dtype=torch.int64, device=dev)
+    token = beam.new_empty(shape)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _run(dev, fn, logits.data_ptr(), dt, s0, s1, scores.data_ptr(), _ptr(finished), *mid, out.data_ptr(),
+         beam.data_ptr(), token.data_ptr(), ws.data_ptr(), nbytes)
     return out, beam, token
+
+
+def _check_reorder(first, beam, lens):
+    dev = _cuda(first, "caches")
+    _need(isinstance(beam, torch.Tensor) and beam.dim() == 2 and beam.dtype in (torch.int64, torch.int32),
+          "beam must be int64 or int32 [B, K]")
+    B, K = beam.shape
+    _vector(beam, "beam", (B, K), beam.dtype, dev)
+    strides = _rows4(first, "caches", first.dtype, dev)
+    states, heads, S, D = first.shape
+    _need(states == B * K, f"caches must have B * K = {B * K} states (got {states})")
+    _disjoint_rows(first, "caches", 3)
+    if lens is not None:
+        _vector(lens, "lens", (B * K,), torch.int32, dev)
+    e = first.element_size()
+    return (dev, (ctypes.c_int64 * 3)(*(s * e for s in strides)), beam.dtype == torch.int64,
+            (B, K, heads, S, D * e), _lib.lib().w8_cache_reorder)
 
 
 def cache_reorder(caches, beam, lens=None):
@@ -335,29 +419,18 @@ def cache_reorder(caches, beam, lens=None):
     many = [caches] if isinstance(caches, torch.Tensor) else list(caches)
     if not many:
         return caches
-    first = many[0]
-    dev = _cuda(first, "caches")
-    _need(isinstance(beam, torch.Tensor) and beam.dim() == 2 and beam.dtype in (torch.int64, torch.int32),
-          "beam must be int64 or int32 [B, K]")
-    _need(beam.device == dev and beam.is_contiguous(), f"beam must be contiguous on {dev}")
-    B, K = beam.shape
-    shape, stride, dt = first.shape, first.stride(), first.dtype
-    _, strides = _rows4(first, "caches", dt, dev)
-    _need(shape[0] == B * K, f"caches must have B * K = {B * K} states (got {shape[0]})")
-    _disjoint_rows(first, "caches", 3)
-    ptrs = []
+    try:
+        layout = _layout(many[0])
+        key = ("cache_reorder", layout, _layout(beam), _layout(lens))
+    except (AttributeError, TypeError):
+        key = None
+    dev, strides, wide, sizes, fn = _known(_check_reorder, key, many[0], beam, lens)
     for t in many:
-        _need(isinstance(t, torch.Tensor) and t.shape == shape and t.stride() == stride and t.dtype == dt
-              and t.device == dev, "caches must share one shape, layout, dtype and device")
-        ptrs.append(t.data_ptr())
-    _need(len(set(ptrs)) == len(ptrs), "caches must be distinct tensors")
-    lp = None
-    if lens is not None:
-        lp = _shape(lens, "lens", (B * K,), torch.int32, dev)
-        _need(lens.is_contiguous(), "lens must be contiguous")
-    if B and K and shape[1]:
-        e = first.element_size()
-        _call(dev, "w8_cache_reorder", (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs),
-              (ctypes.c_int64 * 3)(*(s * e for s in strides)), beam.data_ptr(), beam.dtype == torch.int64, lp, B, K,
-              shape[1], shape[2], shape[3] * e)
+        _need(isinstance(t, torch.Tensor) and (t is many[0] or _layout(t) == layout),
+              "caches must share one shape, layout, dtype and device")
+    ptrs = [t.data_ptr() for t in many]
+    _need(len(set(ptrs)) == len(ptrs) or not many[0].numel(), "caches must be distinct tensors")
+    if sizes[0] and sizes[1] and sizes[2]:
+        _run(dev, fn, (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), strides, beam.data_ptr(), wide, _ptr(lens),
+             *sizes)
     return caches

@@ -301,7 +301,7 @@ typedef struct w8_attention_tree_args {
   void* out;
   const int32_t* lens;   /* [batch] */
   const uint8_t* tree;   /* [batch, n, n], nonzero at (i, j): new token i sees new token j; NULL: j <= i */
-  const int32_t* depth;  /* [batch, n]: the token's distance behind the cache; NULL: its index */
+  const int32_t* depth;  /* [batch, n]: the token's distance behind the cache (< 0 counts as 0); NULL: its index */
   const float* weights;  /* [batch, kv_heads, slots] accumulated weights, or NULL with the two below */
   float* weights_out;    /* the same shape; may be `weights` */
   float* draft_weights;  /* [batch, kv_heads, n] contiguous: the new tokens' own */
@@ -316,7 +316,7 @@ typedef struct w8_attention_tree_args {
  * (a drafted tree's ancestors and itself; NULL: a causal chunk, n = 1 a decode step), all
  * cut to the last `window` positions when window > 0, where slot j stands at position j and
  * new token i at lens[b] + depth[b, i]:
- *   out = softmax(scale q . k) v over what it sees; zeros where it sees nothing.
+ *   out = softmax(scale q . k) v over what it sees (scale > 0); zeros where it sees nothing.
  * Grouped-query heads, head_dim 64, 128, 256 or 512, fp32 softmax and sums.  With weights:
  * weights_out[b, c, j] = weights[b, c, j] + the probabilities of slot j summed over the
  * group's heads and the n tokens (slots behind lens[b] are left alone), and draft_weights

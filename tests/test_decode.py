@@ -16,8 +16,8 @@ def tree_args(**change):
     n = dict(B=1, H=4, KV=2, D=64, S=16, N=2, window=0, dtype=_lib.W8_BF16, scale=1.0)
     for name, v in change.items():
         next(d for d in (p, s, n) if name in d)[name] = v
-    return _lib.ATTENTION_TREE_ARGS.pack(*p.values(), *(x for v in s.values() for x in v), 4, 2, 0, 0, 0, 0, 0,
-                                         *n.values())
+    return _lib.ATTENTION_TREE_POINTERS.pack(*p.values()) + _lib.ATTENTION_TREE_TAIL.pack(
+        *(x for v in s.values() for x in v), 4, 2, 0, 0, 0, 0, 0, *n.values())
 
 
 @pytest.mark.parametrize("change,status", [
@@ -25,6 +25,7 @@ def tree_args(**change):
     (dict(D=96), _lib.W8_ERR_UNSUPPORTED), (dict(dtype=_lib.W8_FP32), _lib.W8_ERR_INVALID_ARG), (dict(q=0), _lib.W8_ERR_INVALID_ARG),
     (dict(lens=0), _lib.W8_ERR_INVALID_ARG), (dict(k=0), _lib.W8_ERR_INVALID_ARG), (dict(tree=4096, window=3), _lib.W8_ERR_INVALID_ARG),
     (dict(weights=4096), _lib.W8_ERR_INVALID_ARG), (dict(k=4104), _lib.W8_ERR_ALIGNMENT), (dict(ks=(64, 64, 60)), _lib.W8_ERR_ALIGNMENT),
+    (dict(scale=0.0), _lib.W8_ERR_INVALID_ARG), (dict(scale=float("nan")), _lib.W8_ERR_INVALID_ARG),
     (dict(N=65537), _lib.W8_ERR_INVALID_ARG)])
 def test_attention_tree_refuses(change, status):
     assert _lib.lib().w8_attention_tree(tree_args(**change), None, 0, None) == status
@@ -40,8 +41,9 @@ def test_struct_sizes_match_the_header():
     import re
 
     text = re.sub(r"/\*.*?\*/", "", open(_lib.HEADER_PATH).read(), flags=re.S)
-    for name, packed in (("w8_attention_tree_args", _lib.ATTENTION_TREE_ARGS), ("w8_cache_append_args", _lib.CACHE_APPEND_ARGS),
-                         ("w8_cache_evict_args", _lib.CACHE_EVICT_ARGS)):
+    for name, head, tail in (("w8_attention_tree_args", _lib.ATTENTION_TREE_POINTERS, _lib.ATTENTION_TREE_TAIL),
+                             ("w8_cache_append_args", _lib.CACHE_APPEND_POINTERS, _lib.CACHE_APPEND_TAIL),
+                             ("w8_cache_evict_args", _lib.CACHE_EVICT_POINTERS, _lib.CACHE_EVICT_TAIL)):
         body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1)
         fields = 0
         for decl in body.split(";"):
@@ -49,13 +51,13 @@ def test_struct_sizes_match_the_header():
                 if item.strip():
                     m = re.search(r"\[(\d+)\]", item)
                     fields += int(m.group(1)) if m else 1
-        assert packed.size == 8 * fields, name
+        assert head.size + tail.size == 8 * fields, name
 
 
 def test_evict_refuses():
     def args(budget=4, sink=0, recent=0, lens=4096, lens_out=8192, row=128):
-        return _lib.CACHE_EVICT_ARGS.pack(4096, 4096, 4096, 4096, lens, 4096, 4096, lens_out, *[128] * 6, *[16] * 8, 1, 1, 16,
-                                          row, budget, sink, recent)
+        return _lib.CACHE_EVICT_POINTERS.pack(4096, 4096, 4096, 4096, lens, 4096, 4096, lens_out) + _lib.CACHE_EVICT_TAIL.pack(
+            *[128] * 6, *[16] * 8, 1, 1, 16, row, budget, sink, recent)
 
     run = _lib.lib().w8_cache_evict
     for a in (args(budget=0), args(sink=-1), args(sink=2, recent=3), args(lens=0), args(lens_out=4096)):
