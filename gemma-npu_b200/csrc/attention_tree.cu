@@ -79,7 +79,8 @@ struct TreeCfg {
   static constexpr int kOffRing = kBM * D * 2;
   static constexpr int kOffP = kOffRing + kSlots * kSlotBytes;
   static constexpr int kOffRed = kOffP + kBM * kTreePPitch * 2;
-  static constexpr int kSmem = kOffRed + kBM * kTreeWarps * 4;
+  static constexpr int kOffPoison = kOffRed + kBM * kTreeWarps * 4;
+  static constexpr int kSmem = kOffPoison + kPoisonWords * 4;
   static_assert(kSmem <= 232448, "shared memory budget exceeded");
 };
 
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs 
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t sq = smem_u32(smem), ring = sq + C::kOffRing, sp = sq + C::kOffP;
   float* red = reinterpret_cast<float*>(smem + C::kOffRed);  // [BM][8]
+  uint32_t* poison = reinterpret_cast<uint32_t*>(smem + C::kOffPoison);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits;
@@ -110,6 +112,8 @@ __global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs 
     if (tid < BM) a.part_ml[part_row + tid] = make_float2(-INFINITY, 0.f);
     return;
   }
+
+  if (tid < kPoisonWords) poison[tid] = 0u;  // (ordered before its first use by the ring's barriers)
 
   // Row r = i * group + g: query head c * group + g of new token i.
   auto q_row = [&](int r) {
@@ -268,8 +272,9 @@ __global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs 
       // A new token's values may be infinite or NaN where some row must not see them, and
       // 0 * NaN is NaN in the product: take them out here, and add them at the end to the
       // rows that do see them.
-      bool bad = false;
+      bool any = false;
       for (int e = tid; e < kTreeBN * CH; e += kTreeThreads) {
+        bool bad = false;
         uint32_t* w = reinterpret_cast<uint32_t*>(smem + C::kOffRing + ((g + 1) % NS) * C::kSlotBytes) + e * 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -280,8 +285,12 @@ __global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs 
             bad = true;
           }
         }
+        if (bad) {
+          poison_mark(poison, key0 + e / CH);
+          any = true;
+        }
       }
-      if (__syncthreads_or(bad)) poisoned = true;
+      if (__syncthreads_or(any)) poisoned = true;
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -330,14 +339,17 @@ __global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs 
       for (int h = 0; h < 2; ++h)
         if (tok[mt][h] >= 0)
 #pragma unroll 1
-          for (int j = j0; j < j1; ++j)
-            if (tree_sees(a, b, tok[mt][h], j, dep[mt][h]))
+          for (int jw = j0; jw < j1; jw += 32) {
+            uint32_t bits = poison_of(poison, jw);
+            if (bits != 0u) bits &= tree_sees32(a, b, tok[mt][h], jw, dep[mt][h]);
+#pragma unroll 1
+            for (; bits != 0u; bits &= bits - 1u)
 #pragma unroll
               for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const uint16_t v = a.vn[b * a.vn_b + c * a.vn_h + j * a.vn_t + warp * (D / 8) + n * 8 +
-                                          (lane & 3) * 2 + e];
+                  const uint16_t v = a.vn[b * a.vn_b + c * a.vn_h + (jw + __ffs(bits) - 1) * a.vn_t + warp * (D / 8) +
+                                          n * 8 + (lane & 3) * 2 + e];
                   // (static register indexes only: both rows are written under a select)
                   const float add = tree_nonfinite<T>(v) ? tree_f32<T>(v) : 0.f;
 #pragma unroll
@@ -346,6 +358,7 @@ __global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs 
                     if (mm == mt && h == 1) o[mm][n][2 + e] += add;
                   }
                 }
+          }
   }
 
   // ---- row sums over the warps, then the output or this split's partial
@@ -522,12 +535,29 @@ static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_
   p.bm = p.tc ? 256 : rows > 16 && d <= 256 ? 32 : 16;
   p.row_tiles = static_cast<int>((rows + p.bm - 1) / p.bm);
   p.items = batch * kv_heads * p.row_tiles;
+  // Keys of one row tile: with a window, those its tokens see.
   const int64_t bn = p.tc ? 128 : w8::kTreeBN;
-  const int64_t keys = window > 0 ? std::min(slots, window + n + bn) : slots;
+  const int64_t tokens = std::min(n, p.bm / group + 2);
+  const int64_t keys = window > 0 ? std::min(slots, window + tokens) : slots;
   const int64_t tiles = (keys + bn - 1) / bn + (n + bn - 1) / bn;
-  const int64_t want = p.tc ? (d == 512 ? sms / 4 : sms / 2) : static_cast<int64_t>(sms) * (d == 512 ? 1 : 2);
-  p.splits = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>({want / std::max<int64_t>(p.items, 1), tiles, w8::kTreeMaxSplits})));
+  p.splits = 1;
+  if (p.tc) {
+    // The number of splits with the least estimated time: waves of clusters, each 1.6 us a tile
+    // and 8 us besides, then 4 us and the partials at 3 TB/s to join them (measured on trees
+    // of 64 drafts at D 256).
+    const int64_t width = d == 512 ? 2 : 1, pairs = sms / 2;
+    double best = 0;
+    for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64); ++s) {
+      const double waves = static_cast<double>((p.items * width * s + pairs - 1) / pairs);
+      double us = waves * (1.6 * static_cast<double>((tiles + s - 1) / s) + 8);
+      if (s > 1) us += 4 + static_cast<double>(p.items * p.bm * d) * 8 * static_cast<double>(s) / 3e6;
+      if (s == 1 || us < best) best = us, p.splits = static_cast<int>(s);
+    }
+  } else {
+    const int64_t want = static_cast<int64_t>(sms) * (d == 512 ? 1 : 2);
+    p.splits = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>({want / std::max<int64_t>(p.items, 1), tiles, w8::kTreeMaxSplits})));
+  }
   return p;
 }
 

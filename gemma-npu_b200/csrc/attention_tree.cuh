@@ -34,6 +34,35 @@ struct TreeArgs {
   int64_t wi_b, wi_h, wo_b, wo_h;
 };
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&p);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 p = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&p);
+}
+template <typename T>
+__device__ __forceinline__ float tree_f32(uint16_t bits);
+template <>
+__device__ __forceinline__ float tree_f32<__nv_bfloat16>(uint16_t bits) {
+  return __uint_as_float(static_cast<uint32_t>(bits) << 16);
+}
+template <>
+__device__ __forceinline__ float tree_f32<__half>(uint16_t bits) {
+  return __half2float(__ushort_as_half(bits));
+}
+// Infinity or NaN: every exponent bit set.
+template <typename T>
+__device__ __forceinline__ bool tree_nonfinite(uint32_t bits) {
+  constexpr uint32_t e = __is_same(T, __half) ? 0x7C00u : 0x7F80u;
+  return (bits & e) == e;
+}
+
 __device__ __forceinline__ float ex2_tree(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -68,6 +97,67 @@ __device__ __forceinline__ bool tree_sees(const TreeArgs& a, int b, int i, int j
   return static_cast<int64_t>(tree_depth(a, b, j)) > static_cast<int64_t>(depth_i) - a.window;
 }
 
+// The same for a packed pair: bit 15 / 31 set for a half that is not finite (the exponent
+// field plus its lowest bit carries into the sign's place only from all ones).
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite_bits(uint32_t pair) {
+  constexpr uint32_t e = __is_same(T, __half) ? 0x7C007C00u : 0x7F807F80u;
+  constexpr uint32_t one = __is_same(T, __half) ? 0x04000400u : 0x00800080u;
+  return ((pair & e) + one) & 0x80008000u;
+}
+
+// The bytes of a word that are not zero, as 4 bits.
+__device__ __forceinline__ uint32_t nonzero_bytes(uint32_t w) {
+  const uint32_t m = __vcmpne4(w, 0u) & 0x08040201u;  // one distinct bit of each byte
+  return (m | (m >> 8) | (m >> 16) | (m >> 24)) & 15u;
+}
+
+// tree_sees of the new tokens j0 .. j0 + 31 as bits (those behind n are 0).  A loop of byte
+// loads would wait for each in turn: the row is read with 16-byte loads where it is aligned
+// and with 32 independent ones where it is not.
+__device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i, int j0, int depth_i) {
+  const int left = a.n - j0;
+  if (left <= 0) return 0u;
+  uint32_t bits = 0;
+  if (a.tree == nullptr) {
+    bits = i < j0 ? 0u : i - j0 >= 31 ? 0xFFFFFFFFu : (2u << (i - j0)) - 1u;
+  } else {
+    const uint8_t* row = a.tree + b * a.tree_b + i * a.tree_i + j0;
+    if (left >= 32 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+      const uint4 lo = *reinterpret_cast<const uint4*>(row), hi = *reinterpret_cast<const uint4*>(row + 16);
+      bits = nonzero_bytes(lo.x) | nonzero_bytes(lo.y) << 4 | nonzero_bytes(lo.z) << 8 | nonzero_bytes(lo.w) << 12 |
+             nonzero_bytes(hi.x) << 16 | nonzero_bytes(hi.y) << 20 | nonzero_bytes(hi.z) << 24 |
+             nonzero_bytes(hi.w) << 28;
+    } else {
+      uint8_t v[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = e < left ? row[e] : 0;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) bits |= v[e] != 0 ? 1u << e : 0u;
+    }
+  }
+  if (left < 32) bits &= (1u << left) - 1u;
+  if (a.window > 0 && bits != 0u) {
+    int d[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) d[e] = e < left ? tree_depth(a, b, j0 + e) : 0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (static_cast<int64_t>(d[e]) <= static_cast<int64_t>(depth_i) - a.window) bits &= ~(1u << e);
+  }
+  return bits;
+}
+
+// New tokens whose values are not all finite, one bit each; tokens 2048 apart share a bit, so
+// a set bit only says that the token's values must be looked at.
+constexpr int kPoisonWords = 64;
+__device__ __forceinline__ void poison_mark(uint32_t* words, int j) {
+  atomicOr(&words[(j >> 5) & (kPoisonWords - 1)], 1u << (j & 31));
+}
+__device__ __forceinline__ uint32_t poison_of(const volatile uint32_t* words, int j0) {  // of j0 .. j0 + 31, j0 % 32 == 0
+  return words[(j0 >> 5) & (kPoisonWords - 1)];
+}
+
 // Tiles of `bn` keys of one row tile of `bm` rows: committed tiles [c0, c1), then draft
 // tiles [0, nd).
 struct TreeSpan {
@@ -85,35 +175,6 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int len, int rt
   s.nd = last / bn + 1;
   if (s.c0 > s.c1) s.c0 = s.c1;
   return s;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&p);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  __half2 p = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&p);
-}
-template <typename T>
-__device__ __forceinline__ float tree_f32(uint16_t bits);
-template <>
-__device__ __forceinline__ float tree_f32<__nv_bfloat16>(uint16_t bits) {
-  return __uint_as_float(static_cast<uint32_t>(bits) << 16);
-}
-template <>
-__device__ __forceinline__ float tree_f32<__half>(uint16_t bits) {
-  return __half2float(__ushort_as_half(bits));
-}
-// Infinity or NaN: every exponent bit set.
-template <typename T>
-__device__ __forceinline__ bool tree_nonfinite(uint32_t bits) {
-  constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, __half) ? 0x7C00u : 0x7F80u;
-  return (bits & e) == e;
 }
 
 }  // namespace w8

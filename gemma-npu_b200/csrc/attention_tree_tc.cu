@@ -50,7 +50,8 @@ struct TtCfg {
   // full[kSlots], empty[kSlots], own[kSlots], q_full, s_full[2], p_full[2], pv_done[2], o_ready
   static constexpr int kNumBars = 3 * kSlots + 8;
   static constexpr int kOffXch = kOffBar + kNumBars * 8 + 16;
-  static constexpr int kSmem = kOffXch + 2 * kTtBM * 4 + 16 + 1024;
+  static constexpr int kOffPoison = kOffXch + 2 * kTtBM * 4;
+  static constexpr int kSmem = kOffPoison + kPoisonWords * 4 + 1024;
   static_assert(kKCols == kDV, "K and V slots have one size");
   static_assert(kSmem <= 232448, "shared memory budget exceeded");
 };
@@ -59,6 +60,10 @@ struct TtCfg {
 // writes to the cluster.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void red_or_cluster(uint32_t addr, uint32_t bits) {
+  asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(bits) : "memory");
 }
 
 template <typename T, int D>
@@ -114,6 +119,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     prefetch_tmap(&tm_kn);
     prefetch_tmap(&tm_vn);
   }
+  if (threadIdx.x < kPoisonWords) reinterpret_cast<uint32_t*>(smem + C::kOffPoison)[threadIdx.x] = 0u;
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(tmem_slot), kTtTmemCols);
     tmem_relinquish_pair();
@@ -261,42 +267,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t p_full_l0 = mapa_shared(p_full(0), 0);
     volatile float* xch = reinterpret_cast<volatile float*>(smem + C::kOffXch);
-    volatile int* poison_flag = reinterpret_cast<volatile int*>(smem + C::kOffXch + 2 * kTtBM * 4);
+    const volatile uint32_t* poison = reinterpret_cast<const volatile uint32_t*>(smem + C::kOffPoison);
     auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
     auto softmax_sync = [&]() { asm volatile("bar.sync 5, %0;" ::"n"(32 * kTtSoftWarps) : "memory"); };
 
     // Q rows (row R = i * group + g: head c * group + g of new token i), swizzled as the TMA
     // would: 64-column blocks of [128 rows x 128 bytes].
-    for (int e = tid; e < kTtBM * (D / 8); e += 32 * kTtSoftWarps) {
-      const int qr = e / (D / 8), ch = e % (D / 8), rr = row0 + qr;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (rr < rows)
-        w = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + rr % a.group) * a.q_h +
-                                            (rr / a.group) * a.q_t + ch * 8);
-      st_shared_v4(base + (ch >> 3) * (kTtBM * 128) + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4), w.x, w.y, w.z, w.w);
+    {
+      // Thread: one 16-byte chunk of every (2048 / D)-th row; 8 loads in flight.
+      constexpr int kStep = 32 * kTtSoftWarps / (D / 8);
+      const int ch = tid % (D / 8);
+#pragma unroll 1
+      for (int q0 = tid / (D / 8); q0 < kTtBM; q0 += 8 * kStep) {
+        uint4 w[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int rr = row0 + q0 + x * kStep;
+          w[x] = make_uint4(0, 0, 0, 0);
+          if (rr < rows)
+            w[x] = *reinterpret_cast<const uint4*>(
+                a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + rr % a.group) * a.q_h + (rr / a.group) * a.q_t + ch * 8);
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int qr = q0 + x * kStep;
+          st_shared_v4(base + (ch >> 3) * (kTtBM * 128) + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4), w[x].x, w[x].y, w[x].z,
+                       w[x].w);
+        }
+      }
     }
-    if (tid == 0) *poison_flag = 0;
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive_cluster(mapa_shared(q_full, 0));
-    softmax_sync();
     const bool drafts = t1 > nc;
     const int j_begin = drafts ? (max(t0, nc) - nc) * kTtBN : 0, j_end = drafts ? min((t1 - nc) * kTtBN, a.n) : 0;
-    if (drafts) {
-      // Does any new token of these tiles have a value that is not finite (in this half's columns)?
-      bool bad = false;
-      const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + half * C::kDV;
-      for (int e = j_begin * (C::kDV / 8) + tid; e < j_end * (C::kDV / 8); e += 32 * kTtSoftWarps) {
-        const uint4 w = *reinterpret_cast<const uint4*>(vn + (e / (C::kDV / 8)) * a.vn_t + (e % (C::kDV / 8)) * 8);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t x = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
-          bad |= tree_nonfinite<T>(x) || tree_nonfinite<T>(x >> 16);
-        }
-      }
-      if (bad) *poison_flag = 1;
-    }
-
     const int rr = row0 + r;
     const int tok = rr < rows ? rr / a.group : -1;
     const int dep = tok >= 0 ? tree_depth(a, b, tok) : 0;
@@ -325,15 +329,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         const int k0 = key0 + 64 * hv;
         if (draft) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t bits = 0;
-            if (tok >= 0)
-              for (int e = 0; e < 32; ++e) {
-                const int key = k0 + 32 * j + e;
-                if (key < a.n && tree_sees(a, b, tok, key, dep)) bits |= 1u << e;
-              }
-            keep[j] = bits;
-          }
+          for (int j = 0; j < 2; ++j) keep[j] = tok >= 0 ? tree_sees32(a, b, tok, k0 + 32 * j, dep) : 0u;
         } else {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
@@ -420,15 +416,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
               if (key0 + row >= len) *w = make_uint4(0, 0, 0, 0);
             } else {
               uint4 x = *w;
-              uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
-              bool bad = false;
+              if (nonfinite_bits<T>(x.x) | nonfinite_bits<T>(x.y) | nonfinite_bits<T>(x.z) | nonfinite_bits<T>(x.w)) {
+                uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const bool lo = tree_nonfinite<T>(xs[q]), hi = tree_nonfinite<T>(xs[q] >> 16);
-                bad |= lo || hi;
-                xs[q] = (lo ? 0u : xs[q] & 0xFFFFu) | (hi ? 0u : xs[q] & 0xFFFF0000u);
+                for (int q = 0; q < 4; ++q)
+                  xs[q] &= ~((nonfinite_bits<T>(xs[q]) >> 15) * 0xFFFFu);
+                *w = x;
+                // Both CTAs' rows may see the token: mark it in both.  (Ordered before the epilogues
+                // by the hand-over of P, the MMA that reads it and its completion.)
+                const int j = key0 + row;
+                const uint32_t word = base + C::kOffPoison + ((j >> 5) & (kPoisonWords - 1)) * 4;
+                red_or_cluster(mapa_shared(word, 0), 1u << (j & 31));
+                red_or_cluster(mapa_shared(word, 1), 1u << (j & 31));
               }
-              if (bad) *w = x;
             }
           }
           fence_proxy_async_smem();
@@ -451,7 +451,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     xch[hv * kTtBM + r] = l;
     softmax_sync();
     const float lt = l + xch[(hv ^ 1) * kTtBM + r];
-    const bool poisoned = drafts && *poison_flag != 0;
+    bool poisoned = false;  // the row sees such a token
+    if (drafts && tok >= 0)
+      for (int j = j_begin; j < j_end && !poisoned; j += 32) {
+        const uint32_t bits = poison_of(poison, j);
+        poisoned = bits != 0u && (bits & tree_sees32(a, b, tok, j, dep)) != 0u;
+      }
+    __syncwarp();
     if (good) {
       tc_fence_after();
       const float inv = lt == 0.f ? 0.f : 1.f / lt;  // a row that sees nothing: zeros
@@ -464,13 +470,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         if (tok >= 0) {
           if (poisoned) {
   #pragma unroll 1
-            for (int j = j_begin; j < j_end; ++j)
-              if (tree_sees(a, b, tok, j, dep)) {
-                const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + j * a.vn_t + half * C::kDV + col;
-  #pragma unroll
+            for (int j0 = j_begin; j0 < j_end; j0 += 32) {
+              uint32_t bits = poison_of(poison, j0);
+              if (bits != 0u) bits &= tree_sees32(a, b, tok, j0, dep);
+              for (; bits != 0u; bits &= bits - 1u) {
+                const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + (j0 + __ffs(bits) - 1) * a.vn_t + half * C::kDV + col;
+#pragma unroll
                 for (int x = 0; x < 32; ++x)
                   if (tree_nonfinite<T>(vn[x])) ov[x] = __float_as_uint(__uint_as_float(ov[x]) + tree_f32<T>(vn[x]));
               }
+            }
           }
           if (a.splits == 1) {
             uint16_t* dst = a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + rr % a.group) * a.o_h + tok * a.o_t +
