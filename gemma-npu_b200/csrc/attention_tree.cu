@@ -117,7 +117,9 @@ __global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs 
 
   // Row r = i * group + g: query head c * group + g of new token i.
   auto q_row = [&](int r) {
-    return a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + r % a.group) * a.q_h + (r / a.group) * a.q_t;
+    int i, g;
+    tree_row(a, r, i, g);
+    return a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + g) * a.q_h + i * a.q_t;
   };
   for (int e = tid; e < BM * CH; e += kTreeThreads) {
     const int r = e / CH, ch = e % CH;
@@ -753,12 +755,18 @@ extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspa
   a.batch = static_cast<int>(x.batch);
   a.kv_heads = static_cast<int>(x.kv_heads);
   a.group = static_cast<int>(group);
+  a.group_rcp = group > 1 ? static_cast<uint32_t>((1ull << 32) / static_cast<uint64_t>(group)) : 0u;
   a.n = static_cast<int>(x.n_new);
   a.slots = static_cast<int>(x.slots);
   a.window = static_cast<int>(x.window);
   a.scale_log2 = scale_log2;
   a.row_tiles = p.row_tiles;
   a.splits = p.splits;
+  // Boxes of 128 query rows: the group divides 128, and no stride of 0.
+  a.q_tma = group <= 128 && (group & (group - 1)) == 0;
+  const int64_t q_sizes[3] = {x.batch, x.heads, x.n_new};
+  for (int j = 0; j < 3; ++j)
+    if (q_sizes[j] > 1 && (x.q_stride[j] <= 0 || x.q_stride[j] >= (1ll << 38))) a.q_tma = 0;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.part_o = reinterpret_cast<float*>(ws + w.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);

@@ -20,6 +20,8 @@ struct TreeArgs {
   const int* depth;      // [B, N] or null: the token's index
   int64_t q_b, q_h, q_t, k_b, k_h, k_s, v_b, v_h, v_s, kn_b, kn_h, kn_t, vn_b, vn_h, vn_t, o_b, o_h, o_t;
   int64_t tree_b, tree_i, depth_b;
+  uint32_t group_rcp;    // floor(2^32 / group), for tree_row
+  int q_tma;             // q's rows load as TMA boxes (tcgen05 schedule)
   int batch, kv_heads, group, n, slots, window;
   float scale_log2;      // scale * log2(e): scores in log2 units
   int row_tiles, splits;
@@ -61,6 +63,14 @@ template <typename T>
 __device__ __forceinline__ bool tree_nonfinite(uint32_t bits) {
   constexpr uint32_t e = __is_same(T, __half) ? 0x7C00u : 0x7F80u;
   return (bits & e) == e;
+}
+
+// Row r = i * group + g as (token i, head g of the group) without a division: the product with
+// the truncated reciprocal is at most one short for r < 2^32.
+__device__ __forceinline__ void tree_row(const TreeArgs& a, int r, int& i, int& g) {
+  i = a.group == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), a.group_rcp));
+  g = r - i * a.group;
+  if (g >= a.group) ++i, g -= a.group;
 }
 
 __device__ __forceinline__ float ex2_tree(float x) {
@@ -121,6 +131,11 @@ __device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i,
   uint32_t bits = 0;
   if (a.tree == nullptr) {
     bits = i < j0 ? 0u : i - j0 >= 31 ? 0xFFFFFFFFu : (2u << (i - j0)) - 1u;
+    if (a.depth == nullptr) {  // a plain chunk: the last `window` tokens up to i
+      const int lo = a.window > 0 ? i - a.window + 1 - j0 : 0;
+      if (lo > 0) bits = lo > 31 ? 0u : bits & (0xFFFFFFFFu << lo);
+      return left < 32 ? bits & ((1u << left) - 1u) : bits;
+    }
   } else {
     const uint8_t* row = a.tree + b * a.tree_b + i * a.tree_i + j0;
     if (left >= 32 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {

@@ -54,6 +54,7 @@ struct TtCfg {
   static constexpr int kSmem = kOffPoison + kPoisonWords * 4 + 1024;
   static_assert(kKCols == kDV, "K and V slots have one size");
   static_assert(kSmem <= 232448, "shared memory budget exceeded");
+  static_assert(kTtBM * (kDV * 4 + 16) <= kOffBar, "the output rows fit over Q and the ring");
 };
 
 // Arrive on a barrier that may lie in the peer CTA, releasing this thread's shared-memory
@@ -68,7 +69,8 @@ __device__ __forceinline__ void red_or_cluster(uint32_t addr, uint32_t bits) {
 
 template <typename T, int D>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
-    attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+    attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_vn,
                         const __grid_constant__ TreeArgs a) {
   using C = TtCfg<D>;
@@ -105,7 +107,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
       mbar_init(empty_bar(s), 1);  // both: one MMA commit
       mbar_init(own_bar(s), 1);    // both: this CTA's bytes of a careful V tile
     }
-    mbar_init(q_full, 2 * kTtSoftWarps);  // leader: the softmax warps of both CTAs wrote Q
+    // leader: one arrive.expect_tx + both CTAs' bytes, or the softmax warps of both CTAs wrote Q
+    mbar_init(q_full, a.q_tma ? 1 : 2 * kTtSoftWarps);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full(i), 1);
       mbar_init(p_full(i), 2 * kTtSoftWarps);  // leader: the softmax warps of both CTAs
@@ -114,6 +117,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     mbar_init(o_ready, 1);
     *abort_flag = 0;
     fence_mbar_init();
+    if (a.q_tma) prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
     prefetch_tmap(&tm_kn);
@@ -142,7 +146,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
   const int64_t part_row = (static_cast<int64_t>(item) * a.splits + split) * (2 * kTtBM) + rank * kTtBM;
   auto is_draft = [&](int i) { return t0 + i >= nc; };
   auto key0_of = [&](int i) { return (t0 + i >= nc ? t0 + i - nc : span.c0 + t0 + i) * kTtBN; };
-  auto careful = [&](int i) { return is_draft(i) || key0_of(i) + kTtBN > len; };
+  // Of a causal chunk's tiles of new tokens, those that every row of the pair sees whole are as
+  // plain as committed ones.
+  const int tok_lo = rt * (2 * kTtBM) / a.group, tok_hi = (min((rt + 1) * (2 * kTtBM), rows) - 1) / a.group;
+  auto careful = [&](int i) {
+    const int key0 = key0_of(i);
+    if (!is_draft(i)) return key0 + kTtBN > len;
+    return a.tree != nullptr || a.depth != nullptr || key0 + kTtBN - 1 > tok_lo ||
+           (a.window > 0 && key0 <= tok_hi - a.window);
+  };
   // Ring position of V_i: K_0, then K_{i+1} and V_i in turn.
   auto v_pos = [&](int i) { return static_cast<uint32_t>(min(i + 2, ntiles) * C::kKSlots + i); };
 
@@ -180,6 +192,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         for (int s = 0; s < C::kKSlots; ++s)
           put(is_draft(i) ? &tm_kn : &tm_k, key0_of(i) + kk0, s * (C::kKCols / 64), false);
       };
+      if (a.q_tma) {
+        if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * C::kQBytes);
+        tma_load_5d_pair(base, &tm_q, mapa_shared(q_full, 0), 0, c * a.group, row0 / a.group, 0, b);
+      }
       put_k(0);
       for (int i = 0; i < ntiles && ok; ++i) {
         if (i + 1 < ntiles) put_k(i + 1);
@@ -271,9 +287,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
     auto softmax_sync = [&]() { asm volatile("bar.sync 5, %0;" ::"n"(32 * kTtSoftWarps) : "memory"); };
 
-    // Q rows (row R = i * group + g: head c * group + g of new token i), swizzled as the TMA
-    // would: 64-column blocks of [128 rows x 128 bytes].
-    {
+    // Q rows that no TMA box describes (128 rows are whole tokens only for a group that divides
+    // 128), swizzled as the TMA would: 64-column blocks of [128 rows x 128 bytes].
+    if (!a.q_tma) {
       // Thread: one 16-byte chunk of every (2048 / D)-th row; 8 loads in flight.
       constexpr int kStep = 32 * kTtSoftWarps / (D / 8);
       const int ch = tid % (D / 8);
@@ -282,11 +298,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         uint4 w[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-          const int rr = row0 + q0 + x * kStep;
+          const int qr = row0 + q0 + x * kStep;
+          int i, g;
+          tree_row(a, qr, i, g);
           w[x] = make_uint4(0, 0, 0, 0);
-          if (rr < rows)
-            w[x] = *reinterpret_cast<const uint4*>(
-                a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + rr % a.group) * a.q_h + (rr / a.group) * a.q_t + ch * 8);
+          if (qr < rows)
+            w[x] = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + g) * a.q_h +
+                                                   i * a.q_t + ch * 8);
         }
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
@@ -295,14 +313,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
                        w[x].w);
         }
       }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(q_full, 0));
     }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive_cluster(mapa_shared(q_full, 0));
     const bool drafts = t1 > nc;
     const int j_begin = drafts ? (max(t0, nc) - nc) * kTtBN : 0, j_end = drafts ? min((t1 - nc) * kTtBN, a.n) : 0;
     const int rr = row0 + r;
-    const int tok = rr < rows ? rr / a.group : -1;
+    int tok, head;
+    tree_row(a, rr, tok, head);
+    if (rr >= rows) tok = -1;
     const int dep = tok >= 0 ? tree_depth(a, b, tok) : 0;
     const int first = tok >= 0 ? tree_first(a, len, dep) : len;
     const float scale = a.scale_log2;
@@ -458,6 +478,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         poisoned = bits != 0u && (bits & tree_sees32(a, b, tok, j, dep)) != 0u;
       }
     __syncwarp();
+    // The rows go through shared memory (Q and the ring are idle: every MMA has completed) to
+    // one bulk copy each: a thread that stores its own row touches 32 rows a warp.
+    const int esz = a.splits == 1 ? 2 : 4;
+    const int pitch = C::kDV * esz + 16;  // an odd number of 16-byte chunks: no bank conflicts
     if (good) {
       tc_fence_after();
       const float inv = lt == 0.f ? 0.f : 1.f / lt;  // a row that sees nothing: zeros
@@ -467,38 +491,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         const int col = (C::kDV / 2) * hv + e * 32;  // of this half
         tmem_ld_32x32b_x32(tmem + lane_off + kTtColO + col, ov);
         tmem_wait_ld();
-        if (tok >= 0) {
-          if (poisoned) {
-  #pragma unroll 1
-            for (int j0 = j_begin; j0 < j_end; j0 += 32) {
-              uint32_t bits = poison_of(poison, j0);
-              if (bits != 0u) bits &= tree_sees32(a, b, tok, j0, dep);
-              for (; bits != 0u; bits &= bits - 1u) {
-                const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + (j0 + __ffs(bits) - 1) * a.vn_t + half * C::kDV + col;
+        if (poisoned) {
+#pragma unroll 1
+          for (int j0 = j_begin; j0 < j_end; j0 += 32) {
+            uint32_t bits = poison_of(poison, j0);
+            if (bits != 0u) bits &= tree_sees32(a, b, tok, j0, dep);
+            for (; bits != 0u; bits &= bits - 1u) {
+              const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + (j0 + __ffs(bits) - 1) * a.vn_t + half * C::kDV + col;
 #pragma unroll
-                for (int x = 0; x < 32; ++x)
-                  if (tree_nonfinite<T>(vn[x])) ov[x] = __float_as_uint(__uint_as_float(ov[x]) + tree_f32<T>(vn[x]));
-              }
+              for (int x = 0; x < 32; ++x)
+                if (tree_nonfinite<T>(vn[x])) ov[x] = __float_as_uint(__uint_as_float(ov[x]) + tree_f32<T>(vn[x]));
             }
-          }
-          if (a.splits == 1) {
-            uint16_t* dst = a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + rr % a.group) * a.o_h + tok * a.o_t +
-                            half * C::kDV + col;
-  #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t w[4];
-  #pragma unroll
-              for (int x = 0; x < 4; ++x)
-                w[x] = pack2<T>(__uint_as_float(ov[8 * j + 2 * x]) * inv, __uint_as_float(ov[8 * j + 2 * x + 1]) * inv);
-              *reinterpret_cast<uint4*>(dst + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(a.part_o + (part_row + r) * D + half * C::kDV + col);
-  #pragma unroll
-            for (int j = 0; j < 8; ++j) dst[j] = make_uint4(ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]);
           }
         }
+        const uint32_t dst = base + r * pitch + col * esz;
+        if (a.splits == 1) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              w[x] = pack2<T>(__uint_as_float(ov[8 * j + 2 * x]) * inv, __uint_as_float(ov[8 * j + 2 * x + 1]) * inv);
+            st_shared_v4(dst + 16 * j, w[0], w[1], w[2], w[3]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) st_shared_v4(dst + 16 * j, ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]);
+        }
         __syncwarp();
+      }
+      fence_proxy_async_smem();
+    }
+    // All softmax warps meet here on every path; the rows are stored only if each has staged its own.
+    uint32_t all_good;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "bar.red.and.pred p, 5, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all_good)
+        : "r"(good ? 1u : 0u), "n"(32 * kTtSoftWarps)
+        : "memory");
+    if (all_good) {
+      if (hv == 0 && tok >= 0) {
+        void* dst = a.splits == 1
+                        ? static_cast<void*>(a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + head) * a.o_h + tok * a.o_t +
+                                             half * C::kDV)
+                        : static_cast<void*>(a.part_o + (part_row + r) * D + half * C::kDV);
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(base + r * pitch),
+                     "r"(C::kDV * esz)
+                     : "memory");
+        bulk_commit_group();
+        bulk_wait_group_read<0>();  // (the grid's completion covers the writes)
       }
       if (half == 0 && hv == 0 && tok >= 0) {
         if (a.splits > 1)
@@ -567,11 +611,38 @@ static int encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, 
   return W8_OK;
 }
 
+// 5-D map over q: (64 columns, head, token, 64-column block, batch).  A box {64, group,
+// 128 / group, d / 64, 1} lands as d / 64 swizzled blocks of 128 rows i * group + g.
+static int encode_q(CUtensorMap* map, const w8::TreeArgs& a, bool half, int64_t d) {
+  TreeEncodeFn enc = tree_encode_fn();
+  if (enc == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from the driver");
+    return W8_ERR_CUDA;
+  }
+  const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
+  auto bytes = [&](int64_t size, int64_t stride) { return static_cast<cuuint64_t>(size > 1 ? stride * 2 : d * 2); };
+  const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(a.n),
+                              static_cast<cuuint64_t>(d / 64), static_cast<cuuint64_t>(a.batch)};
+  const cuuint64_t strides[4] = {bytes(heads, a.q_h), bytes(a.n, a.q_t), 128, bytes(a.batch, a.q_b)};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(w8::kTtBM / a.group),
+                             static_cast<cuuint32_t>(d / 64), 1};
+  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+                         const_cast<uint16_t*>(a.q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled (cache attention, q) failed with CUresult %d", static_cast<int>(r));
+    return W8_ERR_CUDA;
+  }
+  return W8_OK;
+}
+
 template <typename T, int D>
 static int tree_tc_go(const w8::TreeArgs& a, int64_t items, int device, cudaStream_t stream) {
   using C = w8::TtCfg<D>;
   constexpr bool kHalf = __is_same(T, __half);
-  CUtensorMap tk, tv, tkn, tvn;
+  CUtensorMap tq, tk, tv, tkn, tvn;
   const uint32_t kb = C::kKCols / 64, vb = C::kDV / 128;
   int st = encode_rows(&tkn, a.kn, kHalf, D, a.n, a.kv_heads, a.batch, a.kn_b, a.kn_h, a.kn_t, w8::kTtKeysPerCta, kb);
   if (st != W8_OK) return st;
@@ -582,6 +653,11 @@ static int tree_tc_go(const w8::TreeArgs& a, int64_t items, int device, cudaStre
     st = encode_rows(&tk, a.k, kHalf, D, a.slots, a.kv_heads, a.batch, a.k_b, a.k_h, a.k_s, w8::kTtKeysPerCta, kb);
     if (st != W8_OK) return st;
     st = encode_rows(&tv, a.v, kHalf, D, a.slots, a.kv_heads, a.batch, a.v_b, a.v_h, a.v_s, w8::kTtBN, vb);
+    if (st != W8_OK) return st;
+  }
+  tq = tkn;
+  if (a.q_tma) {
+    st = encode_q(&tq, a, kHalf, D);
     if (st != W8_OK) return st;
   }
   static bool done[64] = {};
@@ -602,7 +678,7 @@ static int tree_tc_go(const w8::TreeArgs& a, int64_t items, int device, cudaStre
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, w8::attn_tree_tc_kernel<T, D>, tk, tv, tkn, tvn, a));
+  return cuda_status(cudaLaunchKernelEx(&cfg, w8::attn_tree_tc_kernel<T, D>, tq, tk, tv, tkn, tvn, a));
 }
 
 // The tcgen05 schedule of w8_attention_tree (arguments checked by the caller; rows in tiles of

@@ -26,8 +26,11 @@ constexpr int kBeamThreads = 256;
 constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamVals = 16;                              // logits per thread and tile
 constexpr int kBeamTile = kBeamThreads * kBeamVals;        // logits per tile
-constexpr int kBeamCap = 1024;                             // candidates held in shared memory
-constexpr int kBeamPrune = 256;                            // prune after a tile that leaves more
+constexpr int kBeamSuper = 24;                             // tiles between two collections
+constexpr int kBeamSegs = 128;                             // segments collected at once
+constexpr int kBeamCap = kBeamSegs * kBeamVals;            // candidates held in shared memory
+// CTAs of the chunk kernel per SM: what its registers allow without spilling the logits held.
+constexpr int beam_per_sm(size_t size) { return size == 4 ? 3 : 4; }
 constexpr int kBeamMaxN = 64;
 constexpr int kBeamMaxBeams = 32;
 constexpr int kBeamMaxChunks = 32;
@@ -61,19 +64,70 @@ __device__ __forceinline__ unsigned long long beam_key(float f, int token) {
   return (static_cast<unsigned long long>(beam_bits(f)) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(token));
 }
 
+// 16 bytes of logits as fp32 values (4 of fp32, 8 of the 16-bit types).
+__device__ __forceinline__ void beam_unpack(const uint4& w, float* v, float) {
+  v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void beam_unpack(const uint4& w, float* v, __nv_bfloat16) {
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(x[i] << 16);
+    v[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void beam_unpack(const uint4& w, float* v, __half) {
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+// The type's -inf, which stands for what lies behind a chunk.
+__device__ __forceinline__ void beam_fill(uint32_t* w, int i, float v) { w[i] = __float_as_uint(v); }
+__device__ __forceinline__ void beam_fill(uint32_t* w, int i, __nv_bfloat16 v) {
+  const uint32_t u = __bfloat16_as_ushort(v);
+  w[i >> 1] = (i & 1) ? (w[i >> 1] & 0xFFFFu) | u << 16 : u;
+}
+__device__ __forceinline__ void beam_fill(uint32_t* w, int i, __half v) {
+  const uint32_t u = __half_as_ushort(v);
+  w[i >> 1] = (i & 1) ? (w[i >> 1] & 0xFFFFu) | u << 16 : u;
+}
 template <typename T>
-__device__ __forceinline__ float beam_f32(T v);
-template <>
-__device__ __forceinline__ float beam_f32<float>(float v) {
-  return v;
+__device__ __forceinline__ T beam_ninf() {
+  return static_cast<T>(-INFINITY);
 }
-template <>
-__device__ __forceinline__ float beam_f32<__nv_bfloat16>(__nv_bfloat16 v) {
-  return __bfloat162float(v);
+// Largest and least of a thread's logits (NaN passes over to neither).
+__device__ __forceinline__ void beam_range(const uint4* raw, int groups, float, float& top, float& low) {
+  top = -INFINITY, low = INFINITY;
+#pragma unroll
+  for (int g = 0; g < groups; ++g) {
+    const uint32_t w[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, __uint_as_float(w[i])), low = fminf(low, __uint_as_float(w[i]));
+  }
 }
-template <>
-__device__ __forceinline__ float beam_f32<__half>(__half v) {
-  return __half2float(v);
+template <typename T2>
+__device__ __forceinline__ void beam_range2(const uint4* raw, int groups, float& top, float& low) {
+  T2 t = *reinterpret_cast<const T2*>(&raw[0].x), m = t;
+#pragma unroll
+  for (int g = 0; g < groups; ++g) {
+    const uint32_t w[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T2 x = *reinterpret_cast<const T2*>(&w[i]);
+      t = __hmax2(t, x), m = __hmin2(m, x);
+    }
+  }
+  top = fmaxf(static_cast<float>(t.x), static_cast<float>(t.y));
+  low = fminf(static_cast<float>(m.x), static_cast<float>(m.y));
+}
+__device__ __forceinline__ void beam_range(const uint4* raw, int groups, __nv_bfloat16, float& top, float& low) {
+  beam_range2<__nv_bfloat162>(raw, groups, top, low);
+}
+__device__ __forceinline__ void beam_range(const uint4* raw, int groups, __half, float& top, float& low) {
+  beam_range2<__half2>(raw, groups, top, low);
 }
 
 __device__ __forceinline__ float ex2_beam(float x) {
@@ -94,6 +148,7 @@ __device__ __forceinline__ void beam_prune(unsigned long long* cand, int count, 
     if (at < count) {
       mine[i] = cand[at];
       int r = 0;
+#pragma unroll 8
       for (int j = 0; j < count; ++j) r += cand[j] > mine[i];
       rank[i] = r;
     }
@@ -105,11 +160,23 @@ __device__ __forceinline__ void beam_prune(unsigned long long* cand, int count, 
   __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const BeamArgs a) {
+// The softcap in log2 units, cap tanh(l / cap) log2(e), for |l| <= cap: l times a polynomial in
+// l^2, the least maximum-error odd polynomial of degree 13 for tanh on [-1, 1] (fitted by
+// iteratively reweighted least squares: at most 2e-8 off, 9e-8 evaluated in fp32), its
+// coefficients scaled by the caller.  It runs on packed FMAs, so that a logit costs one
+// operation of the special-function unit (its exponential) instead of three.
+constexpr int kTanhTerms = 7;
+__device__ constexpr float kTanh[kTanhTerms] = {0.9999997019767761f,  -0.33332130312919617f, 0.13319583237171173f,
+                                                -0.053265832364559174f, 0.019973276183009148f, -0.005951274652034044f,
+                                                0.0009637702605687082f};
+
+template <typename T, bool CAP>
+__global__ void __launch_bounds__(kBeamThreads, beam_per_sm(sizeof(T))) beam_chunk_kernel(const BeamArgs a) {
   __shared__ unsigned long long cand[kBeamCap];
-  __shared__ int count;
-  __shared__ uint32_t wbest[kBeamWarps];
+  __shared__ float seg_max[kBeamSuper][kBeamThreads];
+  __shared__ int segs[kBeamSegs];
+  __shared__ int count, seg_count;
+  __shared__ uint32_t wbest[kBeamWarps], wtop[kBeamWarps];
   __shared__ float2 wstat[kBeamWarps];
   constexpr int VEC = 16 / sizeof(T), GROUPS = kBeamVals / VEC;
   constexpr float kLog2e = 1.4426950408889634f;
@@ -122,109 +189,205 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const BeamArgs
   const T* x = static_cast<const T*>(a.logits) + b * a.l_b + k * a.l_k;
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   if (tid == 0) count = 0;
-  float mx = -INFINITY, sum = 0.f;  // log2 units
+  float mx = -INFINITY, sum = 0.f;  // reference (log2 units) and sum of 2^(y - reference)
   unsigned long long thr = 0;       // candidates must beat this key
-  bool first = true;
-  __syncthreads();
-  for (int t0 = begin; t0 < end; t0 += kBeamTile) {
-    float v[kBeamVals];
+  const float cap_in = CAP ? 1.f / a.cap : 0.f, cap_out = CAP ? a.cap * kLog2e : 0.f;
+  // (beyond these caps the scaled coefficients leave fp32's range)
+  const float poly_to = CAP && a.cap >= 1e-2f && a.cap <= 1e3f ? a.cap : 0.f;
+  uint64_t tc[kTanhTerms];
+  if constexpr (CAP) {
+    float f = kLog2e;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      const int at = t0 + (g * kBeamThreads + tid) * VEC;
-      if (vec && at + VEC <= end) {
-        const uint4 w = *reinterpret_cast<const uint4*>(x + at);
-        const T* p = reinterpret_cast<const T*>(&w);
+    for (int i = 0; i < kTanhTerms; ++i, f *= cap_in * cap_in) tc[i] = f2_pack(kTanh[i] * f, kTanh[i] * f);
+  }
+  // The thread's segment of a tile: 16 consecutive logits.
+  auto load = [&](int t0, uint4 (&raw)[GROUPS]) {
+    const int at0 = t0 + tid * kBeamVals;
+    if (vec && at0 + kBeamVals <= end) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[g * VEC + i] = beam_f32<T>(p[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[g * VEC + i] = at + i < end ? beam_f32<T>(x[at + i]) : -INFINITY;
-      }
-    }
-    float tm = v[0];
-#pragma unroll
-    for (int i = 1; i < kBeamVals; ++i) tm = fmaxf(tm, v[i]);
-    // ---- e^y
-    float y[kBeamVals], ym;
-    if (a.cap > 0.f) {
-      // cap tanh(l / cap) log2(e), increasing in l
-      const float in = 1.f / a.cap, out = a.cap * kLog2e;
-#pragma unroll
-      for (int i = 0; i < kBeamVals; ++i)  // (an impossible token, or one past the chunk, stays impossible)
-        y[i] = v[i] == -INFINITY ? -INFINITY : out * (one_plus_tanh(v[i] * in) - 1.f);
-      ym = y[0];
-#pragma unroll
-      for (int i = 1; i < kBeamVals; ++i) ym = fmaxf(ym, y[i]);
+      for (int g = 0; g < GROUPS; ++g) raw[g] = reinterpret_cast<const uint4*>(x + at0)[g];
     } else {
 #pragma unroll
-      for (int i = 0; i < kBeamVals; ++i) y[i] = v[i] * kLog2e;
-      ym = tm * kLog2e;
-    }
-    const float mn = fmaxf(mx, ym), ref = mn == -INFINITY ? 0.f : mn;
-    float part = 0.f;
+      for (int g = 0; g < GROUPS; ++g) {
+        uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < kBeamVals; ++i) part += ex2_beam(y[i] - ref);
-    sum = sum * ex2_beam(mx - ref) + part;
-    mx = mn;
-    // ---- candidates
-    if (first) {
-      // Each warp's ceil(n / 8) largest thread maxima are distinct logits: the least over the
-      // warps of the last of them has at least n logits at or above it.
-      uint32_t u = beam_bits(tm), best = 0;
-      for (int i = 0; i < (a.n + kBeamWarps - 1) / kBeamWarps; ++i) {
-        best = __reduce_max_sync(0xffffffffu, u);
-        const unsigned who = __ballot_sync(0xffffffffu, u == best);
-        if (lane == __ffs(who) - 1) u = 0;
+        for (int i = 0; i < VEC; ++i)
+          beam_fill(w, i, at0 + g * VEC + i < end ? x[at0 + g * VEC + i] : beam_ninf<T>());
+        raw[g] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      if (lane == 0) wbest[warp] = best;
-      __syncthreads();
-      best = wbest[0];
-#pragma unroll
-      for (int i = 1; i < kBeamWarps; ++i) best = min(best, wbest[i]);
-      thr = best > 0 ? (static_cast<unsigned long long>(best) << 32) - 1 : 0;  // all keys of `best` pass
-      first = false;
     }
-    uint32_t todo = 0;
-    const uint32_t tb = static_cast<uint32_t>(thr >> 32);
+  };
+  uint4 next[GROUPS];
+  load(begin, next);
+  for (int s0 = begin; s0 < end; s0 += kBeamSuper * kBeamTile) {
+    const int tiles = min(kBeamSuper, (end - s0 + kBeamTile - 1) / kBeamTile);
+    float best_mine = -INFINITY;
+    // ---- the stream
+#pragma unroll 1
+    for (int j = 0; j < tiles; ++j) {
+      const int t0 = s0 + j * kBeamTile;
+      uint4 raw[GROUPS];
 #pragma unroll
-    for (int i = 0; i < kBeamVals; ++i)
-      if (beam_bits(v[i]) >= tb) todo |= 1u << i;
-    while (true) {
-      if (todo) {
+      for (int g = 0; g < GROUPS; ++g) raw[g] = next[g];
+      if (t0 + kBeamTile < end) load(t0 + kBeamTile, next);  // travels meanwhile
+      float tm, low;
+      beam_range(raw, GROUPS, T{}, tm, low);
+      seg_max[j][tid] = tm;
+      best_mine = fmaxf(best_mine, tm);
+      float ym = tm * kLog2e;
+      if constexpr (CAP) ym = tm == -INFINITY ? -INFINITY : cap_out * (one_plus_tanh(tm * cap_in) - 1.f);
+      if (ym > mx) {
+        sum *= ex2_beam(mx - ym);
+        mx = ym;
+      }
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      const uint64_t nref = f2_pack(-ref, -ref);
+      uint64_t part = 0;  // two sums
+      if (!CAP || (tm <= poly_to && low >= -poly_to)) {
 #pragma unroll
-        for (int i = 0; i < kBeamVals; ++i) {
-          if (todo & (1u << i)) {
-            const int at = t0 + ((i / VEC) * kBeamThreads + tid) * VEC + i % VEC;
-            const unsigned long long key = beam_key(v[i], at);
-            if (at >= end || key <= thr) {
-              todo &= ~(1u << i);
+        for (int g = 0; g < GROUPS; ++g) {
+          float v[VEC];
+          beam_unpack(raw[g], v, T{});
+#pragma unroll
+          for (int i = 0; i < VEC; i += 2) {
+            const uint64_t l = f2_pack(v[i], v[i + 1]);
+            uint64_t e;
+            if constexpr (CAP) {
+              const uint64_t u = f2_mul(l, l);
+              uint64_t p = tc[kTanhTerms - 1];
+#pragma unroll
+              for (int q = kTanhTerms - 2; q >= 0; --q) p = f2_fma(p, u, tc[q]);
+              e = f2_fma(l, p, nref);
             } else {
-              const int p = atomicAdd(&count, 1);
-              if (p < kBeamCap) {
-                cand[p] = key;
-                todo &= ~(1u << i);
-              }
+              e = f2_fma(l, f2_pack(kLog2e, kLog2e), nref);
             }
+            float e0, e1;
+            f2_unpack(e, e0, e1);
+            part = f2_add(part, f2_pack(ex2_beam(e0), ex2_beam(e1)));
           }
+        }
+      } else {
+#pragma unroll 1
+        for (int g = 0; g < GROUPS; ++g) {
+          float v[VEC];
+          uint4 w = raw[0];
+#pragma unroll
+          for (int i = 1; i < GROUPS; ++i)
+            if (g == i) w = raw[i];
+          beam_unpack(w, v, T{});
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {  // (an impossible token, or one past the chunk, stays impossible)
+            const float y = v[i] == -INFINITY ? -INFINITY : cap_out * (one_plus_tanh(v[i] * cap_in) - 1.f);
+            part = f2_add(part, f2_pack(ex2_beam(y - ref), 0.f));
+          }
+        }
+      }
+      float p0, p1;
+      f2_unpack(part, p0, p1);
+      sum += p0 + p1;
+    }
+    // ---- the collection.  The thread maxima are distinct logits: bisect for a value that n of
+    // them reach, and not many more.
+    // Bounds: the largest of all, and the least over the warps of each one's ceil(n / 8)-th
+    // largest, which n reach.
+    const uint32_t mine = beam_bits(best_mine);
+    uint32_t left = mine, top = 0, least = 0;
+    for (int i = 0; i < (a.n + kBeamWarps - 1) / kBeamWarps; ++i) {
+      least = __reduce_max_sync(0xffffffffu, left);
+      if (i == 0) top = least;
+      const unsigned who = __ballot_sync(0xffffffffu, left == least);
+      if (lane == __ffs(who) - 1) left = 0;
+    }
+    if (lane == 0) wbest[warp] = least, wtop[warp] = top;
+    if (tid == 0) seg_count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBeamWarps; ++i) least = min(least, wbest[i]), top = max(top, wtop[i]);
+    ++top;  // (no value's bits are all ones)
+    while (top - least > 1) {
+      const uint32_t mid = least + (top - least) / 2;
+      const int reach = __syncthreads_count(mine >= mid);
+      if (reach >= a.n) {
+        least = mid;
+        if (reach <= a.n + a.n / 4) break;
+      } else {
+        top = mid;
+      }
+    }
+    // A segment's best possible key, its maximum at its first token, must beat the n-th best so
+    // far and reach `least`.
+    auto wanted = [&](int j) {
+      const float f = seg_max[j][tid];
+      return f == f && beam_bits(f) >= least && beam_key(f, s0 + j * kBeamTile + tid * kBeamVals) > thr;
+    };
+    if (mine >= least)
+      for (int j = 0; j < tiles; ++j)
+        if (wanted(j)) {
+          const int p = atomicAdd(&seg_count, 1);
+          if (p < kBeamSegs) segs[p] = j * kBeamThreads + tid;
+        }
+    __syncthreads();
+    const int held = count;  // of the collections before
+    const int found = seg_count;
+    if (found <= kBeamSegs && held + found * kBeamVals <= kBeamCap) {
+      for (int e = tid; e < found * kBeamVals; e += kBeamThreads) {
+        const int at = s0 + segs[e / kBeamVals] * kBeamVals + e % kBeamVals;
+        if (at < end) {
+          const float f = static_cast<float>(x[at]);
+          const unsigned long long key = beam_key(f, at);
+          if (beam_bits(f) >= least && key > thr) cand[atomicAdd(&count, 1)] = key;
         }
       }
       __syncthreads();
       const int c = count;
-      if (c <= kBeamPrune) break;
-      // Prune; what found no room tries again against the raised threshold.
-      const int held = min(c, kBeamCap);
-      beam_prune(cand, held, a.n);
-      if (held >= a.n) thr = cand[a.n - 1];
+      beam_prune(cand, c, a.n);
+      if (c >= a.n) thr = cand[a.n - 1];
+      if (tid == 0) count = min(c, a.n);
       __syncthreads();
-      if (tid == 0) count = min(held, a.n);
-      __syncthreads();
-      if (c <= kBeamCap) break;
+    } else {
+      // Too many segments reach the value (ties): tile by tile in the tokens' order, pruning as
+      // the room runs out; what found none tries again against the raised threshold.
+      for (int j = 0; j < tiles; ++j) {
+        uint32_t todo = wanted(j) ? 0xFFFFFFFFu >> (32 - kBeamVals) : 0u;
+        while (__syncthreads_or(todo != 0u)) {
+          uint4 raw[GROUPS];
+          if (todo) load(s0 + j * kBeamTile, raw);
+          if (todo) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+              float v[VEC];
+              beam_unpack(raw[g], v, T{});
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) {
+                const uint32_t bit = 1u << (g * VEC + i);
+                if (todo & bit) {
+                  const int at = s0 + j * kBeamTile + tid * kBeamVals + g * VEC + i;
+                  const unsigned long long key = beam_key(v[i], at);
+                  if (at >= end || key <= thr) {
+                    todo &= ~bit;
+                  } else {
+                    const int p = atomicAdd(&count, 1);
+                    if (p < kBeamCap) {
+                      cand[p] = key;
+                      todo &= ~bit;
+                    }
+                  }
+                }
+              }
+            }
+          }
+          __syncthreads();
+          const int c = min(count, kBeamCap);
+          beam_prune(cand, c, a.n);
+          if (c >= a.n) thr = cand[a.n - 1];
+          if (tid == 0) count = min(c, a.n);
+          __syncthreads();
+        }
+      }
     }
   }
   // ---- the chunk's sorted list and its sum
-  __syncthreads();
-  const int c = min(count, kBeamCap);
-  beam_prune(cand, c, a.n);
+  const int c = count;
   unsigned long long* out = a.keys + (static_cast<int64_t>(row) * a.chunks + blockIdx.x) * a.n;
   for (int i = tid; i < a.n; i += kBeamThreads) out[i] = i < c ? cand[i] : 0ull;  // 0: none (below every key)
 #pragma unroll
@@ -259,7 +422,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
   double* total = reinterpret_cast<double*>(sm);                                  // [beams][m], not increasing
   unsigned long long* list = reinterpret_cast<unsigned long long*>(total + all);  // per warp: [chunks][n]
   int* token = reinterpret_cast<int*>(list + kMergeWarps * a.chunks * a.n);       // [beams][m]
-  int* win = token + all;                                                         // [n]: candidate of each rank
+  int* rank = token + all;                                                        // [beams][m]
+  int* win = rank + all;                                                          // [n]: candidate of each rank
   pdl_launch_dependents();
   pdl_wait();
   for (int k = warp; k < a.beams; k += kMergeWarps) {
@@ -277,14 +441,17 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
       __syncwarp();
       continue;
     }
-    // Z: the chunks' sums joined in 64 bits, always in the same order.
     float2 st = make_float2(-INFINITY, 0.f);
     if (lane < a.chunks) st = a.stats[static_cast<int64_t>(row) * a.chunks + lane];
+    unsigned long long* mine = list + warp * a.chunks * a.n;
+    const unsigned long long* src = a.keys + static_cast<int64_t>(row) * a.chunks * a.n;
+#pragma unroll 4
+    for (int i = lane; i < a.chunks * a.n; i += 32) mine[i] = src[i];
+    // Z: the chunks' sums joined in 64 bits, always in the same order.
     float mx = st.x;
 #pragma unroll
     for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    double sum = st.x == -INFINITY ? static_cast<double>(st.y)
-                                   : static_cast<double>(st.y) * exp2(static_cast<double>(st.x) - static_cast<double>(mx));
+    double sum = st.x == -INFINITY ? static_cast<double>(st.y) : static_cast<double>(st.y) * exp2f(st.x - mx);
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     const double z = 0.69314718055994530942 * (static_cast<double>(mx) + log2(sum));
@@ -296,9 +463,6 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
       __syncwarp();
       continue;
     }
-    unsigned long long* mine = list + warp * a.chunks * a.n;
-    const unsigned long long* src = a.keys + static_cast<int64_t>(row) * a.chunks * a.n;
-    for (int i = lane; i < a.chunks * a.n; i += 32) mine[i] = src[i];
     __syncwarp();
     int head = 0;
     unsigned long long key = lane < a.chunks ? mine[lane * a.n] : 0ull;
@@ -307,16 +471,19 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
       const bool top = static_cast<uint32_t>(key >> 32) == hi;
       const uint32_t lo = __reduce_max_sync(0xffffffffu, top ? static_cast<uint32_t>(key) : 0u);
       if (top && static_cast<uint32_t>(key) == lo) {  // keys are distinct: one lane (m <= vocab: never a 0 key)
-        const double l = static_cast<double>(beam_value(hi));
-        const double y = a.cap > 0.f && !isinf(l) ? static_cast<double>(a.cap) * tanh(l / static_cast<double>(a.cap))
-                         : l > 0.0 && a.cap > 0.f  ? static_cast<double>(a.cap)
-                                                   : l;
-        const double t = score + (y - z);
         token[k * m + i] = static_cast<int>(0xFFFFFFFFu - lo);
-        total[k * m + i] = isfinite(t) ? t : -INFINITY;
+        total[k * m + i] = static_cast<double>(beam_value(hi));
         ++head;
         key = head < a.n ? mine[lane * a.n + head] : 0ull;
       }
+    }
+    __syncwarp();
+    for (int i = lane; i < m; i += 32) {
+      const double l = total[k * m + i];
+      double y = l;
+      if (a.cap > 0.f) y = l == -INFINITY ? l : static_cast<double>(a.cap) * tanh(l / static_cast<double>(a.cap));
+      const double t = score + (y - z);
+      total[k * m + i] = isfinite(t) ? t : -INFINITY;
     }
     __syncwarp();
     if (a.cap > 0.f) {
@@ -335,24 +502,27 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
     }
   }
   __syncthreads();
-  for (int e = tid; e < all; e += kMergeThreads) {
-    const int k = e / m;
+  // A candidate's rank: its place in its own beam's list and, for each other beam, how many of
+  // that list come before it (ties: the lower beam).
+  for (int e = tid; e < all; e += kMergeThreads) rank[e] = e % m;
+  __syncthreads();
+  for (int p = tid; p < all * (a.beams - 1); p += kMergeThreads) {
+    const int e = p % all, k = e / m;
+    int o = p / all;
+    o += o >= k;
     const double t = total[e];
-    int rank = e % m;
-    for (int o = 0; o < a.beams && rank < a.n; ++o) {
-      if (o == k) continue;
-      // how many of beam o's list come before (ties: the lower beam)
-      int lo = 0, hi = m;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        const double v = total[o * m + mid];
-        if (v > t || (v == t && o < k)) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
+    int lo = 0, hi = m;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      const double v = total[o * m + mid];
+      if (v > t || (v == t && o < k)) lo = mid + 1;
+      else hi = mid;
     }
-    if (rank < a.n) win[rank] = e;
+    if (lo) atomicAdd(&rank[e], lo);
   }
+  __syncthreads();
+  for (int e = tid; e < all; e += kMergeThreads)
+    if (rank[e] < a.n) win[rank[e]] = e;
   __syncthreads();
   if (!a.slot_order) {
     for (int i = tid; i < a.n; i += kMergeThreads) {
@@ -396,12 +566,14 @@ struct BeamPlan {
   int chunks, chunk;
 };
 
-// Chunks of whole tiles, at most 32 (a warp merges one list per lane): enough CTAs for four
-// per SM over all rows, or as many as there are tiles.
+// Chunks of whole tiles, at most 32 (a warp merges one list per lane): about two waves of
+// CTAs, so that finished beams leave no SM idle (24 x 8 beams, 20 % finished: 3 chunks 51.4,
+// 6 chunks 45.1, 11 chunks 48.6 us; one sequence of 4 beams takes all 32: 13.6 us against
+// 16.8 with 11).
 static BeamPlan beam_plan(int64_t rows, int64_t vocab, int sms) {
   const int64_t tiles = std::max<int64_t>(1, (vocab + w8::kBeamTile - 1) / w8::kBeamTile);
-  const int64_t want = std::max<int64_t>(1, (static_cast<int64_t>(sms) * 4 + rows - 1) / std::max<int64_t>(rows, 1));
-  const int64_t n = std::min<int64_t>({tiles, want, w8::kBeamMaxChunks});
+  const int64_t want = 8 * static_cast<int64_t>(sms) / std::max<int64_t>(rows, 1);
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>({want, tiles, w8::kBeamMaxChunks}));
   const int64_t per = (tiles + n - 1) / n;
   BeamPlan p;
   p.chunk = static_cast<int>(per * w8::kBeamTile);
@@ -483,19 +655,23 @@ extern "C" int w8_beam_select(const void* logits, int dtype, int64_t stride_b, i
   a.out_scores = out_scores, a.out_beam = out_beam, a.out_token = out_token, a.slot_order = slot_order;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(p.chunks), static_cast<unsigned>(rows));
+  const bool capped = cap > 0.f;
   if (dtype == W8_FP32)
-    st = launch_beam(w8::beam_chunk_kernel<float>, grid, w8::kBeamThreads, 0, s, a);
+    st = launch_beam(capped ? w8::beam_chunk_kernel<float, true> : w8::beam_chunk_kernel<float, false>, grid,
+                     w8::kBeamThreads, 0, s, a);
   else if (dtype == W8_BF16)
-    st = launch_beam(w8::beam_chunk_kernel<__nv_bfloat16>, grid, w8::kBeamThreads, 0, s, a);
+    st = launch_beam(capped ? w8::beam_chunk_kernel<__nv_bfloat16, true> : w8::beam_chunk_kernel<__nv_bfloat16, false>,
+                     grid, w8::kBeamThreads, 0, s, a);
   else
-    st = launch_beam(w8::beam_chunk_kernel<__half>, grid, w8::kBeamThreads, 0, s, a);
+    st = launch_beam(capped ? w8::beam_chunk_kernel<__half, true> : w8::beam_chunk_kernel<__half, false>, grid,
+                     w8::kBeamThreads, 0, s, a);
   if (st != W8_OK) return st;
   const int64_t all = static_cast<int64_t>(a.beams) * a.m;
-  const int smem = static_cast<int>(all * 12 + static_cast<int64_t>(w8::kMergeWarps) * p.chunks * n * 8 + n * 4 + 16);
+  const int smem = static_cast<int>(all * 16 + static_cast<int64_t>(w8::kMergeWarps) * p.chunks * n * 8 + n * 4 + 16);
   static bool done[64] = {};
   if (!done[device]) {
     // Largest: 32 beams x 64 candidates, 8 warps x 32 chunks x 64 keys.
-    W8_CUDA_TRY(cudaFuncSetAttribute(w8::beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    W8_CUDA_TRY(cudaFuncSetAttribute(w8::beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 168 * 1024));
     done[device] = true;
   }
   return launch_beam(w8::beam_merge_kernel, dim3(static_cast<unsigned>(batch)), w8::kMergeThreads, smem, s, a);
