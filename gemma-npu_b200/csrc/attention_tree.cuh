@@ -10,7 +10,7 @@ namespace w8 {
 
 static __device__ int g_tree_status = 0;  // each source file's own
 
-constexpr int kTreeMaxSplits = 256;
+constexpr int kTreeMaxPieces = 512;  // partial results of one item
 
 struct TreeArgs {
   const uint16_t *q, *k, *v, *kn, *vn;
@@ -24,9 +24,12 @@ struct TreeArgs {
   int q_tma;             // q's rows load as TMA boxes (tcgen05 schedule)
   int batch, kv_heads, group, n, slots, window;
   float scale_log2;      // scale * log2(e): scores in log2 units
-  int row_tiles, splits;
-  float* part_o;         // [item][split][BM][D] fp32, item = (b * kv_heads + c) * row_tiles + rt
-  float2* part_ml;       // [item][split][BM]
+  int row_tiles, splits;  // splits: of each item, tcgen05 schedule only
+  // Partial results of an item (item = (b * kv_heads + c) * row_tiles + rt): piece s in slot
+  // item * splits + s, or where `info` gives (first CTA, pieces) as tree_slot says.
+  float* part_o;         // [slot][BM][D] fp32
+  float2* part_ml;       // [slot][BM]
+  int2* info;            // [items], mma.sync schedule
   float* lse;            // [b * kv_heads + c][R] (log2 units) when the weights are wanted
   float* scores;         // [b * kv_heads + c][R][score_pitch] (log2 units), slots then drafts
   int64_t score_pitch;
@@ -63,6 +66,12 @@ template <typename T>
 __device__ __forceinline__ bool tree_nonfinite(uint32_t bits) {
   constexpr uint32_t e = __is_same(T, __half) ? 0x7C00u : 0x7F80u;
   return (bits & e) == e;
+}
+
+// A CTA's range of tiles holds at most one piece that begins an item it does not finish (its
+// last, slot 2 u + 1) and one that continues an item (its first, slot 2 u).
+__device__ __forceinline__ int64_t tree_slot(int2 info, int s) {
+  return s == 0 ? 2 * static_cast<int64_t>(info.x) + 1 : 2 * (static_cast<int64_t>(info.x) + s);
 }
 
 // Row r = i * group + g as (token i, head g of the group) without a division: the product with
