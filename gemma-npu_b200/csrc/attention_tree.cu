@@ -12,12 +12,15 @@
 // step of 2^-8 or 2^-11 on each weight, averaged over the keys).
 //
 // Decode reads every key once for few rows, so it is bound by HBM: R flops per byte for R
-// rows against about 80 for the mma.sync rate over the copy rate.  One CTA of 8 warps owns
-// a tile of 16 MT rows and a range of 64-key tiles.  K and V tiles stream through a
-// cp.async ring (16-byte chunks, XOR-swizzled rows: ldmatrix without bank conflicts); in
-// the S step each warp scores 8 keys for all rows, in the O step it owns D / 8 output
-// columns, so both K and V fragments are read from shared memory once per row tile, and P
-// and the row maxima cross warps through shared memory.
+// rows against about 80 for the mma.sync rate over the copy rate.  A CTA owns 16 MT rows and
+// a range of tiles of 64 to 256 keys (32 to 64 KB boxes, which the TMA moves at full rate),
+// streamed through a ring.  Each of its 8 warps (a team of two at D = 512, half of the output
+// columns each) takes 16 keys at a time for all rows, with a running
+// maximum, sum and output of its own: S = Q K^T, the softmax and O += P V stay in its
+// registers, P turning from the accumulator's layout into the operand's in place, and no warp
+// waits for another until the end of the item, where the 8 results are joined.  (Warps that
+// shared each tile, exchanging P and the maxima through shared memory with three barriers a
+// tile, executed 6 times the instructions: TIMING.)
 //
 // The work is cut by what is there: all tiles of all sequences, in order, are dealt in equal
 // contiguous ranges to as many CTAs as fit the GPU at once (every CTA adds up the lengths for
@@ -25,38 +28,34 @@
 // CTA writes the items that it holds whole, and partial (m, l, O) of at most two others, which
 // attn_tree_combine_kernel joins.
 #include "attention_tree.cuh"
+#include "attn_tc.cuh"
 
 #include <algorithm>
 
 namespace w8 {
 
-constexpr int kTreeThreads = 256;
 constexpr int kTreeWarps = 8;
-constexpr int kTreePPitch = 72;      // P row pitch (elements): 144 bytes, conflict-free ldmatrix
+constexpr int kTreeThreads = 32 * kTreeWarps;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Arrive on `bar` once every earlier cp.async of this thread has landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
 }
 __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x2_t(uint32_t addr, uint32_t (&r)[2]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
-               : "=r"(r[0]), "=r"(r[1])
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
 }
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -75,18 +74,25 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
 template <int D, int MT>
 struct TreeCfg {
   static constexpr int kBM = 16 * MT;
-  static constexpr int kBN = D == 512 ? 32 : 64;  // keys per tile: 16 to 64 KB of K and V each
-  static constexpr int kSlotBytes = kBN * D * 2;
-  static constexpr int kSlots = D == 512 ? 5 : D == 256 ? 3 : 6;
-  static constexpr int kOffRing = kBM * D * 2;
-  static constexpr int kOffP = kOffRing + kSlots * kSlotBytes;
-  static constexpr int kOffRed = kOffP + kBM * kTreePPitch * 2;
-  static constexpr int kOffPoison = kOffRed + kBM * kTreeWarps * 4;
-  static constexpr int kSmem = kOffPoison + kPoisonWords * 4;
+  static constexpr int kTeam = D == 512 ? 2 : 1;            // warps that share 16 keys
+  static constexpr int kGroups = kTreeWarps / kTeam;
+  static constexpr int kSteps = D == 64 ? 2 : 1;            // 16-key steps of a warp in a tile
+  static constexpr int kBN = kGroups * kSteps * 16;         // keys per tile: 256, 128, 128, 64
+  static constexpr int kSlotBytes = kBN * D * 2;            // 32 KB (D <= 128) or 64 KB
+  static constexpr int kSlots = D <= 128 ? 6 : 3;
+  static constexpr int kPitch = D + 8;                      // fp32 row pitch of the joint outputs
+  static constexpr int kOffRing = 0;
+  static constexpr int kOffQ = kSlots * kSlotBytes;
+  static constexpr int kOffStat = kOffQ + kBM * D * 2;      // float [2][kGroups][kBM]: maxima, sums
+  static constexpr int kOffBar = kOffStat + 2 * kGroups * kBM * 4;
+  static constexpr int kNumBars = 2 * kSlots;               // full, empty
+  static constexpr int kSmem = kOffBar + kNumBars * 8 + 16 + 1024;
   static_assert(kSmem <= 232448, "shared memory budget exceeded");
+  static_assert(kGroups * kBM * kPitch * 4 <= kOffQ, "the joint outputs fit over the ring");
 };
 
 // Sum over the block; `sm`: 16 words of shared memory, free again on return.
@@ -124,370 +130,96 @@ __device__ __forceinline__ long long block_scan(long long v, long long* sm, long
 }
 
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(kTreeThreads, 1)
+    attn_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                     const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_vn,
+                     const __grid_constant__ TreeArgs a) {
   using C = TreeCfg<D, MT>;
   constexpr int BM = C::kBM, BN = C::kBN, NS = C::kSlots, CH = D / 8;  // CH: 16-byte chunks per row
-  constexpr int NT = D / 64;                              // n8 output tiles per warp
-  extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t sq = smem_u32(smem), ring = sq + C::kOffRing, sp = sq + C::kOffP;
-  float* red = reinterpret_cast<float*>(smem + C::kOffRed);  // [BM][8]
-  uint32_t* poison = reinterpret_cast<uint32_t*>(smem + C::kOffPoison);
-
+  constexpr int DW = D / C::kTeam;                                     // output columns of a warp
+  constexpr bool kQRegs = MT == 1 && D <= 128;                         // Q's fragments stay in registers
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const uint32_t sq = base + C::kOffQ, bar0 = base + C::kOffBar;
+  float* stat = reinterpret_cast<float*>(smem + C::kOffStat);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffBar + C::kNumBars * 8);
+  auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (NS + s); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rows = a.group * a.n;
 
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(full_bar(s), a.tma ? 1 : kTreeThreads);  // arrive.expect_tx, or every thread's cp.async
+      mbar_init(empty_bar(s), kTreeWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    if (a.tma) {
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+      prefetch_tmap(&tm_kn);
+      prefetch_tmap(&tm_vn);
+    }
+  }
   pdl_launch_dependents();
   pdl_wait();
   // ---- this CTA's range of all tiles.  A pair (sequence, row tile) has kv_heads items of
-  // `tiles` tiles each; pairs and their heads follow one another.
+  // `nt` tiles each; pairs and their heads follow one another.
   const int pairs = a.batch * a.row_tiles;
   auto pair_tiles = [&](int p) {
     const TreeSpan s = tree_span(a, tree_len(a, p / a.row_tiles), p % a.row_tiles, BM, BN);
     return s.c1 - s.c0 + s.nd;
   };
-  long long* sched = reinterpret_cast<long long*>(smem + C::kOffRing);  // (the ring is not in use yet)
-  long long mine = 0;
-  for (int p = tid; p < pairs; p += kTreeThreads) mine += pair_tiles(p);
-  const long long sum_tiles = block_sum(mine, sched);
-  const long long total = sum_tiles * a.kv_heads;
-  const long long ctas = total < gridDim.x ? total : gridDim.x;
-  if (blockIdx.x >= ctas) return;
-  long long pos = total * blockIdx.x / ctas;
-  const long long stop = total * (blockIdx.x + 1) / ctas;
-  // The pair that holds `pos`: a running sum over rounds of 256 pairs.
-  long long before = 0;
-  for (int p0 = 0;; p0 += kTreeThreads) {
-    const int p = p0 + tid;
-    const long long nt = p < pairs ? pair_tiles(p) : 0;
-    long long round;
-    const long long excl = before + block_scan(nt, sched, round);
-    if (nt > 0 && excl * a.kv_heads <= pos && pos < (excl + nt) * a.kv_heads) {
-      sched[16] = p;
-      sched[17] = excl * a.kv_heads;
+  long long total, pos, stop, ctas, item_pos = 0;  // item_pos: first tile of the current item
+  int pair = 0;
+  if (pairs == 1) {
+    total = static_cast<long long>(pair_tiles(0)) * a.kv_heads;
+    ctas = total < gridDim.x ? total : gridDim.x;
+    if (blockIdx.x >= ctas) return;
+    pos = total * blockIdx.x / ctas;
+    stop = total * (blockIdx.x + 1) / ctas;
+    __syncthreads();  // the barriers are initialised
+  } else {
+    long long* sched = reinterpret_cast<long long*>(smem);  // (the ring is not in use yet)
+    long long mine = 0;
+    for (int p = tid; p < pairs; p += kTreeThreads) mine += pair_tiles(p);
+    total = block_sum(mine, sched) * a.kv_heads;
+    ctas = total < gridDim.x ? total : gridDim.x;
+    if (blockIdx.x >= ctas) return;
+    pos = total * blockIdx.x / ctas;
+    stop = total * (blockIdx.x + 1) / ctas;
+    // The pair that holds `pos`: a running sum over rounds of pairs.
+    long long before = 0;
+    for (int p0 = 0;; p0 += kTreeThreads) {
+      const int p = p0 + tid;
+      const long long nt = p < pairs ? pair_tiles(p) : 0;
+      long long round;
+      const long long excl = before + block_scan(nt, sched, round);
+      if (nt > 0 && excl * a.kv_heads <= pos && pos < (excl + nt) * a.kv_heads) {
+        sched[16] = p;
+        sched[17] = excl * a.kv_heads;
+      }
+      __syncthreads();
+      before += round;
+      if (pos < before * a.kv_heads) break;  // (every pair has tiles, and pos < total)
+      if (p0 + kTreeThreads >= pairs) return;  // only if the lengths changed under the call
     }
+    pair = static_cast<int>(sched[16]);
+    item_pos = sched[17];
+    fence_proxy_async_smem();  // the TMA writes the ring next
     __syncthreads();
-    before += round;
-    if (pos < before * a.kv_heads) break;  // (every pair has tiles, and pos < total)
-    if (p0 + kTreeThreads >= pairs) return;  // only if the lengths changed under the call
   }
-  int pair = static_cast<int>(sched[16]);
-  long long item_pos = sched[17];  // first tile of the current item
-  __syncthreads();
   int b = pair / a.row_tiles, rt = pair % a.row_tiles;
   int len = tree_len(a, b);
   TreeSpan span = tree_span(a, len, rt, BM, BN);
   int nt = span.c1 - span.c0 + span.nd;
   int c = static_cast<int>((pos - item_pos) / nt);
   item_pos += static_cast<long long>(c) * nt;
-
-  if (tid < kPoisonWords) poison[tid] = 0u;  // (ordered before its first use by the ring's barriers)
-  while (true) {
-    const int row0 = rt * BM, bc = b * a.kv_heads + c, nc = span.c1 - span.c0;
-    const int t0 = static_cast<int>(pos - item_pos);
-    const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
-    const bool whole = t0 == 0 && t1 == nt;
-    const int64_t part_row = (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * BM;
-    if (t0 == 0 && tid == 0) {
-      // The CTA that begins an item says where its pieces are: one in each CTA up to its last tile's.
-      const long long last = ((item_pos + nt) * ctas - 1) / total;
-      a.info[bc * a.row_tiles + rt] = make_int2(blockIdx.x, static_cast<int>(last - blockIdx.x) + 1);
-    }
-
-    // Row r = i * group + g: query head c * group + g of new token i.
-    auto q_row = [&](int r) {
-      int i, g;
-      tree_row(a, r, i, g);
-      return a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + g) * a.q_h + i * a.q_t;
-    };
-    for (int e = tid; e < BM * CH; e += kTreeThreads) {
-      const int r = e / CH, ch = e % CH;
-      const bool on = row0 + r < rows;
-      cp_async16(sq + r * (D * 2) + ((ch ^ (r & 7)) << 4), (on ? q_row(row0 + r) : a.q) + ch * 8, on);
-    }
-    // Ring step g = 2 (tile - t0) + (0: K, 1: V).
-    const int steps = 2 * (t1 - t0);
-    auto load = [&](int g) {
-      if (g < steps) {
-        const int t = t0 + (g >> 1);
-        const bool is_v = g & 1;
-        const bool draft = t >= nc;
-        const int key0 = (draft ? t - nc : span.c0 + t) * BN, end = draft ? a.n : len;
-        const uint16_t* base;
-        int64_t pitch;
-        if (draft) {
-          base = is_v ? a.vn + b * a.vn_b + c * a.vn_h : a.kn + b * a.kn_b + c * a.kn_h;
-          pitch = is_v ? a.vn_t : a.kn_t;
-        } else {
-          base = is_v ? a.v + b * a.v_b + c * a.v_h : a.k + b * a.k_b + c * a.k_h;
-          pitch = is_v ? a.v_s : a.k_s;
-        }
-        const uint32_t dst = ring + (g % NS) * C::kSlotBytes;
-#pragma unroll
-        for (int e = tid; e < BN * CH; e += kTreeThreads) {
-          const int r = e / CH, ch = e % CH;
-          const bool on = key0 + r < end;  // rows behind the end read as zeros
-          cp_async16(dst + r * (D * 2) + ((ch ^ (r & 7)) << 4), base + (on ? (key0 + r) * pitch : 0) + ch * 8, on);
-        }
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int g = 0; g < NS - 1; ++g) load(g);
-
-    // This thread's rows of each 16-row tile: lane / 4 and lane / 4 + 8.
-    const int rl = lane >> 2;
-    int tok[MT][2], first[MT][2], dep[MT][2];
-    float m[MT][2], l[MT][2], corr[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = row0 + mt * 16 + rl + 8 * h;
-        tok[mt][h] = r < rows ? r / a.group : -1;
-        dep[mt][h] = r < rows ? tree_depth(a, b, tok[mt][h]) : 0;
-        first[mt][h] = r < rows ? tree_first(a, len, dep[mt][h]) : len;
-        m[mt][h] = -INFINITY;
-        l[mt][h] = 0.f;
-        corr[mt][h] = 1.f;
-      }
-    float o[MT][NT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
-
-    bool poisoned = false;  // a new token's V holds an infinity or NaN (in this CTA's tiles)
-    for (int g = 0; g < steps; g += 2) {
-      const int t = t0 + (g >> 1);
-      const bool draft = t >= nc;
-      const int key0 = (draft ? t - nc : span.c0 + t) * BN;
-      // ---- S step
-      cp_wait<NS - 2>();
-      __syncthreads();
-      load(g + NS - 1);
-      const uint32_t sk = ring + (g % NS) * C::kSlotBytes;
-      float s[MT][2][4];  // two chains of the reduction over D
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[mt][e >> 2][e & 3] = 0.f;
-      const int krow = warp * 8 + (lane & 7), arow = lane & 15;
-      const bool scores_here = warp < BN / 8;  // 8 keys a warp
-      if (scores_here) {
-#pragma unroll
-        for (int kk = 0; kk < D / 32; ++kk) {
-        uint32_t kb[4];
-        ldsm_x4(sk + krow * (D * 2) + (((4 * kk + (lane >> 3)) ^ (krow & 7)) << 4), kb);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t qa[4];
-            const int r = mt * 16 + arow;
-            ldsm_x4(sq + r * (D * 2) + (((4 * kk + 2 * h + (lane >> 4)) ^ (r & 7)) << 4), qa);
-            mma16816<T>(s[mt][h], qa, kb[2 * h], kb[2 * h + 1]);
-          }
-      }
-      }
-      const int col = warp * 8 + (lane & 3) * 2;  // this thread's two keys of the tile
-      float x[MT][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int h = e >> 1, key = key0 + col + (e & 1);
-          bool on;
-          if (!scores_here)
-            on = false;
-          else if (draft)
-            on = tok[mt][h] >= 0 && key < a.n && tree_sees(a, b, tok[mt][h], key, dep[mt][h]);
-          else
-            on = key < len && key >= first[mt][h];
-          x[mt][e] = on ? (s[mt][0][e] + s[mt][1][e]) * a.scale_log2 : -INFINITY;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float mx = fmaxf(x[mt][2 * h], x[mt][2 * h + 1]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          if ((lane & 3) == 0) red[(mt * 16 + rl + 8 * h) * kTreeWarps + warp] = mx;
-        }
-      }
-      if (a.scores != nullptr) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = row0 + mt * 16 + rl + 8 * h;
-            if (r < rows && scores_here) {
-              float* dst = a.scores + (static_cast<int64_t>(bc) * rows + r) * a.score_pitch +
-                           (draft ? a.slots : 0) + key0 + col;
-              const int left = (draft ? a.n : len) - key0 - col;
-              if (left > 0) dst[0] = x[mt][2 * h];
-              if (left > 1) dst[1] = x[mt][2 * h + 1];
-            }
-          }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = mt * 16 + rl + 8 * h;
-          const float4 lo = *reinterpret_cast<const float4*>(red + r * kTreeWarps);
-          const float4 hi = *reinterpret_cast<const float4*>(red + r * kTreeWarps + 4);
-          const float mx = fmaxf(fmaxf(fmaxf(lo.x, lo.y), fmaxf(lo.z, lo.w)),
-                                 fmaxf(fmaxf(hi.x, hi.y), fmaxf(hi.z, hi.w)));
-          const float mn = fmaxf(m[mt][h], mx);
-          const float ref = mn == -INFINITY ? 0.f : mn;
-          corr[mt][h] = ex2_tree(m[mt][h] - ref);
-          m[mt][h] = mn;
-          const float p0 = ex2_tree(x[mt][2 * h] - ref), p1 = ex2_tree(x[mt][2 * h + 1] - ref);
-          l[mt][h] = l[mt][h] * corr[mt][h] + (p0 + p1);
-          *reinterpret_cast<uint32_t*>(smem + C::kOffP + (r * kTreePPitch + col) * 2) = pack2<T>(p0, p1);
-        }
-      // ---- O step
-      cp_wait<NS - 2>();
-      __syncthreads();
-      load(g + NS);
-      const uint32_t sv = ring + ((g + 1) % NS) * C::kSlotBytes;
-      if (draft) {
-        // A new token's values may be infinite or NaN where some row must not see them, and
-        // 0 * NaN is NaN in the product: take them out here, and add them at the end to the
-        // rows that do see them.
-        bool any = false;
-        for (int e = tid; e < BN * CH; e += kTreeThreads) {
-          bool bad = false;
-          uint32_t* w = reinterpret_cast<uint32_t*>(smem + C::kOffRing + ((g + 1) % NS) * C::kSlotBytes) + e * 4;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t v = w[i];
-            const bool lo = tree_nonfinite<T>(v), hi = tree_nonfinite<T>(v >> 16);
-            if (lo || hi) {
-              w[i] = (lo ? 0u : v & 0xFFFFu) | (hi ? 0u : v & 0xFFFF0000u);
-              bad = true;
-            }
-          }
-          if (bad) {
-            poison_mark(poison, key0 + e / CH);
-            any = true;
-          }
-        }
-        if (__syncthreads_or(any)) poisoned = true;
-      }
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if (__any_sync(0xffffffffu, corr[mt][0] != 1.f || corr[mt][1] != 1.f)) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            o[mt][n][0] *= corr[mt][0];
-            o[mt][n][1] *= corr[mt][0];
-            o[mt][n][2] *= corr[mt][1];
-            o[mt][n][3] *= corr[mt][1];
-          }
-        }
-      }
-#pragma unroll
-      for (int ks = 0; ks < BN / 16; ++ks) {
-        uint32_t pa[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-          ldsm_x4(sp + ((mt * 16 + arow) * kTreePPitch + ks * 16 + (lane >> 4) * 8) * 2, pa[mt]);
-        const int vr = ks * 16 + (lane & 15);
-        if constexpr (NT == 1) {
-          uint32_t vb[2];
-          ldsm_x2_t(sv + vr * (D * 2) + (((warp * NT) ^ (vr & 7)) << 4), vb);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) mma16816<T>(o[mt][0], pa[mt], vb[0], vb[1]);
-        } else {
-#pragma unroll
-          for (int n = 0; n < NT; n += 2) {
-            uint32_t vb[4];
-            ldsm_x4_t(sv + vr * (D * 2) + (((warp * NT + n + (lane >> 4)) ^ (vr & 7)) << 4), vb);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma16816<T>(o[mt][n], pa[mt], vb[0], vb[1]);
-              mma16816<T>(o[mt][n + 1], pa[mt], vb[2], vb[3]);
-            }
-          }
-        }
-      }
-    }
-    cp_wait<0>();
-    if (poisoned) {
-      const int j0 = (max(t0, nc) - nc) * BN, j1 = min((t1 - nc) * BN, a.n);
-#pragma unroll 1
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h)
-          if (tok[mt][h] >= 0)
-#pragma unroll 1
-            for (int jw = j0; jw < j1; jw += 32) {
-              uint32_t bits = poison_of(poison, jw);
-              if (bits != 0u) bits &= tree_sees32(a, b, tok[mt][h], jw, dep[mt][h]);
-#pragma unroll 1
-              for (; bits != 0u; bits &= bits - 1u)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) {
-                    const uint16_t v = a.vn[b * a.vn_b + c * a.vn_h + (jw + __ffs(bits) - 1) * a.vn_t + warp * (D / 8) +
-                                            n * 8 + (lane & 3) * 2 + e];
-                    // (static register indexes only: both rows are written under a select)
-                    const float add = tree_nonfinite<T>(v) ? tree_f32<T>(v) : 0.f;
-#pragma unroll
-                    for (int mm = 0; mm < MT; ++mm) {
-                      if (mm == mt && h == 0) o[mm][n][e] += add;
-                      if (mm == mt && h == 1) o[mm][n][2 + e] += add;
-                    }
-                  }
-            }
-    }
-
-    // ---- row sums over the warps, then the output or this split's partial
-    __syncthreads();
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v = l[mt][h];
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        v += __shfl_xor_sync(0xffffffffu, v, 2);
-        if ((lane & 3) == 0) red[(mt * 16 + rl + 8 * h) * kTreeWarps + warp] = v;
-      }
-    __syncthreads();
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = mt * 16 + rl + 8 * h;
-        if (row0 + r >= rows) continue;
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kTreeWarps; ++w) sum += red[r * kTreeWarps + w];
-        const int cols = warp * (D / 8) + (lane & 3) * 2;
-        if (whole) {
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: zeros
-          const int i = (row0 + r) / a.group, gq = (row0 + r) % a.group;
-          uint16_t* dst = a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + gq) * a.o_h + i * a.o_t + cols;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<uint32_t*>(dst + n * 8) = pack2<T>(o[mt][n][2 * h] * inv, o[mt][n][2 * h + 1] * inv);
-          if (a.lse != nullptr && warp == 0 && (lane & 3) == 0)
-            a.lse[static_cast<int64_t>(bc) * rows + row0 + r] = sum == 0.f ? INFINITY : m[mt][h] + log2f(sum);
-        } else {
-          float* dst = a.part_o + (part_row + r) * D + cols;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
-          if (warp == 0 && (lane & 3) == 0) a.part_ml[part_row + r] = make_float2(m[mt][h], sum);
-        }
-      }
-    pos += t1 - t0;
-    if (pos >= stop) break;
-    // ---- the next item: the next head, or the next pair's first
+  // The next item: the next head, or the next pair's first.
+  auto advance = [&]() {
     item_pos += nt;
     if (++c == a.kv_heads) {
       c = 0;
@@ -499,8 +231,374 @@ __global__ void __launch_bounds__(kTreeThreads) attn_tree_kernel(const TreeArgs 
       span = tree_span(a, len, rt, BM, BN);
       nt = span.c1 - span.c0 + span.nd;
     }
-    __syncthreads();  // everybody has left the ring, Q and the row sums
-    if (poisoned && tid < kPoisonWords) poison[tid] = 0u;
+  };
+
+  const int grp = warp / C::kTeam, part = warp % C::kTeam;  // 16-key group of a step; column part
+  const int rl = lane >> 2, arow = lane & 15;
+  uint32_t g = 0;  // ring steps so far (each tile's K, then V)
+  bool ok = true;
+  while (true) {
+    const int row0 = rt * BM, bc = b * a.kv_heads + c, nc = span.c1 - span.c0;
+    const int t0 = static_cast<int>(pos - item_pos);
+    const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
+    const bool whole = t0 == 0 && t1 == nt;
+    const int64_t part_row = (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * BM;
+    if (t0 == 0 && tid == 0) {
+      // The CTA that begins an item says where its pieces are: one in each CTA up to its last tile's.
+      const long long last = ((item_pos + nt) * ctas - 1) / total;
+      a.info[bc * a.row_tiles + rt] = make_int2(blockIdx.x, static_cast<int>(last - blockIdx.x) + 1);
+    }
+    // Ring step `i` of this item (tile t0 + i / 2, K or V) into its slot, once every warp has left
+    // it: one thread's TMA, or (strides that no map takes) every thread's 16-byte copies into
+    // the same layout, rows behind the tensor's end as zeros.
+    const uint32_t g_item = g;
+    auto load = [&](int i) {
+      if (i >= 2 * (t1 - t0)) return;
+      const int t = t0 + (i >> 1), kv = i & 1;
+      const bool draft = t >= nc;
+      const int key0 = (draft ? t - nc : span.c0 + t) * BN;
+      const uint32_t step = g_item + i, slot = step % NS, dst = base + slot * C::kSlotBytes;
+      const bool free = mbar_wait_bounded(empty_bar(slot), ((step / NS) & 1u) ^ 1u, abort_flag, &g_tree_status);
+      if (!free) return;
+      if (a.tma) {
+        mbar_arrive_expect_tx(full_bar(slot), C::kSlotBytes);
+        tma_load_5d(dst, kv ? (draft ? &tm_vn : &tm_v) : (draft ? &tm_kn : &tm_k), full_bar(slot), 0, key0, 0, c, b);
+      } else {
+        const uint16_t* src = kv ? (draft ? a.vn + b * a.vn_b + c * a.vn_h : a.v + b * a.v_b + c * a.v_h)
+                                 : (draft ? a.kn + b * a.kn_b + c * a.kn_h : a.k + b * a.k_b + c * a.k_h);
+        const int64_t pitch = kv ? (draft ? a.vn_t : a.v_s) : (draft ? a.kn_t : a.k_s);
+        const int rows_here = draft ? a.n : a.slots;
+#pragma unroll 2
+        for (int e = tid; e < BN * CH; e += kTreeThreads) {
+          const int r = e / CH, ch = e % CH;
+          const bool on = key0 + r < rows_here;
+          cp_async16(dst + (ch >> 3) * (BN * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
+                     src + (on ? (key0 + r) * pitch : 0) + ch * 8, on);
+        }
+        cp_async_arrive(full_bar(slot));
+      }
+    };
+    // The step NS - 1 ahead loads as a step begins; the warps take turns, so that waiting for the
+    // others to leave the slot holds up one of them only.
+    auto load_ahead = [&](int i) {
+      if (!a.tma || (warp == static_cast<int>((g_item + i) % kTreeWarps) && lane == 0)) load(i + NS - 1);
+      __syncwarp();
+    };
+    if (!a.tma || tid == 0)
+      for (int i = 0; i < NS - 1; ++i) load(i);
+    __syncwarp();
+
+    // Row r = i * group + g: query head c * group + g of new token i.
+    for (int e = tid; e < BM * CH; e += kTreeThreads) {
+      const int r = e / CH, ch = e % CH;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (row0 + r < rows) {
+        int i, gq;
+        tree_row(a, row0 + r, i, gq);
+        w = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + gq) * a.q_h + i * a.q_t +
+                                            ch * 8);
+      }
+      st_shared_v4(sq + r * (D * 2) + ((ch ^ (r & 7)) << 4), w.x, w.y, w.z, w.w);
+    }
+    // This thread's rows of each 16-row tile: lane / 4 and lane / 4 + 8.
+    int tok[MT][2], dep[MT][2], first[MT][2];
+    float m[MT][2], l[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = row0 + mt * 16 + rl + 8 * h;
+        int gq;
+        tree_row(a, r, tok[mt][h], gq);
+        if (r >= rows) tok[mt][h] = -1;
+        dep[mt][h] = r < rows ? tree_depth(a, b, tok[mt][h]) : 0;
+        first[mt][h] = r < rows ? tree_first(a, len, dep[mt][h]) : len;
+        m[mt][h] = -INFINITY;
+        l[mt][h] = 0.f;
+      }
+    float o[MT][DW / 8][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int n = 0; n < DW / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+    __syncthreads();
+    uint32_t qf[kQRegs ? D / 16 : 1][4];
+    if constexpr (kQRegs) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        ldsm_x4(sq + arow * (D * 2) + (((2 * kk + (lane >> 4)) ^ (arow & 7)) << 4), qf[kk]);
+    }
+
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t, g += 2) {
+      const bool draft = t >= nc;
+      const int tile0 = (draft ? t - nc : span.c0 + t) * BN, end = draft ? a.n : len;
+      const uint32_t sk = base + (g % NS) * C::kSlotBytes, sv = base + ((g + 1) % NS) * C::kSlotBytes;
+      load_ahead(2 * (t - t0));
+      if (ok) ok = mbar_wait_bounded(full_bar(g % NS), (g / NS) & 1u, abort_flag, &g_tree_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+#pragma unroll
+      for (int st = 0; st < C::kSteps; ++st) {
+        const int kr = (grp * C::kSteps + st) * 16, key0 = tile0 + kr;  // this step's keys
+        // ---- S = Q K^T, 16 keys
+        float s[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[mt][e >> 2][e & 3] = 0.f;
+        const int krow = kr + (lane & 7) + ((lane >> 4) << 3);
+        const uint32_t kbase = sk + krow * 128;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t kb[4];
+          ldsm_x4(kbase + (kk >> 2) * (BN * 128) + ((((kk & 3) * 2 + ((lane >> 3) & 1)) ^ (krow & 7)) << 4), kb);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            if constexpr (kQRegs) {
+              mma16816<T>(s[mt][0], qf[kk], kb[0], kb[1]);
+              mma16816<T>(s[mt][1], qf[kk], kb[2], kb[3]);
+            } else {
+              uint32_t qa[4];
+              const int r = mt * 16 + arow;
+              ldsm_x4(sq + r * (D * 2) + (((2 * kk + (lane >> 4)) ^ (r & 7)) << 4), qa);
+              mma16816<T>(s[mt][0], qa, kb[0], kb[1]);
+              mma16816<T>(s[mt][1], qa, kb[2], kb[3]);
+            }
+          }
+        }
+        // ---- masks and the running softmax.  Columns of a thread: key0 + 8 n + 2 (lane % 4) + {0, 1}.
+        const int col = (lane & 3) * 2;
+        float mx[MT][2];
+        bool move = false;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key = key0 + 8 * n + col + e;
+                const bool on = draft ? tok[mt][h] >= 0 && key < end && tree_sees(a, b, tok[mt][h], key, dep[mt][h])
+                                      : key < end && key >= first[mt][h];
+                float& v = s[mt][n][2 * h + e];
+                v = on ? v * a.scale_log2 : -INFINITY;
+                x = fmaxf(x, v);
+              }
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            mx[mt][h] = x;
+            move |= x > m[mt][h] + 8.f;
+            if (a.scores != nullptr && part == 0) {
+              const int r = row0 + mt * 16 + rl + 8 * h;
+              if (r < rows) {
+                float* dst = a.scores + (static_cast<int64_t>(bc) * rows + r) * a.score_pitch + (draft ? a.draft_at : 0) +
+                             key0 + col;
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                  const int left = end - key0 - 8 * n - col;
+                  if (left > 1)
+                    *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(s[mt][n][2 * h], s[mt][n][2 * h + 1]);
+                  else if (left > 0)
+                    dst[8 * n] = s[mt][n][2 * h];
+                }
+              }
+            }
+          }
+        // A row's reference moves only when its maximum exceeds it by more than 8 (log2 units), so
+        // the output is seldom rescaled and P <= 2^8.
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const bool mv = mx[mt][h] > m[mt][h] + 8.f;
+              const float corr = mv ? ex2_tree(m[mt][h] - mx[mt][h]) : 1.f;
+              if (mv) m[mt][h] = mx[mt][h];
+              l[mt][h] *= corr;
+#pragma unroll
+              for (int n = 0; n < DW / 8; ++n) {
+                o[mt][n][2 * h] *= corr;
+                o[mt][n][2 * h + 1] *= corr;
+              }
+            }
+        }
+        uint32_t pa[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float ref = m[mt][h] == -INFINITY ? 0.f : m[mt][h];
+            float p[2][2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) p[n][e] = ex2_tree(s[mt][n][2 * h + e] - ref);
+            l[mt][h] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
+            // The accumulator's layout of 16 x 16 is the A operand's.
+            pa[mt][h] = pack2<T>(p[0][0], p[0][1]);
+            pa[mt][2 + h] = pack2<T>(p[1][0], p[1][1]);
+          }
+        if (st == C::kSteps - 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty_bar(g % NS));
+          load_ahead(2 * (t - t0) + 1);  // (into the slot that this warp has just left too)
+        }
+        // ---- O += P V
+        if (st == 0) {
+          ok = mbar_wait_bounded(full_bar((g + 1) % NS), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        uint32_t bad = 0;  // keys of this step whose values are not all finite (new tokens only)
+        if (draft || key0 + 16 > end) {
+          // Rows behind the length may hold anything and 0 * NaN is NaN: zeros.  So may a new token's
+          // values where some row must not see them: cleared here, added below to the rows that do.
+          for (int e = lane; e < 16 * (DW / 8); e += 32) {
+            const int r = e % 16, ch = part * (DW / 8) + e / 16;
+            uint4* w = reinterpret_cast<uint4*>(smem + (sv - base) + (ch >> 3) * (BN * 128) + (kr + r) * 128 +
+                                                (((ch & 7) ^ ((kr + r) & 7)) << 4));
+            if (key0 + r >= end) {
+              *w = make_uint4(0, 0, 0, 0);
+            } else if (draft) {
+              uint4 x = *w;
+              if (nonfinite_bits<T>(x.x) | nonfinite_bits<T>(x.y) | nonfinite_bits<T>(x.z) | nonfinite_bits<T>(x.w)) {
+                uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) xs[q] &= ~((nonfinite_bits<T>(xs[q]) >> 15) * 0xFFFFu);
+                *w = x;
+                bad |= 1u << r;
+              }
+            }
+          }
+          bad = __reduce_or_sync(0xffffffffu, bad);
+          fence_proxy_async_smem();  // (the TMA writes this slot again later)
+          __syncwarp();
+        }
+        const int vrow = kr + arow;
+        const uint32_t vbase = sv + vrow * 128;
+#pragma unroll
+        for (int n = 0; n < DW / 8; n += 2) {
+          uint32_t vb[4];
+          const int ch = part * (DW / 8) + n + (lane >> 4);
+          ldsm_x4_t(vbase + (ch >> 3) * (BN * 128) + (((ch & 7) ^ (vrow & 7)) << 4), vb);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16816<T>(o[mt][n], pa[mt], vb[0], vb[1]);
+            mma16816<T>(o[mt][n + 1], pa[mt], vb[2], vb[3]);
+          }
+        }
+#pragma unroll 1
+        for (; bad != 0u; bad &= bad - 1u) {
+          const int j = key0 + __ffs(bad) - 1;
+          const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + j * a.vn_t + part * DW + (lane & 3) * 2;
+          bool sees[MT][2];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) sees[mt][h] = tok[mt][h] >= 0 && tree_sees(a, b, tok[mt][h], j, dep[mt][h]);
+#pragma unroll
+          for (int n = 0; n < DW / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint16_t v = vn[n * 8 + e];
+              if (tree_nonfinite<T>(v)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h)
+                    if (sees[mt][h]) o[mt][n][2 * h + e] += tree_f32<T>(v);
+              }
+            }
+        }
+      }
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty_bar((g + 1) % NS));
+    }
+
+    // ---- the groups' results joined: M = max m_w, O = sum 2^(m_w - M) O_w over the ring
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
+        l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
+        if ((lane & 3) == 0 && part == 0) {
+          const int r = mt * 16 + rl + 8 * h;
+          stat[grp * BM + r] = m[mt][h];
+          stat[(C::kGroups + grp) * BM + r] = l[mt][h];
+        }
+      }
+    ok = __syncthreads_and(ok);  // everybody has left the ring; the statistics are there
+    float* joint = reinterpret_cast<float*>(smem);  // [group][BM][pitch]
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = mt * 16 + rl + 8 * h;
+        float top = stat[r];
+#pragma unroll
+        for (int w = 1; w < C::kGroups; ++w) top = fmaxf(top, stat[w * BM + r]);
+        const float f = m[mt][h] == -INFINITY ? 0.f : ex2_tree(m[mt][h] - top);
+        float* dst = joint + (grp * BM + r) * C::kPitch + part * DW + (lane & 3) * 2;
+        // (a group that saw nothing adds zeros, except what a NaN score made of it)
+        const bool none = m[mt][h] == -INFINITY && l[mt][h] == 0.f;
+#pragma unroll
+        for (int n = 0; n < DW / 8; ++n) {
+          const float s0 = m[mt][h] == -INFINITY ? 1.f : f;
+          *reinterpret_cast<float2*>(dst + 8 * n) =
+              none ? make_float2(0.f, 0.f) : make_float2(o[mt][n][2 * h] * s0, o[mt][n][2 * h + 1] * s0);
+        }
+      }
+    __syncthreads();
+    if (ok) {
+      constexpr int Q4 = D / 4;  // float4 columns per row
+      for (int e = tid; e < BM * Q4; e += kTreeThreads) {
+        const int r = e / Q4, q4 = e % Q4;
+        if (row0 + r >= rows) break;
+        float top = stat[r];
+#pragma unroll
+        for (int w = 1; w < C::kGroups; ++w) top = fmaxf(top, stat[w * BM + r]);
+        float sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < C::kGroups; ++w) {
+          const float mw = stat[w * BM + r];
+          sum += (mw == -INFINITY ? 1.f : ex2_tree(mw - top)) * stat[(C::kGroups + w) * BM + r];
+          const float4 x = *reinterpret_cast<const float4*>(joint + (w * BM + r) * C::kPitch + 4 * q4);
+          v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: zeros
+          int i, gq;
+          tree_row(a, row0 + r, i, gq);
+          uint16_t* dst = a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + gq) * a.o_h + i * a.o_t + 4 * q4;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+          if (a.lse != nullptr && q4 == 0)
+            a.lse[static_cast<int64_t>(bc) * rows + row0 + r] = sum == 0.f ? INFINITY : top + log2f(sum);
+        } else {
+          *reinterpret_cast<float4*>(a.part_o + (part_row + r) * D + 4 * q4) = v;
+          if (q4 == 0) a.part_ml[part_row + r] = make_float2(top, sum);
+        }
+      }
+    }
+    if (!ok) {
+      // A wait gave up: let the copies in flight land before the CTA exits.
+      const unsigned long long since = globaltimer();
+      while (globaltimer() - since < 50000ull) {
+      }
+      break;
+    }
+    pos += t1 - t0;
+    if (pos >= stop) break;
+    advance();
+    fence_proxy_async_smem();  // the joint outputs lay where the TMA writes next
+    __syncthreads();  // the ring, Q and the statistics are free
   }
 }
 
@@ -542,7 +640,8 @@ __global__ void __launch_bounds__(256) attn_tree_combine_kernel(const TreeArgs a
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kTreeMaxPieces / 256; ++i) {
-    const float f = ml[i].x == -INFINITY ? 0.f : ex2_tree(ml[i].x - mx);
+    // (nothing seen: 0; a maximum of -inf with another sum: NaN scores, which must show)
+    const float f = ml[i].x != -INFINITY ? ex2_tree(ml[i].x - mx) : ml[i].y == 0.f ? 0.f : 1.f;
     if (tid + 256 * i < pieces) {
       w[tid + 256 * i] = f;
       sum += f * ml[i].y;
@@ -585,45 +684,62 @@ __global__ void __launch_bounds__(256) attn_tree_combine_kernel(const TreeArgs a
 
 // Accumulated weights: slot j gets weights[j] + sum over the R rows of p_rj, p from the stored
 // scores and the rows' log-sum-exp (the sums in the rows' order: the same bits every time).
+// Four slots a thread, 16-byte loads of four rows in flight: bound by reading the scores.
 __global__ void __launch_bounds__(256) attn_tree_weights_kernel(const TreeArgs a) {
-  extern __shared__ float sm[];
+  __shared__ float sm_lse[256];
+  __shared__ int sm_first[256];
   const int rows = a.group * a.n, bc = blockIdx.y, b = bc / a.kv_heads, c = bc % a.kv_heads;
   pdl_launch_dependents();
   pdl_wait();
   const int len = tree_len(a, b);
-  const int j = blockIdx.x * 256 + threadIdx.x;  // slots [0, S), then drafts
-  if (blockIdx.x * 256 >= len && (blockIdx.x + 1) * 256 <= a.slots) return;
-  const bool draft = j >= a.slots;
-  const bool on = draft ? j - a.slots < a.n : j < len;
-  const float* x = a.scores + static_cast<int64_t>(bc) * rows * a.score_pitch + j;
-  const float* lse = a.lse + static_cast<int64_t>(bc) * rows;
-  float sum = 0.f;
+  const int j0 = (blockIdx.x * 256 + threadIdx.x) * 4;  // slots [0, draft_at), then new tokens
+  const int begin = blockIdx.x * 1024;
+  if (begin >= len && begin + 1024 <= a.draft_at) return;
+  const bool draft = j0 >= a.draft_at;
+  const int end = draft ? a.draft_at + a.n : len;
+  const float* x = a.scores + static_cast<int64_t>(bc) * rows * a.score_pitch + j0;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int r0 = 0; r0 < rows; r0 += 256) {
     // (lse, first visible slot) of up to 256 rows at a time
     __syncthreads();
     if (r0 + threadIdx.x < rows) {
-      const int r = r0 + threadIdx.x, i = r / a.group;
-      sm[threadIdx.x] = lse[r];
-      reinterpret_cast<int*>(sm + 256)[threadIdx.x] = tree_first(a, len, tree_depth(a, b, i));
+      int i, gq;
+      tree_row(a, r0 + threadIdx.x, i, gq);
+      sm_lse[threadIdx.x] = a.lse[static_cast<int64_t>(bc) * rows + r0 + threadIdx.x];
+      sm_first[threadIdx.x] = tree_first(a, len, tree_depth(a, b, i));
     }
     __syncthreads();
-    if (on) {
+    if (j0 < end) {
       const int n = min(256, rows - r0);
 #pragma unroll 4
       for (int q = 0; q < n; ++q) {
-        const int i = (r0 + q) / a.group;
-        // Keys that no tile of the row covered were never scored.
-        const bool seen = draft ? (a.tree != nullptr || j - a.slots <= i)
-                                : j >= reinterpret_cast<const int*>(sm + 256)[q];
-        if (seen) sum += ex2_tree(x[static_cast<int64_t>(r0 + q) * a.score_pitch] - sm[q]);
+        const float4 v = *reinterpret_cast<const float4*>(x + static_cast<int64_t>(r0 + q) * a.score_pitch);
+        const float e[4] = {v.x, v.y, v.z, v.w};
+        // Of this thread's four, [lo, hi) were scored: no tile of the row covers slots before the
+        // first that it sees, nor a causal chunk's tokens behind it.
+        int lo, hi;
+        if (draft) {
+          int i, gq;
+          tree_row(a, r0 + q, i, gq);
+          lo = 0, hi = a.draft_at + (a.tree != nullptr ? a.n : i + 1) - j0;
+        } else {
+          lo = sm_first[q] - j0, hi = len - j0;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k >= lo && k < hi) sum[k] += ex2_tree(e[k] - sm_lse[q]);
       }
     }
   }
-  if (!on) return;
-  if (draft)
-    a.w_new[static_cast<int64_t>(bc) * a.n + j - a.slots] = sum;
-  else
-    a.w_out[b * a.wo_b + c * a.wo_h + j] = a.w_in[b * a.wi_b + c * a.wi_h + j] + sum;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int j = j0 + k;
+    if (j >= end) break;
+    if (draft)
+      a.w_new[static_cast<int64_t>(bc) * a.n + j - a.draft_at] = sum[k];
+    else
+      a.w_out[b * a.wo_b + c * a.wo_h + j] = a.w_in[b * a.wi_b + c * a.wi_h + j] + sum[k];
+  }
 }
 
 }  // namespace w8
@@ -632,6 +748,8 @@ namespace w8host {
 
 int require_sm100(int* device);
 
+int tree_encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, int64_t n, int64_t heads, int64_t batch,
+                     int64_t s_b, int64_t s_h, int64_t s_n, uint32_t rows, uint32_t blocks);
 int tree_tc(const w8::TreeArgs& a, bool half, int64_t d, int64_t items, int device, cudaStream_t stream);
 int tree_tc_device_status(int clear, int* out);
 
@@ -643,19 +761,19 @@ struct TreePlan {
   int64_t items;
 };
 
-// More than 32 rows a cache head at head_dim >= 128 go to the tcgen05 schedule (`tma`: its
-// maps can describe the tensors), whose tiles take 256 rows; fewer to mma.sync tiles of 16
-// or 32, which a split key axis spreads over more SMs.
+// The tcgen05 schedule takes 256 rows a tile and keeps up with HBM for any number of them, so
+// it is for more rows a cache head than one mma.sync tile has (`tma`: its maps can describe
+// the tensors): with 16 or 32 rows, mma.sync tiles spread a sequence's keys over all SMs.
 static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t n, int64_t d, int64_t slots,
                           int64_t window, int sms, bool tma) {
   TreePlan p;
   const int64_t rows = group * n;
-  p.tc = tma && rows > 32 && d >= 128;
-  p.bm = p.tc ? 256 : rows > 16 && d <= 256 ? 32 : 16;
+  p.tc = tma && d >= 128 && rows > (d == 128 ? 32 : 16);
+  p.bm = p.tc ? 256 : rows > 16 && d <= 128 ? 32 : 16;
   p.row_tiles = static_cast<int>((rows + p.bm - 1) / p.bm);
   p.items = batch * kv_heads * p.row_tiles;
   // Keys of one row tile: with a window, those its tokens see.
-  const int64_t bn = p.tc ? 128 : d == 512 ? 32 : 64;
+  const int64_t bn = p.tc ? 128 : d == 512 ? 64 : d == 64 ? 256 : 128;
   const int64_t tokens = std::min(n, p.bm / group + 2);
   const int64_t keys = window > 0 ? std::min(slots, window + tokens) : slots;
   const int64_t tiles = (keys + bn - 1) / bn + (n + bn - 1) / bn;
@@ -674,15 +792,13 @@ static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_
     }
     p.ctas = 0;
   } else {
-    // What fits at once by shared memory and registers (attn_tree_kernel).
-    const int64_t per_sm = d == 512 || (d == 256 && p.bm == 32) ? 1 : d == 64 ? 3 : 2;
-    p.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms * per_sm, p.items * tiles, w8::kTreeMaxPieces})));
+    p.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms, p.items * tiles, w8::kTreeMaxPieces})));  // one per SM
   }
   return p;
 }
 
 struct TreeWs {
-  int64_t part_o, part_ml, info, lse, scores, total, score_pitch;
+  int64_t part_o, part_ml, info, lse, scores, total, score_pitch, draft_at;
 };
 static TreeWs tree_ws(const TreePlan& p, int64_t batch, int64_t kv_heads, int64_t group, int64_t n, int64_t d,
                       int64_t slots, bool weights) {
@@ -698,7 +814,8 @@ static TreeWs tree_ws(const TreePlan& p, int64_t batch, int64_t kv_heads, int64_
   w.part_ml = take(part_rows * 8);
   w.info = take(p.tc ? 0 : p.items * 8);
   const int64_t rows = batch * kv_heads * group * n;
-  w.score_pitch = (slots + n + 3) / 4 * 4;
+  w.draft_at = (slots + 3) / 4 * 4;
+  w.score_pitch = w.draft_at + (n + 3) / 4 * 4;
   w.lse = take(weights ? rows * 4 : 0);
   w.scores = take(weights ? rows * w.score_pitch * 4 : 0);
   w.total = at;
@@ -737,14 +854,29 @@ static int launch_tree(Kern kern, dim3 grid, int threads, int smem, cudaStream_t
 template <typename T, int D, int MT>
 static int tree_main(const w8::TreeArgs& a, int64_t blocks, int device, cudaStream_t stream) {
   using C = w8::TreeCfg<D, MT>;
+  constexpr bool kHalf = __is_same(T, __half);
   static bool done[64] = {};
   if (!done[device]) {
     W8_CUDA_TRY(cudaFuncSetAttribute(w8::attn_tree_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      C::kSmem));
     done[device] = true;
   }
+  CUtensorMap tk = {}, tv = {}, tkn = {}, tvn = {};
+  if (a.tma) {
+    int st = tree_encode_rows(&tkn, a.kn, kHalf, D, a.n, a.kv_heads, a.batch, a.kn_b, a.kn_h, a.kn_t, C::kBN, D / 64);
+    if (st != W8_OK) return st;
+    st = tree_encode_rows(&tvn, a.vn, kHalf, D, a.n, a.kv_heads, a.batch, a.vn_b, a.vn_h, a.vn_t, C::kBN, D / 64);
+    if (st != W8_OK) return st;
+    tk = tkn, tv = tvn;  // an empty cache: never read
+    if (a.slots > 0) {
+      st = tree_encode_rows(&tk, a.k, kHalf, D, a.slots, a.kv_heads, a.batch, a.k_b, a.k_h, a.k_s, C::kBN, D / 64);
+      if (st != W8_OK) return st;
+      st = tree_encode_rows(&tv, a.v, kHalf, D, a.slots, a.kv_heads, a.batch, a.v_b, a.v_h, a.v_s, C::kBN, D / 64);
+      if (st != W8_OK) return st;
+    }
+  }
   return launch_tree(w8::attn_tree_kernel<T, D, MT>, dim3(static_cast<unsigned>(blocks)), w8::kTreeThreads, C::kSmem,
-                     stream, a);
+                     stream, tk, tv, tkn, tvn, a);
 }
 
 template <typename T, int D>
@@ -754,7 +886,7 @@ static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStr
   int st;
   if (p.tc)
     st = tree_tc(a, __is_same(T, __half), D, p.items, device, stream);
-  else if constexpr (D <= 256)
+  else if constexpr (D <= 128)
     st = p.bm == 32 ? tree_main<T, D, 2>(a, blocks, device, stream) : tree_main<T, D, 1>(a, blocks, device, stream);
   else
     st = tree_main<T, D, 1>(a, blocks, device, stream);
@@ -767,10 +899,10 @@ static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStr
     if (st != W8_OK) return st;
   }
   if (a.scores != nullptr) {
-    const int64_t blocks_w = (a.slots + a.n + 255) / 256;
+    const int64_t blocks_w = (a.score_pitch + 1023) / 1024;
     st = launch_tree(w8::attn_tree_weights_kernel,
-                     dim3(static_cast<unsigned>(blocks_w), static_cast<unsigned>(a.batch * a.kv_heads)), 256, 2048,
-                     stream, a);
+                     dim3(static_cast<unsigned>(blocks_w), static_cast<unsigned>(a.batch * a.kv_heads)), 256, 0, stream,
+                     a);
   }
   return st;
 }
@@ -889,11 +1021,13 @@ extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspa
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.part_o = reinterpret_cast<float*>(ws + w.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+  a.tma = tma ? 1 : 0;
   a.info = p.tc ? nullptr : reinterpret_cast<int2*>(ws + w.info);
   if (weights) {
     a.lse = reinterpret_cast<float*>(ws + w.lse);
     a.scores = reinterpret_cast<float*>(ws + w.scores);
     a.score_pitch = w.score_pitch;
+    a.draft_at = static_cast<int>(w.draft_at);
     a.w_in = x.weights;
     a.w_out = x.weights_out;
     a.w_new = x.draft_weights;

@@ -31,8 +31,10 @@ struct TreeArgs {
   float2* part_ml;       // [slot][BM]
   int2* info;            // [items], mma.sync schedule
   float* lse;            // [b * kv_heads + c][R] (log2 units) when the weights are wanted
-  float* scores;         // [b * kv_heads + c][R][score_pitch] (log2 units), slots then drafts
+  float* scores;         // [b * kv_heads + c][R][score_pitch] (log2 units), new tokens from draft_at on
   int64_t score_pitch;
+  int draft_at;
+  int tma;               // the caches and new rows load as TMA boxes (mma.sync schedule)
   const float* w_in;
   float* w_out;
   float* w_new;          // [B, KV, N]

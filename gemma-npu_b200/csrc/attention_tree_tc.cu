@@ -369,7 +369,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         for (int e = 0; e < 64; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(sv[e >> 5][e & 31]));
         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if (a.scores != nullptr && half == 0 && tok >= 0) {
-          float* dst = a.scores + (static_cast<int64_t>(bc) * rows + rr) * a.score_pitch + (draft ? a.slots : 0) + k0;
+          float* dst = a.scores + (static_cast<int64_t>(bc) * rows + rr) * a.score_pitch + (draft ? a.draft_at : 0) + k0;
           const int left = (draft ? a.n : len) - k0;
 #pragma unroll
           for (int e = 0; e < 64; ++e)
@@ -586,7 +586,7 @@ static TreeEncodeFn tree_encode_fn() {
 // 5-D map over rows [batch, heads, n] of d elements: (64 columns, row, 64-column block, head,
 // batch).  A box {64, rows, blocks, 1, 1} lands as `blocks` 128-byte-swizzled [rows x 64]
 // blocks; rows behind n read as zeros.
-static int encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, int64_t n, int64_t heads, int64_t batch,
+int tree_encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, int64_t n, int64_t heads, int64_t batch,
                        int64_t s_b, int64_t s_h, int64_t s_n, uint32_t rows, uint32_t blocks) {
   TreeEncodeFn enc = tree_encode_fn();
   if (enc == nullptr) {
@@ -644,15 +644,15 @@ static int tree_tc_go(const w8::TreeArgs& a, int64_t items, int device, cudaStre
   constexpr bool kHalf = __is_same(T, __half);
   CUtensorMap tq, tk, tv, tkn, tvn;
   const uint32_t kb = C::kKCols / 64, vb = C::kDV / 128;
-  int st = encode_rows(&tkn, a.kn, kHalf, D, a.n, a.kv_heads, a.batch, a.kn_b, a.kn_h, a.kn_t, w8::kTtKeysPerCta, kb);
+  int st = tree_encode_rows(&tkn, a.kn, kHalf, D, a.n, a.kv_heads, a.batch, a.kn_b, a.kn_h, a.kn_t, w8::kTtKeysPerCta, kb);
   if (st != W8_OK) return st;
-  st = encode_rows(&tvn, a.vn, kHalf, D, a.n, a.kv_heads, a.batch, a.vn_b, a.vn_h, a.vn_t, w8::kTtBN, vb);
+  st = tree_encode_rows(&tvn, a.vn, kHalf, D, a.n, a.kv_heads, a.batch, a.vn_b, a.vn_h, a.vn_t, w8::kTtBN, vb);
   if (st != W8_OK) return st;
   tk = tkn, tv = tvn;  // an empty cache: never read
   if (a.slots > 0) {
-    st = encode_rows(&tk, a.k, kHalf, D, a.slots, a.kv_heads, a.batch, a.k_b, a.k_h, a.k_s, w8::kTtKeysPerCta, kb);
+    st = tree_encode_rows(&tk, a.k, kHalf, D, a.slots, a.kv_heads, a.batch, a.k_b, a.k_h, a.k_s, w8::kTtKeysPerCta, kb);
     if (st != W8_OK) return st;
-    st = encode_rows(&tv, a.v, kHalf, D, a.slots, a.kv_heads, a.batch, a.v_b, a.v_h, a.v_s, w8::kTtBN, vb);
+    st = tree_encode_rows(&tv, a.v, kHalf, D, a.slots, a.kv_heads, a.batch, a.v_b, a.v_h, a.v_s, w8::kTtBN, vb);
     if (st != W8_OK) return st;
   }
   tq = tkn;

@@ -177,6 +177,20 @@ def test_shared_tree_and_strided_out(cuda):
     check_out(out, want_attention(q, k, v, ln, kn, vn, tree[0], depth[0], 40, 0.1), torch.bfloat16)
 
 
+@pytest.mark.parametrize("N", [1, 11, 40])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_expanded_caches(cuda, D, N):
+    """Beams that share one prompt's cache: k and v expanded over the batch (stride 0), q over the
+    heads' batch too."""
+    B, H, KV, S = 5, 4, 2, 333
+    q, k, v, ln, kn, vn = make(D + N, B, H, KV, D, N, S, [333] * B)
+    k, v, q = k[:1].expand(B, KV, S, D), v[:1].expand(B, KV, S, D), q[:, :1].expand(B, H, N, D)
+    ln = torch.tensor([333, 300, 0, 1, 128], dtype=torch.int32, device="cuda")
+    got = w8.attention_tree(q, k, v, ln, kn, vn, window=200, scale=D ** -0.5)
+    check_out(got, want_attention(q, k, v, ln, kn, vn, window=200, scale=D ** -0.5), torch.bfloat16)
+    assert w8.device_status() == 0
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("D", [64, 128, 256, 512])
 def test_infinite_values_stay_with_those_who_see_them(cuda, D, dt):
