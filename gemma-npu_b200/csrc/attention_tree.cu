@@ -83,7 +83,11 @@ struct TreeCfg {
   static constexpr int kSteps = D == 64 ? 2 : 1;            // 16-key steps of a warp in a tile
   static constexpr int kBN = kGroups * kSteps * 16;         // keys per tile: 256, 128, 128, 64
   static constexpr int kSlotBytes = kBN * D * 2;            // 32 KB (D <= 128) or 64 KB
-  static constexpr int kSlots = D <= 128 ? 6 : 3;
+  static constexpr int kPerSm = D == 64 ? 2 : 1;            // CTAs per SM
+  static constexpr int kSlots = D == 128 ? 6 : 3;
+  // Ring steps loaded ahead.  A slot freed one step ago may still be held by a slow warp, whose
+  // turn to load it then waits: with small boxes two steps' grace is worth more than the fifth box.
+  static constexpr int kAhead = kSlots == 6 ? 4 : 2;
   static constexpr int kPitch = D + 8;                      // fp32 row pitch of the joint outputs
   static constexpr int kOffRing = 0;
   static constexpr int kOffQ = kSlots * kSlotBytes;
@@ -91,7 +95,7 @@ struct TreeCfg {
   static constexpr int kOffBar = kOffStat + 2 * kGroups * kBM * 4;
   static constexpr int kNumBars = 2 * kSlots;               // full, empty
   static constexpr int kSmem = kOffBar + kNumBars * 8 + 16 + 1024;
-  static_assert(kSmem <= 232448, "shared memory budget exceeded");
+  static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory budget exceeded");
   static_assert(kGroups * kBM * kPitch * 4 <= kOffQ, "the joint outputs fit over the ring");
 };
 
@@ -130,7 +134,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* sm, long
 }
 
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kTreeThreads, 1)
+__global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
     attn_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                      const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_vn,
                      const __grid_constant__ TreeArgs a) {
@@ -278,27 +282,37 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         cp_async_arrive(full_bar(slot));
       }
     };
-    // The step NS - 1 ahead loads as a step begins; the warps take turns, so that waiting for the
+    // The step kAhead ahead loads as a step begins; the warps take turns, so that waiting for the
     // others to leave the slot holds up one of them only.
     auto load_ahead = [&](int i) {
-      if (!a.tma || (warp == static_cast<int>((g_item + i) % kTreeWarps) && lane == 0)) load(i + NS - 1);
+      if (!a.tma || (warp == static_cast<int>((g_item + i) % kTreeWarps) && lane == 0)) load(i + C::kAhead);
       __syncwarp();
     };
     if (!a.tma || tid == 0)
-      for (int i = 0; i < NS - 1; ++i) load(i);
+      for (int i = 0; i < C::kAhead; ++i) load(i);
     __syncwarp();
 
-    // Row r = i * group + g: query head c * group + g of new token i.
-    for (int e = tid; e < BM * CH; e += kTreeThreads) {
-      const int r = e / CH, ch = e % CH;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (row0 + r < rows) {
-        int i, gq;
-        tree_row(a, row0 + r, i, gq);
-        w = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + gq) * a.q_h + i * a.q_t +
-                                            ch * 8);
+    // Row r = i * group + g: query head c * group + g of new token i.  (Every load is under way
+    // before the first is stored: they may come from HBM.)
+    {
+      constexpr int kEach = (BM * CH + kTreeThreads - 1) / kTreeThreads;
+      uint4 w[kEach];
+#pragma unroll
+      for (int x = 0; x < kEach; ++x) {
+        const int e = tid + x * kTreeThreads, r = e / CH, ch = e % CH;
+        w[x] = make_uint4(0, 0, 0, 0);
+        if (e < BM * CH && row0 + r < rows) {
+          int i, gq;
+          tree_row(a, row0 + r, i, gq);
+          w[x] = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + gq) * a.q_h +
+                                                 i * a.q_t + ch * 8);
+        }
       }
-      st_shared_v4(sq + r * (D * 2) + ((ch ^ (r & 7)) << 4), w.x, w.y, w.z, w.w);
+#pragma unroll
+      for (int x = 0; x < kEach; ++x) {
+        const int e = tid + x * kTreeThreads, r = e / CH, ch = e % CH;
+        if (e < BM * CH) st_shared_v4(sq + r * (D * 2) + ((ch ^ (r & 7)) << 4), w[x].x, w[x].y, w[x].z, w[x].w);
+      }
     }
     // This thread's rows of each 16-row tile: lane / 4 and lane / 4 + 8.
     int tok[MT][2], dep[MT][2], first[MT][2];
@@ -345,10 +359,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         const int kr = (grp * C::kSteps + st) * 16, key0 = tile0 + kr;  // this step's keys
         // ---- S = Q K^T, 16 keys
         float s[MT][2][4];
+        constexpr int kChains = MT == 1 && D >= 256 ? 2 : 1;  // halves of D summed side by side
+        float s2[kChains][MT][2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int ci = 0; ci < kChains; ++ci)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[mt][e >> 2][e & 3] = 0.f;
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s2[ci][mt][e >> 2][e & 3] = 0.f;
         const int krow = kr + (lane & 7) + ((lane >> 4) << 3);
         const uint32_t kbase = sk + krow * 128;
 #pragma unroll
@@ -358,17 +376,22 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             if constexpr (kQRegs) {
-              mma16816<T>(s[mt][0], qf[kk], kb[0], kb[1]);
-              mma16816<T>(s[mt][1], qf[kk], kb[2], kb[3]);
+              mma16816<T>(s2[kk % kChains][mt][0], qf[kk], kb[0], kb[1]);
+              mma16816<T>(s2[kk % kChains][mt][1], qf[kk], kb[2], kb[3]);
             } else {
               uint32_t qa[4];
               const int r = mt * 16 + arow;
               ldsm_x4(sq + r * (D * 2) + (((2 * kk + (lane >> 4)) ^ (r & 7)) << 4), qa);
-              mma16816<T>(s[mt][0], qa, kb[0], kb[1]);
-              mma16816<T>(s[mt][1], qa, kb[2], kb[3]);
+              mma16816<T>(s2[kk % kChains][mt][0], qa, kb[0], kb[1]);
+              mma16816<T>(s2[kk % kChains][mt][1], qa, kb[2], kb[3]);
             }
           }
         }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            s[mt][e >> 2][e & 3] = s2[0][mt][e >> 2][e & 3] + (kChains > 1 ? s2[kChains - 1][mt][e >> 2][e & 3] : 0.f);
         // ---- masks and the running softmax.  Columns of a thread: key0 + 8 n + 2 (lane % 4) + {0, 1}.
         const int col = (lane & 3) * 2;
         float mx[MT][2];
@@ -541,6 +564,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = mt * 16 + rl + 8 * h;
+        if (row0 + r >= rows) continue;
         float top = stat[r];
 #pragma unroll
         for (int w = 1; w < C::kGroups; ++w) top = fmaxf(top, stat[w * BM + r]);
@@ -603,10 +627,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 }
 
 // Joins the pieces of one row: M = max m_s, o = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.
-// One CTA per row and 128 (64) columns: 4 columns a thread, the pieces over thread groups.
-template <typename T, int D>
+// One CTA per row and COLS columns: 4 columns a thread, the pieces over thread groups.  Few
+// rows take 32 columns, so that a long sequence's many pieces are summed by more threads.
+template <typename T, int D, int COLS>
 __global__ void __launch_bounds__(256) attn_tree_combine_kernel(const TreeArgs a, int bm) {
-  constexpr int kCols = D < 128 ? D : 128, kLanes = kCols / 4, kGroups = 256 / kLanes;
+  constexpr int kLanes = COLS / 4, kGroups = 256 / kLanes;
   __shared__ float w[kTreeMaxPieces];
   __shared__ float4 acc[kGroups][kLanes];
   __shared__ float wmax[8], wsum[8];
@@ -655,7 +680,7 @@ __global__ void __launch_bounds__(256) attn_tree_combine_kernel(const TreeArgs a
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum += wsum[i];
   const int ln = tid % kLanes, grp = tid / kLanes;
-  const int col = blockIdx.y * kCols + ln * 4;
+  const int col = blockIdx.y * COLS + ln * 4;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int s = grp; s < pieces; s += kGroups) {
@@ -792,7 +817,7 @@ static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_
     }
     p.ctas = 0;
   } else {
-    p.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms, p.items * tiles, w8::kTreeMaxPieces})));  // one per SM
+    p.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms * (d == 64 ? 2 : 1), p.items * tiles, w8::kTreeMaxPieces})));  // TreeCfg::kPerSm
   }
   return p;
 }
@@ -893,9 +918,13 @@ static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStr
   if (st != W8_OK) return st;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.group * a.n;
   if (p.tc ? p.splits > 1 : p.ctas > 1) {
-    st = launch_tree(w8::attn_tree_combine_kernel<T, D>,
-                     dim3(static_cast<unsigned>(rows), static_cast<unsigned>(D < 128 ? 1 : D / 128)), 256, 0, stream, a,
-                     p.bm);
+    constexpr int kWide = D < 128 ? D : 128;
+    if (rows * (D / 32) <= 1024)
+      st = launch_tree(w8::attn_tree_combine_kernel<T, D, 32>, dim3(static_cast<unsigned>(rows), D / 32), 256, 0, stream,
+                       a, p.bm);
+    else
+      st = launch_tree(w8::attn_tree_combine_kernel<T, D, kWide>, dim3(static_cast<unsigned>(rows), D / kWide), 256, 0,
+                       stream, a, p.bm);
     if (st != W8_OK) return st;
   }
   if (a.scores != nullptr) {
