@@ -6,7 +6,6 @@ sm_100 device.  There is no fallback: if the library is missing, `lib()` raises.
 """
 import ctypes
 import os
-import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -121,26 +120,16 @@ SIGNATURES.update({
 })
 
 SIGNATURES.update({
-    "w8_attention_tree": (_i, [ctypes.c_char_p, _p, _i64, _p]),
+    "w8_attention_tree": (_i, [_p, _p, _i64, _p]),
     "w8_attention_tree_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i]),
-    "w8_cache_append": (_i, [ctypes.c_char_p, _p]),
-    "w8_cache_evict": (_i, [ctypes.c_char_p, _p, _i64, _p]),
+    "w8_cache_append": (_i, [_p, _p]),
+    "w8_cache_evict": (_i, [_p, _p, _i64, _p]),
     "w8_cache_evict_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "w8_beam_select": (_i, [_p, _i, _i64, _i64, _p, _p, _i64, _f, _i64, _i64, _i64, _i64, _i, _p, _p, _p, _p, _i64,
                             _p]),
     "w8_beam_select_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "w8_cache_reorder": (_i, [_p, _i64, _p, _p, _i, _p, _i64, _i64, _i64, _i64, _i64, _p]),
 })
-
-# The argument structs of w8a8_b200.h: 8-byte fields in the header's order, packed as bytes
-# (ctypes passes a bytes object by its address, which is cheaper than filling a Structure):
-# the pointers, which change from call to call, then strides and sizes, which seldom do.
-ATTENTION_TREE_POINTERS = struct.Struct("12Q")
-ATTENTION_TREE_TAIL = struct.Struct("33qd")
-CACHE_APPEND_POINTERS = struct.Struct("11Q")
-CACHE_APPEND_TAIL = struct.Struct("25q")
-CACHE_EVICT_POINTERS = struct.Struct("8Q")
-CACHE_EVICT_TAIL = struct.Struct("21q")
 
 # Element type codes.
 W8_BF16 = 0

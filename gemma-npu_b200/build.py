@@ -1,5 +1,8 @@
 """Build the sm_100a C-ABI library `libw8a8_b200.so` in-tree with nvcc.
 
+Also the Python binding of the decoding operators, `_decode.so`, with the host compiler
+(`csrc/decode_binding.cpp`: torch's C++ API on one side, the C ABI on the other).
+
 Every `csrc/*.cu` is compiled for `arch=compute_100a,code=sm_100a` (nvcc
 cross-compiles without a GPU) into `_build/*.o`, and linked into
 `libw8a8_b200.so` next to this file, where `_lib.py` loads it.  Objects are
@@ -20,6 +23,7 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libw8a8_b200.so")
+BINDING = os.path.join(HERE, "_decode.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
@@ -35,6 +39,30 @@ def nvcc_path():
 
 def _newest(paths):
     return max((os.path.getmtime(p) for p in paths), default=0.0)
+
+
+def build_binding(force=False, quiet=False):
+    """Compile csrc/decode_binding.cpp against this Python and torch; returns its path."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    src = os.path.join(CSRC, "decode_binding.cpp")
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(
+            os.path.getmtime(src), _newest(glob.glob(os.path.join(INCLUDE, "*.h")))):
+        return BINDING
+    if not quiet:
+        print("[build] decode_binding.cpp", flush=True)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
+    dirs = [*include_paths(), cuda, sysconfig.get_paths()["include"]]
+    tmp = BINDING + ".tmp"
+    subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                    *(f"-isystem{d}" for d in dirs), src, "-o", tmp, *(f"-L{d}" for d in library_paths()),
+                    "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"], check=True)
+    os.replace(tmp, BINDING)
+    return BINDING
 
 
 def build(force=False, verbose_ptxas=False, quiet=False):
@@ -62,6 +90,7 @@ def build(force=False, verbose_ptxas=False, quiet=False):
         os.replace(tmp, LIB)
         if not quiet:
             print("[build] linked", LIB, flush=True)
+    build_binding(force=force, quiet=quiet)
     return LIB
 
 

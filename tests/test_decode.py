@@ -1,10 +1,17 @@
 """Host-side checks of the decoding operators, without a GPU: the wrappers refuse host
 tensors, and the C ABI answers bad arguments with status codes before any CUDA call."""
+import struct
+
 import pytest
 import torch
 
 import gemma_npu_b200 as w8
 from gemma_npu_b200 import _lib
+
+# The argument structs of w8a8_b200.h: pointers, then 64-bit integers (and a double).
+TREE_ARGS = struct.Struct("12Q33qd")
+APPEND_ARGS = struct.Struct("11Q25q")
+EVICT_ARGS = struct.Struct("8Q21q")
 
 
 def tree_args(**change):
@@ -16,8 +23,7 @@ def tree_args(**change):
     n = dict(B=1, H=4, KV=2, D=64, S=16, N=2, window=0, dtype=_lib.W8_BF16, scale=1.0)
     for name, v in change.items():
         next(d for d in (p, s, n) if name in d)[name] = v
-    return _lib.ATTENTION_TREE_POINTERS.pack(*p.values()) + _lib.ATTENTION_TREE_TAIL.pack(
-        *(x for v in s.values() for x in v), 4, 2, 0, 0, 0, 0, 0, *n.values())
+    return TREE_ARGS.pack(*p.values(), *(x for v in s.values() for x in v), 4, 2, 0, 0, 0, 0, 0, *n.values())
 
 
 @pytest.mark.parametrize("change,status", [
@@ -41,9 +47,8 @@ def test_struct_sizes_match_the_header():
     import re
 
     text = re.sub(r"/\*.*?\*/", "", open(_lib.HEADER_PATH).read(), flags=re.S)
-    for name, head, tail in (("w8_attention_tree_args", _lib.ATTENTION_TREE_POINTERS, _lib.ATTENTION_TREE_TAIL),
-                             ("w8_cache_append_args", _lib.CACHE_APPEND_POINTERS, _lib.CACHE_APPEND_TAIL),
-                             ("w8_cache_evict_args", _lib.CACHE_EVICT_POINTERS, _lib.CACHE_EVICT_TAIL)):
+    for name, packed in (("w8_attention_tree_args", TREE_ARGS), ("w8_cache_append_args", APPEND_ARGS),
+                         ("w8_cache_evict_args", EVICT_ARGS)):
         body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1)
         fields = 0
         for decl in body.split(";"):
@@ -51,13 +56,13 @@ def test_struct_sizes_match_the_header():
                 if item.strip():
                     m = re.search(r"\[(\d+)\]", item)
                     fields += int(m.group(1)) if m else 1
-        assert head.size + tail.size == 8 * fields, name
+        assert packed.size == 8 * fields, name
 
 
 def test_evict_refuses():
     def args(budget=4, sink=0, recent=0, lens=4096, lens_out=8192, row=128):
-        return _lib.CACHE_EVICT_POINTERS.pack(4096, 4096, 4096, 4096, lens, 4096, 4096, lens_out) + _lib.CACHE_EVICT_TAIL.pack(
-            *[128] * 6, *[16] * 8, 1, 1, 16, row, budget, sink, recent)
+        return EVICT_ARGS.pack(4096, 4096, 4096, 4096, lens, 4096, 4096, lens_out, *[128] * 6, *[16] * 8, 1, 1, 16, row,
+                               budget, sink, recent)
 
     run = _lib.lib().w8_cache_evict
     for a in (args(budget=0), args(sink=-1), args(sink=2, recent=3), args(lens=0), args(lens_out=4096)):
