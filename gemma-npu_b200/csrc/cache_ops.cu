@@ -107,7 +107,8 @@ struct EvictArgs {
   int most;
 };
 
-constexpr int kEvictThreads = 1024;
+constexpr int kEvictThreads = 512;
+constexpr int kEvictLongThreads = 1024;
 
 // Exclusive prefix sum of `v` over the block; `total` is the block's sum.
 __device__ __forceinline__ int evict_scan(int v, int* warp_sums, int& total) {
@@ -143,42 +144,279 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Which slots of one (sequence, cache head) stay: the `budget` largest by (protected,
-// weight, lower slot), by a radix selection of the budget-th key, then one pass in slot
-// order that pairs the i-th evicted slot below the budget with the i-th kept slot behind it.
-__global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictArgs a) {
+// One (sequence, cache head) of an eviction.
+struct EvictRow {
+  const float* w;
+  const int* pos;
+  float* w_out;
+  int* pos_out;
+  int* moves;
+  int len, left;
+};
+__device__ __forceinline__ EvictRow evict_row(const EvictArgs& a, int row) {
+  const int b = row / a.kv_heads, c = row % a.kv_heads;
+  EvictRow r;
+  r.w = a.w + b * a.w_b + c * a.w_h;
+  r.pos = a.pos + b * a.pos_b + c * a.pos_h;
+  r.w_out = a.w_out + b * a.wo_b + c * a.wo_h;
+  r.pos_out = a.pos_out + b * a.po_b + c * a.po_h;
+  r.moves = a.moves + static_cast<int64_t>(row) * (1 + 2 * a.most);
+  r.len = a.lens[b];
+  if (r.len < 0 || r.len > a.slots) {
+    if (threadIdx.x == 0) cache_bad_index();
+    r.len = r.len < 0 ? 0 : a.slots;
+  }
+  r.left = min(r.len, a.budget);
+  if (c == 0 && threadIdx.x == 0) a.lens_out[b] = r.left;
+  return r;
+}
+
+// The small state after the cut: kept slots as they are, holes from their movers, nothing
+// behind.  All threads; w_out / pos_out may be w / pos (what is read is never written before).
+__device__ __forceinline__ void evict_state(const EvictArgs& a, const EvictRow& r, int count, int threads) {
+  const int tid = threadIdx.x;
+  if (tid == 0) r.moves[0] = count;
+  if (r.w_out != r.w || r.pos_out != r.pos)
+#pragma unroll 8
+    for (int s = tid; s < r.left; s += threads) {
+      const float ws = r.w[s];
+      const int ps = r.pos[s];
+      r.w_out[s] = ws;
+      r.pos_out[s] = ps;
+    }
+  __syncthreads();
+#pragma unroll 8
+  for (int i = tid; i < count; i += threads) {
+    const int dst = r.moves[1 + i], src = r.moves[1 + a.most + i];
+    r.w_out[dst] = r.w[src];
+    r.pos_out[dst] = r.pos[src];
+  }
+  __syncthreads();
+#pragma unroll 8
+  for (int s = r.left + tid; s < a.slots; s += threads) {
+    r.w_out[s] = 0.f;
+    r.pos_out[s] = -1;
+  }
+}
+
+// The last position that is not recent.
+__device__ __forceinline__ int evict_recent_after(const EvictArgs& a, int last) {
+  const int64_t after = static_cast<int64_t>(last) - a.recent;
+  return after < INT32_MIN ? INT32_MIN : static_cast<int>(after);
+}
+
+// A slot's place in the order: protected ones (all alike, above every weight) before the others
+// by weight.
+__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, float w, int pos, int recent_after) {
+  return pos < a.sink || pos > recent_after ? 0xFFFFFFFFu : weight_key(w);
+}
+
+// Which slots of a (sequence, cache head) stay: the `budget` largest by (protected, weight,
+// lower slot).  A warp holds the keys of 32 KPT consecutive slots in registers, lane i of step
+// j the slot 32 j + i; the budget-th key is found by bisection on its bits, one count over the
+// block an iteration (some 15 of them: a histogram's shared-memory atomics meet in the few
+// exponents that weights have, and took 19 us where this takes US_SELECT for 3658 slots), until
+// a cut has exactly `budget` keys or, among equal ones, the lowest slots fill it.  Ballots in
+// slot order then pair the i-th evicted slot below the budget with the i-th kept one behind it.
+template <int KPT>
+__global__ void __launch_bounds__(kEvictThreads, KPT <= 32 ? 2 : 1) evict_select_kernel(const EvictArgs a) {
+  constexpr int kWarps = kEvictThreads / 32;
+  __shared__ int counts[2][kWarps];
+  __shared__ int per_warp[3][kWarps];
+  __shared__ uint32_t kept[kWarps][KPT];
+  extern __shared__ uint32_t lists[];  // [most] evicted slots, [budget] sources: 16 bits each
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch_dependents();
+  pdl_wait();
+  const EvictRow r = evict_row(a, blockIdx.x);
+  // Nothing behind the last slot: written first, under the loads, unless the row is cut in place.
+  auto clear = [&]() {
+#pragma unroll 8
+    for (int s = r.left + tid; s < a.slots; s += kEvictThreads) {
+      r.w_out[s] = 0.f;
+      r.pos_out[s] = -1;
+    }
+  };
+  const bool in_place = r.w_out == r.w || r.pos_out == r.pos;
+  if (!in_place) clear();
+  int moved = 0;
+  if (r.len > a.budget) {
+    const int s0 = warp * 32 * KPT + lane;  // slot of step i: s0 + 32 i
+    uint32_t key[KPT];
+    int last = INT32_MIN;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      const int s = s0 + 32 * i;
+      key[i] = s < r.len ? __float_as_uint(r.w[s]) : 0u;
+      if (s < r.len) last = max(last, r.pos[s]);
+    }
+    // The highest position decides what is recent (so the positions are read again, from L2: held
+    // with the keys they would leave no registers for loads in flight).
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) counts[0][warp] = last;
+    __syncthreads();
+    last = __reduce_max_sync(0xffffffffu, counts[0][lane % kWarps]);
+    const int recent_after = evict_recent_after(a, last);
+    uint32_t least = 0xFFFFFFFFu, most = 0u;  // of the keys that are not protected
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {  // 0 behind the length: below every slot's
+      const int s = s0 + 32 * i;
+      key[i] = s < r.len ? evict_key(a, __uint_as_float(key[i]), r.pos[s], recent_after) : 0u;
+      if (key[i] != 0xFFFFFFFFu) most = max(most, key[i]);
+      if (key[i] != 0u) least = min(least, key[i]);
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    __syncthreads();
+    if (lane == 0) counts[0][warp] = static_cast<int>(least), counts[1][warp] = static_cast<int>(most);
+    __syncthreads();
+    least = __reduce_min_sync(0xffffffffu, static_cast<uint32_t>(counts[0][lane % kWarps]));
+    most = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(counts[1][lane % kWarps]));
+    __syncthreads();
+    int turn = 0;
+    auto count = [&](uint32_t at) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < KPT; ++i) n += key[i] >= at ? 1 : 0;
+      n = __reduce_add_sync(0xffffffffu, n);
+      turn ^= 1;  // (two buffers: one barrier an iteration)
+      if (lane == 0) counts[turn][warp] = n;
+      __syncthreads();
+      return __reduce_add_sync(0xffffffffu, lane < kWarps ? counts[turn][lane] : 0);
+    };
+    // Bisect: `reach` keys are >= cut, at least `budget` of them, and fewer are >= over.  The
+    // protected keys (all ones) may fill the budget alone.
+    uint32_t cut = least, over = 0xFFFFFFFFu;
+    int reach = r.len;
+    const int protect = count(0xFFFFFFFFu);
+    if (protect >= a.budget)
+      cut = 0xFFFFFFFFu, reach = protect;
+    else
+      over = most + 1;
+    while (reach != a.budget && over - cut > 1) {
+      const uint32_t mid = cut + (over - cut) / 2;
+      const int n = count(mid);
+      if (n >= a.budget)
+        cut = mid, reach = n;
+      else
+        over = mid;
+    }
+    // Of the keys equal to the cut the last reach - budget in slot order go.
+    __syncthreads();
+    const bool ties = reach != a.budget;  // (the same for all threads)
+    int room = 0;                         // equal keys that stay, counted from this warp's first
+    if (ties) {
+      int eq = 0;
+#pragma unroll
+      for (int i = 0; i < KPT; ++i) eq += __popc(__ballot_sync(0xffffffffu, key[i] == cut));
+      if (lane == 0) per_warp[0][warp] = eq;
+      __syncthreads();
+      const int mine = lane < kWarps ? per_warp[0][lane] : 0;
+      room = __reduce_add_sync(0xffffffffu, mine) - (reach - a.budget) -
+             __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+    }
+    const uint32_t before = (1u << lane) - 1u;
+    auto low_bits = [&](int i) {  // this step's slots below the budget
+      const int n = a.budget - (s0 - lane + 32 * i);
+      return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+    };
+    int holes = 0, movers = 0;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      bool stays = key[i] >= cut;
+      if (ties) {
+        const uint32_t eq = __ballot_sync(0xffffffffu, key[i] == cut);
+        stays = key[i] > cut || (key[i] == cut && __popc(eq & before) < room);
+        room -= __popc(eq);
+      }
+      const uint32_t keep = __ballot_sync(0xffffffffu, stays), low = low_bits(i);
+      if (lane == 0) kept[warp][i] = keep;
+      holes += __popc(~keep & low);
+      movers += __popc(keep & ~low);
+    }
+    if (lane == 0) per_warp[1][warp] = holes, per_warp[2][warp] = movers;
+    __syncthreads();
+    const int wh = lane < kWarps ? per_warp[1][lane] : 0, wm = lane < kWarps ? per_warp[2][lane] : 0;
+    int hole_at = __reduce_add_sync(0xffffffffu, lane < warp ? wh : 0);
+    int mover_at = __reduce_add_sync(0xffffffffu, lane < warp ? wm : 0);
+    moved = __reduce_add_sync(0xffffffffu, wm);
+    // The evicted slots in order, in shared memory; then each mover finds its own, and each slot
+    // below the budget what it will hold.
+    uint16_t* hole_slots = reinterpret_cast<uint16_t*>(lists);
+    uint16_t* src_slots = hole_slots + a.most;
+#pragma unroll 4
+    for (int i = 0; i < KPT; ++i) {
+      const uint32_t low = low_bits(i), h = ~kept[warp][i] & low;
+      if (low == 0u) break;
+      if ((h >> lane) & 1u) hole_slots[hole_at + __popc(h & before)] = static_cast<uint16_t>(s0 + 32 * i);
+      if ((low >> lane) & 1u) src_slots[s0 + 32 * i] = static_cast<uint16_t>(s0 + 32 * i);
+      hole_at += __popc(h);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = 0; i < KPT; ++i) {
+      const uint32_t m = kept[warp][i] & ~low_bits(i);
+      if ((m >> lane) & 1u) {
+        const int j = mover_at + __popc(m & before), dst = hole_slots[j];
+        r.moves[1 + j] = dst;
+        r.moves[1 + a.most + j] = s0 + 32 * i;
+        src_slots[dst] = static_cast<uint16_t>(s0 + 32 * i);
+      }
+      mover_at += __popc(m);
+    }
+    __syncthreads();
+    // The small state.  (In place too: what is read from another slot lies behind the budget.)
+#pragma unroll 8
+    for (int s = tid; s < r.left; s += kEvictThreads) {
+      const int src = src_slots[s];
+      const float ws = r.w[src];
+      const int ps = r.pos[src];
+      r.w_out[s] = ws;
+      r.pos_out[s] = ps;
+    }
+  } else if (r.w_out != r.w || r.pos_out != r.pos) {
+#pragma unroll 8
+    for (int s = tid; s < r.left; s += kEvictThreads) {
+      const float ws = r.w[s];
+      const int ps = r.pos[s];
+      r.w_out[s] = ws;
+      r.pos_out[s] = ps;
+    }
+  }
+  if (tid == 0) r.moves[0] = moved;
+  if (in_place) {
+    __syncthreads();  // every slot's weight and position have been read
+    clear();
+  }
+}
+
+// The same for more slots than registers hold: a radix selection of the budget-th key over four
+// passes of the row, then one in slot order.
+__global__ void __launch_bounds__(kEvictLongThreads) evict_select_long_kernel(const EvictArgs a) {
   __shared__ int hist[256];
   __shared__ int warp_sums[32];
   __shared__ int pick[2];
-  const int row = blockIdx.x, b = row / a.kv_heads, c = row % a.kv_heads, tid = threadIdx.x;
+  const int tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
-  const float* w = a.w + b * a.w_b + c * a.w_h;
-  const int* pos = a.pos + b * a.pos_b + c * a.pos_h;
-  float* w_out = a.w_out + b * a.wo_b + c * a.wo_h;
-  int* pos_out = a.pos_out + b * a.po_b + c * a.po_h;
-  int* moves = a.moves + static_cast<int64_t>(row) * (1 + 2 * a.most);
-  int len = a.lens[b];
-  if (len < 0 || len > a.slots) {
-    if (tid == 0) cache_bad_index();
-    len = len < 0 ? 0 : a.slots;
-  }
-  const int left = min(len, a.budget);
-  if (c == 0 && tid == 0) a.lens_out[b] = left;
+  const EvictRow r = evict_row(a, blockIdx.x);
+  const float* w = r.w;
+  const int* pos = r.pos;
+  int* moves = r.moves;
+  const int len = r.len;
   int count = 0;
   if (len > a.budget) {
     // The highest position decides what is recent.
     int last = INT32_MIN;
-    for (int s = tid; s < len; s += kEvictThreads) last = max(last, pos[s]);
+    for (int s = tid; s < len; s += kEvictLongThreads) last = max(last, pos[s]);
     last = __reduce_max_sync(0xffffffffu, last);
     if ((tid & 31) == 0) warp_sums[tid >> 5] = last;
     __syncthreads();
     last = __reduce_max_sync(0xffffffffu, warp_sums[tid & 31]);
     __syncthreads();
-    const int64_t recent_from = static_cast<int64_t>(last) - a.recent + 1;
+    const int recent_after = evict_recent_after(a, last);
     auto key = [&](int s) {
-      const int p = pos[s];
-      return p < a.sink || p >= recent_from ? 0xFFFFFFFFu : weight_key(w[s]);
+      return evict_key(a, w[s], pos[s], recent_after);
     };
     uint32_t prefix = 0;
     int need = a.budget;  // keys still to take among those that share the prefix
@@ -187,7 +425,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
       if (tid < 256) hist[tid] = 0;
       __syncthreads();
       const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-      for (int s = tid; s < len; s += kEvictThreads) {
+      for (int s = tid; s < len; s += kEvictLongThreads) {
         const uint32_t k = key(s);
         if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
       }
@@ -224,7 +462,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     }
     // In slot order: keys above the cut stay, and the first `need` equal to it.
     int equals = 0, holes = 0, movers = 0;
-    for (int s0 = 0; s0 < len; s0 += kEvictThreads) {
+    for (int s0 = 0; s0 < len; s0 += kEvictLongThreads) {
       const int s = s0 + tid;
       const bool in = s < len;
       const uint32_t k = in ? key(s) : 0u;
@@ -246,26 +484,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     count = movers;
     __syncthreads();
   }
-  if (tid == 0) moves[0] = count;
-  // The small state: kept slots as they are, holes from their movers, nothing behind.
-  if (w_out != w || pos_out != pos)
-    for (int s = tid; s < left; s += kEvictThreads) {
-      const float ws = w[s];
-      const int ps = pos[s];
-      w_out[s] = ws;
-      pos_out[s] = ps;
-    }
-  __syncthreads();
-  for (int i = tid; i < count; i += kEvictThreads) {
-    const int dst = moves[1 + i], src = moves[1 + a.most + i];
-    w_out[dst] = w[src];
-    pos_out[dst] = pos[src];
-  }
-  __syncthreads();
-  for (int s = left + tid; s < a.slots; s += kEvictThreads) {
-    w_out[s] = 0.f;
-    pos_out[s] = -1;
-  }
+  evict_state(a, r, count, kEvictLongThreads);
 }
 
 struct MoveArgs {
@@ -273,27 +492,46 @@ struct MoveArgs {
   int64_t k_b, k_h, k_s, v_b, v_h, v_s;  // bytes
   const int* moves;
   int most, kv_heads, chunks;
+  int shift;  // log2 of the chunks of a row, or -1
 };
 
+constexpr int kMoveChunks = 4;  // 16-byte chunks of a thread in flight
+
 // The moves of one (sequence, head): destinations (below the budget) and sources (behind
-// it) are disjoint, so the rows move in place in any order.
+// it) are disjoint, so the rows move in place in any order.  Bound by HBM: a CTA's 1024
+// chunks are all loaded before the first is stored.
 __global__ void __launch_bounds__(256) evict_move_kernel(const MoveArgs a) {
   const int row = blockIdx.y, b = row / a.kv_heads, c = row % a.kv_heads;
   pdl_launch_dependents();
   pdl_wait();
   const int* moves = a.moves + static_cast<int64_t>(row) * (1 + 2 * a.most);
-  const int count = moves[0];
+  const int64_t work = static_cast<int64_t>(moves[0]) * 2 * a.chunks;
   uint8_t* k = a.k + b * a.k_b + c * a.k_h;
   uint8_t* v = a.v + b * a.v_b + c * a.v_h;
-  const int64_t work = static_cast<int64_t>(count) * 2 * a.chunks;
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < work; e += static_cast<int64_t>(gridDim.x) * 256) {
-    const int ch = static_cast<int>(e % a.chunks);
-    const int64_t m = e / a.chunks;
-    const int i = static_cast<int>(m >> 1);
-    const int64_t dst = moves[1 + i], src = moves[1 + a.most + i];
-    uint8_t* base = (m & 1) ? v : k;
-    const int64_t pitch = (m & 1) ? a.v_s : a.k_s;
-    reinterpret_cast<uint4*>(base + dst * pitch)[ch] = reinterpret_cast<const uint4*>(base + src * pitch)[ch];
+  for (int64_t e0 = static_cast<int64_t>(blockIdx.x) * (256 * kMoveChunks) + threadIdx.x; e0 < work;
+       e0 += static_cast<int64_t>(gridDim.x) * (256 * kMoveChunks)) {
+    uint8_t* dst[kMoveChunks];
+    const uint8_t* src[kMoveChunks];
+    uint4 x[kMoveChunks];
+#pragma unroll
+    for (int i = 0; i < kMoveChunks; ++i) {
+      const int64_t e = e0 + 256 * i;
+      if (e < work) {
+        const int64_t m = a.shift >= 0 ? e >> a.shift : e / a.chunks;  // row: move m / 2's K or V
+        const int64_t ch = (e - m * a.chunks) * 16;
+        const int j = static_cast<int>(m >> 1);
+        uint8_t* base = ((m & 1) ? v : k) + ch;
+        const int64_t pitch = (m & 1) ? a.v_s : a.k_s;
+        dst[i] = base + moves[1 + j] * pitch;
+        src[i] = base + moves[1 + a.most + j] * pitch;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kMoveChunks; ++i)
+      if (e0 + 256 * i < work) x[i] = *reinterpret_cast<const uint4*>(src[i]);
+#pragma unroll
+    for (int i = 0; i < kMoveChunks; ++i)
+      if (e0 + 256 * i < work) *reinterpret_cast<uint4*>(dst[i]) = x[i];
   }
 }
 
@@ -361,10 +599,11 @@ namespace w8host {
 int require_sm100(int* device);
 
 template <typename Kern, typename Args>
-static int launch_cache(Kern kern, dim3 grid, int threads, cudaStream_t stream, const Args& a) {
+static int launch_cache(Kern kern, dim3 grid, int threads, cudaStream_t stream, const Args& a, int smem = 0) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -372,6 +611,16 @@ static int launch_cache(Kern kern, dim3 grid, int threads, cudaStream_t stream, 
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
+}
+
+template <int KPT>
+static int launch_evict(dim3 grid, int lists, int device, cudaStream_t stream, const w8::EvictArgs& e) {
+  static bool done[64] = {};
+  if (!done[device]) {
+    W8_CUDA_TRY(cudaFuncSetAttribute(w8::evict_select_kernel<KPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024));
+    done[device] = true;
+  }
+  return launch_cache(w8::evict_select_kernel<KPT>, grid, w8::kEvictThreads, stream, e, lists);
 }
 
 // Read (and optionally clear) the sticky device status of the cache operations.
@@ -492,14 +741,28 @@ extern "C" int w8_cache_evict(const w8_cache_evict_args* in, void* workspace, in
   e.budget = static_cast<int>(std::min(x.budget, x.slots)), e.sink = static_cast<int>(x.sink);
   e.recent = static_cast<int>(x.recent);
   e.moves = static_cast<int*>(workspace), e.most = static_cast<int>(most);
-  st = launch_cache(w8::evict_select_kernel, dim3(static_cast<unsigned>(rows)), w8::kEvictThreads, s, e);
+  // Keys in registers up to 32768 slots: the fewest that cover the row (3658 slots: 8 a thread).
+  const dim3 each(static_cast<unsigned>(rows));
+  const int64_t per = (x.slots + w8::kEvictThreads - 1) / w8::kEvictThreads;
+  const int lists = static_cast<int>(std::min<int64_t>(2 * (most + e.budget) + 4, 100 * 1024));
+  if (per <= 8)
+    st = launch_evict<8>(each, lists, device, s, e);
+  else if (per <= 16)
+    st = launch_evict<16>(each, lists, device, s, e);
+  else if (per <= 32)
+    st = launch_evict<32>(each, lists, device, s, e);
+  else if (per <= 64)
+    st = launch_evict<64>(each, lists, device, s, e);
+  else
+    st = launch_cache(w8::evict_select_long_kernel, each, w8::kEvictLongThreads, s, e);
   if (st != W8_OK || most == 0) return st;
   w8::MoveArgs m = {};
   m.k = static_cast<uint8_t*>(x.k), m.v = static_cast<uint8_t*>(x.v);
   m.k_b = x.k_stride[0], m.k_h = x.k_stride[1], m.k_s = x.k_stride[2];
   m.v_b = x.v_stride[0], m.v_h = x.v_stride[1], m.v_s = x.v_stride[2];
   m.moves = e.moves, m.most = e.most, m.kv_heads = e.kv_heads, m.chunks = static_cast<int>(x.row_bytes / 16);
-  const int64_t blocks = (most * 2 * m.chunks + 255) / 256;
+  m.shift = (m.chunks & (m.chunks - 1)) == 0 ? __builtin_ctz(m.chunks) : -1;
+  const int64_t blocks = (most * 2 * m.chunks + 256 * w8::kMoveChunks - 1) / (256 * w8::kMoveChunks);
   const int64_t per_row = std::max<int64_t>(1, std::min(blocks, (static_cast<int64_t>(sms) * 16 + rows - 1) / rows));
   return launch_cache(w8::evict_move_kernel, dim3(static_cast<unsigned>(per_row), static_cast<unsigned>(rows)), 256, s, m);
 }
