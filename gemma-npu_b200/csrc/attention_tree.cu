@@ -20,7 +20,8 @@
 // registers, P turning from the accumulator's layout into the operand's in place, and no warp
 // waits for another until the end of the item, where the 8 results are joined.  (Warps that
 // shared each tile, exchanging P and the maxima through shared memory with three barriers a
-// tile, executed 6 times the instructions: TIMING.)
+// tile, executed 6 times the instructions: 32 sequences of 2048 to 8191 keys, 8 heads of 128, 138 us
+// against 118, the copies alone 104.)
 //
 // The work is cut by what is there: all tiles of all sequences, in order, are dealt in equal
 // contiguous ranges to as many CTAs as fit the GPU at once (every CTA adds up the lengths for

@@ -33,63 +33,81 @@ struct AppendArgs {
   int64_t pos_b, pos_h;
   int* lens_out;
   int kv_heads, n, steps, slots, chunks;
+  int shift;  // log2 of the chunks, or -1
 };
 
-constexpr int kAppendRows = 16;  // path entries per CTA
+constexpr int kAppendRows = 32;   // path entries per CTA
+constexpr int kAppendChunks = 4;  // 16-byte chunks of a thread in flight
 
-// One CTA: up to 16 path entries of one (sequence, cache head).  An entry counts if no
-// entry up to it is negative.
-__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+// One CTA: up to 32 path entries of one (sequence, cache head).  An entry counts if no entry up
+// to it is negative.  The chain length, path, row is all latency, so CTAs are small and many
+// enough to wait it out together (256 sequences of 8 heads, paths of 1 to 17: CTAs of 256
+// threads and 16 entries 9.6 us, one CTA for all heads of a sequence 17.7, these 6.6).
+constexpr int kAppendThreads = 128;
+__global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const AppendArgs a) {
   __shared__ int draft[kAppendRows];
   __shared__ int ended;
   const int b = blockIdx.x / a.kv_heads, c = blockIdx.x % a.kv_heads, tid = threadIdx.x;
   const int j0 = blockIdx.y * kAppendRows, j1 = min(j0 + kAppendRows, a.steps);
   pdl_launch_dependents();
   pdl_wait();
+  const int len = a.lens[b];
+  int d = j0 + tid;  // this thread's entry: a draft's index, or -1
+  if (a.path != nullptr) d = tid < j1 - j0 ? a.path[b * a.path_b + j0 + tid] : -1;
   int count = a.steps;  // entries before the first negative one
   if (a.path != nullptr) {
     if (tid == 0) ended = a.steps;
     __syncthreads();
     const int upto = blockIdx.y == 0 && c == 0 ? a.steps : j1;  // the first CTA counts them all
-    for (int j = tid; j < upto; j += 256)
-      if (a.path[b * a.path_b + j] < 0) atomicMin(&ended, j);
+    if (d < 0 && tid < j1 - j0) atomicMin(&ended, j0 + tid);
+    for (int j = tid; j < upto; j += kAppendThreads)
+      if ((j < j0 || j >= j1) && a.path[b * a.path_b + j] < 0) atomicMin(&ended, j);
     __syncthreads();
     count = ended;
   }
-  const int len = a.lens[b];
   const bool ok = len >= 0 && len <= a.slots;
   if (!ok && tid == 0) cache_bad_index();
-  if (c == 0 && blockIdx.y == 0 && tid == 0) {
+  if (blockIdx.y == 0 && c == 0 && tid == 0) {
     a.lens_out[b] = ok ? min(len + count, a.slots) : len;
     if (ok && len + count > a.slots) cache_bad_index();
   }
   if (!ok) return;
-  if (tid < j1 - j0) {
-    const int j = j0 + tid;
-    int d = -1;
-    if (j < count && len + j < a.slots) {
-      d = a.path != nullptr ? a.path[b * a.path_b + j] : j;
-      if (d >= a.n) {
-        cache_bad_index();
-        d = -1;
-      }
+  const int last = min(min(j1, count), a.slots - len) - j0;  // entries of this CTA with a slot
+  if (tid < kAppendRows) {
+    if (tid >= last) {
+      d = -1;
+    } else if (d >= a.n) {
+      cache_bad_index();
+      d = -1;
     }
     draft[tid] = d;
     if (d >= 0) {
-      if (a.w != nullptr) a.w[b * a.w_b + c * a.w_h + len + j] = a.wn != nullptr ? a.wn[b * a.wn_b + c * a.wn_h + d] : 0.f;
-      if (a.pos != nullptr) a.pos[b * a.pos_b + c * a.pos_h + len + j] = a.seen[b] + j;
+      const int64_t slot = len + j0 + tid;
+      if (a.w != nullptr) a.w[b * a.w_b + c * a.w_h + slot] = a.wn != nullptr ? a.wn[b * a.wn_b + c * a.wn_h + d] : 0.f;
+      if (a.pos != nullptr) a.pos[b * a.pos_b + c * a.pos_h + slot] = a.seen[b] + j0 + tid;
     }
   }
   __syncthreads();
-  const int work = (j1 - j0) * 2 * a.chunks;
-  for (int e = tid; e < work; e += 256) {
-    const int ch = e % a.chunks, row = e / a.chunks, j = row >> 1, d = draft[j];
-    if (d < 0) continue;
-    const bool is_v = row & 1;
-    const uint8_t* src = is_v ? a.vn + b * a.vn_b + c * a.vn_h + d * a.vn_t : a.kn + b * a.kn_b + c * a.kn_h + d * a.kn_t;
-    uint8_t* dst = is_v ? a.v + b * a.v_b + c * a.v_h + static_cast<int64_t>(len + j0 + j) * a.v_s
-                        : a.k + b * a.k_b + c * a.k_h + static_cast<int64_t>(len + j0 + j) * a.k_s;
-    reinterpret_cast<uint4*>(dst)[ch] = reinterpret_cast<const uint4*>(src)[ch];
+  const int work = last * 2 * a.chunks;  // chunks of (entry, K or V)
+  for (int e0 = tid; e0 < work; e0 += kAppendThreads * kAppendChunks) {
+    uint4 x[kAppendChunks];
+    uint8_t* dst[kAppendChunks];
+#pragma unroll
+    for (int i = 0; i < kAppendChunks; ++i) {
+      dst[i] = nullptr;
+      const int e = e0 + kAppendThreads * i;
+      if (e >= work) continue;
+      const int row = a.shift >= 0 ? e >> a.shift : e / a.chunks, ch = e - row * a.chunks, j = row >> 1, from = draft[j];
+      if (from < 0) continue;
+      const bool is_v = row & 1;
+      const uint8_t* src = is_v ? a.vn + b * a.vn_b + c * a.vn_h + from * a.vn_t : a.kn + b * a.kn_b + c * a.kn_h + from * a.kn_t;
+      x[i] = reinterpret_cast<const uint4*>(src)[ch];
+      const int64_t slot = len + j0 + j;
+      dst[i] = (is_v ? a.v + b * a.v_b + c * a.v_h + slot * a.v_s : a.k + b * a.k_b + c * a.k_h + slot * a.k_s) + ch * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < kAppendChunks; ++i)
+      if (dst[i] != nullptr) *reinterpret_cast<uint4*>(dst[i]) = x[i];
   }
 }
 
@@ -215,7 +233,7 @@ __device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, float w, int p
 // lower slot).  A warp holds the keys of 32 KPT consecutive slots in registers, lane i of step
 // j the slot 32 j + i; the budget-th key is found by bisection on its bits, one count over the
 // block an iteration (some 15 of them: a histogram's shared-memory atomics meet in the few
-// exponents that weights have, and took 19 us where this takes US_SELECT for 3658 slots), until
+// exponents that weights have, and took 16 us where this takes 8 for 3658 slots), until
 // a cut has exactly `budget` keys or, among equal ones, the lowest slots fill it.  Ballots in
 // slot order then pair the i-th evicted slot below the budget with the i-th kept one behind it.
 template <int KPT>
@@ -660,7 +678,7 @@ extern "C" int w8_cache_append(const w8_cache_append_args* in, w8_stream_t strea
   const w8_cache_append_args& x = *in;
   int st = cache_shape(x.batch, x.kv_heads, x.slots, x.row_bytes);
   if (st != W8_OK) return st;
-  W8_CHECK_ARG(x.n_new >= 0 && x.steps >= 0 && x.n_new < (1ll << 20) && x.steps <= 16 * 65535, "size beyond the limits");
+  W8_CHECK_ARG(x.n_new >= 0 && x.steps >= 0 && x.n_new < (1ll << 20) && x.steps <= (1 << 20), "size beyond the limits");
   W8_CHECK_ARG(x.path != nullptr || x.steps == x.n_new, "without a path every new token is appended (steps = n_new)");
   if (x.batch == 0) return W8_OK;
   W8_CHECK_ARG(x.lens && x.lens_out, "null lens");
@@ -689,9 +707,10 @@ extern "C" int w8_cache_append(const w8_cache_append_args* in, w8_stream_t strea
   a.lens_out = x.lens_out;
   a.kv_heads = static_cast<int>(x.kv_heads), a.n = static_cast<int>(x.n_new), a.steps = static_cast<int>(x.steps);
   a.slots = static_cast<int>(x.slots), a.chunks = static_cast<int>(x.row_bytes / 16);
+  a.shift = (a.chunks & (a.chunks - 1)) == 0 ? __builtin_ctz(a.chunks) : -1;
   const int64_t parts = std::max<int64_t>(1, (x.steps + w8::kAppendRows - 1) / w8::kAppendRows);
   return launch_cache(w8::cache_append_kernel,
-                      dim3(static_cast<unsigned>(x.batch * x.kv_heads), static_cast<unsigned>(parts)), 256,
+                      dim3(static_cast<unsigned>(x.batch * x.kv_heads), static_cast<unsigned>(parts)), w8::kAppendThreads,
                       reinterpret_cast<cudaStream_t>(stream), a);
 }
 
