@@ -178,9 +178,14 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
     const TreeSpan s = tree_span(a, tree_len(a, p / a.row_tiles), p % a.row_tiles, BM, BN);
     return s.c1 - s.c0 + s.nd;
   };
-  long long total, pos, stop, ctas, item_pos = 0;  // item_pos: first tile of the current item
-  int pair = 0;
-  if (pairs == 1) {
+  long long total = 0, pos = 0, stop = 0, ctas = 0, item_pos = 0;  // item_pos: first tile of the current item
+  int pair = 0, c = 0;
+  if (a.direct) {  // this CTA's item is its number's
+    pair = blockIdx.x / a.kv_heads;
+    c = blockIdx.x % a.kv_heads;
+    stop = pair_tiles(pair);
+    __syncthreads();  // the barriers are initialised
+  } else if (pairs == 1) {
     total = static_cast<long long>(pair_tiles(0)) * a.kv_heads;
     ctas = total < gridDim.x ? total : gridDim.x;
     if (blockIdx.x >= ctas) return;
@@ -221,8 +226,10 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
   int len = tree_len(a, b);
   TreeSpan span = tree_span(a, len, rt, BM, BN);
   int nt = span.c1 - span.c0 + span.nd;
-  int c = static_cast<int>((pos - item_pos) / nt);
-  item_pos += static_cast<long long>(c) * nt;
+  if (!a.direct) {
+    c = static_cast<int>((pos - item_pos) / nt);
+    item_pos += static_cast<long long>(c) * nt;
+  }
   // The next item: the next head, or the next pair's first.
   auto advance = [&]() {
     item_pos += nt;
@@ -248,7 +255,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
     const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
     const bool whole = t0 == 0 && t1 == nt;
     const int64_t part_row = (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * BM;
-    if (t0 == 0 && tid == 0) {
+    if (t0 == 0 && tid == 0 && !a.direct) {
       // The CTA that begins an item says where its pieces are: one in each CTA up to its last tile's.
       const long long last = ((item_pos + nt) * ctas - 1) / total;
       a.info[bc * a.row_tiles + rt] = make_int2(blockIdx.x, static_cast<int>(last - blockIdx.x) + 1);
@@ -783,6 +790,7 @@ int tree_tc_device_status(int clear, int* out);
 // or of CTAs that share all tiles (mma.sync).
 struct TreePlan {
   bool tc;  // the tcgen05 schedule (attention_tree_tc.cu)
+  bool direct;  // mma.sync: a CTA for each item
   int bm, row_tiles, splits, ctas;
   int64_t items;
 };
@@ -817,7 +825,11 @@ static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_
       if (s == 1 || us < best) best = us, p.splits = static_cast<int>(s);
     }
     p.ctas = 0;
+    p.direct = false;
   } else {
+    // An item per CTA: up to 4 tiles (a tile is about 1 us, joining pieces a launch and 3 us), or 8
+    // items an SM, whose ragged lengths even out.
+    p.direct = tiles <= 4 || p.items >= 8 * static_cast<int64_t>(sms);
     p.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms * (d == 64 ? 2 : 1), p.items * tiles, w8::kTreeMaxPieces})));  // TreeCfg::kPerSm
   }
   return p;
@@ -835,10 +847,10 @@ static TreeWs tree_ws(const TreePlan& p, int64_t batch, int64_t kv_heads, int64_
     at += (bytes + 255) / 256 * 256;
     return r;
   };
-  const int64_t part_rows = p.tc ? (p.splits > 1 ? p.items * p.splits * p.bm : 0) : 2 * static_cast<int64_t>(p.ctas) * p.bm;
+  const int64_t part_rows = p.tc ? (p.splits > 1 ? p.items * p.splits * p.bm : 0) : p.direct ? 0 : 2 * static_cast<int64_t>(p.ctas) * p.bm;
   w.part_o = take(part_rows * d * 4);
   w.part_ml = take(part_rows * 8);
-  w.info = take(p.tc ? 0 : p.items * 8);
+  w.info = take(p.tc || p.direct ? 0 : p.items * 8);
   const int64_t rows = batch * kv_heads * group * n;
   w.draft_at = (slots + 3) / 4 * 4;
   w.score_pitch = w.draft_at + (n + 3) / 4 * 4;
@@ -908,7 +920,7 @@ static int tree_main(const w8::TreeArgs& a, int64_t blocks, int device, cudaStre
 template <typename T, int D>
 static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStream_t stream) {
   W8_CHECK_ARG(p.items < (1ll << 31) / 2, "too many row tiles");
-  const int64_t blocks = p.ctas;
+  const int64_t blocks = p.direct ? p.items : p.ctas;
   int st;
   if (p.tc)
     st = tree_tc(a, __is_same(T, __half), D, p.items, device, stream);
@@ -918,7 +930,7 @@ static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStr
     st = tree_main<T, D, 1>(a, blocks, device, stream);
   if (st != W8_OK) return st;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.group * a.n;
-  if (p.tc ? p.splits > 1 : p.ctas > 1) {
+  if (p.tc ? p.splits > 1 : !p.direct && p.ctas > 1) {
     constexpr int kWide = D < 128 ? D : 128;
     if (rows * (D / 32) <= 1024)
       st = launch_tree(w8::attn_tree_combine_kernel<T, D, 32>, dim3(static_cast<unsigned>(rows), D / 32), 256, 0, stream,
@@ -1052,6 +1064,7 @@ extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspa
   a.part_o = reinterpret_cast<float*>(ws + w.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
   a.tma = tma ? 1 : 0;
+  a.direct = p.direct ? 1 : 0;
   a.info = p.tc ? nullptr : reinterpret_cast<int2*>(ws + w.info);
   if (weights) {
     a.lse = reinterpret_cast<float*>(ws + w.lse);

@@ -30,6 +30,7 @@ struct TreeArgs {
   float* part_o;         // [slot][BM][D] fp32
   float2* part_ml;       // [slot][BM]
   int2* info;            // [items], mma.sync schedule
+  int direct;            // mma.sync schedule: CTA i takes item i whole
   float* lse;            // [b * kv_heads + c][R] (log2 units) when the weights are wanted
   float* scores;         // [b * kv_heads + c][R][score_pitch] (log2 units), new tokens from draft_at on
   int64_t score_pitch;
