@@ -100,18 +100,25 @@ struct TreeCfg {
   static_assert(kGroups * kBM * kPitch * 4 <= kOffQ, "the joint outputs fit over the ring");
 };
 
-// Sum over the block; `sm`: 16 words of shared memory, free again on return.
-__device__ __forceinline__ long long block_sum(long long v, long long* sm) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-  __syncthreads();
-  long long s = 0;
-#pragma unroll
-  for (int i = 0; i < kTreeWarps; ++i) s += sm[i];
-  __syncthreads();
-  return s;
+// Quotient of a number that is seldom above 32 bits (a 64-bit division is a call of some 150
+// instructions).
+__device__ __forceinline__ long long div_short(long long x, uint32_t by) {
+  return (x >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(x) / by) : x / by;
 }
+
+// How `total` tiles are dealt to `ctas`: the first `more` CTAs hold one more than the others.
+struct TreeDeal {
+  long long each, more;
+};
+__device__ __forceinline__ long long deal_begin(const TreeDeal& d, long long u) {
+  return u * d.each + (u < d.more ? u : d.more);
+}
+__device__ __forceinline__ int deal_owner(const TreeDeal& d, long long tile) {
+  const long long wide = d.more * (d.each + 1);
+  return static_cast<int>(tile < wide ? div_short(tile, static_cast<uint32_t>(d.each + 1))
+                                      : d.more + div_short(tile - wide, static_cast<uint32_t>(d.each)));
+}
+
 // Exclusive prefix sum over the block and the block's sum.
 __device__ __forceinline__ long long block_scan(long long v, long long* sm, long long& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -174,40 +181,94 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
   // ---- this CTA's range of all tiles.  A pair (sequence, row tile) has kv_heads items of
   // `nt` tiles each; pairs and their heads follow one another.
   const int pairs = a.batch * a.row_tiles;
-  auto pair_tiles = [&](int p) {
-    const TreeSpan s = tree_span(a, tree_len(a, p / a.row_tiles), p % a.row_tiles, BM, BN);
-    return s.c1 - s.c0 + s.nd;
+  auto split_pair = [&](int p, int& b, int& rt) {
+    b = p, rt = 0;
+    if (a.row_tiles > 1) b = p / a.row_tiles, rt = p - b * a.row_tiles;
   };
-  long long total = 0, pos = 0, stop = 0, ctas = 0, item_pos = 0;  // item_pos: first tile of the current item
-  int pair = 0, c = 0;
-  if (a.direct) {  // this CTA's item is its number's
-    pair = blockIdx.x / a.kv_heads;
-    c = blockIdx.x % a.kv_heads;
-    stop = pair_tiles(pair);
-    __syncthreads();  // the barriers are initialised
-  } else if (pairs == 1) {
-    total = static_cast<long long>(pair_tiles(0)) * a.kv_heads;
-    ctas = total < gridDim.x ? total : gridDim.x;
-    if (blockIdx.x >= ctas) return;
-    pos = total * blockIdx.x / ctas;
-    stop = total * (blockIdx.x + 1) / ctas;
+  int b, rt, c = 0, len;
+  TreeSpan span;
+  long long pos = 0, stop = 0, item_pos = 0;  // item_pos: first tile of the current item
+  TreeDeal deal = {1, 0};
+  // Q rows r = i * group + g (query head c * group + g of new token i): every load is under way
+  // before the first is stored, and where the first item is known without the lengths, before
+  // those have come.
+  constexpr int kEach = (BM * CH + kTreeThreads - 1) / kTreeThreads;
+  uint4 qw[kEach];
+  auto fetch_q = [&](int b, int c, int rt) {
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+      const int e = tid + x * kTreeThreads, r = rt * BM + e / CH, ch = e % CH;
+      qw[x] = make_uint4(0, 0, 0, 0);
+      if (e < BM * CH && r < rows) {
+        int i, gq;
+        tree_row(a, r, i, gq);
+        qw[x] = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + gq) * a.q_h +
+                                                i * a.q_t + ch * 8);
+      }
+    }
+  };
+  auto store_q = [&]() {
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+      const int e = tid + x * kTreeThreads, r = e / CH, ch = e % CH;
+      if (e < BM * CH) st_shared_v4(sq + r * (D * 2) + ((ch ^ (r & 7)) << 4), qw[x].x, qw[x].y, qw[x].z, qw[x].w);
+    }
+  };
+  bool q_early = false;
+  if (a.direct || pairs == 1) {
+    // One item (this CTA's number's), or those of one pair.
+    int p = 0;
+    if (a.direct) {
+      p = static_cast<int>(blockIdx.x);
+      if (a.kv_heads > 1) p = blockIdx.x / a.kv_heads, c = blockIdx.x - p * a.kv_heads;
+    }
+    split_pair(p, b, rt);
+    q_early = a.direct || a.kv_heads == 1;
+    if (q_early) fetch_q(b, c, rt);
+    len = tree_len(a, b);
+    span = tree_span<BM, BN>(a, len, rt);
+    const int tiles = span.c1 - span.c0 + span.nd;
+    if (a.direct) {
+      stop = tiles;
+    } else {
+      const long long total = static_cast<long long>(tiles) * a.kv_heads;
+      const uint32_t ctas = total < gridDim.x ? static_cast<uint32_t>(total) : gridDim.x;
+      if (blockIdx.x >= ctas) return;
+      deal.each = div_short(total, ctas);
+      deal.more = total - deal.each * ctas;
+      pos = deal_begin(deal, blockIdx.x);
+      stop = deal_begin(deal, blockIdx.x + 1);
+      c = static_cast<int>(div_short(pos, tiles));
+      item_pos = static_cast<long long>(c) * tiles;
+    }
     __syncthreads();  // the barriers are initialised
   } else {
+    auto pair_tiles = [&](int p) {
+      int pb, prt;
+      split_pair(p, pb, prt);
+      const TreeSpan s = tree_span<BM, BN>(a, tree_len(a, pb), prt);
+      return s.c1 - s.c0 + s.nd;
+    };
     long long* sched = reinterpret_cast<long long*>(smem);  // (the ring is not in use yet)
-    long long mine = 0;
-    for (int p = tid; p < pairs; p += kTreeThreads) mine += pair_tiles(p);
-    total = block_sum(mine, sched) * a.kv_heads;
-    ctas = total < gridDim.x ? total : gridDim.x;
+    long long sum = 0, round;
+    for (int p = tid; p < pairs; p += kTreeThreads) sum += pair_tiles(p);
+    long long excl = block_scan(sum, sched, round);  // (of up to 256 pairs also each one's place)
+    const long long total = round * a.kv_heads;
+    const uint32_t ctas = total < gridDim.x ? static_cast<uint32_t>(total) : gridDim.x;
     if (blockIdx.x >= ctas) return;
-    pos = total * blockIdx.x / ctas;
-    stop = total * (blockIdx.x + 1) / ctas;
+    deal.each = div_short(total, ctas);
+    deal.more = total - deal.each * ctas;
+    pos = deal_begin(deal, blockIdx.x);
+    stop = deal_begin(deal, blockIdx.x + 1);
     // The pair that holds `pos`: a running sum over rounds of pairs.
     long long before = 0;
     for (int p0 = 0;; p0 += kTreeThreads) {
       const int p = p0 + tid;
-      const long long nt = p < pairs ? pair_tiles(p) : 0;
-      long long round;
-      const long long excl = before + block_scan(nt, sched, round);
+      long long nt = sum;
+      if (pairs > kTreeThreads) {
+        nt = p < pairs ? pair_tiles(p) : 0;
+        excl = before + block_scan(nt, sched, round);
+      }
       if (nt > 0 && excl * a.kv_heads <= pos && pos < (excl + nt) * a.kv_heads) {
         sched[16] = p;
         sched[17] = excl * a.kv_heads;
@@ -217,19 +278,17 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
       if (pos < before * a.kv_heads) break;  // (every pair has tiles, and pos < total)
       if (p0 + kTreeThreads >= pairs) return;  // only if the lengths changed under the call
     }
-    pair = static_cast<int>(sched[16]);
+    split_pair(static_cast<int>(sched[16]), b, rt);
     item_pos = sched[17];
+    len = tree_len(a, b);
+    span = tree_span<BM, BN>(a, len, rt);
+    const int tiles = span.c1 - span.c0 + span.nd;
+    c = static_cast<int>(div_short(pos - item_pos, tiles));
+    item_pos += static_cast<long long>(c) * tiles;
     fence_proxy_async_smem();  // the TMA writes the ring next
     __syncthreads();
   }
-  int b = pair / a.row_tiles, rt = pair % a.row_tiles;
-  int len = tree_len(a, b);
-  TreeSpan span = tree_span(a, len, rt, BM, BN);
   int nt = span.c1 - span.c0 + span.nd;
-  if (!a.direct) {
-    c = static_cast<int>((pos - item_pos) / nt);
-    item_pos += static_cast<long long>(c) * nt;
-  }
   // The next item: the next head, or the next pair's first.
   auto advance = [&]() {
     item_pos += nt;
@@ -240,7 +299,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
         ++b;
         len = tree_len(a, b);
       }
-      span = tree_span(a, len, rt, BM, BN);
+      span = tree_span<BM, BN>(a, len, rt);
       nt = span.c1 - span.c0 + span.nd;
     }
   };
@@ -257,8 +316,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
     const int64_t part_row = (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * BM;
     if (t0 == 0 && tid == 0 && !a.direct) {
       // The CTA that begins an item says where its pieces are: one in each CTA up to its last tile's.
-      const long long last = ((item_pos + nt) * ctas - 1) / total;
-      a.info[bc * a.row_tiles + rt] = make_int2(blockIdx.x, static_cast<int>(last - blockIdx.x) + 1);
+      const int last = deal_owner(deal, item_pos + nt - 1);
+      a.info[bc * a.row_tiles + rt] = make_int2(blockIdx.x, last - static_cast<int>(blockIdx.x) + 1);
     }
     // Ring step `i` of this item (tile t0 + i / 2, K or V) into its slot, once every warp has left
     // it: one thread's TMA, or (strides that no map takes) every thread's 16-byte copies into
@@ -300,28 +359,9 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
       for (int i = 0; i < C::kAhead; ++i) load(i);
     __syncwarp();
 
-    // Row r = i * group + g: query head c * group + g of new token i.  (Every load is under way
-    // before the first is stored: they may come from HBM.)
-    {
-      constexpr int kEach = (BM * CH + kTreeThreads - 1) / kTreeThreads;
-      uint4 w[kEach];
-#pragma unroll
-      for (int x = 0; x < kEach; ++x) {
-        const int e = tid + x * kTreeThreads, r = e / CH, ch = e % CH;
-        w[x] = make_uint4(0, 0, 0, 0);
-        if (e < BM * CH && row0 + r < rows) {
-          int i, gq;
-          tree_row(a, row0 + r, i, gq);
-          w[x] = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + gq) * a.q_h +
-                                                 i * a.q_t + ch * 8);
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < kEach; ++x) {
-        const int e = tid + x * kTreeThreads, r = e / CH, ch = e % CH;
-        if (e < BM * CH) st_shared_v4(sq + r * (D * 2) + ((ch ^ (r & 7)) << 4), w[x].x, w[x].y, w[x].z, w[x].w);
-      }
-    }
+    if (!q_early) fetch_q(b, c, rt);
+    store_q();
+    q_early = false;
     // This thread's rows of each 16-row tile: lane / 4 and lane / 4 + 8.
     int tok[MT][2], dep[MT][2], first[MT][2];
     float m[MT][2], l[MT][2];
@@ -334,7 +374,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
         tree_row(a, r, tok[mt][h], gq);
         if (r >= rows) tok[mt][h] = -1;
         dep[mt][h] = r < rows ? tree_depth(a, b, tok[mt][h]) : 0;
-        first[mt][h] = r < rows ? tree_first(a, len, dep[mt][h]) : len;
+        first[mt][h] = r < rows ? tree_first(a, len, dep[mt][h]) : INT32_MAX;  // (no row: sees nothing)
         m[mt][h] = -INFINITY;
         l[mt][h] = 0.f;
       }
@@ -402,6 +442,21 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
             s[mt][e >> 2][e & 3] = s2[0][mt][e >> 2][e & 3] + (kChains > 1 ? s2[kChains - 1][mt][e >> 2][e & 3] : 0.f);
         // ---- masks and the running softmax.  Columns of a thread: key0 + 8 n + 2 (lane % 4) + {0, 1}.
         const int col = (lane & 3) * 2;
+        uint32_t keep[MT][2];  // the step's 16 keys that the row sees
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int lo = max(first[mt][h] - key0, 0), hi = min(end - key0, 16);
+            keep[mt][h] = hi <= lo ? 0u : ((1u << hi) - 1u) & (0xFFFFFFFFu << lo);
+          }
+        if (draft) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              keep[mt][h] = tok[mt][h] >= 0 ? tree_sees16(a, b, tok[mt][h], key0, dep[mt][h]) : 0u;
+        }
         float mx[MT][2];
         bool move = false;
 #pragma unroll
@@ -413,11 +468,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
             for (int n = 0; n < 2; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const int key = key0 + 8 * n + col + e;
-                const bool on = draft ? tok[mt][h] >= 0 && key < end && tree_sees(a, b, tok[mt][h], key, dep[mt][h])
-                                      : key < end && key >= first[mt][h];
                 float& v = s[mt][n][2 * h + e];
-                v = on ? v * a.scale_log2 : -INFINITY;
+                v = (keep[mt][h] >> (8 * n + col + e)) & 1u ? v * a.scale_log2 : -INFINITY;
                 x = fmaxf(x, v);
               }
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));

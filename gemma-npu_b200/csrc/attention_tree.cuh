@@ -175,6 +175,38 @@ __device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i,
   return bits;
 }
 
+// tree_sees of the new tokens j0 .. j0 + 15 as bits, in little code (it stands beside the common
+// tiles, which have none of it).
+__device__ __forceinline__ uint32_t tree_sees16(const TreeArgs& a, int b, int i, int j0, int depth_i) {
+  const int left = min(a.n - j0, 16);
+  if (left <= 0) return 0u;
+  uint32_t bits = (1u << left) - 1u;
+  if (a.tree == nullptr) {
+    bits &= i < j0 ? 0u : (2u << min(i - j0, 15)) - 1u;
+  } else {
+    const uint8_t* row = a.tree + b * a.tree_b + i * a.tree_i + j0;
+    uint32_t on = 0;
+    if (left == 16 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+      const uint4 w = *reinterpret_cast<const uint4*>(row);
+      on = nonzero_bytes(w.x) | nonzero_bytes(w.y) << 4 | nonzero_bytes(w.z) << 8 | nonzero_bytes(w.w) << 12;
+    } else {
+      uint8_t v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = e < left ? row[e] : 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) on |= v[e] != 0 ? 1u << e : 0u;
+    }
+    bits &= on;
+  }
+  if (a.window > 0)
+#pragma unroll 1
+    for (uint32_t rest = bits; rest != 0u; rest &= rest - 1u) {
+      const int e = __ffs(rest) - 1;
+      if (static_cast<int64_t>(tree_depth(a, b, j0 + e)) <= static_cast<int64_t>(depth_i) - a.window) bits &= ~(1u << e);
+    }
+  return bits;
+}
+
 // New tokens whose values are not all finite, one bit each; tokens 2048 apart share a bit, so
 // a set bit only says that the token's values must be looked at.
 constexpr int kPoisonWords = 64;
@@ -190,16 +222,19 @@ __device__ __forceinline__ uint32_t poison_of(const volatile uint32_t* words, in
 struct TreeSpan {
   int c0, c1, nd;
 };
-__device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int len, int rt, int bm, int bn) {
+template <int bm, int bn>  // (powers of two)
+__device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int len, int rt) {
   TreeSpan s;
   const int rows = a.group * a.n;
-  const int i0 = rt * bm / a.group, i1 = min((rt + 1) * bm, rows) - 1;
+  int i0, last, g;  // tokens of the first and last row
+  tree_row(a, rt * bm, i0, g);
+  tree_row(a, min((rt + 1) * bm, rows) - 1, last, g);
   // Without given depths the first row's token is the shallowest; with them, 0 is a bound.
-  s.c0 = tree_first(a, len, a.depth != nullptr ? 0 : i0) / bn;
-  s.c1 = (len + bn - 1) / bn;
+  s.c0 = static_cast<uint32_t>(tree_first(a, len, a.depth != nullptr ? 0 : i0)) / bn;
+  s.c1 = static_cast<uint32_t>(len + bn - 1) / bn;
   // A causal chunk's row tile needs the new keys up to its last token only.
-  const int last = a.tree != nullptr ? a.n - 1 : i1 / a.group;
-  s.nd = last / bn + 1;
+  if (a.tree != nullptr) last = a.n - 1;
+  s.nd = static_cast<uint32_t>(last) / bn + 1;
   if (s.c0 > s.c1) s.c0 = s.c1;
   return s;
 }

@@ -138,7 +138,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
   // The pair's tiles: [t0, t1) of its committed, then new-token tiles; a split of an item with
   // fewer tiles than splits has none (both CTAs agree).
   const int len = tree_len(a, b);
-  const TreeSpan span = tree_span(a, len, rt, 2 * kTtBM, kTtBN);
+  const TreeSpan span = tree_span<2 * kTtBM, kTtBN>(a, len, rt);
   const int nc = span.c1 - span.c0, nt = nc + span.nd;
   const int t0 = static_cast<int>(static_cast<int64_t>(nt) * split / a.splits);
   const int t1 = static_cast<int>(static_cast<int64_t>(nt) * (split + 1) / a.splits);
