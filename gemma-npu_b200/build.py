@@ -57,7 +57,9 @@ def build_binding(force=False, quiet=False):
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
     dirs = [*include_paths(), cuda, sysconfig.get_paths()["include"]]
     tmp = BINDING + ".tmp"
-    subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+    # The compiler that nvcc links with: a module with a libstdc++ of its own in it must not meet
+    # torch's.
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                     *(f"-isystem{d}" for d in dirs), src, "-o", tmp, *(f"-L{d}" for d in library_paths()),
                     "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"], check=True)

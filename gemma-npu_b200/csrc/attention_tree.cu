@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              keep[mt][h] = tok[mt][h] >= 0 ? tree_sees16(a, b, tok[mt][h], key0, dep[mt][h]) : 0u;
+              keep[mt][h] = tree_sees16(a, b, tok[mt][h], key0, dep[mt][h]);
         }
         float mx[MT][2];
         bool move = false;

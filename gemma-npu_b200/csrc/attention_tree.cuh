@@ -175,35 +175,62 @@ __device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i,
   return bits;
 }
 
-// tree_sees of the new tokens j0 .. j0 + 15 as bits, in little code (it stands beside the common
-// tiles, which have none of it).
+// What a warp's rows see of the new tokens j0 .. j0 + 63, as bits: each lane brings its row's
+// token (ascending over the lanes, -1 for none) and its depth.  The rows of a token share its
+// line of the tree, which the warp reads once, a byte a lane (any alignment).  All lanes.
+__device__ __forceinline__ void tree_sees64_rows(const TreeArgs& a, int b, int tok, int j0, int depth_i,
+                                                 uint32_t (&keep)[2]) {
+  const int lane = threadIdx.x & 31;
+  keep[0] = keep[1] = 0u;
+  const int j[2] = {j0 + lane, j0 + 32 + lane};
+  int dj[2] = {0, 0};
+  if (a.window > 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (j[h] < a.n) dj[h] = tree_depth(a, b, j[h]);
+  }
+  const int hi = __reduce_max_sync(0xffffffffu, tok);
+  const int lo = __reduce_min_sync(0xffffffffu, tok < 0 ? INT32_MAX : tok);
+#pragma unroll 4
+  for (int t = lo; t <= hi; ++t) {  // (no row at all: lo > hi)
+    const unsigned rows_of = __ballot_sync(0xffffffffu, tok == t);
+    const int dt = __shfl_sync(0xffffffffu, depth_i, rows_of ? __ffs(rows_of) - 1 : 0);
+    const uint8_t* line = a.tree != nullptr ? a.tree + b * a.tree_b + t * a.tree_i : nullptr;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bool on = j[h] < a.n;
+      if (on) on = line != nullptr ? line[j[h]] != 0 : j[h] <= t;
+      if (a.window > 0) on = on && static_cast<int64_t>(dj[h]) > static_cast<int64_t>(dt) - a.window;
+      const uint32_t bits = __ballot_sync(0xffffffffu, on);
+      if (tok == t) keep[h] = bits;
+    }
+  }
+}
+
+// The same for one row's new tokens j0 .. j0 + 15, in little code (it stands beside the common
+// tiles, which have none of it).  All lanes, of the same j0.
 __device__ __forceinline__ uint32_t tree_sees16(const TreeArgs& a, int b, int i, int j0, int depth_i) {
   const int left = min(a.n - j0, 16);
-  if (left <= 0) return 0u;
-  uint32_t bits = (1u << left) - 1u;
+  uint32_t bits = left <= 0 || i < 0 ? 0u : (1u << left) - 1u;
   if (a.tree == nullptr) {
     bits &= i < j0 ? 0u : (2u << min(i - j0, 15)) - 1u;
-  } else {
+  } else if (bits != 0u) {
     const uint8_t* row = a.tree + b * a.tree_b + i * a.tree_i + j0;
-    uint32_t on = 0;
-    if (left == 16 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
-      const uint4 w = *reinterpret_cast<const uint4*>(row);
-      on = nonzero_bytes(w.x) | nonzero_bytes(w.y) << 4 | nonzero_bytes(w.z) << 8 | nonzero_bytes(w.w) << 12;
-    } else {
-      uint8_t v[16];
+    uint8_t v[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = e < left ? row[e] : 0;
+    for (int e = 0; e < 16; ++e) v[e] = e < left ? row[e] : 0;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) on |= v[e] != 0 ? 1u << e : 0u;
-    }
-    bits &= on;
+    for (int e = 0; e < 16; ++e)
+      if (v[e] == 0) bits &= ~(1u << e);
   }
-  if (a.window > 0)
-#pragma unroll 1
-    for (uint32_t rest = bits; rest != 0u; rest &= rest - 1u) {
-      const int e = __ffs(rest) - 1;
-      if (static_cast<int64_t>(tree_depth(a, b, j0 + e)) <= static_cast<int64_t>(depth_i) - a.window) bits &= ~(1u << e);
-    }
+  if (a.window > 0) {
+    const int e0 = threadIdx.x & 15;
+    const int dj = e0 < left ? tree_depth(a, b, j0 + e0) : 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (static_cast<int64_t>(__shfl_sync(0xffffffffu, dj, e)) <= static_cast<int64_t>(depth_i) - a.window)
+        bits &= ~(1u << e);
+  }
   return bits;
 }
 

@@ -348,8 +348,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         uint32_t keep[2];
         const int k0 = key0 + 64 * hv;
         if (draft) {
+          if (a.tree == nullptr && a.depth == nullptr) {  // a plain chunk: closed forms
 #pragma unroll
-          for (int j = 0; j < 2; ++j) keep[j] = tok >= 0 ? tree_sees32(a, b, tok, k0 + 32 * j, dep) : 0u;
+            for (int j = 0; j < 2; ++j) keep[j] = tok >= 0 ? tree_sees32(a, b, tok, k0 + 32 * j, dep) : 0u;
+          } else {
+            tree_sees64_rows(a, b, tok, k0, dep, keep);
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {

@@ -12,7 +12,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <set>
-#include <sstream>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -39,24 +38,27 @@ struct Refused : std::runtime_error {  // ValueError
 };
 struct Raised {};  // a Python exception is set
 
+// Pieces of a message, without iostreams (whose number formatting needs the locale of the one
+// libstdc++ that every library of the process must then share).
+std::string text(const char* s) { return s; }
+std::string text(const std::string& s) { return s; }
+std::string text(int64_t v) { return std::to_string(v); }
+std::string text(at::ScalarType t) { return c10::toString(t); }
+std::string text(const at::Device& d) { return d.str(); }
+std::string text(at::IntArrayRef s) {
+  std::string o = "(";
+  for (size_t i = 0; i < s.size(); ++i) o += (i ? ", " : "") + std::to_string(s[i]);
+  return o + (s.size() == 1 ? ",)" : ")");
+}
+
 template <typename... A>
 [[noreturn]] void refuse(const A&... a) {
-  std::ostringstream s;
-  (s << ... << a);
-  throw Refused(s.str());
+  throw Refused((text(a) + ...));
 }
 #define NEED(cond, ...)            \
   do {                             \
     if (!(cond)) refuse(__VA_ARGS__); \
   } while (0)
-
-std::string shape_text(at::IntArrayRef s) {
-  std::ostringstream o;
-  o << "(";
-  for (size_t i = 0; i < s.size(); ++i) o << (i ? ", " : "") << s[i];
-  o << (s.size() == 1 ? ",)" : ")");
-  return o.str();
-}
 
 bool is_none(PyObject* o) { return o == nullptr || o == Py_None; }
 
@@ -92,7 +94,7 @@ void expect(const Tensor& t, const char* name, at::ScalarType dtype, at::Device 
   NEED(t.device() == dev, name, " must be on ", dev, " (got ", t.device(), ")");
 }
 void expect_shape(const Tensor& t, const char* name, at::IntArrayRef shape) {
-  NEED(t.sizes() == shape, name, " must have shape ", shape_text(shape), " (got ", shape_text(t.sizes()), ")");
+  NEED(t.sizes() == shape, name, " must have shape ", text(shape), " (got ", text(t.sizes()), ")");
 }
 const Tensor& vector(PyObject* o, const char* name, at::IntArrayRef shape, at::ScalarType dtype, at::Device dev) {
   const Tensor& t = tensor(o, name);
@@ -145,7 +147,7 @@ void check(int status, const char* name) {
   PyObject* r = PyObject_CallFunction(check_status, "is", status, name);
   Py_XDECREF(r);
   if (PyErr_Occurred()) throw Raised();
-  refuse(name, ": status ", status);
+  refuse(name, ": status ", static_cast<int64_t>(status));
 }
 
 int type_code(at::ScalarType t) {
