@@ -767,6 +767,49 @@ __global__ void __launch_bounds__(256) attn_tree_combine_kernel(const TreeArgs a
   }
 }
 
+// The same for many rows of few pieces: 4 columns a thread, the pieces in turn, no barrier.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attn_tree_combine_rows_kernel(const TreeArgs a, int bm, int64_t all) {
+  constexpr int kLanes = D / 4;
+  const int rows = a.group * a.n;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = at / kLanes;
+  if (row >= all) return;
+  const int col = static_cast<int>(at % kLanes) * 4;
+  const int bc = static_cast<int>(row / rows), r = static_cast<int>(row % rows);
+  const int64_t item = static_cast<int64_t>(bc) * a.row_tiles + r / bm;
+  const bool dealt = a.info != nullptr;
+  const int2 info = dealt ? a.info[item] : make_int2(0, a.splits);
+  if (info.y <= 1) return;  // written whole
+  auto slot = [&](int s) { return dealt ? tree_slot(info, s) : item * a.splits + s; };
+  float mx = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < info.y; ++s) mx = fmaxf(mx, a.part_ml[slot(s) * bm + r % bm].x);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < info.y; ++s) {
+    const int64_t pr = slot(s) * bm + r % bm;
+    const float2 ml = a.part_ml[pr];
+    const float4 p = *reinterpret_cast<const float4*>(a.part_o + pr * D + col);
+    // (nothing seen: 0, and what stands in the row is not looked at; a maximum of -inf with another
+    // sum: NaN scores, which must show)
+    const float f = ml.x != -INFINITY ? ex2_tree(ml.x - mx) : ml.y == 0.f ? 0.f : 1.f;
+    if (f != 0.f) {
+      sum += f * ml.y;
+      v.x += f * p.x, v.y += f * p.y, v.z += f * p.z, v.w += f * p.w;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int b = bc / a.kv_heads, c = bc % a.kv_heads;
+  int i, gq;
+  tree_row(a, r, i, gq);
+  uint16_t* dst = a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + gq) * a.o_h + i * a.o_t + col;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+  if (a.lse != nullptr && col == 0) a.lse[row] = sum == 0.f ? INFINITY : mx + log2f(sum);
+}
+
 // Accumulated weights: slot j gets weights[j] + sum over the R rows of p_rj, p from the stored
 // scores and the rows' log-sum-exp (the sums in the rows' order: the same bits every time).
 // Four slots a thread, 16-byte loads of four rows in flight: bound by reading the scores.
@@ -879,9 +922,14 @@ static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_
     p.ctas = 0;
     p.direct = false;
   } else {
-    // An item per CTA: up to 4 tiles (a tile is about 1 us, joining pieces a launch and 3 us), or 8
-    // items an SM, whose ragged lengths even out.
-    p.direct = tiles <= 4 || p.items >= 8 * static_cast<int64_t>(sms);
+    // An item per CTA, or all tiles dealt evenly: by estimated times.  A tile is about 1 us (2 us
+    // of 64 KB boxes), an item's start and end 3 us, joining the pieces a launch of 4 us.  From 8
+    // items an SM on ragged lengths even out by themselves.
+    const double tile_us = d >= 256 ? 2.0 : 1.0;
+    const double waves = static_cast<double>((p.items + sms - 1) / std::max(sms, 1));
+    const double alone = waves * (static_cast<double>(tiles) * tile_us + 3);
+    const double dealt = static_cast<double>(p.items) * static_cast<double>(tiles) / sms * tile_us + 3 * (waves + 1) + 4;
+    p.direct = alone <= dealt || p.items >= 8 * static_cast<int64_t>(sms);
     p.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms * (d == 64 ? 2 : 1), p.items * tiles, w8::kTreeMaxPieces})));  // TreeCfg::kPerSm
   }
   return p;
@@ -927,7 +975,7 @@ static int tree_shape(int64_t batch, int64_t heads, int64_t kv_heads, int64_t he
 }
 
 template <typename Kern, typename... Args>
-static int launch_tree(Kern kern, dim3 grid, int threads, int smem, cudaStream_t stream, Args... args) {
+static int launch_tree(Kern kern, dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads, 1, 1);
@@ -983,13 +1031,17 @@ static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStr
   if (st != W8_OK) return st;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.group * a.n;
   if (p.tc ? p.splits > 1 : !p.direct && p.ctas > 1) {
+    // Few rows: a CTA each, or for 32 columns of each, since their pieces may be many.
     constexpr int kWide = D < 128 ? D : 128;
     if (rows * (D / 32) <= 1024)
       st = launch_tree(w8::attn_tree_combine_kernel<T, D, 32>, dim3(static_cast<unsigned>(rows), D / 32), 256, 0, stream,
                        a, p.bm);
-    else
+    else if (rows <= 512)
       st = launch_tree(w8::attn_tree_combine_kernel<T, D, kWide>, dim3(static_cast<unsigned>(rows), D / kWide), 256, 0,
                        stream, a, p.bm);
+    else
+      st = launch_tree(w8::attn_tree_combine_rows_kernel<T, D>, dim3(static_cast<unsigned>((rows * (D / 4) + 255) / 256)),
+                       256, 0, stream, a, p.bm, rows);
     if (st != W8_OK) return st;
   }
   if (a.scores != nullptr) {
