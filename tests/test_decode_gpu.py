@@ -121,6 +121,15 @@ SHAPES = [
     (40, 32, 8, 128, 1, 100, [(7 * i) % 101 for i in range(40)], 0),
     (1, 8, 1, 256, 300, 600, [600], 512),
     (2, 16, 2, 256, 33, 500, [500, 64], 0),
+    # many pieces of many rows: tiles dealt over CTAs (mma.sync), splits of row tiles (tcgen05)
+    (10, 64, 4, 128, 1, 3000, [3000, 1, 700, 2999, 128, 129, 0, 2000, 64, 1500], 0),
+    (10, 64, 4, 64, 1, 3000, [3000, 1, 700, 2999, 256, 257, 0, 2000, 64, 1500], 900),
+    (3, 24, 2, 512, 1, 2000, [2000, 3, 1111], 0),
+    (3, 8, 2, 128, 40, 4000, [4000, 2222, 31], 0),
+    (1, 6, 2, 256, 50, 3000, [2900], 0),
+    (300, 4, 2, 128, 1, 300, [(37 * i) % 301 for i in range(300)], 100),
+    (1, 8, 1, 256, 64, 0, [0], 0),
+    (1, 16, 1, 512, 3, 0, [0], 2),
 ]
 
 
@@ -251,8 +260,9 @@ def test_weights(cuda, shape, in_place):
         assert torch.equal(w, prev)
 
 
-def test_same_bits_every_time(cuda):
-    a = make(1, 2, 8, 1, 256, 3, 3000, [3000, 1234])
+@pytest.mark.parametrize("N", [1, 3, 60])
+def test_same_bits_every_time(cuda, N):
+    a = make(1, 2, 8, 1, 256, N, 3000, [3000, 1234])
     w = torch.rand((2, 1, 3000), device="cuda")
     first = w8.attention_tree(*a, scale=0.06, weights=w, weights_out=torch.zeros_like(w))
     for _ in range(3):
