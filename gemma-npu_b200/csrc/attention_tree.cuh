@@ -248,6 +248,7 @@ __device__ __forceinline__ uint32_t poison_of(const volatile uint32_t* words, in
 // tiles [0, nd).
 struct TreeSpan {
   int c0, c1, nd;
+  int low;  // first committed slot that a row may see: what lies before it may hold anything
 };
 template <int bm, int bn>  // (powers of two)
 __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int len, int rt) {
@@ -257,7 +258,8 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int len, int rt
   tree_row(a, rt * bm, i0, g);
   tree_row(a, min((rt + 1) * bm, rows) - 1, last, g);
   // Without given depths the first row's token is the shallowest; with them, 0 is a bound.
-  s.c0 = static_cast<uint32_t>(tree_first(a, len, a.depth != nullptr ? 0 : i0)) / bn;
+  s.low = tree_first(a, len, a.depth != nullptr ? 0 : i0);
+  s.c0 = static_cast<uint32_t>(s.low) / bn;
   s.c1 = static_cast<uint32_t>(len + bn - 1) / bn;
   // A causal chunk's row tile needs the new keys up to its last token only.
   if (a.tree != nullptr) last = a.n - 1;

@@ -14,10 +14,10 @@
 // group, 4000 keys: 672 us).  The key axis is split over clusters while they would leave
 // SMs idle, and the partial outputs joined by the combine kernel of attention_tree.cu.
 //
-// What a decode adds to prefill is ragged: the committed length ends inside a tile, whose
-// rows behind it may hold NaN, and so may a new token's V (0 * NaN is NaN in the product).
-// In such a tile ("careful": the last committed one if it is partial, and every tile of new
-// tokens) V completes on a barrier of its own CTA, the softmax threads clear what must not
+// What a decode adds to prefill is ragged: the committed length ends (and the window begins)
+// inside a tile, whose rows beyond may hold NaN, and so may a new token's V (0 * NaN is NaN in
+// the product).  In such a tile ("careful": the first and last committed ones if they are
+// partial, and tiles of new tokens that some row does not see whole) V completes on a barrier of its own CTA, the softmax threads clear what must not
 // count before they hand over P, and non-finite values are added at the end to the rows that
 // do see them.  Every wait is bounded, as in attention_tc.cu.
 #include "attention_tree.cuh"
@@ -151,7 +151,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
   const int tok_lo = rt * (2 * kTtBM) / a.group, tok_hi = (min((rt + 1) * (2 * kTtBM), rows) - 1) / a.group;
   auto careful = [&](int i) {
     const int key0 = key0_of(i);
-    if (!is_draft(i)) return key0 + kTtBN > len;
+    if (!is_draft(i)) return key0 + kTtBN > len || key0 < span.low;
     return a.tree != nullptr || a.depth != nullptr || key0 + kTtBN - 1 > tok_lo ||
            (a.window > 0 && key0 <= tok_hi - a.window);
   };
@@ -437,7 +437,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
             const int row = (e >> 3) & (kTtBN - 1);  // blocks of [128 keys x 128 bytes]
             uint4* w = reinterpret_cast<uint4*>(vs) + e;
             if (!draft) {
-              if (key0 + row >= len) *w = make_uint4(0, 0, 0, 0);
+              if (key0 + row >= len || key0 + row < span.low) *w = make_uint4(0, 0, 0, 0);
             } else {
               uint4 x = *w;
               if (nonfinite_bits<T>(x.x) | nonfinite_bits<T>(x.y) | nonfinite_bits<T>(x.z) | nonfinite_bits<T>(x.w)) {

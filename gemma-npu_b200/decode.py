@@ -79,7 +79,12 @@ def attention_tree(q, k, v, lens, k_new, v_new, tree=None, depth=None, window=0,
     With `weights` fp32 [B, KV, S] returns (out, weights_out, draft_weights): weights_out =
     weights plus the probabilities of each committed slot summed over the group's heads and
     the N tokens (in place unless weights_out is given; slots behind lens are left alone),
-    draft_weights fp32 [B, KV, N] the same sums of the new tokens."""
+    draft_weights fp32 [B, KV, N] the same sums of the new tokens.  Every row of q counts, a
+    padding draft's too.
+
+    A new token's values may be infinite or NaN where some token must not see them, and so may
+    slots that no window reaches; the committed slots that one reaches must be finite.  out
+    must not overlap the inputs."""
     return (_binding or _c()).attention_tree(q, k, v, lens, k_new, v_new, tree, depth, window, scale, out, weights,
                                              weights_out, draft_weights)
 

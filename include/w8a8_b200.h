@@ -320,8 +320,11 @@ typedef struct w8_attention_tree_args {
  * Grouped-query heads, head_dim 64, 128, 256 or 512, fp32 softmax and sums.  With weights:
  * weights_out[b, c, j] = weights[b, c, j] + the probabilities of slot j summed over the
  * group's heads and the n tokens (slots behind lens[b] are left alone), and draft_weights
- * the same sums for the new tokens.  Values of a new token that some token must not see may
- * be infinite or NaN; those of a committed slot that any token sees must be finite.
+ * the same sums for the new tokens (every row of q counts, a padding one too).  A new token's
+ * values may be infinite or NaN where some token must not see them; those of the committed
+ * slots that any token's window reaches must be finite (with depths given, a window is taken
+ * to reach as far back as depth 0's).  out must not overlap the inputs, weights_out nothing
+ * but weights.
  * Replaces full_attention / sliding_attention behind cached keys (pipeline.py:133-180) and
  * the decode attention (local_attn.py:44-83). */
 int w8_attention_tree(const w8_attention_tree_args* args, void* workspace, int64_t workspace_bytes,
@@ -347,7 +350,8 @@ typedef struct w8_cache_append_args {
 
 /* Rows path[b, 0], path[b, 1], ... of the new keys and values go to the slots lens[b],
  * lens[b] + 1, ... (a drafted tree's accepted path, or the new token itself), with their
- * weights and positions; lens_out[b] = lens[b] + their number. */
+ * weights and positions; lens_out[b] = lens[b] + their number.  The new rows must not overlap
+ * the caches. */
 int w8_cache_append(const w8_cache_append_args* args, w8_stream_t stream);
 
 typedef struct w8_cache_evict_args {
@@ -382,7 +386,7 @@ int64_t w8_cache_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t 
  * -inf and come last, in their own order.  slot_order != 0 (n = beams): the best
  * continuation of a surviving beam stands in that beam's slot and the others fill the free
  * slots, best first, so that w8_cache_reorder moves as little as can be.  At most 32 beams
- * and 64 continuations. */
+ * and 64 continuations, batch * beams at most 65535. */
 int w8_beam_select(const void* logits, int dtype, int64_t stride_b, int64_t stride_k, const float* scores,
                    const uint8_t* finished, int64_t pad, float cap, int64_t batch, int64_t beams, int64_t vocab,
                    int64_t n, int slot_order, float* out_scores, int64_t* out_beam, int64_t* out_token,
@@ -394,8 +398,8 @@ int64_t w8_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t voc
  * same for all; 16-byte aligned) state i of a group takes the first lens[parent] slots
  * (NULL: all) of state beam[i] of its group.  Any map of beams is right, the same parent
  * twice and swaps included.  beam is int64 (beam_i64 != 0) or int32 [groups, beams], lens
- * [groups * beams].  `tensors` and `strides` are host arrays, read before the call returns;
- * at most 32 beams. */
+ * [groups * beams].  The tensors must not overlap.  `tensors` and `strides` are host arrays,
+ * read before the call returns; at most 32 beams, groups * heads at most 65535. */
 int w8_cache_reorder(void* const* tensors, int64_t count, const int64_t* strides, const void* beam, int beam_i64,
                      const int32_t* lens, int64_t groups, int64_t beams, int64_t heads, int64_t slots,
                      int64_t row_bytes, w8_stream_t stream);

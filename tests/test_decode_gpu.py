@@ -225,6 +225,19 @@ def test_infinite_values_stay_with_those_who_see_them(cuda, D, dt):
     assert got[0, :, 35:, 7].isnan().all() and got[1, :, 20:].isnan().all()
 
 
+@pytest.mark.parametrize("N", [1, 40])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_slots_before_the_window_may_hold_anything(cuda, D, N):
+    """NaN in the committed slots that no token's window reaches, inside the first tile read."""
+    B, H, KV, S, W = 2, 4, 1, 700, 100
+    q, k, v, ln, kn, vn = make(D + N, B, H, KV, D, N, S, [700, 333])
+    want = want_attention(q, k, v, ln, kn, vn, window=W, scale=D ** -0.5)
+    for b, n in enumerate([700, 333]):
+        k[b, :, :n - W + 1] = math.nan
+        v[b, :, :n - W + 1] = math.nan
+    check_out(w8.attention_tree(q, k, v, ln, kn, vn, window=W, scale=D ** -0.5), want, torch.bfloat16)
+
+
 WEIGHTS = [
     (1, 8, 1, 256, 1, 3000, [2900], 0, False),
     (4, 8, 2, 128, 1, 300, [300, 0, 64, 131], 0, False),
