@@ -1104,6 +1104,13 @@ extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspa
   const bool weights = x.weights != nullptr || x.weights_out != nullptr || x.draft_weights != nullptr;
   W8_CHECK_ARG(!weights || (x.draft_weights && (x.slots == 0 || (x.weights && x.weights_out))),
                "weights, weights_out and draft_weights come together");
+  // In place only with the same layout: rows of one would be other rows of the other.
+  W8_CHECK_ARG(!weights || x.weights != x.weights_out ||
+                   ((x.batch == 1 || x.weights_stride[0] == x.weights_out_stride[0]) &&
+                    (x.kv_heads == 1 || x.weights_stride[1] == x.weights_out_stride[1])),
+               "weights_out is weights with other strides");
+  W8_CHECK_ARG(x.out != x.q && x.out != x.k && x.out != x.v && x.out != x.k_new && x.out != x.v_new,
+               "out must not be an input");
   const void* ptrs[6] = {x.q, x.k, x.v, x.k_new, x.v_new, x.out};
   const int64_t* strides[6] = {x.q_stride, x.k_stride, x.v_stride, x.k_new_stride, x.v_new_stride, x.out_stride};
   for (int i = 0; i < 6; ++i) {

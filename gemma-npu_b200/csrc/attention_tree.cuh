@@ -237,9 +237,6 @@ __device__ __forceinline__ uint32_t tree_sees16(const TreeArgs& a, int b, int i,
 // New tokens whose values are not all finite, one bit each; tokens 2048 apart share a bit, so
 // a set bit only says that the token's values must be looked at.
 constexpr int kPoisonWords = 64;
-__device__ __forceinline__ void poison_mark(uint32_t* words, int j) {
-  atomicOr(&words[(j >> 5) & (kPoisonWords - 1)], 1u << (j & 31));
-}
 __device__ __forceinline__ uint32_t poison_of(const volatile uint32_t* words, int j0) {  // of j0 .. j0 + 31, j0 % 32 == 0
   return words[(j0 >> 5) & (kPoisonWords - 1)];
 }

@@ -9,17 +9,19 @@
 //                      back into the S buffer
 //   O   += P_j V_j     A = P_j from TMEM, each CTA staging half of V's columns
 // m moves only when a tile's maximum exceeds it by more than 8 (log2 units).  Many rows per
-// key make this bound by the MMAs and the softmax's exponentials, not by HBM; mma.sync
-// reaches a fifth of the rate here (a tree of 64 drafts for 16 sequences, D 256, 8 heads a
-// group, 4000 keys: 672 us).  The key axis is split over clusters while they would leave
-// SMs idle, and the partial outputs joined by the combine kernel of attention_tree.cu.
+// key make this bound by the MMAs and the softmax's exponentials, not by HBM: trees of 64
+// drafts for 16 sequences, D 256, 8 heads a group, 2000 to 4000 keys take 65 us here (a tile
+// some 2650 clocks of a pair, its MMAs 2048) and 672 with mma.sync.  The key axis is split over
+// clusters while they would leave SMs idle, and the partial outputs joined by the combine
+// kernel of attention_tree.cu.
 //
 // What a decode adds to prefill is ragged: the committed length ends (and the window begins)
 // inside a tile, whose rows beyond may hold NaN, and so may a new token's V (0 * NaN is NaN in
 // the product).  In such a tile ("careful": the first and last committed ones if they are
-// partial, and tiles of new tokens that some row does not see whole) V completes on a barrier of its own CTA, the softmax threads clear what must not
-// count before they hand over P, and non-finite values are added at the end to the rows that
-// do see them.  Every wait is bounded, as in attention_tc.cu.
+// partial, and tiles of new tokens that some row does not see whole) V completes on a barrier
+// of its own CTA, the softmax threads clear what must not count before they hand over P, and
+// non-finite values are added at the end to the rows that do see them.  Every wait is bounded,
+// as in attention_tc.cu.
 #include "attention_tree.cuh"
 #include "attn_tc.cuh"
 

@@ -6,14 +6,16 @@
 // and per sequence the n largest totals over all (k, t), ties to the lower beam, then the
 // lower token.  Within a beam the order of totals is the order of the logits, so one pass
 // over the logits yields everything: each CTA streams a chunk of one beam's logits, keeping
-// a running maximum and sum of e^y per thread and, in shared memory, the chunk's n best
-// (value, token) keys; a second kernel merges the chunks' sorted lists per beam, forms the
-// totals in 64 bits and merges the beams.
+// a running maximum and sum of e^y per thread and the maximum of every segment of 16 logits;
+// after 24 tiles a value that at least n logits reach is found from the threads' maxima, and
+// only the segments that reach it are read again for candidates (value, token), of which the
+// n best stay.  A second kernel merges the chunks' sorted lists per beam, forms the totals in
+// 64 bits and merges the beams.
 //
-// Bound by reading the logits once.  A logit costs one comparison against the current
-// threshold (the n-th best key so far) besides its exponential; only the few that pass it
-// go to shared memory.  The first tile's threshold comes from the warps' largest thread
-// maxima, later ones from pruning the candidates to n.
+// The bytes are the logits once, but a logit's softcap and exponential cost more issue slots
+// than its bytes: 24 x 8 beams of 262144 bf16 logits, softcapped, take 34 us (3.0 TB/s) and
+// the merge 8 us; the stream with a tanh of the special-function unit, or with comparisons of
+// every logit against a threshold and barriers between tiles, took 76 us.
 #include "common.cuh"
 
 #include <cuda_fp16.h>

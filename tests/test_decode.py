@@ -37,6 +37,27 @@ def test_attention_tree_refuses(change, status):
     assert _lib.lib().w8_attention_tree(tree_args(**change), None, 0, None) == status
 
 
+@pytest.mark.parametrize("same", ["q", "k", "v", "k_new", "v_new"])
+def test_attention_tree_refuses_to_overwrite_an_input(same):
+    at = {name: 4096 + 256 * i for i, name in enumerate(["q", "k", "v", "k_new", "v_new"])}[same]
+    assert _lib.lib().w8_attention_tree(tree_args(out=at), None, 0, None) == _lib.W8_ERR_INVALID_ARG
+    assert b"out must not" in _lib.lib().w8_last_error()
+
+
+def test_in_place_needs_one_layout():
+    """Weights updated in place through strides other than their own would mix up the heads."""
+    raw = bytearray(tree_args(B=2, weights=4096, weights_out=4096, draft_weights=8192))
+    strides = 12 * 8 + (18 + 3) * 8  # weights_stride[2], weights_out_stride[2]
+    raw[strides:strides + 32] = struct.pack("4q", 32, 16, 16, 32)
+    assert _lib.lib().w8_attention_tree(bytes(raw), None, 0, None) == _lib.W8_ERR_INVALID_ARG
+    assert b"other strides" in _lib.lib().w8_last_error()
+    for w_to, p_to in ((16384, 24576), (16384, 40960), (32768, 24576)):
+        evict = EVICT_ARGS.pack(4096, 8192, 16384, 24576, 4096, w_to, p_to, 8192, *[128] * 6, 32, 16, 32, 16, 16, 32, 16, 32,
+                                2, 2, 16, 128, 4, 0, 0)
+        assert _lib.lib().w8_cache_evict(evict, 4096, 1 << 20, None) == _lib.W8_ERR_INVALID_ARG
+        assert b"other strides" in _lib.lib().w8_last_error()
+
+
 def test_empty_attention_is_a_no_op():
     assert _lib.lib().w8_attention_tree(tree_args(B=0), None, 0, None) == _lib.W8_OK
     assert _lib.lib().w8_attention_tree(tree_args(N=0), None, 0, None) == _lib.W8_OK
