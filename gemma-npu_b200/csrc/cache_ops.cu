@@ -124,9 +124,11 @@ struct EvictArgs {
   int kv_heads, slots, budget, sink, recent;
   int* moves;  // per (sequence, head): count, then [most] destinations, then [most] sources
   int most;
+  int cluster;  // CTAs of a row
 };
 
 constexpr int kEvictThreads = 512;
+constexpr int kEvictCluster = 8;  // CTAs of a row at most (portable)
 constexpr int kEvictLongThreads = 1024;
 
 // Exclusive prefix sum of `v` over the block; `total` is the block's sum.
@@ -172,7 +174,7 @@ struct EvictRow {
   int* moves;
   int len, left;
 };
-__device__ __forceinline__ EvictRow evict_row(const EvictArgs& a, int row) {
+__device__ __forceinline__ EvictRow evict_row(const EvictArgs& a, int row, int rank) {
   const int b = row / a.kv_heads, c = row % a.kv_heads;
   EvictRow r;
   r.w = a.w + b * a.w_b + c * a.w_h;
@@ -182,11 +184,11 @@ __device__ __forceinline__ EvictRow evict_row(const EvictArgs& a, int row) {
   r.moves = a.moves + static_cast<int64_t>(row) * (1 + 2 * a.most);
   r.len = a.lens[b];
   if (r.len < 0 || r.len > a.slots) {
-    if (threadIdx.x == 0) cache_bad_index();
+    if (threadIdx.x == 0 && rank == 0) cache_bad_index();
     r.len = r.len < 0 ? 0 : a.slots;
   }
   r.left = min(r.len, a.budget);
-  if (c == 0 && threadIdx.x == 0) a.lens_out[b] = r.left;
+  if (c == 0 && threadIdx.x == 0 && rank == 0) a.lens_out[b] = r.left;
   return r;
 }
 
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(kEvictThreads, KPT <= 32 ? 2 : 1) evict_select
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   pdl_wait();
-  const EvictRow r = evict_row(a, blockIdx.x);
+  const EvictRow r = evict_row(a, blockIdx.x, 0);
   // Nothing behind the last slot: written first, under the loads, unless the row is cut in place.
   auto clear = [&]() {
 #pragma unroll 8
@@ -409,7 +411,228 @@ __global__ void __launch_bounds__(kEvictThreads, KPT <= 32 ? 2 : 1) evict_select
   }
 }
 
-// The same for more slots than registers hold: a radix selection of the budget-th key over four
+// The same for few rows or long ones: a row is held in the registers of a cluster of 2 to 8 CTAs,
+// its slots in chunks of 32 KPT dealt to the CTAs in turn, a warp a chunk.  A barrier of the
+// cluster costs more than a block's, so a step of the search counts the keys at three places
+// between the bounds (every warp writes its counts into all CTAs' shared memory, one barrier a
+// step).  Evicted slots meet their movers through the list that the moves read too, and a
+// slot's weight and position are read by one thread only, so the cut may be in place.  One row
+// of 16001 slots 17 us where one CTA takes 30, of 40000 32 where evict_select_long_kernel takes
+// 115; 144 rows of 16001 slots, which fill the SMs by themselves, 58 and more against 56.
+template <int KPT>
+__global__ void __launch_bounds__(kEvictThreads, KPT <= 16 ? 2 : 1) evict_select_cluster_kernel(const EvictArgs a) {
+  constexpr int kWarps = kEvictThreads / 32, kChunks = kWarps * kEvictCluster;
+  constexpr bool kHeld = KPT <= 8;  // weights and positions too stay in registers
+  __shared__ uint4 counts[2][kChunks];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ctas = a.cluster, rank = static_cast<int>(cluster_ctarank());
+  const int chunks = kWarps * ctas, chunk = warp * ctas + rank;  // (chunks in slot order)
+  pdl_launch_dependents();
+  cluster_sync();  // all CTAs run: their shared memory may be written
+  pdl_wait();
+  const EvictRow r = evict_row(a, blockIdx.x / ctas, rank);
+  if (r.len <= a.budget) {
+    if (rank == 0 && tid == 0) r.moves[0] = 0;
+    const int step = ctas * kEvictThreads;
+    if (r.w_out != r.w || r.pos_out != r.pos) {
+#pragma unroll 4
+      for (int s = rank * kEvictThreads + tid; s < r.len; s += step) {
+        const float ws = r.w[s];
+        const int ps = r.pos[s];
+        r.w_out[s] = ws;
+        r.pos_out[s] = ps;
+      }
+    }
+#pragma unroll 4
+    for (int s = r.len + rank * kEvictThreads + tid; s < a.slots; s += step) {
+      r.w_out[s] = 0.f;
+      r.pos_out[s] = -1;
+    }
+    return;  // (the same for the whole cluster)
+  }
+  // One value of every chunk to all CTAs; `turn` alternates, so that one barrier a step is enough.
+  int turn = 0;
+  auto exchange = [&](uint32_t x, uint32_t y, uint32_t z) {
+    turn ^= 1;
+    if (lane < ctas)
+      asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                       mapa_shared(smem_u32(&counts[turn][chunk]), static_cast<uint32_t>(lane))),
+                   "r"(x), "r"(y), "r"(z), "r"(0u)
+                   : "memory");
+    cluster_sync();
+  };
+  const int first = chunk * 32 * KPT, s0 = first + lane;  // slot of step i: s0 + 32 i
+  uint32_t key[KPT];
+  float wv[kHeld ? KPT : 1];
+  int pv[kHeld ? KPT : 1];
+  int last = INT32_MIN;
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const int s = s0 + 32 * i;
+    const float w = s < r.len ? r.w[s] : 0.f;
+    const int p = s < r.len ? r.pos[s] : INT32_MIN;
+    if constexpr (kHeld) wv[i] = w, pv[i] = p;
+    key[i] = __float_as_uint(w);
+    last = max(last, p);
+  }
+  // The highest position decides what is recent.
+  last = __reduce_max_sync(0xffffffffu, last);
+  exchange(static_cast<uint32_t>(last), 0u, 0u);
+  last = INT32_MIN;
+  for (int i = lane; i < chunks; i += 32) last = max(last, static_cast<int>(counts[turn][i].x));
+  last = __reduce_max_sync(0xffffffffu, last);
+  const int recent_after = evict_recent_after(a, last);
+  uint32_t least = 0xFFFFFFFFu, most = 0u, protect = 0u;  // the bounds of the keys that are not protected
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {  // 0 behind the length: below every slot's
+    const int s = s0 + 32 * i;
+    if (s < r.len) {
+      int p;
+      if constexpr (kHeld)
+        p = pv[i];
+      else
+        p = r.pos[s];
+      key[i] = evict_key(a, __uint_as_float(key[i]), p, recent_after);
+      if (key[i] == 0xFFFFFFFFu)
+        ++protect;
+      else
+        most = max(most, key[i]);
+      least = min(least, key[i]);
+    } else {
+      key[i] = 0u;
+    }
+  }
+  exchange(__reduce_min_sync(0xffffffffu, least), __reduce_max_sync(0xffffffffu, most),
+           __reduce_add_sync(0xffffffffu, protect));
+  least = 0xFFFFFFFFu, most = 0u, protect = 0u;
+  for (int i = lane; i < chunks; i += 32) {
+    const uint4 c = counts[turn][i];
+    least = min(least, c.x), most = max(most, c.y), protect += c.z;
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  const int safe = static_cast<int>(__reduce_add_sync(0xffffffffu, protect));
+  // `reach` keys are >= cut, at least `budget` of them, and fewer are >= over.  The protected
+  // keys (all ones) may fill the budget alone.
+  uint32_t cut = least, over = most + 1;
+  int reach = r.len;
+  if (safe >= a.budget) cut = over = 0xFFFFFFFFu, reach = safe;
+  while (reach != a.budget && over - cut > 1) {
+    const uint32_t width = over - cut, q = max(width / 4, 1u);
+    uint32_t at[3], n[3] = {0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 3; ++j) at[j] = cut + min((j + 1) * q, width);
+    if (first < r.len) {
+#pragma unroll
+      for (int i = 0; i < KPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) n[j] += key[i] >= at[j] ? 1u : 0u;
+      const uint32_t two = __reduce_add_sync(0xffffffffu, n[0] | n[1] << 16);  // (at most 1024 each)
+      n[0] = two & 0xFFFFu, n[1] = two >> 16, n[2] = __reduce_add_sync(0xffffffffu, n[2]);
+    }
+    exchange(n[0], n[1], n[2]);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) n[j] = 0u;
+    for (int i = lane; i < chunks; i += 32) {
+      const uint4 c = counts[turn][i];
+      n[0] += c.x, n[1] += c.y, n[2] += c.z;
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) n[j] = __reduce_add_sync(0xffffffffu, n[j]);
+    uint32_t lo = cut, hi = over;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {  // (counts fall: the places that `budget` keys reach come first)
+      if (static_cast<int>(n[j]) >= a.budget)
+        lo = at[j], reach = static_cast<int>(n[j]);
+      else
+        hi = min(hi, at[j]);
+    }
+    cut = lo, over = hi;
+  }
+  // Of the keys equal to the cut the last reach - budget in slot order go.
+  const bool ties = reach != a.budget;  // (the same for the whole cluster)
+  int room = 0;                         // equal keys that stay, counted from this chunk's first
+  if (ties) {
+    int eq = 0;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) eq += __popc(__ballot_sync(0xffffffffu, key[i] == cut));
+    exchange(static_cast<uint32_t>(eq), 0u, 0u);
+    for (int i = lane; i < chunks; i += 32) {
+      const int c = static_cast<int>(counts[turn][i].x);
+      room += i < chunk ? 0 : c;
+    }
+    room = __reduce_add_sync(0xffffffffu, room) - (reach - a.budget);
+  }
+  const uint32_t before = (1u << lane) - 1u;
+  auto low_bits = [&](int i) {  // step i's slots below the budget
+    const int n = a.budget - (first + 32 * i);
+    return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+  };
+  uint32_t kept = 0;  // lane i: step i's slots that stay
+  int holes = 0, movers = 0;
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    bool stays = key[i] >= cut;
+    if (ties) {
+      const uint32_t eq = __ballot_sync(0xffffffffu, key[i] == cut);
+      stays = key[i] > cut || (key[i] == cut && __popc(eq & before) < room);
+      room -= __popc(eq);
+    }
+    const uint32_t keep = __ballot_sync(0xffffffffu, stays), low = low_bits(i);
+    if (lane == i) kept = keep;
+    holes += __popc(~keep & low);
+    movers += __popc(keep & ~low);
+  }
+  exchange(static_cast<uint32_t>(holes), static_cast<uint32_t>(movers), 0u);
+  int hole_at = 0, mover_at = 0, moved = 0;
+  for (int i = lane; i < chunks; i += 32) {
+    const uint4 c = counts[turn][i];
+    if (i < chunk) hole_at += c.x, mover_at += c.y;
+    moved += c.y;
+  }
+  hole_at = __reduce_add_sync(0xffffffffu, hole_at);
+  mover_at = __reduce_add_sync(0xffffffffu, mover_at);
+  moved = __reduce_add_sync(0xffffffffu, moved);
+  if (rank == 0 && tid == 0) r.moves[0] = moved;
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const uint32_t low = low_bits(i);
+    if (low == 0u) break;
+    const uint32_t h = ~__shfl_sync(0xffffffffu, kept, i) & low;
+    if ((h >> lane) & 1u) r.moves[1 + hole_at + __popc(h & before)] = s0 + 32 * i;
+    hole_at += __popc(h);
+  }
+  cluster_sync();
+  // The small state: each slot's thread puts what it holds where it goes.
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const int s = s0 + 32 * i;
+    const uint32_t keep = __shfl_sync(0xffffffffu, kept, i), low = low_bits(i), m = keep & ~low;
+    if (((keep | ~low) >> lane) & 1u && s < a.slots) {  // (a hole is its mover's to write)
+      const bool stays = (keep >> lane) & 1u;
+      float ws = 0.f;
+      int ps = -1;
+      if (stays) {
+        if constexpr (kHeld)
+          ws = wv[i], ps = pv[i];
+        else
+          ws = r.w[s], ps = r.pos[s];
+      }
+      if ((m >> lane) & 1u) {
+        const int j = mover_at + __popc(m & before), dst = __ldcg(r.moves + 1 + j);
+        r.moves[1 + a.most + j] = s;
+        r.w_out[dst] = ws;
+        r.pos_out[dst] = ps;
+        ws = 0.f, ps = -1;
+      }
+      r.w_out[s] = ws;
+      r.pos_out[s] = ps;
+    }
+    mover_at += __popc(m);
+  }
+}
+
+// The same for more slots than a cluster's registers hold: a radix selection of the budget-th key over four
 // passes of the row, then one in slot order.
 __global__ void __launch_bounds__(kEvictLongThreads) evict_select_long_kernel(const EvictArgs a) {
   __shared__ int hist[256];
@@ -418,7 +641,7 @@ __global__ void __launch_bounds__(kEvictLongThreads) evict_select_long_kernel(co
   const int tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
-  const EvictRow r = evict_row(a, blockIdx.x);
+  const EvictRow r = evict_row(a, blockIdx.x, 0);
   const float* w = r.w;
   const int* pos = r.pos;
   int* moves = r.moves;
@@ -644,6 +867,23 @@ static int launch_evict(dim3 grid, int lists, int device, cudaStream_t stream, c
   return launch_cache(w8::evict_select_kernel<KPT>, grid, w8::kEvictThreads, stream, e, lists);
 }
 
+template <int KPT>
+static int launch_evict_cluster(int64_t rows, cudaStream_t stream, const w8::EvictArgs& e) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * e.cluster));
+  cfg.blockDim = dim3(w8::kEvictThreads, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(e.cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cuda_status(cudaLaunchKernelEx(&cfg, w8::evict_select_cluster_kernel<KPT>, e));
+}
+
 // Read (and optionally clear) the sticky device status of the cache operations.
 int cache_device_status(int clear, int* out) {
   int v = 0;
@@ -771,20 +1011,27 @@ extern "C" int w8_cache_evict(const w8_cache_evict_args* in, void* workspace, in
   e.budget = static_cast<int>(std::min(x.budget, x.slots)), e.sink = static_cast<int>(x.sink);
   e.recent = static_cast<int>(x.recent);
   e.moves = static_cast<int*>(workspace), e.most = static_cast<int>(most);
-  // Keys in registers up to 32768 slots: the fewest that cover the row (3658 slots: 8 a thread).
+  // Keys in registers, the fewest a thread that cover the row: up to 32768 slots of one CTA, up to
+  // 131072 of a cluster, which takes rows above 8192 slots too while all their CTAs have an SM
+  // of their own (the kernel's comment has both sides).
+  e.cluster = 1;
+  while (e.cluster < w8::kEvictCluster && (x.slots > (e.cluster == 1 ? 32768 : 16384 * e.cluster) ||
+                                           (x.slots > 8192 && rows * e.cluster * 2 <= sms)))
+    e.cluster *= 2;
+  const int64_t per = (x.slots + w8::kEvictThreads * e.cluster - 1) / (w8::kEvictThreads * e.cluster);
   const dim3 each(static_cast<unsigned>(rows));
-  const int64_t per = (x.slots + w8::kEvictThreads - 1) / w8::kEvictThreads;
   const int lists = static_cast<int>(std::min<int64_t>(2 * (most + e.budget) + 4, 100 * 1024));
-  if (per <= 8)
-    st = launch_evict<8>(each, lists, device, s, e);
-  else if (per <= 16)
-    st = launch_evict<16>(each, lists, device, s, e);
-  else if (per <= 32)
-    st = launch_evict<32>(each, lists, device, s, e);
-  else if (per <= 64)
-    st = launch_evict<64>(each, lists, device, s, e);
+  if (e.cluster > 1)
+    st = per <= 4    ? launch_evict_cluster<4>(rows, s, e)
+         : per <= 8  ? launch_evict_cluster<8>(rows, s, e)
+         : per <= 16 ? launch_evict_cluster<16>(rows, s, e)
+         : per <= 32 ? launch_evict_cluster<32>(rows, s, e)
+                     : launch_cache(w8::evict_select_long_kernel, each, w8::kEvictLongThreads, s, e);
   else
-    st = launch_cache(w8::evict_select_long_kernel, each, w8::kEvictLongThreads, s, e);
+    st = per <= 8    ? launch_evict<8>(each, lists, device, s, e)
+         : per <= 16 ? launch_evict<16>(each, lists, device, s, e)
+         : per <= 32 ? launch_evict<32>(each, lists, device, s, e)
+                     : launch_evict<64>(each, lists, device, s, e);
   if (st != W8_OK || most == 0) return st;
   w8::MoveArgs m = {};
   m.k = static_cast<uint8_t*>(x.k), m.v = static_cast<uint8_t*>(x.v);

@@ -395,6 +395,13 @@ EVICTS = [(1, 1, 64, 10, [10], 4, 0, 0), (3, 2, 128, 700, [700, 100, 0], 100, 4,
           (1, 1, 64, 40, [33], 60, 0, 0), (1, 1, 512, 33000, [33000], 5000, 8, 100), (2, 1, 64, 5000, [5000, 4097], 4096, 0, 4096)]
 
 
+# Rows above 8192 slots, few and many, up to and beyond what a cluster's registers hold.
+EVICTS += [(1, 1, 64, 8193, [8193], 1000, 4, 100), (1, 3, 64, 16500, [16385], 12000, 0, 11000), (9, 1, 64, 9000, [9000, 0, 500, 8999, 1, 501, 499, 4096, 8193], 500, 4, 20),
+           (30, 1, 64, 8200, [8200 - 250 * i for i in range(30)], 700, 4, 20), (40, 2, 64, 9000, [9000 - 200 * i for i in range(40)], 700, 4, 20),
+           (2, 1, 64, 32769, [32769, 20000], 20000, 4, 20), (1, 1, 64, 70000, [69990], 3000, 4, 100), (1, 1, 64, 131072, [131072], 65536, 1, 1),
+           (1, 1, 64, 131100, [131100], 4000, 1, 1), (1, 1, 64, 100000, [100000], 99999, 50000, 49999), (1, 1, 64, 40000, [3000], 3000, 0, 0)]
+
+
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("kind", ["random", "ties", "odd"])
 @pytest.mark.parametrize("shape", EVICTS, ids=[str(i) for i in range(len(EVICTS))])
