@@ -84,8 +84,8 @@ struct TreeCfg {
   static constexpr int kSteps = D == 64 ? 2 : 1;            // 16-key steps of a warp in a tile
   static constexpr int kBN = kGroups * kSteps * 16;         // keys per tile: 256, 128, 128, 64
   static constexpr int kSlotBytes = kBN * D * 2;            // 32 KB (D <= 128) or 64 KB
-  static constexpr int kPerSm = D == 64 ? 2 : 1;            // CTAs per SM
-  static constexpr int kSlots = D == 128 ? 6 : 3;
+  static constexpr int kPerSm = D == 64 && MT == 1 ? 2 : 1; // CTAs per SM (two of 32 rows would spill)
+  static constexpr int kSlots = kSlotBytes > 32768 ? 3 : 6 / kPerSm;
   // Ring steps loaded ahead.  A slot freed one step ago may still be held by a slow warp, whose
   // turn to load it then waits: with small boxes two steps' grace is worth more than the fifth box.
   static constexpr int kAhead = kSlots == 6 ? 4 : 2;
@@ -892,12 +892,14 @@ struct TreePlan {
 
 // The tcgen05 schedule takes 256 rows a tile and keeps up with HBM for any number of them, so
 // it is for more rows a cache head than one mma.sync tile has (`tma`: its maps can describe
-// the tensors): with 16 or 32 rows, mma.sync tiles spread a sequence's keys over all SMs.
+// the tensors): with 16 or 32 rows, mma.sync tiles spread a sequence's keys over all SMs.  At
+// D 64, which it runs as 128, two mma.sync tiles are still better (256 cache heads of 4000 keys:
+// 32 rows 80 us against 241, 64 rows 150 against 237; four would take 300).
 static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t n, int64_t d, int64_t slots,
                           int64_t window, int sms, bool tma) {
   TreePlan p;
   const int64_t rows = group * n;
-  p.tc = tma && d >= 128 && rows > (d == 128 ? 32 : 16);
+  p.tc = tma && rows > (d == 64 ? 64 : d == 128 ? 32 : 16);
   p.bm = p.tc ? 256 : rows > 16 && d <= 128 ? 32 : 16;
   p.row_tiles = static_cast<int>((rows + p.bm - 1) / p.bm);
   p.items = batch * kv_heads * p.row_tiles;
@@ -925,12 +927,12 @@ static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_
     // An item per CTA, or all tiles dealt evenly: by estimated times.  A tile is about 1 us (2 us
     // of 64 KB boxes), an item's start and end 3 us, joining the pieces a launch of 4 us.  From 8
     // items an SM on ragged lengths even out by themselves.
-    const double tile_us = d >= 256 ? 2.0 : 1.0;
+    const double tile_us = d >= 256 || (d == 64 && p.bm == 32) ? 2.0 : 1.0;
     const double waves = static_cast<double>((p.items + sms - 1) / std::max(sms, 1));
     const double alone = waves * (static_cast<double>(tiles) * tile_us + 3);
     const double dealt = static_cast<double>(p.items) * static_cast<double>(tiles) / sms * tile_us + 3 * (waves + 1) + 4;
     p.direct = alone <= dealt || p.items >= 8 * static_cast<int64_t>(sms);
-    p.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms * (d == 64 ? 2 : 1), p.items * tiles, w8::kTreeMaxPieces})));  // TreeCfg::kPerSm
+    p.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms * (d == 64 && p.bm == 16 ? 2 : 1), p.items * tiles, w8::kTreeMaxPieces})));  // TreeCfg::kPerSm
   }
   return p;
 }

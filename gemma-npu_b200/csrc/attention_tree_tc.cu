@@ -69,7 +69,10 @@ __device__ __forceinline__ void red_or_cluster(uint32_t addr, uint32_t bits) {
   asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(bits) : "memory");
 }
 
-template <typename T, int D>
+// DR: columns of a head in memory.  Heads of 64 run as 128 whose upper half the boxes fill with
+// zeros (S and O do not change, and only the lower half is stored): the MMAs do twice their work
+// and 216 row tiles of 680 rows over 1085 keys take 194 us where mma.sync took 626.
+template <typename T, int D, int DR>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v,
@@ -304,7 +307,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
           int i, g;
           tree_row(a, qr, i, g);
           w[x] = make_uint4(0, 0, 0, 0);
-          if (qr < rows)
+          if (qr < rows && ch < DR / 8)
             w[x] = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + g) * a.q_h +
                                                    i * a.q_t + ch * 8);
         }
@@ -497,7 +500,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         const int col = (C::kDV / 2) * hv + e * 32;  // of this half
         tmem_ld_32x32b_x32(tmem + lane_off + kTtColO + col, ov);
         tmem_wait_ld();
-        if (poisoned) {
+        if (poisoned && col < DR) {
 #pragma unroll 1
           for (int j0 = j_begin; j0 < j_end; j0 += 32) {
             uint32_t bits = poison_of(poison, j0);
@@ -543,9 +546,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         void* dst = a.splits == 1
                         ? static_cast<void*>(a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + head) * a.o_h + tok * a.o_t +
                                              half * C::kDV)
-                        : static_cast<void*>(a.part_o + (part_row + r) * D + half * C::kDV);
+                        : static_cast<void*>(a.part_o + (part_row + r) * DR + half * C::kDV);
         asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(base + r * pitch),
-                     "r"(C::kDV * esz)
+                     "r"((DR < C::kDV ? DR : C::kDV) * esz)
                      : "memory");
         bulk_commit_group();
         bulk_wait_group_read<0>();  // (the grid's completion covers the writes)
@@ -591,7 +594,7 @@ static TreeEncodeFn tree_encode_fn() {
 
 // 5-D map over rows [batch, heads, n] of d elements: (64 columns, row, 64-column block, head,
 // batch).  A box {64, rows, blocks, 1, 1} lands as `blocks` 128-byte-swizzled [rows x 64]
-// blocks; rows behind n read as zeros.
+// blocks; rows behind n and blocks behind d / 64 read as zeros.
 int tree_encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, int64_t n, int64_t heads, int64_t batch,
                        int64_t s_b, int64_t s_h, int64_t s_n, uint32_t rows, uint32_t blocks) {
   TreeEncodeFn enc = tree_encode_fn();
@@ -618,8 +621,9 @@ int tree_encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, in
 }
 
 // 5-D map over q: (64 columns, head, token, 64-column block, batch).  A box {64, group,
-// 128 / group, d / 64, 1} lands as d / 64 swizzled blocks of 128 rows i * group + g.
-static int encode_q(CUtensorMap* map, const w8::TreeArgs& a, bool half, int64_t d) {
+// 128 / group, blocks, 1} lands as `blocks` swizzled blocks of 128 rows i * group + g, zeros
+// behind the d / 64-th.
+static int encode_q(CUtensorMap* map, const w8::TreeArgs& a, bool half, int64_t d, uint32_t blocks) {
   TreeEncodeFn enc = tree_encode_fn();
   if (enc == nullptr) {
     set_error("cuTensorMapEncodeTiled is not available from the driver");
@@ -631,7 +635,7 @@ static int encode_q(CUtensorMap* map, const w8::TreeArgs& a, bool half, int64_t 
                               static_cast<cuuint64_t>(d / 64), static_cast<cuuint64_t>(a.batch)};
   const cuuint64_t strides[4] = {bytes(heads, a.q_h), bytes(a.n, a.q_t), 128, bytes(a.batch, a.q_b)};
   const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(w8::kTtBM / a.group),
-                             static_cast<cuuint32_t>(d / 64), 1};
+                             blocks, 1};
   const cuuint32_t one[5] = {1, 1, 1, 1, 1};
   const CUresult r = enc(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                          const_cast<uint16_t*>(a.q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -644,31 +648,31 @@ static int encode_q(CUtensorMap* map, const w8::TreeArgs& a, bool half, int64_t 
   return W8_OK;
 }
 
-template <typename T, int D>
+template <typename T, int D, int DR = D>
 static int tree_tc_go(const w8::TreeArgs& a, int64_t items, int device, cudaStream_t stream) {
   using C = w8::TtCfg<D>;
   constexpr bool kHalf = __is_same(T, __half);
   CUtensorMap tq, tk, tv, tkn, tvn;
   const uint32_t kb = C::kKCols / 64, vb = C::kDV / 128;
-  int st = tree_encode_rows(&tkn, a.kn, kHalf, D, a.n, a.kv_heads, a.batch, a.kn_b, a.kn_h, a.kn_t, w8::kTtKeysPerCta, kb);
+  int st = tree_encode_rows(&tkn, a.kn, kHalf, DR, a.n, a.kv_heads, a.batch, a.kn_b, a.kn_h, a.kn_t, w8::kTtKeysPerCta, kb);
   if (st != W8_OK) return st;
-  st = tree_encode_rows(&tvn, a.vn, kHalf, D, a.n, a.kv_heads, a.batch, a.vn_b, a.vn_h, a.vn_t, w8::kTtBN, vb);
+  st = tree_encode_rows(&tvn, a.vn, kHalf, DR, a.n, a.kv_heads, a.batch, a.vn_b, a.vn_h, a.vn_t, w8::kTtBN, vb);
   if (st != W8_OK) return st;
   tk = tkn, tv = tvn;  // an empty cache: never read
   if (a.slots > 0) {
-    st = tree_encode_rows(&tk, a.k, kHalf, D, a.slots, a.kv_heads, a.batch, a.k_b, a.k_h, a.k_s, w8::kTtKeysPerCta, kb);
+    st = tree_encode_rows(&tk, a.k, kHalf, DR, a.slots, a.kv_heads, a.batch, a.k_b, a.k_h, a.k_s, w8::kTtKeysPerCta, kb);
     if (st != W8_OK) return st;
-    st = tree_encode_rows(&tv, a.v, kHalf, D, a.slots, a.kv_heads, a.batch, a.v_b, a.v_h, a.v_s, w8::kTtBN, vb);
+    st = tree_encode_rows(&tv, a.v, kHalf, DR, a.slots, a.kv_heads, a.batch, a.v_b, a.v_h, a.v_s, w8::kTtBN, vb);
     if (st != W8_OK) return st;
   }
   tq = tkn;
   if (a.q_tma) {
-    st = encode_q(&tq, a, kHalf, D);
+    st = encode_q(&tq, a, kHalf, DR, D / 64);
     if (st != W8_OK) return st;
   }
   static bool done[64] = {};
   if (!done[device]) {
-    W8_CUDA_TRY(cudaFuncSetAttribute(w8::attn_tree_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    W8_CUDA_TRY(cudaFuncSetAttribute(w8::attn_tree_tc_kernel<T, D, DR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      C::kSmem));
     done[device] = true;
   }
@@ -684,12 +688,15 @@ static int tree_tc_go(const w8::TreeArgs& a, int64_t items, int device, cudaStre
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, w8::attn_tree_tc_kernel<T, D>, tq, tk, tv, tkn, tvn, a));
+  return cuda_status(cudaLaunchKernelEx(&cfg, w8::attn_tree_tc_kernel<T, D, DR>, tq, tk, tv, tkn, tvn, a));
 }
 
 // The tcgen05 schedule of w8_attention_tree (arguments checked by the caller; rows in tiles of
 // 256).
 int tree_tc(const w8::TreeArgs& a, bool half, int64_t d, int64_t items, int device, cudaStream_t stream) {
+  if (d == 64)
+    return half ? tree_tc_go<__half, 128, 64>(a, items, device, stream)
+                : tree_tc_go<__nv_bfloat16, 128, 64>(a, items, device, stream);
   if (d == 128)
     return half ? tree_tc_go<__half, 128>(a, items, device, stream) : tree_tc_go<__nv_bfloat16, 128>(a, items, device, stream);
   if (d == 256)

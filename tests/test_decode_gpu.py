@@ -130,6 +130,13 @@ SHAPES = [
     (300, 4, 2, 128, 1, 300, [(37 * i) % 301 for i in range(300)], 100),
     (1, 8, 1, 256, 64, 0, [0], 0),
     (1, 16, 1, 512, 3, 0, [0], 2),
+    # heads of 64 of many rows: whole and odd groups, splits, windows, an empty cache
+    (2, 8, 1, 64, 300, 600, [600, 0], 512),
+    (1, 6, 2, 64, 50, 3000, [2900], 0),
+    (9, 16, 2, 64, 40, 300, [300, 0, 1, 127, 128, 129, 255, 256, 257], 50),
+    (1, 33, 1, 64, 1, 700, [650], 0),
+    (1, 8, 8, 64, 130, 0, [0], 0),
+    (40, 32, 1, 64, 1, 300, [(13 * i) % 301 for i in range(40)], 0),
 ]
 
 
@@ -151,6 +158,9 @@ TREES = [
     (2, 8, 1, 256, 64, 400, [400, 31], 100, 4),
     (1, 4, 4, 128, 130, 90, [90], 3, 1),
     (2, 16, 2, 256, 64, 700, [700, 640], 0, 4),
+    (2, 16, 2, 64, 64, 700, [700, 640], 0, 4),
+    (2, 6, 2, 64, 45, 300, [300, 0], 100, 5),
+    (1, 4, 4, 64, 130, 90, [90], 3, 1),
 ]
 
 
