@@ -811,18 +811,24 @@ __global__ void __launch_bounds__(256) attn_tree_combine_rows_kernel(const TreeA
 }
 
 // Accumulated weights: slot j gets weights[j] + sum over the R rows of p_rj, p from the stored
-// scores and the rows' log-sum-exp (the sums in the rows' order: the same bits every time).
-// Four slots a thread, 16-byte loads of four rows in flight: bound by reading the scores.
+// scores and the rows' log-sum-exp (summed in a fixed order: the same bits every time).  Four
+// slots a thread, 16-byte loads of several rows in flight: bound by reading the scores.  Many
+// rows are dealt to SPLIT groups of threads, joined at the end: one thread that walks 968 rows
+// waits 280 us for its loads (1 cache head, 131 slots), eight 39.
+template <int SPLIT>  // 1, or 8: a warp each
 __global__ void __launch_bounds__(256) attn_tree_weights_kernel(const TreeArgs a) {
+  constexpr int kThreads = 256 / SPLIT, kSlots = 4 * kThreads;  // of a group; slots of a CTA
   __shared__ float sm_lse[256];
   __shared__ int sm_first[256];
+  __shared__ float4 sm_sum[SPLIT][SPLIT > 1 ? kThreads : 1];
+  const int part = SPLIT > 1 ? threadIdx.x / kThreads : 0, at = threadIdx.x % kThreads;
   const int rows = a.group * a.n, bc = blockIdx.y, b = bc / a.kv_heads, c = bc % a.kv_heads;
   pdl_launch_dependents();
   pdl_wait();
   const int len = tree_len(a, b);
-  const int j0 = (blockIdx.x * 256 + threadIdx.x) * 4;  // slots [0, draft_at), then new tokens
-  const int begin = blockIdx.x * 1024;
-  if (begin >= len && begin + 1024 <= a.draft_at) return;
+  const int begin = blockIdx.x * kSlots;
+  const int j0 = begin + at * 4;  // slots [0, draft_at), then new tokens
+  if (begin >= len && begin + kSlots <= a.draft_at) return;
   const bool draft = j0 >= a.draft_at;
   const int end = draft ? a.draft_at + a.n : len;
   const float* x = a.scores + static_cast<int64_t>(bc) * rows * a.score_pitch + j0;
@@ -839,8 +845,8 @@ __global__ void __launch_bounds__(256) attn_tree_weights_kernel(const TreeArgs a
     __syncthreads();
     if (j0 < end) {
       const int n = min(256, rows - r0);
-#pragma unroll 4
-      for (int q = 0; q < n; ++q) {
+#pragma unroll SPLIT == 1 ? 4 : 8
+      for (int q = part; q < n; q += SPLIT) {
         const float4 v = *reinterpret_cast<const float4*>(x + static_cast<int64_t>(r0 + q) * a.score_pitch);
         const float e[4] = {v.x, v.y, v.z, v.w};
         // Of this thread's four, [lo, hi) were scored: no tile of the row covers slots before the
@@ -857,6 +863,16 @@ __global__ void __launch_bounds__(256) attn_tree_weights_kernel(const TreeArgs a
         for (int k = 0; k < 4; ++k)
           if (k >= lo && k < hi) sum[k] += ex2_tree(e[k] - sm_lse[q]);
       }
+    }
+  }
+  if constexpr (SPLIT > 1) {
+    sm_sum[part][at] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int s = 1; s < SPLIT; ++s) {
+      const float4 v = sm_sum[s][at];
+      sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
     }
   }
 #pragma unroll
@@ -1047,10 +1063,11 @@ static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStr
     if (st != W8_OK) return st;
   }
   if (a.scores != nullptr) {
-    const int64_t blocks_w = (a.score_pitch + 1023) / 1024;
-    st = launch_tree(w8::attn_tree_weights_kernel,
-                     dim3(static_cast<unsigned>(blocks_w), static_cast<unsigned>(a.batch * a.kv_heads)), 256, 0, stream,
-                     a);
+    const bool split = a.group * a.n > 16;  // (16 rows are four rounds of loads)
+    const int64_t slots = split ? 128 : 1024;
+    const dim3 grid(static_cast<unsigned>((a.score_pitch + slots - 1) / slots), static_cast<unsigned>(a.batch * a.kv_heads));
+    st = split ? launch_tree(w8::attn_tree_weights_kernel<8>, grid, 256, 0, stream, a)
+               : launch_tree(w8::attn_tree_weights_kernel<1>, grid, 256, 0, stream, a);
   }
   return st;
 }

@@ -380,9 +380,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         if (a.scores != nullptr && half == 0 && tok >= 0) {
           float* dst = a.scores + (static_cast<int64_t>(bc) * rows + rr) * a.score_pitch + (draft ? a.draft_at : 0) + k0;
           const int left = (draft ? a.n : len) - k0;
+          // (16 bytes at a time: the row's two parts begin and end on multiples of 4 slots, so the last
+          // store passes its end by up to 3 slots that nothing reads.)
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (e < left) dst[e] = __uint_as_float(sv[e >> 5][e & 31]) * scale;
+          for (int e = 0; e < 64; e += 4)
+            if (e < left)
+              *reinterpret_cast<float4*>(dst + e) =
+                  make_float4(__uint_as_float(sv[e >> 5][e & 31]) * scale, __uint_as_float(sv[e >> 5][(e + 1) & 31]) * scale,
+                              __uint_as_float(sv[e >> 5][(e + 2) & 31]) * scale,
+                              __uint_as_float(sv[e >> 5][(e + 3) & 31]) * scale);
         }
       }
       __syncwarp();

@@ -255,6 +255,11 @@ WEIGHTS = [
     (2, 8, 1, 256, 40, 200, [200, 0], 0, True),
     (1, 8, 1, 512, 10, 150, [149], 60, True),
     (24, 32, 8, 128, 1, 500, [20 * i + 7 for i in range(24)], 0, False),
+    # many rows
+    (2, 16, 2, 64, 121, 14, [14, 3], 0, True),
+    (1, 8, 1, 128, 90, 1100, [1030], 300, False),
+    (2, 17, 1, 64, 1, 600, [600, 129], 0, False),
+    (2, 8, 1, 256, 35, 260, [255, 0], 64, True),
 ]
 
 
