@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(kBeamThreads, beam_per_sm(sizeof(T))) beam_chu
       }
     }
   };
+  int held = 0;  // candidates kept so far: `count` between two collections, the same in every thread
   uint4 next[GROUPS];
   load(begin, next);
   for (int s0 = begin; s0 < end; s0 += kBeamSuper * kBeamTile) {
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(kBeamThreads, beam_per_sm(sizeof(T))) beam_chu
           if (p < kBeamSegs) segs[p] = j * kBeamThreads + tid;
         }
     __syncthreads();
-    const int held = count;  // of the collections before
+    // Which branch is taken must not depend on `count`: a fast warp adds to it at once in the first.
     const int found = seg_count;
     if (found <= kBeamSegs && held + found * kBeamVals <= kBeamCap) {
       for (int e = tid; e < found * kBeamVals; e += kBeamThreads) {
@@ -344,7 +345,8 @@ __global__ void __launch_bounds__(kBeamThreads, beam_per_sm(sizeof(T))) beam_chu
       const int c = count;
       beam_prune(cand, c, a.n);
       if (c >= a.n) thr = cand[a.n - 1];
-      if (tid == 0) count = min(c, a.n);
+      held = min(c, a.n);
+      if (tid == 0) count = held;
       __syncthreads();
     } else {
       // Too many segments reach the value (ties): tile by tile in the tokens' order, pruning as
@@ -382,16 +384,16 @@ __global__ void __launch_bounds__(kBeamThreads, beam_per_sm(sizeof(T))) beam_chu
           const int c = min(count, kBeamCap);
           beam_prune(cand, c, a.n);
           if (c >= a.n) thr = cand[a.n - 1];
-          if (tid == 0) count = min(c, a.n);
+          held = min(c, a.n);
+          if (tid == 0) count = held;
           __syncthreads();
         }
       }
     }
   }
   // ---- the chunk's sorted list and its sum
-  const int c = count;
   unsigned long long* out = a.keys + (static_cast<int64_t>(row) * a.chunks + blockIdx.x) * a.n;
-  for (int i = tid; i < a.n; i += kBeamThreads) out[i] = i < c ? cand[i] : 0ull;  // 0: none (below every key)
+  for (int i = tid; i < a.n; i += kBeamThreads) out[i] = i < held ? cand[i] : 0ull;  // 0: none (below every key)
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
     const float om = __shfl_xor_sync(0xffffffffu, mx, d), os = __shfl_xor_sync(0xffffffffu, sum, d);

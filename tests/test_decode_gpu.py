@@ -554,6 +554,26 @@ def test_select_strided_and_unaligned_rows(cuda):
     check_select(got, want_select(logits, scores, None, 0, 3, 0.0, "score"), 24.0, 1001, 0.0)
 
 
+@pytest.mark.parametrize("n", [2, 64])
+@pytest.mark.parametrize("found", [64, 100, 121, 125, 126, 127, 128, 129, 200])
+def test_select_segments_that_nearly_fill_the_candidates(cuda, found, n):
+    """The best value in `found` segments of 16 logits (their first one, or all of them): as many
+    candidates as are held at once, one segment less or more, while the collection adds to their number."""
+    B, V = 6, 4096
+    gen = torch.Generator(device="cuda").manual_seed(found)
+    logits = -torch.rand((B, 1, V), generator=gen, device="cuda") - 1
+    for b in range(B):
+        at = torch.randperm(V // 16, generator=gen, device="cuda")[:found]
+        if b % 2:
+            logits[b].view(-1, 16)[at] = 2.0
+        else:
+            logits[b].view(-1, 16)[at, 0] = 2.0
+    scores = torch.linspace(-1, -1.5, B, device="cuda")[:, None].contiguous()
+    for _ in range(20):
+        got = w8.beam_select(logits, scores, n=n)
+    check_select(got, want_select(logits, scores, None, 0, n, 0.0, "score"), 2.0, V, 0.0)
+
+
 REORDERS = [(1, 4, 1, 256, 100, 3), (2, 3, 2, 64, 33, 1), (3, 8, 2, 128, 64, 5), (1, 32, 1, 64, 17, 2), (2, 16, 3, 64, 50, 70), (4, 1, 1, 64, 5, 1)]
 
 
