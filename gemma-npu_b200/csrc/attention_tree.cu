@@ -575,6 +575,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
             mma16816<T>(o[mt][n + 1], pa[mt], vb[2], vb[3]);
           }
         }
+        const bool any_bad = bad != 0u;
 #pragma unroll 1
         for (; bad != 0u; bad &= bad - 1u) {
           const int j = key0 + __ffs(bad) - 1;
@@ -598,6 +599,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
               }
             }
         }
+        if (any_bad) __syncwarp();  // (the next step's loads are aligned)
       }
       if (!ok) break;
       __syncwarp();

@@ -468,6 +468,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
           }
           fence_proxy_async_smem();
         }
+        __syncwarp();  // (the wait below is aligned)
       }
       tmem_wait_st();
       tc_fence_before();

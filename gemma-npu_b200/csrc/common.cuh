@@ -257,8 +257,10 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-// All threads of both CTAs: release our writes, wait for the peer's.
+// All threads of every CTA of the cluster: release our writes, wait for the others'.  The aligned
+// barrier wants the warp converged, which no caller's divergent code before it ensures.
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }

@@ -80,6 +80,22 @@ def test_struct_sizes_match_the_header():
         assert packed.size == 8 * fields, name
 
 
+def test_cluster_barriers_find_their_warps_converged():
+    """`barrier.cluster.*.aligned` needs every thread of the warp at it: the one place that issues it
+    converges the warp first."""
+    import glob
+    import os
+
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    for path in glob.glob(os.path.join(csrc, "*.cu*")):
+        text = open(path).read()
+        if os.path.basename(path) == "common.cuh":
+            body = text.split("void cluster_sync() {", 1)[1].split("}", 1)[0]
+            assert body.index("__syncwarp();") < body.index("barrier.cluster.arrive")
+            text = text.replace(body, "")
+        assert "barrier.cluster." not in text, path
+
+
 def test_evict_refuses():
     def args(budget=4, sink=0, recent=0, lens=4096, lens_out=8192, row=128):
         return EVICT_ARGS.pack(4096, 4096, 4096, 4096, lens, 4096, 4096, lens_out, *[128] * 6, *[16] * 8, 1, 1, 16, row,

@@ -235,6 +235,27 @@ def test_infinite_values_stay_with_those_who_see_them(cuda, D, dt):
     assert got[0, :, 35:, 7].isnan().all() and got[1, :, 20:].isnan().all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_infinite_values_in_every_step_of_a_tile(cuda, D):
+    """One non-finite value in each 16 new tokens of a warp's, few rows (mma.sync) of a tree in which
+    half of the drafts see it: what follows in the same tile is computed as ever."""
+    B, H, KV, N, S = 1, 1, 1, 16, 5
+    q, k, v, ln, kn, vn = make(D, B, H, KV, D, 33 if D == 64 else N, S, [5])
+    N = q.shape[2]
+    tree = torch.ones((N, N), dtype=torch.bool, device="cuda").tril()
+    tree[1::2, 0::16] = False
+    tree.fill_diagonal_(True)
+    clean = vn.clone()
+    vn[0, 0, 0::16, 3] = math.inf
+    clean[0, 0, 0::16, 3] = 0
+    got = w8.attention_tree(q, k, v, ln, kn, vn, tree=tree, scale=D ** -0.5)
+    want = want_attention(q, k, v, ln, kn, clean, tree, None, 0, D ** -0.5)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[0, 0, :, 3] = tree[:, 0::16].any(1)
+    check_out(torch.where(bad, want[0].to(got.dtype), got), want, torch.bfloat16)
+    assert (got[bad] == math.inf).all()
+
+
 @pytest.mark.parametrize("N", [1, 40])
 @pytest.mark.parametrize("D", [64, 128, 256, 512])
 def test_slots_before_the_window_may_hold_anything(cuda, D, N):
