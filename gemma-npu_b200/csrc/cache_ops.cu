@@ -905,6 +905,13 @@ static int cache_shape(int64_t batch, int64_t kv_heads, int64_t slots, int64_t r
   return W8_OK;
 }
 
+// Whether two int32 arrays share memory (what one CTA writes of one, another may yet have to read
+// of the other).
+static bool arrays_meet(const int32_t* p, int64_t n, const int32_t* q, int64_t m) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return p != nullptr && q != nullptr && a < b + 4 * static_cast<uintptr_t>(m) && b < a + 4 * static_cast<uintptr_t>(n);
+}
+
 static int cache_rows(const char* name, const void* p, const int64_t* strides) {
   W8_CHECK_ARG(p != nullptr, "%s is null", name);
   W8_CHECK_ALIGN(aligned(p, 16), "%s must be 16-byte aligned", name);
@@ -925,8 +932,13 @@ extern "C" int w8_cache_append(const w8_cache_append_args* in, w8_stream_t strea
   W8_CHECK_ARG(x.path != nullptr || x.steps == x.n_new, "without a path every new token is appended (steps = n_new)");
   if (x.batch == 0) return W8_OK;
   W8_CHECK_ARG(x.lens && x.lens_out, "null lens");
-  W8_CHECK_ARG(x.lens != x.lens_out, "lens_out must not be lens");
+  W8_CHECK_ARG(!arrays_meet(x.lens, x.batch, x.lens_out, x.batch), "lens_out must not be lens nor overlap it");
   W8_CHECK_ARG(!x.positions || x.seen, "positions need seen");
+  W8_CHECK_ARG(!x.positions || !arrays_meet(x.seen, x.batch, x.lens_out, x.batch),
+               "lens_out must not be seen nor overlap it");
+  if (x.path && x.steps > 0 && arrays_meet(x.path, (x.batch - 1) * x.path_stride + x.steps, x.lens_out, x.batch))
+    for (int64_t b = 0; b < x.batch; ++b)  // (it may lie between the rows)
+      W8_CHECK_ARG(!arrays_meet(x.path + b * x.path_stride, x.steps, x.lens_out, x.batch), "lens_out must not overlap path");
   W8_CHECK_ARG(!x.draft_weights || x.weights, "draft_weights need weights");
   if (x.slots > 0 && x.n_new > 0) {
     if ((st = cache_rows("k", x.k, x.k_stride)) != W8_OK) return st;
@@ -977,7 +989,7 @@ extern "C" int w8_cache_evict(const w8_cache_evict_args* in, void* workspace, in
   W8_CHECK_ARG(x.batch * x.kv_heads <= 65535, "batch * kv_heads beyond 65535");
   if (x.batch == 0) return W8_OK;
   W8_CHECK_ARG(x.lens && x.lens_out, "null lens");
-  W8_CHECK_ARG(x.lens != x.lens_out, "lens_out must not be lens");
+  W8_CHECK_ARG(!arrays_meet(x.lens, x.batch, x.lens_out, x.batch), "lens_out must not be lens nor overlap it");
   if (x.slots > 0) {
     W8_CHECK_ARG(x.weights && x.positions && x.weights_out && x.positions_out, "null weights or positions");
     // In place only with the same layout: rows of one would be other rows of the other.

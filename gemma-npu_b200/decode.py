@@ -99,7 +99,8 @@ def cache_append(k, v, k_new, v_new, lens, path=None, weights=None, draft_weight
     (None: all N tokens in order).  With `weights` fp32 [B, KV, S] the slots take their
     weight from draft_weights [B, KV, N] (None: 0), with `positions` int32 [B, KV, S] the
     positions seen[b], seen[b] + 1, ... (seen int32 [B]: the tokens so far, evicted ones
-    included).  Returns lens_out int32 [B] (not `lens` itself)."""
+    included).  Returns lens_out int32 [B] (a tensor apart from lens, seen and path).  k_new and
+    v_new must not overlap the caches."""
     return (_binding or _c()).cache_append(k, v, k_new, v_new, lens, path, weights, draft_weights, positions, seen,
                                            lens_out)
 
@@ -118,7 +119,7 @@ def cache_evict(k, v, weights, positions, lens, budget, sink=0, recent=0, weight
     order of a cache's slots means nothing to attention without a window, and positions_out
     says which token stands where.  weights_out and positions_out (new tensors unless given;
     the inputs themselves are allowed) hold 0 and -1 behind the last slot; lens_out =
-    min(lens, budget) is not `lens` itself."""
+    min(lens, budget) is a tensor apart from lens."""
     return (_binding or _c()).cache_evict(k, v, weights, positions, lens, budget, sink, recent, weights_out,
                                           positions_out, lens_out)
 

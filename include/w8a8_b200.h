@@ -342,7 +342,7 @@ typedef struct w8_cache_append_args {
   const float* draft_weights;  /* [batch, kv_heads, n_new] or NULL (new slots then start at 0) */
   int32_t* positions;          /* [batch, kv_heads, slots] or NULL */
   const int32_t* seen;         /* [batch]: position of the first appended token (with positions) */
-  int32_t* lens_out;           /* [batch], not lens itself */
+  int32_t* lens_out;           /* [batch], of no memory in common with lens, seen or path */
   int64_t k_stride[3], v_stride[3], k_new_stride[3], v_new_stride[3]; /* batch, head, row; bytes */
   int64_t path_stride, weights_stride[2], draft_weights_stride[2], positions_stride[2]; /* elements */
   int64_t batch, kv_heads, slots, n_new, steps, row_bytes;
@@ -361,7 +361,7 @@ typedef struct w8_cache_evict_args {
   const int32_t* lens;     /* [batch] */
   float* weights_out;      /* like weights; may be `weights` */
   int32_t* positions_out;  /* like positions; may be `positions` */
-  int32_t* lens_out;       /* [batch], not lens itself */
+  int32_t* lens_out;       /* [batch], of no memory in common with lens */
   int64_t k_stride[3], v_stride[3]; /* batch, head, slot; bytes */
   int64_t weights_stride[2], positions_stride[2], weights_out_stride[2], positions_out_stride[2]; /* elements */
   int64_t batch, kv_heads, slots, row_bytes, budget, sink, recent;

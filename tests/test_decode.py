@@ -96,6 +96,32 @@ def test_cluster_barriers_find_their_warps_converged():
         assert "barrier.cluster." not in text, path
 
 
+def test_lens_out_stands_apart():
+    """What one CTA writes to lens_out another may yet read from lens, seen or path: the same array, or
+    one that overlaps it at another address, is refused."""
+    def append(lens=4096, path=0, seen=16384, lens_out=32768, positions=24576, stride=3, draft=0):
+        return APPEND_ARGS.pack(4096, 8192, 12288, 16384, lens, path, 0, draft, positions, seen, lens_out, *[128] * 12,
+                                stride, 0, 0, 0, 0, 64, 16, 4, 2, 64, 8, 8, 128)
+
+    run = _lib.lib().w8_cache_append
+    for kw in (dict(lens=32768), dict(lens=32768 + 4), dict(lens=32768 - 12), dict(seen=32768), dict(seen=32768 + 12),
+               dict(seen=32768 - 4), dict(path=32768, stride=8), dict(path=32768 - 4, stride=8), dict(path=32768 - 3 * 32 - 28, stride=8)):
+        assert run(append(**kw), None) == _lib.W8_ERR_INVALID_ARG, kw
+        assert b"lens_out" in _lib.lib().w8_last_error()
+    # Beside it, between the rows of a path, and positions that are not kept: nothing of that to refuse
+    # (and so that nothing runs, draft weights without weights, which is looked at next).
+    for kw in (dict(lens=32768 + 16), dict(seen=32768 - 16), dict(path=32768 - 32, stride=100), dict(seen=32768, positions=0)):
+        assert run(append(draft=4096, **kw), None) == _lib.W8_ERR_INVALID_ARG
+        assert b"draft_weights need weights" in _lib.lib().w8_last_error(), kw
+
+    def evict(lens):
+        return EVICT_ARGS.pack(4096, 4096, 4096, 4096, lens, 4096, 4096, 8192, *[128] * 6, *[16] * 8, 4, 1, 16, 128, 4, 0, 0)
+
+    for lens in (8192, 8188, 8204):
+        assert _lib.lib().w8_cache_evict(evict(lens), 4096, 1 << 20, None) == _lib.W8_ERR_INVALID_ARG
+        assert b"lens_out" in _lib.lib().w8_last_error()
+
+
 def test_evict_refuses():
     def args(budget=4, sink=0, recent=0, lens=4096, lens_out=8192, row=128):
         return EVICT_ARGS.pack(4096, 4096, 4096, 4096, lens, 4096, 4096, lens_out, *[128] * 6, *[16] * 8, 1, 1, 16, row,

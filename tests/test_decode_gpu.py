@@ -395,6 +395,19 @@ def test_append_skips_what_is_out_of_range(cuda):
     assert w8.device_status() == 0
 
 
+def test_append_refuses_to_write_lengths_over_what_it_reads(cuda):
+    _, k, v, ln, kn, vn = make(5, 2, 2, 2, 64, 3, 20, [4, 9])
+    pos = torch.zeros((2, 2, 20), dtype=torch.int32, device="cuda")
+    buf = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for kw in (dict(positions=pos, seen=buf[:2], lens_out=buf[:2]), dict(positions=pos, seen=buf[:2], lens_out=buf[1:3]),
+               dict(path=buf[:2].view(2, 1), lens_out=buf[1:3])):
+        with pytest.raises(w8._lib.W8InvalidArgument, match="lens_out"):
+            w8.cache_append(k, v, kn, vn, ln, **kw)
+    with pytest.raises(w8._lib.W8InvalidArgument, match="lens_out"):
+        w8.cache_append(k, v, kn, vn, buf[:2], lens_out=buf[1:3])
+    assert not buf.any() and w8.device_status() == 0
+
+
 @pytest.mark.parametrize("dt", [torch.int8, torch.float32, torch.float16])
 def test_append_moves_any_rows(cuda, dt):
     k, v = (torch.zeros((2, 3, 9, 16), dtype=dt, device="cuda") for _ in range(2))
