@@ -9,7 +9,7 @@
 // with the softmax in one pass over the keys (running maximum m and sum l of each row, the
 // output rescaled when m moves), fp32 scores, statistics and output sums; P is rounded to
 // the operands' 16-bit type for the second product, as the prefill attention does (half a
-// step of 2^-8 or 2^-11 on each weight, averaged over the keys).
+// step of 2^-8 or 2^-11 on each weight, averaged over the keys; TreeRef has fp16's range).
 //
 // Decode reads every key once for few rows, so it is bound by HBM: R flops per byte for R
 // rows against about 80 for the mma.sync rate over the copy rate.  A CTA owns 16 MT rows and
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
             mx[mt][h] = x;
-            move |= x > m[mt][h] + 8.f;
+            move |= x > m[mt][h] + TreeRef<T>::kSlack;
             if (a.scores != nullptr && part == 0) {
               const int r = row0 + mt * 16 + rl + 8 * h;
               if (r < rows) {
@@ -492,16 +492,15 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
               }
             }
           }
-        // A row's reference moves only when its maximum exceeds it by more than 8 (log2 units), so
-        // the output is seldom rescaled and P <= 2^8.
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const bool mv = mx[mt][h] > m[mt][h] + 8.f;
-              const float corr = mv ? ex2_tree(m[mt][h] - mx[mt][h]) : 1.f;
-              if (mv) m[mt][h] = mx[mt][h];
+              const bool mv = mx[mt][h] > m[mt][h] + TreeRef<T>::kSlack;
+              const float to = mx[mt][h] - TreeRef<T>::kBelow;
+              const float corr = mv ? ex2_tree(m[mt][h] - to) : 1.f;
+              if (mv) m[mt][h] = to;
               l[mt][h] *= corr;
 #pragma unroll
               for (int n = 0; n < DW / 8; ++n) {

@@ -71,6 +71,18 @@ __device__ __forceinline__ bool tree_nonfinite(uint32_t bits) {
   return (bits & e) == e;
 }
 
+// The softmax's running reference.  p = 2^(x - m) is rounded to the operands' type, in which fp16
+// ends at 2^-24 (halves of it round to 0) and 65504: there m stands 2^7 below the row's maximum, so
+// that what a long tail of small probabilities sums to is not lost beside one large one (each is at
+// most 2^-25 off against a sum of 2^7 at least: 2^-32 of the output a key).  m moves only when a
+// maximum exceeds it by more than 8 above that, so the output is seldom rescaled: p <= 2^15, 2^8 for
+// bf16, which has fp32's exponents and needs no such room.
+template <typename T>
+struct TreeRef {
+  static constexpr float kBelow = __is_same(T, __half) ? 7.f : 0.f;  // of m under the maximum it is set to
+  static constexpr float kSlack = 8.f + kBelow;                     // a maximum this far above m moves it
+};
+
 // A CTA's range of tiles holds at most one piece that begins an item it does not finish (its
 // last, slot 2 u + 1) and one that continues an item (its first, slot 2 u).
 __device__ __forceinline__ int64_t tree_slot(int2 info, int s) {

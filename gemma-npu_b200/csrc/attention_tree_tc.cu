@@ -8,7 +8,7 @@
 //   P_j  = 2^(c S_j - m)   two threads a row (64 keys each): mask, maximum, sum; P_j 16-bit
 //                      back into the S buffer
 //   O   += P_j V_j     A = P_j from TMEM, each CTA staging half of V's columns
-// m moves only when a tile's maximum exceeds it by more than 8 (log2 units).  Many rows per
+// m moves only when a tile's maximum exceeds it by enough (TreeRef).  Many rows per
 // key make this bound by the MMAs and the softmax's exponentials, not by HBM: trees of 64
 // drafts for 16 sequences, D 256, 8 heads a group, 2000 to 4000 keys take 65 us here (a tile
 // some 2650 clocks of a pair, its MMAs 2048) and 672 with mma.sync.  The key axis is split over
@@ -400,9 +400,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
       pair_sync();  // the partner's maximum is read before either posts the next one
       if (!ok) continue;
       const float mt = mx * scale;
-      const bool move = mt > m + 8.f;
+      const bool move = mt > m + TreeRef<T>::kSlack;
       if (__any_sync(0xffffffffu, move)) {
-        const float mn = move ? mt : m;
+        const float mn = move ? mt - TreeRef<T>::kBelow : m;
         const float corr = move ? ex2_tc(m - mn) : 1.f;
         if (i > 0) {
           ok = mbar_wait_bounded(pv_done((i - 1) & 1), ((i - 1) >> 1) & 1, abort_flag, &g_tree_status);

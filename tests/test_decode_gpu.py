@@ -256,6 +256,44 @@ def test_infinite_values_in_every_step_of_a_tile(cuda, D):
     assert (got[bad] == math.inf).all()
 
 
+def long_tail(B, H, N, D, S, large):
+    """Equal keys with values 1, and keys `large` that weigh e^17.5 times as much with values 0."""
+    dt = torch.float16
+    q = torch.zeros((1, H, N, D), dtype=dt, device="cuda")
+    q[..., 0] = 1.0
+    k, v = torch.zeros((1, 1, S, D), dtype=dt, device="cuda"), torch.ones((1, 1, S, D), dtype=dt, device="cuda")
+    k[0, 0, large, 0], v[0, 0, large] = 17.5, 0.0
+    kn, vn = torch.zeros((1, 1, N, D), dtype=dt, device="cuda"), torch.ones((1, 1, N, D), dtype=dt, device="cuda")
+    lens = torch.full((B,), S, dtype=torch.int32, device="cuda")
+    one = q, k, v, lens[:1], kn, vn
+    return one, [x.expand(B, *x.shape[1:]) for x in (q, k, v)] + [lens] + [x.expand(B, *x.shape[1:]) for x in (kn, vn)]
+
+
+# Each of fp16's probabilities may be half a step of its least one off (2^-25) where the sum is at
+# least 2^7: 2^-32 a key, whose values are at most 1 here.  Lost altogether they would sum to some
+# S e^-17.5 / (number of large keys): 1.5e-3 and 4.7e-5 against bounds of 1.4e-5 and 7.4e-6.
+@pytest.mark.parametrize("case", [(1, 70, 64, 60000), (1, 40, 128, 60000), (1, 20, 256, 60000), (1, 20, 512, 60000),
+                                  (1200, 1, 64, 30000), (1200, 1, 128, 30000)], ids=str)
+def test_fp16_keeps_a_long_tail_of_small_weights(cuda, case):
+    """tcgen05 (one large key), and the warps of mma.sync CTAs that hold a whole sequence each (a
+    large key in every 16 of their first ones)."""
+    B, N, D, S = case
+    one, all_of = long_tail(B, 8 if B == 1 else 1, N, D, S, [100] if B == 1 else list(range(0, 256, 16)))
+    o, tol, pv = want_attention(*one)[:3]
+    err = (w8.attention_tree(*all_of).double() - o).abs()
+    assert bool((err <= HALF[torch.float16] * (pv + o) + tol + 2.0 ** -24 + 2.0 ** -32 * (S + N)).all()), float(err.max())
+
+
+@pytest.mark.parametrize("D,N", [(64, 1), (128, 40), (256, 2), (512, 20)])
+def test_fp16_accumulated_weights_of_a_long_tail(cuda, D, N):
+    one, _ = long_tail(1, 8, N, D, 9000, [100])
+    w = torch.zeros((1, 1, 9000), device="cuda")
+    _, wo, dw = w8.attention_tree(*one, weights=w)
+    want = want_attention(*one)
+    rel = 2 * want[5] + (8 * N + 4) * 2.0 ** -24 + 2.0 ** -21
+    assert ((wo.double() - want[3]).abs() <= rel * want[3]).all() and ((dw.double() - want[4]).abs() <= rel * want[4]).all()
+
+
 @pytest.mark.parametrize("N", [1, 40])
 @pytest.mark.parametrize("D", [64, 128, 256, 512])
 def test_slots_before_the_window_may_hold_anything(cuda, D, N):
