@@ -1073,6 +1073,27 @@ static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStr
   return st;
 }
 
+// A call without new tokens adds nothing to the weights, which still go where they are wanted.
+static int tree_no_tokens(const w8_attention_tree_args& x, cudaStream_t stream) {
+  if (x.weights == x.weights_out || x.slots == 0) return W8_OK;
+  W8_CHECK_ARG(x.weights && x.weights_out && x.lens, "weights, weights_out and draft_weights come together");
+  W8_CHECK_ARG(x.batch * x.kv_heads <= 65535, "batch * kv_heads beyond 65535 with weights");
+  int device = 0;
+  const int st = require_sm100(&device);
+  if (st != W8_OK) return st;
+  w8::TreeArgs a = {};
+  a.lens = x.lens;
+  a.batch = static_cast<int>(x.batch), a.kv_heads = static_cast<int>(x.kv_heads), a.slots = static_cast<int>(x.slots);
+  a.group = static_cast<int>(x.heads / x.kv_heads);
+  a.draft_at = (a.slots + 3) / 4 * 4;
+  a.w_in = x.weights, a.w_out = x.weights_out;
+  a.wi_b = x.weights_stride[0], a.wi_h = x.weights_stride[1];
+  a.wo_b = x.weights_out_stride[0], a.wo_h = x.weights_out_stride[1];
+  return launch_tree(w8::attn_tree_weights_kernel<1>,
+                     dim3(static_cast<unsigned>((a.draft_at + 1023) / 1024), static_cast<unsigned>(x.batch * x.kv_heads)), 256,
+                     0, stream, a);
+}
+
 // Read (and optionally clear) the sticky device status of the cache attention.
 int tree_device_status(int clear, int* out) {
   int v = 0;
@@ -1113,7 +1134,13 @@ extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspa
   int st = tree_shape(x.batch, x.heads, x.kv_heads, x.head_dim, x.slots, x.n_new, x.window);
   if (st != W8_OK) return st;
   W8_CHECK_ARG(x.dtype == W8_BF16 || x.dtype == W8_FP16, "dtype must be W8_BF16 or W8_FP16");
-  if (x.batch == 0 || x.n_new == 0) return W8_OK;
+  if (x.batch == 0) return W8_OK;
+  // In place only with the same layout: rows of one would be other rows of the other.
+  W8_CHECK_ARG(x.weights == nullptr || x.weights != x.weights_out ||
+                   ((x.batch == 1 || x.weights_stride[0] == x.weights_out_stride[0]) &&
+                    (x.kv_heads == 1 || x.weights_stride[1] == x.weights_out_stride[1])),
+               "weights_out is weights with other strides");
+  if (x.n_new == 0) return tree_no_tokens(x, reinterpret_cast<cudaStream_t>(stream));
   // (positive in the kernels' fp32 log2 units too: a masked score is -inf times it)
   const float scale_log2 = static_cast<float>(x.scale * 1.4426950408889634);
   W8_CHECK_ARG(scale_log2 > 0.f && scale_log2 < 3e38f, "scale must be positive and finite");
@@ -1124,11 +1151,6 @@ extern "C" int w8_attention_tree(const w8_attention_tree_args* in, void* workspa
   const bool weights = x.weights != nullptr || x.weights_out != nullptr || x.draft_weights != nullptr;
   W8_CHECK_ARG(!weights || (x.draft_weights && (x.slots == 0 || (x.weights && x.weights_out))),
                "weights, weights_out and draft_weights come together");
-  // In place only with the same layout: rows of one would be other rows of the other.
-  W8_CHECK_ARG(!weights || x.weights != x.weights_out ||
-                   ((x.batch == 1 || x.weights_stride[0] == x.weights_out_stride[0]) &&
-                    (x.kv_heads == 1 || x.weights_stride[1] == x.weights_out_stride[1])),
-               "weights_out is weights with other strides");
   W8_CHECK_ARG(x.out != x.q && x.out != x.k && x.out != x.v && x.out != x.k_new && x.out != x.v_new,
                "out must not be an input");
   const void* ptrs[6] = {x.q, x.k, x.v, x.k_new, x.v_new, x.out};

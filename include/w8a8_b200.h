@@ -320,7 +320,7 @@ typedef struct w8_attention_tree_args {
  * Grouped-query heads, head_dim 64, 128, 256 or 512, fp32 softmax and sums.  With weights:
  * weights_out[b, c, j] = weights[b, c, j] + the probabilities of slot j summed over the
  * group's heads and the n tokens (slots behind lens[b] are left alone), and draft_weights
- * the same sums for the new tokens (every row of q counts, a padding one too).  A new token's
+ * the same sums for the new tokens (every row of q counts, a padding one too; n = 0 adds nothing).  A new token's
  * values may be infinite or NaN where some token must not see them; those of the committed
  * slots that any token's window reaches must be finite (with depths given, a window is taken
  * to reach as far back as depth 0's).  out must not overlap the inputs, weights_out nothing

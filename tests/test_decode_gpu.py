@@ -347,6 +347,22 @@ def test_weights(cuda, shape, in_place):
         assert torch.equal(w, prev)
 
 
+def test_weights_of_no_new_tokens(cuda):
+    """N = 0 adds nothing: the weights of the committed slots still go to weights_out."""
+    S, lens = 2600, [2600, 5, 0]
+    q, k, v, ln, kn, vn = make(1, 3, 4, 2, 64, 3, S, lens)
+    wide = torch.rand((3, 2, S + 9), device="cuda")
+    w, to = wide[..., 2:S + 2], torch.full((3, 2, S), -3.0, device="cuda")
+    empty = q[:, :, :0], k, v, ln, kn[:, :, :0], vn[:, :, :0]
+    o, wo, dw = w8.attention_tree(*empty, weights=w, weights_out=to)
+    assert o.shape == (3, 4, 0, 64) and wo is to and dw.shape == (3, 2, 0)
+    for b, n in enumerate(lens):
+        assert torch.equal(to[b, :, :n], w[b, :, :n]) and (to[b, :, n:] == -3).all()
+    before = wide.clone()
+    assert w8.attention_tree(*empty, weights=w)[1] is w and torch.equal(wide, before)
+    assert w8.device_status() == 0
+
+
 @pytest.mark.parametrize("N", [1, 3, 60])
 def test_same_bits_every_time(cuda, N):
     a = make(1, 2, 8, 1, 256, N, 3000, [3000, 1234])
