@@ -172,7 +172,10 @@ __device__ constexpr float kTanh[kTanhTerms] = {0.9999997019767761f,  -0.3333213
                                                 -0.053265832364559174f, 0.019973276183009148f, -0.005951274652034044f,
                                                 0.0009637702605687082f};
 
-template <typename T, bool CAP>
+// CAP: 0 no softcap, 1 one up to 1000, 2 a larger one (a kernel of its own: the branch in the stream
+// cost the 24 x 8 beams 1 us of 43).
+constexpr float kBeamLargeCap = 1e3f;
+template <typename T, int CAP>
 __global__ void __launch_bounds__(kBeamThreads, beam_per_sm(sizeof(T))) beam_chunk_kernel(const BeamArgs a) {
   __shared__ unsigned long long cand[kBeamCap];
   __shared__ float seg_max[kBeamSuper][kBeamThreads];
@@ -194,14 +197,29 @@ __global__ void __launch_bounds__(kBeamThreads, beam_per_sm(sizeof(T))) beam_chu
   float mx = -INFINITY, sum = 0.f;  // reference (log2 units) and sum of 2^(y - reference)
   unsigned long long thr = 0;       // candidates must beat this key
   const float cap_in = CAP ? 1.f / a.cap : 0.f, cap_out = CAP ? a.cap * kLog2e : 0.f;
-  // (beyond these caps the scaled coefficients leave fp32's range)
-  const float poly_to = CAP && a.cap >= 1e-2f && a.cap <= 1e3f ? a.cap : 0.f;
+  // (beyond 1e-2 .. 1e3 the scaled coefficients leave fp32's range: no segment is in this one)
+  const float poly_to = CAP == 1 && a.cap >= 1e-2f ? a.cap : -1.f;
   uint64_t tc[kTanhTerms];
   if constexpr (CAP) {
     float f = kLog2e;
 #pragma unroll
     for (int i = 0; i < kTanhTerms; ++i, f *= cap_in * cap_in) tc[i] = f2_pack(kTanh[i] * f, kTanh[i] * f);
   }
+  // The softcap of any logit.  1 + tanh - 1 is off by some 2^-22 of the cap, which is nothing to a cap
+  // that the logits reach; below a large one they take the polynomial, off by 2^-21 of themselves.
+  auto soft = [&](float l) {
+    const float t = l * cap_in;
+    if constexpr (CAP == 2) {
+      if (fabsf(t) <= 1.f) {
+        const float u = t * t;
+        float p = kTanh[kTanhTerms - 1];
+#pragma unroll
+        for (int q = kTanhTerms - 2; q >= 0; --q) p = fmaf(p, u, kTanh[q]);
+        return l * kLog2e * p;
+      }
+    }
+    return cap_out * (one_plus_tanh(t) - 1.f);
+  };
   // The thread's segment of a tile: 16 consecutive logits.
   auto load = [&](int t0, uint4 (&raw)[GROUPS]) {
     const int at0 = t0 + tid * kBeamVals;
@@ -238,7 +256,7 @@ __global__ void __launch_bounds__(kBeamThreads, beam_per_sm(sizeof(T))) beam_chu
       seg_max[j][tid] = tm;
       best_mine = fmaxf(best_mine, tm);
       float ym = tm * kLog2e;
-      if constexpr (CAP) ym = tm == -INFINITY ? -INFINITY : cap_out * (one_plus_tanh(tm * cap_in) - 1.f);
+      if constexpr (CAP) ym = tm == -INFINITY ? -INFINITY : soft(tm);
       if (ym > mx) {
         sum *= ex2_beam(mx - ym);
         mx = ym;
@@ -280,7 +298,7 @@ __global__ void __launch_bounds__(kBeamThreads, beam_per_sm(sizeof(T))) beam_chu
           beam_unpack(w, v, T{});
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {  // (an impossible token, or one past the chunk, stays impossible)
-            const float y = v[i] == -INFINITY ? -INFINITY : cap_out * (one_plus_tanh(v[i] * cap_in) - 1.f);
+            const float y = v[i] == -INFINITY ? -INFINITY : soft(v[i]);
             part = f2_add(part, f2_pack(ex2_beam(y - ref), 0.f));
           }
         }
@@ -602,6 +620,12 @@ static int64_t beam_ws(int64_t rows, const BeamPlan& p, int64_t n) {
   return rows * p.chunks * (n * 8 + 8);
 }
 
+template <typename T>
+static auto beam_chunk(float cap) {
+  return !(cap > 0.f) ? w8::beam_chunk_kernel<T, 0>
+         : cap <= w8::kBeamLargeCap ? w8::beam_chunk_kernel<T, 1> : w8::beam_chunk_kernel<T, 2>;
+}
+
 template <typename Kern>
 static int launch_beam(Kern kern, dim3 grid, int threads, int smem, cudaStream_t stream, const w8::BeamArgs& a) {
   cudaLaunchConfig_t cfg = {};
@@ -636,6 +660,7 @@ extern "C" int w8_beam_select(const void* logits, int dtype, int64_t stride_b, i
   if (st != W8_OK) return st;
   W8_CHECK_ARG(dtype == W8_BF16 || dtype == W8_FP16 || dtype == W8_FP32, "dtype must be W8_BF16, W8_FP16 or W8_FP32");
   W8_CHECK_ARG(!slot_order || n == beams, "slot order needs as many continuations as beams");
+  W8_CHECK_ARG(cap <= 0.f || (cap >= 1e-30f && cap <= 1e30f), "cap must be 0 (none) or between 1e-30 and 1e30");
   W8_CHECK_ARG(pad >= 0 && pad < vocab, "pad %lld is not a token", (long long)pad);
   if (batch == 0) return W8_OK;
   W8_CHECK_ARG(logits && scores && out_scores && out_beam && out_token, "null pointer");
@@ -659,16 +684,9 @@ extern "C" int w8_beam_select(const void* logits, int dtype, int64_t stride_b, i
   a.out_scores = out_scores, a.out_beam = out_beam, a.out_token = out_token, a.slot_order = slot_order;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(p.chunks), static_cast<unsigned>(rows));
-  const bool capped = cap > 0.f;
-  if (dtype == W8_FP32)
-    st = launch_beam(capped ? w8::beam_chunk_kernel<float, true> : w8::beam_chunk_kernel<float, false>, grid,
-                     w8::kBeamThreads, 0, s, a);
-  else if (dtype == W8_BF16)
-    st = launch_beam(capped ? w8::beam_chunk_kernel<__nv_bfloat16, true> : w8::beam_chunk_kernel<__nv_bfloat16, false>,
-                     grid, w8::kBeamThreads, 0, s, a);
-  else
-    st = launch_beam(capped ? w8::beam_chunk_kernel<__half, true> : w8::beam_chunk_kernel<__half, false>, grid,
-                     w8::kBeamThreads, 0, s, a);
+  st = dtype == W8_FP32   ? launch_beam(beam_chunk<float>(cap), grid, w8::kBeamThreads, 0, s, a)
+       : dtype == W8_BF16 ? launch_beam(beam_chunk<__nv_bfloat16>(cap), grid, w8::kBeamThreads, 0, s, a)
+                          : launch_beam(beam_chunk<__half>(cap), grid, w8::kBeamThreads, 0, s, a);
   if (st != W8_OK) return st;
   const int64_t all = static_cast<int64_t>(a.beams) * a.m;
   const int smem = static_cast<int>(all * 16 + static_cast<int64_t>(w8::kMergeWarps) * p.chunks * n * 8 + n * 4 + 16);

@@ -374,6 +374,8 @@ PyObject* beam_select(PyObject* const* arg, Py_ssize_t nargs) {
                       : static_cast<const uint8_t*>(vector(arg[2], "finished", {B, K}, at::kBool, dev).const_data_ptr());
   const int64_t pad = integer(arg[3], "pad"), n = is_none(arg[4]) ? K : integer(arg[4], "n");
   const double cap = is_none(arg[5]) ? 0.0 : real(arg[5], "cap");
+  // (checked here too: a double outside fp32's range would become another cap)
+  NEED(cap <= 0.0 || (cap >= 1e-30 && cap <= 1e30), "cap must be 0 (none) or between 1e-30 and 1e30");
   NEED(n >= 1, "n = ", n, " must be positive");
   const char* order = PyUnicode_Check(arg[6]) ? PyUnicode_AsUTF8(arg[6]) : "";
   const bool slot = std::string("slot") == order;
@@ -382,7 +384,7 @@ PyObject* beam_select(PyObject* const* arg, Py_ssize_t nargs) {
   if (B > 0) {
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor ws = workspace(fn_select_ws(B, K, V, n), dev);
-    check(fn_select(x.const_data_ptr(), dt, x.stride(0), x.stride(1), scores, finished, pad, static_cast<float>(cap), B, K,
+    check(fn_select(x.const_data_ptr(), dt, x.stride(0), x.stride(1), scores, finished, pad, cap > 0.0 ? static_cast<float>(cap) : 0.f, B, K,
                     V, n, slot, static_cast<float*>(out.data_ptr()), beam.data_ptr<int64_t>(), token.data_ptr<int64_t>(),
                     ws.data_ptr(), ws.numel(), stream_of(dev)),
           "w8_beam_select");

@@ -131,7 +131,8 @@ def beam_select(logits, scores, finished=None, pad=0, n=None, cap=0.0, order="sc
 
     logits fp32, bf16 or fp16 [B, K, V] (unit stride along V), scores fp32 [B, K] the beams'
     log probabilities so far; a continuation's score is scores + log_softmax(y), y = cap *
-    tanh(logits / cap) with cap > 0, else the logits; a logit of -inf is an impossible token.
+    tanh(logits / cap) with cap > 0 (1e-30 to 1e30), else the logits; a logit of -inf is an
+    impossible token, under a cap too.
     Best first; equal scores to the lower beam, then the lower token.  A beam with finished
     (bool [B, K]) set has one continuation, the token `pad` at an unchanged score; a beam
     whose score or log sum is not finite has none.  Impossible continuations have score -inf

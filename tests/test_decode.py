@@ -146,6 +146,13 @@ def test_select_refuses():
     assert run(logits=4098) == _lib.W8_ERR_ALIGNMENT
 
 
+@pytest.mark.parametrize("cap", [float("nan"), float("inf"), 1e-31, 1e31])
+def test_select_refuses_caps_it_cannot_scale(cap):
+    assert _lib.lib().w8_beam_select(4096, _lib.W8_FP32, 20, 10, 4096, None, 0, cap, 1, 2, 10, 2, 0, 4096, 4096, 4096, 4096,
+                                     1 << 20, None) == _lib.W8_ERR_INVALID_ARG
+    assert b"cap must be" in _lib.lib().w8_last_error()
+
+
 def test_wrappers_refuse_host_tensors():
     x = torch.zeros((1, 1, 4, 64), dtype=torch.bfloat16)
     ln = torch.zeros(1, dtype=torch.int32)

@@ -620,6 +620,31 @@ def test_select_impossible(cuda, n, cap):
     check_select(got, want, 16.0, V, cap)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("cap", [1e-30, 1e-4, 5e-3, 0.5, 999.0, 1001.0, 1e4, 1e6, 1e30])
+def test_select_scores_under_any_cap(cuda, cap, dt):
+    """Caps far below and far above the logits; whole segments of zeros.  A softcapped logit is off by
+    at most 2^-21 of the smaller of the cap and the logit."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    B, K, V, n = 2, 3, 9000, 4
+    logits = rows(gen, (B, K, V), dt, 4.0)
+    logits[:, :, 160:320] = 0
+    scores = torch.randn((B, K), generator=gen, device="cuda") - 5
+    got = w8.beam_select(logits, scores, n=n, cap=cap)[0].double()
+    total = scores.double()[:, :, None] + torch.log_softmax(cap * torch.tanh(logits.double() / cap), 2)
+    want = torch.topk(total.reshape(B, -1), n).values
+    tol = 2.0 ** -22 + 2.0 ** -23 * 24 * 1.45 * 2 + (V / 256 + 40) * 2.0 ** -24 + 2.0 ** -21 * min(cap, 24.0) * 1.45
+    assert ((got - want).abs() <= tol + 2.0 ** -24 * want.abs()).all(), (got - want).abs().max()
+
+
+@pytest.mark.parametrize("cap", [math.nan, math.inf, 1e-46, 1e-31, 1e31, 1e300])
+def test_select_refuses_caps_it_cannot_scale(cuda, cap):
+    logits, scores = torch.zeros((1, 2, 9), device="cuda"), torch.zeros((1, 2), device="cuda")
+    with pytest.raises(ValueError, match="cap must be"):
+        w8.beam_select(logits, scores, cap=cap)
+    assert w8.beam_select(logits, scores, cap=-cap if cap == cap else -1.0)[0].isfinite().all()  # not positive: none
+
+
 @pytest.mark.parametrize("kind", ["rising", "falling", "equal", "first"])
 def test_select_orders_that_fill_the_candidates(cuda, kind):
     """Ascending logits pass every threshold; equal ones tie on all of them."""
