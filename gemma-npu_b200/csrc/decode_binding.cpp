@@ -377,9 +377,9 @@ PyObject* beam_select(PyObject* const* arg, Py_ssize_t nargs) {
   // (checked here too: a double outside fp32's range would become another cap)
   NEED(cap <= 0.0 || (cap >= 1e-30 && cap <= 1e30), "cap must be 0 (none) or between 1e-30 and 1e30");
   NEED(n >= 1, "n = ", n, " must be positive");
-  const char* order = PyUnicode_Check(arg[6]) ? PyUnicode_AsUTF8(arg[6]) : "";
-  const bool slot = std::string("slot") == order;
-  NEED(slot || std::string("score") == order, "order must be one of ('score', 'slot')");
+  const auto is = [&](const char* s) { return PyUnicode_Check(arg[6]) && PyUnicode_CompareWithASCIIString(arg[6], s) == 0; };
+  const bool slot = is("slot");
+  NEED(slot || is("score"), "order must be one of ('score', 'slot')");
   const Tensor out = make({B, n}, at::kFloat, dev), beam = make({B, n}, at::kLong, dev), token = make({B, n}, at::kLong, dev);
   if (B > 0) {
     const c10::cuda::CUDAGuard guard(dev);
@@ -439,8 +439,12 @@ PyObject* cache_reorder(PyObject* const* arg, Py_ssize_t nargs) {
 // bind(library path, check): take the entry points from the loaded library.
 PyObject* bind(PyObject* const* arg, Py_ssize_t nargs) {
   NEED(nargs == 2 && PyUnicode_Check(arg[0]) && PyCallable_Check(arg[1]), "bind(path, check)");
-  void* lib = dlopen(PyUnicode_AsUTF8(arg[0]), RTLD_NOW);
-  NEED(lib != nullptr, "cannot load ", PyUnicode_AsUTF8(arg[0]));
+  PyObject* name = nullptr;  // the path's bytes, which need not be UTF-8
+  if (!PyUnicode_FSConverter(arg[0], &name)) throw Raised();
+  const std::string path = PyBytes_AS_STRING(name);
+  Py_DECREF(name);
+  void* lib = dlopen(path.c_str(), RTLD_NOW);
+  NEED(lib != nullptr, "cannot load ", path);
   auto get = [&](auto& fn, const char* name) {
     fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(dlsym(lib, name));
     NEED(fn != nullptr, name, " is missing from the library");
@@ -457,6 +461,14 @@ PyObject* bind(PyObject* const* arg, Py_ssize_t nargs) {
   Py_RETURN_NONE;
 }
 
+// (A message may quote a path, which need not be UTF-8.)
+void raise(PyObject* type, const char* what) {
+  PyObject* text = PyUnicode_DecodeUTF8(what, static_cast<Py_ssize_t>(std::char_traits<char>::length(what)), "replace");
+  if (text == nullptr) return;
+  PyErr_SetObject(type, text);
+  Py_DECREF(text);
+}
+
 // No C++ exception passes into Python.
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
 PyObject* entry(PyObject*, PyObject* const* arg, Py_ssize_t nargs) {
@@ -464,9 +476,9 @@ PyObject* entry(PyObject*, PyObject* const* arg, Py_ssize_t nargs) {
     return F(arg, nargs);
   } catch (const Raised&) {
   } catch (const Refused& x) {
-    PyErr_SetString(PyExc_ValueError, x.what());
+    raise(PyExc_ValueError, x.what());
   } catch (const std::exception& x) {  // torch's own, out of memory among them
-    PyErr_SetString(PyExc_RuntimeError, x.what());
+    raise(PyExc_RuntimeError, x.what());
   } catch (...) {
     PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
   }

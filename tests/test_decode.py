@@ -153,6 +153,31 @@ def test_select_refuses_caps_it_cannot_scale(cap):
     assert b"cap must be" in _lib.lib().w8_last_error()
 
 
+def test_binding_loads_a_library_under_any_name(tmp_path):
+    """The library's path need not be UTF-8 (a process of its own: this one's binding stays bound)."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+
+    from gemma_npu_b200 import decode
+
+    try:
+        odd = os.path.join(os.fsencode(str(tmp_path)), b"lib-\xff.so")
+        os.symlink(os.fsencode(_lib.LIB_PATH), odd)
+    except OSError:
+        shutil.copy(_lib.LIB_PATH, tmp_path / "lib.so")
+        odd = os.fsencode(str(tmp_path / "lib.so"))
+    code = ("import importlib.util, os, sys, torch\n"
+            "spec = importlib.util.spec_from_file_location('_decode', sys.argv[1])\n"
+            "m = importlib.util.module_from_spec(spec); spec.loader.exec_module(m)\n"
+            "m.bind(sys.argv[2], print)\n"
+            "try:\n    m.bind(sys.argv[2] + '.none', print)\n"
+            "except ValueError as e:\n    assert str(e).startswith('cannot load')\n"
+            "else:\n    raise SystemExit(1)\n")
+    subprocess.run([sys.executable, "-c", code, decode.BINDING_PATH, odd], check=True, timeout=300)
+
+
 def test_wrappers_refuse_host_tensors():
     x = torch.zeros((1, 1, 4, 64), dtype=torch.bfloat16)
     ln = torch.zeros(1, dtype=torch.int32)

@@ -645,6 +645,13 @@ def test_select_refuses_caps_it_cannot_scale(cuda, cap):
     assert w8.beam_select(logits, scores, cap=-cap if cap == cap else -1.0)[0].isfinite().all()  # not positive: none
 
 
+@pytest.mark.parametrize("order", ["", "scores", "\udc80", "sl\0ot", "slot\0", b"slot", None, 0])
+def test_select_refuses_other_orders(cuda, order):
+    """Text that no UTF-8 encodes among them."""
+    with pytest.raises(ValueError, match="order must be"):
+        w8.beam_select(torch.zeros((1, 2, 9), device="cuda"), torch.zeros((1, 2), device="cuda"), order=order)
+
+
 @pytest.mark.parametrize("kind", ["rising", "falling", "equal", "first"])
 def test_select_orders_that_fill_the_candidates(cuda, kind):
     """Ascending logits pass every threshold; equal ones tie on all of them."""
