@@ -419,8 +419,11 @@ PyObject* cache_reorder(PyObject* const* arg, Py_ssize_t nargs) {
   ptrs.reserve(static_cast<size_t>(count));
   for (Py_ssize_t i = 0; i < count; ++i) {
     const Tensor& t = tensor(items[i], "caches");
-    NEED(t.sizes() == first.sizes() && t.strides() == first.strides() && t.scalar_type() == first.scalar_type() &&
-             t.device() == dev,
+    NEED(t.sizes() == first.sizes() && t.scalar_type() == first.scalar_type() && t.device() == dev,
+         "caches must share one shape, layout, dtype and device");
+    int64_t own[3];  // (a dimension of one element has no stride to speak of: 0 in both)
+    rows4(items[i], "caches", first.scalar_type(), dev, own, first.element_size());
+    NEED(own[0] == strides[0] && own[1] == strides[1] && own[2] == strides[2],
          "caches must share one shape, layout, dtype and device");
     ptrs.push_back(t.data_ptr());
   }

@@ -720,6 +720,19 @@ def test_reorder(cuda, shape, ragged, index):
     assert w8.device_status() == 0
 
 
+def test_reorder_takes_one_layout_whatever_its_idle_strides(cuda):
+    """Dimensions of one element may have any stride; any other difference of layout is refused."""
+    x, y = torch.randn((4, 1, 8, 16), device="cuda"), torch.randn((4, 8, 1, 16), device="cuda").transpose(1, 2)
+    assert x.stride() != y.stride()
+    beam, src = torch.tensor([[1, 0], [0, 0]], device="cuda"), [1, 0, 2, 2]
+    want = [x[src], y[src]]
+    w8.cache_reorder([x, y], beam)
+    assert torch.equal(x, want[0]) and torch.equal(y, want[1])
+    for other in (torch.randn((4, 1, 9, 16), device="cuda")[:, :, :8], torch.randn((8, 4, 1, 16), device="cuda").permute(1, 2, 0, 3)):
+        with pytest.raises(ValueError, match="one shape, layout"):
+            w8.cache_reorder([x, other], beam)
+
+
 def test_reorder_bad_parents_are_reported(cuda):
     x = torch.randn((4, 1, 8, 16), device="cuda")
     want = x.clone()
