@@ -4,7 +4,8 @@
 //
 //   total(k, t) = scores[k] + y_kt - Z_k,   y = cap tanh(l / cap) (or l),  Z_k = log sum_t e^y
 // and per sequence the n largest totals over all (k, t), ties to the lower beam, then the
-// lower token.  Within a beam the order of totals is the order of the logits, so one pass
+// lower token.  Within a beam the order of totals is the order of the logits (which is kept
+// where the softcap's or a total's rounding makes different logits equal), so one pass
 // over the logits yields everything: each CTA streams a chunk of one beam's logits, keeping
 // a running maximum and sum of e^y per thread and the maximum of every segment of 16 logits;
 // after 24 tiles a value that at least n logits reach is found from the threads' maxima, and

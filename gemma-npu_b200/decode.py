@@ -133,7 +133,9 @@ def beam_select(logits, scores, finished=None, pad=0, n=None, cap=0.0, order="sc
     log probabilities so far; a continuation's score is scores + log_softmax(y), y = cap *
     tanh(logits / cap) with cap > 0 (1e-30 to 1e30), else the logits; a logit of -inf is an
     impossible token, under a cap too.
-    Best first; equal scores to the lower beam, then the lower token.  A beam with finished
+    Best first; equal scores to the lower beam.  Within a beam the order is that of the logits,
+    equal ones to the lower token, also where the softcap or the rounding of a score makes the
+    scores of different logits equal (far above the cap, say).  A beam with finished
     (bool [B, K]) set has one continuation, the token `pad` at an unchanged score; a beam
     whose score or log sum is not finite has none.  Impossible continuations have score -inf
     and come last.  At most 32 beams and n = 64.

@@ -379,8 +379,9 @@ int64_t w8_cache_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t 
 
 /* Beam search's selection: of all (beam, token) of a sequence the n with the largest
  *   total = scores[beam] + y - log sum e^y,  y = cap tanh(logit / cap) (cap <= 0: the logit),
- * best first, equal totals to the lower beam, then the lower token; a positive cap is between
- * 1e-30 and 1e30.  logits [batch, beams,
+ * best first, equal totals (in 64 bits) to the lower beam; within a beam in the order of the
+ * logits, equal ones to the lower token, also where different logits' totals round to one; a
+ * positive cap is between 1e-30 and 1e30.  logits [batch, beams,
  * vocab] of `dtype` with strides stride_b, stride_k (elements); a logit of -inf is an
  * impossible token.  A finished beam's only continuation is `pad`, at an unchanged score; a
  * beam whose score or log sum is not finite has none: impossible continuations have total

@@ -620,6 +620,32 @@ def test_select_impossible(cuda, n, cap):
     check_select(got, want, 16.0, V, cap)
 
 
+@pytest.mark.parametrize("kind", ["saturated", "rounded"])
+@pytest.mark.parametrize("n", [1, 5, 24])
+def test_select_orders_a_beam_by_its_logits(cuda, n, kind):
+    """Different logits whose scores are equal in 64 bits, by a saturated softcap or by rounding:
+    the logits decide within a beam, the lower beam between beams."""
+    B, K, V, cap = 2, 3, 500, 30.0 if kind == "saturated" else 0.0
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    few = torch.randint(0, 40, (B, K, V), generator=gen, device="cuda").float()
+    logits = 700 + 5 * few if kind == "saturated" else 1e-20 * few
+    logits[:, 2, 100:] = -5.0
+    scores = torch.tensor([[-1.0, -1.0, -1.0], [-2.0, -1.0, -1.5]], device="cuda")
+    got = w8.beam_select(logits, scores, n=n, cap=cap)
+    for b in range(B):
+        every = []
+        for k in range(K):
+            x = logits[b, k].double()
+            y = cap * torch.tanh(x / cap) if cap else x
+            total = (scores[b, k].double() + (y - torch.logsumexp(y, 0))).tolist()
+            order = sorted(range(V), key=lambda t: (-x[t].item(), t))[:n]
+            assert len({total[t] for t in order}) == 1 and (n < 24 or len({x[t].item() for t in order}) > 1)
+            every += [(-total[t], k, i, t) for i, t in enumerate(order)]
+        every = sorted(every)[:n]
+        assert got[1][b].tolist() == [e[1] for e in every] and got[2][b].tolist() == [e[3] for e in every]
+        assert all(abs(s + e[0]) <= 1e-4 for s, e in zip(got[0][b].tolist(), every))
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("cap", [1e-30, 1e-4, 5e-3, 0.5, 999.0, 1001.0, 1e4, 1e6, 1e30])
 def test_select_scores_under_any_cap(cuda, cap, dt):
