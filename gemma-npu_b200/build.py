@@ -1,7 +1,8 @@
 """Build the sm_100a C-ABI library `libw8a8_b200.so` in-tree with nvcc.
 
 Also the Python binding of the decoding operators, `_decode.so`, with the host compiler
-(`csrc/decode_binding.cpp`: torch's C++ API on one side, the C ABI on the other).
+(`csrc/decode_binding.cpp`: torch's C++ API on one side, the C ABI on the other).  Where torch is
+not installed there is nothing to bind: only the library is built.
 
 Every `csrc/*.cu` is compiled for `arch=compute_100a,code=sm_100a` (nvcc
 cross-compiles without a GPU) into `_build/*.o`, and linked into
@@ -12,6 +13,7 @@ usage: python gemma-npu_b200/build.py [--force] [--verbose-ptxas]
 """
 import argparse
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -92,7 +94,10 @@ def build(force=False, verbose_ptxas=False, quiet=False):
         os.replace(tmp, LIB)
         if not quiet:
             print("[build] linked", LIB, flush=True)
-    build_binding(force=force, quiet=quiet)
+    if importlib.util.find_spec("torch") is not None:
+        build_binding(force=force, quiet=quiet)
+    elif not quiet:
+        print("[build] no torch: without the Python binding of the decoding operators", flush=True)
     return LIB
 
 
