@@ -7,7 +7,8 @@ not installed there is nothing to bind: only the library is built.
 Every `csrc/*.cu` is compiled for `arch=compute_100a,code=sm_100a` (nvcc
 cross-compiles without a GPU) into `_build/*.o`, and linked into
 `libw8a8_b200.so` next to this file, where `_lib.py` loads it.  Objects are
-rebuilt when their source or any header under `csrc/` or `include/` is newer.
+rebuilt when their source or any header under `csrc/` or `include/` is newer, the binding
+also for another torch or Python than it was built for.
 
 usage: python gemma-npu_b200/build.py [--force] [--verbose-ptxas]
 """
@@ -51,9 +52,13 @@ def build_binding(force=False, quiet=False):
     from torch.utils.cpp_extension import include_paths, library_paths
 
     src = os.path.join(CSRC, "decode_binding.cpp")
-    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(
-            os.path.getmtime(src), _newest(glob.glob(os.path.join(INCLUDE, "*.h")))):
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    built_for = f"torch {torch.__version__}, Python {sysconfig.get_config_var('SOABI')}, C++11 ABI {abi}\n"
+    note = os.path.join(BUILD, "decode_binding.txt")
+    if not force and os.path.exists(BINDING) and os.path.exists(note) and open(note).read() == built_for and (
+            os.path.getmtime(BINDING) >= max(os.path.getmtime(src), _newest(glob.glob(os.path.join(INCLUDE, "*.h"))))):
         return BINDING
+    os.makedirs(BUILD, exist_ok=True)
     if not quiet:
         print("[build] decode_binding.cpp", flush=True)
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
@@ -62,10 +67,12 @@ def build_binding(force=False, quiet=False):
     # The compiler that nvcc links with: a module with a libstdc++ of its own in it must not meet
     # torch's.
     subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
-                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
                     *(f"-isystem{d}" for d in dirs), src, "-o", tmp, *(f"-L{d}" for d in library_paths()),
                     "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"], check=True)
     os.replace(tmp, BINDING)
+    with open(note, "w") as f:
+        f.write(built_for)
     return BINDING
 
 

@@ -41,3 +41,20 @@ def test_without_torch_the_library_is_built(compiler, monkeypatch, capsys):
     assert build.build() == build.LIB and os.path.exists(build.LIB)
     assert compiler == ["nvcc"] and not os.path.exists(build.BINDING)
     assert "no torch" in capsys.readouterr().out
+
+
+def test_the_binding_is_built_anew_for_another_torch_or_python(compiler, monkeypatch):
+    import sysconfig
+
+    import torch
+
+    build.build_binding(quiet=True)
+    assert compiler == ["g++"]
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    build.build_binding(quiet=True)
+    assert compiler == ["g++"] * 2
+    build.build_binding(quiet=True)
+    assert compiler == ["g++"] * 2
+    monkeypatch.setattr(sysconfig, "get_config_var", lambda name: "another")
+    build.build_binding(quiet=True)
+    assert compiler == ["g++"] * 3
