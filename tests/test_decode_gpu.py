@@ -150,6 +150,78 @@ def test_chain(cuda, shape, dt):
     assert w8.device_status() == 0
 
 
+# What few rows need more than one CTA's time for: all tiles of all sequences dealt to the resident
+# CTAs.  Each head size and row tile, more than 256 sequences (which a CTA looks through in rounds),
+# a window, and each of the three ways to join the pieces.
+DEALT = [
+    (300, 4, 1, 128, 1, 2100, [(7 * i * i) % 2101 for i in range(300)], 0),
+    (300, 4, 1, 64, 1, 8000, [(31 * i * i) % 8001 for i in range(300)], 0),
+    (300, 2, 1, 256, 1, 1500, [(7 * i * i) % 1501 for i in range(300)], 0),
+    (300, 2, 1, 512, 1, 1000, [(7 * i * i) % 1001 for i in range(300)], 0),
+    (600, 2, 1, 128, 1, 2100, [2100 - i for i in range(600)], 2000),
+    (10, 64, 4, 64, 1, 20000, [20000, 1, 7000, 19999, 8000, 8193, 0, 16384, 64, 12345], 8000),
+    (40, 64, 2, 128, 1, 2100, [(29 * i * i) % 2101 for i in range(40)], 0),
+    (20, 64, 4, 64, 2, 3000, [(67 * i * i) % 3001 for i in range(20)], 0),
+    (24, 8, 1, 256, 1, 5000, [5000 - 200 * i for i in range(24)], 0),
+    (1, 32, 1, 128, 1, 3000, [2999], 0),
+    (1, 16, 1, 64, 1, 9000, [9000], 0),
+    (1, 11, 1, 128, 2, 3000, [3000], 2500),
+]
+
+
+def is_dealt(B, H, KV, D, N, S, window):
+    """Few rows: only dealt tiles need a workspace when no weights are wanted."""
+    assert N * H // KV <= {64: 64, 128: 32}.get(D, 16)
+    return w8._lib.lib().w8_attention_tree_workspace_bytes(B, H, KV, D, S, N, window, 0) > 0
+
+
+@pytest.mark.parametrize("weights", [False, True], ids=["", "weights"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("shape", DEALT, ids=[str(i) for i in range(len(DEALT))])
+def test_dealt_tiles(cuda, shape, dt, weights):
+    B, H, KV, D, N, S, lens, window = shape
+    assert is_dealt(B, H, KV, D, N, S, window)
+    a = make(B + D + N, B, H, KV, D, N, S, lens, dt)
+    prev = torch.rand((B, KV, S), device="cuda") if weights else None
+    w = prev.clone() if weights else None
+    got = w8.attention_tree(*a, window=window, scale=D ** -0.5, weights=w)
+    want = want_attention(*a, window=window, scale=D ** -0.5)
+    check_out(got[0] if weights else got, want, dt)
+    if weights:
+        seen = torch.arange(S, device="cuda") < a[3][:, None, None]
+        exact = prev.double() + torch.where(seen, want[3], 0.0)
+        rel = 2 * want[5] + (N * H // KV + 4) * 2.0 ** -24 + 2.0 ** -21
+        assert ((w.double() - exact).abs() <= torch.where(seen, rel * want[3] + 2.0 ** -23 * exact, 0.0)).all()
+        assert ((got[2].double() - want[4]).abs() <= rel * want[4] + 1e-30).all()
+    assert w8.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(60, 4, 1, 128, 40, 1000), (60, 4, 1, 64, 40, 2000), (60, 4, 1, 256, 20, 700)], ids=str)
+def test_expanded_caches_of_many_row_tiles(cuda, shape):
+    """One cache for 60 sequences of several row tiles each: no TMA, rounds of pairs, tiles dealt."""
+    B, H, KV, D, N, S = shape
+    q, k, v, ln, kn, vn = make(D, B, H, KV, D, N, S, [S] * B)
+    k, v = k[:1].expand(B, KV, S, D), v[:1].expand(B, KV, S, D)
+    ln = torch.tensor([(7 * i * i) % (S + 1) for i in range(B)], dtype=torch.int32, device="cuda")
+    got = w8.attention_tree(q, k, v, ln, kn, vn, scale=D ** -0.5)
+    check_out(got, want_attention(q, k, v, ln, kn, vn, scale=D ** -0.5), torch.bfloat16)
+
+
+# Many rows: a key axis split between clusters, of one and of two row tiles.
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("shape", [(1, 8, 1, 512, 20, 4000, [3999], 0), (1, 8, 1, 512, 40, 1500, [1500], 0), (1, 8, 1, 128, 64, 4000, [3900], 0),
+                                   (2, 6, 1, 256, 50, 3000, [2900, 17], 2000)], ids=str)
+def test_split_keys_of_many_rows(cuda, shape, dt):
+    B, H, KV, D, N, S, lens, window = shape
+    a = make(B + D + N, B, H, KV, D, N, S, lens, dt)
+    w = torch.zeros((B, KV, S), device="cuda")
+    got, w, _ = w8.attention_tree(*a, window=window, scale=D ** -0.5, weights=w)
+    want = want_attention(*a, window=window, scale=D ** -0.5)
+    check_out(got, want, dt)
+    rel = 2 * want[5] + (N * H // KV + 4) * 2.0 ** -24 + 2.0 ** -21
+    assert ((w.double() - want[3]).abs() <= (rel + 2.0 ** -23) * want[3]).all()
+
+
 TREES = [
     (2, 8, 1, 256, 24, 300, [300, 0], 0, 0),
     (2, 8, 2, 128, 64, 150, [150, 77], 0, 5),
@@ -718,6 +790,28 @@ def test_select_segments_that_nearly_fill_the_candidates(cuda, found, n):
     for _ in range(20):
         got = w8.beam_select(logits, scores, n=n)
     check_select(got, want_select(logits, scores, None, 0, n, 0.0, "score"), 2.0, V, 0.0)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("n", [4, 64])
+@pytest.mark.parametrize("kind", ["random", "late", "ties"])
+def test_select_in_several_collections(cuda, kind, n, dt):
+    """Chunks of more than 24 tiles, whose later collections start from the candidates of the first:
+    random logits, the best in the later tiles, and few values (ties across the collections)."""
+    B, K, V, tile = 50, 8, 262144, 4096
+    ws = w8._lib.lib().w8_beam_select_workspace_bytes(B, K, V, n)
+    chunks = ws // (B * K * (n * 8 + 8))
+    assert V // tile // chunks > 24
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    logits = rows(gen, (B, K, V), torch.float32, 4.0)
+    if kind == "late":
+        logits += 3.0 * ((torch.arange(V, device="cuda") // tile) % (V // tile // chunks) >= 24)
+    if kind == "ties":
+        logits = logits.round().clamp(max=11.0)
+    logits = logits.to(dt)
+    scores = torch.randn((B, K), generator=gen, device="cuda") - 9
+    got = w8.beam_select(logits, scores, n=n)
+    check_select(got, want_select(logits, scores, None, 0, n, 0.0, "score"), 28.0, V, 0.0)
 
 
 REORDERS = [(1, 4, 1, 256, 100, 3), (2, 3, 2, 64, 33, 1), (3, 8, 2, 128, 64, 5), (1, 32, 1, 64, 17, 2), (2, 16, 3, 64, 50, 70), (4, 1, 1, 64, 5, 1)]
