@@ -180,7 +180,8 @@ def last_schedule():
 
 
 def device_status(clear=True):
-    """Sticky device-side status (syncs the device); raises W8DeviceTimeout if a wait gave up."""
+    """Sticky device-side status (syncs the device); raises W8DeviceTimeout if a wait gave up,
+    W8InvalidArgument if a length or index in device memory lay outside its range."""
     st = lib().w8_device_status(1 if clear else 0)
     if st == W8_ERR_DEVICE_TIMEOUT:
         raise W8DeviceTimeout(st, "device", "a bounded device-side wait timed out")

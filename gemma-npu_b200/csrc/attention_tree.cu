@@ -20,14 +20,16 @@
 // accumulator's layout into the operand's in place, and no warp waits for another until the end
 // of the item, where the 8 results are joined.  (Warps that shared each tile, exchanging P and
 // the maxima through shared memory with three barriers a tile, executed 6 times the
-// instructions.)  Reading 32 sequences of 2048 to 8191 keys, 8 heads of 128: 118 us, 5.7 TB/s;
-// equal lengths 6.5 TB/s, heads of 256 6.7 TB/s.
+// instructions.)  32 sequences of 2048 to 8191 keys, 8 heads of 128 (671 MB) take 112 us with the
+// joining of their pieces, 6.0 TB/s; of 8191 keys each 162 us, 6.6 TB/s, heads of 256 6.7 TB/s.
 //
 // The work is cut by what is there: all tiles of all sequences, in order, are dealt in equal
 // contiguous ranges to as many CTAs as fit the GPU at once (every CTA adds up the lengths for
 // itself), so ragged lengths leave no SM idle and a single long sequence fills them all.  A
 // CTA writes the items that it holds whole, and partial (m, l, O) of at most two others, which
-// attn_tree_combine_kernel joins.
+// attn_tree_combine_kernel joins.  (A cache that sequences share by expansion has no tensor map and
+// is read by cp.async, once for every sequence: 40 sequences over one cache of 4000 slots, 8 heads of
+// 128, take 167 us where 40 caches of their own take 106.)
 #include "attention_tree.cuh"
 #include "attn_tc.cuh"
 
@@ -928,8 +930,12 @@ static TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_
   p.splits = 1;
   if (p.tc) {
     // The number of splits with the least estimated time: waves of clusters, each 1.6 us a tile
-    // and 8 us besides, then 4 us and the partials at 3 TB/s to join them (measured on trees
-    // of 64 drafts at D 256).
+    // and 8 us besides, then 4 us and the partials at 3 TB/s to join them.  Measured on trees of 64
+    // drafts at D 256, which other head sizes share though it does not fit them as well (320 items
+    // of 1000 keys at D 512: 201 us estimated, 276 measured), and with lengths near the capacity,
+    // which is all that the host knows: sequences that fill little of a large cache are split into
+    // more pieces than they have tiles (the tree of 60 over 4000 slots of 4096 takes 65 us, of 131072
+    // 159).
     const int64_t width = d == 512 ? 2 : 1, pairs = sms / 2;
     double best = 0;
     for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64); ++s) {

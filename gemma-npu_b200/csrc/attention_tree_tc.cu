@@ -10,7 +10,7 @@
 //   O   += P_j V_j     A = P_j from TMEM, each CTA staging half of V's columns
 // m moves only when a tile's maximum exceeds it by enough (TreeRef).  Many rows per
 // key make this bound by the MMAs and the softmax's exponentials, not by HBM: trees of 64
-// drafts for 16 sequences, D 256, 8 heads a group, 2000 to 4000 keys take 65 us here (a tile
+// drafts for 16 sequences, D 256, 8 heads a group, 2000 to 4000 keys take 64 us here (a tile
 // some 2650 clocks of a pair, its MMAs 2048) and 672 with mma.sync.  The key axis is split over
 // clusters while they would leave SMs idle, and the partial outputs joined by the combine
 // kernel of attention_tree.cu.

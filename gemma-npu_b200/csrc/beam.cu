@@ -14,9 +14,12 @@
 // 64 bits and merges the beams.
 //
 // The bytes are the logits once, but a logit's softcap and exponential cost more issue slots
-// than its bytes: 24 x 8 beams of 262144 bf16 logits, softcapped, take 34 us (3.0 TB/s) and
-// the merge 8 us; the stream with a tanh of the special-function unit, or with comparisons of
-// every logit against a threshold and barriers between tiles, took 76 us.
+// than its bytes: 24 x 8 beams of 262144 bf16 logits, softcapped, take 47 us, the merge's 8 among
+// them (100.7 MB, 2.6 TB/s of the rest), and 43 us with 29 of the 192 finished, whose logits are not
+// read; the stream with a tanh of the special-function unit, or with comparisons of every logit
+// against a threshold and barriers between tiles, took 76 us.  So it still does, 71 to 76 us, where
+// most segments hold a logit above the cap, with caps below 0.01 or above 1000, and with rows that
+// are not 16-byte aligned (an odd vocabulary), which are loaded a logit at a time.
 #include "common.cuh"
 
 #include <cuda_fp16.h>

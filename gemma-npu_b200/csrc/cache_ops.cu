@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kEvictThreads, KPT <= 32 ? 2 : 1) evict_select
 // between the bounds (every warp writes its counts into all CTAs' shared memory, one barrier a
 // step).  Evicted slots meet their movers through the list that the moves read too, and a
 // slot's weight and position are read by one thread only, so the cut may be in place.  One row
-// of 16001 slots 17 us where one CTA takes 30, of 40000 32 where evict_select_long_kernel takes
+// of 16001 slots 17 us where one CTA takes 30, of 40000 27 where evict_select_long_kernel takes
 // 115; 144 rows of 16001 slots, which fill the SMs by themselves, 58 and more against 56.
 template <int KPT>
 __global__ void __launch_bounds__(kEvictThreads, KPT <= 16 ? 2 : 1) evict_select_cluster_kernel(const EvictArgs a) {
@@ -742,7 +742,7 @@ constexpr int kMoveChunks = 4;  // 16-byte chunks of a thread in flight
 // The moves of one (sequence, head): destinations (below the budget) and sources (behind
 // it) are disjoint, so the rows move in place in any order.  Bound by HBM and its rows' order: a
 // CTA's 1024 chunks are all loaded before the first is stored (24 sequences of 8 heads of 128,
-// up to 16001 slots cut to 4096: some 70 us, 5 TB/s of single rows of 256 bytes).
+// up to 16001 slots cut to 4096: some 70 us, 4.6 TB/s of single rows of 256 bytes).
 __global__ void __launch_bounds__(256) evict_move_kernel(const MoveArgs a) {
   const int row = blockIdx.y, b = row / a.kv_heads, c = row % a.kv_heads;
   pdl_launch_dependents();
