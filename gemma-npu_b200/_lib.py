@@ -129,6 +129,11 @@ SIGNATURES.update({
                             _p]),
     "w8_beam_select_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "w8_cache_reorder": (_i, [_p, _i64, _p, _p, _i, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "w8_attention_paged": (_i, [_p, _p, _i64, _p]),
+    "w8_attention_paged_workspace_bytes": (_i64, [_p]),
+    "w8_paged_append": (_i, [_p, _p]),
+    "w8_page_assign": (_i, [_p, _p]),
+    "w8_draft_verify": (_i, [_p, _p]),
 })
 
 # Element type codes.

@@ -19,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -83,7 +84,7 @@ def build(force=False, verbose_ptxas=False, quiet=False):
     sources = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     headers = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
     hdr_time = _newest(headers)
-    objs = []
+    objs, stale = [], []
     for src in sources:
         obj = os.path.join(BUILD, os.path.basename(src)[:-3] + ".o")
         objs.append(obj)
@@ -92,9 +93,15 @@ def build(force=False, verbose_ptxas=False, quiet=False):
         cmd = [nvcc, *ARCH, *NVCC_FLAGS, "-c", src, "-o", obj]
         if verbose_ptxas:
             cmd.insert(1, "-Xptxas=-v")
+        stale.append((src, cmd))
+
+    def compile_one(job):
         if not quiet:
-            print("[build]", os.path.basename(src), flush=True)
-        subprocess.run(cmd, check=True)
+            print("[build]", os.path.basename(job[0]), flush=True)
+        subprocess.run(job[1], check=True)
+
+    with ThreadPoolExecutor(max(1, os.cpu_count() or 1)) as pool:
+        list(pool.map(compile_one, stale))
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < _newest(objs):
         tmp = LIB + ".tmp"
         subprocess.run([nvcc, *ARCH, "-shared", "-o", tmp, *objs], check=True)

@@ -1,0 +1,1127 @@
+// Attention of new tokens (one, a chunk or a drafted tree) over a paged 8-bit cache: the
+// contract of attention_tree.cu, with the committed keys and values where a serving cache keeps
+// them.  The reference attends to 16-bit keys that it concatenates (pipeline.py:133-180,
+// local_attn.py:44-83).
+//
+// Per sequence b and cache head c, R = G N query rows share the keys
+//   k_j = ks[page, c] k8_j,  v_j = vs[page, c] v8_j   (full pages, signed 8 bits)
+// then the 16-bit rows of the partial page and of the new tokens:
+//   x_rj = scale q_r . k_j,   p = softmax over the keys row r may see,   o_r = sum_j p_rj v_j
+//
+// Decode reads each key once for few rows and is bound by HBM, at half the bytes of a 16-bit
+// cache, so the unpacking has to keep up with 23 values a clock and SM.  Both products run as
+// fp16 mma.sync with fp32 sums.  A thread's 4 neighbouring bytes become 4 fp16 values in 5
+// instructions (paged_unpack, exact), and are one B operand of 16 x 8 as they are if the order
+// of the reduction is permuted alike on both sides: the columns of Q when it is staged for K,
+// and for V the columns of the output, which a thread then holds as 4 neighbours (`natural`
+// puts them back in order, once an item).  Q is scaled by a power of two a row into fp16's range
+// (largest element 2^14: what falls below 2^-24 is 2^-38 of that).  ks multiplies the scores; vs
+// goes into P relative to a power of two not below any vs so far (paged_unit), in which unit O is
+// held: O is rescaled when that grows or a row's maximum does, and P is rounded to fp16, half a
+// step of 2^-11 on each weight (TreeRef has the range).
+//
+// The schedule is attention_tree.cu's: all tiles of all sequences dealt in equal contiguous
+// ranges to the CTAs, each of 8 warps 16 keys at a time with a running softmax of its own, joined
+// at the end of an item; pieces joined by attn_tree_combine_kernel.  A ninth warp walks the page
+// table ahead, a page a lane: TMA boxes of a page's rows into the ring, and its scales.  Pages
+// that no row sees are not read (nor their table entries followed), so a window's old pages may
+// be gone.
+#include "attention_paged.cuh"
+#include "attn_mma.cuh"
+#include "attn_tc.cuh"
+
+#include <algorithm>
+
+namespace w8 {
+
+// Two warpgroups of 8 working warps and one whose first warp loads.  168 registers a thread at
+// launch (12 warps), dealt as 216 to the working ones and 72 to the others: 64512 both ways.
+constexpr int kPagedWarps = kTreeWarps + 4;
+constexpr int kPagedThreads = 32 * kPagedWarps;
+__device__ __forceinline__ void paged_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
+__device__ __forceinline__ void paged_fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
+
+template <int D, int MT>
+struct PagedCfg {
+  static constexpr int kBM = 16 * MT;
+  static constexpr int kTeam = D == 512 ? 2 : 1;           // warps that share 16 keys
+  static constexpr int kGroups = kTreeWarps / kTeam;
+  static constexpr int kSteps = D == 64 ? 2 : 1;           // 16-key steps of a warp in a tile
+  static constexpr int kBN = kGroups * kSteps * 16;        // keys of a tile of pages: 256, 128, 128, 64
+  static constexpr int kBN16 = kBN / 2;                    // of a 16-bit tile, which is as large
+  static constexpr int kSlotBytes = kBN * D;               // 16 KB (D <= 128) or 32 KB
+  static constexpr int kSlots = 196608 / kSlotBytes;
+  static constexpr int kPitch = D + 8;                     // fp32 row pitch of the joint outputs
+  static constexpr int kOffQ8 = kSlots * kSlotBytes;       // Q as fp16, scaled and permuted
+  static constexpr int kOffQ16 = kOffQ8 + kBM * D * 2;     // Q as it is
+  static constexpr int kOffStat = kOffQ16 + kBM * D * 2;   // float [2][kGroups][kBM]: maxima, sums
+  static constexpr int kOffFac = kOffStat + 2 * kGroups * kBM * 4;  // float [kBM]: Q's scale taken back
+  static constexpr int kOffScale = kOffFac + kBM * 4;      // float [kSlots][kPagedMaxBoxes]
+  static constexpr int kOffMask = kOffScale + kSlots * kPagedMaxBoxes * 4;  // uint32 [kSlots]: boxes that are there
+  static constexpr int kOffBar = kOffMask + kSlots * 4;
+  static constexpr int kNumBars = 2 * kSlots;              // full, empty
+  static constexpr int kSmem = kOffBar + kNumBars * 8 + 16 + 1024;
+  static_assert(kSmem <= 232448, "shared memory budget exceeded");
+  static_assert(kGroups * kBM * kPitch * 4 <= kOffQ8, "the joint outputs fit over the ring");
+  static_assert(kOffBar % 8 == 0 && kOffScale % 16 == 0, "alignment");
+};
+
+__device__ __forceinline__ float paged_ks(const PagedArgs& a, int page, int c) { return a.ks[page * a.ks_p + c * a.ks_h]; }
+__device__ __forceinline__ float paged_vs(const PagedArgs& a, int page, int c) { return a.vs[page * a.vs_p + c * a.vs_h]; }
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kPagedThreads, 1)
+    attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                      const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
+                      const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_vn,
+                      const __grid_constant__ PagedArgs pa) {
+  using C = PagedCfg<D, MT>;
+  using H = __half;
+  constexpr int BM = C::kBM, BN = C::kBN, BN16 = C::kBN16, NS = C::kSlots, CH = D / 8;  // CH: 16-byte chunks of a 16-bit row
+  constexpr int DW = D / C::kTeam;                   // output columns of a warp
+  constexpr bool kQRegs = MT == 1 && D <= 128;       // Q's fragments stay in registers
+  constexpr int kRowBytes = D < 128 ? D : 128;       // of a box's row in shared memory
+  const TreeArgs& a = pa.t;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const uint32_t sq8 = base + C::kOffQ8, sq16 = base + C::kOffQ16, bar0 = base + C::kOffBar;
+  float* stat = reinterpret_cast<float*>(smem + C::kOffStat);
+  float* qfac = reinterpret_cast<float*>(smem + C::kOffFac);
+  volatile float* scales = reinterpret_cast<volatile float*>(smem + C::kOffScale);
+  volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(smem + C::kOffMask);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffBar + C::kNumBars * 8);
+  auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (NS + s); };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rows = a.group * a.n;
+  const int box_shift = min(pa.shift, 31 - __clz(BN)), box = 1 << box_shift;  // keys of a box
+  const int boxes = BN >> box_shift;
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(full_bar(s), 1);  // the producer's arrive.expect_tx
+      mbar_init(empty_bar(s), kTreeWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    prefetch_tmap(&tm_kt);
+    prefetch_tmap(&tm_vt);
+    prefetch_tmap(&tm_kn);
+    prefetch_tmap(&tm_vn);
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  // ---- this CTA's range of all tiles.  A pair (sequence, row tile) has kv_heads items of
+  // `nt` tiles each; pairs and their heads follow one another.
+  const int pairs = a.batch * a.row_tiles;
+  auto split_pair = [&](int p, int& b, int& rt) {
+    b = p, rt = 0;
+    if (a.row_tiles > 1) b = p / a.row_tiles, rt = p - b * a.row_tiles;
+  };
+  int b, rt, c = 0, len;
+  PagedSpan span;
+  long long pos = 0, stop = 0, item_pos = 0;  // item_pos: first tile of the current item
+  TreeDeal deal = {1, 0};
+  if (a.direct || pairs == 1) {
+    // One item (this CTA's number's), or those of one pair.
+    int p = 0;
+    if (a.direct) {
+      p = static_cast<int>(blockIdx.x);
+      if (a.kv_heads > 1) p = blockIdx.x / a.kv_heads, c = blockIdx.x - p * a.kv_heads;
+    }
+    split_pair(p, b, rt);
+    len = tree_len(a, b);
+    span = paged_span<BM, BN, BN16>(pa, len, rt);
+    const int tiles = span.tiles();
+    if (a.direct) {
+      stop = tiles;
+    } else {
+      const long long total = static_cast<long long>(tiles) * a.kv_heads;
+      const uint32_t ctas = total < gridDim.x ? static_cast<uint32_t>(total) : gridDim.x;
+      if (blockIdx.x >= ctas) return;
+      deal.each = div_short(total, ctas);
+      deal.more = total - deal.each * ctas;
+      pos = deal_begin(deal, blockIdx.x);
+      stop = deal_begin(deal, blockIdx.x + 1);
+      c = static_cast<int>(div_short(pos, tiles));
+      item_pos = static_cast<long long>(c) * tiles;
+    }
+    __syncthreads();  // the barriers are initialised
+  } else {
+    auto pair_tiles = [&](int p) {
+      int pb, prt;
+      split_pair(p, pb, prt);
+      return paged_span<BM, BN, BN16>(pa, tree_len(a, pb), prt).tiles();
+    };
+    long long* sched = reinterpret_cast<long long*>(smem);  // (the ring is not in use yet)
+    long long sum = 0, round;
+    for (int p = tid; p < pairs; p += kPagedThreads) sum += pair_tiles(p);
+    long long excl = block_scan<kPagedWarps>(sum, sched, round);  // (of few pairs also each one's place)
+    const long long total = round * a.kv_heads;
+    const uint32_t ctas = total < gridDim.x ? static_cast<uint32_t>(total) : gridDim.x;
+    if (blockIdx.x >= ctas) return;
+    deal.each = div_short(total, ctas);
+    deal.more = total - deal.each * ctas;
+    pos = deal_begin(deal, blockIdx.x);
+    stop = deal_begin(deal, blockIdx.x + 1);
+    // The pair that holds `pos`: a running sum over rounds of pairs.
+    long long before = 0;
+    for (int p0 = 0;; p0 += kPagedThreads) {
+      const int p = p0 + tid;
+      long long nt = sum;
+      if (pairs > kPagedThreads) {
+        nt = p < pairs ? pair_tiles(p) : 0;
+        excl = before + block_scan<kPagedWarps>(nt, sched, round);
+      }
+      if (nt > 0 && excl * a.kv_heads <= pos && pos < (excl + nt) * a.kv_heads) {
+        sched[16] = p;
+        sched[17] = excl * a.kv_heads;
+      }
+      __syncthreads();
+      before += round;
+      if (pos < before * a.kv_heads) break;  // (every pair has tiles, and pos < total)
+      if (p0 + kPagedThreads >= pairs) return;  // only if the lengths changed under the call
+    }
+    split_pair(static_cast<int>(sched[16]), b, rt);
+    item_pos = sched[17];
+    len = tree_len(a, b);
+    span = paged_span<BM, BN, BN16>(pa, len, rt);
+    const int tiles = span.tiles();
+    c = static_cast<int>(div_short(pos - item_pos, tiles));
+    item_pos += static_cast<long long>(c) * tiles;
+    fence_proxy_async_smem();  // the TMA writes the ring next
+    __syncthreads();
+  }
+  int nt = span.tiles();
+  // The next item: the next head, or the next pair's first.
+  auto advance = [&]() {
+    item_pos += nt;
+    if (++c == a.kv_heads) {
+      c = 0;
+      if (++rt == a.row_tiles) {
+        rt = 0;
+        ++b;
+        len = tree_len(a, b);
+      }
+      span = paged_span<BM, BN, BN16>(pa, len, rt);
+      nt = span.tiles();
+    }
+  };
+  // Tile t of the item: its first key (of its kind).
+  enum : int { kPages = 0, kTail = 1, kNew = 2 };
+  auto kind_of = [&](int t) { return t < span.pages() ? kPages : t < span.pages() + span.tail ? kTail : kNew; };
+  auto key0_of = [&](int t) {
+    if (t < span.ns) return t * BN;
+    if (t < span.pages()) return (span.c0 + t - span.ns) * BN;
+    t -= span.pages();
+    return (t < span.tail ? t : t - span.tail) * BN16;
+  };
+
+  auto rows_sync = [&]() {  // of the 8 warps without the producer
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(kTreeThreads) : "memory");
+  };
+  auto rows_sync_and = [&](bool on) {
+    uint32_t all;
+    __syncwarp();
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "bar.red.and.pred p, 1, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all)
+        : "r"(on ? 1u : 0u), "n"(kTreeThreads)
+        : "memory");
+    return all != 0u;
+  };
+  const int grp = warp / C::kTeam, part = warp % C::kTeam;  // 16-key group of a step; column part
+  const int rl = lane >> 2, arow = lane & 15;
+  uint32_t g = 0;  // ring steps so far (each tile's K, then V)
+  bool ok = true;
+  // Between items the producer and the 8 warps meet twice: everybody has left the ring (and no wait
+  // gave up), and it may be filled again.
+  auto item_done = [&](bool on) {
+    uint32_t all;
+    __syncwarp();
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "bar.red.and.pred p, 2, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all)
+        : "r"(on ? 1u : 0u), "n"(kTreeThreads + 32)
+        : "memory");
+    return all != 0u;
+  };
+  auto item_free = [&]() {
+    __syncwarp();
+    asm volatile("bar.sync 3, %0;" ::"n"(kTreeThreads + 32) : "memory");
+  };
+  __syncwarp();
+  if (warp >= kTreeWarps) {
+    // ---- the producer: each tile's K and V boxes into the ring as its slots are left, the table
+    // entries and scales of the next tile under way meanwhile.
+    paged_fewer_registers();
+    if (warp > kTreeWarps) return;
+    while (true) {
+      const int t0 = static_cast<int>(pos - item_pos);
+      const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
+      const int* table = pa.table + b * pa.table_b;
+      // Lane j's box of tile t: its page, or -1 (not a page tile, nothing there that a row sees).
+      auto page_of = [&](int t) {
+        if (t >= t1 || kind_of(t) != kPages || lane >= boxes) return -1;
+        const int k0 = key0_of(t) + (lane << box_shift);
+        if (!paged_needs(pa, span, k0, k0 + box)) return -1;
+        const int p = table[k0 >> pa.shift];
+        if (p < 0 || p >= pa.pages) {
+          atomicExch(&g_tree_status, W8_ERR_INVALID_ARG);
+          return -1;
+        }
+        return p;
+      };
+      int page = page_of(t0);
+      float ks = page >= 0 ? paged_ks(pa, page, c) : 0.f, vs = page >= 0 ? paged_vs(pa, page, c) : 0.f;
+      bool put = true;
+      for (int t = t0; t < t1 && put; ++t) {
+        const int kind = kind_of(t), key0 = key0_of(t);
+        const int next = page_of(t + 1);
+        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t step = g + 2 * (t - t0) + kv, slot = step % NS, dst = base + slot * C::kSlotBytes;
+          put = put && mbar_wait_bounded(empty_bar(slot), ((step / NS) & 1u) ^ 1u, abort_flag, &g_tree_status);
+          put = __all_sync(0xffffffffu, put);
+          if (!put) break;
+          if (kind == kPages) {
+            if (lane < boxes) scales[slot * kPagedMaxBoxes + lane] = kv ? vs : ks;
+            if (lane == 0) masks[slot] = there;
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(full_bar(slot), __popc(there) * (box * D));
+            __syncwarp();
+            if (page >= 0)
+              tma_load_5d(dst + lane * (box * D), kv ? &tm_v : &tm_k, full_bar(slot), 0,
+                          (key0 + (lane << box_shift)) & ((1 << pa.shift) - 1), 0, c, page);
+          } else if (lane == 0) {
+            mbar_arrive_expect_tx(full_bar(slot), C::kSlotBytes);
+            const CUtensorMap* map = kind == kTail ? (kv ? &tm_vt : &tm_kt) : (kv ? &tm_vn : &tm_kn);
+            tma_load_5d(dst, map, full_bar(slot), 0, key0, 0, c, b);
+          }
+          __syncwarp();
+        }
+        page = next;
+        if (page >= 0) ks = paged_ks(pa, page, c), vs = paged_vs(pa, page, c);
+      }
+      ok = put;
+      g += 2 * (t1 - t0);
+      if (!item_done(ok)) break;
+      pos += t1 - t0;
+      if (pos >= stop) break;
+      advance();
+      item_free();
+    }
+    if (!ok) {
+      // A wait gave up: let the copies in flight land before the CTA exits.
+      const unsigned long long since = globaltimer();
+      while (globaltimer() - since < 50000ull) {
+      }
+    }
+  } else {
+    paged_more_registers();
+    while (true) {
+      const int row0 = rt * BM, bc = b * a.kv_heads + c;
+      const int t0 = static_cast<int>(pos - item_pos);
+      const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
+      const bool whole = t0 == 0 && t1 == nt;
+      const int64_t part_row = (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * BM;
+      const int sink_left = a.sink - len;
+      if (t0 == 0 && tid == 0 && !a.direct) {
+        // The CTA that begins an item says where its pieces are: one in each CTA up to its last tile's.
+        const int last = deal_owner(deal, item_pos + nt - 1);
+        a.info[bc * a.row_tiles + rt] = make_int2(blockIdx.x, last - static_cast<int>(blockIdx.x) + 1);
+      }
+      // Q rows r = i * group + g (query head c * group + g of new token i).
+      for (int e = tid; e < BM * CH; e += kTreeThreads) {
+        const int r = e / CH, ch = e % CH;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (row0 + r < rows) {
+          int i, gq;
+          tree_row(a, row0 + r, i, gq);
+          w = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + gq) * a.q_h +
+                                              i * a.q_t + ch * 8);
+        }
+        st_shared_v4(sq16 + r * (D * 2) + ((ch ^ (r & 7)) << 4), w.x, w.y, w.z, w.w);
+      }
+      rows_sync();
+      // The same scaled into fp16's range, 16 columns at a time in the order in which a thread's 4
+      // bytes of K come: columns 4 t .. 4 t + 3 as elements 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+      for (int r = warp; r < BM; r += kTreeWarps) {
+        float most = 0.f;
+        uint4 w[(CH + 31) / 32];
+#pragma unroll
+        for (int x = 0; x < (CH + 31) / 32; ++x) {
+          const int ch = lane + 32 * x;
+          w[x] = make_uint4(0, 0, 0, 0);
+          if (ch < CH) w[x] = *reinterpret_cast<const uint4*>(smem + C::kOffQ16 + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+          const uint32_t ws[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            most = fmaxf(most, fmaxf(fabsf(tree_f32<T>(ws[e] & 0xFFFFu)), fabsf(tree_f32<T>(ws[e] >> 16))));
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        // 2^(14 - exponent), at most 2^100; 1 for a row of zeros or infinities.
+        const int ex = static_cast<int>(__float_as_uint(most) >> 23);
+        const int up = ex == 0 || ex == 255 ? 0 : min(14 + 127 - ex, 100);
+        const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+        if (lane == 0) qfac[r] = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+#pragma unroll
+        for (int x = 0; x < (CH + 31) / 32; ++x) {
+          const int ch = lane + 32 * x;
+          if (ch >= CH) break;
+          const uint32_t ws[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+          uint32_t h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h[e] = pack2<H>(tree_f32<T>(ws[e] & 0xFFFFu) * f, tree_f32<T>(ws[e] >> 16) * f);
+          uint8_t* row = smem + C::kOffQ8 + r * (D * 2) + 8 * (ch & 1);
+          *reinterpret_cast<uint2*>(row + (((ch & ~1) ^ (r & 7)) << 4)) = make_uint2(h[0], h[2]);
+          *reinterpret_cast<uint2*>(row + (((ch | 1) ^ (r & 7)) << 4)) = make_uint2(h[1], h[3]);
+        }
+      }
+      float m[MT][2], l[MT][2];
+      float o[MT][DW / 8][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) m[mt][h] = -INFINITY, l[mt][h] = 0.f;
+#pragma unroll
+        for (int n = 0; n < DW / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+      }
+      // This thread's rows of each 16-row tile: lane / 4 and lane / 4 + 8.
+      int tok[MT][2], dep[MT][2], first[MT][2];
+      float fac[MT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = row0 + mt * 16 + rl + 8 * h;
+          int gq;
+          tree_row(a, r, tok[mt][h], gq);
+          if (r >= rows) tok[mt][h] = -1;
+          dep[mt][h] = r < rows ? tree_depth(a, b, tok[mt][h]) : 0;
+          first[mt][h] = r < rows ? tree_first(a, len, dep[mt][h]) : INT32_MAX;  // (no row: sees nothing)
+        }
+      rows_sync();
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) fac[mt][h] = qfac[mt * 16 + rl + 8 * h] * a.scale_log2;
+      uint32_t qf[kQRegs ? D / 16 : 1][4];
+      if constexpr (kQRegs) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          ldsm_x4(sq8 + arow * (D * 2) + (((2 * kk + (lane >> 4)) ^ (arow & 7)) << 4), qf[kk]);
+      }
+      // The committed positions p0 .. p0 + 15 below `end` that a row sees, as bits.
+      auto sees = [&](int mt, int h, int p0, int end) {
+        const int hi = min(end - p0, 16);
+        uint32_t bits = hi <= 0 ? 0u : (1u << hi) - 1u;
+        const int lo = first[mt][h] - p0;
+        if (lo > 0) {
+          uint32_t on = lo > 15 ? 0u : 0xFFFFFFFFu << lo;
+          const int sk = tok[mt][h] < 0 ? 0 : min(a.sink - p0, 16);
+          if (sk > 0) on |= (1u << sk) - 1u;
+          bits &= on;
+        }
+        return bits;
+      };
+      // Scores to weights: a row's maximum of the step, m moved if it must be, O and l with it by
+      // `unit` (the change of O's unit) besides.
+      auto move_rows = [&](const float (&mx)[MT][2], float unit) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const bool mv = mx[mt][h] > m[mt][h] + TreeRef<H>::kSlack;
+            const float to = mx[mt][h] - TreeRef<H>::kBelow;
+            const float corr = mv ? ex2_tree(m[mt][h] - to) : 1.f;
+            if (mv) m[mt][h] = to;
+            l[mt][h] *= corr;
+            const float f = corr * unit;
+#pragma unroll
+            for (int n = 0; n < DW / 8; ++n) {
+              o[mt][n][2 * h] *= f;
+              o[mt][n][2 * h + 1] *= f;
+            }
+          }
+      };
+      float unit = __uint_as_float(0x00800000u);  // of O (2^-126: nothing added yet)
+      bool permuted = true;
+      // O in order and in units of 1: of each 16 columns a thread holds 4 t .. 4 t + 3 (the 8-column
+      // accumulators as even and odd columns) and gets 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t.
+      auto natural = [&]() {
+        permuted = false;
+        const int s0 = (lane & ~3) | ((lane & 3) >> 1), s1 = s0 + 2;
+        const bool up = lane & 1;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int n = 0; n < DW / 8; n += 2)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float v0 = o[mt][n][2 * h] * unit, v1 = o[mt][n + 1][2 * h] * unit;
+              const float v2 = o[mt][n][2 * h + 1] * unit, v3 = o[mt][n + 1][2 * h + 1] * unit;
+              const float a0 = __shfl_sync(0xffffffffu, v0, s0), a2 = __shfl_sync(0xffffffffu, v2, s0);
+              const float a1 = __shfl_sync(0xffffffffu, v1, s0), a3 = __shfl_sync(0xffffffffu, v3, s0);
+              const float b0 = __shfl_sync(0xffffffffu, v0, s1), b2 = __shfl_sync(0xffffffffu, v2, s1);
+              const float b1 = __shfl_sync(0xffffffffu, v1, s1), b3 = __shfl_sync(0xffffffffu, v3, s1);
+              o[mt][n][2 * h] = up ? a2 : a0;
+              o[mt][n][2 * h + 1] = up ? a3 : a1;
+              o[mt][n + 1][2 * h] = up ? b2 : b0;
+              o[mt][n + 1][2 * h + 1] = up ? b3 : b1;
+            }
+      };
+      const int col = (lane & 3) * 2;  // a thread's columns of an 8-column tile: col, col + 1
+
+#pragma unroll 1
+      for (int t = t0; t < t1; ++t, g += 2) {
+        const int kind = kind_of(t), tile0 = key0_of(t);
+        const uint32_t slot_k = g % NS, slot_v = (g + 1) % NS;
+        const uint32_t sk = base + slot_k * C::kSlotBytes, sv = base + slot_v * C::kSlotBytes;
+        if (ok) ok = mbar_wait_bounded(full_bar(slot_k), (g / NS) & 1u, abort_flag, &g_tree_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (kind == kPages) {
+          const uint32_t there = masks[slot_k];
+#pragma unroll
+          for (int st = 0; st < C::kSteps; ++st) {
+            const int kr = (grp * C::kSteps + st) * 16, key0 = tile0 + kr;  // this step's keys
+            const int bx = kr >> box_shift, br = kr & (box - 1);            // their box, and row in it
+            const uint32_t kbox = sk + bx * (box * D), vbox = sv + bx * (box * D);
+            // ---- S = Q K^T, 16 keys; a chunk of 16 bytes is one step of the reduction
+            float s[MT][2][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) s[mt][e >> 2][e & 3] = 0.f;
+            const int krow = br + ((lane >> 4) << 3) + (lane & 7);
+#pragma unroll
+            for (int k2 = 0; k2 < D / 32; ++k2) {
+              uint32_t kb[4];
+              const int ch = 2 * k2 + ((lane >> 3) & 1);
+              if constexpr (D >= 128)
+                ldsm_x4(kbox + (ch >> 3) * (box * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), kb);
+              else
+                ldsm_x4(kbox + krow * kRowBytes + ((ch ^ ((krow >> 1) & 3)) << 4), kb);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t b00, b01, b10, b11;
+                paged_unpack<H>(kb[e], 0x4140u, 0x4342u, b00, b01);
+                paged_unpack<H>(kb[2 + e], 0x4140u, 0x4342u, b10, b11);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  if constexpr (kQRegs) {
+                    mma16816<H>(s[mt][0], qf[2 * k2 + e], b00, b01);
+                    mma16816<H>(s[mt][1], qf[2 * k2 + e], b10, b11);
+                  } else {
+                    uint32_t qa[4];
+                    const int r = mt * 16 + arow;
+                    ldsm_x4(sq8 + r * (D * 2) + (((2 * (2 * k2 + e) + (lane >> 4)) ^ (r & 7)) << 4), qa);
+                    mma16816<H>(s[mt][0], qa, b00, b01);
+                    mma16816<H>(s[mt][1], qa, b10, b11);
+                  }
+                }
+              }
+            }
+            // ---- masks and the running softmax.  Columns of a thread: key0 + 8 n + col + {0, 1}.
+            const float ks = scales[slot_k * kPagedMaxBoxes + bx];
+            const bool on = (there >> bx) & 1u;
+            uint32_t keep[MT][2];
+            float mx[MT][2];
+            bool move = false;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                keep[mt][h] = on ? sees(mt, h, key0, span.full) : 0u;
+                const float f = fac[mt][h] * ks;
+                float x = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    float& v = s[mt][n][2 * h + e];
+                    v = (keep[mt][h] >> (8 * n + col + e)) & 1u ? v * f : -INFINITY;
+                    x = fmaxf(x, v);
+                  }
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                mx[mt][h] = x;
+                move |= x > m[mt][h] + TreeRef<H>::kSlack;
+              }
+            if (st == C::kSteps - 1) {
+              __syncwarp();
+              if (lane == 0) mbar_arrive(empty_bar(slot_k));
+            }
+            if (st == 0) {
+              ok = mbar_wait_bounded(full_bar(slot_v), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+            }
+            const float vs = on ? scales[slot_v * kPagedMaxBoxes + bx] : 0.f;
+            const float need = paged_unit(vs);
+            if (__any_sync(0xffffffffu, move) || need > unit) {
+              const float to = fmaxf(need, unit);
+              move_rows(mx, unit * paged_unit_rcp(to));
+              unit = to;
+            }
+            const float vr = vs * paged_unit_rcp(unit);
+            uint32_t pw[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float ref = m[mt][h] == -INFINITY ? 0.f : m[mt][h];
+                float p[2][2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) p[n][e] = ex2_tree(s[mt][n][2 * h + e] - ref);
+                l[mt][h] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) p[n][e] *= vr;
+                if (vr != vr) {  // (a NaN scale is for the rows that see the page)
+#pragma unroll
+                  for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                      if (!((keep[mt][h] >> (8 * n + col + e)) & 1u)) p[n][e] = 0.f;
+                }
+                // The accumulator's layout of 16 x 16 is the A operand's.
+                pw[mt][h] = pack2<H>(p[0][0], p[0][1]);
+                pw[mt][2 + h] = pack2<H>(p[1][0], p[1][1]);
+              }
+            // ---- O += P V: of 16 bytes of a row of V the even columns are one operand, the odd ones
+            // the next.
+            const int vrow = br + ((lane >> 3) & 1) * 8 + (lane & 7);
+#pragma unroll
+            for (int c2 = 0; c2 < DW / 32; ++c2) {
+              uint32_t vb[4];
+              const int ch = part * (DW / 16) + 2 * c2 + (lane >> 4);
+              if constexpr (D >= 128)
+                ldsm_x4_t(vbox + (ch >> 3) * (box * 128) + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4), vb);
+              else
+                ldsm_x4_t(vbox + vrow * kRowBytes + ((ch ^ ((vrow >> 1) & 3)) << 4), vb);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t e0, e1, o0, o1;
+                paged_unpack<H>(vb[2 * e], 0x4240u, 0x4341u, e0, o0);
+                paged_unpack<H>(vb[2 * e + 1], 0x4240u, 0x4341u, e1, o1);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  mma16816<H>(o[mt][4 * c2 + 2 * e], pw[mt], e0, e1);
+                  mma16816<H>(o[mt][4 * c2 + 2 * e + 1], pw[mt], o0, o1);
+                }
+              }
+            }
+          }
+          if (!ok) break;
+        } else {
+          if (permuted) natural();
+          const bool fresh = kind == kNew;
+          const int kr = grp * 16, key0 = tile0 + kr;  // this step's keys (rows of the tail, or new tokens)
+          const int end = fresh ? a.n : len - span.full;
+          const bool work = kr < BN16 && key0 < end;   // (the same for the whole warp)
+          uint32_t pw[MT][4];
+          if (work) {
+            float s[MT][2][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) s[mt][e >> 2][e & 3] = 0.f;
+            const int krow = kr + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              uint32_t kb[4];
+              ldsm_x4(sk + krow * 128 + (kk >> 2) * (BN16 * 128) + ((((kk & 3) * 2 + ((lane >> 3) & 1)) ^ (krow & 7)) << 4), kb);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                uint32_t qa[4];
+                const int r = mt * 16 + arow;
+                ldsm_x4(sq16 + r * (D * 2) + (((2 * kk + (lane >> 4)) ^ (r & 7)) << 4), qa);
+                mma16816<T>(s[mt][0], qa, kb[0], kb[1]);
+                mma16816<T>(s[mt][1], qa, kb[2], kb[3]);
+              }
+            }
+            float mx[MT][2];
+            bool move = false;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                // (all lanes: the new tokens' masks are read by the warp)
+                const uint32_t keep = fresh ? tree_sees16(a, b, tok[mt][h], key0, dep[mt][h], sink_left)
+                                            : sees(mt, h, span.full + key0, len);
+                float x = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    float& v = s[mt][n][2 * h + e];
+                    v = (keep >> (8 * n + col + e)) & 1u ? v * a.scale_log2 : -INFINITY;
+                    x = fmaxf(x, v);
+                  }
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                mx[mt][h] = x;
+                move |= x > m[mt][h] + TreeRef<H>::kSlack;
+              }
+            if (__any_sync(0xffffffffu, move)) move_rows(mx, 1.f);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float ref = m[mt][h] == -INFINITY ? 0.f : m[mt][h];
+                float p[2][2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) p[n][e] = ex2_tree(s[mt][n][2 * h + e] - ref);
+                l[mt][h] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
+                pw[mt][h] = pack2<T>(p[0][0], p[0][1]);
+                pw[mt][2 + h] = pack2<T>(p[1][0], p[1][1]);
+              }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty_bar(slot_k));
+          ok = mbar_wait_bounded(full_bar(slot_v), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (work) {
+            // Rows behind the length or before the window may hold anything and 0 * NaN is NaN: zeros.
+            // So may a new token's values where some row must not see them: cleared here, added below
+            // to the rows that do.
+            uint32_t bad = 0;  // keys of this step whose values are not all finite (new tokens only)
+            if (fresh || key0 + 16 > end || span.full + key0 < span.low) {
+              for (int e = lane; e < 16 * (DW / 8); e += 32) {
+                const int r = e % 16, ch = part * (DW / 8) + e / 16, p = span.full + key0 + r;
+                uint4* w = reinterpret_cast<uint4*>(smem + (sv - base) + (ch >> 3) * (BN16 * 128) + (kr + r) * 128 +
+                                                    (((ch & 7) ^ ((kr + r) & 7)) << 4));
+                if (key0 + r >= end || (!fresh && p < span.low && p >= a.sink)) {
+                  *w = make_uint4(0, 0, 0, 0);
+                } else if (fresh) {
+                  uint4 x = *w;
+                  if (nonfinite_bits<T>(x.x) | nonfinite_bits<T>(x.y) | nonfinite_bits<T>(x.z) | nonfinite_bits<T>(x.w)) {
+                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) xs[q] &= ~((nonfinite_bits<T>(xs[q]) >> 15) * 0xFFFFu);
+                    *w = x;
+                    bad |= 1u << r;
+                  }
+                }
+              }
+              bad = __reduce_or_sync(0xffffffffu, bad);
+              fence_proxy_async_smem();  // (the TMA writes this slot again later)
+              __syncwarp();
+            }
+            const int vrow = kr + arow;
+#pragma unroll
+            for (int n = 0; n < DW / 8; n += 2) {
+              uint32_t vb[4];
+              const int ch = part * (DW / 8) + n + (lane >> 4);
+              ldsm_x4_t(sv + vrow * 128 + (ch >> 3) * (BN16 * 128) + (((ch & 7) ^ (vrow & 7)) << 4), vb);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                mma16816<T>(o[mt][n], pw[mt], vb[0], vb[1]);
+                mma16816<T>(o[mt][n + 1], pw[mt], vb[2], vb[3]);
+              }
+            }
+            const bool any_bad = bad != 0u;
+#pragma unroll 1
+            for (; bad != 0u; bad &= bad - 1u) {
+              const int j = key0 + __ffs(bad) - 1;
+              const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + j * a.vn_t + part * DW + (lane & 3) * 2;
+              bool on[MT][2];
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  on[mt][h] = tok[mt][h] >= 0 && tree_sees(a, b, tok[mt][h], j, dep[mt][h], sink_left);
+#pragma unroll
+              for (int n = 0; n < DW / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const uint16_t v = vn[n * 8 + e];
+                  if (tree_nonfinite<T>(v)) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                      for (int h = 0; h < 2; ++h)
+                        if (on[mt][h]) o[mt][n][2 * h + e] += tree_f32<T>(v);
+                  }
+                }
+            }
+            if (any_bad) __syncwarp();  // (the next step's loads are aligned)
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty_bar(slot_v));
+      }
+      if (permuted) natural();
+
+      // ---- the groups' results joined: M = max m_w, O = sum 2^(m_w - M) O_w over the ring
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
+            l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
+            if ((lane & 3) == 0 && part == 0) {
+              const int r = mt * 16 + rl + 8 * h;
+              stat[grp * BM + r] = m[mt][h];
+              stat[(C::kGroups + grp) * BM + r] = l[mt][h];
+            }
+          }
+      ok = rows_sync_and(ok);  // everybody has left the ring; the statistics are there
+      float* joint = reinterpret_cast<float*>(smem);  // [group][BM][pitch]
+      {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = mt * 16 + rl + 8 * h;
+            if (row0 + r >= rows) continue;
+            float top = stat[r];
+#pragma unroll
+            for (int w = 1; w < C::kGroups; ++w) top = fmaxf(top, stat[w * BM + r]);
+            const float f = m[mt][h] == -INFINITY ? 1.f : ex2_tree(m[mt][h] - top);
+            float* dst = joint + (grp * BM + r) * C::kPitch + part * DW + (lane & 3) * 2;
+            // (a group that saw nothing adds zeros, except what a NaN score made of it)
+            const bool none = m[mt][h] == -INFINITY && l[mt][h] == 0.f;
+#pragma unroll
+            for (int n = 0; n < DW / 8; ++n)
+              *reinterpret_cast<float2*>(dst + 8 * n) =
+                  none ? make_float2(0.f, 0.f) : make_float2(o[mt][n][2 * h] * f, o[mt][n][2 * h + 1] * f);
+          }
+      }
+      rows_sync();
+      if (ok) {
+        constexpr int Q4 = D / 4;  // float4 columns per row
+        for (int e = tid; e < BM * Q4; e += kTreeThreads) {
+          const int r = e / Q4, q4 = e % Q4;
+          if (row0 + r >= rows) break;
+          float top = stat[r];
+#pragma unroll
+          for (int w = 1; w < C::kGroups; ++w) top = fmaxf(top, stat[w * BM + r]);
+          float sum = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < C::kGroups; ++w) {
+            const float mw = stat[w * BM + r];
+            sum += (mw == -INFINITY ? 1.f : ex2_tree(mw - top)) * stat[(C::kGroups + w) * BM + r];
+            const float4 x = *reinterpret_cast<const float4*>(joint + (w * BM + r) * C::kPitch + 4 * q4);
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+          }
+          if (whole) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: zeros
+            int i, gq;
+            tree_row(a, row0 + r, i, gq);
+            uint16_t* dst = a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + gq) * a.o_h + i * a.o_t + 4 * q4;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+          } else {
+            *reinterpret_cast<float4*>(a.part_o + (part_row + r) * D + 4 * q4) = v;
+            if (q4 == 0) a.part_ml[part_row + r] = make_float2(top, sum);
+          }
+        }
+      }
+      ok = item_done(ok);
+      if (!ok) break;  // (the producer waits for the copies in flight)
+      pos += t1 - t0;
+      if (pos >= stop) break;
+      advance();
+      fence_proxy_async_smem();  // the joint outputs lay where the TMA writes next
+      item_free();               // the ring, Q and the statistics are free
+    }
+  }
+}
+
+}  // namespace w8
+
+namespace w8host {
+
+int require_sm100(int* device);
+
+int tree_encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, int64_t n, int64_t heads, int64_t batch,
+                     int64_t s_b, int64_t s_h, int64_t s_n, uint32_t rows, uint32_t blocks);
+int tree_encode(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, const cuuint64_t* dims,
+                const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle, const char* what);
+int tree_join(const w8::TreeArgs& a, bool half, int64_t d, int bm, cudaStream_t stream);
+
+// How a call is cut: rows per tile, row tiles, and the CTAs that share all tiles, or an item each.
+struct PagedPlan {
+  bool direct;
+  int bm, row_tiles, ctas;
+  int64_t items;
+};
+
+static PagedPlan paged_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t n, int64_t d, int64_t slots,
+                            int64_t window, int64_t sink, int sms) {
+  PagedPlan p;
+  const int64_t rows = group * n;
+  p.bm = rows > 16 && d <= 128 ? 32 : 16;
+  p.row_tiles = static_cast<int>((rows + p.bm - 1) / p.bm);
+  p.items = batch * kv_heads * p.row_tiles;
+  // Keys of one row tile: with a window, those its tokens see.
+  const int64_t bn = d == 512 ? 64 : d == 64 ? 256 : 128;
+  const int64_t tokens = std::min(n, p.bm / group + 2);
+  const int64_t keys = window > 0 ? std::min(slots, window + tokens + sink) : slots;
+  const int64_t tiles = (keys + bn - 1) / bn + 1 + (2 * n + bn - 1) / bn;
+  // An item per CTA, or all tiles dealt evenly: by estimated times.  A tile is about 1 us, an item's
+  // start and end 3 us, joining the pieces a launch of 4 us.  From 8 items an SM on ragged lengths
+  // even out by themselves.
+  const double waves = static_cast<double>((p.items + sms - 1) / std::max(sms, 1));
+  const double alone = waves * (static_cast<double>(tiles) + 3);
+  const double dealt = static_cast<double>(p.items) * static_cast<double>(tiles) / sms + 3 * (waves + 1) + 4;
+  p.direct = alone <= dealt || p.items >= 8 * static_cast<int64_t>(sms);
+  p.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms, p.items * tiles, w8::kTreeMaxPieces})));
+  return p;
+}
+
+struct PagedWs {
+  int64_t part_o, part_ml, info, total;
+};
+static PagedWs paged_ws(const PagedPlan& p, int64_t d) {
+  PagedWs w;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t r = at;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  };
+  const int64_t part_rows = p.direct ? 0 : 2 * static_cast<int64_t>(p.ctas) * p.bm;
+  w.part_o = take(part_rows * d * 4);
+  w.part_ml = take(part_rows * 8);
+  w.info = take(p.direct ? 0 : p.items * 8);
+  w.total = at;
+  return w;
+}
+
+static int paged_shape(const w8_attention_paged_args& x) {
+  W8_CHECK_ARG(x.batch >= 0 && x.heads >= 1 && x.kv_heads >= 1 && x.pages >= 0 && x.table_pages >= 0 && x.n_new >= 0,
+               "negative size");
+  W8_CHECK_ARG(x.heads % x.kv_heads == 0, "heads %lld must be a multiple of kv_heads %lld", (long long)x.heads,
+               (long long)x.kv_heads);
+  W8_CHECK_ARG(x.window >= 0 && x.window < (1ll << 31), "window must be 0 (none) or positive, below 2^31");
+  W8_CHECK_ARG(x.sink >= 0 && x.sink < (1ll << 30), "sink must not be negative, and below 2^30");
+  W8_CHECK_ARG(x.sink == 0 || x.window > 0, "sinks go with a window");
+  if (x.page != 16 && x.page != 32 && x.page != 64 && x.page != 128) {
+    set_error("pages of %lld tokens are not of 16, 32, 64 or 128", (long long)x.page);
+    return W8_ERR_UNSUPPORTED;
+  }
+  W8_CHECK_ARG(x.table_pages < (1ll << 30) / x.page && x.pages < (1ll << 31) && x.n_new <= 65536 &&
+                   x.batch <= (1ll << 20) && x.heads <= 65536,
+               "size beyond the limits");
+  if (x.head_dim != 64 && x.head_dim != 128 && x.head_dim != 256 && x.head_dim != 512) {
+    set_error("head_dim %lld is not 64, 128, 256 or 512", (long long)x.head_dim);
+    return W8_ERR_UNSUPPORTED;
+  }
+  W8_CHECK_ARG(x.batch * x.heads * x.n_new < (1ll << 31), "too many query rows");
+  return W8_OK;
+}
+
+// 5-D map over pages of 8-bit rows: (128 bytes, row, 128-byte block, head, page).  A box
+// {128, rows, blocks, 1, 1} lands as `blocks` swizzled [rows x 128] blocks (of 64 for D = 64).
+static int paged_encode(CUtensorMap* map, const void* ptr, int64_t d, int64_t page, int64_t heads, int64_t pages,
+                        const int64_t* stride, uint32_t rows) {
+  const int64_t wide = std::min<int64_t>(d, 128);
+  auto bytes = [&](int64_t size, int64_t s) { return static_cast<cuuint64_t>(size > 1 ? s : d); };
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(wide), static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(d / wide),
+                              static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(pages)};
+  const cuuint64_t strides[4] = {bytes(page, stride[2]), static_cast<cuuint64_t>(wide), bytes(heads, stride[1]),
+                                 bytes(pages, stride[0])};
+  const cuuint32_t box[5] = {static_cast<cuuint32_t>(wide), rows, static_cast<cuuint32_t>(d / wide), 1, 1};
+  return tree_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, dims, strides, box,
+                     d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, "pages");
+}
+
+template <typename T, int D, int MT>
+static int paged_main(const w8_attention_paged_args& x, const w8::PagedArgs& pa, int64_t blocks, int device,
+                      cudaStream_t stream) {
+  using C = w8::PagedCfg<D, MT>;
+  constexpr bool kHalf = __is_same(T, __half);
+  const w8::TreeArgs& a = pa.t;
+  static bool done[64] = {};
+  if (!done[device]) {
+    W8_CUDA_TRY(cudaFuncSetAttribute(w8::attn_paged_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     C::kSmem));
+    done[device] = true;
+  }
+  CUtensorMap tk, tv, tkt, tvt, tkn, tvn;
+  auto rows = [&](CUtensorMap* map, const void* p, int64_t n, const int64_t* s) {
+    return tree_encode_rows(map, p, kHalf, D, n, a.kv_heads, a.batch, s[0], s[1], s[2], C::kBN16, D / 64);
+  };
+  int st = rows(&tkn, x.k_new, a.n, x.k_new_stride);
+  if (st == W8_OK) st = rows(&tvn, x.v_new, a.n, x.v_new_stride);
+  if (st == W8_OK) st = rows(&tkt, x.k_tail, x.page, x.k_tail_stride);
+  if (st == W8_OK) st = rows(&tvt, x.v_tail, x.page, x.v_tail_stride);
+  tk = tkn, tv = tvn;  // an empty pool: never read
+  const uint32_t box = static_cast<uint32_t>(std::min<int64_t>(x.page, C::kBN));
+  if (st == W8_OK && x.pages > 0) st = paged_encode(&tk, x.k, D, x.page, x.kv_heads, x.pages, x.k_stride, box);
+  if (st == W8_OK && x.pages > 0) st = paged_encode(&tv, x.v, D, x.page, x.kv_heads, x.pages, x.v_stride, box);
+  if (st != W8_OK) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+  cfg.blockDim = dim3(w8::kPagedThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, w8::attn_paged_kernel<T, D, MT>, tk, tv, tkt, tvt, tkn, tvn, pa));
+}
+
+template <typename T, int D>
+static int paged_go(const w8_attention_paged_args& x, const w8::PagedArgs& a, const PagedPlan& p, int device,
+                    cudaStream_t stream) {
+  W8_CHECK_ARG(p.items < (1ll << 31) / 2, "too many row tiles");
+  const int64_t blocks = p.direct ? p.items : p.ctas;
+  int st;
+  if constexpr (D <= 128)
+    st = p.bm == 32 ? paged_main<T, D, 2>(x, a, blocks, device, stream) : paged_main<T, D, 1>(x, a, blocks, device, stream);
+  else
+    st = paged_main<T, D, 1>(x, a, blocks, device, stream);
+  if (st != W8_OK || p.direct || p.ctas <= 1) return st;
+  return tree_join(a.t, __is_same(T, __half), D, p.bm, stream);
+}
+
+// Read (and optionally clear) the sticky device status of the paged attention.
+int paged_device_status(int clear, int* out) {
+  W8_CUDA_TRY(cudaMemcpyFromSymbol(out, w8::g_tree_status, sizeof(int)));
+  if (clear) {
+    const int zero = 0;
+    W8_CUDA_TRY(cudaMemcpyToSymbol(w8::g_tree_status, &zero, sizeof(int)));
+  }
+  return W8_OK;
+}
+
+}  // namespace w8host
+
+extern "C" int64_t w8_attention_paged_workspace_bytes(const w8_attention_paged_args* in) {
+  using namespace w8host;
+  if (in == nullptr || paged_shape(*in) != W8_OK) return -1;
+  const w8_attention_paged_args& x = *in;
+  int sms = 148;
+  if (num_sms(&sms) != W8_OK) sms = 148;
+  const PagedPlan p = paged_plan(x.batch, x.kv_heads, x.heads / x.kv_heads, x.n_new, x.head_dim, x.table_pages * x.page,
+                                 x.window, x.sink, sms);
+  return paged_ws(p, x.head_dim).total;
+}
+
+extern "C" int w8_attention_paged(const w8_attention_paged_args* in, void* workspace, int64_t workspace_bytes,
+                                  w8_stream_t stream) {
+  using namespace w8host;
+  W8_CHECK_ARG(in != nullptr, "null arguments");
+  const w8_attention_paged_args& x = *in;
+  int st = paged_shape(x);
+  if (st != W8_OK) return st;
+  W8_CHECK_ARG(x.dtype == W8_BF16 || x.dtype == W8_FP16, "dtype must be W8_BF16 or W8_FP16");
+  if (x.batch == 0 || x.n_new == 0) return W8_OK;
+  // (positive in the kernels' fp32 log2 units too: a masked score is -inf times it)
+  const float scale_log2 = static_cast<float>(x.scale * 1.4426950408889634);
+  W8_CHECK_ARG(scale_log2 > 0.f && scale_log2 < 3e38f, "scale must be positive and finite");
+  W8_CHECK_ARG(x.q && x.k_tail && x.v_tail && x.k_new && x.v_new && x.out && x.lens, "null pointer");
+  W8_CHECK_ARG(x.pages == 0 || (x.k && x.v && x.k_scale && x.v_scale), "null pages");
+  W8_CHECK_ARG(x.table_pages == 0 || x.table, "null table");
+  W8_CHECK_ARG(x.tree == nullptr || x.window == 0 || x.depth != nullptr, "a tree with a window needs the tokens' depths");
+  W8_CHECK_ARG(x.out != x.q && x.out != x.k && x.out != x.v && x.out != x.k_tail && x.out != x.v_tail &&
+                   x.out != x.k_new && x.out != x.v_new,
+               "out must not be an input");
+  const void* ptrs[8] = {x.q, x.out, x.k_tail, x.v_tail, x.k_new, x.v_new, x.k, x.v};
+  const int64_t* strides[8] = {x.q_stride, x.out_stride, x.k_tail_stride, x.v_tail_stride, x.k_new_stride, x.v_new_stride,
+                               x.k_stride, x.v_stride};
+  const int64_t KV = x.kv_heads;
+  const int64_t sizes[8][3] = {{x.batch, x.heads, x.n_new}, {x.batch, x.heads, x.n_new}, {x.batch, KV, x.page},
+                               {x.batch, KV, x.page},       {x.batch, KV, x.n_new},     {x.batch, KV, x.n_new},
+                               {x.pages, KV, x.page},       {x.pages, KV, x.page}};
+  for (int i = 0; i < 8; ++i) {
+    const int64_t of = i < 6 ? 8 : 16;
+    W8_CHECK_ALIGN(aligned(ptrs[i], 16), "q, pages, tails, k_new, v_new and out must be 16-byte aligned");
+    for (int j = 0; j < 3; ++j) {
+      if (sizes[i][j] <= 1) continue;
+      W8_CHECK_ALIGN(strides[i][j] % of == 0, "the strides of q, tails, k_new, v_new and out must be multiples of 8, of pages of 16");
+      W8_CHECK_ARG(i < 2 || (strides[i][j] > 0 && strides[i][j] < (1ll << 38)),
+                   "the strides of pages, tails, k_new and v_new must be positive and below 2^38");
+    }
+  }
+  int device = 0, sms = 0;
+  st = require_sm100(&device);
+  if (st != W8_OK) return st;
+  st = num_sms(&sms);
+  if (st != W8_OK) return st;
+  const int64_t group = x.heads / x.kv_heads;
+  const PagedPlan p = paged_plan(x.batch, KV, group, x.n_new, x.head_dim, x.table_pages * x.page, x.window, x.sink, sms);
+  const PagedWs w = paged_ws(p, x.head_dim);
+  W8_CHECK_ARG(w.total == 0 || (workspace != nullptr && workspace_bytes >= w.total),
+               "workspace of %lld bytes needed (got %lld)", (long long)w.total, (long long)workspace_bytes);
+  W8_CHECK_ALIGN(aligned(workspace, 16), "workspace must be 16-byte aligned");
+  w8::PagedArgs pa = {};
+  w8::TreeArgs& a = pa.t;
+  a.q = static_cast<const uint16_t*>(x.q);
+  a.kn = static_cast<const uint16_t*>(x.k_new);
+  a.vn = static_cast<const uint16_t*>(x.v_new);
+  a.o = static_cast<uint16_t*>(x.out);
+  a.lens = x.lens;
+  a.tree = x.tree;
+  a.depth = x.depth;
+  a.q_b = x.q_stride[0], a.q_h = x.q_stride[1], a.q_t = x.q_stride[2];
+  a.kn_b = x.k_new_stride[0], a.kn_h = x.k_new_stride[1], a.kn_t = x.k_new_stride[2];
+  a.vn_b = x.v_new_stride[0], a.vn_h = x.v_new_stride[1], a.vn_t = x.v_new_stride[2];
+  a.o_b = x.out_stride[0], a.o_h = x.out_stride[1], a.o_t = x.out_stride[2];
+  a.tree_b = x.tree_stride[0], a.tree_i = x.tree_stride[1];
+  a.depth_b = x.depth_stride;
+  a.batch = static_cast<int>(x.batch);
+  a.kv_heads = static_cast<int>(KV);
+  a.group = static_cast<int>(group);
+  a.group_rcp = group > 1 ? static_cast<uint32_t>((1ull << 32) / static_cast<uint64_t>(group)) : 0u;
+  a.n = static_cast<int>(x.n_new);
+  a.slots = static_cast<int>(x.table_pages * x.page);
+  a.window = static_cast<int>(x.window);
+  a.sink = static_cast<int>(x.sink);
+  a.scale_log2 = scale_log2;
+  a.row_tiles = p.row_tiles;
+  a.splits = 1;
+  a.direct = p.direct ? 1 : 0;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.part_o = reinterpret_cast<float*>(ws + w.part_o);
+  a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+  a.info = reinterpret_cast<int2*>(ws + w.info);
+  pa.table = x.table;
+  pa.table_b = x.table_stride;
+  pa.table_pages = static_cast<int>(x.table_pages);
+  pa.pages = static_cast<int>(x.pages);
+  pa.shift = x.page == 16 ? 4 : x.page == 32 ? 5 : x.page == 64 ? 6 : 7;
+  pa.ks = x.k_scale, pa.vs = x.v_scale;
+  pa.ks_p = x.k_scale_stride[0], pa.ks_h = x.k_scale_stride[1];
+  pa.vs_p = x.v_scale_stride[0], pa.vs_h = x.v_scale_stride[1];
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const bool bf = x.dtype == W8_BF16;
+  switch (x.head_dim) {
+    case 64:
+      return bf ? paged_go<__nv_bfloat16, 64>(x, pa, p, device, s) : paged_go<__half, 64>(x, pa, p, device, s);
+    case 128:
+      return bf ? paged_go<__nv_bfloat16, 128>(x, pa, p, device, s) : paged_go<__half, 128>(x, pa, p, device, s);
+    case 256:
+      return bf ? paged_go<__nv_bfloat16, 256>(x, pa, p, device, s) : paged_go<__half, 256>(x, pa, p, device, s);
+    default:
+      return bf ? paged_go<__nv_bfloat16, 512>(x, pa, p, device, s) : paged_go<__half, 512>(x, pa, p, device, s);
+  }
+}

@@ -31,52 +31,12 @@
 // is read by cp.async, once for every sequence: 40 sequences over one cache of 4000 slots, 8 heads of
 // 128, take 167 us where 40 caches of their own take 106.)
 #include "attention_tree.cuh"
+#include "attn_mma.cuh"
 #include "attn_tc.cuh"
 
 #include <algorithm>
 
 namespace w8 {
-
-constexpr int kTreeWarps = 8;
-constexpr int kTreeThreads = 32 * kTreeWarps;
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  const int n = on ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-// Arrive on `bar` once every earlier cp.async of this thread has landed.
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 template <int D, int MT>
 struct TreeCfg {
@@ -101,47 +61,6 @@ struct TreeCfg {
   static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory budget exceeded");
   static_assert(kGroups * kBM * kPitch * 4 <= kOffQ, "the joint outputs fit over the ring");
 };
-
-// Quotient of a number that is seldom above 32 bits (a 64-bit division is a call of some 150
-// instructions).
-__device__ __forceinline__ long long div_short(long long x, uint32_t by) {
-  return (x >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(x) / by) : x / by;
-}
-
-// How `total` tiles are dealt to `ctas`: the first `more` CTAs hold one more than the others.
-struct TreeDeal {
-  long long each, more;
-};
-__device__ __forceinline__ long long deal_begin(const TreeDeal& d, long long u) {
-  return u * d.each + (u < d.more ? u : d.more);
-}
-__device__ __forceinline__ int deal_owner(const TreeDeal& d, long long tile) {
-  const long long wide = d.more * (d.each + 1);
-  return static_cast<int>(tile < wide ? div_short(tile, static_cast<uint32_t>(d.each + 1))
-                                      : d.more + div_short(tile - wide, static_cast<uint32_t>(d.each)));
-}
-
-// Exclusive prefix sum over the block and the block's sum.
-__device__ __forceinline__ long long block_scan(long long v, long long* sm, long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = v;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, d);
-    if (lane >= d) x += y;
-  }
-  if (lane == 31) sm[warp] = x;
-  __syncthreads();
-  long long before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kTreeWarps; ++i) {
-    if (i < warp) before += sm[i];
-    total += sm[i];
-  }
-  __syncthreads();
-  return before + x - v;
-}
 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
@@ -254,7 +173,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
     long long* sched = reinterpret_cast<long long*>(smem);  // (the ring is not in use yet)
     long long sum = 0, round;
     for (int p = tid; p < pairs; p += kTreeThreads) sum += pair_tiles(p);
-    long long excl = block_scan(sum, sched, round);  // (of up to 256 pairs also each one's place)
+    long long excl = block_scan<kTreeWarps>(sum, sched, round);  // (of up to 256 pairs also each one's place)
     const long long total = round * a.kv_heads;
     const uint32_t ctas = total < gridDim.x ? static_cast<uint32_t>(total) : gridDim.x;
     if (blockIdx.x >= ctas) return;
@@ -269,7 +188,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeCfg<D, MT>::kPerSm)
       long long nt = sum;
       if (pairs > kTreeThreads) {
         nt = p < pairs ? pair_tiles(p) : 0;
-        excl = before + block_scan(nt, sched, round);
+        excl = before + block_scan<kTreeWarps>(nt, sched, round);
       }
       if (nt > 0 && excl * a.kv_heads <= pos && pos < (excl + nt) * a.kv_heads) {
         sched[16] = p;
@@ -1042,6 +961,33 @@ static int tree_main(const w8::TreeArgs& a, int64_t blocks, int device, cudaStre
                      stream, tk, tv, tkn, tvn, a);
 }
 
+// The pieces of all items joined.  Few rows: a CTA each, or for 32 columns of each, since their
+// pieces may be many.
+template <typename T, int D>
+static int tree_join_go(const w8::TreeArgs& a, int bm, cudaStream_t stream) {
+  constexpr int kWide = D < 128 ? D : 128;
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.group * a.n;
+  if (rows * (D / 32) <= 1024)
+    return launch_tree(w8::attn_tree_combine_kernel<T, D, 32>, dim3(static_cast<unsigned>(rows), D / 32), 256, 0, stream, a,
+                       bm);
+  if (rows <= 512)
+    return launch_tree(w8::attn_tree_combine_kernel<T, D, kWide>, dim3(static_cast<unsigned>(rows), D / kWide), 256, 0,
+                       stream, a, bm);
+  return launch_tree(w8::attn_tree_combine_rows_kernel<T, D>, dim3(static_cast<unsigned>((rows * (D / 4) + 255) / 256)),
+                     256, 0, stream, a, bm, rows);
+}
+
+// The same for the paged cache's attention.
+int tree_join(const w8::TreeArgs& a, bool half, int64_t d, int bm, cudaStream_t stream) {
+  using B = __nv_bfloat16;
+  switch (d) {
+    case 64: return half ? tree_join_go<__half, 64>(a, bm, stream) : tree_join_go<B, 64>(a, bm, stream);
+    case 128: return half ? tree_join_go<__half, 128>(a, bm, stream) : tree_join_go<B, 128>(a, bm, stream);
+    case 256: return half ? tree_join_go<__half, 256>(a, bm, stream) : tree_join_go<B, 256>(a, bm, stream);
+    default: return half ? tree_join_go<__half, 512>(a, bm, stream) : tree_join_go<B, 512>(a, bm, stream);
+  }
+}
+
 template <typename T, int D>
 static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStream_t stream) {
   W8_CHECK_ARG(p.items < (1ll << 31) / 2, "too many row tiles");
@@ -1054,19 +1000,8 @@ static int tree_go(const w8::TreeArgs& a, const TreePlan& p, int device, cudaStr
   else
     st = tree_main<T, D, 1>(a, blocks, device, stream);
   if (st != W8_OK) return st;
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.group * a.n;
   if (p.tc ? p.splits > 1 : !p.direct && p.ctas > 1) {
-    // Few rows: a CTA each, or for 32 columns of each, since their pieces may be many.
-    constexpr int kWide = D < 128 ? D : 128;
-    if (rows * (D / 32) <= 1024)
-      st = launch_tree(w8::attn_tree_combine_kernel<T, D, 32>, dim3(static_cast<unsigned>(rows), D / 32), 256, 0, stream,
-                       a, p.bm);
-    else if (rows <= 512)
-      st = launch_tree(w8::attn_tree_combine_kernel<T, D, kWide>, dim3(static_cast<unsigned>(rows), D / kWide), 256, 0,
-                       stream, a, p.bm);
-    else
-      st = launch_tree(w8::attn_tree_combine_rows_kernel<T, D>, dim3(static_cast<unsigned>((rows * (D / 4) + 255) / 256)),
-                       256, 0, stream, a, p.bm, rows);
+    st = tree_join_go<T, D>(a, p.bm, stream);
     if (st != W8_OK) return st;
   }
   if (a.scores != nullptr) {

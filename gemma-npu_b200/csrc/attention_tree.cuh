@@ -23,6 +23,7 @@ struct TreeArgs {
   uint32_t group_rcp;    // floor(2^32 / group), for tree_row
   int q_tma;             // q's rows load as TMA boxes (tcgen05 schedule)
   int batch, kv_heads, group, n, slots, window;
+  int sink;              // positions below it stay visible behind a window (0: none)
   float scale_log2;      // scale * log2(e): scores in log2 units
   int row_tiles, splits;  // splits: of each item, tcgen05 schedule only
   // Partial results of an item (item = (b * kv_heads + c) * row_tiles + rt): piece s in slot
@@ -125,10 +126,12 @@ __device__ __forceinline__ int tree_depth(const TreeArgs& a, int b, int i) {
 }
 
 // Whether token i sees new token j (both < n).
-__device__ __forceinline__ bool tree_sees(const TreeArgs& a, int b, int i, int j, int depth_i) {
+// `sink_left`: a.sink less the committed length; new tokens of a smaller depth are sinks.
+__device__ __forceinline__ bool tree_sees(const TreeArgs& a, int b, int i, int j, int depth_i, int sink_left = 0) {
   const bool on = a.tree != nullptr ? a.tree[b * a.tree_b + i * a.tree_i + j] != 0 : j <= i;
   if (!on || a.window <= 0) return on;
-  return static_cast<int64_t>(tree_depth(a, b, j)) > static_cast<int64_t>(depth_i) - a.window;
+  const int dj = tree_depth(a, b, j);
+  return static_cast<int64_t>(dj) > static_cast<int64_t>(depth_i) - a.window || dj < sink_left;
 }
 
 // The same for a packed pair: bit 15 / 31 set for a half that is not finite (the exponent
@@ -149,7 +152,8 @@ __device__ __forceinline__ uint32_t nonzero_bytes(uint32_t w) {
 // tree_sees of the new tokens j0 .. j0 + 31 as bits (those behind n are 0).  A loop of byte
 // loads would wait for each in turn: the row is read with 16-byte loads where it is aligned
 // and with 32 independent ones where it is not.
-__device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i, int j0, int depth_i) {
+__device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i, int j0, int depth_i,
+                                                int sink_left = 0) {
   const int left = a.n - j0;
   if (left <= 0) return 0u;
   uint32_t bits = 0;
@@ -157,7 +161,8 @@ __device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i,
     bits = i < j0 ? 0u : i - j0 >= 31 ? 0xFFFFFFFFu : (2u << (i - j0)) - 1u;
     if (a.depth == nullptr) {  // a plain chunk: the last `window` tokens up to i
       const int lo = a.window > 0 ? i - a.window + 1 - j0 : 0;
-      if (lo > 0) bits = lo > 31 ? 0u : bits & (0xFFFFFFFFu << lo);
+      const uint32_t sinks = sink_left <= j0 ? 0u : sink_left - j0 > 31 ? 0xFFFFFFFFu : (1u << (sink_left - j0)) - 1u;
+      if (lo > 0) bits &= (lo > 31 ? 0u : 0xFFFFFFFFu << lo) | sinks;
       return left < 32 ? bits & ((1u << left) - 1u) : bits;
     }
   } else {
@@ -182,7 +187,7 @@ __device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i,
     for (int e = 0; e < 32; ++e) d[e] = e < left ? tree_depth(a, b, j0 + e) : 0;
 #pragma unroll
     for (int e = 0; e < 32; ++e)
-      if (static_cast<int64_t>(d[e]) <= static_cast<int64_t>(depth_i) - a.window) bits &= ~(1u << e);
+      if (static_cast<int64_t>(d[e]) <= static_cast<int64_t>(depth_i) - a.window && d[e] >= sink_left) bits &= ~(1u << e);
   }
   return bits;
 }
@@ -191,7 +196,7 @@ __device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i,
 // token (ascending over the lanes, -1 for none) and its depth.  The rows of a token share its
 // line of the tree, which the warp reads once, a byte a lane (any alignment).  All lanes.
 __device__ __forceinline__ void tree_sees64_rows(const TreeArgs& a, int b, int tok, int j0, int depth_i,
-                                                 uint32_t (&keep)[2]) {
+                                                 uint32_t (&keep)[2], int sink_left = 0) {
   const int lane = threadIdx.x & 31;
   keep[0] = keep[1] = 0u;
   const int j[2] = {j0 + lane, j0 + 32 + lane};
@@ -212,7 +217,8 @@ __device__ __forceinline__ void tree_sees64_rows(const TreeArgs& a, int b, int t
     for (int h = 0; h < 2; ++h) {
       bool on = j[h] < a.n;
       if (on) on = line != nullptr ? line[j[h]] != 0 : j[h] <= t;
-      if (a.window > 0) on = on && static_cast<int64_t>(dj[h]) > static_cast<int64_t>(dt) - a.window;
+      if (a.window > 0)
+        on = on && (static_cast<int64_t>(dj[h]) > static_cast<int64_t>(dt) - a.window || dj[h] < sink_left);
       const uint32_t bits = __ballot_sync(0xffffffffu, on);
       if (tok == t) keep[h] = bits;
     }
@@ -221,7 +227,8 @@ __device__ __forceinline__ void tree_sees64_rows(const TreeArgs& a, int b, int t
 
 // The same for one row's new tokens j0 .. j0 + 15, in little code (it stands beside the common
 // tiles, which have none of it).  All lanes, of the same j0.
-__device__ __forceinline__ uint32_t tree_sees16(const TreeArgs& a, int b, int i, int j0, int depth_i) {
+__device__ __forceinline__ uint32_t tree_sees16(const TreeArgs& a, int b, int i, int j0, int depth_i,
+                                                int sink_left = 0) {
   const int left = min(a.n - j0, 16);
   uint32_t bits = left <= 0 || i < 0 ? 0u : (1u << left) - 1u;
   if (a.tree == nullptr) {
@@ -239,9 +246,10 @@ __device__ __forceinline__ uint32_t tree_sees16(const TreeArgs& a, int b, int i,
     const int e0 = threadIdx.x & 15;
     const int dj = e0 < left ? tree_depth(a, b, j0 + e0) : 0;
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (static_cast<int64_t>(__shfl_sync(0xffffffffu, dj, e)) <= static_cast<int64_t>(depth_i) - a.window)
-        bits &= ~(1u << e);
+    for (int e = 0; e < 16; ++e) {
+      const int d = __shfl_sync(0xffffffffu, dj, e);
+      if (static_cast<int64_t>(d) <= static_cast<int64_t>(depth_i) - a.window && d >= sink_left) bits &= ~(1u << e);
+    }
   }
   return bits;
 }

@@ -599,43 +599,43 @@ static TreeEncodeFn tree_encode_fn() {
   return fn;
 }
 
-// 5-D map over rows [batch, heads, n] of d elements: (64 columns, row, 64-column block, head,
-// batch).  A box {64, rows, blocks, 1, 1} lands as `blocks` 128-byte-swizzled [rows x 64]
-// blocks; rows behind n and blocks behind d / 64 read as zeros.
-int tree_encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, int64_t n, int64_t heads, int64_t batch,
-                       int64_t s_b, int64_t s_h, int64_t s_n, uint32_t rows, uint32_t blocks) {
+// A 5-D map of a cache's rows or pages.
+int tree_encode(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, const cuuint64_t* dims,
+                const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle, const char* what) {
   TreeEncodeFn enc = tree_encode_fn();
   if (enc == nullptr) {
     set_error("cuTensorMapEncodeTiled is not available from the driver");
     return W8_ERR_CUDA;
   }
+  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(map, type, 5, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled (cache attention, %s) failed with CUresult %d", what, static_cast<int>(r));
+    return W8_ERR_CUDA;
+  }
+  return W8_OK;
+}
+
+// 5-D map over rows [batch, heads, n] of d elements: (64 columns, row, 64-column block, head,
+// batch).  A box {64, rows, blocks, 1, 1} lands as `blocks` 128-byte-swizzled [rows x 64]
+// blocks; rows behind n and blocks behind d / 64 read as zeros.
+int tree_encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, int64_t n, int64_t heads, int64_t batch,
+                       int64_t s_b, int64_t s_h, int64_t s_n, uint32_t rows, uint32_t blocks) {
   // A dimension of one element has no stride to speak of: any valid one.
   auto bytes = [&](int64_t size, int64_t stride) { return static_cast<cuuint64_t>(size > 1 ? stride * 2 : d * 2); };
   const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(d / 64),
                               static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(batch)};
   const cuuint64_t strides[4] = {bytes(n, s_n), 128, bytes(heads, s_h), bytes(batch, s_b)};
   const cuuint32_t box[5] = {64, rows, blocks, 1, 1};
-  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
-  const CUresult r = enc(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
-                         const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    set_error("cuTensorMapEncodeTiled (cache attention) failed with CUresult %d", static_cast<int>(r));
-    return W8_ERR_CUDA;
-  }
-  return W8_OK;
+  return tree_encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ptr, dims, strides,
+                     box, CU_TENSOR_MAP_SWIZZLE_128B, "rows");
 }
 
 // 5-D map over q: (64 columns, head, token, 64-column block, batch).  A box {64, group,
 // 128 / group, blocks, 1} lands as `blocks` swizzled blocks of 128 rows i * group + g, zeros
 // behind the d / 64-th.
 static int encode_q(CUtensorMap* map, const w8::TreeArgs& a, bool half, int64_t d, uint32_t blocks) {
-  TreeEncodeFn enc = tree_encode_fn();
-  if (enc == nullptr) {
-    set_error("cuTensorMapEncodeTiled is not available from the driver");
-    return W8_ERR_CUDA;
-  }
   const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
   auto bytes = [&](int64_t size, int64_t stride) { return static_cast<cuuint64_t>(size > 1 ? stride * 2 : d * 2); };
   const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(a.n),
@@ -643,16 +643,8 @@ static int encode_q(CUtensorMap* map, const w8::TreeArgs& a, bool half, int64_t 
   const cuuint64_t strides[4] = {bytes(heads, a.q_h), bytes(a.n, a.q_t), 128, bytes(a.batch, a.q_b)};
   const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(w8::kTtBM / a.group),
                              blocks, 1};
-  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
-  const CUresult r = enc(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
-                         const_cast<uint16_t*>(a.q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    set_error("cuTensorMapEncodeTiled (cache attention, q) failed with CUresult %d", static_cast<int>(r));
-    return W8_ERR_CUDA;
-  }
-  return W8_OK;
+  return tree_encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.q, dims, strides,
+                     box, CU_TENSOR_MAP_SWIZZLE_128B, "q");
 }
 
 template <typename T, int D, int DR = D>

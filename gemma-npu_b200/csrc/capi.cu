@@ -70,6 +70,9 @@ int attention_device_status(int clear, int* out);
 int peer_device_status(int clear, int* out);
 int tree_device_status(int clear, int* out);
 int cache_device_status(int clear, int* out);
+int paged_device_status(int clear, int* out);
+int paged_ops_device_status(int clear, int* out);
+int verify_device_status(int clear, int* out);
 
 }  // namespace w8host
 
@@ -107,13 +110,24 @@ extern "C" int w8_device_status(int clear) {
   if (st != W8_OK) return st;
   st = w8host::cache_device_status(clear, &vc);
   if (st != W8_OK) return st;
+  int vg = W8_OK, vo = W8_OK, vv = W8_OK;
+  st = w8host::paged_device_status(clear, &vg);
+  if (st != W8_OK) return st;
+  st = w8host::paged_ops_device_status(clear, &vo);
+  if (st != W8_OK) return st;
+  st = w8host::verify_device_status(clear, &vv);
+  if (st != W8_OK) return st;
   // A wait that gave up says more than an index that was skipped.
-  for (const int s : {v, va, vp, vt, vc})
+  for (const int s : {v, va, vp, vt, vc, vg, vo, vv})
     if (s == W8_ERR_DEVICE_TIMEOUT) return s;
-  if (vt != W8_OK || vc != W8_OK)
-    w8host::set_error("a length or index in device memory lay outside its range (%s)",
-                      vt != W8_OK ? "attention over a cache" : "cache operation");
-  for (const int s : {v, va, vp, vt, vc})
+  const char* where = vt != W8_OK   ? "attention over a cache"
+                      : vc != W8_OK ? "cache operation"
+                      : vg != W8_OK ? "attention over a paged cache"
+                      : vo != W8_OK ? "paged cache operation"
+                      : vv != W8_OK ? "draft verification"
+                                    : nullptr;
+  if (where != nullptr) w8host::set_error("a length or index in device memory lay outside its range (%s)", where);
+  for (const int s : {v, va, vp, vt, vc, vg, vo, vv})
     if (s != W8_OK) return s;
   return W8_OK;
 }

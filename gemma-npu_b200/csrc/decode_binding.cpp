@@ -31,6 +31,11 @@ decltype(&w8_cache_evict_workspace_bytes) fn_evict_ws = nullptr;
 decltype(&w8_beam_select) fn_select = nullptr;
 decltype(&w8_beam_select_workspace_bytes) fn_select_ws = nullptr;
 decltype(&w8_cache_reorder) fn_reorder = nullptr;
+decltype(&w8_attention_paged) fn_paged = nullptr;
+decltype(&w8_attention_paged_workspace_bytes) fn_paged_ws = nullptr;
+decltype(&w8_paged_append) fn_paged_append = nullptr;
+decltype(&w8_page_assign) fn_assign = nullptr;
+decltype(&w8_draft_verify) fn_verify = nullptr;
 PyObject* check_status = nullptr;  // _lib.check(status, name): raises
 
 struct Refused : std::runtime_error {  // ValueError
@@ -170,6 +175,36 @@ PyObject* same(PyObject* o) {
   NEED(check_status != nullptr, "the binding is not bound to the library");       \
   NEED(nargs == (count), "wrong number of arguments");
 
+// A drafted tree's mask and its tokens' depths, each for all sequences or one for each.
+template <typename Args>
+void tree_depth(PyObject* tree, PyObject* depth, Args& a, int64_t B, int64_t N, at::Device dev) {
+  if (!is_none(tree)) {
+    const Tensor& t = tensor(tree, "tree");
+    NEED(t.dim() == 2 || t.dim() == 3, "tree must be [N, N] or [B, N, N]");
+    expect(t, "tree", at::kBool, dev);
+    if (t.dim() == 2)
+      expect_shape(t, "tree", {N, N});
+    else
+      expect_shape(t, "tree", {B, N, N});
+    unit_last(t, "tree");
+    a.tree = static_cast<const uint8_t*>(t.const_data_ptr());
+    a.tree_stride[0] = t.dim() == 3 ? t.stride(0) : 0;
+    a.tree_stride[1] = t.stride(t.dim() - 2);
+  }
+  if (!is_none(depth)) {
+    const Tensor& t = tensor(depth, "depth");
+    NEED(t.dim() == 1 || t.dim() == 2, "depth must be [N] or [B, N]");
+    expect(t, "depth", at::kInt, dev);
+    if (t.dim() == 1)
+      expect_shape(t, "depth", {N});
+    else
+      expect_shape(t, "depth", {B, N});
+    unit_last(t, "depth");
+    a.depth = t.const_data_ptr<int32_t>();
+    a.depth_stride = t.dim() == 2 ? t.stride(0) : 0;
+  }
+}
+
 // q, k, v, lens, k_new, v_new, tree, depth, window, scale, out, weights, weights_out, draft_weights
 PyObject* attention_tree(PyObject* const* arg, Py_ssize_t nargs) {
   ENTRY(14)
@@ -191,31 +226,7 @@ PyObject* attention_tree(PyObject* const* arg, Py_ssize_t nargs) {
   a.lens = vector(arg[3], "lens", {B}, at::kInt, dev).const_data_ptr<int32_t>();
   a.window = integer(arg[8], "window");
   a.scale = real(arg[9], "scale");
-  if (!is_none(arg[6])) {
-    const Tensor& t = tensor(arg[6], "tree");
-    NEED(t.dim() == 2 || t.dim() == 3, "tree must be [N, N] or [B, N, N]");
-    expect(t, "tree", at::kBool, dev);
-    if (t.dim() == 2)
-      expect_shape(t, "tree", {N, N});
-    else
-      expect_shape(t, "tree", {B, N, N});
-    unit_last(t, "tree");
-    a.tree = static_cast<const uint8_t*>(t.const_data_ptr());
-    a.tree_stride[0] = t.dim() == 3 ? t.stride(0) : 0;
-    a.tree_stride[1] = t.stride(t.dim() - 2);
-  }
-  if (!is_none(arg[7])) {
-    const Tensor& t = tensor(arg[7], "depth");
-    NEED(t.dim() == 1 || t.dim() == 2, "depth must be [N] or [B, N]");
-    expect(t, "depth", at::kInt, dev);
-    if (t.dim() == 1)
-      expect_shape(t, "depth", {N});
-    else
-      expect_shape(t, "depth", {B, N});
-    unit_last(t, "depth");
-    a.depth = t.const_data_ptr<int32_t>();
-    a.depth_stride = t.dim() == 2 ? t.stride(0) : 0;
-  }
+  tree_depth(arg[6], arg[7], a, B, N, dev);
   NEED(a.tree == nullptr || a.window == 0 || a.depth != nullptr || N == 0, "a tree with a window needs the tokens' depths");
   Tensor out;
   if (is_none(arg[10])) {
@@ -439,6 +450,223 @@ PyObject* cache_reorder(PyObject* const* arg, Py_ssize_t nargs) {
   Py_RETURN_NONE;
 }
 
+// The pool, tails and table of a paged cache as the C ABI takes them: arg k, v, k_scale, v_scale,
+// k_tail, v_tail, table, lens.
+template <typename Args>
+void paged_cache(PyObject* const* arg, Args& a, at::ScalarType dt, at::Device dev, bool written) {
+  const Tensor& k = rows4(arg[0], "k", at::kChar, dev, a.k_stride, 1);
+  const Tensor& v = rows4(arg[1], "v", at::kChar, dev, a.v_stride, 1);
+  const int64_t pages = k.size(0), KV = k.size(1), P = k.size(2), D = k.size(3);
+  NEED(v.sizes() == k.sizes(), "v must have the shape of k");
+  NEED(KV >= 1, "pages have no heads");
+  const char* scale_names[2] = {"k_scale", "v_scale"};
+  const char* tail_names[2] = {"k_tail", "v_tail"};
+  int64_t* scale_strides[2] = {a.k_scale_stride, a.v_scale_stride};
+  int64_t* tail_strides[2] = {a.k_tail_stride, a.v_tail_stride};
+  const Tensor* scales[2];
+  const Tensor* tails[2];
+  for (int i = 0; i < 2; ++i) {
+    const Tensor& s = tensor(arg[2 + i], scale_names[i]);
+    expect(s, scale_names[i], at::kFloat, dev);
+    expect_shape(s, scale_names[i], {pages, KV});
+    scale_strides[i][0] = s.stride(0), scale_strides[i][1] = s.stride(1);
+    scales[i] = &s;
+    const Tensor& t = rows4(arg[4 + i], tail_names[i], dt, dev, tail_strides[i], 1);
+    tails[i] = &t;
+    NEED(t.size(1) == KV && t.size(2) == P && t.size(3) == D, tail_names[i], " must be [B, KV, P, D] with the pages' KV, P and D");
+    if (written) {
+      disjoint(s, scale_names[i], 2);
+      disjoint(t, tail_names[i], 3);
+    }
+  }
+  const int64_t B = tails[0]->size(0);
+  NEED(tails[1]->size(0) == B, "v_tail must have the shape of k_tail");
+  if (written) {
+    disjoint(k, "k", 3);
+    disjoint(v, "v", 3);
+  }
+  const Tensor& table = tensor(arg[6], "table");
+  expect(table, "table", at::kInt, dev);
+  NEED(table.dim() == 2 && table.size(0) == B, "table must be [B, pages of a sequence]");
+  unit_last(table, "table");
+  a.table = table.const_data_ptr<int32_t>();
+  a.table_stride = table.stride(0);
+  a.table_pages = table.size(1);
+  a.lens = vector(arg[7], "lens", {B}, at::kInt, dev).const_data_ptr<int32_t>();
+  // (written only where `written` is true: the two structs differ in const)
+  a.k = static_cast<int8_t*>(const_cast<void*>(k.const_data_ptr()));
+  a.v = static_cast<int8_t*>(const_cast<void*>(v.const_data_ptr()));
+  a.k_scale = static_cast<float*>(const_cast<void*>(scales[0]->const_data_ptr()));
+  a.v_scale = static_cast<float*>(const_cast<void*>(scales[1]->const_data_ptr()));
+  a.k_tail = const_cast<void*>(tails[0]->const_data_ptr());
+  a.v_tail = const_cast<void*>(tails[1]->const_data_ptr());
+  a.batch = B, a.kv_heads = KV, a.head_dim = D, a.pages = pages, a.page = P, a.dtype = type_code(dt);
+}
+
+// q, k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_new, tree, depth, window, sink, scale, out
+PyObject* attention_paged(PyObject* const* arg, Py_ssize_t nargs) {
+  ENTRY(17)
+  w8_attention_paged_args a = {};
+  const Tensor& q = cuda_tensor(arg[0], "q");
+  const at::Device dev = q.device();
+  const at::ScalarType dt = q.scalar_type();
+  NEED(dt == at::kBFloat16 || dt == at::kHalf, "q must be bfloat16 or float16 (got ", dt, ")");
+  rows4(arg[0], "q", dt, dev, a.q_stride, 1);
+  paged_cache(arg + 1, a, dt, dev, false);
+  const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
+  NEED(a.batch == B && a.head_dim == D, "pages and tails must have q's batch and head size");
+  NEED(H % a.kv_heads == 0, "H = ", H, " must be a multiple of KV = ", a.kv_heads);
+  const Tensor& kn = rows4(arg[9], "k_new", dt, dev, a.k_new_stride, 1);
+  const Tensor& vn = rows4(arg[10], "v_new", dt, dev, a.v_new_stride, 1);
+  const int64_t new_shape[4] = {B, a.kv_heads, N, D};
+  NEED(kn.sizes() == at::IntArrayRef(new_shape) && vn.sizes() == kn.sizes(), "k_new and v_new must be [B, KV, N, D]");
+  a.window = integer(arg[13], "window");
+  a.sink = integer(arg[14], "sink");
+  a.scale = real(arg[15], "scale");
+  tree_depth(arg[11], arg[12], a, B, N, dev);
+  NEED(a.tree == nullptr || a.window == 0 || a.depth != nullptr || N == 0, "a tree with a window needs the tokens' depths");
+  Tensor out;
+  if (is_none(arg[16])) {
+    out = make({B, H, N, D}, dt, dev);
+    a.out_stride[0] = H * N * D, a.out_stride[1] = N * D, a.out_stride[2] = D;
+  } else {
+    out = rows4(arg[16], "out", dt, dev, a.out_stride, 1);
+    expect_shape(out, "out", q.sizes());
+    disjoint(out, "out", 3);
+  }
+  a.q = q.const_data_ptr(), a.k_new = kn.const_data_ptr(), a.v_new = vn.const_data_ptr(), a.out = out.data_ptr();
+  a.heads = H, a.n_new = N;
+  {
+    const c10::cuda::CUDAGuard guard(dev);
+    const Tensor ws = workspace(fn_paged_ws(&a), dev);
+    check(fn_paged(&a, ws.data_ptr(), ws.numel(), stream_of(dev)), "w8_attention_paged");
+  }
+  return is_none(arg[16]) ? wrap(out) : same(arg[16]);
+}
+
+// k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_new, path, count, lens_out
+PyObject* paged_append(PyObject* const* arg, Py_ssize_t nargs) {
+  ENTRY(13)
+  w8_paged_append_args a = {};
+  const Tensor& kn = cuda_tensor(arg[8], "k_new");
+  const at::Device dev = kn.device();
+  const at::ScalarType dt = kn.scalar_type();
+  NEED(dt == at::kBFloat16 || dt == at::kHalf, "k_new must be bfloat16 or float16 (got ", dt, ")");
+  rows4(arg[8], "k_new", dt, dev, a.k_new_stride, 1);
+  const Tensor& vn = rows4(arg[9], "v_new", dt, dev, a.v_new_stride, 1);
+  paged_cache(arg, a, dt, dev, true);
+  const int64_t B = a.batch, N = kn.size(2);
+  const int64_t new_shape[4] = {B, a.kv_heads, N, a.head_dim};
+  NEED(kn.sizes() == at::IntArrayRef(new_shape) && vn.sizes() == kn.sizes(), "k_new and v_new must be [B, KV, N, D]");
+  a.n_new = a.steps = N;
+  if (!is_none(arg[10])) {
+    const Tensor& p = tensor(arg[10], "path");
+    NEED(p.dim() == 2, "path must be [B, steps]");
+    expect(p, "path", at::kInt, dev);
+    a.steps = p.size(1);
+    expect_shape(p, "path", {B, a.steps});
+    unit_last(p, "path");
+    // An empty path is a path: nothing is appended and nothing of it is read.
+    a.path = a.steps > 0 ? p.const_data_ptr<int32_t>() : a.lens;
+    a.path_stride = p.stride(0);
+  }
+  if (!is_none(arg[11])) a.count = vector(arg[11], "count", {B}, at::kInt, dev).const_data_ptr<int32_t>();
+  const Tensor to = is_none(arg[12]) ? make({B}, at::kInt, dev) : vector(arg[12], "lens_out", {B}, at::kInt, dev);
+  a.k_new = kn.const_data_ptr(), a.v_new = vn.const_data_ptr();
+  a.lens_out = to.data_ptr<int32_t>();
+  {
+    const c10::cuda::CUDAGuard guard(dev);
+    check(fn_paged_append(&a, stream_of(dev)), "w8_paged_append");
+  }
+  return is_none(arg[12]) ? wrap(to) : same(arg[12]);
+}
+
+// table, lens, free, top, page, room, active, window, sink
+PyObject* page_assign(PyObject* const* arg, Py_ssize_t nargs) {
+  ENTRY(9)
+  w8_page_assign_args a = {};
+  const Tensor& table = cuda_tensor(arg[0], "table");
+  const at::Device dev = table.device();
+  expect(table, "table", at::kInt, dev);
+  NEED(table.dim() == 2, "table must be [B, pages of a sequence]");
+  unit_last(table, "table");
+  disjoint(table, "table", 1);
+  const int64_t B = table.size(0);
+  a.table = table.data_ptr<int32_t>();
+  a.table_stride = table.stride(0);
+  a.batch = B, a.table_pages = table.size(1);
+  a.lens = vector(arg[1], "lens", {B}, at::kInt, dev).const_data_ptr<int32_t>();
+  const Tensor& free = tensor(arg[2], "free");
+  NEED(free.dim() == 1, "free must be one-dimensional");
+  vector(arg[2], "free", {free.size(0)}, at::kInt, dev);
+  a.free = free.data_ptr<int32_t>();
+  a.free_pages = free.size(0);
+  a.top = vector(arg[3], "top", {1}, at::kInt, dev).data_ptr<int32_t>();
+  a.page = integer(arg[4], "page");
+  a.room = integer(arg[5], "room");
+  if (!is_none(arg[6]))
+    a.active = static_cast<const uint8_t*>(vector(arg[6], "active", {B}, at::kBool, dev).const_data_ptr());
+  a.window = integer(arg[7], "window");
+  a.sink = integer(arg[8], "sink");
+  const Tensor ok = make({B}, at::kBool, dev);
+  a.ok = static_cast<uint8_t*>(ok.data_ptr());
+  {
+    const c10::cuda::CUDAGuard guard(dev);
+    check(fn_assign(&a, stream_of(dev)), "w8_page_assign");
+  }
+  return wrap(ok);
+}
+
+// logits, tokens, uniform, parent, draft, temperature, cap
+PyObject* draft_verify(PyObject* const* arg, Py_ssize_t nargs) {
+  ENTRY(7)
+  w8_draft_verify_args a = {};
+  const Tensor& x = cuda_tensor(arg[0], "logits");
+  const at::Device dev = x.device();
+  const at::ScalarType dt = x.scalar_type();
+  NEED(type_code(dt) >= 0, "logits must be float32, bfloat16 or float16 (got ", dt, ")");
+  NEED(x.dim() == 3, "logits must be [B, N, V]");
+  const int64_t B = x.size(0), N = x.size(1), V = x.size(2);
+  unit_last(x, "logits");
+  a.logits = x.const_data_ptr();
+  a.logits_stride[0] = x.stride(0), a.logits_stride[1] = x.stride(1);
+  a.tokens = vector(arg[1], "tokens", {B, N}, at::kLong, dev).const_data_ptr<int64_t>();
+  a.temperature = real(arg[5], "temperature");
+  a.cap = is_none(arg[6]) ? 0.0 : real(arg[6], "cap");
+  if (!is_none(arg[2]))
+    a.uniform = static_cast<const float*>(vector(arg[2], "uniform", {B, N}, at::kFloat, dev).const_data_ptr());
+  else
+    NEED(a.temperature == 0.0, "uniform is needed but at temperature 0");
+  if (!is_none(arg[3])) {
+    const Tensor& t = tensor(arg[3], "parent");
+    NEED(t.dim() == 1 || t.dim() == 2, "parent must be [N] or [B, N]");
+    expect(t, "parent", at::kInt, dev);
+    if (t.dim() == 1)
+      expect_shape(t, "parent", {N});
+    else
+      expect_shape(t, "parent", {B, N});
+    unit_last(t, "parent");
+    a.parent = t.const_data_ptr<int32_t>();
+    a.parent_stride = t.dim() == 2 ? t.stride(0) : 0;
+  }
+  if (!is_none(arg[4])) {
+    const Tensor& t = tensor(arg[4], "draft");
+    expect(t, "draft", dt, dev);
+    expect_shape(t, "draft", x.sizes());
+    unit_last(t, "draft");
+    a.draft = t.const_data_ptr();
+    a.draft_stride[0] = t.stride(0), a.draft_stride[1] = t.stride(1);
+  }
+  const Tensor path = make({B, N}, at::kInt, dev), taken = make({B}, at::kInt, dev), token = make({B}, at::kLong, dev);
+  a.path = path.data_ptr<int32_t>(), a.taken = taken.data_ptr<int32_t>(), a.token = token.data_ptr<int64_t>();
+  a.batch = B, a.n_new = N, a.vocab = V, a.dtype = type_code(dt);
+  {
+    const c10::cuda::CUDAGuard guard(dev);
+    check(fn_verify(&a, stream_of(dev)), "w8_draft_verify");
+  }
+  return tuple_of({wrap(path), wrap(taken), wrap(token)});
+}
+
 // bind(library path, check): take the entry points from the loaded library.
 PyObject* bind(PyObject* const* arg, Py_ssize_t nargs) {
   NEED(nargs == 2 && PyUnicode_Check(arg[0]) && PyCallable_Check(arg[1]), "bind(path, check)");
@@ -460,6 +688,11 @@ PyObject* bind(PyObject* const* arg, Py_ssize_t nargs) {
   get(fn_select, "w8_beam_select");
   get(fn_select_ws, "w8_beam_select_workspace_bytes");
   get(fn_reorder, "w8_cache_reorder");
+  get(fn_paged, "w8_attention_paged");
+  get(fn_paged_ws, "w8_attention_paged_workspace_bytes");
+  get(fn_paged_append, "w8_paged_append");
+  get(fn_assign, "w8_page_assign");
+  get(fn_verify, "w8_draft_verify");
   check_status = same(arg[1]);
   Py_RETURN_NONE;
 }
@@ -497,6 +730,10 @@ PyMODINIT_FUNC PyInit__decode(void) {
       {"cache_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<cache_append>)), METH_FASTCALL, nullptr},
       {"cache_evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<cache_evict>)), METH_FASTCALL, nullptr},
       {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<beam_select>)), METH_FASTCALL, nullptr},
+      {"attention_paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<attention_paged>)), METH_FASTCALL, nullptr},
+      {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<paged_append>)), METH_FASTCALL, nullptr},
+      {"page_assign", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<page_assign>)), METH_FASTCALL, nullptr},
+      {"draft_verify", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<draft_verify>)), METH_FASTCALL, nullptr},
       {"cache_reorder", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<cache_reorder>)), METH_FASTCALL, nullptr},
       {nullptr, nullptr, 0, nullptr}};
   static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decode", "Binding of the decoding operators.", -1, methods,

@@ -11,12 +11,26 @@ new tokens to what came before, and keep it:
     beam_select(logits, scores, ..)                  beam search's selection over beams and
                       vocabulary, with the final softcap (pipeline.py:335-338) fused
     cache_reorder(caches, beam, lens)                the beams' states follow their parents
+    page_assign(table, lens, free, top, page, ..)    pages of a paged 8-bit cache given out and taken
+                      back, on the device
+    attention_paged(q, k, v, .., table, lens, k_new, v_new, ..)  attention_tree over such a cache,
+                      with a sliding window and sinks
+    paged_append(k, v, .., table, lens, k_new, v_new, path)      the accepted path into it
+    draft_verify(logits, tokens, uniform, ..)        which drafted tokens stand, and the token after
+                      them, from given random numbers
 
 A cache is [B, KV, S, D] (unit stride along D, any other strides: head-major, token-major, a
 slice of a bigger buffer); `lens` int32 [B] on its device counts each sequence's committed
 slots, and what lies behind them is not touched.  q, k_new and v_new have the head-major
 layout that `kernels.qkv_norm_rope` returns: for B sequences of N tokens,
 `q.unflatten(1, (B, N)).transpose(0, 1)` is the [B, H, N, D] view.
+
+A paged 8-bit cache (of one layer) is a pool of pages k, v int8 [pages, KV, P, D] with scales
+k_scale, v_scale fp32 [pages, KV] (a value is its 8 bits times its page's and head's scale), P =
+16, 32, 64 or 128, and the 16-bit rows of every sequence's last, partial page, k_tail, v_tail
+[B, KV, P, D].  table int32 [B, M] names a sequence's pages in order (negative: none), lens
+int32 [B] counts its positions: position p is row p % P of page table[b, p // P], or of the
+tail where p >= lens // P * P.  Table and lengths are shared by layers of one kind.
 
 Like every function of `kernels`, these check dtype, shape and layout on the host, run on
 torch's current stream of the tensors' device, copy nothing to the host and raise a W8Error
@@ -157,3 +171,80 @@ def cache_reorder(caches, beam, lens=None):
     slot costs nothing.  At most 32 beams."""
     (_binding or _c()).cache_reorder(caches if isinstance(caches, (list, tuple)) else [caches], beam, lens)
     return caches
+
+
+def page_assign(table, lens, free, top, page, room=1, active=None, window=0, sink=0):
+    """Give every request the pages that its next `room` tokens need, take back those that it
+    does not need, all on the device; returns ok bool [B].
+
+    table int32 [B, M] and the stack of free pages, free int32 [F] with top int32 [1] (free[0] to
+    free[top - 1] are free), are updated in place.  A request needs the pages (of `page` tokens:
+    16, 32, 64 or 128) of its first lens[b] + room positions; none if active (bool [B]) says that
+    it has ended; and with window W > 0 not those that lie wholly before the window of position
+    lens[b] and behind the first `sink` positions.  What a request holds and does not need goes
+    back first, then what is missing is given out, both in the order of the requests and their
+    tables, the stack's top first.  ok[b]: the request has all that it needs.  It is served if what
+    it and all requests before it miss is there, and always if it misses nothing; one that needs
+    more than M pages is not served.  A page belongs to one request; at most 8192 requests."""
+    return (_binding or _c()).page_assign(table, lens, free, top, page, room, active, window, sink)
+
+
+def attention_paged(q, k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_new, tree=None, depth=None,
+                    window=0, sink=0, scale=1.0, out=None):
+    """`attention_tree` over a paged 8-bit cache: N new tokens per sequence over its committed
+    positions and over one another; returns out [B, H, N, D].
+
+    q, k_new, v_new, tree, depth, scale and out as for attention_tree (bf16 or fp16, the tails
+    alike; D 64, 128, 256 or 512; 16-byte aligned, strides multiples of 8, pages' of 16).  With
+    window W > 0 a token sees the last W positions, its own included, and the positions below
+    `sink`, which stay visible (a tree then needs its depths).  Pages that no token sees are not
+    read and need not be in the table; a page that is needed and missing is skipped and
+    reported by `device_status`.
+
+    k_new and v_new may be infinite or NaN where some token must not see them; tail rows that a
+    window reaches, or sinks, must be finite.  Only q and out may be expanded or have other than
+    positive strides.  out must not overlap the inputs.  Inference only."""
+    return (_binding or _c()).attention_paged(q, k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_new,
+                                              tree, depth, window, sink, scale, out)
+
+
+def paged_append(k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_new, path=None, count=None,
+                 lens_out=None):
+    """Put new tokens' rows into a paged 8-bit cache, in place, and return the new lengths.
+
+    Rows path[b, 0], path[b, 1], ... of k_new, v_new [B, KV, N, D] (bf16 or fp16) go to the
+    positions lens[b], lens[b] + 1, ...; path int32 [B, steps] ends at a negative entry (None: all
+    N tokens in order), and with count int32 [B] at count[b] entries (prompts of several lengths).
+    They wait in the tail as they are; a page that becomes full is rounded to 8 bits at once, per
+    head: scale = m / 127 for its largest magnitude m, values round(127 x / m), halves to even.  A
+    page with an infinity or a NaN gets a scale of NaN.  The page must be in the table
+    (`page_assign`): one that is not is lost and reported by `device_status`.  Returns lens_out
+    int32 [B] (a tensor apart from lens, path and count).  k_new and v_new must not overlap the
+    cache."""
+    return (_binding or _c()).paged_append(k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_new, path,
+                                           count, lens_out)
+
+
+def draft_verify(logits, tokens, uniform, parent=None, draft=None, temperature=1.0, cap=0.0):
+    """Which nodes of a drafted tree stand, and the token after them: (path int32 [B, N], taken
+    int32 [B], token int64 [B]).
+
+    logits fp32, bf16 or fp16 [B, N, V] (unit stride along V) are the target's after each node,
+    tokens int64 [B, N] the nodes' tokens (node 0's is committed already), parent int32 [N] or
+    [B, N] each node's parent, which comes before it (negative: the node is not there; None: a
+    chain).  Speculative sampling: with p = softmax(y / temperature), y = cap * tanh(logits /
+    cap) with cap > 0 (1e-3 to 1e6), else the logits, and q = softmax(draft / temperature) of the
+    draft model's logits [B, N, V] after the same node, a node's children c in order:
+    c stands if uniform[b, c] * q(its token) < w(its token), w = p at first, and if not w becomes
+    max(w - q, 0) over its sum.  draft=None: the drafts were chosen, not sampled, q is 1 at the
+    child's token.  From the last node that stands the token is drawn from w, the first whose
+    running sum exceeds uniform[b, 0] of the whole.  uniform fp32 [B, N] in [0, 1).  The tokens then
+    have the target's distribution, whatever the drafts.
+
+    temperature=0 (else 1e-3 to 1e3): a child stands if it is the largest logit (equal ones: the
+    lowest token), which is also the token after the last; uniform may be None.  A logit of -inf
+    is an impossible token.  A node whose target logits hold a NaN or no finite largest one ends
+    the walk with token -1; one whose draft logits do keeps no child.  path (node 0 first, then
+    -1) is what `cache_append` and `paged_append` take.  At most 1024 nodes; a token outside [0, V)
+    does not stand and is reported by `device_status`."""
+    return (_binding or _c()).draft_verify(logits, tokens, uniform, parent, draft, temperature, cap)

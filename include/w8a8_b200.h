@@ -406,6 +406,116 @@ int w8_cache_reorder(void* const* tensors, int64_t count, const int64_t* strides
                      const int32_t* lens, int64_t groups, int64_t beams, int64_t heads, int64_t slots,
                      int64_t row_bytes, w8_stream_t stream);
 
+/* ---- a paged 8-bit cache ------------------------------------------------ */
+
+/* The keys and values of a position whose page is full are signed 8-bit values of one scale a
+ * page and cache head; the positions of a sequence's last, partial page are 16-bit rows of its
+ * tail.  Position p < lens[b] / page * page of sequence b is row p % page of the pool's page
+ * table[b, p / page], a later one row p % page of tail b. */
+typedef struct w8_attention_paged_args {
+  const void* q;                  /* [batch, heads, n_new] rows of head_dim */
+  const int8_t *k, *v;            /* pool: [pages, kv_heads, page] rows of head_dim bytes */
+  const float *k_scale, *v_scale; /* [pages, kv_heads]: k8 * scale is the key */
+  const void *k_tail, *v_tail;    /* [batch, kv_heads, page] rows */
+  const void *k_new, *v_new;      /* [batch, kv_heads, n_new] rows */
+  void* out;                      /* [batch, heads, n_new] rows */
+  const int32_t* table;           /* [batch, table_pages]: page numbers; negative: none */
+  const int32_t* lens;            /* [batch] committed positions */
+  const uint8_t* tree;            /* as in w8_attention_tree_args, and depth */
+  const int32_t* depth;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch or page, head, row; elements */
+  int64_t k_scale_stride[2], v_scale_stride[2];
+  int64_t k_tail_stride[3], v_tail_stride[3], k_new_stride[3], v_new_stride[3], out_stride[3];
+  int64_t table_stride, tree_stride[2], depth_stride;
+  int64_t batch, heads, kv_heads, head_dim, pages, page, table_pages, n_new, window, sink, dtype;
+  double scale;
+} w8_attention_paged_args;
+
+/* w8_attention_tree over such a cache (without weights): new token i of sequence b sees the
+ * committed positions j < lens[b] and the new tokens that tree names, with window > 0 cut to the
+ * last `window` positions and those below `sink`, which stay visible.  Pages of 16, 32, 64 or
+ * 128 tokens; head_dim 64, 128, 256 or 512.  A page that holds nothing any row sees is not read
+ * and its table entry not followed; one that is needed and not in the pool is skipped and
+ * reported by w8_device_status.  Tails, new rows and pages have positive strides; new values may
+ * be infinite or NaN where some token must not see them; tail rows that any token's window
+ * reaches, or sinks, must be finite.  out must not overlap the inputs. */
+int w8_attention_paged(const w8_attention_paged_args* args, void* workspace, int64_t workspace_bytes,
+                       w8_stream_t stream);
+/* Workspace in bytes (16-byte aligned; -1 on a bad shape); only the sizes are looked at. */
+int64_t w8_attention_paged_workspace_bytes(const w8_attention_paged_args* args);
+
+typedef struct w8_paged_append_args {
+  int8_t *k, *v;                 /* the pool, as in w8_attention_paged_args */
+  float *k_scale, *v_scale;
+  void *k_tail, *v_tail;
+  const int32_t* table;
+  const int32_t* lens;
+  const void *k_new, *v_new;     /* [batch, kv_heads, n_new] rows of head_dim */
+  const int32_t* path;           /* [batch, steps] indexes of new tokens, ended by a negative one; NULL: in order */
+  const int32_t* count;          /* [batch]: at most so many of them; NULL: all */
+  int32_t* lens_out;             /* [batch], of no memory in common with lens, path or count */
+  int64_t k_stride[3], v_stride[3], k_scale_stride[2], v_scale_stride[2]; /* elements */
+  int64_t k_tail_stride[3], v_tail_stride[3], k_new_stride[3], v_new_stride[3];
+  int64_t table_stride, path_stride;
+  int64_t batch, kv_heads, head_dim, pages, page, table_pages, n_new, steps, dtype; /* steps = n_new without a path */
+} w8_paged_append_args;
+
+/* Rows path[b, 0], path[b, 1], ... of the new keys and values go to the positions lens[b],
+ * lens[b] + 1, ... of a paged 8-bit cache; lens_out[b] = lens[b] + their number.  A page that
+ * becomes full gets scale = m / 127 (m its head's largest magnitude) and round(127 x / m),
+ * halves to even, from the 16-bit rows; the rows behind the last full page go into the tail.  A
+ * page with an infinity or a NaN gets a scale of NaN.  A page that the table does not have is lost
+ * and reported by w8_device_status, and so are positions behind the table.  The new rows must not
+ * overlap the pages and tails, and no page may stand in the table twice. */
+int w8_paged_append(const w8_paged_append_args* args, w8_stream_t stream);
+
+typedef struct w8_page_assign_args {
+  int32_t* table;        /* [batch, table_pages]: page numbers; negative: none */
+  const int32_t* lens;   /* [batch] */
+  const uint8_t* active; /* [batch], or NULL: all requests are */
+  int32_t* free;         /* [free_pages], a stack: free[0 .. *top - 1] are free pages */
+  int32_t* top;          /* one number */
+  uint8_t* ok;           /* [batch]: the request has what it needs */
+  int64_t table_stride, batch, table_pages, free_pages, page, room, window, sink;
+} w8_page_assign_args;
+
+/* Page tables for the next step: request b needs the pages of its first lens[b] + room
+ * positions, none if it is not active, and with window > 0 none that lies wholly before the
+ * window of position lens[b] and behind the first `sink` positions.  First every page that a
+ * request holds and does not need goes back onto the stack, by request and place in the table;
+ * then the missing ones are given out in the same order from its top.  A request is served if
+ * what it and all requests before it miss is there; one that misses nothing is, and one that
+ * needs more pages than a table has is not and does not count.  A request whose length is out of
+ * range keeps what it has.  At most 8192 requests. */
+int w8_page_assign(const w8_page_assign_args* args, w8_stream_t stream);
+
+typedef struct w8_draft_verify_args {
+  const void* logits;    /* [batch, n_new, vocab]: the target's after each node */
+  const void* draft;     /* the draft model's, like logits; NULL: the drafts were chosen, not sampled */
+  const int64_t* tokens; /* [batch, n_new]: node 0's is committed already */
+  const int32_t* parent; /* [batch, n_new]: parent[i] < i; negative: not there; NULL: i - 1 */
+  const float* uniform;  /* [batch, n_new] in [0, 1): of the next token at 0, then of each draft; may be NULL when greedy */
+  int32_t* path;         /* [batch, n_new] nodes that stand, node 0 first, then -1 */
+  int32_t* taken;        /* [batch] their number */
+  int64_t* token;        /* [batch] the token after them */
+  int64_t logits_stride[2], draft_stride[2], parent_stride; /* batch, node; elements; parent 0: shared */
+  int64_t batch, n_new, vocab, dtype; /* W8_BF16, W8_FP16 or W8_FP32, of both logits */
+  double temperature, cap;            /* 0: greedy, the largest logit; cap 0: none */
+} w8_draft_verify_args;
+
+/* Speculative sampling over a drafted tree.  With p_i = softmax(y / temperature) of node i's
+ * logits, y = cap tanh(logit / cap), and q_i = softmax(draft logits / temperature) (without draft
+ * logits 1 at the child's token), from node 0: node i's children c in order, w = p_i,
+ *   c stands if uniform[c] q_i(t_c) < w(t_c);  else w = max(w - q_i, 0) over its sum
+ * (unchanged if nothing is left), and the walk goes on from the child that stands.  Where none
+ * does, token is the first t with sum_{v <= t} w(v) > uniform[0] sum_v w(v).  Probabilities and
+ * sums that decide a token are held in 64 bits.  At temperature 0 a child stands if its token is
+ * the largest logit's, the lowest of equal ones, and token is the last node's largest.  A logit of
+ * -inf is an impossible token.  A node whose target row has a NaN or no finite largest logit ends
+ * the walk with token -1; one whose draft row has none keeps no child.  At most 1024 nodes; a
+ * token out of range does not stand and is reported by w8_device_status. */
+int w8_draft_verify(const w8_draft_verify_args* args, w8_stream_t stream);
+
 /* ---- quantisation ------------------------------------------------------ */
 
 /* Per-row symmetric int8: s[r] = max(absmax(x[r,:]), 1e-8) / 127 (fp32, IEEE divide),
