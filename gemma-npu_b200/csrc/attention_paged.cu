@@ -41,45 +41,53 @@ constexpr int kPagedThreads = 32 * kPagedWarps;
 __device__ __forceinline__ void paged_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
 __device__ __forceinline__ void paged_fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
 
-template <int D, int MT>
+template <int D, int NT>
 struct PagedCfg {
-  static constexpr int kBM = 16 * MT;
-  static constexpr int kTeam = D == 512 ? 2 : 1;           // warps that share 16 keys
-  static constexpr int kGroups = kTreeWarps / kTeam;
+  static constexpr int kBM = 8 * NT;
+  static constexpr int kTeams = D == 512 ? 2 : 1;          // sets of warps that take the tiles in turn
+  static constexpr int kGroups = kTreeWarps / kTeams;
   static constexpr int kSteps = D == 64 ? 2 : 1;           // 16-key steps of a warp in a tile
   static constexpr int kBN = kGroups * kSteps * 16;        // keys of a tile of pages: 256, 128, 128, 64
   static constexpr int kBN16 = kBN / 2;                    // of a 16-bit tile, which is as large
   static constexpr int kSlotBytes = kBN * D;               // 16 KB (D <= 128) or 32 KB
-  static constexpr int kSlots = 196608 / kSlotBytes;
-  static constexpr int kPitch = D + 8;                     // fp32 row pitch of the joint outputs
+  static constexpr int kSlots = 163840 / kSlotBytes;       // 10 or 5
+  static constexpr int kJoin = 1024 / kBM < D ? 1024 / kBM : D;  // columns of the outputs joined at a time
+  static constexpr int kPitch = kJoin + 4;                 // their fp32 row pitch
   static constexpr int kOffQ8 = kSlots * kSlotBytes;       // Q as fp16, scaled and permuted
   static constexpr int kOffQ16 = kOffQ8 + kBM * D * 2;     // Q as it is
-  static constexpr int kOffStat = kOffQ16 + kBM * D * 2;   // float [2][kGroups][kBM]: maxima, sums
-  static constexpr int kOffFac = kOffStat + 2 * kGroups * kBM * 4;  // float [kBM]: Q's scale taken back
-  static constexpr int kOffScale = kOffFac + kBM * 4;      // float [kSlots][kPagedMaxBoxes]
+  static constexpr int kOffJoin = kOffQ16 + kBM * D * 2;   // float [8][kBM][kPitch]
+  static constexpr int kOffStat = kOffJoin + kTreeWarps * kBM * kPitch * 4;  // float [2][8][kBM]: maxima, sums
+  static constexpr int kOffRow = kOffStat + 2 * kTreeWarps * kBM * 4;  // int4 [kBM]: token, depth, first key, Q's scale taken back
+  static constexpr int kOffScale = kOffRow + kBM * 16;     // float [kSlots][kPagedMaxBoxes]
   static constexpr int kOffMask = kOffScale + kSlots * kPagedMaxBoxes * 4;  // uint32 [kSlots]: boxes that are there
-  static constexpr int kOffBar = kOffMask + kSlots * 4;
+  static constexpr int kOffBar = kOffMask + (kSlots * 4 + 15) / 16 * 16;
   static constexpr int kNumBars = 2 * kSlots;              // full, empty
   static constexpr int kSmem = kOffBar + kNumBars * 8 + 16 + 1024;
   static_assert(kSmem <= 232448, "shared memory budget exceeded");
-  static_assert(kGroups * kBM * kPitch * 4 <= kOffQ8, "the joint outputs fit over the ring");
-  static_assert(kOffBar % 8 == 0 && kOffScale % 16 == 0, "alignment");
+  static_assert(kOffBar % 16 == 0 && kOffScale % 16 == 0 && kOffRow % 16 == 0, "alignment");
 };
 
 __device__ __forceinline__ float paged_ks(const PagedArgs& a, int page, int c) { return a.ks[page * a.ks_p + c * a.ks_h]; }
 __device__ __forceinline__ float paged_vs(const PagedArgs& a, int page, int c) { return a.vs[page * a.vs_p + c * a.vs_h]; }
 
-template <typename T, int D, int MT>
+// 8 x 8 values of 16 bits across a warp, transposed: from a thread's (row lane / 4, columns 2 (lane % 4)
+// and the next) to its (column lane / 4, rows 2 (lane % 4) and the next).
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kPagedThreads, 1)
     attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
                       const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_vn,
                       const __grid_constant__ PagedArgs pa) {
-  using C = PagedCfg<D, MT>;
+  using C = PagedCfg<D, NT>;
   using H = __half;
   constexpr int BM = C::kBM, BN = C::kBN, BN16 = C::kBN16, NS = C::kSlots, CH = D / 8;  // CH: 16-byte chunks of a 16-bit row
-  constexpr int DW = D / C::kTeam;                   // output columns of a warp
-  constexpr bool kQRegs = MT == 1 && D <= 128;       // Q's fragments stay in registers
+  constexpr bool kQRegs = NT * D <= 256;             // Q's fragments stay in registers
   constexpr int kRowBytes = D < 128 ? D : 128;       // of a box's row in shared memory
   const TreeArgs& a = pa.t;
   extern __shared__ uint8_t smem_raw[];
@@ -87,8 +95,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
   const uint32_t sq8 = base + C::kOffQ8, sq16 = base + C::kOffQ16, bar0 = base + C::kOffBar;
+  float* joint = reinterpret_cast<float*>(smem + C::kOffJoin);
   float* stat = reinterpret_cast<float*>(smem + C::kOffStat);
-  float* qfac = reinterpret_cast<float*>(smem + C::kOffFac);
+  int4* row_info = reinterpret_cast<int4*>(smem + C::kOffRow);
   volatile float* scales = reinterpret_cast<volatile float*>(smem + C::kOffScale);
   volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(smem + C::kOffMask);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffBar + C::kNumBars * 8);
@@ -157,7 +166,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       split_pair(p, pb, prt);
       return paged_span<BM, BN, BN16>(pa, tree_len(a, pb), prt).tiles();
     };
-    long long* sched = reinterpret_cast<long long*>(smem);  // (the ring is not in use yet)
+    long long* sched = reinterpret_cast<long long*>(joint);  // (not in use yet)
     long long sum = 0, round;
     for (int p = tid; p < pairs; p += kPagedThreads) sum += pair_tiles(p);
     long long excl = block_scan<kPagedWarps>(sum, sched, round);  // (of few pairs also each one's place)
@@ -193,7 +202,6 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     const int tiles = span.tiles();
     c = static_cast<int>(div_short(pos - item_pos, tiles));
     item_pos += static_cast<long long>(c) * tiles;
-    fence_proxy_async_smem();  // the TMA writes the ring next
     __syncthreads();
   }
   int nt = span.tiles();
@@ -221,53 +229,15 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     return (t < span.tail ? t : t - span.tail) * BN16;
   };
 
-  auto rows_sync = [&]() {  // of the 8 warps without the producer
-    __syncwarp();
-    asm volatile("bar.sync 1, %0;" ::"n"(kTreeThreads) : "memory");
-  };
-  auto rows_sync_and = [&](bool on) {
-    uint32_t all;
-    __syncwarp();
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 q, %1, 0;\n\t"
-        "bar.red.and.pred p, 1, %2, q;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(all)
-        : "r"(on ? 1u : 0u), "n"(kTreeThreads)
-        : "memory");
-    return all != 0u;
-  };
-  const int grp = warp / C::kTeam, part = warp % C::kTeam;  // 16-key group of a step; column part
-  const int rl = lane >> 2, arow = lane & 15;
   uint32_t g = 0;  // ring steps so far (each tile's K, then V)
   bool ok = true;
-  // Between items the producer and the 8 warps meet twice: everybody has left the ring (and no wait
-  // gave up), and it may be filled again.
-  auto item_done = [&](bool on) {
-    uint32_t all;
-    __syncwarp();
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 q, %1, 0;\n\t"
-        "bar.red.and.pred p, 2, %2, q;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(all)
-        : "r"(on ? 1u : 0u), "n"(kTreeThreads + 32)
-        : "memory");
-    return all != 0u;
-  };
-  auto item_free = [&]() {
-    __syncwarp();
-    asm volatile("bar.sync 3, %0;" ::"n"(kTreeThreads + 32) : "memory");
-  };
   __syncwarp();
   if (warp >= kTreeWarps) {
     // ---- the producer: each tile's K and V boxes into the ring as its slots are left, the table
     // entries and scales of the next tile under way meanwhile.
     paged_fewer_registers();
     if (warp > kTreeWarps) return;
-    while (true) {
+    while (ok) {
       const int t0 = static_cast<int>(pos - item_pos);
       const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
       const int* table = pa.table + b * pa.table_b;
@@ -285,17 +255,16 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       };
       int page = page_of(t0);
       float ks = page >= 0 ? paged_ks(pa, page, c) : 0.f, vs = page >= 0 ? paged_vs(pa, page, c) : 0.f;
-      bool put = true;
-      for (int t = t0; t < t1 && put; ++t) {
+      for (int t = t0; t < t1 && ok; ++t) {
         const int kind = kind_of(t), key0 = key0_of(t);
         const int next = page_of(t + 1);
         const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t step = g + 2 * (t - t0) + kv, slot = step % NS, dst = base + slot * C::kSlotBytes;
-          put = put && mbar_wait_bounded(empty_bar(slot), ((step / NS) & 1u) ^ 1u, abort_flag, &g_tree_status);
-          put = __all_sync(0xffffffffu, put);
-          if (!put) break;
+        for (int kv = 0; kv < 2; ++kv, ++g) {
+          const uint32_t slot = g % NS, dst = base + slot * C::kSlotBytes;
+          ok = ok && mbar_wait_bounded(empty_bar(slot), ((g / NS) & 1u) ^ 1u, abort_flag, &g_tree_status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           if (kind == kPages) {
             if (lane < boxes) scales[slot * kPagedMaxBoxes + lane] = kv ? vs : ks;
             if (lane == 0) masks[slot] = there;
@@ -315,13 +284,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         page = next;
         if (page >= 0) ks = paged_ks(pa, page, c), vs = paged_vs(pa, page, c);
       }
-      ok = put;
-      g += 2 * (t1 - t0);
-      if (!item_done(ok)) break;
       pos += t1 - t0;
       if (pos >= stop) break;
       advance();
-      item_free();
     }
     if (!ok) {
       // A wait gave up: let the copies in flight land before the CTA exits.
@@ -329,526 +294,523 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       while (globaltimer() - since < 50000ull) {
       }
     }
-  } else {
-    paged_more_registers();
-    while (true) {
-      const int row0 = rt * BM, bc = b * a.kv_heads + c;
-      const int t0 = static_cast<int>(pos - item_pos);
-      const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
-      const bool whole = t0 == 0 && t1 == nt;
-      const int64_t part_row = (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * BM;
-      const int sink_left = a.sink - len;
-      if (t0 == 0 && tid == 0 && !a.direct) {
-        // The CTA that begins an item says where its pieces are: one in each CTA up to its last tile's.
-        const int last = deal_owner(deal, item_pos + nt - 1);
-        a.info[bc * a.row_tiles + rt] = make_int2(blockIdx.x, last - static_cast<int>(blockIdx.x) + 1);
+    return;
+  }
+  paged_more_registers();
+  auto rows_sync = [&]() {  // of the 8 warps without the producer
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(kTreeThreads) : "memory");
+  };
+  auto rows_sync_and = [&](bool on) {
+    uint32_t all;
+    __syncwarp();
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "bar.red.and.pred p, 1, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all)
+        : "r"(on ? 1u : 0u), "n"(kTreeThreads)
+        : "memory");
+    return all != 0u;
+  };
+  const int team = warp / C::kGroups, grp = warp % C::kGroups;  // 16-key group of a step
+  const int gl = lane >> 2, tl = lane & 3;  // a thread's keys (or columns) gl, gl + 8 and rows 2 tl, 2 tl + 1
+  while (true) {
+    const int row0 = rt * BM, bc = b * a.kv_heads + c;
+    const int t0 = static_cast<int>(pos - item_pos);
+    const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
+    const bool whole = t0 == 0 && t1 == nt;
+    const int64_t part_row = (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * BM;
+    const int sink_left = a.sink - len;
+    if (t0 == 0 && tid == 0 && !a.direct) {
+      // The CTA that begins an item says where its pieces are: one in each CTA up to its last tile's.
+      const int last = deal_owner(deal, item_pos + nt - 1);
+      a.info[bc * a.row_tiles + rt] = make_int2(blockIdx.x, last - static_cast<int>(blockIdx.x) + 1);
+    }
+    // Q rows r = i * group + g (query head c * group + g of new token i), a row a warp: as they
+    // are, and scaled into fp16's range with 16 columns at a time in the order in which a thread's 4
+    // bytes of K come: columns 4 t .. 4 t + 3 as elements 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+    for (int r = warp; r < BM; r += kTreeWarps) {
+      float most = 0.f;
+      uint4 w[(CH + 31) / 32];
+      int i = -1, gq = 0, dep = 0, first = INT32_MAX;  // (no row: sees nothing)
+      if (row0 + r < rows) {
+        tree_row(a, row0 + r, i, gq);
+        dep = tree_depth(a, b, i);
+        first = tree_first(a, len, dep);
       }
-      // Q rows r = i * group + g (query head c * group + g of new token i).
-      for (int e = tid; e < BM * CH; e += kTreeThreads) {
-        const int r = e / CH, ch = e % CH;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (row0 + r < rows) {
-          int i, gq;
-          tree_row(a, row0 + r, i, gq);
-          w = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + gq) * a.q_h +
-                                              i * a.q_t + ch * 8);
-        }
-        st_shared_v4(sq16 + r * (D * 2) + ((ch ^ (r & 7)) << 4), w.x, w.y, w.z, w.w);
+#pragma unroll
+      for (int x = 0; x < (CH + 31) / 32; ++x) {
+        const int ch = lane + 32 * x;
+        w[x] = make_uint4(0, 0, 0, 0);
+        if (ch < CH && i >= 0)
+          w[x] = *reinterpret_cast<const uint4*>(a.q + b * a.q_b + (static_cast<int64_t>(c) * a.group + gq) * a.q_h +
+                                                 i * a.q_t + ch * 8);
+        const uint32_t ws[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          most = fmaxf(most, fmaxf(fabsf(tree_f32<T>(ws[e] & 0xFFFFu)), fabsf(tree_f32<T>(ws[e] >> 16))));
+        if (ch < CH) st_shared_v4(sq16 + r * (D * 2) + ((ch ^ (r & 7)) << 4), w[x].x, w[x].y, w[x].z, w[x].w);
       }
-      rows_sync();
-      // The same scaled into fp16's range, 16 columns at a time in the order in which a thread's 4
-      // bytes of K come: columns 4 t .. 4 t + 3 as elements 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
-      for (int r = warp; r < BM; r += kTreeWarps) {
-        float most = 0.f;
-        uint4 w[(CH + 31) / 32];
 #pragma unroll
-        for (int x = 0; x < (CH + 31) / 32; ++x) {
-          const int ch = lane + 32 * x;
-          w[x] = make_uint4(0, 0, 0, 0);
-          if (ch < CH) w[x] = *reinterpret_cast<const uint4*>(smem + C::kOffQ16 + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-          const uint32_t ws[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+      for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+      // 2^(14 - exponent), at most 2^100; 1 for a row of zeros or infinities.
+      const int ex = static_cast<int>(__float_as_uint(most) >> 23);
+      const int up = ex == 0 || ex == 255 ? 0 : min(14 + 127 - ex, 100);
+      const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+      if (lane == 0) row_info[r] = make_int4(i, dep, first, (127 - up) << 23);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            most = fmaxf(most, fmaxf(fabsf(tree_f32<T>(ws[e] & 0xFFFFu)), fabsf(tree_f32<T>(ws[e] >> 16))));
-        }
+      for (int x = 0; x < (CH + 31) / 32; ++x) {
+        const int ch = lane + 32 * x;
+        if (ch >= CH) break;
+        const uint32_t ws[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+        uint32_t h[4];
 #pragma unroll
-        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        // 2^(14 - exponent), at most 2^100; 1 for a row of zeros or infinities.
-        const int ex = static_cast<int>(__float_as_uint(most) >> 23);
-        const int up = ex == 0 || ex == 255 ? 0 : min(14 + 127 - ex, 100);
-        const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-        if (lane == 0) qfac[r] = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
-#pragma unroll
-        for (int x = 0; x < (CH + 31) / 32; ++x) {
-          const int ch = lane + 32 * x;
-          if (ch >= CH) break;
-          const uint32_t ws[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
-          uint32_t h[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) h[e] = pack2<H>(tree_f32<T>(ws[e] & 0xFFFFu) * f, tree_f32<T>(ws[e] >> 16) * f);
-          uint8_t* row = smem + C::kOffQ8 + r * (D * 2) + 8 * (ch & 1);
-          *reinterpret_cast<uint2*>(row + (((ch & ~1) ^ (r & 7)) << 4)) = make_uint2(h[0], h[2]);
-          *reinterpret_cast<uint2*>(row + (((ch | 1) ^ (r & 7)) << 4)) = make_uint2(h[1], h[3]);
-        }
+        for (int e = 0; e < 4; ++e) h[e] = pack2<H>(tree_f32<T>(ws[e] & 0xFFFFu) * f, tree_f32<T>(ws[e] >> 16) * f);
+        uint8_t* row = smem + C::kOffQ8 + r * (D * 2) + 8 * (ch & 1);
+        *reinterpret_cast<uint2*>(row + (((ch & ~1) ^ (r & 7)) << 4)) = make_uint2(h[0], h[2]);
+        *reinterpret_cast<uint2*>(row + (((ch | 1) ^ (r & 7)) << 4)) = make_uint2(h[1], h[3]);
       }
-      float m[MT][2], l[MT][2];
-      float o[MT][DW / 8][4];
+    }
+    rows_sync();
+    float m[NT][2], l[NT][2], fac[NT][2];
+    float o[NT][D / 16][4];  // O transposed: columns gl and gl + 8 of 16 (or 2 gl and 2 gl + 1), rows 2 tl, 2 tl + 1
+    int last_first = 0;      // the latest first key of the item's rows
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) m[mt][h] = -INFINITY, l[mt][h] = 0.f;
-#pragma unroll
-        for (int n = 0; n < DW / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+      for (int h = 0; h < 2; ++h) {
+        const int4 info = row_info[8 * n + 2 * tl + h];
+        m[n][h] = -INFINITY, l[n][h] = 0.f;
+        fac[n][h] = __int_as_float(info.w) * a.scale_log2;
+        if (info.x >= 0) last_first = max(last_first, info.z);
       }
-      // This thread's rows of each 16-row tile: lane / 4 and lane / 4 + 8.
-      int tok[MT][2], dep[MT][2], first[MT][2];
-      float fac[MT][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][k][e] = 0.f;
+    }
+    last_first = __reduce_max_sync(0xffffffffu, last_first);
+    // Q^T as the B operand, two steps of the reduction (32 columns) at a time.
+    auto load_q = [&](uint32_t sq, int n, int k2, uint32_t (&q)[4]) {
+      const int r = 8 * n + (lane & 7);
+      ldsm_x4(sq + r * (D * 2) + (((4 * k2 + (lane >> 3)) ^ (r & 7)) << 4), q);
+    };
+    uint32_t qf[kQRegs ? NT : 1][kQRegs ? D / 32 : 1][4];
+    if constexpr (kQRegs) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k2 = 0; k2 < D / 32; ++k2) load_q(sq8, n, k2, qf[n][k2]);
+    }
+    // Whether row 8 n + 2 tl + h sees committed positions p0 + gl and p0 + gl + 8 (below `end`), as bits 0 and 1.
+    auto sees = [&](int n, int h, int p0, int end) {
+      const int4 info = row_info[8 * n + 2 * tl + h];
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int p = p0 + gl + 8 * e;
+        if (p < end && (p >= info.z || (p < a.sink && info.x >= 0))) bits |= 1u << e;
+      }
+      return bits;
+    };
+    // m moved where a row's maximum of the step (of this thread's keys: mx) asks for it; O and l with
+    // it, O by `unit` (the change of its unit) besides.
+    auto move_rows = [&](float (&mx)[NT][2], float unit) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int r = row0 + mt * 16 + rl + 8 * h;
-          int gq;
-          tree_row(a, r, tok[mt][h], gq);
-          if (r >= rows) tok[mt][h] = -1;
-          dep[mt][h] = r < rows ? tree_depth(a, b, tok[mt][h]) : 0;
-          first[mt][h] = r < rows ? tree_first(a, len, dep[mt][h]) : INT32_MAX;  // (no row: sees nothing)
+          float x = mx[n][h];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          const bool mv = x > m[n][h] + TreeRef<H>::kSlack;
+          const float to = x - TreeRef<H>::kBelow;
+          const float corr = mv ? ex2_tree(m[n][h] - to) : 1.f;
+          if (mv) m[n][h] = to;
+          l[n][h] *= corr;
+          const float f = corr * unit;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            o[n][k][h] *= f;
+            o[n][k][2 + h] *= f;
+          }
         }
-      rows_sync();
+    };
+    // The step's scores s (keys gl: 0, 1; gl + 8: 2, 3) to weights, and l.
+    auto weigh = [&](float (&s)[NT][4]) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) fac[mt][h] = qfac[mt * 16 + rl + 8 * h] * a.scale_log2;
-      uint32_t qf[kQRegs ? D / 16 : 1][4];
-      if constexpr (kQRegs) {
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          ldsm_x4(sq8 + arow * (D * 2) + (((2 * kk + (lane >> 4)) ^ (arow & 7)) << 4), qf[kk]);
-      }
-      // The committed positions p0 .. p0 + 15 below `end` that a row sees, as bits.
-      auto sees = [&](int mt, int h, int p0, int end) {
-        const int hi = min(end - p0, 16);
-        uint32_t bits = hi <= 0 ? 0u : (1u << hi) - 1u;
-        const int lo = first[mt][h] - p0;
-        if (lo > 0) {
-          uint32_t on = lo > 15 ? 0u : 0xFFFFFFFFu << lo;
-          const int sk = tok[mt][h] < 0 ? 0 : min(a.sink - p0, 16);
-          if (sk > 0) on |= (1u << sk) - 1u;
-          bits &= on;
+        for (int h = 0; h < 2; ++h) {
+          const float ref = m[n][h] == -INFINITY ? 0.f : m[n][h];
+          s[n][h] = ex2_tree(s[n][h] - ref);
+          s[n][2 + h] = ex2_tree(s[n][2 + h] - ref);
+          l[n][h] += s[n][h] + s[n][2 + h];
         }
-        return bits;
-      };
-      // Scores to weights: a row's maximum of the step, m moved if it must be, O and l with it by
-      // `unit` (the change of O's unit) besides.
-      auto move_rows = [&](const float (&mx)[MT][2], float unit) {
+    };
+    float unit = __uint_as_float(0x00800000u);  // of O (2^-126: nothing added yet)
+    bool permuted = true;
+    // O in order and in units of 1: of each 16 columns a thread holds 2 gl and 2 gl + 1 (the even and
+    // odd bytes of V's rows) and gets gl and gl + 8.
+    auto natural = [&]() {
+      permuted = false;
+      const int s0 = ((gl >> 1) << 2) | tl, s1 = s0 + 16;
+      const bool odd = gl & 1;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const bool mv = mx[mt][h] > m[mt][h] + TreeRef<H>::kSlack;
-            const float to = mx[mt][h] - TreeRef<H>::kBelow;
-            const float corr = mv ? ex2_tree(m[mt][h] - to) : 1.f;
-            if (mv) m[mt][h] = to;
-            l[mt][h] *= corr;
-            const float f = corr * unit;
-#pragma unroll
-            for (int n = 0; n < DW / 8; ++n) {
-              o[mt][n][2 * h] *= f;
-              o[mt][n][2 * h + 1] *= f;
-            }
+            const float v0 = o[n][k][h] * unit, v1 = o[n][k][2 + h] * unit;
+            const float a0 = __shfl_sync(0xffffffffu, v0, s0), a1 = __shfl_sync(0xffffffffu, v1, s0);
+            const float b0 = __shfl_sync(0xffffffffu, v0, s1), b1 = __shfl_sync(0xffffffffu, v1, s1);
+            o[n][k][h] = odd ? a1 : a0;
+            o[n][k][2 + h] = odd ? b1 : b0;
           }
-      };
-      float unit = __uint_as_float(0x00800000u);  // of O (2^-126: nothing added yet)
-      bool permuted = true;
-      // O in order and in units of 1: of each 16 columns a thread holds 4 t .. 4 t + 3 (the 8-column
-      // accumulators as even and odd columns) and gets 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t.
-      auto natural = [&]() {
-        permuted = false;
-        const int s0 = (lane & ~3) | ((lane & 3) >> 1), s1 = s0 + 2;
-        const bool up = lane & 1;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int n = 0; n < DW / 8; n += 2)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float v0 = o[mt][n][2 * h] * unit, v1 = o[mt][n + 1][2 * h] * unit;
-              const float v2 = o[mt][n][2 * h + 1] * unit, v3 = o[mt][n + 1][2 * h + 1] * unit;
-              const float a0 = __shfl_sync(0xffffffffu, v0, s0), a2 = __shfl_sync(0xffffffffu, v2, s0);
-              const float a1 = __shfl_sync(0xffffffffu, v1, s0), a3 = __shfl_sync(0xffffffffu, v3, s0);
-              const float b0 = __shfl_sync(0xffffffffu, v0, s1), b2 = __shfl_sync(0xffffffffu, v2, s1);
-              const float b1 = __shfl_sync(0xffffffffu, v1, s1), b3 = __shfl_sync(0xffffffffu, v3, s1);
-              o[mt][n][2 * h] = up ? a2 : a0;
-              o[mt][n][2 * h + 1] = up ? a3 : a1;
-              o[mt][n + 1][2 * h] = up ? b2 : b0;
-              o[mt][n + 1][2 * h + 1] = up ? b3 : b1;
-            }
-      };
-      const int col = (lane & 3) * 2;  // a thread's columns of an 8-column tile: col, col + 1
+    };
 
 #pragma unroll 1
-      for (int t = t0; t < t1; ++t, g += 2) {
-        const int kind = kind_of(t), tile0 = key0_of(t);
-        const uint32_t slot_k = g % NS, slot_v = (g + 1) % NS;
-        const uint32_t sk = base + slot_k * C::kSlotBytes, sv = base + slot_v * C::kSlotBytes;
-        if (ok) ok = mbar_wait_bounded(full_bar(slot_k), (g / NS) & 1u, abort_flag, &g_tree_status);
+    for (int t = t0; t < t1; ++t, g += 2) {
+      const uint32_t slot_k = g % NS, slot_v = (g + 1) % NS;
+      if (ok) ok = mbar_wait_bounded(full_bar(slot_k), (g / NS) & 1u, abort_flag, &g_tree_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (C::kTeams > 1 && ((t - t0) & (C::kTeams - 1)) != team) {
+        // Another team's tile (waited for all the same: a barrier's phase must not pass unseen).
+        ok = mbar_wait_bounded(full_bar(slot_v), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (kind == kPages) {
-          const uint32_t there = masks[slot_k];
+        if (lane == 0) {
+          mbar_arrive(empty_bar(slot_k));
+          mbar_arrive(empty_bar(slot_v));
+        }
+        __syncwarp();
+        continue;
+      }
+      const int kind = kind_of(t), tile0 = key0_of(t);
+      const uint32_t sk = base + slot_k * C::kSlotBytes, sv = base + slot_v * C::kSlotBytes;
+      if (kind == kPages) {
+        const uint32_t there = masks[slot_k];
 #pragma unroll
-          for (int st = 0; st < C::kSteps; ++st) {
-            const int kr = (grp * C::kSteps + st) * 16, key0 = tile0 + kr;  // this step's keys
-            const int bx = kr >> box_shift, br = kr & (box - 1);            // their box, and row in it
-            const uint32_t kbox = sk + bx * (box * D), vbox = sv + bx * (box * D);
-            // ---- S = Q K^T, 16 keys; a chunk of 16 bytes is one step of the reduction
-            float s[MT][2][4];
+        for (int st = 0; st < C::kSteps; ++st) {
+          const int kr = (grp * C::kSteps + st) * 16, key0 = tile0 + kr;  // this step's keys
+          const int bx = kr >> box_shift, br = kr & (box - 1);            // their box, and row in it
+          // Rows of 16 bytes that a lane names for ldmatrix: 8 keys, the next 8, and the next 16 columns
+          // of both.
+          const int lrow = br + (lane & 15);
+          const uint32_t off = bx * (box * D) + lrow * kRowBytes;
+          auto chunk = [&](int ch) -> uint32_t {
+            if constexpr (D >= 128) return (ch >> 3) * (box * 128) + (((ch & 7) ^ (lrow & 7)) << 4);
+            return (ch ^ ((lrow >> 1) & 3)) << 4;
+          };
+          // ---- S^T = K Q^T, 16 keys
+          float s[NT][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int e = 0; e < 8; ++e) s[mt][e >> 2][e & 3] = 0.f;
-            const int krow = br + ((lane >> 4) << 3) + (lane & 7);
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
-            for (int k2 = 0; k2 < D / 32; ++k2) {
-              uint32_t kb[4];
-              const int ch = 2 * k2 + ((lane >> 3) & 1);
-              if constexpr (D >= 128)
-                ldsm_x4(kbox + (ch >> 3) * (box * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), kb);
-              else
-                ldsm_x4(kbox + krow * kRowBytes + ((ch ^ ((krow >> 1) & 3)) << 4), kb);
+          for (int k2 = 0; k2 < D / 32; ++k2) {
+            uint32_t kb[4], x0[4], x1[4];
+            ldsm_x4(sk + off + chunk(2 * k2 + (lane >> 4)), kb);
+            paged_unpack<H>(kb[0], 0x4140u, 0x4342u, x0[0], x0[2]);
+            paged_unpack<H>(kb[1], 0x4140u, 0x4342u, x0[1], x0[3]);
+            paged_unpack<H>(kb[2], 0x4140u, 0x4342u, x1[0], x1[2]);
+            paged_unpack<H>(kb[3], 0x4140u, 0x4342u, x1[1], x1[3]);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                uint32_t b00, b01, b10, b11;
-                paged_unpack<H>(kb[e], 0x4140u, 0x4342u, b00, b01);
-                paged_unpack<H>(kb[2 + e], 0x4140u, 0x4342u, b10, b11);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                  if constexpr (kQRegs) {
-                    mma16816<H>(s[mt][0], qf[2 * k2 + e], b00, b01);
-                    mma16816<H>(s[mt][1], qf[2 * k2 + e], b10, b11);
-                  } else {
-                    uint32_t qa[4];
-                    const int r = mt * 16 + arow;
-                    ldsm_x4(sq8 + r * (D * 2) + (((2 * (2 * k2 + e) + (lane >> 4)) ^ (r & 7)) << 4), qa);
-                    mma16816<H>(s[mt][0], qa, b00, b01);
-                    mma16816<H>(s[mt][1], qa, b10, b11);
-                  }
-                }
-              }
-            }
-            // ---- masks and the running softmax.  Columns of a thread: key0 + 8 n + col + {0, 1}.
-            const float ks = scales[slot_k * kPagedMaxBoxes + bx];
-            const bool on = (there >> bx) & 1u;
-            uint32_t keep[MT][2];
-            float mx[MT][2];
-            bool move = false;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                keep[mt][h] = on ? sees(mt, h, key0, span.full) : 0u;
-                const float f = fac[mt][h] * ks;
-                float x = -INFINITY;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) {
-                    float& v = s[mt][n][2 * h + e];
-                    v = (keep[mt][h] >> (8 * n + col + e)) & 1u ? v * f : -INFINITY;
-                    x = fmaxf(x, v);
-                  }
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                mx[mt][h] = x;
-                move |= x > m[mt][h] + TreeRef<H>::kSlack;
-              }
-            if (st == C::kSteps - 1) {
-              __syncwarp();
-              if (lane == 0) mbar_arrive(empty_bar(slot_k));
-            }
-            if (st == 0) {
-              ok = mbar_wait_bounded(full_bar(slot_v), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-            }
-            const float vs = on ? scales[slot_v * kPagedMaxBoxes + bx] : 0.f;
-            const float need = paged_unit(vs);
-            if (__any_sync(0xffffffffu, move) || need > unit) {
-              const float to = fmaxf(need, unit);
-              move_rows(mx, unit * paged_unit_rcp(to));
-              unit = to;
-            }
-            const float vr = vs * paged_unit_rcp(unit);
-            uint32_t pw[MT][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float ref = m[mt][h] == -INFINITY ? 0.f : m[mt][h];
-                float p[2][2];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) p[n][e] = ex2_tree(s[mt][n][2 * h + e] - ref);
-                l[mt][h] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) p[n][e] *= vr;
-                if (vr != vr) {  // (a NaN scale is for the rows that see the page)
-#pragma unroll
-                  for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                      if (!((keep[mt][h] >> (8 * n + col + e)) & 1u)) p[n][e] = 0.f;
-                }
-                // The accumulator's layout of 16 x 16 is the A operand's.
-                pw[mt][h] = pack2<H>(p[0][0], p[0][1]);
-                pw[mt][2 + h] = pack2<H>(p[1][0], p[1][1]);
-              }
-            // ---- O += P V: of 16 bytes of a row of V the even columns are one operand, the odd ones
-            // the next.
-            const int vrow = br + ((lane >> 3) & 1) * 8 + (lane & 7);
-#pragma unroll
-            for (int c2 = 0; c2 < DW / 32; ++c2) {
-              uint32_t vb[4];
-              const int ch = part * (DW / 16) + 2 * c2 + (lane >> 4);
-              if constexpr (D >= 128)
-                ldsm_x4_t(vbox + (ch >> 3) * (box * 128) + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4), vb);
-              else
-                ldsm_x4_t(vbox + vrow * kRowBytes + ((ch ^ ((vrow >> 1) & 3)) << 4), vb);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                uint32_t e0, e1, o0, o1;
-                paged_unpack<H>(vb[2 * e], 0x4240u, 0x4341u, e0, o0);
-                paged_unpack<H>(vb[2 * e + 1], 0x4240u, 0x4341u, e1, o1);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                  mma16816<H>(o[mt][4 * c2 + 2 * e], pw[mt], e0, e1);
-                  mma16816<H>(o[mt][4 * c2 + 2 * e + 1], pw[mt], o0, o1);
-                }
+            for (int n = 0; n < NT; ++n) {
+              if constexpr (kQRegs) {
+                mma16816<H>(s[n], x0, qf[n][k2][0], qf[n][k2][1]);
+                mma16816<H>(s[n], x1, qf[n][k2][2], qf[n][k2][3]);
+              } else {
+                uint32_t q[4];
+                load_q(sq8, n, k2, q);
+                mma16816<H>(s[n], x0, q[0], q[1]);
+                mma16816<H>(s[n], x1, q[2], q[3]);
               }
             }
           }
-          if (!ok) break;
-        } else {
-          if (permuted) natural();
-          const bool fresh = kind == kNew;
-          const int kr = grp * 16, key0 = tile0 + kr;  // this step's keys (rows of the tail, or new tokens)
-          const int end = fresh ? a.n : len - span.full;
-          const bool work = kr < BN16 && key0 < end;   // (the same for the whole warp)
-          uint32_t pw[MT][4];
-          if (work) {
-            float s[MT][2][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) s[mt][e >> 2][e & 3] = 0.f;
-            const int krow = kr + (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              uint32_t kb[4];
-              ldsm_x4(sk + krow * 128 + (kk >> 2) * (BN16 * 128) + ((((kk & 3) * 2 + ((lane >> 3) & 1)) ^ (krow & 7)) << 4), kb);
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                uint32_t qa[4];
-                const int r = mt * 16 + arow;
-                ldsm_x4(sq16 + r * (D * 2) + (((2 * kk + (lane >> 4)) ^ (r & 7)) << 4), qa);
-                mma16816<T>(s[mt][0], qa, kb[0], kb[1]);
-                mma16816<T>(s[mt][1], qa, kb[2], kb[3]);
-              }
-            }
-            float mx[MT][2];
-            bool move = false;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                // (all lanes: the new tokens' masks are read by the warp)
-                const uint32_t keep = fresh ? tree_sees16(a, b, tok[mt][h], key0, dep[mt][h], sink_left)
-                                            : sees(mt, h, span.full + key0, len);
-                float x = -INFINITY;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) {
-                    float& v = s[mt][n][2 * h + e];
-                    v = (keep >> (8 * n + col + e)) & 1u ? v * a.scale_log2 : -INFINITY;
-                    x = fmaxf(x, v);
-                  }
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                mx[mt][h] = x;
-                move |= x > m[mt][h] + TreeRef<H>::kSlack;
-              }
-            if (__any_sync(0xffffffffu, move)) move_rows(mx, 1.f);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float ref = m[mt][h] == -INFINITY ? 0.f : m[mt][h];
-                float p[2][2];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) p[n][e] = ex2_tree(s[mt][n][2 * h + e] - ref);
-                l[mt][h] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
-                pw[mt][h] = pack2<T>(p[0][0], p[0][1]);
-                pw[mt][2 + h] = pack2<T>(p[1][0], p[1][1]);
-              }
+          if (st == C::kSteps - 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty_bar(slot_k));
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(empty_bar(slot_k));
-          ok = mbar_wait_bounded(full_bar(slot_v), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (work) {
-            // Rows behind the length or before the window may hold anything and 0 * NaN is NaN: zeros.
-            // So may a new token's values where some row must not see them: cleared here, added below
-            // to the rows that do.
-            uint32_t bad = 0;  // keys of this step whose values are not all finite (new tokens only)
-            if (fresh || key0 + 16 > end || span.full + key0 < span.low) {
-              for (int e = lane; e < 16 * (DW / 8); e += 32) {
-                const int r = e % 16, ch = part * (DW / 8) + e / 16, p = span.full + key0 + r;
-                uint4* w = reinterpret_cast<uint4*>(smem + (sv - base) + (ch >> 3) * (BN16 * 128) + (kr + r) * 128 +
-                                                    (((ch & 7) ^ ((kr + r) & 7)) << 4));
-                if (key0 + r >= end || (!fresh && p < span.low && p >= a.sink)) {
-                  *w = make_uint4(0, 0, 0, 0);
-                } else if (fresh) {
-                  uint4 x = *w;
-                  if (nonfinite_bits<T>(x.x) | nonfinite_bits<T>(x.y) | nonfinite_bits<T>(x.z) | nonfinite_bits<T>(x.w)) {
-                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+          // ---- scores in log2 units, masks, the running softmax
+          const float ks = scales[slot_k * kPagedMaxBoxes + bx];
+          const bool on = (there >> bx) & 1u;
+          const bool plain = on && key0 + 16 <= span.full && key0 >= last_first;  // all rows see all keys
+          float mx[NT][2];
+          bool move = false;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) xs[q] &= ~((nonfinite_bits<T>(xs[q]) >> 15) * 0xFFFFu);
-                    *w = x;
-                    bad |= 1u << r;
-                  }
-                }
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float f = fac[n][h] * ks;
+              s[n][h] *= f, s[n][2 + h] *= f;
+              if (!plain) {
+                const uint32_t keep = on ? sees(n, h, key0, span.full) : 0u;
+                if (!(keep & 1u)) s[n][h] = -INFINITY;
+                if (!(keep & 2u)) s[n][2 + h] = -INFINITY;
               }
-              bad = __reduce_or_sync(0xffffffffu, bad);
-              fence_proxy_async_smem();  // (the TMA writes this slot again later)
-              __syncwarp();
+              mx[n][h] = fmaxf(s[n][h], s[n][2 + h]);
+              move |= mx[n][h] > m[n][h] + TreeRef<H>::kSlack;
             }
-            const int vrow = kr + arow;
+          if (st == 0) {
+            ok = mbar_wait_bounded(full_bar(slot_v), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+          }
+          const float vs = on ? scales[slot_v * kPagedMaxBoxes + bx] : 0.f;
+          const float need = paged_unit(vs);
+          if (__any_sync(0xffffffffu, move) || need > unit) {
+            const float to = fmaxf(need, unit);
+            move_rows(mx, unit * paged_unit_rcp(to));
+            unit = to;
+          }
+          const float vr = vs * paged_unit_rcp(unit);
+          bool seen[NT][4];  // (looked at below only if vs is NaN)
 #pragma unroll
-            for (int n = 0; n < DW / 8; n += 2) {
-              uint32_t vb[4];
-              const int ch = part * (DW / 8) + n + (lane >> 4);
-              ldsm_x4_t(sv + vrow * 128 + (ch >> 3) * (BN16 * 128) + (((ch & 7) ^ (vrow & 7)) << 4), vb);
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                mma16816<T>(o[mt][n], pw[mt], vb[0], vb[1]);
-                mma16816<T>(o[mt][n + 1], pw[mt], vb[2], vb[3]);
+            for (int e = 0; e < 4; ++e) seen[n][e] = s[n][e] != -INFINITY;
+          weigh(s);
+          uint32_t pw[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[e] = s[n][e] * vr;
+            if (vr != vr) {  // (a NaN scale is for the rows that see the page)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!seen[n][e]) p[e] = 0.f;
+            }
+            pw[n][0] = transpose8x8(pack2<H>(p[0], p[1]));
+            pw[n][1] = transpose8x8(pack2<H>(p[2], p[3]));
+          }
+          // ---- O^T += V^T P^T: of 16 bytes of a row of V the even columns are 8 rows of the operand, the
+          // odd ones the others.
+#pragma unroll
+          for (int c2 = 0; c2 < D / 32; ++c2) {
+            uint32_t vb[4], x0[4], x1[4];
+            ldsm_x4_t(sv + off + chunk(2 * c2 + (lane >> 4)), vb);
+            paged_unpack<H>(vb[0], 0x4240u, 0x4341u, x0[0], x0[1]);
+            paged_unpack<H>(vb[1], 0x4240u, 0x4341u, x0[2], x0[3]);
+            paged_unpack<H>(vb[2], 0x4240u, 0x4341u, x1[0], x1[1]);
+            paged_unpack<H>(vb[3], 0x4240u, 0x4341u, x1[2], x1[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma16816<H>(o[n][2 * c2], x0, pw[n][0], pw[n][1]);
+              mma16816<H>(o[n][2 * c2 + 1], x1, pw[n][0], pw[n][1]);
+            }
+          }
+        }
+        if (!ok) break;
+      } else {
+        if (permuted) natural();
+        const bool fresh = kind == kNew;
+        const int kr = grp * 16, key0 = tile0 + kr;  // this step's keys (rows of the tail, or new tokens)
+        const int end = fresh ? a.n : len - span.full;
+        const bool work = kr < BN16 && key0 < end;   // (the same for the whole warp)
+        const int lrow = kr + (lane & 15);
+        auto chunk = [&](int ch) { return lrow * 128 + (ch >> 3) * (BN16 * 128) + (((ch & 7) ^ (lrow & 7)) << 4); };
+        uint32_t pw[NT][2];
+        if (work) {
+          float s[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+          for (int k2 = 0; k2 < D / 32; ++k2) {
+            uint32_t x0[4], x1[4];
+            ldsm_x4(sk + chunk(4 * k2 + (lane >> 4)), x0);
+            ldsm_x4(sk + chunk(4 * k2 + 2 + (lane >> 4)), x1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              uint32_t q[4];
+              load_q(sq16, n, k2, q);
+              mma16816<T>(s[n], x0, q[0], q[1]);
+              mma16816<T>(s[n], x1, q[2], q[3]);
+            }
+          }
+          float mx[NT][2];
+          bool move = false;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              // (all lanes: the new tokens' depths are read by the warp)
+              uint32_t keep;
+              if (fresh) {
+                const int4 info = row_info[8 * n + 2 * tl + h];
+                const uint32_t bits = tree_sees16(a, b, info.x, key0, info.y, sink_left);
+                keep = ((bits >> gl) & 1u) | ((bits >> (gl + 7)) & 2u);
+              } else {
+                keep = sees(n, h, span.full + key0, len);
               }
+              s[n][h] = keep & 1u ? s[n][h] * a.scale_log2 : -INFINITY;
+              s[n][2 + h] = keep & 2u ? s[n][2 + h] * a.scale_log2 : -INFINITY;
+              mx[n][h] = fmaxf(s[n][h], s[n][2 + h]);
+              move |= mx[n][h] > m[n][h] + TreeRef<H>::kSlack;
             }
-            const bool any_bad = bad != 0u;
-#pragma unroll 1
-            for (; bad != 0u; bad &= bad - 1u) {
-              const int j = key0 + __ffs(bad) - 1;
-              const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + j * a.vn_t + part * DW + (lane & 3) * 2;
-              bool on[MT][2];
+          if (__any_sync(0xffffffffu, move)) move_rows(mx, 1.f);
+          weigh(s);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                  on[mt][h] = tok[mt][h] >= 0 && tree_sees(a, b, tok[mt][h], j, dep[mt][h], sink_left);
-#pragma unroll
-              for (int n = 0; n < DW / 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const uint16_t v = vn[n * 8 + e];
-                  if (tree_nonfinite<T>(v)) {
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                      for (int h = 0; h < 2; ++h)
-                        if (on[mt][h]) o[mt][n][2 * h + e] += tree_f32<T>(v);
-                  }
-                }
-            }
-            if (any_bad) __syncwarp();  // (the next step's loads are aligned)
+          for (int n = 0; n < NT; ++n) {
+            pw[n][0] = transpose8x8(pack2<T>(s[n][0], s[n][1]));
+            pw[n][1] = transpose8x8(pack2<T>(s[n][2], s[n][3]));
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(empty_bar(slot_v));
-      }
-      if (permuted) natural();
-
-      // ---- the groups' results joined: M = max m_w, O = sum 2^(m_w - M) O_w over the ring
+        if (lane == 0) mbar_arrive(empty_bar(slot_k));
+        ok = mbar_wait_bounded(full_bar(slot_v), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (work) {
+          // Rows behind the length or before the window may hold anything and 0 * NaN is NaN: zeros.
+          // So may a new token's values where some row must not see them: cleared here, added below
+          // to the rows that do.
+          uint32_t bad = 0;  // keys of this step whose values are not all finite (new tokens only)
+          if (fresh || key0 + 16 > end || span.full + key0 < span.low) {
+            for (int e = lane; e < 16 * CH; e += 32) {
+              const int r = e % 16, ch = e / 16, p = span.full + key0 + r;
+              uint4* w = reinterpret_cast<uint4*>(smem + (sv - base) + (ch >> 3) * (BN16 * 128) + (kr + r) * 128 +
+                                                  (((ch & 7) ^ ((kr + r) & 7)) << 4));
+              if (key0 + r >= end || (!fresh && p < span.low && p >= a.sink)) {
+                *w = make_uint4(0, 0, 0, 0);
+              } else if (fresh) {
+                uint4 x = *w;
+                if (nonfinite_bits<T>(x.x) | nonfinite_bits<T>(x.y) | nonfinite_bits<T>(x.z) | nonfinite_bits<T>(x.w)) {
+                  uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
-            l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
-            if ((lane & 3) == 0 && part == 0) {
-              const int r = mt * 16 + rl + 8 * h;
-              stat[grp * BM + r] = m[mt][h];
-              stat[(C::kGroups + grp) * BM + r] = l[mt][h];
+                  for (int q = 0; q < 4; ++q) xs[q] &= ~((nonfinite_bits<T>(xs[q]) >> 15) * 0xFFFFu);
+                  *w = x;
+                  bad |= 1u << r;
+                }
+              }
             }
+            bad = __reduce_or_sync(0xffffffffu, bad);
+            fence_proxy_async_smem();  // (the TMA writes this slot again later)
+            __syncwarp();
           }
-      ok = rows_sync_and(ok);  // everybody has left the ring; the statistics are there
-      float* joint = reinterpret_cast<float*>(smem);  // [group][BM][pitch]
-      {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+          for (int k = 0; k < D / 16; ++k) {
+            // (transposed 8 x 8 blocks: columns 0-7 and 8-15 of keys 0-7, then of keys 8-15)
+            uint32_t x[4], y[4];
+            ldsm_x4_t(sv + chunk(2 * k + (lane >> 4)), y);
+            x[0] = y[0], x[1] = y[2], x[2] = y[1], x[3] = y[3];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = mt * 16 + rl + 8 * h;
-            if (row0 + r >= rows) continue;
-            float top = stat[r];
-#pragma unroll
-            for (int w = 1; w < C::kGroups; ++w) top = fmaxf(top, stat[w * BM + r]);
-            const float f = m[mt][h] == -INFINITY ? 1.f : ex2_tree(m[mt][h] - top);
-            float* dst = joint + (grp * BM + r) * C::kPitch + part * DW + (lane & 3) * 2;
-            // (a group that saw nothing adds zeros, except what a NaN score made of it)
-            const bool none = m[mt][h] == -INFINITY && l[mt][h] == 0.f;
-#pragma unroll
-            for (int n = 0; n < DW / 8; ++n)
-              *reinterpret_cast<float2*>(dst + 8 * n) =
-                  none ? make_float2(0.f, 0.f) : make_float2(o[mt][n][2 * h] * f, o[mt][n][2 * h + 1] * f);
+            for (int n = 0; n < NT; ++n) mma16816<T>(o[n][k], x, pw[n][0], pw[n][1]);
           }
-      }
-      rows_sync();
-      if (ok) {
-        constexpr int Q4 = D / 4;  // float4 columns per row
-        for (int e = tid; e < BM * Q4; e += kTreeThreads) {
-          const int r = e / Q4, q4 = e % Q4;
-          if (row0 + r >= rows) break;
-          float top = stat[r];
+          const bool any_bad = bad != 0u;
+#pragma unroll 1
+          for (; bad != 0u; bad &= bad - 1u) {
+            const int j = key0 + __ffs(bad) - 1;
+            const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + j * a.vn_t + gl;
 #pragma unroll
-          for (int w = 1; w < C::kGroups; ++w) top = fmaxf(top, stat[w * BM + r]);
-          float sum = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int w = 0; w < C::kGroups; ++w) {
-            const float mw = stat[w * BM + r];
-            sum += (mw == -INFINITY ? 1.f : ex2_tree(mw - top)) * stat[(C::kGroups + w) * BM + r];
-            const float4 x = *reinterpret_cast<const float4*>(joint + (w * BM + r) * C::kPitch + 4 * q4);
-            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+              for (int h = 0; h < 2; ++h) {
+                const int4 info = row_info[8 * n + 2 * tl + h];
+                if (info.x < 0 || !tree_sees(a, b, info.x, j, info.y, sink_left)) continue;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const uint16_t v = vn[16 * k + 8 * e];
+                    if (tree_nonfinite<T>(v)) o[n][k][2 * e + h] += tree_f32<T>(v);
+                  }
+              }
           }
-          if (whole) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: zeros
-            int i, gq;
-            tree_row(a, row0 + r, i, gq);
-            uint16_t* dst = a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + gq) * a.o_h + i * a.o_t + 4 * q4;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
-          } else {
-            *reinterpret_cast<float4*>(a.part_o + (part_row + r) * D + 4 * q4) = v;
-            if (q4 == 0) a.part_ml[part_row + r] = make_float2(top, sum);
-          }
+          if (any_bad) __syncwarp();  // (the next step's loads are aligned)
         }
       }
-      ok = item_done(ok);
-      if (!ok) break;  // (the producer waits for the copies in flight)
-      pos += t1 - t0;
-      if (pos >= stop) break;
-      advance();
-      fence_proxy_async_smem();  // the joint outputs lay where the TMA writes next
-      item_free();               // the ring, Q and the statistics are free
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty_bar(slot_v));
     }
+    if (permuted) natural();
+
+    // ---- the warps' results joined: M = max m_w, O = sum 2^(m_w - M) O_w, some columns at a time
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], 4);
+        l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], 8);
+        l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], 16);
+        if (gl == 0) {
+          const int r = 8 * n + 2 * tl + h;
+          stat[warp * BM + r] = m[n][h];
+          stat[(kTreeWarps + warp) * BM + r] = l[n][h];
+        }
+      }
+    ok = rows_sync_and(ok);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = 8 * n + 2 * tl + h;
+        float top = stat[r];
+#pragma unroll
+        for (int w = 1; w < kTreeWarps; ++w) top = fmaxf(top, stat[w * BM + r]);
+        // (a warp that saw nothing adds zeros, except what a NaN score made of it)
+        const bool none = m[n][h] == -INFINITY && l[n][h] == 0.f;
+        fac[n][h] = none ? -1.f : m[n][h] == -INFINITY ? 1.f : ex2_tree(m[n][h] - top);
+      }
+#pragma unroll
+    for (int j = 0; j < D / C::kJoin; ++j) {
+      if (j > 0) rows_sync();
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float* dst = joint + (warp * BM + 8 * n + 2 * tl + h) * C::kPitch + gl;
+#pragma unroll
+          for (int k = 0; k < C::kJoin / 16; ++k) {
+            const float* v = o[n][j * (C::kJoin / 16) + k];
+            dst[16 * k] = fac[n][h] < 0.f ? 0.f : v[h] * fac[n][h];
+            dst[16 * k + 8] = fac[n][h] < 0.f ? 0.f : v[2 + h] * fac[n][h];
+          }
+        }
+      rows_sync();
+      if (!ok) continue;
+      constexpr int Q4 = C::kJoin / 4;  // float4 columns
+      for (int e = tid; e < BM * Q4; e += kTreeThreads) {
+        const int r = e / Q4, q4 = e % Q4, col = j * C::kJoin + 4 * q4;
+        if (row0 + r >= rows) break;
+        float top = stat[r];
+#pragma unroll
+        for (int w = 1; w < kTreeWarps; ++w) top = fmaxf(top, stat[w * BM + r]);
+        float sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kTreeWarps; ++w) {
+          const float mw = stat[w * BM + r];
+          sum += (mw == -INFINITY ? 1.f : ex2_tree(mw - top)) * stat[(kTreeWarps + w) * BM + r];
+          const float4 x = *reinterpret_cast<const float4*>(joint + (w * BM + r) * C::kPitch + 4 * q4);
+          v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: zeros
+          int i, gq;
+          tree_row(a, row0 + r, i, gq);
+          uint16_t* dst = a.o + b * a.o_b + (static_cast<int64_t>(c) * a.group + gq) * a.o_h + i * a.o_t + col;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+        } else {
+          *reinterpret_cast<float4*>(a.part_o + (part_row + r) * D + col) = v;
+          if (col == 0) a.part_ml[part_row + r] = make_float2(top, sum);
+        }
+      }
+    }
+    if (!ok) break;  // (the producer waits for the copies in flight)
+    pos += t1 - t0;
+    if (pos >= stop) break;
+    advance();
+    rows_sync();  // Q, the statistics and the joint outputs are free
   }
 }
 
@@ -875,7 +837,7 @@ static PagedPlan paged_plan(int64_t batch, int64_t kv_heads, int64_t group, int6
                             int64_t window, int64_t sink, int sms) {
   PagedPlan p;
   const int64_t rows = group * n;
-  p.bm = rows > 16 && d <= 128 ? 32 : 16;
+  p.bm = rows <= 8 || d == 512 ? 8 : rows <= 16 || d == 256 ? 16 : 32;
   p.row_tiles = static_cast<int>((rows + p.bm - 1) / p.bm);
   p.items = batch * kv_heads * p.row_tiles;
   // Keys of one row tile: with a window, those its tokens see.
@@ -951,15 +913,15 @@ static int paged_encode(CUtensorMap* map, const void* ptr, int64_t d, int64_t pa
                      d == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, "pages");
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int NT>
 static int paged_main(const w8_attention_paged_args& x, const w8::PagedArgs& pa, int64_t blocks, int device,
                       cudaStream_t stream) {
-  using C = w8::PagedCfg<D, MT>;
+  using C = w8::PagedCfg<D, NT>;
   constexpr bool kHalf = __is_same(T, __half);
   const w8::TreeArgs& a = pa.t;
   static bool done[64] = {};
   if (!done[device]) {
-    W8_CUDA_TRY(cudaFuncSetAttribute(w8::attn_paged_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    W8_CUDA_TRY(cudaFuncSetAttribute(w8::attn_paged_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      C::kSmem));
     done[device] = true;
   }
@@ -986,7 +948,7 @@ static int paged_main(const w8_attention_paged_args& x, const w8::PagedArgs& pa,
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, w8::attn_paged_kernel<T, D, MT>, tk, tv, tkt, tvt, tkn, tvn, pa));
+  return cuda_status(cudaLaunchKernelEx(&cfg, w8::attn_paged_kernel<T, D, NT>, tk, tv, tkt, tvt, tkn, tvn, pa));
 }
 
 template <typename T, int D>
@@ -995,10 +957,19 @@ static int paged_go(const w8_attention_paged_args& x, const w8::PagedArgs& a, co
   W8_CHECK_ARG(p.items < (1ll << 31) / 2, "too many row tiles");
   const int64_t blocks = p.direct ? p.items : p.ctas;
   int st;
-  if constexpr (D <= 128)
-    st = p.bm == 32 ? paged_main<T, D, 2>(x, a, blocks, device, stream) : paged_main<T, D, 1>(x, a, blocks, device, stream);
-  else
+  if (p.bm == 8) {
     st = paged_main<T, D, 1>(x, a, blocks, device, stream);
+  } else if constexpr (D <= 256) {
+    if (p.bm == 16) {
+      st = paged_main<T, D, 2>(x, a, blocks, device, stream);
+    } else if constexpr (D <= 128) {
+      st = paged_main<T, D, 4>(x, a, blocks, device, stream);
+    } else {
+      return W8_ERR_UNSUPPORTED;  // (no plan has it)
+    }
+  } else {
+    return W8_ERR_UNSUPPORTED;
+  }
   if (st != W8_OK || p.direct || p.ctas <= 1) return st;
   return tree_join(a.t, __is_same(T, __half), D, p.bm, stream);
 }
