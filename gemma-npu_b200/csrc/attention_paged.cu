@@ -34,31 +34,27 @@
 
 namespace w8 {
 
-// Two warpgroups of 8 working warps and one whose first warp loads.  168 registers a thread at
-// launch (12 warps), dealt as 216 to the working ones and 72 to the others: 64512 both ways.
-constexpr int kPagedWarps = kTreeWarps + 4;
-constexpr int kPagedThreads = 32 * kPagedWarps;
-__device__ __forceinline__ void paged_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
-__device__ __forceinline__ void paged_fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
-
 template <int D, int NT>
 struct PagedCfg {
   static constexpr int kBM = 8 * NT;
+  static constexpr int kWarps = 8;                         // working; a ninth loads
+  static constexpr int kThreads = 32 * (kWarps + 1);
+  static constexpr int kKT = D <= 128 ? 2 : 1;             // 16-key tiles of a warp's step
   static constexpr int kTeams = D == 512 ? 2 : 1;          // sets of warps that take the tiles in turn
-  static constexpr int kGroups = kTreeWarps / kTeams;
-  static constexpr int kSteps = D == 64 ? 2 : 1;           // 16-key steps of a warp in a tile
-  static constexpr int kBN = kGroups * kSteps * 16;        // keys of a tile of pages: 256, 128, 128, 64
+  static constexpr int kGroups = kWarps / kTeams;          // warps of a tile
+  static constexpr int kBN = kGroups * kKT * 16;           // keys of a tile of pages: 256, 256, 128, 64
   static constexpr int kBN16 = kBN / 2;                    // of a 16-bit tile, which is as large
-  static constexpr int kSlotBytes = kBN * D;               // 16 KB (D <= 128) or 32 KB
+  static constexpr int kSlotBytes = kBN * D;               // 16 KB (D = 64) or 32 KB
   static constexpr int kSlots = 163840 / kSlotBytes;       // 10 or 5
-  static constexpr int kJoin = 1024 / kBM < D ? 1024 / kBM : D;  // columns of the outputs joined at a time
+  static constexpr int kJoin = 8192 / (kBM * kWarps) < D ? 8192 / (kBM * kWarps) : D;  // columns of the outputs joined at a time
   static constexpr int kPitch = kJoin + 4;                 // their fp32 row pitch
   static constexpr int kOffQ8 = kSlots * kSlotBytes;       // Q as fp16, scaled and permuted
   static constexpr int kOffQ16 = kOffQ8 + kBM * D * 2;     // Q as it is
-  static constexpr int kOffJoin = kOffQ16 + kBM * D * 2;   // float [8][kBM][kPitch]
-  static constexpr int kOffStat = kOffJoin + kTreeWarps * kBM * kPitch * 4;  // float [2][8][kBM]: maxima, sums
-  static constexpr int kOffRow = kOffStat + 2 * kTreeWarps * kBM * 4;  // int4 [kBM]: token, depth, first key, Q's scale taken back
-  static constexpr int kOffScale = kOffRow + kBM * 16;     // float [kSlots][kPagedMaxBoxes]
+  static constexpr int kOffJoin = kOffQ16 + kBM * D * 2;   // float [kWarps][kBM][kPitch]
+  static constexpr int kOffStat = kOffJoin + kWarps * kBM * kPitch * 4;  // float [2][kWarps][kBM]: maxima, sums
+  static constexpr int kOffRow = kOffStat + 2 * kWarps * kBM * 4;  // int4 [kBM]: token, depth, first key, Q's scale taken back
+  static constexpr int kOffSum = kOffRow + kBM * 16;       // float [kBM]: -1152 times the sum of Q as fp16
+  static constexpr int kOffScale = kOffSum + (kBM * 4 + 15) / 16 * 16;     // float [kSlots][kPagedMaxBoxes]
   static constexpr int kOffMask = kOffScale + kSlots * kPagedMaxBoxes * 4;  // uint32 [kSlots]: boxes that are there
   static constexpr int kOffBar = kOffMask + (kSlots * 4 + 15) / 16 * 16;
   static constexpr int kNumBars = 2 * kSlots;              // full, empty
@@ -79,7 +75,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kPagedThreads, 1)
+__global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
     attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
                       const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_vn,
@@ -87,7 +83,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   using C = PagedCfg<D, NT>;
   using H = __half;
   constexpr int BM = C::kBM, BN = C::kBN, BN16 = C::kBN16, NS = C::kSlots, CH = D / 8;  // CH: 16-byte chunks of a 16-bit row
-  constexpr bool kQRegs = NT * D <= 256;             // Q's fragments stay in registers
+  constexpr bool kQRegs = NT * D <= 128;             // Q's fragments stay in registers
   constexpr int kRowBytes = D < 128 ? D : 128;       // of a box's row in shared memory
   const TreeArgs& a = pa.t;
   extern __shared__ uint8_t smem_raw[];
@@ -98,6 +94,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   float* joint = reinterpret_cast<float*>(smem + C::kOffJoin);
   float* stat = reinterpret_cast<float*>(smem + C::kOffStat);
   int4* row_info = reinterpret_cast<int4*>(smem + C::kOffRow);
+  float* row_sum = reinterpret_cast<float*>(smem + C::kOffSum);
   volatile float* scales = reinterpret_cast<volatile float*>(smem + C::kOffScale);
   volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(smem + C::kOffMask);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffBar + C::kNumBars * 8);
@@ -111,7 +108,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(full_bar(s), 1);  // the producer's arrive.expect_tx
-      mbar_init(empty_bar(s), kTreeWarps);
+      mbar_init(empty_bar(s), C::kWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -168,8 +165,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     };
     long long* sched = reinterpret_cast<long long*>(joint);  // (not in use yet)
     long long sum = 0, round;
-    for (int p = tid; p < pairs; p += kPagedThreads) sum += pair_tiles(p);
-    long long excl = block_scan<kPagedWarps>(sum, sched, round);  // (of few pairs also each one's place)
+    for (int p = tid; p < pairs; p += C::kThreads) sum += pair_tiles(p);
+    long long excl = block_scan<C::kWarps + 1>(sum, sched, round);  // (of few pairs also each one's place)
     const long long total = round * a.kv_heads;
     const uint32_t ctas = total < gridDim.x ? static_cast<uint32_t>(total) : gridDim.x;
     if (blockIdx.x >= ctas) return;
@@ -179,24 +176,24 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     stop = deal_begin(deal, blockIdx.x + 1);
     // The pair that holds `pos`: a running sum over rounds of pairs.
     long long before = 0;
-    for (int p0 = 0;; p0 += kPagedThreads) {
+    for (int p0 = 0;; p0 += C::kThreads) {
       const int p = p0 + tid;
       long long nt = sum;
-      if (pairs > kPagedThreads) {
+      if (pairs > C::kThreads) {
         nt = p < pairs ? pair_tiles(p) : 0;
-        excl = before + block_scan<kPagedWarps>(nt, sched, round);
+        excl = before + block_scan<C::kWarps + 1>(nt, sched, round);
       }
       if (nt > 0 && excl * a.kv_heads <= pos && pos < (excl + nt) * a.kv_heads) {
-        sched[16] = p;
-        sched[17] = excl * a.kv_heads;
+        sched[32] = p;
+        sched[33] = excl * a.kv_heads;
       }
       __syncthreads();
       before += round;
       if (pos < before * a.kv_heads) break;  // (every pair has tiles, and pos < total)
-      if (p0 + kPagedThreads >= pairs) return;  // only if the lengths changed under the call
+      if (p0 + C::kThreads >= pairs) return;  // only if the lengths changed under the call
     }
-    split_pair(static_cast<int>(sched[16]), b, rt);
-    item_pos = sched[17];
+    split_pair(static_cast<int>(sched[32]), b, rt);
+    item_pos = sched[33];
     len = tree_len(a, b);
     span = paged_span<BM, BN, BN16>(pa, len, rt);
     const int tiles = span.tiles();
@@ -232,11 +229,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   uint32_t g = 0;  // ring steps so far (each tile's K, then V)
   bool ok = true;
   __syncwarp();
-  if (warp >= kTreeWarps) {
+  if (warp >= C::kWarps) {
     // ---- the producer: each tile's K and V boxes into the ring as its slots are left, the table
     // entries and scales of the next tile under way meanwhile.
-    paged_fewer_registers();
-    if (warp > kTreeWarps) return;
     while (ok) {
       const int t0 = static_cast<int>(pos - item_pos);
       const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
@@ -296,10 +291,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     }
     return;
   }
-  paged_more_registers();
   auto rows_sync = [&]() {  // of the 8 warps without the producer
     __syncwarp();
-    asm volatile("bar.sync 1, %0;" ::"n"(kTreeThreads) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kWarps) : "memory");
   };
   auto rows_sync_and = [&](bool on) {
     uint32_t all;
@@ -310,7 +304,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         "bar.red.and.pred p, 1, %2, q;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(all)
-        : "r"(on ? 1u : 0u), "n"(kTreeThreads)
+        : "r"(on ? 1u : 0u), "n"(32 * C::kWarps)
         : "memory");
     return all != 0u;
   };
@@ -331,8 +325,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     // Q rows r = i * group + g (query head c * group + g of new token i), a row a warp: as they
     // are, and scaled into fp16's range with 16 columns at a time in the order in which a thread's 4
     // bytes of K come: columns 4 t .. 4 t + 3 as elements 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
-    for (int r = warp; r < BM; r += kTreeWarps) {
-      float most = 0.f;
+    for (int r = warp; r < BM; r += C::kWarps) {
+      float most = 0.f, sum = 0.f;
       uint4 w[(CH + 31) / 32];
       int i = -1, gq = 0, dep = 0, first = INT32_MAX;  // (no row: sees nothing)
       if (row0 + r < rows) {
@@ -359,7 +353,6 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       const int ex = static_cast<int>(__float_as_uint(most) >> 23);
       const int up = ex == 0 || ex == 255 ? 0 : min(14 + 127 - ex, 100);
       const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-      if (lane == 0) row_info[r] = make_int4(i, dep, first, (127 - up) << 23);
 #pragma unroll
       for (int x = 0; x < (CH + 31) / 32; ++x) {
         const int ch = lane + 32 * x;
@@ -367,23 +360,36 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         const uint32_t ws[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
         uint32_t h[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = pack2<H>(tree_f32<T>(ws[e] & 0xFFFFu) * f, tree_f32<T>(ws[e] >> 16) * f);
+        for (int e = 0; e < 4; ++e) {
+          h[e] = pack2<H>(tree_f32<T>(ws[e] & 0xFFFFu) * f, tree_f32<T>(ws[e] >> 16) * f);
+          sum += tree_f32<H>(h[e] & 0xFFFFu) + tree_f32<H>(h[e] >> 16);
+        }
         uint8_t* row = smem + C::kOffQ8 + r * (D * 2) + 8 * (ch & 1);
         *reinterpret_cast<uint2*>(row + (((ch & ~1) ^ (r & 7)) << 4)) = make_uint2(h[0], h[2]);
         *reinterpret_cast<uint2*>(row + (((ch | 1) ^ (r & 7)) << 4)) = make_uint2(h[1], h[3]);
       }
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane == 0) {
+        row_info[r] = make_int4(i, dep, first, (127 - up) << 23);
+        row_sum[r] = -1152.f * sum;
+      }
     }
     rows_sync();
+    // A row's reference: no maximum yet is kNone, which every score exceeds.
+    constexpr float kNone = -1e30f;
     float m[NT][2], l[NT][2], fac[NT][2];
     float o[NT][D / 16][4];  // O transposed: columns gl and gl + 8 of 16 (or 2 gl and 2 gl + 1), rows 2 tl, 2 tl + 1
+    float qsum[NT][2];
     int last_first = 0;      // the latest first key of the item's rows
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int4 info = row_info[8 * n + 2 * tl + h];
-        m[n][h] = -INFINITY, l[n][h] = 0.f;
+        m[n][h] = kNone, l[n][h] = 0.f;
         fac[n][h] = __int_as_float(info.w) * a.scale_log2;
+        qsum[n][h] = row_sum[8 * n + 2 * tl + h];
         if (info.x >= 0) last_first = max(last_first, info.z);
       }
 #pragma unroll
@@ -415,9 +421,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       }
       return bits;
     };
-    // m moved where a row's maximum of the step (of this thread's keys: mx) asks for it; O and l with
-    // it, O by `unit` (the change of its unit) besides.
-    auto move_rows = [&](float (&mx)[NT][2], float unit) {
+    // m moved where a row's maximum of the step (of this thread's keys: mx) asks for it; O and l with it,
+    // O by `unit` (the change of its unit) besides.
+    auto move_rows = [&](const float (&mx)[NT][2], float unit) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -437,18 +443,6 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
             o[n][k][h] *= f;
             o[n][k][2 + h] *= f;
           }
-        }
-    };
-    // The step's scores s (keys gl: 0, 1; gl + 8: 2, 3) to weights, and l.
-    auto weigh = [&](float (&s)[NT][4]) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float ref = m[n][h] == -INFINITY ? 0.f : m[n][h];
-          s[n][h] = ex2_tree(s[n][h] - ref);
-          s[n][2 + h] = ex2_tree(s[n][2 + h] - ref);
-          l[n][h] += s[n][h] + s[n][2 + h];
         }
     };
     float unit = __uint_as_float(0x00800000u);  // of O (2^-126: nothing added yet)
@@ -494,121 +488,176 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       const int kind = kind_of(t), tile0 = key0_of(t);
       const uint32_t sk = base + slot_k * C::kSlotBytes, sv = base + slot_v * C::kSlotBytes;
       if (kind == kPages) {
-        const uint32_t there = masks[slot_k];
+        const int kr = grp * (C::kKT * 16), key0 = tile0 + kr;  // this step's keys
+        // Rows of 16 bytes that a lane names for ldmatrix: 8 keys, the next 8, and the next 16 columns of
+        // both.  A row's chunks are swizzled, a matter of one XOR as a row begins on 128 (64) bytes.
+        uint32_t off[C::kKT];  // in the slot, of chunk lane / 16
+        int bx[C::kKT];        // the 16 keys' box
 #pragma unroll
-        for (int st = 0; st < C::kSteps; ++st) {
-          const int kr = (grp * C::kSteps + st) * 16, key0 = tile0 + kr;  // this step's keys
-          const int bx = kr >> box_shift, br = kr & (box - 1);            // their box, and row in it
-          // Rows of 16 bytes that a lane names for ldmatrix: 8 keys, the next 8, and the next 16 columns
-          // of both.
-          const int lrow = br + (lane & 15);
-          const uint32_t off = bx * (box * D) + lrow * kRowBytes;
-          auto chunk = [&](int ch) -> uint32_t {
-            if constexpr (D >= 128) return (ch >> 3) * (box * 128) + (((ch & 7) ^ (lrow & 7)) << 4);
-            return (ch ^ ((lrow >> 1) & 3)) << 4;
-          };
-          // ---- S^T = K Q^T, 16 keys
-          float s[NT][4];
+        for (int kt = 0; kt < C::kKT; ++kt) {
+          bx[kt] = (kr + 16 * kt) >> box_shift;
+          const int lrow = ((kr + 16 * kt) & (box - 1)) + (lane & 15);
+          off[kt] = bx[kt] * (box * D) + lrow * kRowBytes + (((lane >> 4) ^ (D >= 128 ? lrow & 7 : (lrow >> 1) & 3)) << 4);
+        }
+        auto chunks = [&](uint32_t slot, int kt, int c2) {  // chunks 2 c2 and 2 c2 + 1
+          return slot + (D > 128 ? (c2 >> 2) * (box * 128) : 0) + (off[kt] ^ ((c2 & 3) << 5));
+        };
+        // ---- S^T = K Q^T.  The 8-bit values go in as 1024 + 128 + k8, exact in fp16, and the sums start
+        // from -1152 times Q's: the products cancel to S with what fp32 sums lose at their size, about
+        // 2^-23 of 1152 |sum q| against a score's 30 |q| sqrt(D): 10^-5 of it.
+        float s[C::kKT][NT][4];
+#pragma unroll
+        for (int kt = 0; kt < C::kKT; ++kt)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+            for (int e = 0; e < 4; ++e) s[kt][n][e] = qsum[n][e & 1];
 #pragma unroll
-          for (int k2 = 0; k2 < D / 32; ++k2) {
-            uint32_t kb[4], x0[4], x1[4];
-            ldsm_x4(sk + off + chunk(2 * k2 + (lane >> 4)), kb);
-            paged_unpack<H>(kb[0], 0x4140u, 0x4342u, x0[0], x0[2]);
-            paged_unpack<H>(kb[1], 0x4140u, 0x4342u, x0[1], x0[3]);
-            paged_unpack<H>(kb[2], 0x4140u, 0x4342u, x1[0], x1[2]);
-            paged_unpack<H>(kb[3], 0x4140u, 0x4342u, x1[1], x1[3]);
+        for (int k2 = 0; k2 < D / 32; ++k2) {
+          uint32_t x0[C::kKT][4], x1[C::kKT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              if constexpr (kQRegs) {
-                mma16816<H>(s[n], x0, qf[n][k2][0], qf[n][k2][1]);
-                mma16816<H>(s[n], x1, qf[n][k2][2], qf[n][k2][3]);
-              } else {
-                uint32_t q[4];
-                load_q(sq8, n, k2, q);
-                mma16816<H>(s[n], x0, q[0], q[1]);
-                mma16816<H>(s[n], x1, q[2], q[3]);
-              }
+          for (int kt = 0; kt < C::kKT; ++kt) {
+            uint32_t kb[4];
+            ldsm_x4(chunks(sk, kt, k2), kb);
+            paged_raise(kb[0], 0x4140u, 0x4342u, x0[kt][0], x0[kt][2]);
+            paged_raise(kb[1], 0x4140u, 0x4342u, x0[kt][1], x0[kt][3]);
+            paged_raise(kb[2], 0x4140u, 0x4342u, x1[kt][0], x1[kt][2]);
+            paged_raise(kb[3], 0x4140u, 0x4342u, x1[kt][1], x1[kt][3]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint32_t q[4];
+            if constexpr (kQRegs) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) q[e] = qf[n][k2][e];
+            } else {
+              load_q(sq8, n, k2, q);
+            }
+#pragma unroll
+            for (int kt = 0; kt < C::kKT; ++kt) {
+              mma16816<H>(s[kt][n], x0[kt], q[0], q[1]);
+              mma16816<H>(s[kt][n], x1[kt], q[2], q[3]);
             }
           }
-          if (st == C::kSteps - 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty_bar(slot_k));
+        }
+        const uint32_t there = masks[slot_k];
+        float ks[C::kKT];
+        bool on[C::kKT], plain = true;  // plain: all rows see all keys
+#pragma unroll
+        for (int kt = 0; kt < C::kKT; ++kt) {
+          ks[kt] = scales[slot_k * kPagedMaxBoxes + bx[kt]];
+          on[kt] = (there >> bx[kt]) & 1u;
+          plain = plain && on[kt];
+        }
+        plain = plain && key0 + 16 * C::kKT <= span.full && key0 >= last_first;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty_bar(slot_k));
+        // ---- scores in log2 units, less m; masks
+        float y[C::kKT][NT][4], most = -INFINITY;
+        uint32_t hidden = 0u;  // bit (kt NT + n) 4 + e: the row does not see the key
+        auto score = [&]() {
+#pragma unroll
+          for (int kt = 0; kt < C::kKT; ++kt)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[kt][n][e] = fmaf(s[kt][n][e], fac[n][e & 1] * ks[kt], -m[n][e & 1]);
+          if (!plain) {
+#pragma unroll
+            for (int kt = 0; kt < C::kKT; ++kt)
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if ((hidden >> ((kt * NT + n) * 4 + e)) & 1u) y[kt][n][e] = -INFINITY;
           }
-          // ---- scores in log2 units, masks, the running softmax
-          const float ks = scales[slot_k * kPagedMaxBoxes + bx];
-          const bool on = (there >> bx) & 1u;
-          const bool plain = on && key0 + 16 <= span.full && key0 >= last_first;  // all rows see all keys
+        };
+        if (!plain) {
+#pragma unroll
+          for (int kt = 0; kt < C::kKT; ++kt)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t keep = on[kt] ? sees(n, h, key0 + 16 * kt, span.full) : 0u;
+                hidden |= (~keep & 1u) << ((kt * NT + n) * 4 + h) | ((~keep >> 1) & 1u) << ((kt * NT + n) * 4 + 2 + h);
+              }
+        }
+        score();
+#pragma unroll
+        for (int kt = 0; kt < C::kKT; ++kt)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, y[kt][n][e]);
+        ok = mbar_wait_bounded(full_bar(slot_v), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float vs[C::kKT], need = unit;
+#pragma unroll
+        for (int kt = 0; kt < C::kKT; ++kt) {
+          vs[kt] = on[kt] ? scales[slot_v * kPagedMaxBoxes + bx[kt]] : 0.f;
+          need = fmaxf(need, paged_unit(vs[kt]));
+        }
+        if (__any_sync(0xffffffffu, most > TreeRef<H>::kSlack) || need > unit) {
           float mx[NT][2];
-          bool move = false;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float f = fac[n][h] * ks;
-              s[n][h] *= f, s[n][2 + h] *= f;
-              if (!plain) {
-                const uint32_t keep = on ? sees(n, h, key0, span.full) : 0u;
-                if (!(keep & 1u)) s[n][h] = -INFINITY;
-                if (!(keep & 2u)) s[n][2 + h] = -INFINITY;
-              }
-              mx[n][h] = fmaxf(s[n][h], s[n][2 + h]);
-              move |= mx[n][h] > m[n][h] + TreeRef<H>::kSlack;
+              mx[n][h] = -INFINITY;
+#pragma unroll
+              for (int kt = 0; kt < C::kKT; ++kt)
+#pragma unroll
+                for (int e = h; e < 4; e += 2)
+                  if (!((hidden >> ((kt * NT + n) * 4 + e)) & 1u))
+                    mx[n][h] = fmaxf(mx[n][h], s[kt][n][e] * (fac[n][h] * ks[kt]));
             }
-          if (st == 0) {
-            ok = mbar_wait_bounded(full_bar(slot_v), ((g + 1) / NS) & 1u, abort_flag, &g_tree_status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-          }
-          const float vs = on ? scales[slot_v * kPagedMaxBoxes + bx] : 0.f;
-          const float need = paged_unit(vs);
-          if (__any_sync(0xffffffffu, move) || need > unit) {
-            const float to = fmaxf(need, unit);
-            move_rows(mx, unit * paged_unit_rcp(to));
-            unit = to;
-          }
-          const float vr = vs * paged_unit_rcp(unit);
-          bool seen[NT][4];  // (looked at below only if vs is NaN)
+          move_rows(mx, unit * paged_unit_rcp(need));
+          unit = need;
+          score();
+        }
+        // ---- weights, and P in O's unit
+        uint32_t pw[C::kKT][NT][2];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) seen[n][e] = s[n][e] != -INFINITY;
-          weigh(s);
-          uint32_t pw[NT][2];
+        for (int kt = 0; kt < C::kKT; ++kt) {
+          const float vr = vs[kt] * paged_unit_rcp(unit);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float p[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] = s[n][e] * vr;
+            for (int e = 0; e < 4; ++e) p[e] = ex2_tree(y[kt][n][e]);
+            l[n][0] += p[0] + p[2];
+            l[n][1] += p[1] + p[3];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[e] *= vr;
             if (vr != vr) {  // (a NaN scale is for the rows that see the page)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (!seen[n][e]) p[e] = 0.f;
+                if ((hidden >> ((kt * NT + n) * 4 + e)) & 1u) p[e] = 0.f;
             }
-            pw[n][0] = transpose8x8(pack2<H>(p[0], p[1]));
-            pw[n][1] = transpose8x8(pack2<H>(p[2], p[3]));
+            pw[kt][n][0] = transpose8x8(pack2<H>(p[0], p[1]));
+            pw[kt][n][1] = transpose8x8(pack2<H>(p[2], p[3]));
           }
-          // ---- O^T += V^T P^T: of 16 bytes of a row of V the even columns are 8 rows of the operand, the
-          // odd ones the others.
+        }
+        // ---- O^T += V^T P^T: of 16 bytes of a row of V the even columns are 8 rows of the operand, the
+        // odd ones the others.
 #pragma unroll
-          for (int c2 = 0; c2 < D / 32; ++c2) {
+        for (int c2 = 0; c2 < D / 32; ++c2)
+#pragma unroll
+          for (int kt = 0; kt < C::kKT; ++kt) {
             uint32_t vb[4], x0[4], x1[4];
-            ldsm_x4_t(sv + off + chunk(2 * c2 + (lane >> 4)), vb);
+            ldsm_x4_t(chunks(sv, kt, c2), vb);
             paged_unpack<H>(vb[0], 0x4240u, 0x4341u, x0[0], x0[1]);
             paged_unpack<H>(vb[1], 0x4240u, 0x4341u, x0[2], x0[3]);
             paged_unpack<H>(vb[2], 0x4240u, 0x4341u, x1[0], x1[1]);
             paged_unpack<H>(vb[3], 0x4240u, 0x4341u, x1[2], x1[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              mma16816<H>(o[n][2 * c2], x0, pw[n][0], pw[n][1]);
-              mma16816<H>(o[n][2 * c2 + 1], x1, pw[n][0], pw[n][1]);
+              mma16816<H>(o[n][2 * c2], x0, pw[kt][n][0], pw[kt][n][1]);
+              mma16816<H>(o[n][2 * c2 + 1], x1, pw[kt][n][0], pw[kt][n][1]);
             }
           }
-        }
-        if (!ok) break;
       } else {
         if (permuted) natural();
         const bool fresh = kind == kNew;
@@ -637,8 +686,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
               mma16816<T>(s[n], x1, q[2], q[3]);
             }
           }
-          float mx[NT][2];
-          bool move = false;
+          float mx[NT][2], most = -INFINITY;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -655,14 +703,18 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
               s[n][h] = keep & 1u ? s[n][h] * a.scale_log2 : -INFINITY;
               s[n][2 + h] = keep & 2u ? s[n][2 + h] * a.scale_log2 : -INFINITY;
               mx[n][h] = fmaxf(s[n][h], s[n][2 + h]);
-              move |= mx[n][h] > m[n][h] + TreeRef<H>::kSlack;
+              most = fmaxf(most, mx[n][h] - m[n][h]);
             }
-          if (__any_sync(0xffffffffu, move)) move_rows(mx, 1.f);
-          weigh(s);
+          if (__any_sync(0xffffffffu, most > TreeRef<H>::kSlack)) move_rows(mx, 1.f);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            pw[n][0] = transpose8x8(pack2<T>(s[n][0], s[n][1]));
-            pw[n][1] = transpose8x8(pack2<T>(s[n][2], s[n][3]));
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[e] = ex2_tree(s[n][e] - m[n][e & 1]);
+            l[n][0] += p[0] + p[2];
+            l[n][1] += p[1] + p[3];
+            pw[n][0] = transpose8x8(pack2<T>(p[0], p[1]));
+            pw[n][1] = transpose8x8(pack2<T>(p[2], p[3]));
           }
         }
         __syncwarp();
@@ -744,8 +796,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], 16);
         if (gl == 0) {
           const int r = 8 * n + 2 * tl + h;
-          stat[warp * BM + r] = m[n][h];
-          stat[(kTreeWarps + warp) * BM + r] = l[n][h];
+          stat[warp * BM + r] = m[n][h] == kNone ? -INFINITY : m[n][h];
+          stat[(C::kWarps + warp) * BM + r] = l[n][h];
         }
       }
     ok = rows_sync_and(ok);
@@ -756,10 +808,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         const int r = 8 * n + 2 * tl + h;
         float top = stat[r];
 #pragma unroll
-        for (int w = 1; w < kTreeWarps; ++w) top = fmaxf(top, stat[w * BM + r]);
+        for (int w = 1; w < C::kWarps; ++w) top = fmaxf(top, stat[w * BM + r]);
         // (a warp that saw nothing adds zeros, except what a NaN score made of it)
-        const bool none = m[n][h] == -INFINITY && l[n][h] == 0.f;
-        fac[n][h] = none ? -1.f : m[n][h] == -INFINITY ? 1.f : ex2_tree(m[n][h] - top);
+        const bool none = m[n][h] == kNone && l[n][h] == 0.f;
+        fac[n][h] = none ? -1.f : m[n][h] == kNone ? 1.f : ex2_tree(m[n][h] - top);
       }
 #pragma unroll
     for (int j = 0; j < D / C::kJoin; ++j) {
@@ -779,18 +831,18 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       rows_sync();
       if (!ok) continue;
       constexpr int Q4 = C::kJoin / 4;  // float4 columns
-      for (int e = tid; e < BM * Q4; e += kTreeThreads) {
+      for (int e = tid; e < BM * Q4; e += 32 * C::kWarps) {
         const int r = e / Q4, q4 = e % Q4, col = j * C::kJoin + 4 * q4;
         if (row0 + r >= rows) break;
         float top = stat[r];
 #pragma unroll
-        for (int w = 1; w < kTreeWarps; ++w) top = fmaxf(top, stat[w * BM + r]);
+        for (int w = 1; w < C::kWarps; ++w) top = fmaxf(top, stat[w * BM + r]);
         float sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kTreeWarps; ++w) {
+        for (int w = 0; w < C::kWarps; ++w) {
           const float mw = stat[w * BM + r];
-          sum += (mw == -INFINITY ? 1.f : ex2_tree(mw - top)) * stat[(kTreeWarps + w) * BM + r];
+          sum += (mw == -INFINITY ? 1.f : ex2_tree(mw - top)) * stat[(C::kWarps + w) * BM + r];
           const float4 x = *reinterpret_cast<const float4*>(joint + (w * BM + r) * C::kPitch + 4 * q4);
           v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
         }
@@ -841,7 +893,7 @@ static PagedPlan paged_plan(int64_t batch, int64_t kv_heads, int64_t group, int6
   p.row_tiles = static_cast<int>((rows + p.bm - 1) / p.bm);
   p.items = batch * kv_heads * p.row_tiles;
   // Keys of one row tile: with a window, those its tokens see.
-  const int64_t bn = d == 512 ? 64 : d == 64 ? 256 : 128;
+  const int64_t bn = d == 512 ? 64 : d == 256 ? 128 : 256;
   const int64_t tokens = std::min(n, p.bm / group + 2);
   const int64_t keys = window > 0 ? std::min(slots, window + tokens + sink) : slots;
   const int64_t tiles = (keys + bn - 1) / bn + 1 + (2 * n + bn - 1) / bn;
@@ -940,7 +992,7 @@ static int paged_main(const w8_attention_paged_args& x, const w8::PagedArgs& pa,
   if (st != W8_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
-  cfg.blockDim = dim3(w8::kPagedThreads, 1, 1);
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr;

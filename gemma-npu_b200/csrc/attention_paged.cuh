@@ -87,6 +87,13 @@ __device__ __forceinline__ void paged_unpack<__nv_bfloat16>(uint32_t x, uint32_t
   p1 = one(sel1);
 }
 
+// The same less 1152 still to be taken off, in fp16: 1024 + 128 + x.
+__device__ __forceinline__ void paged_raise(uint32_t x, uint32_t sel0, uint32_t sel1, uint32_t& p0, uint32_t& p1) {
+  const uint32_t u = x ^ 0x80808080u;
+  p0 = __byte_perm(u, 0x64646464u, sel0);
+  p1 = __byte_perm(u, 0x64646464u, sel1);
+}
+
 // The smallest power of two that is not below a scale (of 2^-126 to 2^126), and its reciprocal:
 // the unit in which the sums of values are held while pages of different scales add to them.
 __device__ __forceinline__ float paged_unit(float scale) {
