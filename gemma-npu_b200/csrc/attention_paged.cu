@@ -877,11 +877,16 @@ int tree_encode_rows(CUtensorMap* map, const void* ptr, bool half, int64_t d, in
 int tree_encode(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, const cuuint64_t* dims,
                 const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle, const char* what);
 int tree_join(const w8::TreeArgs& a, bool half, int64_t d, int bm, cudaStream_t stream);
+int paged_tc(const w8_attention_paged_args& x, const w8::PagedArgs& a, bool half, int64_t items, int device,
+             cudaStream_t stream);
+int tree_tc_device_status(int clear, int* out);
 
-// How a call is cut: rows per tile, row tiles, and the CTAs that share all tiles, or an item each.
+// How a call is cut: rows per tile, row tiles, and over the keys a number of splits (tcgen05) or of
+// CTAs that share all tiles, or an item each (mma.sync).
 struct PagedPlan {
+  bool tc;  // the tcgen05 schedule (attention_tree_tc.cu)
   bool direct;
-  int bm, row_tiles, ctas;
+  int bm, row_tiles, splits, ctas;
   int64_t items;
 };
 
@@ -889,14 +894,30 @@ static PagedPlan paged_plan(int64_t batch, int64_t kv_heads, int64_t group, int6
                             int64_t window, int64_t sink, int sms) {
   PagedPlan p;
   const int64_t rows = group * n;
-  p.bm = rows <= 8 || d == 512 ? 8 : rows <= 16 || d == 256 ? 16 : 32;
+  p.tc = rows > (d == 512 ? 8 : 16);
+  p.bm = p.tc ? 256 : rows <= 8 ? 8 : 16;
   p.row_tiles = static_cast<int>((rows + p.bm - 1) / p.bm);
   p.items = batch * kv_heads * p.row_tiles;
   // Keys of one row tile: with a window, those its tokens see.
-  const int64_t bn = d == 512 ? 64 : d == 256 ? 128 : 256;
+  const int64_t bn = p.tc ? 128 : d == 512 ? 64 : d == 256 ? 128 : 256;
   const int64_t tokens = std::min(n, p.bm / group + 2);
   const int64_t keys = window > 0 ? std::min(slots, window + tokens + sink) : slots;
-  const int64_t tiles = (keys + bn - 1) / bn + 1 + (2 * n + bn - 1) / bn;
+  const int64_t tiles = (keys + bn - 1) / bn + 1 + ((p.tc ? 1 : 2) * n + bn - 1) / bn;
+  p.splits = 1;
+  p.direct = false;
+  p.ctas = 0;
+  if (p.tc) {
+    // The number of splits with the least estimated time, as tree_plan has it.
+    const int64_t width = d == 512 ? 2 : 1, pairs = sms / 2;
+    double best = 0;
+    for (int64_t s = 1; s <= std::min<int64_t>(tiles, 64); ++s) {
+      const double waves = static_cast<double>((p.items * width * s + pairs - 1) / pairs);
+      double us = waves * (1.6 * static_cast<double>((tiles + s - 1) / s) + 8);
+      if (s > 1) us += 4 + static_cast<double>(p.items * p.bm * d) * 8 * static_cast<double>(s) / 3e6;
+      if (s == 1 || us < best) best = us, p.splits = static_cast<int>(s);
+    }
+    return p;
+  }
   // An item per CTA, or all tiles dealt evenly: by estimated times.  A tile is about 1 us, an item's
   // start and end 3 us, joining the pieces a launch of 4 us.  From 8 items an SM on ragged lengths
   // even out by themselves.
@@ -919,10 +940,12 @@ static PagedWs paged_ws(const PagedPlan& p, int64_t d) {
     at += (bytes + 255) / 256 * 256;
     return r;
   };
-  const int64_t part_rows = p.direct ? 0 : 2 * static_cast<int64_t>(p.ctas) * p.bm;
+  const int64_t part_rows = p.tc      ? (p.splits > 1 ? p.items * p.splits * p.bm : 0)
+                            : p.direct ? 0
+                                       : 2 * static_cast<int64_t>(p.ctas) * p.bm;
   w.part_o = take(part_rows * d * 4);
   w.part_ml = take(part_rows * 8);
-  w.info = take(p.direct ? 0 : p.items * 8);
+  w.info = take(p.tc || p.direct ? 0 : p.items * 8);
   w.total = at;
   return w;
 }
@@ -1008,22 +1031,20 @@ static int paged_go(const w8_attention_paged_args& x, const w8::PagedArgs& a, co
                     cudaStream_t stream) {
   W8_CHECK_ARG(p.items < (1ll << 31) / 2, "too many row tiles");
   const int64_t blocks = p.direct ? p.items : p.ctas;
+  constexpr bool kHalf = __is_same(T, __half);
   int st;
-  if (p.bm == 8) {
+  if (p.tc) {
+    st = paged_tc(x, a, kHalf, p.items, device, stream);
+  } else if (p.bm == 8) {
     st = paged_main<T, D, 1>(x, a, blocks, device, stream);
-  } else if constexpr (D <= 256) {
-    if (p.bm == 16) {
-      st = paged_main<T, D, 2>(x, a, blocks, device, stream);
-    } else if constexpr (D <= 128) {
-      st = paged_main<T, D, 4>(x, a, blocks, device, stream);
-    } else {
-      return W8_ERR_UNSUPPORTED;  // (no plan has it)
-    }
   } else {
-    return W8_ERR_UNSUPPORTED;
+    if constexpr (D <= 256)
+      st = paged_main<T, D, 2>(x, a, blocks, device, stream);
+    else
+      st = W8_ERR_UNSUPPORTED;  // (no plan has it)
   }
-  if (st != W8_OK || p.direct || p.ctas <= 1) return st;
-  return tree_join(a.t, __is_same(T, __half), D, p.bm, stream);
+  if (st != W8_OK || (p.tc ? p.splits == 1 : p.direct || p.ctas <= 1)) return st;
+  return tree_join(a.t, kHalf, D, p.bm, stream);
 }
 
 // Read (and optionally clear) the sticky device status of the paged attention.
@@ -1121,12 +1142,16 @@ extern "C" int w8_attention_paged(const w8_attention_paged_args* in, void* works
   a.sink = static_cast<int>(x.sink);
   a.scale_log2 = scale_log2;
   a.row_tiles = p.row_tiles;
-  a.splits = 1;
+  a.splits = p.splits;
+  // Boxes of 128 query rows: the group divides 128, and no stride of 0.
+  a.q_tma = group <= 128 && (group & (group - 1)) == 0;
+  for (int j = 0; j < 3; ++j)
+    if (sizes[0][j] > 1 && (x.q_stride[j] <= 0 || x.q_stride[j] >= (1ll << 38))) a.q_tma = 0;
   a.direct = p.direct ? 1 : 0;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.part_o = reinterpret_cast<float*>(ws + w.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
-  a.info = reinterpret_cast<int2*>(ws + w.info);
+  a.info = p.tc ? nullptr : reinterpret_cast<int2*>(ws + w.info);
   pa.table = x.table;
   pa.table_b = x.table_stride;
   pa.table_pages = static_cast<int>(x.table_pages);

@@ -22,7 +22,7 @@
 // of its own CTA, the softmax threads clear what must not count before they hand over P, and
 // non-finite values are added at the end to the rows that do see them.  Every wait is bounded,
 // as in attention_tc.cu.
-#include "attention_tree.cuh"
+#include "attention_paged.cuh"
 #include "attn_tc.cuh"
 
 #include <algorithm>
@@ -33,27 +33,37 @@ namespace w8 {
 constexpr int kTtBM = 128;                 // rows per CTA; 256 per pair
 constexpr int kTtBN = 128;                 // keys per tile
 constexpr int kTtSoftWarps = 8;
-constexpr int kTtThreads = 32 * (2 + kTtSoftWarps);
+constexpr int kTtUnpackWarps = 2;          // of a paged cache
+constexpr int kTtScales = 8;               // tiles whose pages' scales are held
+__device__ __forceinline__ const TreeArgs& tree_args(const TreeArgs& a) { return a; }
+__device__ __forceinline__ const TreeArgs& tree_args(const PagedArgs& a) { return a.t; }
 constexpr int kTtKeysPerCta = kTtBN / 2;
 constexpr uint32_t kTtTmemCols = 512;
 constexpr uint32_t kTtColO = 2 * kTtBN;
 
-template <int D>
+template <int D, bool kPaged>
 struct TtCfg {
+  static constexpr int kThreads = 32 * (2 + kTtSoftWarps + (kPaged ? kTtUnpackWarps : 0));
   static constexpr int kDV = D < 256 ? D : 256;           // output columns per pair
   static constexpr int kSplitD = D / kDV;                 // clusters per row block (D = 512: 2)
   static constexpr int kQBytes = kTtBM * D * 2;
   static constexpr int kKCols = D < 256 ? D : 256;        // columns of the reduction per K slot
   static constexpr int kKSlots = D / kKCols;              // slots per K tile
   static constexpr int kSlotBytes = kTtBN * kDV;          // K: 64 keys x kKCols; V: 128 keys x kDV / 2
-  static constexpr int kSlots = D == 512 ? 3 : D == 256 ? 5 : 8;
+  static constexpr int kSlots = kPaged ? (D == 512 ? 2 : D == 256 ? 4 : 8) : D == 512 ? 3 : D == 256 ? 5 : 8;
+  static constexpr int kStageBytes = kSlotBytes / 2;      // a slot's values while they are 8 bits
+  static constexpr int kStages = kPaged ? (D < 256 ? 4 : 2) : 0;
   static constexpr int kOffRing = kQBytes;
-  static constexpr int kOffBar = kOffRing + kSlots * kSlotBytes;
-  // full[kSlots], empty[kSlots], own[kSlots], q_full, s_full[2], p_full[2], pv_done[2], o_ready
-  static constexpr int kNumBars = 3 * kSlots + 8;
+  static constexpr int kOffStage = kOffRing + kSlots * kSlotBytes;
+  static constexpr int kOffBar = kOffStage + kStages * kStageBytes;
+  // full[kSlots], empty[kSlots], own[kSlots], q_full, s_full[2], p_full[2], pv_done[2], o_ready,
+  // staged[kStages], unpacked[kStages]
+  static constexpr int kNumBars = 3 * kSlots + 8 + 2 * kStages;
   static constexpr int kOffXch = kOffBar + kNumBars * 8 + 16;
   static constexpr int kOffPoison = kOffXch + 2 * kTtBM * 4;
-  static constexpr int kSmem = kOffPoison + kPoisonWords * 4 + 1024;
+  // Of the last tiles of pages: [key / 16] the scales of K and V, and bits of the 16 keys that are there.
+  static constexpr int kOffScale = kOffPoison + kPoisonWords * 4;
+  static constexpr int kSmem = kOffScale + (kPaged ? kTtScales * (2 * 8 + 1) * 4 : 0) + 1024;
   static_assert(kKCols == kDV, "K and V slots have one size");
   static_assert(kSmem <= 232448, "shared memory budget exceeded");
   static_assert(kTtBM * (kDV * 4 + 16) <= kOffBar, "the output rows fit over Q and the ring");
@@ -72,13 +82,20 @@ __device__ __forceinline__ void red_or_cluster(uint32_t addr, uint32_t bits) {
 // DR: columns of a head in memory.  Heads of 64 run as 128 whose upper half the boxes fill with
 // zeros (S and O do not change, and only the lower half is stored): the MMAs do twice their work
 // and 216 row tiles of 680 rows over 1085 keys take 194 us where mma.sync took 626.
-template <typename T, int D, int DR>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
+// Over a paged 8-bit cache (kPaged; tm_k and tm_v then are the tails' and tm_k8, tm_v8 the pool's):
+// each CTA's share of a tile's pages comes by TMA as it is into a staging slot, and two warps
+// unpack it to T into the ring's slot, which is exact; the scale of K multiplies the scores, that of
+// V goes into P relative to a power of two, in which O is held (paged_unit; the first tile of 16-bit
+// rows brings it to 1).  Pages are never careful: 8-bit values are finite, whatever they are.
+template <typename T, int D, int DR, bool kPaged, typename Args>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kThreads, 1)
     attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_vn,
-                        const __grid_constant__ TreeArgs a) {
-  using C = TtCfg<D>;
+                        const __grid_constant__ CUtensorMap tm_k8, const __grid_constant__ CUtensorMap tm_v8,
+                        const __grid_constant__ Args args) {
+  using C = TtCfg<D, kPaged>;
+  const TreeArgs& a = tree_args(args);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -95,6 +112,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
   auto p_full = [&](int b) { return q_full + 8u * (3 + b); };
   auto pv_done = [&](int b) { return q_full + 8u * (5 + b); };
   const uint32_t o_ready = q_full + 8u * 7;
+  auto staged_bar = [&](uint32_t s) { return q_full + 8u * (8 + s); };
+  auto unpacked_bar = [&](uint32_t s) { return q_full + 8u * (8 + C::kStages + s); };
+  float* const scales = reinterpret_cast<float*>(smem + C::kOffScale);                  // [kTtScales][K, V][8]
+  uint32_t* const there_bits = reinterpret_cast<uint32_t*>(scales + kTtScales * 2 * 8);  // [kTtScales]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();  // 0 = the CTA that issues the MMAs
@@ -108,7 +129,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kSlots; ++s) {
-      mbar_init(full_bar(s), 1);   // leader: one arrive.expect_tx + both CTAs' bytes
+      // leader: one arrive.expect_tx + both CTAs' bytes, or (pages) the unpacking warps of both CTAs
+      mbar_init(full_bar(s), kPaged ? 2 * kTtUnpackWarps : 1);
       mbar_init(empty_bar(s), 1);  // both: one MMA commit
       mbar_init(own_bar(s), 1);    // both: this CTA's bytes of a careful V tile
     }
@@ -120,6 +142,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
       mbar_init(pv_done(i), 1);
     }
     mbar_init(o_ready, 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(staged_bar(s), 1);
+      mbar_init(unpacked_bar(s), kTtUnpackWarps);
+    }
     *abort_flag = 0;
     fence_mbar_init();
     if (a.q_tma) prefetch_tmap(&tm_q);
@@ -127,6 +153,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     prefetch_tmap(&tm_v);
     prefetch_tmap(&tm_kn);
     prefetch_tmap(&tm_vn);
+    if constexpr (kPaged) {
+      prefetch_tmap(&tm_k8);
+      prefetch_tmap(&tm_v8);
+    }
   }
   if (threadIdx.x < kPoisonWords) reinterpret_cast<uint32_t*>(smem + C::kOffPoison)[threadIdx.x] = 0u;
   if (warp == 1) {
@@ -143,20 +173,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
   // The pair's tiles: [t0, t1) of its committed, then new-token tiles; a split of an item with
   // fewer tiles than splits has none (both CTAs agree).
   const int len = tree_len(a, b);
-  const TreeSpan span = tree_span<2 * kTtBM, kTtBN>(a, len, rt);
-  const int nc = span.c1 - span.c0, nt = nc + span.nd;
+  auto span_of = [&]() {
+    if constexpr (kPaged)
+      return paged_span<2 * kTtBM, kTtBN, kTtBN>(args, len, rt);
+    else
+      return tree_span<2 * kTtBM, kTtBN>(a, len, rt);
+  };
+  const auto span = span_of();
+  // Tiles of pages, of committed keys (the pages' and the tail's, if paged) and all.
+  int np = 0, nc, full = 0;
+  if constexpr (kPaged)
+    np = span.pages(), nc = np + span.tail, full = span.full;
+  else
+    nc = span.c1 - span.c0;
+  const int nt = nc + span.nd;
   const int t0 = static_cast<int>(static_cast<int64_t>(nt) * split / a.splits);
   const int t1 = static_cast<int>(static_cast<int64_t>(nt) * (split + 1) / a.splits);
   const int ntiles = t1 - t0;
   const int64_t part_row = (static_cast<int64_t>(item) * a.splits + split) * (2 * kTtBM) + rank * kTtBM;
   auto is_draft = [&](int i) { return t0 + i >= nc; };
-  auto key0_of = [&](int i) { return (t0 + i >= nc ? t0 + i - nc : span.c0 + t0 + i) * kTtBN; };
+  auto is_page = [&](int i) { return kPaged && t0 + i < np; };
+  // First key of a tile: a position, a row of the tail or a new token.
+  auto key0_of = [&](int i) {
+    if constexpr (kPaged) {
+      const int t = t0 + i;
+      if (t < np) return (t < span.ns ? t : span.c0 + t - span.ns) * kTtBN;
+      return (t < nc ? t - np : t - nc) * kTtBN;
+    }
+    return (t0 + i >= nc ? t0 + i - nc : span.c0 + t0 + i) * kTtBN;
+  };
+  const int sink_left = a.sink - len;  // (negative or 0 without sinks: len >= 0)
   // Of a causal chunk's tiles of new tokens, those that every row of the pair sees whole are as
   // plain as committed ones.
   const int tok_lo = rt * (2 * kTtBM) / a.group, tok_hi = (min((rt + 1) * (2 * kTtBM), rows) - 1) / a.group;
   auto careful = [&](int i) {
+    if (is_page(i)) return false;
     const int key0 = key0_of(i);
-    if (!is_draft(i)) return key0 + kTtBN > len || key0 < span.low;
+    if (!is_draft(i)) return full + key0 + kTtBN > len || full + key0 < span.low;
     return a.tree != nullptr || a.depth != nullptr || key0 + kTtBN - 1 > tok_lo ||
            (a.window > 0 && key0 <= tok_hi - a.window);
   };
@@ -169,7 +222,115 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
       if (warp < 6 && half == 0) a.part_ml[part_row + r] = make_float2(-INFINITY, 0.f);
     }
   } else if (warp == 0) {
-    if (lane == 0) {
+    if constexpr (kPaged) {
+      // ---- TMA producer (both CTAs), a page a lane: the ring in the MMA order, 16-bit tiles into its
+      // slots as below, pages into the staging slots once the ring's slot is free.
+      uint32_t g = 0, st = 0;  // ring steps; staged ones
+      bool ok = true;
+      const int box_v = min(args.shift, 7), box_k = min(args.shift, 6);  // log2 of the keys of a box
+      const int* table = args.table + b * args.table_b;
+      // Lane j's 16 keys (of 128) of tile i: their page, or -1.
+      auto page_of = [&](int i) {
+        if (i >= ntiles || !is_page(i) || lane >= kTtBN / 16) return -1;
+        const int k0 = key0_of(i) + lane * 16, p0 = k0 >> args.shift << args.shift;
+        // (whether a page is needed is decided for all of it within the tile)
+        const int lo = max(p0, key0_of(i)), hi = min(p0 + (1 << args.shift), key0_of(i) + kTtBN);
+        if (!paged_needs(args, span, lo, hi)) return -1;
+        const int p = table[k0 >> args.shift];
+        if (p < 0 || p >= args.pages) {
+          atomicExch(&g_tree_status, W8_ERR_INVALID_ARG);
+          return -1;
+        }
+        return p;
+      };
+      auto wait_slot = [&]() {
+        ok = ok && wait_phase(empty_bar(g % C::kSlots), ((g / C::kSlots) & 1u) ^ 1u, abort_flag, &g_tree_status);
+        ok = __all_sync(0xffffffffu, ok);
+        return ok;
+      };
+      auto put = [&](const CUtensorMap* m, int key0, int block0, bool own) {  // 16-bit rows
+        if (!wait_slot()) return;
+        const uint32_t slot = g % C::kSlots;
+        if (lane == 0) {
+          uint32_t bar;
+          if (own) {
+            mbar_arrive_expect_tx(own_bar(slot), C::kSlotBytes);
+            bar = mapa_shared(own_bar(slot), rank);
+            if (rank == 0) mbar_arrive_count(full_bar(slot), 2 * kTtUnpackWarps);  // the MMA thread goes by P's barrier
+          } else {
+            if (rank == 0) {
+              mbar_arrive_expect_tx(full_bar(slot), 2 * C::kSlotBytes);
+              mbar_arrive_count(full_bar(slot), 2 * kTtUnpackWarps - 1);
+            }
+            bar = mapa_shared(full_bar(slot), 0);
+          }
+          tma_load_5d_pair(ring + slot * C::kSlotBytes, m, bar, 0, key0, block0, c, b);
+        }
+        __syncwarp();
+        ++g;
+      };
+      // `n` boxes of 2^shift keys from key `from` of the tile and column x into the next staging slot.
+      auto put_pages = [&](const CUtensorMap* m, int page, int key0, int from, int n, int shift, int bytes, int x) {
+        if (!wait_slot()) return;
+        const uint32_t s = st % C::kStages;
+        ok = wait_phase(unpacked_bar(s), ((st / C::kStages) & 1u) ^ 1u, abort_flag, &g_tree_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        const int mine = __shfl_sync(0xffffffffu, page, (from + (lane << shift)) / 16 & 31);
+        const bool on = lane < n && mine >= 0;
+        const int count = __popc(__ballot_sync(0xffffffffu, on));
+        if (lane == 0) mbar_arrive_expect_tx(staged_bar(s), count * bytes);
+        __syncwarp();
+        if (on)
+          tma_load_5d(base + C::kOffStage + s * C::kStageBytes + lane * bytes, m, staged_bar(s), x,
+                      (key0 + from + (lane << shift)) & ((1 << args.shift) - 1), 0, c, mine);
+        __syncwarp();
+        ++g, ++st;
+      };
+      const int kk0 = static_cast<int>(rank) * kTtKeysPerCta;
+      const int vb0 = half * (C::kDV / 64) + static_cast<int>(rank) * (C::kDV / 128);
+      auto put_k = [&](int i, int page) {
+        if (is_page(i)) {
+          // The scales first: whoever sees the tile's scores sees them.
+          if (lane < kTtBN / 16) {
+            float* sc = scales + (i % kTtScales) * 16 + lane;
+            sc[0] = page >= 0 ? args.ks[page * args.ks_p + c * args.ks_h] : 0.f;
+            sc[8] = page >= 0 ? args.vs[page * args.vs_p + c * args.vs_h] : 0.f;
+          }
+          const uint32_t on = __ballot_sync(0xffffffffu, page >= 0);
+          if (lane == 0) there_bits[i % kTtScales] = on;
+          __syncwarp();
+          for (int s = 0; s < C::kKSlots && ok; ++s)
+            put_pages(&tm_k8, page, key0_of(i), kk0, kTtKeysPerCta >> box_k, box_k, C::kKCols << box_k, s * C::kKCols);
+        } else {
+          for (int s = 0; s < C::kKSlots && ok; ++s)
+            put(is_draft(i) ? &tm_kn : &tm_k, key0_of(i) + kk0, s * (C::kKCols / 64), false);
+        }
+      };
+      if (a.q_tma && lane == 0) {
+        if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * C::kQBytes);
+        tma_load_5d_pair(base, &tm_q, mapa_shared(q_full, 0), 0, c * a.group, row0 / a.group, 0, b);
+      }
+      __syncwarp();
+      int page = page_of(0);  // of this tile
+      put_k(0, page);
+      for (int i = 0; i < ntiles && ok; ++i) {
+        const int next = page_of(i + 1);
+        if (i + 1 < ntiles) put_k(i + 1, next);
+        if (!ok) break;
+        if (is_page(i))
+          put_pages(&tm_v8, page, key0_of(i), 0, kTtBN >> box_v, box_v, (C::kDV / 2) << box_v, vb0 * 64);
+        else
+          put(is_draft(i) ? &tm_vn : &tm_v, key0_of(i), vb0, careful(i));
+        page = next;
+      }
+      // As below: copies that nobody awaits any more get time to land.
+      if (!ok) {
+        const unsigned long long since = globaltimer();
+        while (globaltimer() - since < 50000ull) {
+        }
+      }
+    } else if (lane == 0) {
       // ---- TMA producer (both CTAs): the ring in the MMA order; copies complete on the
       // leader's barrier, which expects both CTAs' bytes, or for a careful V on this CTA's.
       uint32_t g = 0;
@@ -279,6 +440,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
       mma_commit_pair(mapa_shared(o_ready, peer));
       mbar_wait_bounded(o_ready, 0, nullptr, &g_tree_status);  // no MMA may still write TMEM when it is freed
     }
+  } else if (kPaged && warp >= 2 + kTtSoftWarps) {
+    if constexpr (kPaged) {
+      // ---- unpacking: a staging slot's 16 bytes a thread to 32 in the ring's slot, in the MMA order.
+      const int tid = threadIdx.x - 32 * (2 + kTtSoftWarps);
+      uint32_t g = 0, st = 0;
+      bool ok = true;
+      auto unpack = [&](bool pages, bool is_v) {
+        if (!pages) {
+          ++g;
+          return;
+        }
+        const uint32_t slot = g % C::kSlots, s = st % C::kStages;
+        if (ok) ok = mbar_wait_bounded(staged_bar(s), (st / C::kStages) & 1u, abort_flag, &g_tree_status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        const uint32_t from = base + C::kOffStage + s * C::kStageBytes, to = ring + slot * C::kSlotBytes;
+        // K: [64 keys x kKCols], V: [128 keys x kDV / 2], both of half a slot.
+        const int chunks = (is_v ? C::kDV / 2 : C::kKCols) / 16, keys = is_v ? kTtBN : kTtKeysPerCta;
+#pragma unroll 4
+        for (int e = tid; e < C::kStageBytes / 16; e += 32 * kTtUnpackWarps) {
+          const int row = e / chunks, ch = e % chunks;  // (powers of two)
+          uint32_t x[4], y[8];
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(from + e * 16)
+                       : "memory");
+#pragma unroll
+          for (int q = 0; q < 4; ++q) paged_unpack<T>(x[q], 0x4140u, 0x4342u, y[2 * q], y[2 * q + 1]);
+          const uint32_t line = to + (ch >> 2) * (keys * 128) + row * 128;
+          st_shared_v4(line + (((2 * ch & 7) ^ (row & 7)) << 4), y[0], y[1], y[2], y[3]);
+          st_shared_v4(line + (((2 * ch + 1 & 7) ^ (row & 7)) << 4), y[4], y[5], y[6], y[7]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(unpacked_bar(s));
+          mbar_arrive_cluster(mapa_shared(full_bar(slot), 0));
+        }
+        __syncwarp();
+        ++g, ++st;
+      };
+      for (int s = 0; s < C::kKSlots; ++s) unpack(is_page(0), false);
+      for (int i = 0; i < ntiles && ok && is_page(i); ++i) {
+        if (i + 1 < ntiles)
+          for (int s = 0; s < C::kKSlots; ++s) unpack(is_page(i + 1), false);
+        unpack(true, true);
+      }
+    }
   } else {
     // ---- softmax: row r = TMEM lane r is shared by warps w and w + 4, 64 keys each.
     const int quarter = warp & 3;
@@ -332,6 +541,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     const int first = tok >= 0 ? tree_first(a, len, dep) : len;
     const float scale = a.scale_log2;
     float m = -INFINITY, l = 0.f;
+    float unit = kPaged ? __uint_as_float(0x00800000u) : 1.f;  // of O (2^-126: nothing added yet)
     bool ok = true;
     uint32_t own_phase = 0;  // next parity of each own_bar
     // Every warp runs every iteration and meets its partner at the same pair barriers on
@@ -355,16 +565,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
         if (draft) {
           if (a.tree == nullptr && a.depth == nullptr) {  // a plain chunk: closed forms
 #pragma unroll
-            for (int j = 0; j < 2; ++j) keep[j] = tok >= 0 ? tree_sees32(a, b, tok, k0 + 32 * j, dep) : 0u;
+            for (int j = 0; j < 2; ++j) keep[j] = tok >= 0 ? tree_sees32(a, b, tok, k0 + 32 * j, dep, sink_left) : 0u;
           } else {
-            tree_sees64_rows(a, b, tok, k0, dep, keep);
+            tree_sees64_rows(a, b, tok, k0, dep, keep, sink_left);
           }
         } else {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const int lo = max(first - k0 - 32 * j, 0), hi = min(len - 1 - k0 - 32 * j, 31);
-            keep[j] = hi < lo ? 0u : (0xFFFFFFFFu >> (31 - hi)) & (0xFFFFFFFFu << lo);
+            if constexpr (kPaged) {
+              // Positions from p0 on, below the full pages' end or (the tail) the length.
+              const int p0 = (is_page(i) ? 0 : full) + k0 + 32 * j, hi = min((is_page(i) ? full : len) - 1 - p0, 31);
+              const int lo = max(first - p0, 0), sk = tok >= 0 ? min(a.sink - p0, 32) : 0;
+              uint32_t on = lo > 31 ? 0u : 0xFFFFFFFFu << lo;
+              if (a.window > 0 && sk > 0) on |= 0xFFFFFFFFu >> (32 - sk);
+              keep[j] = hi < 0 ? 0u : (0xFFFFFFFFu >> (31 - hi)) & on;
+              if (is_page(i)) {
+                const uint32_t on16 = there_bits[i % kTtScales] >> (4 * hv + 2 * j);
+                if (!(on16 & 1u)) keep[j] &= 0xFFFF0000u;
+                if (!(on16 & 2u)) keep[j] &= 0x0000FFFFu;
+              }
+            } else {
+              const int lo = max(first - k0 - 32 * j, 0), hi = min(len - 1 - k0 - 32 * j, 31);
+              keep[j] = hi < lo ? 0u : (0xFFFFFFFFu >> (31 - hi)) & (0xFFFFFFFFu << lo);
+            }
           }
+        }
+        if constexpr (kPaged) {  // the scores in log2 units
+          float f[4] = {scale, scale, scale, scale};
+          if (is_page(i)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) f[q] *= scales[(i % kTtScales) * 16 + 4 * hv + q];
+          }
+#pragma unroll
+          for (int e = 0; e < 64; ++e) sv[e >> 5][e & 31] = __float_as_uint(__uint_as_float(sv[e >> 5][e & 31]) * f[e >> 4]);
         }
         if (!__all_sync(0xffffffffu, (keep[0] & keep[1]) == 0xFFFFFFFFu)) {
 #pragma unroll
@@ -399,11 +632,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
       mx = fmaxf(mx, xch[(hv ^ 1) * kTtBM + r]);
       pair_sync();  // the partner's maximum is read before either posts the next one
       if (!ok) continue;
-      const float mt = mx * scale;
+      const float mt = kPaged ? mx : mx * scale;
       const bool move = mt > m + TreeRef<T>::kSlack;
-      if (__any_sync(0xffffffffu, move)) {
+      // O's unit: not below any scale of V so far, 1 from the first 16-bit rows on (the same in all
+      // threads of the pair).
+      float vr[4] = {1.f, 1.f, 1.f, 1.f}, to = 1.f;
+      if constexpr (kPaged) {
+        if (is_page(i)) {
+          to = unit;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) to = fmaxf(to, paged_unit(scales[(i % kTtScales) * 16 + 8 + q]));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) vr[q] = scales[(i % kTtScales) * 16 + 8 + 4 * hv + q] * paged_unit_rcp(to);
+        }
+      }
+      const bool other = kPaged && to != unit;
+      if (__any_sync(0xffffffffu, move) || other) {
         const float mn = move ? mt - TreeRef<T>::kBelow : m;
-        const float corr = move ? ex2_tc(m - mn) : 1.f;
+        float corr = move ? ex2_tc(m - mn) : 1.f;
+        l *= corr;
+        if constexpr (kPaged) corr *= unit * paged_unit_rcp(to);
+        unit = to;
         if (i > 0) {
           ok = mbar_wait_bounded(pv_done((i - 1) & 1), ((i - 1) >> 1) & 1, abort_flag, &g_tree_status);
           ok = __all_sync(0xffffffffu, ok);
@@ -420,7 +669,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
             tmem_st_32x32b_x32(tmem + lane_off + col, ov);
           }
         }
-        l *= corr;
         m = mn;
       }
       const float ref = m == -INFINITY ? 0.f : m;
@@ -428,9 +676,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
       uint32_t pw[32];
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
-        const float p0 = ex2_tc(fmaf(__uint_as_float(sv[e >> 4][(2 * e) & 31]), scale, -ref));
-        const float p1 = ex2_tc(fmaf(__uint_as_float(sv[e >> 4][(2 * e + 1) & 31]), scale, -ref));
+        const float x0 = __uint_as_float(sv[e >> 4][(2 * e) & 31]), x1 = __uint_as_float(sv[e >> 4][(2 * e + 1) & 31]);
+        float p0 = ex2_tc(kPaged ? x0 - ref : fmaf(x0, scale, -ref));
+        float p1 = ex2_tc(kPaged ? x1 - ref : fmaf(x1, scale, -ref));
         l4[e & 3] += p0 + p1;
+        if constexpr (kPaged) {  // (a NaN scale is for the rows that see the page)
+          p0 = x0 == -INFINITY ? 0.f : p0 * vr[e >> 3];
+          p1 = x1 == -INFINITY ? 0.f : p1 * vr[e >> 3];
+        }
         pw[e] = pack2<T>(p0, p1);
       }
       tmem_st_32x32b_x32(tmem + lane_off + u * kTtBN + 32 * hv, pw);
@@ -448,7 +701,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
             const int row = (e >> 3) & (kTtBN - 1);  // blocks of [128 keys x 128 bytes]
             uint4* w = reinterpret_cast<uint4*>(vs) + e;
             if (!draft) {
-              if (key0 + row >= len || key0 + row < span.low) *w = make_uint4(0, 0, 0, 0);
+              const int p = full + key0 + row;
+              if (p >= len || (p < span.low && p >= a.sink)) *w = make_uint4(0, 0, 0, 0);
             } else {
               uint4 x = *w;
               if (nonfinite_bits<T>(x.x) | nonfinite_bits<T>(x.y) | nonfinite_bits<T>(x.z) | nonfinite_bits<T>(x.w)) {
@@ -491,7 +745,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     if (drafts && tok >= 0)
       for (int j = j_begin; j < j_end && !poisoned; j += 32) {
         const uint32_t bits = poison_of(poison, j);
-        poisoned = bits != 0u && (bits & tree_sees32(a, b, tok, j, dep)) != 0u;
+        poisoned = bits != 0u && (bits & tree_sees32(a, b, tok, j, dep, sink_left)) != 0u;
       }
     __syncwarp();
     // The rows go through shared memory (Q and the ring are idle: every MMA has completed) to
@@ -501,17 +755,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTtThreads, 1)
     if (good) {
       tc_fence_after();
       const float inv = lt == 0.f ? 0.f : 1.f / lt;  // a row that sees nothing: zeros
+      // (O in units of 1; a value of a row whose every P was 0 stays 0)
+      auto whole = [&](uint32_t (&ov)[32]) {
+        if (kPaged && unit != 1.f) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) ov[x] = __float_as_uint(__uint_as_float(ov[x]) * unit);
+        }
+      };
 #pragma unroll 1
       for (int e = 0; e < C::kDV / 64; ++e) {
         uint32_t ov[32];
         const int col = (C::kDV / 2) * hv + e * 32;  // of this half
         tmem_ld_32x32b_x32(tmem + lane_off + kTtColO + col, ov);
         tmem_wait_ld();
+        whole(ov);
         if (poisoned && col < DR) {
 #pragma unroll 1
           for (int j0 = j_begin; j0 < j_end; j0 += 32) {
             uint32_t bits = poison_of(poison, j0);
-            if (bits != 0u) bits &= tree_sees32(a, b, tok, j0, dep);
+            if (bits != 0u) bits &= tree_sees32(a, b, tok, j0, dep, sink_left);
             for (; bits != 0u; bits &= bits - 1u) {
               const uint16_t* vn = a.vn + b * a.vn_b + c * a.vn_h + (j0 + __ffs(bits) - 1) * a.vn_t + half * C::kDV + col;
 #pragma unroll
@@ -647,11 +909,43 @@ static int encode_q(CUtensorMap* map, const w8::TreeArgs& a, bool half, int64_t 
                      box, CU_TENSOR_MAP_SWIZZLE_128B, "q");
 }
 
+template <typename T, int D, int DR, bool kPaged, typename Args>
+static int launch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn, const CUtensorMap& tvn,
+                     const CUtensorMap& tk8, const CUtensorMap& tv8, const w8::TreeArgs& a, const Args& args,
+                     int64_t items, int device, cudaStream_t stream) {
+  using C = w8::TtCfg<D, kPaged>;
+  CUtensorMap tq = tkn;
+  if (a.q_tma) {
+    const int st = encode_q(&tq, a, __is_same(T, __half), DR, D / 64);
+    if (st != W8_OK) return st;
+  }
+  static bool done[64] = {};
+  if (!done[device]) {
+    W8_CUDA_TRY(cudaFuncSetAttribute(w8::attn_tree_tc_kernel<T, D, DR, kPaged, Args>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    done[device] = true;
+  }
+  const int64_t blocks = 2 * items * a.splits * C::kSplitD;
+  W8_CHECK_ARG(blocks < (1ll << 31), "too many row tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_status(
+      cudaLaunchKernelEx(&cfg, w8::attn_tree_tc_kernel<T, D, DR, kPaged, Args>, tq, tk, tv, tkn, tvn, tk8, tv8, args));
+}
+
 template <typename T, int D, int DR = D>
 static int tree_tc_go(const w8::TreeArgs& a, int64_t items, int device, cudaStream_t stream) {
-  using C = w8::TtCfg<D>;
+  using C = w8::TtCfg<D, false>;
   constexpr bool kHalf = __is_same(T, __half);
-  CUtensorMap tq, tk, tv, tkn, tvn;
+  CUtensorMap tk, tv, tkn, tvn;
   const uint32_t kb = C::kKCols / 64, vb = C::kDV / 128;
   int st = tree_encode_rows(&tkn, a.kn, kHalf, DR, a.n, a.kv_heads, a.batch, a.kn_b, a.kn_h, a.kn_t, w8::kTtKeysPerCta, kb);
   if (st != W8_OK) return st;
@@ -664,30 +958,7 @@ static int tree_tc_go(const w8::TreeArgs& a, int64_t items, int device, cudaStre
     st = tree_encode_rows(&tv, a.v, kHalf, DR, a.slots, a.kv_heads, a.batch, a.v_b, a.v_h, a.v_s, w8::kTtBN, vb);
     if (st != W8_OK) return st;
   }
-  tq = tkn;
-  if (a.q_tma) {
-    st = encode_q(&tq, a, kHalf, DR, D / 64);
-    if (st != W8_OK) return st;
-  }
-  static bool done[64] = {};
-  if (!done[device]) {
-    W8_CUDA_TRY(cudaFuncSetAttribute(w8::attn_tree_tc_kernel<T, D, DR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     C::kSmem));
-    done[device] = true;
-  }
-  const int64_t blocks = 2 * items * a.splits * C::kSplitD;
-  W8_CHECK_ARG(blocks < (1ll << 31), "too many row tiles");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
-  cfg.blockDim = dim3(w8::kTtThreads, 1, 1);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, w8::attn_tree_tc_kernel<T, D, DR>, tq, tk, tv, tkn, tvn, a));
+  return launch_tc<T, D, DR, false>(tk, tv, tkn, tvn, tkn, tvn, a, a, items, device, stream);
 }
 
 // The tcgen05 schedule of w8_attention_tree (arguments checked by the caller; rows in tiles of
@@ -701,6 +972,61 @@ int tree_tc(const w8::TreeArgs& a, bool half, int64_t d, int64_t items, int devi
   if (d == 256)
     return half ? tree_tc_go<__half, 256>(a, items, device, stream) : tree_tc_go<__nv_bfloat16, 256>(a, items, device, stream);
   return half ? tree_tc_go<__half, 512>(a, items, device, stream) : tree_tc_go<__nv_bfloat16, 512>(a, items, device, stream);
+}
+
+// 5-D map over pages of 8-bit rows: (byte, row, 1, head, page).  A box {bytes, rows, 1, 1, 1} lands
+// as rows of so many bytes, zeros behind the head's.
+static int encode_pages(CUtensorMap* map, const void* ptr, int64_t d, int64_t page, int64_t heads, int64_t pages,
+                        const int64_t* stride, uint32_t bytes, uint32_t rows) {
+  auto of = [&](int64_t size, int64_t s) { return static_cast<cuuint64_t>(size > 1 ? s : d); };
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(page), 1, static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(pages)};
+  const cuuint64_t strides[4] = {of(page, stride[2]), static_cast<cuuint64_t>(d), of(heads, stride[1]), of(pages, stride[0])};
+  const cuuint32_t box[5] = {bytes, rows, 1, 1, 1};
+  return tree_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, "pages");
+}
+
+template <typename T, int D, int DR = D>
+static int paged_tc_go(const w8_attention_paged_args& x, const w8::PagedArgs& pa, int64_t items, int device,
+                       cudaStream_t stream) {
+  using C = w8::TtCfg<D, true>;
+  constexpr bool kHalf = __is_same(T, __half);
+  const w8::TreeArgs& a = pa.t;
+  CUtensorMap tkn, tvn, tkt, tvt, tk8, tv8;
+  auto rows = [&](CUtensorMap* map, const void* p, int64_t n, const int64_t* s, bool v) {
+    return tree_encode_rows(map, p, kHalf, DR, n, a.kv_heads, a.batch, s[0], s[1], s[2], v ? w8::kTtBN : w8::kTtKeysPerCta,
+                            v ? C::kDV / 128 : C::kKCols / 64);
+  };
+  int st = rows(&tkn, x.k_new, a.n, x.k_new_stride, false);
+  if (st == W8_OK) st = rows(&tvn, x.v_new, a.n, x.v_new_stride, true);
+  if (st == W8_OK) st = rows(&tkt, x.k_tail, x.page, x.k_tail_stride, false);
+  if (st == W8_OK) st = rows(&tvt, x.v_tail, x.page, x.v_tail_stride, true);
+  tk8 = tkn, tv8 = tvn;  // an empty pool: never read
+  const uint32_t box_k = static_cast<uint32_t>(std::min<int64_t>(x.page, w8::kTtKeysPerCta));
+  const uint32_t box_v = static_cast<uint32_t>(std::min<int64_t>(x.page, w8::kTtBN));
+  if (st == W8_OK && x.pages > 0)
+    st = encode_pages(&tk8, x.k, DR, x.page, x.kv_heads, x.pages, x.k_stride, C::kKCols, box_k);
+  if (st == W8_OK && x.pages > 0)
+    st = encode_pages(&tv8, x.v, DR, x.page, x.kv_heads, x.pages, x.v_stride, C::kDV / 2, box_v);
+  if (st != W8_OK) return st;
+  return launch_tc<T, D, DR, true>(tkt, tvt, tkn, tvn, tk8, tv8, a, pa, items, device, stream);
+}
+
+// The same of w8_attention_paged.
+int paged_tc(const w8_attention_paged_args& x, const w8::PagedArgs& a, bool half, int64_t items, int device,
+             cudaStream_t stream) {
+  using B = __nv_bfloat16;
+  switch (x.head_dim) {
+    case 64:
+      return half ? paged_tc_go<__half, 128, 64>(x, a, items, device, stream)
+                  : paged_tc_go<B, 128, 64>(x, a, items, device, stream);
+    case 128:
+      return half ? paged_tc_go<__half, 128>(x, a, items, device, stream) : paged_tc_go<B, 128>(x, a, items, device, stream);
+    case 256:
+      return half ? paged_tc_go<__half, 256>(x, a, items, device, stream) : paged_tc_go<B, 256>(x, a, items, device, stream);
+    default:
+      return half ? paged_tc_go<__half, 512>(x, a, items, device, stream) : paged_tc_go<B, 512>(x, a, items, device, stream);
+  }
 }
 
 // Read (and optionally clear) this schedule's sticky device status.
