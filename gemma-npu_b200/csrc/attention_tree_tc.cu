@@ -27,13 +27,15 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 namespace w8 {
 
 constexpr int kTtBM = 128;                 // rows per CTA; 256 per pair
 constexpr int kTtBN = 128;                 // keys per tile
 constexpr int kTtSoftWarps = 8;
-constexpr int kTtUnpackWarps = 2;          // of a paged cache
+constexpr int kTtUnpackWarps = 6;          // of a paged cache, in two teams that take its slots in turn
+constexpr int kTtUnpackTeam = kTtUnpackWarps / 2;
 constexpr int kTtScales = 8;               // tiles whose pages' scales are held
 __device__ __forceinline__ const TreeArgs& tree_args(const TreeArgs& a) { return a; }
 __device__ __forceinline__ const TreeArgs& tree_args(const PagedArgs& a) { return a.t; }
@@ -68,6 +70,12 @@ struct TtCfg {
   static_assert(kSmem <= 232448, "shared memory budget exceeded");
   static_assert(kTtBM * (kDV * 4 + 16) <= kOffBar, "the output rows fit over Q and the ring");
 };
+
+__device__ __forceinline__ float lg2_tc(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // Arrive on a barrier that may lie in the peer CTA, releasing this thread's shared-memory
 // writes to the cluster.
@@ -130,7 +138,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kSlots; ++s) {
       // leader: one arrive.expect_tx + both CTAs' bytes, or (pages) the unpacking warps of both CTAs
-      mbar_init(full_bar(s), kPaged ? 2 * kTtUnpackWarps : 1);
+      mbar_init(full_bar(s), kPaged ? 2 * kTtUnpackTeam : 1);
       mbar_init(empty_bar(s), 1);  // both: one MMA commit
       mbar_init(own_bar(s), 1);    // both: this CTA's bytes of a careful V tile
     }
@@ -144,7 +152,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
     mbar_init(o_ready, 1);
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(staged_bar(s), 1);
-      mbar_init(unpacked_bar(s), kTtUnpackWarps);
+      mbar_init(unpacked_bar(s), kTtUnpackTeam);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -229,17 +237,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
       bool ok = true;
       const int box_v = min(args.shift, 7), box_k = min(args.shift, 6);  // log2 of the keys of a box
       const int* table = args.table + b * args.table_b;
-      // Lane j's 16 keys (of 128) of tile i: their page, or -1.
-      auto page_of = [&](int i) {
+      // Lane j's 16 keys (of 128) of tile i: the table's entry if some row needs it, or -1; the page it
+      // names; its scales.  Each is read a tile before the next needs it.
+      auto entry_of = [&](int i) {
         if (i >= ntiles || !is_page(i) || lane >= kTtBN / 16) return -1;
         const int k0 = key0_of(i) + lane * 16, p0 = k0 >> args.shift << args.shift;
         // (whether a page is needed is decided for all of it within the tile)
         const int lo = max(p0, key0_of(i)), hi = min(p0 + (1 << args.shift), key0_of(i) + kTtBN);
         if (!paged_needs(args, span, lo, hi)) return -1;
         const int p = table[k0 >> args.shift];
-        if (p < 0 || p >= args.pages) {
+        return p < 0 ? INT32_MAX : p;
+      };
+      struct Page {
+        int at;
+        float ks, vs;
+      };
+      auto page_of = [&](int entry) {
+        Page p = {entry, 0.f, 0.f};
+        if (entry >= args.pages) {
           atomicExch(&g_tree_status, W8_ERR_INVALID_ARG);
-          return -1;
+          p.at = -1;
+        }
+        if (p.at >= 0) {
+          p.ks = args.ks[p.at * args.ks_p + c * args.ks_h];
+          p.vs = args.vs[p.at * args.vs_p + c * args.vs_h];
         }
         return p;
       };
@@ -256,11 +277,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
           if (own) {
             mbar_arrive_expect_tx(own_bar(slot), C::kSlotBytes);
             bar = mapa_shared(own_bar(slot), rank);
-            if (rank == 0) mbar_arrive_count(full_bar(slot), 2 * kTtUnpackWarps);  // the MMA thread goes by P's barrier
+            if (rank == 0) mbar_arrive_count(full_bar(slot), 2 * kTtUnpackTeam);  // the MMA thread goes by P's barrier
           } else {
             if (rank == 0) {
               mbar_arrive_expect_tx(full_bar(slot), 2 * C::kSlotBytes);
-              mbar_arrive_count(full_bar(slot), 2 * kTtUnpackWarps - 1);
+              mbar_arrive_count(full_bar(slot), 2 * kTtUnpackTeam - 1);
             }
             bar = mapa_shared(full_bar(slot), 0);
           }
@@ -289,19 +310,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
       };
       const int kk0 = static_cast<int>(rank) * kTtKeysPerCta;
       const int vb0 = half * (C::kDV / 64) + static_cast<int>(rank) * (C::kDV / 128);
-      auto put_k = [&](int i, int page) {
+      auto put_k = [&](int i, const Page& page) {
         if (is_page(i)) {
           // The scales first: whoever sees the tile's scores sees them.
           if (lane < kTtBN / 16) {
             float* sc = scales + (i % kTtScales) * 16 + lane;
-            sc[0] = page >= 0 ? args.ks[page * args.ks_p + c * args.ks_h] : 0.f;
-            sc[8] = page >= 0 ? args.vs[page * args.vs_p + c * args.vs_h] : 0.f;
+            sc[0] = page.ks;
+            sc[8] = page.vs;
           }
-          const uint32_t on = __ballot_sync(0xffffffffu, page >= 0);
+          const uint32_t on = __ballot_sync(0xffffffffu, page.at >= 0);
           if (lane == 0) there_bits[i % kTtScales] = on;
           __syncwarp();
           for (int s = 0; s < C::kKSlots && ok; ++s)
-            put_pages(&tm_k8, page, key0_of(i), kk0, kTtKeysPerCta >> box_k, box_k, C::kKCols << box_k, s * C::kKCols);
+            put_pages(&tm_k8, page.at, key0_of(i), kk0, kTtKeysPerCta >> box_k, box_k, C::kKCols << box_k, s * C::kKCols);
         } else {
           for (int s = 0; s < C::kKSlots && ok; ++s)
             put(is_draft(i) ? &tm_kn : &tm_k, key0_of(i) + kk0, s * (C::kKCols / 64), false);
@@ -312,17 +333,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
         tma_load_5d_pair(base, &tm_q, mapa_shared(q_full, 0), 0, c * a.group, row0 / a.group, 0, b);
       }
       __syncwarp();
-      int page = page_of(0);  // of this tile
+      Page page = page_of(entry_of(0)), next = page_of(entry_of(1));  // of this tile and the next
+      int entry = entry_of(2);
       put_k(0, page);
       for (int i = 0; i < ntiles && ok; ++i) {
-        const int next = page_of(i + 1);
+        const Page after = page_of(entry);
+        entry = entry_of(i + 3);
         if (i + 1 < ntiles) put_k(i + 1, next);
         if (!ok) break;
         if (is_page(i))
-          put_pages(&tm_v8, page, key0_of(i), 0, kTtBN >> box_v, box_v, (C::kDV / 2) << box_v, vb0 * 64);
+          put_pages(&tm_v8, page.at, key0_of(i), 0, kTtBN >> box_v, box_v, (C::kDV / 2) << box_v, vb0 * 64);
         else
           put(is_draft(i) ? &tm_vn : &tm_v, key0_of(i), vb0, careful(i));
-        page = next;
+        page = next, next = after;
       }
       // As below: copies that nobody awaits any more get time to land.
       if (!ok) {
@@ -442,13 +465,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
     }
   } else if (kPaged && warp >= 2 + kTtSoftWarps) {
     if constexpr (kPaged) {
-      // ---- unpacking: a staging slot's 16 bytes a thread to 32 in the ring's slot, in the MMA order.
-      const int tid = threadIdx.x - 32 * (2 + kTtSoftWarps);
+      // ---- unpacking: a staging slot's 16 bytes a thread to 32 in the ring's slot, in the MMA order.  A
+      // release to the cluster drains a thread's stores first, some 1000 clocks: two teams of warps
+      // take the staging slots in turn, so that one unpacks while the other waits (PLACEHOLDER).
+      const int team = (warp - 2 - kTtSoftWarps) / kTtUnpackTeam;
+      const int tid = threadIdx.x - 32 * (2 + kTtSoftWarps + team * kTtUnpackTeam);
+      static_assert(C::kStages % 2 == 0, "a staging slot is one team's");
       uint32_t g = 0, st = 0;
       bool ok = true;
-      auto unpack = [&](bool pages, bool is_v) {
-        if (!pages) {
+      auto unpack = [&](bool pages, auto columns) {  // (columns: of a row, a constant)
+        if (!pages || (st & 1) != team) {
           ++g;
+          st += pages;
           return;
         }
         const uint32_t slot = g % C::kSlots, s = st % C::kStages;
@@ -457,20 +485,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
         if (!ok) return;
         const uint32_t from = base + C::kOffStage + s * C::kStageBytes, to = ring + slot * C::kSlotBytes;
         // K: [64 keys x kKCols], V: [128 keys x kDV / 2], both of half a slot.
-        const int chunks = (is_v ? C::kDV / 2 : C::kKCols) / 16, keys = is_v ? kTtBN : kTtKeysPerCta;
-#pragma unroll 4
-        for (int e = tid; e < C::kStageBytes / 16; e += 32 * kTtUnpackWarps) {
-          const int row = e / chunks, ch = e % chunks;  // (powers of two)
-          uint32_t x[4], y[8];
-          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                       : "r"(from + e * 16)
-                       : "memory");
+        constexpr int chunks = decltype(columns)::value / 16, keys = C::kStageBytes / 16 / chunks;
+        constexpr int kAll = C::kStageBytes / 16, kStep = 32 * kTtUnpackTeam, kBatch = 4;
+#pragma unroll 1
+        for (int e0 = tid; e0 < kAll; e0 += kBatch * kStep) {
+          uint32_t x[kBatch][4];  // (all loads before the first store)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) paged_unpack<T>(x[q], 0x4140u, 0x4342u, y[2 * q], y[2 * q + 1]);
-          const uint32_t line = to + (ch >> 2) * (keys * 128) + row * 128;
-          st_shared_v4(line + (((2 * ch & 7) ^ (row & 7)) << 4), y[0], y[1], y[2], y[3]);
-          st_shared_v4(line + (((2 * ch + 1 & 7) ^ (row & 7)) << 4), y[4], y[5], y[6], y[7]);
+          for (int k = 0; k < kBatch; ++k) {
+            const int e = min(e0 + k * kStep, kAll - 1);
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(x[k][0]), "=r"(x[k][1]), "=r"(x[k][2]), "=r"(x[k][3])
+                         : "r"(from + e * 16)
+                         : "memory");
+          }
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            const int e = e0 + k * kStep, row = e / chunks, ch = e % chunks;
+            if (e >= kAll) break;
+            uint32_t y[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) paged_unpack<T>(x[k][q], 0x4140u, 0x4342u, y[2 * q], y[2 * q + 1]);
+            const uint32_t line = to + (ch >> 2) * (keys * 128) + row * 128;
+            st_shared_v4(line + (((2 * ch & 7) ^ (row & 7)) << 4), y[0], y[1], y[2], y[3]);
+            st_shared_v4(line + (((2 * ch + 1 & 7) ^ (row & 7)) << 4), y[4], y[5], y[6], y[7]);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -481,11 +519,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
         __syncwarp();
         ++g, ++st;
       };
-      for (int s = 0; s < C::kKSlots; ++s) unpack(is_page(0), false);
+      using K = std::integral_constant<int, C::kKCols>;
+      using V = std::integral_constant<int, C::kDV / 2>;
+      for (int s = 0; s < C::kKSlots; ++s) unpack(is_page(0), K());
       for (int i = 0; i < ntiles && ok && is_page(i); ++i) {
         if (i + 1 < ntiles)
-          for (int s = 0; s < C::kKSlots; ++s) unpack(is_page(i + 1), false);
-        unpack(true, true);
+          for (int s = 0; s < C::kKSlots; ++s) unpack(is_page(i + 1), K());
+        unpack(true, V());
       }
     }
   } else {
@@ -554,6 +594,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
       ok = __all_sync(0xffffffffu, ok);
       uint32_t sv[2][32];
       float mx = -INFINITY;
+      float to_log2[4] = {scale, scale, scale, scale};  // of 16 keys each
       if (ok) {
         tc_fence_after();
         tmem_ld_32x32b_x32(tmem + lane_off + u * kTtBN + 64 * hv, sv[0]);
@@ -590,15 +631,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
             }
           }
         }
-        if constexpr (kPaged) {  // the scores in log2 units
-          float f[4] = {scale, scale, scale, scale};
-          if (is_page(i)) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) f[q] *= scales[(i % kTtScales) * 16 + 4 * hv + q];
-          }
-#pragma unroll
-          for (int e = 0; e < 64; ++e) sv[e >> 5][e & 31] = __float_as_uint(__uint_as_float(sv[e >> 5][e & 31]) * f[e >> 4]);
-        }
         if (!__all_sync(0xffffffffu, (keep[0] & keep[1]) == 0xFFFFFFFFu)) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
@@ -607,8 +639,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
               if (!((keep[j] >> e) & 1u)) sv[j][e] = __float_as_uint(-INFINITY);
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if constexpr (kPaged) {  // 16 keys have one scale; in log2 units
 #pragma unroll
-        for (int e = 0; e < 64; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(sv[e >> 5][e & 31]));
+          for (int e = 0; e < 64; ++e) m4[e >> 4] = fmaxf(m4[e >> 4], __uint_as_float(sv[e >> 5][e & 31]));
+          if (is_page(i)) {
+            // (not 0, times which a hidden key's -inf would be NaN: a page's keys may all be 0)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) to_log2[q] = fmaxf(scales[(i % kTtScales) * 16 + 4 * hv + q] * scale, 1e-30f);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) to_log2[q] = scale;
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) m4[q] *= to_log2[q];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(sv[e >> 5][e & 31]));
+        }
         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if (a.scores != nullptr && half == 0 && tok >= 0) {
           float* dst = a.scores + (static_cast<int64_t>(bc) * rows + rr) * a.score_pitch + (draft ? a.draft_at : 0) + k0;
@@ -674,17 +721,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
       const float ref = m == -INFINITY ? 0.f : m;
       float l4[4] = {0.f, 0.f, 0.f, 0.f};
       uint32_t pw[32];
+      if constexpr (kPaged) {
+        // P in O's unit, the scale of V in the exponent: 2^(x - m + log2 vr); l takes it back, 16 keys
+        // at a time.  (A scale of 0 is 2^-100 here: the values are 0.)
+        bool odd = false;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const float x0 = __uint_as_float(sv[e >> 4][(2 * e) & 31]), x1 = __uint_as_float(sv[e >> 4][(2 * e + 1) & 31]);
-        float p0 = ex2_tc(kPaged ? x0 - ref : fmaf(x0, scale, -ref));
-        float p1 = ex2_tc(kPaged ? x1 - ref : fmaf(x1, scale, -ref));
-        l4[e & 3] += p0 + p1;
-        if constexpr (kPaged) {  // (a NaN scale is for the rows that see the page)
-          p0 = x0 == -INFINITY ? 0.f : p0 * vr[e >> 3];
-          p1 = x1 == -INFINITY ? 0.f : p1 * vr[e >> 3];
+        for (int q = 0; q < 4; ++q) odd |= vr[q] != vr[q];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float v = fmaxf(vr[q], 0x1p-100f), ref_q = ref - lg2_tc(v);
+#pragma unroll
+          for (int e = 8 * q; e < 8 * q + 8; ++e) {
+            const float p0 = ex2_tc(fmaf(__uint_as_float(sv[e >> 4][(2 * e) & 31]), to_log2[q], -ref_q));
+            const float p1 = ex2_tc(fmaf(__uint_as_float(sv[e >> 4][(2 * e + 1) & 31]), to_log2[q], -ref_q));
+            l4[q] += p0 + p1;
+            pw[e] = pack2<T>(p0, p1);
+          }
+          l4[q] *= 1.f / v;
         }
-        pw[e] = pack2<T>(p0, p1);
+        if (odd) {  // a NaN scale is for the rows that see the page
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (vr[e >> 3] != vr[e >> 3]) {
+              const bool on0 = __uint_as_float(sv[e >> 4][(2 * e) & 31]) != -INFINITY;
+              const bool on1 = __uint_as_float(sv[e >> 4][(2 * e + 1) & 31]) != -INFINITY;
+              pw[e] = pack2<T>(on0 ? vr[e >> 3] : 0.f, on1 ? vr[e >> 3] : 0.f);
+            }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float p0 = ex2_tc(fmaf(__uint_as_float(sv[e >> 4][(2 * e) & 31]), scale, -ref));
+          const float p1 = ex2_tc(fmaf(__uint_as_float(sv[e >> 4][(2 * e + 1) & 31]), scale, -ref));
+          l4[e & 3] += p0 + p1;
+          pw[e] = pack2<T>(p0, p1);
+        }
       }
       tmem_st_32x32b_x32(tmem + lane_off + u * kTtBN + 32 * hv, pw);
       l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
