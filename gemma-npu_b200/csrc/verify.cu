@@ -47,7 +47,7 @@ struct VerifyArgs {
 
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
-constexpr int kVerifyCluster = 8;    // CTAs at most (portable)
+constexpr int kVerifyCluster = 16;   // CTAs at most (8 where the GPU has no 16 free together)
 constexpr int kVerifyNodes = 1024;   // of a tree at most
 constexpr int kVerifyVec = 8;        // values of a thread at a time
 
@@ -77,37 +77,47 @@ __device__ __forceinline__ void load8(const E* row, int v, int end, bool wide, f
   }
 }
 
-// 2^x: x = n + j / 32 + g, |g| <= 1 / 64, 2^(j / 32) from the table, 2^g a polynomial (its next
-// term, (g ln 2)^6 / 720, is below 2^-48 of 1); 0 below 2^-1000.
-__device__ __forceinline__ double exp2_64(double x, const double* table) {
-  const double t = fmin(fmax(x, -1000.0), 1000.0);
+// 2^t, |t| < 1000: t = n + j / 32 + g, |g| <= 1 / 64, 2^(j / 32) from the table, 2^g a polynomial (its
+// next term, (g ln 2)^6 / 720, is below 2^-48 of 1).
+__device__ __forceinline__ double exp2_64(double t, const double* table) {
   const double big = t + 0x1.8p52 / 32.0;  // rounded to a multiple of 1 / 32
   const int k = __double2loint(big);
-  const double g = (t - (big - 0x1.8p52 / 32.0)) * 0.6931471805599453;
-  double p = fma(g, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(g, p, 1.0 / 6.0);
-  p = fma(g, p, 0.5);
-  p = fma(g, p, 1.0);
-  p = fma(g, p, 1.0);
-  const double s = table[k & 31] * p;
-  // (k >> 5 is within 1000 of 0: the exponent stays normal)
-  const double r = __hiloint2double(__double2hiint(s) + ((k >> 5) << 20), __double2loint(s));
-  return x < -1000.0 ? 0.0 : r;
+  const double g = t - (big - 0x1.8p52 / 32.0);
+  double p = fma(g, 1.333355814642844e-3, 9.618129107628477e-3);  // (ln 2)^5 / 5!, (ln 2)^4 / 4!
+  p = fma(g, p, 5.550410866482158e-2);
+  p = fma(g, p, 2.402265069591007e-1);
+  p = fma(g, p, 6.931471805599453e-1);
+  const double u = table[k & 31], s = fma(u * g, p, u);
+  return __hiloint2double(__double2hiint(s) + ((k >> 5) << 20), __double2loint(s));
 }
-// A logit in log2 units of its probability (up to the row's constant).
-__device__ __forceinline__ double level_64(float x, double cap, double slope, const double* table) {
-  if (cap == 0.0) return static_cast<double>(x) * slope;
-  if (x == -INFINITY) return -INFINITY;
-  // tanh(z) = 1 - 2 / (1 + e^2z)
-  const double e = exp2_64(static_cast<double>(x) * (2.0 * 1.4426950408889634 / cap), table);
-  return cap * slope * (1.0 - 2.0 / (1.0 + e));
+// Weights of a row's logits: 2^(level - top), the level a logit in log2 units of its probability.
+struct VerifyScale {
+  bool capped;
+  float most;               // 20 caps: tanh is 1 to 2^-57 from there on
+  float slope, two_over_cap, cap_slope;  // for fp32
+  double in, out, twice;    // log2(e) 2 / cap, cap slope (slope without a cap), 2 cap slope
+};
+// In 64 bits; `top` the row's largest level to fp32.  What is below 2^-160 counts as 0.
+__device__ __forceinline__ double weight_64(float x, const VerifyScale& c, float top, const double* table) {
+  if (!c.capped) {
+    const float d = fmaf(x, c.slope, -top);
+    return d < -160.f ? 0.0 : exp2_64(fma(static_cast<double>(x), c.out, -static_cast<double>(top)), table);
+  }
+  // tanh(z) = 1 - 2 / (1 + e^2z); the reciprocal by one step of Newton's iteration from 22 bits
+  const float xc = fminf(fmaxf(x, -c.most), c.most);
+  const double d = 1.0 + exp2_64(static_cast<double>(xc) * c.in, table);
+  float r32;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r32) : "f"(static_cast<float>(d)));
+  const double r0 = static_cast<double>(r32), r = fma(r0, fma(-d, r0, 1.0), r0);
+  const double t = fma(-c.twice, r, c.out - static_cast<double>(top));
+  return x == -INFINITY || t < -160.0 ? 0.0 : exp2_64(t, table);
 }
-__device__ __forceinline__ float level_32(float x, float two_over_cap, float cap_slope, float slope) {
-  if (two_over_cap == 0.f) return x * slope;
+__device__ __forceinline__ float level_32(float x, const VerifyScale& c) {
+  if (!c.capped) return x * c.slope;
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * two_over_cap));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * c.two_over_cap));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return x == -INFINITY ? -INFINITY : cap_slope * (1.f - 2.f * r);
+  return x == -INFINITY ? -INFINITY : c.cap_slope * (1.f - 2.f * r);
 }
 __device__ __forceinline__ float ex2_32(float x) {
   float y;
@@ -117,7 +127,8 @@ __device__ __forceinline__ float ex2_32(float x) {
 
 // One row's probabilities 2^(level - top) / sum.
 struct VerifyRow {
-  double top, sum;
+  float top;
+  double sum;
   bool fine;  // the row has a finite largest logit and no NaN
 };
 
@@ -226,11 +237,8 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
   };
 
   // ---- sampling: a row's maximum and sum in fp32 ...
-  const float two_over_cap = a.cap > 0.0 ? static_cast<float>(2.0 * 1.4426950408889634 / a.cap) : 0.f;
-  const float cap_slope = static_cast<float>(a.cap * a.slope), slope32 = static_cast<float>(a.slope);
-  auto stats = [&](const E* row, bool capped) {
+  auto stats = [&](const E* row, const VerifyScale& scale) {
     const bool wide = aligned16(row);
-    const float toc = capped ? two_over_cap : 0.f;
     float top = -INFINITY, sum = 0.f;  // in log2 units
     bool bad = false;
 #pragma unroll 2
@@ -241,7 +249,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
 #pragma unroll
       for (int i = 0; i < kVerifyVec; ++i) {
         bad |= !(x[i] < INFINITY);
-        x[i] = level_32(x[i], toc, cap_slope, slope32);
+        x[i] = level_32(x[i], scale);
         most = fmaxf(most, x[i]);
       }
       if (most > top) sum *= ex2_32(top - most), top = most;
@@ -256,19 +264,19 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
     __syncthreads();
     if (lane == 0) wide_a[warp] = high;
     bad = __syncthreads_or(bad);
-    double mine = wide_a[0];
+    float mine = static_cast<float>(wide_a[0]);
 #pragma unroll
-    for (int w = 1; w < kVerifyWarps; ++w) mine = fmax(mine, wide_a[w]);
-    double part = top == -INFINITY ? 0.0 : static_cast<double>(sum) * ex2_32(top - static_cast<float>(mine)), none = 0.0;
+    for (int w = 1; w < kVerifyWarps; ++w) mine = fmaxf(mine, static_cast<float>(wide_a[w]));
+    double part = top == -INFINITY ? 0.0 : static_cast<double>(sum) * ex2_32(top - mine), none = 0.0;
     block_sums(part, none);
     exchange(mine, bad ? __longlong_as_double(0x7FF8000000000000ll) : part);
     VerifyRow r;
-    r.top = shared_a[turn][0];
-    for (int k = 1; k < ranks; ++k) r.top = fmax(r.top, shared_a[turn][k]);
+    r.top = static_cast<float>(shared_a[turn][0]);
+    for (int k = 1; k < ranks; ++k) r.top = fmaxf(r.top, static_cast<float>(shared_a[turn][k]));
     r.sum = 0.0;
     for (int k = 0; k < ranks; ++k) {
       const double s = shared_b[turn][k];  // (NaN: the row is not fine)
-      if (s != 0.0) r.sum += s * ex2_32(static_cast<float>(shared_a[turn][k] - r.top));
+      if (s != 0.0) r.sum += s * ex2_32(static_cast<float>(shared_a[turn][k]) - r.top);
     }
     r.fine = r.sum > 0.0 && isfinite(r.sum) && isfinite(r.top);
     return r;
@@ -280,6 +288,20 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       if (zs[i] > 0.0) p = fmax(p - q, 0.0) * zs[i];
     return p;
   };
+
+  VerifyScale drafted = {};
+  drafted.slope = static_cast<float>(a.slope);
+  drafted.out = a.slope;
+  VerifyScale target = drafted;
+  if (a.cap > 0.0) {
+    target.capped = true;
+    target.most = static_cast<float>(20.0 * a.cap);
+    target.two_over_cap = static_cast<float>(2.0 * 1.4426950408889634 / a.cap);
+    target.cap_slope = static_cast<float>(a.cap * a.slope);
+    target.in = 2.0 * 1.4426950408889634 / a.cap;
+    target.out = a.cap * a.slope;
+    target.twice = 2.0 * target.out;
+  }
 
   int cur = 0, taken = 1;
   int64_t next = -1;
@@ -308,14 +330,15 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       const E* xr = row_of(a.x, a.x_b, a.x_n, cur);
       const E* dr = a.d != nullptr ? row_of(a.d, a.d_b, a.d_n, cur) : nullptr;
       int c = child_after(cur);
-      VerifyRow p = stats(xr, true), q = {0.0, 1.0, true};
-      if (dr != nullptr && c < a.n) q = stats(dr, false);
+      VerifyRow p = stats(xr, target), q = {0.f, 1.0, true};
+      if (dr != nullptr && c < a.n) q = stats(dr, drafted);
       if (!p.fine) break;
       int rejected = 0;
       bool sharp = false;  // the sums are in 64 bits
+      double last_z = 0.0;
       // The weights of one value after all rejections so far.
-      auto p_of = [&](float x) { return exp2_64(level_64(x, a.cap, a.slope, table) - p.top, table) / p.sum; };
-      auto q_of = [&](float x) { return exp2_64(static_cast<double>(x) * a.slope - q.top, table) / q.sum; };
+      auto p_of = [&](float x) { return weight_64(x, target, p.top, table) / p.sum; };
+      auto q_of = [&](float x) { return weight_64(x, drafted, q.top, table) / q.sum; };
       if (q.fine)
         for (; c < a.n; c = child_after(c)) {
           const int64_t t = tokens[c];
@@ -352,8 +375,8 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
               load8<E>(dr, v, hi, wd, y);
 #pragma unroll
               for (int i = 0; i < kVerifyVec; ++i) {
-                sp += exp2_64(level_64(x[i], a.cap, a.slope, table) - p.top, table);
-                sq += exp2_64(static_cast<double>(y[i]) * a.slope - q.top, table);
+                sp += weight_64(x[i], target, p.top, table);
+                sq += weight_64(y[i], drafted, q.top, table);
               }
             }
             cluster_sums(sp, sq);
@@ -368,12 +391,13 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
             load8<E>(dr, v, hi, wd, y);
 #pragma unroll
             for (int i = 0; i < kVerifyVec; ++i) {
-              const double pv = exp2_64(level_64(x[i], a.cap, a.slope, table) - p.top, table) * rp;
-              const double qv = exp2_64(static_cast<double>(y[i]) * a.slope - q.top, table) * rq;
+              const double pv = weight_64(x[i], target, p.top, table) * rp;
+              const double qv = weight_64(y[i], drafted, q.top, table) * rq;
               z += fmax(left_after(pv, qv, rejected) - qv, 0.0);
             }
           }
           cluster_sums(z, none);
+          last_z = z;
           if (tid == 0) zs[rejected] = z > 0.0 ? 1.0 / z : 0.0;
           ++rejected;
           __syncthreads();
@@ -383,14 +407,20 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
         const bool wx = aligned16(xr), wd = dr != nullptr && aligned16(dr);
         const double rp = 1.0 / p.sum, rq = 1.0 / q.sum;
         const bool residual = dr != nullptr && rejected > 0;
+        // What is left after the last rejection has been summed already (not yet over its sum).
+        const bool summed = residual && last_z > 0.0;
         auto weights = [&](int v, double (&f)[kVerifyVec]) {
           float x[kVerifyVec], y[kVerifyVec];
           load8<E>(xr, v, hi, wx, x);
           if (residual) load8<E>(dr, v, hi, wd, y);
 #pragma unroll
           for (int i = 0; i < kVerifyVec; ++i) {
-            f[i] = exp2_64(level_64(x[i], a.cap, a.slope, table) - p.top, table) * rp;
-            if (residual) f[i] = left_after(f[i], exp2_64(static_cast<double>(y[i]) * a.slope - q.top, table) * rq, rejected);
+            f[i] = weight_64(x[i], target, p.top, table) * rp;
+            if (residual) {
+              const double qv = weight_64(y[i], drafted, q.top, table) * rq;
+              f[i] = left_after(f[i], qv, summed ? rejected - 1 : rejected);
+              if (summed) f[i] = fmax(f[i] - qv, 0.0);
+            }
           }
           if (dr == nullptr)
             for (int k = 0; k < rejected; ++k)
@@ -400,8 +430,8 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
                   if (gone[k] == v + i) f[i] = 0.0;
               }
         };
-        double total;
-        while (true) {
+        double total = last_z;
+        while (!summed) {
           double part = 0.0, none = 0.0;
           for (int v = lo + tid * kVerifyVec; v < hi; v += kStep) {
             double f[kVerifyVec];
@@ -515,18 +545,36 @@ int verify_device_status(int clear, int* out) {
 }
 
 template <typename E>
-static int verify_go(const w8::VerifyArgs& a, int64_t batch, int cluster, cudaStream_t stream) {
+static int verify_go(w8::VerifyArgs a, int64_t batch, int device, int sms, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(batch * cluster), 1, 1);
   cfg.blockDim = dim3(w8::kVerifyThreads, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
+  static int most[64] = {};  // CTAs of a cluster that the device takes
+  if (most[device] == 0) {
+    W8_CUDA_TRY(cudaFuncSetAttribute(w8::draft_verify_kernel<E>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cfg.gridDim = dim3(w8::kVerifyCluster, 1, 1);
+    attr[0].val.clusterDim.x = w8::kVerifyCluster;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, w8::draft_verify_kernel<E>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      clusters = 0;
+    }
+    most[device] = clusters > 0 ? w8::kVerifyCluster : 8;
+  }
+  // CTAs of a sequence: as many as give each an SM to itself (64 bits keep an SM's pipes busy, and two
+  // CTAs on some SMs would be what the others wait for), each with at least 2048 values.
+  const int64_t fill = std::max<int64_t>(1, sms / batch), fit = std::max<int64_t>(1, a.vocab / 2048);
+  const int cluster = static_cast<int>(std::min<int64_t>({most[device], fill, fit}));
+  a.per = static_cast<int>(((a.vocab + cluster - 1) / cluster + 7) / 8 * 8);
+  cfg.gridDim = dim3(static_cast<unsigned>(batch * cluster), 1, 1);
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   cfg.numAttrs = 2;
   return cuda_status(cudaLaunchKernelEx(&cfg, w8::draft_verify_kernel<E>, a));
 }
@@ -565,12 +613,8 @@ extern "C" int w8_draft_verify(const w8_draft_verify_args* in, w8_stream_t strea
   a.greedy = greedy;
   a.cap = greedy ? 0.0 : x.cap;
   a.slope = greedy ? 1.0 : 1.4426950408889634 / x.temperature;
-  // CTAs of a sequence: what fills the GPU twice over, each with at least 2048 values.
-  int cluster = 1;
-  while (cluster < w8::kVerifyCluster && x.batch * cluster * 2 <= 2 * sms && x.vocab >= 4096ll * cluster) cluster *= 2;
-  a.per = static_cast<int>(((x.vocab + cluster - 1) / cluster + 7) / 8 * 8);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (x.dtype == W8_FP32) return verify_go<float>(a, x.batch, cluster, s);
-  if (x.dtype == W8_BF16) return verify_go<__nv_bfloat16>(a, x.batch, cluster, s);
-  return verify_go<__half>(a, x.batch, cluster, s);
+  if (x.dtype == W8_FP32) return verify_go<float>(a, x.batch, device, sms, s);
+  if (x.dtype == W8_BF16) return verify_go<__nv_bfloat16>(a, x.batch, device, sms, s);
+  return verify_go<__half>(a, x.batch, device, sms, s);
 }
