@@ -93,24 +93,35 @@ __device__ __forceinline__ double exp2_64(double t, const double* table) {
 // Weights of a row's logits: 2^(level - top), the level a logit in log2 units of its probability.
 struct VerifyScale {
   bool capped;
+  bool deep;                // a capped row's levels may differ by more than 900
   float most;               // 20 caps: tanh is 1 to 2^-57 from there on
   float slope, two_over_cap, cap_slope;  // for fp32
   double in, out, twice;    // log2(e) 2 / cap, cap slope (slope without a cap), 2 cap slope
 };
-// In 64 bits; `top` the row's largest level to fp32.  What is below 2^-160 counts as 0.
-__device__ __forceinline__ double weight_64(float x, const VerifyScale& c, float top, const double* table) {
+// In 64 bits; `top` the row's largest level to fp32, `least` the logit whose level is 1000 below it:
+// less counts as 0.  Without branches: the values of a thread are to be under way together.
+__device__ __forceinline__ double weight_64(float x, const VerifyScale& c, float top, float least, const double* table) {
+  double w;
+  bool none;
   if (!c.capped) {
-    const float d = fmaf(x, c.slope, -top);
-    return d < -160.f ? 0.0 : exp2_64(fma(static_cast<double>(x), c.out, -static_cast<double>(top)), table);
+    none = x < least;
+    w = exp2_64(fma(static_cast<double>(fmaxf(x, least)), c.out, -static_cast<double>(top)), table);
+  } else {
+    // tanh(z) = 1 - 2 / (1 + e^2z); the reciprocal by one step of Newton's iteration from 22 bits
+    const float xc = fminf(fmaxf(x, -c.most), c.most);
+    const double d = 1.0 + exp2_64(static_cast<double>(xc) * c.in, table);
+    float r32;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r32) : "f"(static_cast<float>(d)));
+    const double r0 = static_cast<double>(r32), r = fma(r0, fma(-d, r0, 1.0), r0);
+    double t = fma(-c.twice, r, c.out - static_cast<double>(top));
+    none = x == -INFINITY;
+    if (c.deep) {
+      none = none || t < -1000.0;
+      t = fmax(t, -1000.0);
+    }
+    w = exp2_64(t, table);
   }
-  // tanh(z) = 1 - 2 / (1 + e^2z); the reciprocal by one step of Newton's iteration from 22 bits
-  const float xc = fminf(fmaxf(x, -c.most), c.most);
-  const double d = 1.0 + exp2_64(static_cast<double>(xc) * c.in, table);
-  float r32;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r32) : "f"(static_cast<float>(d)));
-  const double r0 = static_cast<double>(r32), r = fma(r0, fma(-d, r0, 1.0), r0);
-  const double t = fma(-c.twice, r, c.out - static_cast<double>(top));
-  return x == -INFINITY || t < -160.0 ? 0.0 : exp2_64(t, table);
+  return __hiloint2double(none ? 0 : __double2hiint(w), none ? 0 : __double2loint(w));
 }
 __device__ __forceinline__ float level_32(float x, const VerifyScale& c) {
   if (!c.capped) return x * c.slope;
@@ -127,7 +138,7 @@ __device__ __forceinline__ float ex2_32(float x) {
 
 // One row's probabilities 2^(level - top) / sum.
 struct VerifyRow {
-  float top;
+  float top, least;  // the largest level; the logit 1000 below it
   double sum;
   bool fine;  // the row has a finite largest logit and no NaN
 };
@@ -138,9 +149,6 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
   __shared__ double wide_a[kVerifyWarps], wide_b[kVerifyWarps];
   __shared__ double shared_a[2][kVerifyCluster], shared_b[2][kVerifyCluster];  // every CTA's results, by turns
   __shared__ int parents[kVerifyNodes];
-  // Of the rejections at this node: 1 / Z (0: nothing was left, w stays), or without draft logits the
-  // weights that were taken.
-  __shared__ double zs[kVerifyNodes];
   __shared__ int64_t gone[kVerifyNodes];   // without draft logits: tokens whose weight is taken
   __shared__ int found;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -279,14 +287,8 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       if (s != 0.0) r.sum += s * ex2_32(static_cast<float>(shared_a[turn][k]) - r.top);
     }
     r.fine = r.sum > 0.0 && isfinite(r.sum) && isfinite(r.top);
+    r.least = fmaxf((r.top - 1000.f) / scale.slope, -3e38f);
     return r;
-  };
-
-  // What is left of a value after the first `k` rejections: p and q are its probabilities.
-  auto left_after = [&](double p, double q, int k) {
-    for (int i = 0; i < k; ++i)
-      if (zs[i] > 0.0) p = fmax(p - q, 0.0) * zs[i];
-    return p;
   };
 
   VerifyScale drafted = {};
@@ -301,6 +303,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
     target.in = 2.0 * 1.4426950408889634 / a.cap;
     target.out = a.cap * a.slope;
     target.twice = 2.0 * target.out;
+    target.deep = target.twice > 900.0;
   }
 
   int cur = 0, taken = 1;
@@ -330,15 +333,17 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       const E* xr = row_of(a.x, a.x_b, a.x_n, cur);
       const E* dr = a.d != nullptr ? row_of(a.d, a.d_b, a.d_n, cur) : nullptr;
       int c = child_after(cur);
-      VerifyRow p = stats(xr, target), q = {0.f, 1.0, true};
+      bool summed = false;  // the CTAs' parts of what is left stand in shared_a[turn]
+      VerifyRow p = stats(xr, target), q = {0.f, 0.f, 1.0, true};
       if (dr != nullptr && c < a.n) q = stats(dr, drafted);
       if (!p.fine) break;
-      int rejected = 0;
+      // After rejections w is max(p - c q, 0) / left: c = 0 and left = 1 at first, and of that less q what
+      // is positive is max(p - (c + left) q, 0).
+      double c_q = 0.0, left = 1.0;
+      int rejected = 0;  // without draft logits: their tokens' weights are taken, `left` stays
       bool sharp = false;  // the sums are in 64 bits
-      double last_z = 0.0;
-      // The weights of one value after all rejections so far.
-      auto p_of = [&](float x) { return weight_64(x, target, p.top, table) / p.sum; };
-      auto q_of = [&](float x) { return weight_64(x, drafted, q.top, table) / q.sum; };
+      auto p_of = [&](float x) { return weight_64(x, target, p.top, p.least, table) / p.sum; };
+      auto q_of = [&](float x) { return weight_64(x, drafted, q.top, q.least, table) / q.sum; };
       if (q.fine)
         for (; c < a.n; c = child_after(c)) {
           const int64_t t = tokens[c];
@@ -346,81 +351,72 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
           const double pt = p_of(logit_f32<E>(xr[t]));
           if (dr == nullptr) {
             bool was = false;
-            double rest = 1.0;
-            for (int i = 0; i < rejected; ++i) was |= gone[i] == t, rest -= zs[i];
-            if (uc < (was ? 0.0 : rest > 0.0 ? pt / rest : pt)) {
+            for (int i = 0; i < rejected; ++i) was |= gone[i] == t;
+            if (uc < (was ? 0.0 : left > 0.0 ? pt / left : pt)) {
               went = c;
               break;
             }
             __syncthreads();
             if (!was) {
-              if (tid == 0) gone[rejected] = t, zs[rejected] = pt;
+              if (tid == 0) gone[rejected] = t;
               ++rejected;
+              left -= pt;
             }
             __syncthreads();
             continue;
           }
           const double qt = q_of(logit_f32<E>(dr[t]));
-          if (uc * qt < left_after(pt, qt, rejected)) {
+          if (uc * qt < fmax(pt - c_q * qt, 0.0) / left) {
             went = c;
             break;
           }
-          // Rejected: the sum of what is left, in 64 bits.
+          // Rejected: what is left, in 64 bits.  With the sums of p and q by themselves over the values that
+          // stay positive, the first pass gives the sums over all besides: which values stay does not
+          // need them so exactly (where p and q are equal to 2^-23, what is left is 2^-23 of them).
           const bool wx = aligned16(xr), wd = aligned16(dr);
-          if (!sharp) {
-            double sp = 0.0, sq = 0.0;
-            for (int v = lo + tid * kVerifyVec; v < hi; v += kStep) {
-              float x[kVerifyVec], y[kVerifyVec];
-              load8<E>(xr, v, hi, wx, x);
-              load8<E>(dr, v, hi, wd, y);
-#pragma unroll
-              for (int i = 0; i < kVerifyVec; ++i) {
-                sp += weight_64(x[i], target, p.top, table);
-                sq += weight_64(y[i], drafted, q.top, table);
-              }
-            }
-            cluster_sums(sp, sq);
-            p.sum = sp, q.sum = sq;
-            sharp = true;
-          }
-          double z = 0.0, none = 0.0;
-          const double rp = 1.0 / p.sum, rq = 1.0 / q.sum;
+          const double to_c = c_q + (rejected == 0 ? 1.0 : left);
+          const double rp = 1.0 / p.sum, rq = to_c / q.sum;
+          double sp = 0.0, sq = 0.0, over_p = 0.0, over_q = 0.0;
           for (int v = lo + tid * kVerifyVec; v < hi; v += kStep) {
             float x[kVerifyVec], y[kVerifyVec];
             load8<E>(xr, v, hi, wx, x);
             load8<E>(dr, v, hi, wd, y);
 #pragma unroll
             for (int i = 0; i < kVerifyVec; ++i) {
-              const double pv = weight_64(x[i], target, p.top, table) * rp;
-              const double qv = weight_64(y[i], drafted, q.top, table) * rq;
-              z += fmax(left_after(pv, qv, rejected) - qv, 0.0);
+              const double pv = weight_64(x[i], target, p.top, p.least, table);
+              const double qv = weight_64(y[i], drafted, q.top, q.least, table);
+              const bool stays = fma(pv, rp, -(qv * rq)) > 0.0;
+              sp += pv, sq += qv;
+              over_p += stays ? pv : 0.0;
+              over_q += stays ? qv : 0.0;
             }
           }
-          cluster_sums(z, none);
-          last_z = z;
-          if (tid == 0) zs[rejected] = z > 0.0 ? 1.0 / z : 0.0;
+          if (!sharp) {
+            cluster_sums(sp, sq);
+            p.sum = sp, q.sum = sq;
+            sharp = true;
+          }
+          block_sums(over_p, over_q);
+          exchange(over_p / p.sum - to_c * over_q / q.sum, 0.0);
+          double z = 0.0;
+          for (int k = 0; k < ranks; ++k) z += fmax(shared_a[turn][k], 0.0);
           ++rejected;
-          __syncthreads();
+          if (z > 0.0) c_q = to_c, left = z;  // (nothing left: w stays)
+          summed = z > 0.0;
         }
       if (went < 0) {
         // ---- the next token: the weights' sum over the CTAs, then the place in one of them
         const bool wx = aligned16(xr), wd = dr != nullptr && aligned16(dr);
-        const double rp = 1.0 / p.sum, rq = 1.0 / q.sum;
-        const bool residual = dr != nullptr && rejected > 0;
-        // What is left after the last rejection has been summed already (not yet over its sum).
-        const bool summed = residual && last_z > 0.0;
+        const double rp = 1.0 / p.sum, rq = c_q / q.sum;
+        const bool residual = c_q > 0.0;
         auto weights = [&](int v, double (&f)[kVerifyVec]) {
           float x[kVerifyVec], y[kVerifyVec];
           load8<E>(xr, v, hi, wx, x);
           if (residual) load8<E>(dr, v, hi, wd, y);
 #pragma unroll
           for (int i = 0; i < kVerifyVec; ++i) {
-            f[i] = weight_64(x[i], target, p.top, table) * rp;
-            if (residual) {
-              const double qv = weight_64(y[i], drafted, q.top, table) * rq;
-              f[i] = left_after(f[i], qv, summed ? rejected - 1 : rejected);
-              if (summed) f[i] = fmax(f[i] - qv, 0.0);
-            }
+            f[i] = weight_64(x[i], target, p.top, p.least, table) * rp;
+            if (residual) f[i] = fmax(fma(-rq, weight_64(y[i], drafted, q.top, q.least, table), f[i]), 0.0);
           }
           if (dr == nullptr)
             for (int k = 0; k < rejected; ++k)
@@ -430,7 +426,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
                   if (gone[k] == v + i) f[i] = 0.0;
               }
         };
-        double total = last_z;
+        double total = left;
         while (!summed) {
           double part = 0.0, none = 0.0;
           for (int v = lo + tid * kVerifyVec; v < hi; v += kStep) {
@@ -451,7 +447,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
         int owner = -1, last = -1;
         double owner_before = 0.0, last_before = 0.0;
         for (int k = 0; k < ranks; ++k) {
-          const double s = shared_a[turn][k];
+          const double s = fmax(shared_a[turn][k], 0.0);
           if (s > 0.0) last = k, last_before = before;
           if (owner < 0 && before + s > aim) owner = k, owner_before = before;
           before += s;
@@ -517,7 +513,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
     if (rank == 0 && tid == 0) a.path[static_cast<int64_t>(b) * a.n + taken] = went;
     ++taken;
     cur = went;
-    __syncthreads();  // (zs and gone are free)
+    __syncthreads();  // (gone is free)
   }
   if (rank == 0) {
     for (int i = taken + tid; i < a.n; i += kVerifyThreads) a.path[static_cast<int64_t>(b) * a.n + i] = -1;
