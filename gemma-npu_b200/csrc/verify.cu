@@ -25,6 +25,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace w8 {
 
@@ -50,6 +51,7 @@ constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyCluster = 16;   // CTAs at most (8 where the GPU has no 16 free together)
 constexpr int kVerifyNodes = 1024;   // of a tree at most
 constexpr int kVerifyVec = 8;        // values of a thread at a time
+constexpr int kVerifyChunks = 1024;  // of a CTA's part of the vocabulary at most: a warp's turns of 256 values
 
 template <typename E>
 __device__ __forceinline__ float logit_f32(E v);
@@ -60,17 +62,27 @@ __device__ __forceinline__ float logit_f32<__nv_bfloat16>(__nv_bfloat16 v) { ret
 template <>
 __device__ __forceinline__ float logit_f32<__half>(__half v) { return __half2float(v); }
 
-// Values v .. v + 7 of a row, -inf behind `end`.
+// 8 neighbouring values of a row as they are: loads that nothing waits for until they are looked at.
 template <typename E>
-__device__ __forceinline__ void load8(const E* row, int v, int end, bool wide, float (&x)[kVerifyVec]) {
-  if (wide && v + kVerifyVec <= end) {
-    constexpr int kWords = sizeof(E) * kVerifyVec / 16;
-    uint4 w[kWords];
+struct Raw8 {
+  uint4 w[sizeof(E) * kVerifyVec / 16];
+  __device__ __forceinline__ void load(const E* row) {  // (16-byte aligned)
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint4*>(row + v)[i];
+    for (int i = 0; i < static_cast<int>(sizeof(E)) * kVerifyVec / 16; ++i) w[i] = reinterpret_cast<const uint4*>(row)[i];
+  }
+  __device__ __forceinline__ void get(float (&x)[kVerifyVec]) const {
     const E* e = reinterpret_cast<const E*>(w);
 #pragma unroll
     for (int i = 0; i < kVerifyVec; ++i) x[i] = logit_f32<E>(e[i]);
+  }
+};
+// Values v .. v + 7 of a row, -inf behind `end`.
+template <typename E>
+__device__ __forceinline__ void load8(const E* row, int v, int end, bool on16, float (&x)[kVerifyVec]) {
+  if (on16 && v + kVerifyVec <= end) {
+    Raw8<E> r;
+    r.load(row + v);
+    r.get(x);
   } else {
 #pragma unroll
     for (int i = 0; i < kVerifyVec; ++i) x[i] = v + i < end ? logit_f32<E>(row[v + i]) : -INFINITY;
@@ -92,20 +104,25 @@ __device__ __forceinline__ double exp2_64(double t, const double* table) {
 }
 // Weights of a row's logits: 2^(level - top), the level a logit in log2 units of its probability.
 struct VerifyScale {
-  bool capped;
   bool deep;                // a capped row's levels may differ by more than 900
   float most;               // 20 caps: tanh is 1 to 2^-57 from there on
   float slope, two_over_cap, cap_slope;  // for fp32
   double in, out, twice;    // log2(e) 2 / cap, cap slope (slope without a cap), 2 cap slope
 };
-// In 64 bits; `top` the row's largest level to fp32, `least` the logit whose level is 1000 below it:
-// less counts as 0.  Without branches: the values of a thread are to be under way together.
-__device__ __forceinline__ double weight_64(float x, const VerifyScale& c, float top, float least, const double* table) {
+// One row's probabilities: 2^(level - top) / sum.
+struct VerifyRow {
+  float top, least;  // the largest level; the logit 1000 below it, less than which counts as 0
+  double sum;
+  bool fine;  // the row has a finite largest logit and no NaN
+};
+// In 64 bits, without branches: the values of a thread are to be under way together.
+template <bool kCapped>
+__device__ __forceinline__ double weight_64(float x, const VerifyScale& c, const VerifyRow& row, const double* table) {
   double w;
   bool none;
-  if (!c.capped) {
-    none = x < least;
-    w = exp2_64(fma(static_cast<double>(fmaxf(x, least)), c.out, -static_cast<double>(top)), table);
+  if constexpr (!kCapped) {
+    none = x < row.least;
+    w = exp2_64(fma(static_cast<double>(fmaxf(x, row.least)), c.out, -static_cast<double>(row.top)), table);
   } else {
     // tanh(z) = 1 - 2 / (1 + e^2z); the reciprocal by one step of Newton's iteration from 22 bits
     const float xc = fminf(fmaxf(x, -c.most), c.most);
@@ -113,7 +130,7 @@ __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, float
     float r32;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r32) : "f"(static_cast<float>(d)));
     const double r0 = static_cast<double>(r32), r = fma(r0, fma(-d, r0, 1.0), r0);
-    double t = fma(-c.twice, r, c.out - static_cast<double>(top));
+    double t = fma(-c.twice, r, c.out - static_cast<double>(row.top));
     none = x == -INFINITY;
     if (c.deep) {
       none = none || t < -1000.0;
@@ -123,8 +140,9 @@ __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, float
   }
   return __hiloint2double(none ? 0 : __double2hiint(w), none ? 0 : __double2loint(w));
 }
+template <bool kCapped>
 __device__ __forceinline__ float level_32(float x, const VerifyScale& c) {
-  if (!c.capped) return x * c.slope;
+  if constexpr (!kCapped) return x * c.slope;
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * c.two_over_cap));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
@@ -136,167 +154,168 @@ __device__ __forceinline__ float ex2_32(float x) {
   return y;
 }
 
-// One row's probabilities 2^(level - top) / sum.
-struct VerifyRow {
-  float top, least;  // the largest level; the logit 1000 below it
-  double sum;
-  bool fine;  // the row has a finite largest logit and no NaN
+// What both kernels know of their sequence: a cluster of CTAs, each with a part of the vocabulary.
+struct VerifyPlace {
+  int b, rank, ranks, lo, hi;
 };
+__device__ __forceinline__ VerifyPlace verify_place(const VerifyArgs& a) {
+  VerifyPlace p;
+  uint32_t ranks;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
+  p.ranks = static_cast<int>(ranks), p.rank = static_cast<int>(cluster_ctarank());
+  p.b = blockIdx.x / p.ranks;
+  p.lo = min(p.rank * a.per, a.vocab), p.hi = min(p.lo + a.per, a.vocab);
+  return p;
+}
+__device__ __forceinline__ void st_cluster_f64(const double* at, int rank, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(at), rank)), "d"(v) : "memory");
+}
+// The tree as the walk needs it.  The node's next child behind `i`: parents come before children.
+struct VerifyTree {
+  int parents[kVerifyNodes], tokens[kVerifyNodes];  // token -1: out of range
+};
+__device__ __forceinline__ void verify_tree(const VerifyArgs& a, const VerifyPlace& p, VerifyTree& t) {
+  for (int i = threadIdx.x; i < a.n; i += kVerifyThreads) {
+    t.parents[i] = a.parent != nullptr ? a.parent[p.b * a.parent_b + i] : i - 1;
+    const int64_t token = a.tokens[static_cast<int64_t>(p.b) * a.n + i];
+    t.tokens[i] = token >= 0 && token < a.vocab ? static_cast<int>(token) : -1;
+  }
+}
+__device__ __forceinline__ int child_after(const VerifyArgs& a, const VerifyPlace& p, const VerifyTree& t, int node, int i) {
+  for (++i; i < a.n; ++i)
+    if (t.parents[i] == node) {
+      if (t.tokens[i] >= 0) break;
+      if (p.rank == 0 && threadIdx.x == 0) atomicExch(&g_verify_status, W8_ERR_INVALID_ARG);  // skipped
+    }
+  return i;
+}
+
+constexpr int kVerifyStep = kVerifyThreads * kVerifyVec;
 
 template <typename E>
-__global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const VerifyArgs a) {
-  __shared__ double table[32];
-  __shared__ double wide_a[kVerifyWarps], wide_b[kVerifyWarps];
-  __shared__ double shared_a[2][kVerifyCluster], shared_b[2][kVerifyCluster];  // every CTA's results, by turns
-  __shared__ int parents[kVerifyNodes];
-  __shared__ int64_t gone[kVerifyNodes];   // without draft logits: tokens whose weight is taken
-  __shared__ int found;
+__device__ __forceinline__ const E* verify_row(const void* p, int64_t sb, int64_t sn, int b, int i) {
+  return static_cast<const E*>(p) + b * sb + i * sn;
+}
+template <typename E>
+__device__ __forceinline__ bool verify_on16(const E* row) {
+  return (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+}
+
+// ---------------------------------------------------------------- greedy
+// The largest logit of a node, the lowest of equal ones, is the token after it; the child with that
+// token stands.
+template <typename E>
+__global__ void __launch_bounds__(kVerifyThreads) draft_verify_greedy_kernel(const VerifyArgs a) {
+  __shared__ VerifyTree tree;
+  __shared__ unsigned long long keys[kVerifyWarps];
+  __shared__ unsigned long long all[2][kVerifyCluster];  // every CTA's largest, by turns
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint32_t ranks_u;
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks_u));
-  const int ranks = static_cast<int>(ranks_u), rank = static_cast<int>(cluster_ctarank());
-  const int b = blockIdx.x / ranks;
-  const int lo = min(rank * a.per, a.vocab), hi = min(lo + a.per, a.vocab);
-  if (tid < 32) table[tid] = exp2(tid / 32.0);
+  const VerifyPlace p = verify_place(a);
   pdl_launch_dependents();
   pdl_wait();
-  for (int i = tid; i < a.n; i += kVerifyThreads) parents[i] = a.parent != nullptr ? a.parent[b * a.parent_b + i] : i - 1;
-  const int64_t* tokens = a.tokens + static_cast<int64_t>(b) * a.n;
-  const float* u = a.u != nullptr ? a.u + static_cast<int64_t>(b) * a.n : nullptr;
+  verify_tree(a, p, tree);
   cluster_sync();
-
-  int turn = 0;
-  // Every CTA's (va, vb) to every CTA, which then reads them at shared_a / shared_b[turn].
-  auto exchange = [&](double va, double vb) {  // (of thread 0 .. ranks - 1)
-    turn ^= 1;
-    if (tid < ranks) {
-      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&shared_a[turn][rank]), tid)), "d"(va)
-                   : "memory");
-      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&shared_b[turn][rank]), tid)), "d"(vb)
-                   : "memory");
-    }
-    cluster_sync();
-  };
-  // Sums over the CTA, in every thread.
-  auto block_sums = [&](double& va, double& vb) {
-#pragma unroll
-    for (int s = 16; s; s >>= 1) {
-      va += __shfl_xor_sync(0xffffffffu, va, s);
-      vb += __shfl_xor_sync(0xffffffffu, vb, s);
-    }
-    __syncthreads();
-    if (lane == 0) wide_a[warp] = va, wide_b[warp] = vb;
-    __syncthreads();
-    va = vb = 0.0;
-#pragma unroll
-    for (int w = 0; w < kVerifyWarps; ++w) va += wide_a[w], vb += wide_b[w];
-  };
-  auto cluster_sums = [&](double& va, double& vb) {
-    block_sums(va, vb);
-    exchange(va, vb);
-    va = vb = 0.0;
-    for (int k = 0; k < ranks; ++k) va += shared_a[turn][k], vb += shared_b[turn][k];
-  };
-  constexpr int kStep = kVerifyThreads * kVerifyVec;
-  auto row_of = [&](const void* p, int64_t sb, int64_t sn, int i) { return static_cast<const E*>(p) + b * sb + i * sn; };
-  auto aligned16 = [&](const E* row) { return (reinterpret_cast<uintptr_t>(row) & 15) == 0; };
-
-  // ---- greedy: the largest logit, the lowest of equal ones (-1: none is finite, or a NaN)
-  auto best_of = [&](int node) -> int64_t {
-    const E* row = row_of(a.x, a.x_b, a.x_n, node);
-    const bool wide = aligned16(row);
+  int cur = 0, taken = 1, turn = 0;
+  int64_t next;
+  while (true) {
+    const E* row = verify_row<E>(a.x, a.x_b, a.x_n, p.b, cur);
+    const bool on16 = verify_on16(row);
     float top = -INFINITY;
     int at = 0x7FFFFFFF;
     bool bad = false;
-#pragma unroll 2
-    for (int v = lo + tid * kVerifyVec; v < hi; v += kStep) {
-      float x[kVerifyVec];
-      load8<E>(row, v, hi, wide, x);
+    auto take = [&](const float (&x)[kVerifyVec], int v) {
 #pragma unroll
       for (int i = 0; i < kVerifyVec; ++i) {
         bad |= !(x[i] < INFINITY);
         if (x[i] > top) top = x[i], at = v + i;
       }
-    }
-    bad = __syncthreads_or(bad);
-    // (the order-preserving bits of the value, then the lower index)
-    auto key_of = [&](float x, int i) {
-      const uint32_t s = __float_as_uint(x == 0.f ? 0.f : x);
-      return static_cast<unsigned long long>(s & 0x80000000u ? ~s : s | 0x80000000u) << 32 |
-             (0xFFFFFFFFu - static_cast<uint32_t>(i));
     };
-    unsigned long long key = at == 0x7FFFFFFF ? 0ull : key_of(top, at);
+    constexpr int kBatch = 4;  // loads of a thread under way
+    int v = p.lo + tid * kVerifyVec;
+    if (on16)
+      for (; v + (kBatch - 1) * kVerifyStep + kVerifyVec <= p.hi; v += kBatch * kVerifyStep) {
+        Raw8<E> r[kBatch];
 #pragma unroll
-    for (int s = 16; s; s >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, s);
-      key = other > key ? other : key;
+        for (int k = 0; k < kBatch; ++k) r[k].load(row + v + k * kVerifyStep);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          float x[kVerifyVec];
+          r[k].get(x);
+          take(x, v + k * kVerifyStep);
+        }
+      }
+#pragma unroll 1
+    for (; v < p.hi; v += kVerifyStep) {
+      float x[kVerifyVec];
+      load8<E>(row, v, p.hi, on16, x);
+      take(x, v);
     }
-    unsigned long long* keys = reinterpret_cast<unsigned long long*>(wide_a);
+    // The order-preserving bits of the value, then the lower index; a NaN or an infinity above all.
+    const uint32_t s = __float_as_uint(top == 0.f ? 0.f : top);
+    unsigned long long key = at == 0x7FFFFFFF ? 0ull
+                                              : static_cast<unsigned long long>(s & 0x80000000u ? ~s : s | 0x80000000u) << 32 |
+                                                    (0xFFFFFFFFu - static_cast<uint32_t>(at));
+    if (bad) key = ~0ull;
+    auto largest = [&](unsigned long long k) {
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, d);
+        k = other > k ? other : k;
+      }
+      return k;
+    };
+    key = largest(key);
     if (lane == 0) keys[warp] = key;
     __syncthreads();
-    for (int w = 0; w < kVerifyWarps; ++w) key = keys[w] > key ? keys[w] : key;
-    exchange(__longlong_as_double(static_cast<long long>(key)), bad ? 1.0 : 0.0);
-    for (int k = 0; k < ranks; ++k) {
-      const unsigned long long other = static_cast<unsigned long long>(__double_as_longlong(shared_a[turn][k]));
-      key = other > key ? other : key;
-      bad |= shared_b[turn][k] != 0.0;
+    turn ^= 1;
+    if (warp == 0) {
+      key = largest(lane < kVerifyWarps ? keys[lane] : 0ull);
+      if (lane < p.ranks)
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&all[turn][p.rank]), lane)), "l"(key)
+                     : "memory");
     }
-    return bad || key == 0ull ? -1 : static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
-  };
+    cluster_sync();
+    key = largest(lane < p.ranks ? all[turn][lane] : 0ull);
+    next = key == 0ull || key == ~0ull ? -1 : static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
+    int went = -1;
+    if (next >= 0)
+      for (int c = child_after(a, p, tree, cur, cur); c < a.n; c = child_after(a, p, tree, cur, c))
+        if (tree.tokens[c] == next) {
+          went = c;
+          break;
+        }
+    if (went < 0) break;
+    if (p.rank == 0 && tid == 0) a.path[static_cast<int64_t>(p.b) * a.n + taken] = went;
+    ++taken;
+    cur = went;
+  }
+  if (p.rank == 0) {
+    int* path = a.path + static_cast<int64_t>(p.b) * a.n;
+    for (int i = taken + tid; i < a.n; i += kVerifyThreads) path[i] = -1;
+    if (tid == 0) path[0] = 0, a.taken[p.b] = taken, a.token[p.b] = next;
+  }
+}
 
-  // ---- sampling: a row's maximum and sum in fp32 ...
-  auto stats = [&](const E* row, const VerifyScale& scale) {
-    const bool wide = aligned16(row);
-    float top = -INFINITY, sum = 0.f;  // in log2 units
-    bool bad = false;
-#pragma unroll 2
-    for (int v = lo + tid * kVerifyVec; v < hi; v += kStep) {
-      float x[kVerifyVec];
-      load8<E>(row, v, hi, wide, x);
-      float most = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kVerifyVec; ++i) {
-        bad |= !(x[i] < INFINITY);
-        x[i] = level_32(x[i], scale);
-        most = fmaxf(most, x[i]);
-      }
-      if (most > top) sum *= ex2_32(top - most), top = most;
-      const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int i = 0; i < kVerifyVec; ++i) sum += ex2_32(x[i] - ref);
-    }
-    // The CTA's, then the cluster's.
-    float high = top;
-#pragma unroll
-    for (int s = 16; s; s >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, s));
-    __syncthreads();
-    if (lane == 0) wide_a[warp] = high;
-    bad = __syncthreads_or(bad);
-    float mine = static_cast<float>(wide_a[0]);
-#pragma unroll
-    for (int w = 1; w < kVerifyWarps; ++w) mine = fmaxf(mine, static_cast<float>(wide_a[w]));
-    double part = top == -INFINITY ? 0.0 : static_cast<double>(sum) * ex2_32(top - mine), none = 0.0;
-    block_sums(part, none);
-    exchange(mine, bad ? __longlong_as_double(0x7FF8000000000000ll) : part);
-    VerifyRow r;
-    r.top = static_cast<float>(shared_a[turn][0]);
-    for (int k = 1; k < ranks; ++k) r.top = fmaxf(r.top, static_cast<float>(shared_a[turn][k]));
-    r.sum = 0.0;
-    for (int k = 0; k < ranks; ++k) {
-      const double s = shared_b[turn][k];  // (NaN: the row is not fine)
-      if (s != 0.0) r.sum += s * ex2_32(static_cast<float>(shared_a[turn][k]) - r.top);
-    }
-    r.fine = r.sum > 0.0 && isfinite(r.sum) && isfinite(r.top);
-    r.least = fmaxf((r.top - 1000.f) / scale.slope, -3e38f);
-    return r;
-  };
-
+// ---------------------------------------------------------------- sampling
+template <typename E, bool kCapped, bool kDraft>
+__global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const VerifyArgs a) {
+  __shared__ VerifyTree tree;
+  __shared__ double table[32];
+  __shared__ float2 tops[2][kVerifyWarps];               // (largest level, sum) of a warp's part of p and q
+  __shared__ float2 all_tops[2][2][kVerifyCluster];      // of a CTA's, by turns
+  __shared__ double wide[4][kVerifyWarps];               // a warp's sums
+  __shared__ double shared[2][4][kVerifyCluster];        // a CTA's, by turns
+  __shared__ double chunk_p[kVerifyChunks], chunk_q[kDraft ? kVerifyChunks : 1];  // of a warp's parts of the last pass
+  __shared__ int gone[kDraft ? 1 : kVerifyNodes];        // without draft logits: tokens whose weight is taken
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const VerifyPlace at = verify_place(a);
+  const int b = at.b, rank = at.rank, ranks = at.ranks, lo = at.lo, hi = at.hi;
+  if (tid < 32) table[tid] = exp2(tid / 32.0);
   VerifyScale drafted = {};
   drafted.slope = static_cast<float>(a.slope);
   drafted.out = a.slope;
   VerifyScale target = drafted;
-  if (a.cap > 0.0) {
-    target.capped = true;
+  if constexpr (kCapped) {
     target.most = static_cast<float>(20.0 * a.cap);
     target.two_over_cap = static_cast<float>(2.0 * 1.4426950408889634 / a.cap);
     target.cap_slope = static_cast<float>(a.cap * a.slope);
@@ -305,67 +324,262 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
     target.twice = 2.0 * target.out;
     target.deep = target.twice > 900.0;
   }
+  // Chunks of `turns` times 256 values, a warp each.
+  const int turns = max(1, (a.per + 256 * kVerifyChunks - 1) / (256 * kVerifyChunks));
+  const int chunks = hi > lo ? (hi - lo + 256 * turns - 1) / (256 * turns) : 0;
+  pdl_launch_dependents();
+  pdl_wait();
+  verify_tree(a, at, tree);
+  const float* u = a.u + static_cast<int64_t>(b) * a.n;
+  const double u0 = static_cast<double>(u[0]);
+  cluster_sync();
+
+  // Sums over a warp's first lanes, in every lane (the same order in every warp and CTA).
+  auto warp_sum = [&](double v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+  };
+  auto warp_max = [&](float v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    return v;
+  };
+  int turn = 0, top_turn = 0;
+  // The CTA's sums, then every CTA's to every CTA, at shared[turn].
+  auto exchange_sums = [&](double (&v)[4]) {
+    constexpr int n = kDraft ? 4 : 3;  // (without q the last is 0)
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = warp_sum(v[i]);
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) wide[i][warp] = v[i];
+    }
+    __syncthreads();
+    turn ^= 1;
+    if (warp < n) {
+      const double s = warp_sum(lane < kVerifyWarps ? wide[warp][lane] : 0.0);
+      if (lane < ranks) st_cluster_f64(&shared[turn][warp][rank], lane, s);
+    }
+    cluster_sync();
+  };
+  auto shared_sum = [&](int i) { return warp_sum(lane < ranks ? shared[turn][i][lane] : 0.0); };
+
+  // The largest levels and the sums of a target row and (if asked for) a draft row in fp32.
+  auto stats = [&](const E* xr, const E* dr, bool two, VerifyRow& p, VerifyRow& q) {
+    const bool wx = verify_on16(xr), wd = verify_on16(dr);
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // in log2 units
+    bool bad[2] = {false, false};
+    auto add = [&](const float (&y)[kVerifyVec], int r) {
+      float most = y[0];
+#pragma unroll
+      for (int i = 1; i < kVerifyVec; ++i) most = fmaxf(most, y[i]);
+      // (without a branch: the sum is rescaled by 1 where the maximum stays)
+      const float to = fmaxf(top[r], most), ref = to == -INFINITY ? 0.f : to;
+      float s = sum[r] * ex2_32(top[r] - ref);
+#pragma unroll
+      for (int i = 0; i < kVerifyVec; ++i) s += ex2_32(y[i] - ref);
+      sum[r] = s;
+      top[r] = to;
+    };
+    auto take = [&](const float (&x)[kVerifyVec], int r) {
+      float y[kVerifyVec];
+#pragma unroll
+      for (int i = 0; i < kVerifyVec; ++i) {
+        bad[r] |= !(x[i] < INFINITY);
+        y[i] = r == 0 ? level_32<kCapped>(x[i], target) : level_32<false>(x[i], drafted);
+      }
+      add(y, r);
+    };
+    constexpr int kBatch = 2;  // loads of a thread and row under way
+    int v = lo + tid * kVerifyVec;
+    if (wx && (!kDraft || !two || wd))
+      for (; v + (kBatch - 1) * kVerifyStep + kVerifyVec <= hi; v += kBatch * kVerifyStep) {
+        Raw8<E> rx[kBatch], ry[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) rx[k].load(xr + v + k * kVerifyStep);
+        if (kDraft && two) {
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) ry[k].load(dr + v + k * kVerifyStep);
+        }
+        float x[kVerifyVec];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          rx[k].get(x);
+          take(x, 0);
+        }
+        if (kDraft && two) {
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            ry[k].get(x);
+            take(x, 1);
+          }
+        }
+      }
+#pragma unroll 1
+    for (; v < hi; v += kVerifyStep) {
+      float x[kVerifyVec];
+      load8<E>(xr, v, hi, wx, x);
+      take(x, 0);
+      if (kDraft && two) {
+        load8<E>(dr, v, hi, wd, x);
+        take(x, 1);
+      }
+    }
+    // A warp's, the CTA's, then the cluster's: sums relative to the largest level so far.
+    auto join = [&](float2 t) {
+      const float to = warp_max(t.x);
+      float s = t.x == -INFINITY ? t.y : t.y * ex2_32(t.x - to);  // (a NaN stays)
+#pragma unroll
+      for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+      return make_float2(to, s);
+    };
+    constexpr int kRows = kDraft ? 2 : 1;
+    float2 t[2];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      t[r] = join(make_float2(top[r], bad[r] ? __uint_as_float(0x7FC00000u) : sum[r]));
+      if (lane == 0) tops[r][warp] = t[r];
+    }
+    __syncthreads();
+    top_turn ^= 1;
+    if (warp < kRows) {
+      const float2 c = join(lane < kVerifyWarps ? tops[warp][lane] : make_float2(-INFINITY, 0.f));
+      if (lane < ranks)
+        st_cluster_f64(reinterpret_cast<const double*>(&all_tops[top_turn][warp][rank]), lane,
+                       __hiloint2double(__float_as_int(c.y), __float_as_int(c.x)));
+    }
+    cluster_sync();
+    auto row = [&](int r, const VerifyScale& scale) {
+      const float2 c = join(lane < ranks ? all_tops[top_turn][r][lane] : make_float2(-INFINITY, 0.f));
+      VerifyRow out;
+      out.top = c.x;
+      out.sum = static_cast<double>(c.y);
+      out.fine = c.y > 0.f && c.y < INFINITY && c.x > -INFINITY && c.x < INFINITY;
+      out.least = fmaxf((out.top - 1000.f) / scale.slope, -3e38f);
+      return out;
+    };
+    p = row(0, target);
+    if (kDraft && two) q = row(1, drafted);
+  };
 
   int cur = 0, taken = 1;
   int64_t next = -1;
-  if (rank == 0 && tid == 0) a.path[static_cast<int64_t>(b) * a.n] = 0;
+  bool written = false;
   while (true) {
-    // The node's next child behind `i`: parents come before children.
-    auto child_after = [&](int i) {
-      for (++i; i < a.n; ++i)
-        if (parents[i] == cur) {
-          const int64_t t = tokens[i];
-          if (t >= 0 && t < a.vocab) break;
-          if (rank == 0 && tid == 0) atomicExch(&g_verify_status, W8_ERR_INVALID_ARG);  // skipped
-        }
-      return i;
-    };
     int went = -1;
-    if (a.greedy) {
-      next = best_of(cur);
-      if (next >= 0)
-        for (int c = child_after(cur); c < a.n; c = child_after(c))
-          if (tokens[c] == next) {
+    const E* xr = verify_row<E>(a.x, a.x_b, a.x_n, b, cur);
+    const E* dr = kDraft ? verify_row<E>(a.d, a.d_b, a.d_n, b, cur) : xr;
+    int c = child_after(a, at, tree, cur, cur);
+    // What decides the first child comes with the row.
+    const int c0 = c;
+    float x0 = 0.f, d0 = 0.f, u_c0 = 0.f;
+    if (c0 < a.n) {
+      x0 = logit_f32<E>(xr[tree.tokens[c0]]);
+      if (kDraft) d0 = logit_f32<E>(dr[tree.tokens[c0]]);
+      u_c0 = u[c0];
+    }
+    VerifyRow p, q = {0.f, 0.f, 1.0, true};
+    stats(xr, dr, c < a.n, p, q);
+    if (!p.fine) break;
+    // After rejections w is max(p - c q, 0) / left: c = 0 and left = 1 at first, and of that less q what
+    // is positive is max(p - (c + left) q, 0).
+    double c_q = 0.0, left = 1.0;
+    int rejected = 0;     // without draft logits: their tokens' weights are taken, `left` stays
+    bool sharp = false;   // the sums are in 64 bits
+    bool summed = false;  // shared[turn][2, 3] and the chunks have the last pass's parts of p and q
+    const bool wx = verify_on16(xr), wd = kDraft && verify_on16(dr);
+    auto p_of = [&](float x) { return weight_64<kCapped>(x, target, p, table); };
+    auto q_of = [&](float x) { return weight_64<false>(x, drafted, q, table); };
+    auto taken_away = [&](int v) {  // (without draft logits)
+      bool was = false;
+      for (int i = 0; i < rejected; ++i) was |= gone[i] == v;
+      return was;
+    };
+    // A pass in 64 bits over the CTA's part, a chunk of a warp at a time: sums of p and q, and of those
+    // with p > rq / rp q (two) or not taken away, which are also the chunk's.
+    auto pass = [&](auto both, double (&sums)[4], double rp, double rq) {
+      constexpr bool two = decltype(both)::value;
+      // (the next turn's values are under way while this one's weights are computed)
+      Raw8<E> rx, ry;
+      auto fetch = [&](int v) {
+        if (wx && v + kVerifyVec <= hi) rx.load(xr + v);
+        if (two && wd && v + kVerifyVec <= hi) ry.load(dr + v);
+      };
+      auto first_of = [&](int k) { return lo + k * turns * 256 + lane * kVerifyVec; };
+      if (warp < chunks) fetch(first_of(warp));
+#pragma unroll 1
+      for (int k = warp; k < chunks; k += kVerifyWarps) {
+        double part[2] = {0.0, 0.0};
+#pragma unroll 1
+        for (int j = 0; j < turns; ++j) {
+          const int v = first_of(k) + j * 256;
+          float x[kVerifyVec], y[kVerifyVec];
+          if (wx && v + kVerifyVec <= hi)
+            rx.get(x);
+          else
+            load8<E>(xr, v, hi, false, x);
+          if constexpr (two) {
+            if (wd && v + kVerifyVec <= hi)
+              ry.get(y);
+            else
+              load8<E>(dr, v, hi, false, y);
+          }
+          fetch(j + 1 < turns ? v + 256 : first_of(k + kVerifyWarps));
+          double pv[kVerifyVec], qv[kVerifyVec];
+#pragma unroll
+          for (int i = 0; i < kVerifyVec; ++i) {
+            pv[i] = p_of(x[i]);
+            if constexpr (two) qv[i] = q_of(y[i]);
+          }
+          if constexpr (two) {
+#pragma unroll
+            for (int i = 0; i < kVerifyVec; ++i) {
+              sums[0] += pv[i], sums[1] += qv[i];
+              // (a weight that does not stay becomes 0 in its bits)
+              const bool stays = __double2hiint(fma(-rq, qv[i], pv[i] * rp)) >= 0;
+              part[0] += __hiloint2double(stays ? __double2hiint(pv[i]) : 0, stays ? __double2loint(pv[i]) : 0);
+              part[1] += __hiloint2double(stays ? __double2hiint(qv[i]) : 0, stays ? __double2loint(qv[i]) : 0);
+            }
+          } else {
+            if (!kDraft && rejected > 0) {
+#pragma unroll
+              for (int i = 0; i < kVerifyVec; ++i)
+                if (taken_away(v + i)) pv[i] = 0.0;
+            }
+#pragma unroll
+            for (int i = 0; i < kVerifyVec; ++i) part[0] += pv[i];
+          }
+        }
+        sums[2] += part[0], sums[3] += part[1];
+        part[0] = warp_sum(part[0]);
+        if constexpr (two) part[1] = warp_sum(part[1]);
+        if (lane == 0) {
+          chunk_p[k] = part[0];
+          if constexpr (kDraft) chunk_q[k] = part[1];
+        }
+      }
+    };
+    if (q.fine)
+      for (; c < a.n; c = child_after(a, at, tree, cur, c)) {
+        const int t = tree.tokens[c];
+        const double uc = static_cast<double>(c == c0 ? u_c0 : u[c]);
+        const double pt = p_of(c == c0 ? x0 : logit_f32<E>(xr[t])) / p.sum;
+        if constexpr (!kDraft) {
+          const bool was = taken_away(t);
+          if (uc < (was ? 0.0 : left > 0.0 ? pt / left : pt)) {
             went = c;
             break;
           }
-    } else {
-      const E* xr = row_of(a.x, a.x_b, a.x_n, cur);
-      const E* dr = a.d != nullptr ? row_of(a.d, a.d_b, a.d_n, cur) : nullptr;
-      int c = child_after(cur);
-      bool summed = false;  // the CTAs' parts of what is left stand in shared_a[turn]
-      VerifyRow p = stats(xr, target), q = {0.f, 0.f, 1.0, true};
-      if (dr != nullptr && c < a.n) q = stats(dr, drafted);
-      if (!p.fine) break;
-      // After rejections w is max(p - c q, 0) / left: c = 0 and left = 1 at first, and of that less q what
-      // is positive is max(p - (c + left) q, 0).
-      double c_q = 0.0, left = 1.0;
-      int rejected = 0;  // without draft logits: their tokens' weights are taken, `left` stays
-      bool sharp = false;  // the sums are in 64 bits
-      auto p_of = [&](float x) { return weight_64(x, target, p.top, p.least, table) / p.sum; };
-      auto q_of = [&](float x) { return weight_64(x, drafted, q.top, q.least, table) / q.sum; };
-      if (q.fine)
-        for (; c < a.n; c = child_after(c)) {
-          const int64_t t = tokens[c];
-          const double uc = static_cast<double>(u[c]);
-          const double pt = p_of(logit_f32<E>(xr[t]));
-          if (dr == nullptr) {
-            bool was = false;
-            for (int i = 0; i < rejected; ++i) was |= gone[i] == t;
-            if (uc < (was ? 0.0 : left > 0.0 ? pt / left : pt)) {
-              went = c;
-              break;
-            }
-            __syncthreads();
-            if (!was) {
-              if (tid == 0) gone[rejected] = t;
-              ++rejected;
-              left -= pt;
-            }
-            __syncthreads();
-            continue;
+          __syncthreads();
+          if (!was) {
+            if (tid == 0) gone[rejected] = t;
+            ++rejected;
+            left -= pt;
           }
-          const double qt = q_of(logit_f32<E>(dr[t]));
+          __syncthreads();
+        } else {
+          const double qt = q_of(c == c0 ? d0 : logit_f32<E>(dr[t])) / q.sum;
           if (uc * qt < fmax(pt - c_q * qt, 0.0) / left) {
             went = c;
             break;
@@ -373,102 +587,89 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
           // Rejected: what is left, in 64 bits.  With the sums of p and q by themselves over the values that
           // stay positive, the first pass gives the sums over all besides: which values stay does not
           // need them so exactly (where p and q are equal to 2^-23, what is left is 2^-23 of them).
-          const bool wx = aligned16(xr), wd = aligned16(dr);
           const double to_c = c_q + (rejected == 0 ? 1.0 : left);
-          const double rp = 1.0 / p.sum, rq = to_c / q.sum;
-          double sp = 0.0, sq = 0.0, over_p = 0.0, over_q = 0.0;
-          for (int v = lo + tid * kVerifyVec; v < hi; v += kStep) {
+          double sums[4] = {0.0, 0.0, 0.0, 0.0};
+          pass(std::true_type(), sums, 1.0 / p.sum, to_c / q.sum);
+          exchange_sums(sums);
+          if (!sharp) p.sum = shared_sum(0), q.sum = shared_sum(1);
+          sharp = true;
+          const double z = shared_sum(2) / p.sum - to_c * (shared_sum(3) / q.sum);
+          // (Nothing but rounding is left where p and q are equal: w stays.)
+          summed = z > 1e-13;
+          if (summed) c_q = to_c, left = z;
+          ++rejected;
+        }
+      }
+    if (went < 0) {
+      // ---- the next token: the weights' sums over the CTAs, then over one CTA's chunks, then a chunk
+      while (!summed) {
+        // (after a residual of nothing but rounding the one before it is summed again)
+        double sums[4] = {0.0, 0.0, 0.0, 0.0};
+        if (kDraft && c_q > 0.0)
+          pass(std::bool_constant<kDraft>(), sums, 1.0 / p.sum, c_q / q.sum);
+        else
+          pass(std::false_type(), sums, 0.0, 0.0);
+        exchange_sums(sums);
+        if (kDraft || rejected == 0 || shared_sum(2) > 0.0) break;
+        rejected = 0;  // the weights taken were all there were: the target's own
+      }
+      const double rp = 1.0 / p.sum, rq = kDraft ? c_q / q.sum : 0.0;
+      auto part_of = [&](int k) { return kDraft ? fma(-rq, shared[turn][3][k], shared[turn][2][k] * rp) : shared[turn][2][k] * rp; };
+      const double aim = u0 * warp_sum(lane < ranks ? fmax(part_of(lane), 0.0) : 0.0);
+      // The first of `n` parts whose running sum passes the aim, or the last with any weight (-1: none).
+      auto place = [&](int n, auto part, double& before) {
+        int last = -1;
+        double run = before, last_run = before;
+        for (int k = 0; k < n; ++k) {
+          const double s = part(k);
+          if (s > 0.0) {
+            last = k, last_run = run;
+            if (run + s > aim) break;
+            run += s;
+          }
+        }
+        before = last_run;
+        return last;
+      };
+      if (warp == 0) {
+        double before = 0.0;
+        const int owner = place(ranks, part_of, before);
+        if (owner == rank) {
+          // (the chunks' sums are there: the cluster has met since)  A lane's run of chunks, then the lane.
+          const int run = (chunks + 31) / 32, k0 = min(lane * run, chunks), k1 = min(k0 + run, chunks);
+          auto of = [&](int k) { return fmax(kDraft ? fma(-rq, chunk_q[kDraft ? k : 0], chunk_p[k] * rp) : chunk_p[k] * rp, 0.0); };
+          double mine = 0.0;
+          for (int k = k0; k < k1; ++k) mine += of(k);
+          double incl = mine;
+#pragma unroll
+          for (int s = 1; s < 32; s <<= 1) {
+            const double o = __shfl_up_sync(0xffffffffu, incl, s);
+            if (lane >= s) incl += o;
+          }
+          const uint32_t some = __ballot_sync(0xffffffffu, mine > 0.0);
+          uint32_t over = __ballot_sync(0xffffffffu, mine > 0.0 && before + incl > aim);
+          const int l = over ? __ffs(over) - 1 : max(31 - __clz(some), 0);
+          double sum_at = before + incl - mine;
+          int k = place(k1 - k0, [&](int i) { return of(k0 + i); }, sum_at) + k0;
+          k = max(__shfl_sync(0xffffffffu, k, l), 0);  // (a CTA with weight has such a chunk, but for rounding)
+          sum_at = __shfl_sync(0xffffffffu, sum_at, l);
+          // The chunk's values, 256 at a time.
+          int last = -1, token = -1;
+#pragma unroll 1
+          for (int j = 0; j < turns && token < 0; ++j) {
+            const int v = lo + (k * turns + j) * 256 + lane * kVerifyVec;
             float x[kVerifyVec], y[kVerifyVec];
+            double f[kVerifyVec], sum = 0.0;
             load8<E>(xr, v, hi, wx, x);
-            load8<E>(dr, v, hi, wd, y);
+            if (kDraft && c_q > 0.0) load8<E>(dr, v, hi, wd, y);
+            int end = -1;
 #pragma unroll
             for (int i = 0; i < kVerifyVec; ++i) {
-              const double pv = weight_64(x[i], target, p.top, p.least, table);
-              const double qv = weight_64(y[i], drafted, q.top, q.least, table);
-              const bool stays = fma(pv, rp, -(qv * rq)) > 0.0;
-              sp += pv, sq += qv;
-              over_p += stays ? pv : 0.0;
-              over_q += stays ? qv : 0.0;
-            }
-          }
-          if (!sharp) {
-            cluster_sums(sp, sq);
-            p.sum = sp, q.sum = sq;
-            sharp = true;
-          }
-          block_sums(over_p, over_q);
-          exchange(over_p / p.sum - to_c * over_q / q.sum, 0.0);
-          double z = 0.0;
-          for (int k = 0; k < ranks; ++k) z += fmax(shared_a[turn][k], 0.0);
-          ++rejected;
-          if (z > 0.0) c_q = to_c, left = z;  // (nothing left: w stays)
-          summed = z > 0.0;
-        }
-      if (went < 0) {
-        // ---- the next token: the weights' sum over the CTAs, then the place in one of them
-        const bool wx = aligned16(xr), wd = dr != nullptr && aligned16(dr);
-        const double rp = 1.0 / p.sum, rq = c_q / q.sum;
-        const bool residual = c_q > 0.0;
-        auto weights = [&](int v, double (&f)[kVerifyVec]) {
-          float x[kVerifyVec], y[kVerifyVec];
-          load8<E>(xr, v, hi, wx, x);
-          if (residual) load8<E>(dr, v, hi, wd, y);
-#pragma unroll
-          for (int i = 0; i < kVerifyVec; ++i) {
-            f[i] = weight_64(x[i], target, p.top, p.least, table) * rp;
-            if (residual) f[i] = fmax(fma(-rq, weight_64(y[i], drafted, q.top, q.least, table), f[i]), 0.0);
-          }
-          if (dr == nullptr)
-            for (int k = 0; k < rejected; ++k)
-              if (gone[k] >= v && gone[k] < v + kVerifyVec) {
-#pragma unroll
-                for (int i = 0; i < kVerifyVec; ++i)
-                  if (gone[k] == v + i) f[i] = 0.0;
-              }
-        };
-        double total = left;
-        while (!summed) {
-          double part = 0.0, none = 0.0;
-          for (int v = lo + tid * kVerifyVec; v < hi; v += kStep) {
-            double f[kVerifyVec];
-            weights(v, f);
-#pragma unroll
-            for (int i = 0; i < kVerifyVec; ++i) part += f[i];
-          }
-          block_sums(part, none);
-          exchange(part, 0.0);
-          total = 0.0;
-          for (int k = 0; k < ranks; ++k) total += shared_a[turn][k];
-          if (total > 0.0 || rejected == 0) break;
-          rejected = 0;  // the weights taken were all there were: the target's own
-        }
-        const double aim = static_cast<double>(u[0]) * total;
-        double before = 0.0;
-        int owner = -1, last = -1;
-        double owner_before = 0.0, last_before = 0.0;
-        for (int k = 0; k < ranks; ++k) {
-          const double s = fmax(shared_a[turn][k], 0.0);
-          if (s > 0.0) last = k, last_before = before;
-          if (owner < 0 && before + s > aim) owner = k, owner_before = before;
-          before += s;
-        }
-        if (owner < 0) owner = last, owner_before = last_before;
-        if (owner == rank) {
-          if (tid == 0) found = 0x7FFFFFFF;
-          __shared__ int positive;
-          if (tid == 0) positive = -1;
-          double run = owner_before;
-          for (int v0 = lo; v0 < hi; v0 += kStep) {
-            const int v = v0 + tid * kVerifyVec;
-            double f[kVerifyVec], sum = 0.0;
-            int end = -1;
-            if (v < hi) {
-              weights(v, f);
-#pragma unroll
-              for (int i = 0; i < kVerifyVec; ++i) {
-                sum += f[i];
-                if (f[i] > 0.0) end = v + i;
-              }
+              f[i] = p_of(x[i]) * rp;
+              if (kDraft && c_q > 0.0) f[i] = fmax(fma(-rq, q_of(y[i]), f[i]), 0.0);
+              if (!kDraft && rejected > 0 && taken_away(v + i)) f[i] = 0.0;
+              sum += f[i];
+              if (f[i] > 0.0) end = v + i;
             }
             double incl = sum;
 #pragma unroll
@@ -476,50 +677,39 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
               const double o = __shfl_up_sync(0xffffffffu, incl, s);
               if (lane >= s) incl += o;
             }
-            __syncthreads();
-            if (lane == 31) wide_a[warp] = incl;
-            __syncthreads();
-            double base = run, all = 0.0;
-#pragma unroll
-            for (int w = 0; w < kVerifyWarps; ++w) {
-              if (w < warp) base += wide_a[w];
-              all += wide_a[w];
-            }
-            if (end >= 0) atomicMax(&positive, end);
-            // (the sums before a thread differ a little from those in it: the first that passes wins)
-            if (v < hi && base + incl > aim) {
-              double s = base + incl - sum;
+            last = max(last, __reduce_max_sync(0xffffffffu, end));
+            over = __ballot_sync(0xffffffffu, end >= 0 && sum_at + incl > aim);
+            if (over) {
+              double s = sum_at + incl - sum;
+              int mine_token = -1;
 #pragma unroll
               for (int i = 0; i < kVerifyVec; ++i) {
                 s += f[i];
-                if (f[i] > 0.0 && s > aim) {
-                  atomicMin(&found, v + i);
-                  break;
-                }
+                if (mine_token < 0 && f[i] > 0.0 && s > aim) mine_token = v + i;
               }
+              if (mine_token < 0) mine_token = end;  // (rounding may leave the sum at the aim: the last)
+              token = __shfl_sync(0xffffffffu, mine_token, __ffs(over) - 1);
             }
-            run += all;
-            __syncthreads();
-            if (found != 0x7FFFFFFF) break;
+            sum_at += __shfl_sync(0xffffffffu, incl, 31);
           }
-          if (tid == 0) a.token[b] = found != 0x7FFFFFFF ? found : positive;
-        } else if (owner < 0 && rank == 0 && tid == 0) {
-          a.token[b] = -1;
+          if (lane == 0) a.token[b] = token >= 0 ? token : last >= 0 ? last : lo + k * turns * 256;
         }
-        next = -2;  // (written)
       }
+      written = true;
+      break;
     }
-    if (went < 0) break;
     if (rank == 0 && tid == 0) a.path[static_cast<int64_t>(b) * a.n + taken] = went;
     ++taken;
     cur = went;
     __syncthreads();  // (gone is free)
   }
   if (rank == 0) {
-    for (int i = taken + tid; i < a.n; i += kVerifyThreads) a.path[static_cast<int64_t>(b) * a.n + i] = -1;
+    int* path = a.path + static_cast<int64_t>(b) * a.n;
+    for (int i = taken + tid; i < a.n; i += kVerifyThreads) path[i] = -1;
     if (tid == 0) {
+      path[0] = 0;
       a.taken[b] = taken;
-      if (next != -2) a.token[b] = next;
+      if (!written) a.token[b] = next;
     }
   }
 }
@@ -540,8 +730,9 @@ int verify_device_status(int clear, int* out) {
   return W8_OK;
 }
 
-template <typename E>
-static int verify_go(w8::VerifyArgs a, int64_t batch, int device, int sms, cudaStream_t stream) {
+template <typename Kern>
+static int verify_launch(Kern kern, int (&held)[64][w8::kVerifyCluster + 1], w8::VerifyArgs a, int64_t batch, int device,
+                         cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(w8::kVerifyThreads, 1, 1);
   cfg.stream = stream;
@@ -551,28 +742,51 @@ static int verify_go(w8::VerifyArgs a, int64_t batch, int device, int sms, cudaS
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  static int most[64] = {};  // CTAs of a cluster that the device takes
-  if (most[device] == 0) {
-    W8_CUDA_TRY(cudaFuncSetAttribute(w8::draft_verify_kernel<E>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    cfg.gridDim = dim3(w8::kVerifyCluster, 1, 1);
-    attr[0].val.clusterDim.x = w8::kVerifyCluster;
+  // Clusters of each size that the device holds at once: its SMs come in groups, which clusters do not
+  // cross (15 clusters of 8 or of 9, 22 of 6, 26 of 5).
+  if (held[device][1] == 0) {
+    W8_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cfg.numAttrs = 1;
-    int clusters = 0;
-    if (cudaOccupancyMaxActiveClusters(&clusters, w8::draft_verify_kernel<E>, &cfg) != cudaSuccess) {
-      cudaGetLastError();
-      clusters = 0;
+    for (int c = w8::kVerifyCluster; c >= 1; --c) {
+      cfg.gridDim = dim3(static_cast<unsigned>(c), 1, 1);
+      attr[0].val.clusterDim.x = static_cast<unsigned>(c);
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+      }
+      held[device][c] = c == 1 ? std::max(n, 1) : n;
     }
-    most[device] = clusters > 0 ? w8::kVerifyCluster : 8;
   }
-  // CTAs of a sequence: as many as give each an SM to itself (64 bits keep an SM's pipes busy, and two
-  // CTAs on some SMs would be what the others wait for), each with at least 2048 values.
-  const int64_t fill = std::max<int64_t>(1, sms / batch), fit = std::max<int64_t>(1, a.vocab / 2048);
-  const int cluster = static_cast<int>(std::min<int64_t>({most[device], fill, fit}));
+  // CTAs of a sequence: the most with which all sequences run at once (64 bits keep an SM's pipes busy,
+  // and a second wave would double the time), each with at least 2048 values.
+  int cluster = 1;
+  for (int c = 2; c <= w8::kVerifyCluster && c * 2048ll <= a.vocab; ++c)
+    if (held[device][c] >= batch) cluster = c;
   a.per = static_cast<int>(((a.vocab + cluster - 1) / cluster + 7) / 8 * 8);
   cfg.gridDim = dim3(static_cast<unsigned>(batch * cluster), 1, 1);
   attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   cfg.numAttrs = 2;
-  return cuda_status(cudaLaunchKernelEx(&cfg, w8::draft_verify_kernel<E>, a));
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
+}
+
+template <typename E, bool kCapped, bool kDraft>
+static int verify_sample(const w8::VerifyArgs& a, int64_t batch, int device, cudaStream_t stream) {
+  static int held[64][w8::kVerifyCluster + 1] = {};
+  return verify_launch(w8::draft_verify_kernel<E, kCapped, kDraft>, held, a, batch, device, stream);
+}
+
+template <typename E>
+static int verify_go(const w8::VerifyArgs& a, int64_t batch, int device, cudaStream_t stream) {
+  if (a.greedy) {
+    static int held[64][w8::kVerifyCluster + 1] = {};
+    return verify_launch(w8::draft_verify_greedy_kernel<E>, held, a, batch, device, stream);
+  }
+  if (a.cap > 0.0)
+    return a.d != nullptr ? verify_sample<E, true, true>(a, batch, device, stream)
+                          : verify_sample<E, true, false>(a, batch, device, stream);
+  return a.d != nullptr ? verify_sample<E, false, true>(a, batch, device, stream)
+                        : verify_sample<E, false, false>(a, batch, device, stream);
 }
 
 }  // namespace w8host
@@ -591,10 +805,8 @@ extern "C" int w8_draft_verify(const w8_draft_verify_args* in, w8_stream_t strea
   if (x.batch == 0) return W8_OK;
   const bool greedy = x.temperature == 0.0;
   W8_CHECK_ARG(x.logits && x.tokens && x.path && x.taken && x.token && (greedy || x.uniform), "null pointer");
-  int device = 0, sms = 0;
-  int st = require_sm100(&device);
-  if (st != W8_OK) return st;
-  st = num_sms(&sms);
+  int device = 0;
+  const int st = require_sm100(&device);
   if (st != W8_OK) return st;
   w8::VerifyArgs a = {};
   a.x = x.logits, a.d = greedy ? nullptr : x.draft;
@@ -610,7 +822,7 @@ extern "C" int w8_draft_verify(const w8_draft_verify_args* in, w8_stream_t strea
   a.cap = greedy ? 0.0 : x.cap;
   a.slope = greedy ? 1.0 : 1.4426950408889634 / x.temperature;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (x.dtype == W8_FP32) return verify_go<float>(a, x.batch, device, sms, s);
-  if (x.dtype == W8_BF16) return verify_go<__nv_bfloat16>(a, x.batch, device, sms, s);
-  return verify_go<__half>(a, x.batch, device, sms, s);
+  if (x.dtype == W8_FP32) return verify_go<float>(a, x.batch, device, s);
+  if (x.dtype == W8_BF16) return verify_go<__nv_bfloat16>(a, x.batch, device, s);
+  return verify_go<__half>(a, x.batch, device, s);
 }
