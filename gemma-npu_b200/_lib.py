@@ -132,7 +132,8 @@ SIGNATURES.update({
     "w8_attention_paged": (_i, [_p, _p, _i64, _p]),
     "w8_attention_paged_workspace_bytes": (_i64, [_p]),
     "w8_paged_append": (_i, [_p, _p]),
-    "w8_page_assign": (_i, [_p, _p]),
+    "w8_page_assign": (_i, [_p, _p, _i64, _p]),
+    "w8_page_assign_workspace_bytes": (_i64, [_i64, _i64]),
     "w8_draft_verify": (_i, [_p, _p]),
 })
 

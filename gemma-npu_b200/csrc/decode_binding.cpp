@@ -35,6 +35,7 @@ decltype(&w8_attention_paged) fn_paged = nullptr;
 decltype(&w8_attention_paged_workspace_bytes) fn_paged_ws = nullptr;
 decltype(&w8_paged_append) fn_paged_append = nullptr;
 decltype(&w8_page_assign) fn_assign = nullptr;
+decltype(&w8_page_assign_workspace_bytes) fn_assign_ws = nullptr;
 decltype(&w8_draft_verify) fn_verify = nullptr;
 PyObject* check_status = nullptr;  // _lib.check(status, name): raises
 
@@ -612,7 +613,8 @@ PyObject* page_assign(PyObject* const* arg, Py_ssize_t nargs) {
   a.ok = static_cast<uint8_t*>(ok.data_ptr());
   {
     const c10::cuda::CUDAGuard guard(dev);
-    check(fn_assign(&a, stream_of(dev)), "w8_page_assign");
+    const Tensor ws = workspace(fn_assign_ws(B, a.table_pages), dev);
+    check(fn_assign(&a, ws.data_ptr(), ws.numel(), stream_of(dev)), "w8_page_assign");
   }
   return wrap(ok);
 }
@@ -692,6 +694,7 @@ PyObject* bind(PyObject* const* arg, Py_ssize_t nargs) {
   get(fn_paged_ws, "w8_attention_paged_workspace_bytes");
   get(fn_paged_append, "w8_paged_append");
   get(fn_assign, "w8_page_assign");
+  get(fn_assign_ws, "w8_page_assign_workspace_bytes");
   get(fn_verify, "w8_draft_verify");
   check_status = same(arg[1]);
   Py_RETURN_NONE;

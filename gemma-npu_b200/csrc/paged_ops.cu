@@ -54,13 +54,29 @@ __device__ __forceinline__ float paged_f32<__half>(uint32_t bits) {
 // 11), and so is which side of a half the quotient lies on: it differs from a half by at least
 // 2^-2 over m's 8 or 11 bits where the quotient is in [64, 128), by 2^-10 over them in
 // [1/4, 1), relative to it 2^-20 or more, so that the quotient rounded to fp32 never becomes
-// a half that it was not.  A product with the reciprocal (off by less than 127 2^-22) decides
-// all but what is near a half.
-__device__ __forceinline__ int paged_round(float x, float m, float r) {
-  const float t = x * r;
-  float q = rintf(t);
-  if (fabsf(fabsf(t - q) - 0.5f) < 1e-4f) q = rintf(__fdiv_rn(x * 127.f, m));
-  return static_cast<int>(q);
+// a half that it was not.
+__device__ __forceinline__ uint32_t paged_divide(float x, float m) {
+  return static_cast<uint32_t>(static_cast<int>(rintf(__fdiv_rn(x * 127.f, m)))) & 0xFFu;
+}
+// Four such bytes.  A product with the reciprocal (off by less than 127 2^-22) decides all but what is
+// near a half; adding 1.5 2^23 leaves the integer in the sum's low bits, without a conversion
+// (those and the rounding instruction have an eighth of an addition's rate: 47 us with them where
+// this takes PLACEHOLDER).
+__device__ __forceinline__ uint32_t paged_round4(const float (&x)[4], float m, float r, bool slow) {
+  constexpr float kBig = 12582912.f;
+  float far = 0.f;
+  uint32_t bits[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = __fmul_rn(x[i], r), q = __fadd_rn(t, kBig);
+    bits[i] = __float_as_uint(q);
+    far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(q, kBig))));
+  }
+  if (far > 0.4999f || slow) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits[i] = paged_divide(x[i], m);
+  }
+  return __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
 }
 
 // One CTA: K or V of one cache head of one sequence, and the page that is `blockIdx.y` behind the
@@ -178,10 +194,15 @@ __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedA
         uint32_t out[2] = {0, 0};
         if (finite && m > 0.f) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float v = paged_f32<T>((ws[k >> 1] >> (16 * (k & 1))) & 0xFFFFu) * down;
-            const int q = slow ? static_cast<int>(rintf(__fdiv_rn(v * 127.f, m))) : paged_round(v, m, r);
-            out[k >> 2] |= (static_cast<uint32_t>(q) & 0xFFu) << (8 * (k & 3));
+          for (int k = 0; k < 2; ++k) {
+            float v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = paged_f32<T>((ws[2 * k + (q >> 1)] >> (16 * (q & 1))) & 0xFFFFu);
+            if (down != 1.f) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) v[q] *= down;
+            }
+            out[k] = paged_round4(v, m, r, slow);
           }
         }
         *reinterpret_cast<uint2*>(dst + row * a.page_r[kv] + ch * 8) = make_uint2(out[0], out[1]);
@@ -211,6 +232,7 @@ struct AssignArgs {
   uint8_t* ok;
   int batch, width, free_size, shift, room, window, sink;
   int wide;  // rows of the table load as 16-byte vectors
+  int4* counts;  // [batch] of a large table, counted by a kernel of its own; or null
 };
 
 constexpr int kAssignThreads = 512;
@@ -241,12 +263,64 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
+// What a warp finds in request b's table: entries that go back, missing ones, and the range [lo, hi) of
+// both, in every lane.
+__device__ __forceinline__ int4 assign_count(const AssignArgs& a, int b) {
+  const int lane = threadIdx.x & 31;
+  const AssignRow r = assign_row(a, b);
+  const int* row = a.table + b * a.table_b;
+  int nb = 0, nm = 0, first = a.width, last = 0;
+  auto see = [&](int i, int v) {
+    const bool want = r.want(i);
+    const bool bk = v >= 0 && !want, ms = v < 0 && want && r.fits;
+    nb += bk, nm += ms;
+    if (bk || ms) first = min(first, i), last = i + 1;
+  };
+  if (r.valid) {
+    int i = 0;
+    if (a.wide) {
+      const int4* row4 = reinterpret_cast<const int4*>(row);
+      const int n4 = a.width >> 2;
+      for (int v0 = lane; v0 < n4; v0 += 32 * 8) {
+        int4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = v0 + 32 * u < n4 ? row4[v0 + 32 * u] : make_int4(-1, -1, -1, -1);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (v0 + 32 * u < n4) {
+            const int at = 4 * (v0 + 32 * u);
+            see(at, x[u].x), see(at + 1, x[u].y), see(at + 2, x[u].z), see(at + 3, x[u].w);
+          }
+      }
+      i = n4 * 4;
+    }
+    for (i += lane; i < a.width; i += 32) see(i, row[i]);
+  } else if (lane == 0) {
+    paged_bad_index();
+  }
+  nb = __reduce_add_sync(0xffffffffu, nb);
+  nm = __reduce_add_sync(0xffffffffu, nm);
+  first = __reduce_min_sync(0xffffffffu, first);
+  last = __reduce_max_sync(0xffffffffu, last);
+  return make_int4(nb, nm, first, last);
+}
+
+constexpr int kCountWarps = 4;
+__global__ void __launch_bounds__(32 * kCountWarps) page_count_kernel(const AssignArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.x * kCountWarps + (threadIdx.x >> 5);
+  if (b >= a.batch) return;
+  const int4 c = assign_count(a, b);
+  if ((threadIdx.x & 31) == 0) a.counts[b] = c;
+}
+
 // One cluster for the whole table, each CTA a contiguous range of requests, a warp a request.
-// A first pass over the table counts what goes back and what is missing, prefix sums (over a
+// What goes back and what is missing is counted (of more than 16384 entries by page_count_kernel on
+// all SMs: 512 tables of 2048 take PLACEHOLDER where this cluster alone took 25), prefix sums (over a
 // CTA's requests, then the cluster's CTAs) give every request its place in the stack, and a
 // second pass, over the entries between a request's first and last change only, moves the pages:
-// first all that go back, then, behind a barrier of the cluster, those that are given out.  The
-// table is read once by few SMs, so it is bound by the loads they have under way.
+// first all that go back, then, behind a barrier of the cluster, those that are given out.
 __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const AssignArgs a) {
   __shared__ int back[kAssignRequests], miss[kAssignRequests];        // counts, then what comes before
   __shared__ int lo[kAssignRequests], hi[kAssignRequests];            // a request's changes lie in [lo, hi)
@@ -267,43 +341,16 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
   const bool bad_top = top0 < 0 || top0 > a.free_size;
   const int top = bad_top ? (top0 < 0 ? 0 : a.free_size) : top0;
   if (bad_top && rank == 0 && tid == 0) paged_bad_index();
-  for (int q = warp; q < count; q += kAssignWarps) {
-    const AssignRow r = assign_row(a, b0 + q);
-    const int* row = a.table + (b0 + q) * a.table_b;
-    int nb = 0, nm = 0, first = a.width, last = 0;
-    auto see = [&](int i, int v) {
-      const bool want = r.want(i);
-      const bool bk = v >= 0 && !want, ms = v < 0 && want && r.fits;
-      nb += bk, nm += ms;
-      if (bk || ms) first = min(first, i), last = i + 1;
-    };
-    if (r.valid) {
-      int i = 0;
-      if (a.wide) {
-        const int4* row4 = reinterpret_cast<const int4*>(row);
-        const int n4 = a.width >> 2;
-        for (int v0 = lane; v0 < n4; v0 += 32 * 8) {
-          int4 x[8];
-#pragma unroll
-          for (int u = 0; u < 8; ++u) x[u] = v0 + 32 * u < n4 ? row4[v0 + 32 * u] : make_int4(-1, -1, -1, -1);
-#pragma unroll
-          for (int u = 0; u < 8; ++u)
-            if (v0 + 32 * u < n4) {
-              const int at = 4 * (v0 + 32 * u);
-              see(at, x[u].x), see(at + 1, x[u].y), see(at + 2, x[u].z), see(at + 3, x[u].w);
-            }
-        }
-        i = n4 * 4;
-      }
-      for (i += lane; i < a.width; i += 32) see(i, row[i]);
-    } else if (lane == 0) {
-      paged_bad_index();
+  if (a.counts != nullptr) {
+    for (int q = tid; q < count; q += kAssignThreads) {
+      const int4 c = a.counts[b0 + q];
+      back[q] = c.x, miss[q] = c.y, lo[q] = c.z, hi[q] = c.w;
     }
-    nb = __reduce_add_sync(0xffffffffu, nb);
-    nm = __reduce_add_sync(0xffffffffu, nm);
-    first = __reduce_min_sync(0xffffffffu, first);
-    last = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0) back[q] = nb, miss[q] = nm, lo[q] = first, hi[q] = last;
+  } else {
+    for (int q = warp; q < count; q += kAssignWarps) {
+      const int4 c = assign_count(a, b0 + q);
+      if (lane == 0) back[q] = c.x, miss[q] = c.y, lo[q] = c.z, hi[q] = c.w;
+    }
   }
   __syncthreads();
   // Exclusive prefix sums over the CTA's requests (each thread a run of them).
@@ -519,7 +566,12 @@ extern "C" int w8_paged_append(const w8_paged_append_args* in, w8_stream_t strea
                             : launch_paged(w8::paged_append_kernel<__half>, grid, threads, 0, s, a);
 }
 
-extern "C" int w8_page_assign(const w8_page_assign_args* in, w8_stream_t stream) {
+extern "C" int64_t w8_page_assign_workspace_bytes(int64_t batch, int64_t table_pages) {
+  return batch > 0 && table_pages > 0 && batch * table_pages > 16384 ? batch * 16 : 0;
+}
+
+extern "C" int w8_page_assign(const w8_page_assign_args* in, void* workspace, int64_t workspace_bytes,
+                              w8_stream_t stream) {
   using namespace w8host;
   W8_CHECK_ARG(in != nullptr, "null arguments");
   const w8_page_assign_args& x = *in;
@@ -558,11 +610,19 @@ extern "C" int w8_page_assign(const w8_page_assign_args* in, w8_stream_t stream)
   a.window = static_cast<int>(x.window);
   a.sink = static_cast<int>(x.sink);
   a.wide = aligned(x.table, 16) && (x.batch == 1 || x.table_stride % 4 == 0);
-  // CTAs of the cluster: one for each 16 K entries, and as many as the requests need.
+  const int64_t need = w8_page_assign_workspace_bytes(x.batch, x.table_pages);
+  W8_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace of %lld bytes needed (got %lld)",
+               (long long)need, (long long)workspace_bytes);
+  W8_CHECK_ALIGN(aligned(workspace, 16), "workspace must be 16-byte aligned");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (need > 0) {
+    a.counts = static_cast<int4*>(workspace);
+    const int blocks = static_cast<int>((x.batch + w8::kCountWarps - 1) / w8::kCountWarps);
+    const int st2 = launch_paged(w8::page_count_kernel, dim3(static_cast<unsigned>(blocks)), 32 * w8::kCountWarps, 0, s, a);
+    if (st2 != W8_OK) return st2;
+  }
+  // CTAs of the cluster: a request a warp, and as many as the requests need.
   int cluster = 1;
-  while (cluster < w8::kAssignCluster &&
-         (x.batch * x.table_pages > static_cast<int64_t>(cluster) * 16384 || x.batch > static_cast<int64_t>(cluster) * w8::kAssignRequests))
-    cluster *= 2;
-  return launch_paged(w8::page_assign_kernel, dim3(static_cast<unsigned>(cluster)), w8::kAssignThreads, cluster,
-                      reinterpret_cast<cudaStream_t>(stream), a);
+  while (cluster < w8::kAssignCluster && x.batch > static_cast<int64_t>(cluster) * 2 * w8::kAssignWarps) cluster *= 2;
+  return launch_paged(w8::page_assign_kernel, dim3(static_cast<unsigned>(cluster)), w8::kAssignThreads, cluster, s, a);
 }

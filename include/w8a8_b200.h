@@ -487,7 +487,9 @@ typedef struct w8_page_assign_args {
  * what it and all requests before it miss is there; one that misses nothing is, and one that
  * needs more pages than a table has is not and does not count.  A request whose length is out of
  * range keeps what it has.  At most 8192 requests. */
-int w8_page_assign(const w8_page_assign_args* args, w8_stream_t stream);
+int w8_page_assign(const w8_page_assign_args* args, void* workspace, int64_t workspace_bytes, w8_stream_t stream);
+/* Workspace in bytes (16-byte aligned). */
+int64_t w8_page_assign_workspace_bytes(int64_t batch, int64_t table_pages);
 
 typedef struct w8_draft_verify_args {
   const void* logits;    /* [batch, n_new, vocab]: the target's after each node */
