@@ -38,8 +38,7 @@ struct PagedAppendArgs {
   int table_pages, pages, shift, kv_heads, n, steps, chunk_shift;  // 1 << chunk_shift 16-byte chunks a row
 };
 
-constexpr int kPageVecs = 8;       // 16-byte chunks of a thread
-constexpr int kPageThreads = 1024; // at most: a page of 128 rows of 512 values
+constexpr int kPageThreads = 1024;  // at most, with 4 16-byte chunks each, 8 for a page of 128 rows of 512 values
 
 template <typename T>
 __device__ __forceinline__ float paged_f32(uint32_t bits);
@@ -85,7 +84,7 @@ __device__ __forceinline__ uint32_t paged_round4(const float (&x)[4], float m, f
 // writes the rows that stay in the tail, which are all new: the tail's old rows, if the page was
 // filled, are read before.  Bound by HBM for prompts (2 bytes read, 1 written a value: 13,000
 // tokens of 8 heads of 128 take PLACEHOLDER) and by the chain length, table, row for a token.
-template <typename T>
+template <typename T, int kVecs>
 __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedAppendArgs a) {
   __shared__ int sm_took;
   __shared__ uint32_t sm_max[32];
@@ -95,19 +94,17 @@ __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedA
   pdl_launch_dependents();
   pdl_wait();
   const int len = a.lens[b];
+  const int given = a.count != nullptr ? a.count[b] : a.steps;
   const int room = a.table_pages << a.shift;
   const bool first = j == 0 && c == 0 && kv == 0 && tid == 0;
   if (len < 0 || len > room) {
     if (first) paged_bad_index(), a.lens_out[b] = len;
     return;
   }
-  int took = a.steps;
-  if (a.count != nullptr) {
-    took = a.count[b];
-    if (took < 0 || took > a.steps) {
-      if (first) paged_bad_index();
-      took = took < 0 ? 0 : a.steps;
-    }
+  int took = given;
+  if (took < 0 || took > a.steps) {
+    if (first) paged_bad_index();
+    took = took < 0 ? 0 : a.steps;
   }
   const int* path = a.path != nullptr ? a.path + b * a.path_b : nullptr;
   if (path != nullptr) {  // entries before the first negative one
@@ -144,16 +141,12 @@ __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedA
     return fresh + i * a.new_r[kv];
   };
   if (j < full) {
-    int page = a.table[b * a.table_b + (len >> a.shift) + j];
-    if (page < 0 || page >= a.pages) {
-      if (tid == 0) paged_bad_index();
-      page = -1;
-    }
+    const int entry = a.table[b * a.table_b + (len >> a.shift) + j];  // (looked at when the rows have come)
     const int vecs = page_rows << a.chunk_shift;
-    uint4 x[kPageVecs];
+    uint4 x[kVecs];
     uint32_t most = 0;  // of the magnitudes' bits, two at a time: they order as the magnitudes do
 #pragma unroll
-    for (int i = 0; i < kPageVecs; ++i) {
+    for (int i = 0; i < kVecs; ++i) {
       const int e = tid + i * threads;
       x[i] = make_uint4(0, 0, 0, 0);
       if (e >= vecs) continue;
@@ -162,7 +155,7 @@ __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedA
       if (row != nullptr) x[i] = *reinterpret_cast<const uint4*>(row + ch * 8);
     }
 #pragma unroll
-    for (int i = 0; i < kPageVecs; ++i) {
+    for (int i = 0; i < kVecs; ++i) {
       most = __vmaxu2(most, x[i].x & 0x7FFF7FFFu);
       most = __vmaxu2(most, x[i].y & 0x7FFF7FFFu);
       most = __vmaxu2(most, x[i].z & 0x7FFF7FFFu);
@@ -182,11 +175,13 @@ __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedA
     const float r = finite && m > 0.f ? 127.f / m : 0.f;
     // (magnitudes so small that 127 / m overflows are divided one by one)
     const bool slow = finite && m > 0.f && !(r < 0x1p120f);
+    const int page = entry >= 0 && entry < a.pages ? entry : -1;
+    if (page < 0 && tid == 0) paged_bad_index();
     if (page >= 0) {
       if (tid == 0) a.scale[kv][page * a.scale_p[kv] + c * a.scale_h[kv]] = scale;
       int8_t* dst = a.page[kv] + page * a.page_p[kv] + c * a.page_h[kv];
 #pragma unroll
-      for (int i = 0; i < kPageVecs; ++i) {
+      for (int i = 0; i < kVecs; ++i) {
         const int e = tid + i * threads;
         if (e >= vecs) break;
         const int row = e >> a.chunk_shift, ch = e & ((1 << a.chunk_shift) - 1);
@@ -562,8 +557,12 @@ extern "C" int w8_paged_append(const w8_paged_append_args* in, w8_stream_t strea
   const int threads = static_cast<int>(std::min<int64_t>(w8::kPageThreads, std::max<int64_t>(64, vecs / 4)));
   const dim3 grid(static_cast<unsigned>(2 * x.batch * x.kv_heads), static_cast<unsigned>(most));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return x.dtype == W8_BF16 ? launch_paged(w8::paged_append_kernel<__nv_bfloat16>, grid, threads, 0, s, a)
-                            : launch_paged(w8::paged_append_kernel<__half>, grid, threads, 0, s, a);
+  using B = __nv_bfloat16;
+  if (vecs <= 4 * threads)
+    return x.dtype == W8_BF16 ? launch_paged(w8::paged_append_kernel<B, 4>, grid, threads, 0, s, a)
+                              : launch_paged(w8::paged_append_kernel<__half, 4>, grid, threads, 0, s, a);
+  return x.dtype == W8_BF16 ? launch_paged(w8::paged_append_kernel<B, 8>, grid, threads, 0, s, a)
+                            : launch_paged(w8::paged_append_kernel<__half, 8>, grid, threads, 0, s, a);
 }
 
 extern "C" int64_t w8_page_assign_workspace_bytes(int64_t batch, int64_t table_pages) {
