@@ -49,6 +49,21 @@ __device__ __forceinline__ float paged_f32<__half>(uint32_t bits) {
   return __half2float(__ushort_as_half(static_cast<uint16_t>(bits)));
 }
 
+// The larger magnitude of each half of two pairs, a NaN above all (one instruction; the maxima of 16-bit
+// integers are made of ten).
+template <typename T>
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t larger2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <>
+__device__ __forceinline__ uint32_t larger2<__half>(uint32_t a, uint32_t b) {
+  const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+
 // round(127 x / m) to nearest even, |x| <= m.  127 x is exact in fp32 (7 more bits than x's 8 or
 // 11), and so is which side of a half the quotient lies on: it differs from a half by at least
 // 2^-2 over m's 8 or 11 bits where the quotient is in [64, 128), by 2^-10 over them in
@@ -57,25 +72,28 @@ __device__ __forceinline__ float paged_f32<__half>(uint32_t bits) {
 __device__ __forceinline__ uint32_t paged_divide(float x, float m) {
   return static_cast<uint32_t>(static_cast<int>(rintf(__fdiv_rn(x * 127.f, m)))) & 0xFFu;
 }
-// Four such bytes.  A product with the reciprocal (off by less than 127 2^-22) decides all but what is
+// Eight such bytes.  A product with the reciprocal (off by less than 127 2^-22) decides all but what is
 // near a half; adding 1.5 2^23 leaves the integer in the sum's low bits, without a conversion
 // (those and the rounding instruction have an eighth of an addition's rate: 47 us with them where
 // this takes PLACEHOLDER).
-__device__ __forceinline__ uint32_t paged_round4(const float (&x)[4], float m, float r, bool slow) {
+__device__ __forceinline__ uint2 paged_round8(const float (&x)[8], float m, float r, bool slow) {
   constexpr float kBig = 12582912.f;
   float far = 0.f;
-  uint32_t bits[4];
+  uint32_t bits[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const float t = __fmul_rn(x[i], r), q = __fadd_rn(t, kBig);
     bits[i] = __float_as_uint(q);
     far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(q, kBig))));
   }
   if (far > 0.4999f || slow) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bits[i] = paged_divide(x[i], m);
+    for (int i = 0; i < 8; ++i) bits[i] = paged_divide(x[i], m);
   }
-  return __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
+  auto four = [&](int i) {
+    return __byte_perm(__byte_perm(bits[i], bits[i + 1], 0x0040), __byte_perm(bits[i + 2], bits[i + 3], 0x0040), 0x5410);
+  };
+  return make_uint2(four(0), four(4));
 }
 
 // One CTA: K or V of one cache head of one sequence, and the page that is `blockIdx.y` behind the
@@ -142,24 +160,33 @@ __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedA
   };
   if (j < full) {
     const int entry = a.table[b * a.table_b + (len >> a.shift) + j];  // (looked at when the rows have come)
-    const int vecs = page_rows << a.chunk_shift;
+    // This thread's chunk of every (threads / chunks)-th row: addresses by steps.
+    const int vecs = page_rows << a.chunk_shift, ch = tid & ((1 << a.chunk_shift) - 1), r0 = tid >> a.chunk_shift;
+    const int step = threads >> a.chunk_shift, at0 = (j << a.shift) + r0;
     uint4 x[kVecs];
-    uint32_t most = 0;  // of the magnitudes' bits, two at a time: they order as the magnitudes do
+    uint32_t most = 0;  // the largest magnitudes, two at a time
+    const uint16_t* in_tail = tail + at0 * a.tail_r[kv] + ch * 8;
+    const uint16_t* in_new = fresh + (at0 - off) * a.new_r[kv] + ch * 8;
+    const int64_t tail_step = step * a.tail_r[kv], new_step = step * a.new_r[kv];
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int e = tid + i * threads;
+    for (int i = 0; i < kVecs; ++i, in_tail += tail_step, in_new += new_step) {
       x[i] = make_uint4(0, 0, 0, 0);
-      if (e >= vecs) continue;
-      const int r = e >> a.chunk_shift, ch = e & ((1 << a.chunk_shift) - 1), at = (j << a.shift) + r;
-      const uint16_t* row = at < off ? tail + at * a.tail_r[kv] : new_row(at);
-      if (row != nullptr) x[i] = *reinterpret_cast<const uint4*>(row + ch * 8);
+      if (tid + i * threads >= vecs) continue;
+      const int at = at0 + i * step;
+      const uint16_t* row = in_tail;
+      if (at >= off) {
+        row = in_new;
+        if (path != nullptr) {
+          row = new_row(at);
+          if (row != nullptr) row += ch * 8;
+        }
+      }
+      if (row != nullptr) x[i] = *reinterpret_cast<const uint4*>(row);
     }
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      most = __vmaxu2(most, x[i].x & 0x7FFF7FFFu);
-      most = __vmaxu2(most, x[i].y & 0x7FFF7FFFu);
-      most = __vmaxu2(most, x[i].z & 0x7FFF7FFFu);
-      most = __vmaxu2(most, x[i].w & 0x7FFF7FFFu);
+      most = larger2<T>(most, larger2<T>(larger2<T>(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu),
+                                         larger2<T>(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
     }
     most = __reduce_max_sync(0xffffffffu, max(most & 0xFFFFu, most >> 16));
     if ((tid & 31) == 0) sm_max[tid >> 5] = most;
@@ -179,28 +206,24 @@ __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedA
     if (page < 0 && tid == 0) paged_bad_index();
     if (page >= 0) {
       if (tid == 0) a.scale[kv][page * a.scale_p[kv] + c * a.scale_h[kv]] = scale;
-      int8_t* dst = a.page[kv] + page * a.page_p[kv] + c * a.page_h[kv];
+      int8_t* dst = a.page[kv] + page * a.page_p[kv] + c * a.page_h[kv] + r0 * a.page_r[kv] + ch * 8;
+      const int64_t dst_step = step * a.page_r[kv];
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        const int e = tid + i * threads;
-        if (e >= vecs) break;
-        const int row = e >> a.chunk_shift, ch = e & ((1 << a.chunk_shift) - 1);
+      for (int i = 0; i < kVecs; ++i, dst += dst_step) {
+        if (tid + i * threads >= vecs) break;
         const uint32_t ws[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        uint32_t out[2] = {0, 0};
+        uint2 out = make_uint2(0, 0);
         if (finite && m > 0.f) {
+          float v[8];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float v[4];
+          for (int q = 0; q < 8; ++q) v[q] = paged_f32<T>((ws[q >> 1] >> (16 * (q & 1))) & 0xFFFFu);
+          if (down != 1.f) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = paged_f32<T>((ws[2 * k + (q >> 1)] >> (16 * (q & 1))) & 0xFFFFu);
-            if (down != 1.f) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) v[q] *= down;
-            }
-            out[k] = paged_round4(v, m, r, slow);
+            for (int q = 0; q < 8; ++q) v[q] *= down;
           }
+          out = paged_round8(v, m, r, slow);
         }
-        *reinterpret_cast<uint2*>(dst + row * a.page_r[kv] + ch * 8) = make_uint2(out[0], out[1]);
+        *reinterpret_cast<uint2*>(dst) = out;
       }
     }
   }
