@@ -645,7 +645,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
           if (is_page(i)) {
             // (not 0, times which a hidden key's -inf would be NaN: a page's keys may all be 0)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) to_log2[q] = fmaxf(scales[(i % kTtScales) * 16 + 4 * hv + q] * scale, 1e-30f);
+            for (int q = 0; q < 4; ++q) {
+              const float f = scales[(i % kTtScales) * 16 + 4 * hv + q] * scale;
+              to_log2[q] = f < 1e-30f ? 1e-30f : f;  // (a NaN stays)
+            }
           } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q) to_log2[q] = scale;
@@ -724,11 +727,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
       if constexpr (kPaged) {
         // P in O's unit, the scale of V in the exponent: 2^(x - m + log2 vr); l takes it back, 16 keys
         // at a time.  (A scale of 0 is 2^-100 here: the values are 0.)
-        bool odd = false;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) odd |= vr[q] != vr[q];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+          const float odd = to_log2[q] + vr[q];
+          if (odd != odd) {  // a NaN scale is for the rows that see the page (the same in the whole warp)
+#pragma unroll
+            for (int e = 8 * q; e < 8 * q + 8; ++e) {
+              const bool on0 = __uint_as_float(sv[e >> 4][(2 * e) & 31]) != -INFINITY;
+              const bool on1 = __uint_as_float(sv[e >> 4][(2 * e + 1) & 31]) != -INFINITY;
+              pw[e] = pack2<T>(on0 ? odd : 0.f, on1 ? odd : 0.f);
+              if (on0 || on1) l4[q] = odd;
+            }
+            continue;
+          }
           const float v = fmaxf(vr[q], 0x1p-100f), ref_q = ref - lg2_tc(v);
 #pragma unroll
           for (int e = 8 * q; e < 8 * q + 8; ++e) {
@@ -738,15 +749,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
             pw[e] = pack2<T>(p0, p1);
           }
           l4[q] *= 1.f / v;
-        }
-        if (odd) {  // a NaN scale is for the rows that see the page
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (vr[e >> 3] != vr[e >> 3]) {
-              const bool on0 = __uint_as_float(sv[e >> 4][(2 * e) & 31]) != -INFINITY;
-              const bool on1 = __uint_as_float(sv[e >> 4][(2 * e + 1) & 31]) != -INFINITY;
-              pw[e] = pack2<T>(on0 ? vr[e >> 3] : 0.f, on1 ? vr[e >> 3] : 0.f);
-            }
         }
       } else {
 #pragma unroll

@@ -905,13 +905,6 @@ static int cache_shape(int64_t batch, int64_t kv_heads, int64_t slots, int64_t r
   return W8_OK;
 }
 
-// Whether two int32 arrays share memory (what one CTA writes of one, another may yet have to read
-// of the other).
-static bool arrays_meet(const int32_t* p, int64_t n, const int32_t* q, int64_t m) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-  return p != nullptr && q != nullptr && a < b + 4 * static_cast<uintptr_t>(m) && b < a + 4 * static_cast<uintptr_t>(n);
-}
-
 static int cache_rows(const char* name, const void* p, const int64_t* strides) {
   W8_CHECK_ARG(p != nullptr, "%s is null", name);
   W8_CHECK_ALIGN(aligned(p, 16), "%s must be 16-byte aligned", name);

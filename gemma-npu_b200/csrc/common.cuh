@@ -491,6 +491,13 @@ void set_error(const char* fmt, ...);
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+// Whether two int32 arrays share memory (what one CTA writes of one, another may yet have to read
+// of the other).
+inline bool arrays_meet(const int32_t* p, int64_t n, const int32_t* q, int64_t m) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return p != nullptr && q != nullptr && a < b + 4 * static_cast<uintptr_t>(m) && b < a + 4 * static_cast<uintptr_t>(n);
+}
+
 int num_sms(int* out);
 
 }  // namespace w8host

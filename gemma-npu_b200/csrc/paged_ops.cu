@@ -522,8 +522,11 @@ extern "C" int w8_paged_append(const w8_paged_append_args* in, w8_stream_t strea
   W8_CHECK_ARG(x.path != nullptr || x.steps == x.n_new, "without a path the steps are the new tokens");
   if (x.batch == 0) return W8_OK;
   W8_CHECK_ARG(x.lens && x.lens_out && x.k_tail && x.v_tail && (x.n_new == 0 || (x.k_new && x.v_new)), "null pointer");
-  W8_CHECK_ARG(x.lens != x.lens_out && x.lens_out != x.count && x.lens_out != x.path,
-               "lens_out must be apart from lens, count and path");
+  W8_CHECK_ARG(!arrays_meet(x.lens, x.batch, x.lens_out, x.batch), "lens_out must not be lens nor overlap it");
+  W8_CHECK_ARG(!arrays_meet(x.count, x.batch, x.lens_out, x.batch), "lens_out must not be count nor overlap it");
+  if (x.path && x.steps > 0 && arrays_meet(x.path, (x.batch - 1) * x.path_stride + x.steps, x.lens_out, x.batch))
+    for (int64_t b = 0; b < x.batch; ++b)  // (it may lie between the rows)
+      W8_CHECK_ARG(!arrays_meet(x.path + b * x.path_stride, x.steps, x.lens_out, x.batch), "lens_out must not overlap path");
   W8_CHECK_ARG(x.pages == 0 || (x.k && x.v && x.k_scale && x.v_scale), "null pages");
   W8_CHECK_ARG(x.table_pages == 0 || x.table, "null table");
   const void* ptrs[6] = {x.k_tail, x.v_tail, x.k_new, x.v_new, x.k, x.v};
@@ -613,6 +616,21 @@ extern "C" int w8_page_assign(const w8_page_assign_args* in, void* workspace, in
                "size beyond the limits");
   if (x.batch == 0) return W8_OK;
   W8_CHECK_ARG(x.lens && x.top && x.ok && (x.free_pages == 0 || x.free) && (x.table_pages == 0 || x.table), "null pointer");
+  W8_CHECK_ARG(x.table_pages == 0 || x.batch == 1 || x.table_stride >= x.table_pages, "the rows of the table overlap");
+  W8_CHECK_ARG(!arrays_meet(x.lens, x.batch, x.top, 1) && !arrays_meet(x.lens, x.batch, x.free, x.free_pages) &&
+                   !arrays_meet(x.free, x.free_pages, x.top, 1),
+               "lens, free and top must not overlap");
+  auto on_table = [&](int64_t row, int64_t n) {
+    const int32_t* at = x.table + row * x.table_stride;
+    return arrays_meet(at, n, x.lens, x.batch) || arrays_meet(at, n, x.top, 1) || arrays_meet(at, n, x.free, x.free_pages);
+  };
+  if (x.table_pages > 0 && on_table(0, (x.batch - 1) * x.table_stride + x.table_pages))
+    for (int64_t b = 0; b < x.batch; ++b)  // (they may lie between the rows)
+      W8_CHECK_ARG(!on_table(b, x.table_pages), "the table must not overlap lens, free and top");
+  const int64_t need = w8_page_assign_workspace_bytes(x.batch, x.table_pages);
+  W8_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace of %lld bytes needed (got %lld)",
+               (long long)need, (long long)workspace_bytes);
+  W8_CHECK_ALIGN(aligned(workspace, 16), "workspace must be 16-byte aligned");
   int device = 0;
   const int st = require_sm100(&device);
   if (st != W8_OK) return st;
@@ -632,10 +650,6 @@ extern "C" int w8_page_assign(const w8_page_assign_args* in, void* workspace, in
   a.window = static_cast<int>(x.window);
   a.sink = static_cast<int>(x.sink);
   a.wide = aligned(x.table, 16) && (x.batch == 1 || x.table_stride % 4 == 0);
-  const int64_t need = w8_page_assign_workspace_bytes(x.batch, x.table_pages);
-  W8_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace of %lld bytes needed (got %lld)",
-               (long long)need, (long long)workspace_bytes);
-  W8_CHECK_ALIGN(aligned(workspace, 16), "workspace must be 16-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (need > 0) {
     a.counts = static_cast<int4*>(workspace);

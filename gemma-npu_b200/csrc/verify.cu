@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
         if (kDraft || rejected == 0 || shared_sum(2) > 0.0) break;
         rejected = 0;  // the weights taken were all there were: the target's own
       }
-      const double rp = 1.0 / p.sum, rq = kDraft ? c_q / q.sum : 0.0;
+      const double rp = 1.0 / p.sum, rq = kDraft && c_q > 0.0 ? c_q / q.sum : 0.0;  // (a draft row may be NaN)
       auto part_of = [&](int k) { return kDraft ? fma(-rq, shared[turn][3][k], shared[turn][2][k] * rp) : shared[turn][2][k] * rp; };
       const double aim = u0 * warp_sum(lane < ranks ? fmax(part_of(lane), 0.0) : 0.0);
       // The first of `n` parts whose running sum passes the aim, or the last with any weight (-1: none).
@@ -693,6 +693,8 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
             sum_at += __shfl_sync(0xffffffffu, incl, 31);
           }
           if (lane == 0) a.token[b] = token >= 0 ? token : last >= 0 ? last : lo + k * turns * 256;
+        } else if (owner < 0 && rank == 0 && lane == 0) {
+          a.token[b] = -1;
         }
       }
       written = true;
