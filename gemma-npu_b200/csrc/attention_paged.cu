@@ -45,8 +45,9 @@ struct PagedCfg {
   static constexpr int kBN = kGroups * kKT * 16;           // keys of a tile of pages: 256, 256, 128, 64
   static constexpr int kBN16 = kBN / 2;                    // of a 16-bit tile, which is as large
   static constexpr int kSlotBytes = kBN * D;               // 16 KB (D = 64) or 32 KB
-  static constexpr int kSlots = 163840 / kSlotBytes;       // 10 or 5
-  static constexpr int kJoin = 8192 / (kBM * kWarps) < D ? 8192 / (kBM * kWarps) : D;  // columns of the outputs joined at a time
+  // Columns of the outputs joined at a time, and the ring beside them.
+  static constexpr int kJoin = NT == 2 ? 64 : D < 256 ? D : 256;
+  static constexpr int kSlots = (D < 256 || NT == 2 ? 163840 : 131072) / kSlotBytes;  // 10, 5 or 4
   static constexpr int kPitch = kJoin + 4;                 // their fp32 row pitch
   static constexpr int kOffQ8 = kSlots * kSlotBytes;       // Q as fp16, scaled and permuted
   static constexpr int kOffQ16 = kOffQ8 + kBM * D * 2;     // Q as it is
@@ -261,14 +262,19 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (kind == kPages) {
-            if (lane < boxes) scales[slot * kPagedMaxBoxes + lane] = kv ? vs : ks;
-            if (lane == 0) masks[slot] = there;
-            __syncwarp();
-            if (lane == 0) mbar_arrive_expect_tx(full_bar(slot), __popc(there) * (box * D));
-            __syncwarp();
+            // The copies first: the scales, which the barrier's one arrival follows, are yet to come.
             if (page >= 0)
               tma_load_5d(dst + lane * (box * D), kv ? &tm_v : &tm_k, full_bar(slot), 0,
                           (key0 + (lane << box_shift)) & ((1 << pa.shift) - 1), 0, c, page);
+            if (kv == 0) continue;
+            const uint32_t before = (g - 1) % NS;  // (K's slot: its arrival waits for the same loads)
+            if (lane < boxes) scales[before * kPagedMaxBoxes + lane] = ks, scales[slot * kPagedMaxBoxes + lane] = vs;
+            if (lane == 0) masks[before] = there;
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive_expect_tx(full_bar(before), __popc(there) * (box * D));
+              mbar_arrive_expect_tx(full_bar(slot), __popc(there) * (box * D));
+            }
           } else if (lane == 0) {
             mbar_arrive_expect_tx(full_bar(slot), C::kSlotBytes);
             const CUtensorMap* map = kind == kTail ? (kv ? &tm_vt : &tm_kt) : (kv ? &tm_vn : &tm_kn);
@@ -451,6 +457,7 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
     // odd bytes of V's rows) and gets gl and gl + 8.
     auto natural = [&]() {
       permuted = false;
+      if (unit == __uint_as_float(0x00800000u)) return;  // (O is 0 as yet)
       const int s0 = ((gl >> 1) << 2) | tl, s1 = s0 + 16;
       const bool odd = gl & 1;
 #pragma unroll
@@ -727,14 +734,17 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
           // So may a new token's values where some row must not see them: cleared here, added below
           // to the rows that do.
           uint32_t bad = 0;  // keys of this step whose values are not all finite (new tokens only)
+          // (New rows behind the last are zeros already: the box ends there.)
           if (fresh || key0 + 16 > end || span.full + key0 < span.low) {
-            for (int e = lane; e < 16 * CH; e += 32) {
-              const int r = e % 16, ch = e / 16, p = span.full + key0 + r;
+            const int r0 = !fresh && span.full + key0 >= span.low ? end - key0 : 0;  // rows [r0, r1) are looked at
+            const int r1 = fresh ? min(end - key0, 16) : 16;
+            for (int e = lane; e < (r1 - r0) * CH; e += 32) {
+              const int r = r0 + e / CH, ch = e % CH, p = span.full + key0 + r;
               uint4* w = reinterpret_cast<uint4*>(smem + (sv - base) + (ch >> 3) * (BN16 * 128) + (kr + r) * 128 +
                                                   (((ch & 7) ^ ((kr + r) & 7)) << 4));
-              if (key0 + r >= end || (!fresh && p < span.low && p >= a.sink)) {
-                *w = make_uint4(0, 0, 0, 0);
-              } else if (fresh) {
+              if (!fresh) {
+                if (key0 + r >= end || (p < span.low && p >= a.sink)) *w = make_uint4(0, 0, 0, 0);
+              } else {
                 uint4 x = *w;
                 if (nonfinite_bits<T>(x.x) | nonfinite_bits<T>(x.y) | nonfinite_bits<T>(x.z) | nonfinite_bits<T>(x.w)) {
                   uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
@@ -784,7 +794,6 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(empty_bar(slot_v));
     }
-    if (permuted) natural();
 
     // ---- the warps' results joined: M = max m_w, O = sum 2^(m_w - M) O_w, some columns at a time
 #pragma unroll
@@ -820,12 +829,22 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float* dst = joint + (warp * BM + 8 * n + 2 * tl + h) * C::kPitch + gl;
+          float* dst = joint + (warp * BM + 8 * n + 2 * tl + h) * C::kPitch;
+          if (permuted) {  // (pages only: columns 2 gl and 2 gl + 1, in O's unit)
+            const float f = fac[n][h] * unit;
 #pragma unroll
-          for (int k = 0; k < C::kJoin / 16; ++k) {
-            const float* v = o[n][j * (C::kJoin / 16) + k];
-            dst[16 * k] = fac[n][h] < 0.f ? 0.f : v[h] * fac[n][h];
-            dst[16 * k + 8] = fac[n][h] < 0.f ? 0.f : v[2 + h] * fac[n][h];
+            for (int k = 0; k < C::kJoin / 16; ++k) {
+              const float* v = o[n][j * (C::kJoin / 16) + k];
+              *reinterpret_cast<float2*>(dst + 16 * k + 2 * gl) =
+                  fac[n][h] < 0.f ? make_float2(0.f, 0.f) : make_float2(v[h] * f, v[2 + h] * f);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < C::kJoin / 16; ++k) {
+              const float* v = o[n][j * (C::kJoin / 16) + k];
+              dst[16 * k + gl] = fac[n][h] < 0.f ? 0.f : v[h] * fac[n][h];
+              dst[16 * k + gl + 8] = fac[n][h] < 0.f ? 0.f : v[2 + h] * fac[n][h];
+            }
           }
         }
       rows_sync();
