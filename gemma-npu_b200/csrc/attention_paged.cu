@@ -237,24 +237,36 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
       const int t0 = static_cast<int>(pos - item_pos);
       const int t1 = static_cast<int>(stop - item_pos < nt ? stop - item_pos : nt);
       const int* table = pa.table + b * pa.table_b;
-      // Lane j's box of tile t: its page, or -1 (not a page tile, nothing there that a row sees).
-      auto page_of = [&](int t) {
+      // Lane j's box of tile t: the table's entry if some row needs it, or -1; the page it names; its
+      // scales.  Each is asked for a tile before the next needs it.
+      auto entry_of = [&](int t) {
         if (t >= t1 || kind_of(t) != kPages || lane >= boxes) return -1;
         const int k0 = key0_of(t) + (lane << box_shift);
         if (!paged_needs(pa, span, k0, k0 + box)) return -1;
         const int p = table[k0 >> pa.shift];
-        if (p < 0 || p >= pa.pages) {
+        return p < 0 ? INT32_MAX : p;
+      };
+      struct Page {
+        int at;
+        float ks, vs;
+      };
+      auto page_of = [&](int entry) {
+        Page p = {entry, 0.f, 0.f};
+        if (entry >= pa.pages) {
           atomicExch(&g_tree_status, W8_ERR_INVALID_ARG);
-          return -1;
+          p.at = -1;
         }
+        if (p.at >= 0) p.ks = paged_ks(pa, p.at, c), p.vs = paged_vs(pa, p.at, c);
         return p;
       };
-      int page = page_of(t0);
-      float ks = page >= 0 ? paged_ks(pa, page, c) : 0.f, vs = page >= 0 ? paged_vs(pa, page, c) : 0.f;
+      int entry = entry_of(t0), entry1 = entry_of(t0 + 1);
+      Page page = page_of(entry), next = page_of(entry1);
+      entry = entry_of(t0 + 2);
       for (int t = t0; t < t1 && ok; ++t) {
         const int kind = kind_of(t), key0 = key0_of(t);
-        const int next = page_of(t + 1);
-        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+        const Page after = page_of(entry);
+        entry = entry_of(t + 3);
+        const uint32_t there = __ballot_sync(0xffffffffu, page.at >= 0);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++g) {
           const uint32_t slot = g % NS, dst = base + slot * C::kSlotBytes;
@@ -263,12 +275,12 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
           if (!ok) break;
           if (kind == kPages) {
             // The copies first: the scales, which the barrier's one arrival follows, are yet to come.
-            if (page >= 0)
+            if (page.at >= 0)
               tma_load_5d(dst + lane * (box * D), kv ? &tm_v : &tm_k, full_bar(slot), 0,
-                          (key0 + (lane << box_shift)) & ((1 << pa.shift) - 1), 0, c, page);
+                          (key0 + (lane << box_shift)) & ((1 << pa.shift) - 1), 0, c, page.at);
             if (kv == 0) continue;
             const uint32_t before = (g - 1) % NS;  // (K's slot: its arrival waits for the same loads)
-            if (lane < boxes) scales[before * kPagedMaxBoxes + lane] = ks, scales[slot * kPagedMaxBoxes + lane] = vs;
+            if (lane < boxes) scales[before * kPagedMaxBoxes + lane] = page.ks, scales[slot * kPagedMaxBoxes + lane] = page.vs;
             if (lane == 0) masks[before] = there;
             __syncwarp();
             if (lane == 0) {
@@ -282,8 +294,7 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
           }
           __syncwarp();
         }
-        page = next;
-        if (page >= 0) ks = paged_ks(pa, page, c), vs = paged_vs(pa, page, c);
+        page = next, next = after;
       }
       pos += t1 - t0;
       if (pos >= stop) break;
