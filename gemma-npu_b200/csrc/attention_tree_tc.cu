@@ -36,7 +36,14 @@ constexpr int kTtBN = 128;                 // keys per tile
 constexpr int kTtSoftWarps = 8;
 constexpr int kTtUnpackWarps = 6;          // of a paged cache, in two teams that take its slots in turn
 constexpr int kTtUnpackTeam = kTtUnpackWarps / 2;
-constexpr int kTtScales = 8;               // tiles whose pages' scales are held
+// What the producer makes of a tile's scales, for the softmax threads: of 16 keys each the factor of a
+// score in log2 units, the logarithm of V's scale in O's unit and its reciprocal; then what a change of
+// the unit does to O, the unit, and bits of the 16 keys that are there.
+struct TtScales {
+  float to_log2[8], lg_v[8], rcp_v[8], change, unit;
+  uint32_t there;
+  uint32_t pad;
+};
 __device__ __forceinline__ const TreeArgs& tree_args(const TreeArgs& a) { return a; }
 __device__ __forceinline__ const TreeArgs& tree_args(const PagedArgs& a) { return a.t; }
 constexpr int kTtKeysPerCta = kTtBN / 2;
@@ -63,9 +70,12 @@ struct TtCfg {
   static constexpr int kNumBars = 3 * kSlots + 8 + 2 * kStages;
   static constexpr int kOffXch = kOffBar + kNumBars * 8 + 16;
   static constexpr int kOffPoison = kOffXch + 2 * kTtBM * 4;
-  // Of the last tiles of pages: [key / 16] the scales of K and V, and bits of the 16 keys that are there.
+  // The scales of the tiles from the one in the softmax to the producer's: when it writes those of tile
+  // i + kScales, V_i's slot has been left (the ring holds kSlots steps in the MMAs' order).
+  static constexpr int kScales = kPaged ? (D < 256 ? 8 : 4) : 0;
   static constexpr int kOffScale = kOffPoison + kPoisonWords * 4;
-  static constexpr int kSmem = kOffScale + (kPaged ? kTtScales * (2 * 8 + 1) * 4 : 0) + 1024;
+  static constexpr int kSmem = kOffScale + kScales * static_cast<int>(sizeof(TtScales)) + 1024;
+  static_assert(!kPaged || (kOffScale % 16 == 0 && sizeof(TtScales) % 16 == 0), "alignment");
   static_assert(kKCols == kDV, "K and V slots have one size");
   static_assert(kSmem <= 232448, "shared memory budget exceeded");
   static_assert(kTtBM * (kDV * 4 + 16) <= kOffBar, "the output rows fit over Q and the ring");
@@ -122,8 +132,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
   const uint32_t o_ready = q_full + 8u * 7;
   auto staged_bar = [&](uint32_t s) { return q_full + 8u * (8 + s); };
   auto unpacked_bar = [&](uint32_t s) { return q_full + 8u * (8 + C::kStages + s); };
-  float* const scales = reinterpret_cast<float*>(smem + C::kOffScale);                  // [kTtScales][K, V][8]
-  uint32_t* const there_bits = reinterpret_cast<uint32_t*>(scales + kTtScales * 2 * 8);  // [kTtScales]
+  TtScales* const scales = reinterpret_cast<TtScales*>(smem + C::kOffScale);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();  // 0 = the CTA that issues the MMAs
@@ -310,16 +319,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
       };
       const int kk0 = static_cast<int>(rank) * kTtKeysPerCta;
       const int vb0 = half * (C::kDV / 64) + static_cast<int>(rank) * (C::kDV / 128);
+      float unit = __uint_as_float(0x00800000u);  // of O (2^-126: nothing added yet)
       auto put_k = [&](int i, const Page& page) {
         if (is_page(i)) {
           // The scales first: whoever sees the tile's scores sees them.
-          if (lane < kTtBN / 16) {
-            float* sc = scales + (i % kTtScales) * 16 + lane;
-            sc[0] = page.ks;
-            sc[8] = page.vs;
-          }
+          const float need = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(paged_unit(page.vs))));
+          const float to = fmaxf(unit, need), rcp = paged_unit_rcp(to);
           const uint32_t on = __ballot_sync(0xffffffffu, page.at >= 0);
-          if (lane == 0) there_bits[i % kTtScales] = on;
+          TtScales& out = scales[i % C::kScales];
+          if (lane < kTtBN / 16) {
+            // (Not 0, times which a hidden key's -inf would be NaN, or whose logarithm is -inf: a page's
+            // values may all be 0.  A NaN stays.)
+            const float f = page.ks * a.scale_log2, x = page.vs * rcp, v = x < 0x1p-100f ? 0x1p-100f : x;
+            out.to_log2[lane] = f < 1e-30f ? 1e-30f : f;
+            out.lg_v[lane] = lg2_tc(v);
+            out.rcp_v[lane] = 1.f / v;
+          }
+          if (lane == 0) out.change = unit * rcp, out.unit = to, out.there = on;
+          unit = to;
           __syncwarp();
           for (int s = 0; s < C::kKSlots && ok; ++s)
             put_pages(&tm_k8, page.at, key0_of(i), kk0, kTtKeysPerCta >> box_k, box_k, C::kKCols << box_k, s * C::kKCols);
@@ -621,7 +638,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
               if (a.window > 0 && sk > 0) on |= 0xFFFFFFFFu >> (32 - sk);
               keep[j] = hi < 0 ? 0u : (0xFFFFFFFFu >> (31 - hi)) & on;
               if (is_page(i)) {
-                const uint32_t on16 = there_bits[i % kTtScales] >> (4 * hv + 2 * j);
+                const uint32_t on16 = scales[i % C::kScales].there >> (4 * hv + 2 * j);
                 if (!(on16 & 1u)) keep[j] &= 0xFFFF0000u;
                 if (!(on16 & 2u)) keep[j] &= 0x0000FFFFu;
               }
@@ -643,15 +660,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
 #pragma unroll
           for (int e = 0; e < 64; ++e) m4[e >> 4] = fmaxf(m4[e >> 4], __uint_as_float(sv[e >> 5][e & 31]));
           if (is_page(i)) {
-            // (not 0, times which a hidden key's -inf would be NaN: a page's keys may all be 0)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float f = scales[(i % kTtScales) * 16 + 4 * hv + q] * scale;
-              to_log2[q] = f < 1e-30f ? 1e-30f : f;  // (a NaN stays)
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) to_log2[q] = scale;
+            const float4 f = *reinterpret_cast<const float4*>(&scales[i % C::kScales].to_log2[4 * hv]);
+            to_log2[0] = f.x, to_log2[1] = f.y, to_log2[2] = f.z, to_log2[3] = f.w;
           }
 #pragma unroll
           for (int q = 0; q < 4; ++q) m4[q] *= to_log2[q];
@@ -686,23 +696,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
       const bool move = mt > m + TreeRef<T>::kSlack;
       // O's unit: not below any scale of V so far, 1 from the first 16-bit rows on (the same in all
       // threads of the pair).
-      float vr[4] = {1.f, 1.f, 1.f, 1.f}, to = 1.f;
+      float change = unit;
       if constexpr (kPaged) {
-        if (is_page(i)) {
-          to = unit;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) to = fmaxf(to, paged_unit(scales[(i % kTtScales) * 16 + 8 + q]));
-#pragma unroll
-          for (int q = 0; q < 4; ++q) vr[q] = scales[(i % kTtScales) * 16 + 8 + 4 * hv + q] * paged_unit_rcp(to);
-        }
+        if (is_page(i)) change = scales[i % C::kScales].change;
       }
-      const bool other = kPaged && to != unit;
+      const bool other = kPaged && change != 1.f;
       if (__any_sync(0xffffffffu, move) || other) {
         const float mn = move ? mt - TreeRef<T>::kBelow : m;
         float corr = move ? ex2_tc(m - mn) : 1.f;
         l *= corr;
-        if constexpr (kPaged) corr *= unit * paged_unit_rcp(to);
-        unit = to;
+        if constexpr (kPaged) {
+          corr *= change;
+          unit = is_page(i) ? scales[i % C::kScales].unit : 1.f;
+        }
         if (i > 0) {
           ok = mbar_wait_bounded(pv_done((i - 1) & 1), ((i - 1) >> 1) & 1, abort_flag, &g_tree_status);
           ok = __all_sync(0xffffffffu, ok);
@@ -723,34 +729,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
       }
       const float ref = m == -INFINITY ? 0.f : m;
       float l4[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t pw[32];
       if constexpr (kPaged) {
-        // P in O's unit, the scale of V in the exponent: 2^(x - m + log2 vr); l takes it back, 16 keys
-        // at a time.  (A scale of 0 is 2^-100 here: the values are 0.)
+        // P in O's unit, the scale of V in the exponent: 2^(x - m + log2 v); l takes it back, 16 keys
+        // at a time.
+        float4 lg = make_float4(0.f, 0.f, 0.f, 0.f), rv = make_float4(1.f, 1.f, 1.f, 1.f);
+        if (is_page(i)) {
+          lg = *reinterpret_cast<const float4*>(&scales[i % C::kScales].lg_v[4 * hv]);
+          rv = *reinterpret_cast<const float4*>(&scales[i % C::kScales].rcp_v[4 * hv]);
+        }
+        const float lgs[4] = {lg.x, lg.y, lg.z, lg.w}, rvs[4] = {rv.x, rv.y, rv.z, rv.w};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float odd = to_log2[q] + vr[q];
-          if (odd != odd) {  // a NaN scale is for the rows that see the page (the same in the whole warp)
+        for (int half16 = 0; half16 < 2; ++half16) {
+          uint32_t pw[16];
+#pragma unroll
+          for (int q = 2 * half16; q < 2 * half16 + 2; ++q) {
+            const float odd = to_log2[q] + lgs[q], ref_q = ref - lgs[q];
 #pragma unroll
             for (int e = 8 * q; e < 8 * q + 8; ++e) {
-              const bool on0 = __uint_as_float(sv[e >> 4][(2 * e) & 31]) != -INFINITY;
-              const bool on1 = __uint_as_float(sv[e >> 4][(2 * e + 1) & 31]) != -INFINITY;
-              pw[e] = pack2<T>(on0 ? odd : 0.f, on1 ? odd : 0.f);
-              if (on0 || on1) l4[q] = odd;
+              const float x0 = __uint_as_float(sv[e >> 4][(2 * e) & 31]), x1 = __uint_as_float(sv[e >> 4][(2 * e + 1) & 31]);
+              const float p0 = ex2_tc(fmaf(x0, to_log2[q], -ref_q)), p1 = ex2_tc(fmaf(x1, to_log2[q], -ref_q));
+              l4[q] += p0 + p1;
+              pw[e & 15] = pack2<T>(p0, p1);
             }
-            continue;
-          }
-          const float v = fmaxf(vr[q], 0x1p-100f), ref_q = ref - lg2_tc(v);
+            l4[q] *= rvs[q];
+            if (odd != odd) {  // a NaN scale is for the rows that see the page (the same in the whole warp)
+              l4[q] = 0.f;
 #pragma unroll
-          for (int e = 8 * q; e < 8 * q + 8; ++e) {
-            const float p0 = ex2_tc(fmaf(__uint_as_float(sv[e >> 4][(2 * e) & 31]), to_log2[q], -ref_q));
-            const float p1 = ex2_tc(fmaf(__uint_as_float(sv[e >> 4][(2 * e + 1) & 31]), to_log2[q], -ref_q));
-            l4[q] += p0 + p1;
-            pw[e] = pack2<T>(p0, p1);
+              for (int e = 8 * q; e < 8 * q + 8; ++e) {
+                const bool on0 = __uint_as_float(sv[e >> 4][(2 * e) & 31]) != -INFINITY;
+                const bool on1 = __uint_as_float(sv[e >> 4][(2 * e + 1) & 31]) != -INFINITY;
+                pw[e & 15] = pack2<T>(on0 ? odd : 0.f, on1 ? odd : 0.f);
+                if (on0 || on1) l4[q] = odd;
+              }
+            }
           }
-          l4[q] *= 1.f / v;
+          tmem_st_32x32b_x16(tmem + lane_off + u * kTtBN + 32 * hv + 16 * half16, pw);
         }
       } else {
+        uint32_t pw[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const float p0 = ex2_tc(fmaf(__uint_as_float(sv[e >> 4][(2 * e) & 31]), scale, -ref));
@@ -758,8 +774,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
           l4[e & 3] += p0 + p1;
           pw[e] = pack2<T>(p0, p1);
         }
+        tmem_st_32x32b_x32(tmem + lane_off + u * kTtBN + 32 * hv, pw);
       }
-      tmem_st_32x32b_x32(tmem + lane_off + u * kTtBN + 32 * hv, pw);
       l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
       if (care) {
         // This CTA's columns of V: rows behind the length read as zeros, and of new tokens
