@@ -18,13 +18,22 @@
 // when it crosses u_0, and the boundaries' errors add up.  In fp32 (about 1e-8 each) one draw in
 // a thousand would differ, so what is drawn from is computed in 64 bits: 2^x from a table of 32
 // and a polynomial of degree 5 (P. T. P. Tang, "Table-driven implementation of the exponential
-// function in IEEE floating-point arithmetic", ACM TOMS 15(2), 1989), 14 operations a value, good
-// to 2^-50, and sums in double.
+// function in IEEE floating-point arithmetic", ACM TOMS 15(2), 1989), 10 operations a value, good
+// to 2^-48, and sums in double.
+//
+// After k rejections w is max(p - c q, 0) / Z with one c: of max(p - c q, 0) / Z less q, what is
+// positive is max(p - (c + Z) q, 0).  So nothing is stored: a rejection costs one pass over both rows,
+// which gives Z, and by warps' chunks what the draw then needs to find its token.
+//
+// What bounds it: the 64-bit operations of the passes (an SM has 62 a clock) and, for short walks, the
+// chain of a node (its children, a pass, two meetings of the cluster: some 4 us).  One chain of 5 drafts
+// over 262144 values takes 25 us; 24 trees take 195, as long as their longest walk.
 #include "common.cuh"
 
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 namespace w8 {
@@ -746,6 +755,8 @@ static int verify_launch(Kern kern, int (&held)[64][w8::kVerifyCluster + 1], w8:
   cfg.attrs = attr;
   // Clusters of each size that the device holds at once: its SMs come in groups, which clusters do not
   // cross (15 clusters of 8 or of 9, 22 of 6, 26 of 5).
+  static std::mutex filling;
+  std::unique_lock<std::mutex> lock(filling);
   if (held[device][1] == 0) {
     W8_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cfg.numAttrs = 1;
@@ -760,6 +771,7 @@ static int verify_launch(Kern kern, int (&held)[64][w8::kVerifyCluster + 1], w8:
       held[device][c] = c == 1 ? std::max(n, 1) : n;
     }
   }
+  lock.unlock();
   // CTAs of a sequence: the most with which all sequences run at once (64 bits keep an SM's pipes busy,
   // and a second wave would double the time), each with at least 2048 values.
   int cluster = 1;
