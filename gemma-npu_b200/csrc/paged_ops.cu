@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t paged_divide(float x, float m) {
 // Eight such bytes.  A product with the reciprocal (off by less than 127 2^-22) decides all but what is
 // near a half; adding 1.5 2^23 leaves the integer in the sum's low bits, without a conversion
 // (those and the rounding instruction have an eighth of an addition's rate: 47 us with them where
-// this takes PLACEHOLDER).
+// this takes 31).
 __device__ __forceinline__ uint2 paged_round8(const float (&x)[8], float m, float r, bool slow) {
   constexpr float kBig = 12582912.f;
   float far = 0.f;
@@ -100,8 +100,9 @@ __device__ __forceinline__ uint2 paged_round8(const float (&x)[8], float m, floa
 // first partial one: filled from the tail (the first page only) and the new rows, its largest
 // magnitude found and its values rounded from the registers, if the call fills it.  CTA 0 then
 // writes the rows that stay in the tail, which are all new: the tail's old rows, if the page was
-// filled, are read before.  Bound by HBM for prompts (2 bytes read, 1 written a value: 13,000
-// tokens of 8 heads of 128 take PLACEHOLDER) and by the chain length, table, row for a token.
+// filled, are read before.  Bound by the issue of its arithmetic for prompts (some 20 instructions a value of 2
+// bytes read and 1 written: 4 prompts of 400 to 4000 tokens, 8 heads of 128, take 31 us where the
+// bytes alone would take 12) and by the chain length, table, row for a token (3.1 us for 8 sequences).
 template <typename T, int kVecs>
 __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedAppendArgs a) {
   __shared__ int sm_took;
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(32 * kCountWarps) page_count_kernel(const Assi
 
 // One cluster for the whole table, each CTA a contiguous range of requests, a warp a request.
 // What goes back and what is missing is counted (of more than 16384 entries by page_count_kernel on
-// all SMs: 512 tables of 2048 take PLACEHOLDER where this cluster alone took 25), prefix sums (over a
+// all SMs: for 512 tables of 2048 a call takes 13 us where this cluster alone took 25), prefix sums (over a
 // CTA's requests, then the cluster's CTAs) give every request its place in the stack, and a
 // second pass, over the entries between a request's first and last change only, moves the pages:
 // first all that go back, then, behind a barrier of the cluster, those that are given out.
@@ -353,6 +354,7 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
   const int b1 = static_cast<int>(static_cast<int64_t>(a.batch) * (rank + 1) / ranks);
   const int count = b1 - b0;
   if (tid == 0) given = 0;
+  cluster_started();
   pdl_launch_dependents();
   pdl_wait();
   const int top0 = *a.top;
@@ -390,6 +392,7 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
     if (w < warp) xb += scan[0][w], xm += scan[1][w];
     tb += scan[0][w], tm += scan[1][w];
   }
+  cluster_all_started();
   if (tid < static_cast<int>(ranks))
     st_cluster_u64(mapa_shared(smem_u32(&sums[0][rank]), tid),
                    static_cast<unsigned long long>(static_cast<uint32_t>(tb)) << 32 | static_cast<uint32_t>(tm));
@@ -529,6 +532,10 @@ extern "C" int w8_paged_append(const w8_paged_append_args* in, w8_stream_t strea
       W8_CHECK_ARG(!arrays_meet(x.path + b * x.path_stride, x.steps, x.lens_out, x.batch), "lens_out must not overlap path");
   W8_CHECK_ARG(x.pages == 0 || (x.k && x.v && x.k_scale && x.v_scale), "null pages");
   W8_CHECK_ARG(x.table_pages == 0 || x.table, "null table");
+  if (x.table_pages > 0 && arrays_meet(x.table, (x.batch - 1) * x.table_stride + x.table_pages, x.lens_out, x.batch))
+    for (int64_t b = 0; b < x.batch; ++b)  // (it may lie between the rows)
+      W8_CHECK_ARG(!arrays_meet(x.table + b * x.table_stride, x.table_pages, x.lens_out, x.batch),
+                   "lens_out must not overlap table");
   const void* ptrs[6] = {x.k_tail, x.v_tail, x.k_new, x.v_new, x.k, x.v};
   const int64_t* strides[6] = {x.k_tail_stride, x.v_tail_stride, x.k_new_stride, x.v_new_stride, x.k_stride, x.v_stride};
   const int64_t sizes[6][3] = {{x.batch, x.kv_heads, x.page},  {x.batch, x.kv_heads, x.page},
@@ -612,7 +619,7 @@ extern "C" int w8_page_assign(const w8_page_assign_args* in, void* workspace, in
   constexpr int64_t kMost = static_cast<int64_t>(w8::kAssignRequests) * w8::kAssignCluster;
   W8_CHECK_ARG(x.batch <= kMost, "more than %lld requests", (long long)kMost);
   W8_CHECK_ARG(x.table_pages < (1ll << 30) / x.page && x.room < (1ll << 30) && x.free_pages < (1ll << 30) &&
-                   x.batch * x.table_pages < (1ll << 31),
+                   x.batch * x.table_pages < (1ll << 30),
                "size beyond the limits");
   if (x.batch == 0) return W8_OK;
   W8_CHECK_ARG(x.lens && x.top && x.ok && (x.free_pages == 0 || x.free) && (x.table_pages == 0 || x.table), "null pointer");

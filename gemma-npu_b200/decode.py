@@ -26,11 +26,12 @@ layout that `kernels.qkv_norm_rope` returns: for B sequences of N tokens,
 `q.unflatten(1, (B, N)).transpose(0, 1)` is the [B, H, N, D] view.
 
 A paged 8-bit cache (of one layer) is a pool of pages k, v int8 [pages, KV, P, D] with scales
-k_scale, v_scale fp32 [pages, KV] (a value is its 8 bits times its page's and head's scale), P =
-16, 32, 64 or 128, and the 16-bit rows of every sequence's last, partial page, k_tail, v_tail
-[B, KV, P, D].  table int32 [B, M] names a sequence's pages in order (negative: none), lens
-int32 [B] counts its positions: position p is row p % P of page table[b, p // P], or of the
-tail where p >= lens // P * P.  Table and lengths are shared by layers of one kind.
+k_scale, v_scale fp32 [pages, KV] (a value is its 8 bits times its page's and head's scale,
+which is not negative), P = 16, 32, 64 or 128, and the 16-bit rows of every sequence's last,
+partial page, k_tail, v_tail [B, KV, P, D].  table int32 [B, M] names a sequence's pages in
+order (negative: none), lens int32 [B] counts its positions: position p is row p % P of page
+table[b, p // P], or of the tail where p >= lens // P * P.  Table and lengths are shared by
+layers of one kind.
 
 Like every function of `kernels`, these check dtype, shape and layout on the host, run on
 torch's current stream of the tensors' device, copy nothing to the host and raise a W8Error
@@ -218,8 +219,8 @@ def paged_append(k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_n
     They wait in the tail as they are; a page that becomes full is rounded to 8 bits at once, per
     head: scale = m / 127 for its largest magnitude m, values round(127 x / m), halves to even.  A
     page with an infinity or a NaN gets a scale of NaN.  The page must be in the table
-    (`page_assign`): one that is not is lost and reported by `device_status`.  Returns lens_out
-    int32 [B] (a tensor apart from lens, path and count).  k_new and v_new must not overlap the
+    (`page_assign`), and there only once: one that is not is lost and reported by `device_status`.
+    Returns lens_out int32 [B] (a tensor apart from lens, path, count and table).  k_new and v_new must not overlap the
     cache."""
     return (_binding or _c()).paged_append(k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_new, path,
                                            count, lens_out)

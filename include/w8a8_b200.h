@@ -411,7 +411,7 @@ int w8_cache_reorder(void* const* tensors, int64_t count, const int64_t* strides
 /* The keys and values of a position whose page is full are signed 8-bit values of one scale a
  * page and cache head; the positions of a sequence's last, partial page are 16-bit rows of its
  * tail.  Position p < lens[b] / page * page of sequence b is row p % page of the pool's page
- * table[b, p / page], a later one row p % page of tail b. */
+ * table[b, p / page], a later one row p % page of tail b.  Scales are not negative. */
 typedef struct w8_attention_paged_args {
   const void* q;                  /* [batch, heads, n_new] rows of head_dim */
   const int8_t *k, *v;            /* pool: [pages, kv_heads, page] rows of head_dim bytes */
@@ -453,7 +453,7 @@ typedef struct w8_paged_append_args {
   const void *k_new, *v_new;     /* [batch, kv_heads, n_new] rows of head_dim */
   const int32_t* path;           /* [batch, steps] indexes of new tokens, ended by a negative one; NULL: in order */
   const int32_t* count;          /* [batch]: at most so many of them; NULL: all */
-  int32_t* lens_out;             /* [batch], of no memory in common with lens, path or count */
+  int32_t* lens_out;             /* [batch], of no memory in common with lens, path, count or table */
   int64_t k_stride[3], v_stride[3], k_scale_stride[2], v_scale_stride[2]; /* elements */
   int64_t k_tail_stride[3], v_tail_stride[3], k_new_stride[3], v_new_stride[3];
   int64_t table_stride, path_stride;
@@ -466,7 +466,7 @@ typedef struct w8_paged_append_args {
  * halves to even, from the 16-bit rows; the rows behind the last full page go into the tail.  A
  * page with an infinity or a NaN gets a scale of NaN.  A page that the table does not have is lost
  * and reported by w8_device_status, and so are positions behind the table.  The new rows must not
- * overlap the pages and tails, and no page may stand in the table twice. */
+ * overlap the pages and tails, and a page that the call fills may stand in the table only once. */
 int w8_paged_append(const w8_paged_append_args* args, w8_stream_t stream);
 
 typedef struct w8_page_assign_args {
@@ -486,7 +486,7 @@ typedef struct w8_page_assign_args {
  * then the missing ones are given out in the same order from its top.  A request is served if
  * what it and all requests before it miss is there; one that misses nothing is, and one that
  * needs more pages than a table has is not and does not count.  A request whose length is out of
- * range keeps what it has.  At most 8192 requests. */
+ * range keeps what it has.  At most 8192 requests, and 2^30 entries in all. */
 int w8_page_assign(const w8_page_assign_args* args, void* workspace, int64_t workspace_bytes, w8_stream_t stream);
 /* Workspace in bytes (16-byte aligned). */
 int64_t w8_page_assign_workspace_bytes(int64_t batch, int64_t table_pages);

@@ -98,10 +98,11 @@ def test_append_refuses(change, status):
 
 
 def test_append_lens_out_stands_apart():
-    """What one CTA writes to lens_out another may yet read from lens, count or path."""
+    """What one CTA writes to lens_out another may yet read from lens, count, path or the table."""
     at = 4096 * (list(APPEND).index("lens_out") + 1)
     for kw in (dict(lens=at), dict(lens=at + 4), dict(lens=at - 12), dict(count=at), dict(count=at - 4), dict(path=at),
-               dict(path=at - 4, path_stride=100, steps=2), dict(path=at - 3 * 400 - 4, path_stride=100)):
+               dict(path=at - 4, path_stride=100, steps=2), dict(path=at - 3 * 400 - 4, path_stride=100),
+               dict(table=at), dict(table=at - 3 * 400, table_stride=100)):
         assert run("w8_paged_append", batch=4, **kw) == BAD, kw
         assert b"lens_out" in _lib.lib().w8_last_error()
 
@@ -110,6 +111,7 @@ def test_append_lens_out_stands_apart():
     (dict(batch=-1), BAD), (dict(batch=8193), BAD), (dict(page=33), UNSUPPORTED), (dict(room=-1), BAD), (dict(window=-1), BAD),
     (dict(sink=2), BAD), (dict(lens=0), BAD), (dict(top=0), BAD), (dict(free=0), BAD), (dict(table=0), BAD), (dict(ok=0), BAD),
     (dict(table_stride=3), BAD), (dict(top=8192), BAD), (dict(lens=4096), BAD), (dict(free=4096 + 8), BAD),
+    (dict(batch=8192, table_pages=1 << 17, table_stride=1 << 17, free=0), BAD),
     (dict(batch=100, table_pages=1000, table_stride=1000, free=1 << 30, top=1 << 31, lens=1 << 32), BAD)])
 def test_assign_refuses(change, status):
     assert run("w8_page_assign", **change) == status
