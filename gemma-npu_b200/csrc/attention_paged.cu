@@ -10,22 +10,31 @@
 //
 // Decode reads each key once for few rows and is bound by HBM, at half the bytes of a 16-bit
 // cache, so the unpacking has to keep up with 23 values a clock and SM.  Both products run as
-// fp16 mma.sync with fp32 sums.  A thread's 4 neighbouring bytes become 4 fp16 values in 5
-// instructions (paged_unpack, exact), and are one B operand of 16 x 8 as they are if the order
-// of the reduction is permuted alike on both sides: the columns of Q when it is staged for K,
-// and for V the columns of the output, which a thread then holds as 4 neighbours (`natural`
-// puts them back in order, once an item).  Q is scaled by a power of two a row into fp16's range
-// (largest element 2^14: what falls below 2^-24 is 2^-38 of that).  ks multiplies the scores; vs
-// goes into P relative to a power of two not below any vs so far (paged_unit), in which unit O is
-// held: O is rescaled when that grows or a row's maximum does, and P is rounded to fp16, half a
-// step of 2^-11 on each weight (TreeRef has the range).
+// fp16 mma.sync with fp32 sums, the cache as the 16-row operand and the query rows as the 8
+// columns: S^T = K Q^T, O^T = V^T P^T.  (The other way round few rows would fill half of the 16
+// and twice the instructions would be issued for them: 136 us where this took 91.)  ldmatrix
+// brings 8-bit rows as pairs of bytes, of which a thread makes fp16 pairs without a conversion: V
+// exactly (paged_unpack), K as 1152 + k8 (paged_raise, an instruction less a pair), whose 1152 times
+// the sum of the row's q the scores start from with the opposite sign.  The order of the reduction
+// is permuted alike on both sides, in Q when it is staged and in O's columns, which `natural` puts
+// back for the 16-bit tiles and the result.  P^T is the second product's operand after movmatrix.
+// Q is scaled by a power of two a row into fp16's range (largest element 2^14: what falls below
+// 2^-24 is 2^-38 of that).  ks multiplies the scores; vs goes into P relative to a power of two not
+// below any vs so far (paged_unit), in which unit O is held: O is rescaled when that grows or a
+// row's maximum does, and P is rounded to fp16, half a step of 2^-11 on each weight (TreeRef has
+// the range).
 //
 // The schedule is attention_tree.cu's: all tiles of all sequences dealt in equal contiguous
-// ranges to the CTAs, each of 8 warps 16 keys at a time with a running softmax of its own, joined
-// at the end of an item; pieces joined by attn_tree_combine_kernel.  A ninth warp walks the page
+// ranges to the CTAs, each of 8 warps 16 or (D <= 128: 91 -> 72 us) 32 keys at a time with a running
+// softmax of its own, joined at the end of an item; pieces joined by attn_tree_combine_kernel.  A ninth warp walks the page
 // table ahead, a page a lane: TMA boxes of a page's rows into the ring, and its scales.  Pages
 // that no row sees are not read (nor their table entries followed), so a window's old pages may
 // be gone.
+//
+// 32 sequences of 2000 to 8191 tokens, 8 cache heads of 128, 4 query heads each: 69 us, 74% of what a
+// copy moves, of which reading alone takes 62; what is left is the unpacking (some 9 instructions
+// for 4 values and both products) that no longer hides behind the loads.  One sequence of one
+// token is a chain (table, page, join, combine): 15 us for 3658 keys of 512.
 #include "attention_paged.cuh"
 #include "attn_mma.cuh"
 #include "attn_tc.cuh"
@@ -394,7 +403,7 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
     }
     rows_sync();
     // A row's reference: no maximum yet is kNone, which every score exceeds.
-    constexpr float kNone = -1e30f;
+    constexpr float kNone = -3e38f;
     float m[NT][2], l[NT][2], fac[NT][2];
     float o[NT][D / 16][4];  // O transposed: columns gl and gl + 8 of 16 (or 2 gl and 2 gl + 1), rows 2 tl, 2 tl + 1
     float qsum[NT][2];

@@ -484,7 +484,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
     if constexpr (kPaged) {
       // ---- unpacking: a staging slot's 16 bytes a thread to 32 in the ring's slot, in the MMA order.  A
       // release to the cluster drains a thread's stores first, some 1000 clocks: two teams of warps
-      // take the staging slots in turn, so that one unpacks while the other waits (PLACEHOLDER).
+      // take the staging slots in turn, so that one unpacks while the other waits.
       const int team = (warp - 2 - kTtSoftWarps) / kTtUnpackTeam;
       const int tid = threadIdx.x - 32 * (2 + kTtSoftWarps + team * kTtUnpackTeam);
       static_assert(C::kStages % 2 == 0, "a staging slot is one team's");

@@ -305,6 +305,22 @@ def test_attention_lengths_out_of_range(cuda):
     assert bool(got.eq(attend(c, *a, scale=0.125)).all()) and w8.device_status() == 0
 
 
+@pytest.mark.parametrize("H,N", [(2, 2), (6, 4)])
+def test_attention_scores_far_below_zero(cuda, H, N):
+    """Few rows, scores of -2^106 and less, powers of two that fp32 holds: the largest have all the weight."""
+    D, P, lens = 64, 16, [37, 20]
+    c = cache(3, 2, D, P, lens)
+    q, kn, vn = new(3, 2, H, 2, D, N, torch.bfloat16)
+    q[:] = 2.0 ** 60
+    for x in ("k", "k_tail"):
+        c[x][:] = (-(2 ** (torch.arange(P, device="cuda") % 5)))[:, None].to(c[x].dtype)
+    c["k_tail"] *= 2.0 ** 40
+    c["k_scale"][:] = 2.0 ** 40
+    kn[:] = -2.0 ** 41
+    o, _, pv = want_attention(c, q, kn, vn)
+    check_out(attend(c, q, kn, vn), (o, 2.0 ** -20 * pv + 2.0 ** -18 * float(pv.max()), pv), torch.bfloat16)
+
+
 def test_attention_offsets_beyond_32_bits(cuda):
     """A pool of more than 2^31 bytes, its last pages in use."""
     pages, P, D = 66000, 128, 256
