@@ -45,6 +45,9 @@ struct TtScales {
   uint32_t pad;
 };
 __device__ __forceinline__ const TreeArgs& tree_args(const TreeArgs& a) { return a; }
+struct TtPagedArgs : PagedArgs {
+  CUtensorMap k8, v8;  // the pool's
+};
 __device__ __forceinline__ const TreeArgs& tree_args(const PagedArgs& a) { return a.t; }
 constexpr int kTtKeysPerCta = kTtBN / 2;
 constexpr uint32_t kTtTmemCols = 512;
@@ -59,22 +62,24 @@ struct TtCfg {
   static constexpr int kKCols = D < 256 ? D : 256;        // columns of the reduction per K slot
   static constexpr int kKSlots = D / kKCols;              // slots per K tile
   static constexpr int kSlotBytes = kTtBN * kDV;          // K: 64 keys x kKCols; V: 128 keys x kDV / 2
-  static constexpr int kSlots = kPaged ? (D == 512 ? 2 : D == 256 ? 4 : 8) : D == 512 ? 3 : D == 256 ? 5 : 8;
+  static constexpr int kSlots = kPaged ? (D == 512 ? 2 : D == 256 ? 3 : 8) : D == 512 ? 3 : D == 256 ? 5 : 8;
   static constexpr int kStageBytes = kSlotBytes / 2;      // a slot's values while they are 8 bits
-  static constexpr int kStages = kPaged ? (D < 256 ? 4 : 2) : 0;
+  static constexpr int kStages = kPaged ? (D == 512 ? 2 : 4) : 0;
   static constexpr int kOffRing = kQBytes;
   static constexpr int kOffStage = kOffRing + kSlots * kSlotBytes;
   static constexpr int kOffBar = kOffStage + kStages * kStageBytes;
   // full[kSlots], empty[kSlots], own[kSlots], q_full, s_full[2], p_full[2], pv_done[2], o_ready,
   // staged[kStages], unpacked[kStages]
   static constexpr int kNumBars = 3 * kSlots + 8 + 2 * kStages;
-  static constexpr int kOffXch = kOffBar + kNumBars * 8 + 16;
+  static constexpr int kOffXch = kOffBar + (kNumBars * 8 + 31) / 16 * 16;
   static constexpr int kOffPoison = kOffXch + 2 * kTtBM * 4;
-  // The scales of the tiles from the one in the softmax to the producer's: when it writes those of tile
-  // i + kScales, V_i's slot has been left (the ring holds kSlots steps in the MMAs' order).
-  static constexpr int kScales = kPaged ? (D < 256 ? 8 : 4) : 0;
+  // The scales of the tiles from the one in the softmax to the producer's.  It writes those of tile j when
+  // the staging slot of K_j's first step is free: the step kStages before has been unpacked, so the ring's
+  // slot of the step kSlots before that had been left.  Steps are K_0 K_1 V_0 K_2 V_1 ..; that one is V_j-5
+  // (D = 256), V_j-3 (512), or K_j-6 (S_j-6 follows P_j-8's product).
+  static constexpr int kScales = kPaged ? (D < 256 ? 8 : D == 256 ? 5 : 4) : 0;
   static constexpr int kOffScale = kOffPoison + kPoisonWords * 4;
-  static constexpr int kSmem = kOffScale + kScales * static_cast<int>(sizeof(TtScales)) + 1024;
+  static constexpr int kSmem = kOffScale + kScales * static_cast<int>(sizeof(TtScales)) + 1008;  // (shared memory begins on 16 bytes)
   static_assert(!kPaged || (kOffScale % 16 == 0 && sizeof(TtScales) % 16 == 0), "alignment");
   static_assert(kKCols == kDV, "K and V slots have one size");
   static_assert(kSmem <= 232448, "shared memory budget exceeded");
@@ -100,9 +105,9 @@ __device__ __forceinline__ void red_or_cluster(uint32_t addr, uint32_t bits) {
 // DR: columns of a head in memory.  Heads of 64 run as 128 whose upper half the boxes fill with
 // zeros (S and O do not change, and only the lower half is stored): the MMAs do twice their work
 // and 216 row tiles of 680 rows over 1085 keys take 194 us where mma.sync took 626.
-// Over a paged 8-bit cache (kPaged; tm_k and tm_v then are the tails' and tm_k8, tm_v8 the pool's):
-// each CTA's share of a tile's pages comes by TMA as it is into a staging slot, and two warps
-// unpack it to T into the ring's slot, which is exact; the scale of K multiplies the scores, that of
+// Over a paged 8-bit cache (kPaged; tm_k and tm_v then are the tails'): each CTA's share of a tile's
+// pages comes by TMA as it is into a staging slot, and a team of three warps unpacks it to T into
+// the ring's slot, which is exact; the scale of K multiplies the scores, that of
 // V goes into P relative to a power of two, in which O is held (paged_unit; the first tile of 16-bit
 // rows brings it to 1).  Pages are never careful: 8-bit values are finite, whatever they are.
 template <typename T, int D, int DR, bool kPaged, typename Args>
@@ -110,7 +115,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
     attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_vn,
-                        const __grid_constant__ CUtensorMap tm_k8, const __grid_constant__ CUtensorMap tm_v8,
                         const __grid_constant__ Args args) {
   using C = TtCfg<D, kPaged>;
   const TreeArgs& a = tree_args(args);
@@ -171,8 +175,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
     prefetch_tmap(&tm_kn);
     prefetch_tmap(&tm_vn);
     if constexpr (kPaged) {
-      prefetch_tmap(&tm_k8);
-      prefetch_tmap(&tm_v8);
+      prefetch_tmap(&args.k8);
+      prefetch_tmap(&args.v8);
     }
   }
   if (threadIdx.x < kPoisonWords) reinterpret_cast<uint32_t*>(smem + C::kOffPoison)[threadIdx.x] = 0u;
@@ -219,7 +223,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
     }
     return (t0 + i >= nc ? t0 + i - nc : span.c0 + t0 + i) * kTtBN;
   };
-  const int sink_left = a.sink - len;  // (negative or 0 without sinks: len >= 0)
+  const int sink_left = kPaged ? a.sink - len : 0;  // (negative or 0 without sinks: len >= 0)
   // Of a causal chunk's tiles of new tokens, those that every row of the pair sees whole are as
   // plain as committed ones.
   const int tok_lo = rt * (2 * kTtBM) / a.group, tok_hi = (min((rt + 1) * (2 * kTtBM), rows) - 1) / a.group;
@@ -299,13 +303,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
         __syncwarp();
         ++g;
       };
+      auto wait_stage = [&]() {  // (the ring's slot is the unpacking warps' to wait for)
+        ok = ok && wait_phase(unpacked_bar(st % C::kStages), ((st / C::kStages) & 1u) ^ 1u, abort_flag, &g_tree_status);
+        ok = __all_sync(0xffffffffu, ok);
+        return ok;
+      };
       // `n` boxes of 2^shift keys from key `from` of the tile and column x into the next staging slot.
       auto put_pages = [&](const CUtensorMap* m, int page, int key0, int from, int n, int shift, int bytes, int x) {
-        if (!wait_slot()) return;
+        if (!wait_stage()) return;
         const uint32_t s = st % C::kStages;
-        ok = wait_phase(unpacked_bar(s), ((st / C::kStages) & 1u) ^ 1u, abort_flag, &g_tree_status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
         const int mine = __shfl_sync(0xffffffffu, page, (from + (lane << shift)) / 16 & 31);
         const bool on = lane < n && mine >= 0;
         const int count = __popc(__ballot_sync(0xffffffffu, on));
@@ -322,6 +328,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
       float unit = __uint_as_float(0x00800000u);  // of O (2^-126: nothing added yet)
       auto put_k = [&](int i, const Page& page) {
         if (is_page(i)) {
+          if (!wait_stage()) return;
           // The scales first: whoever sees the tile's scores sees them.
           const float need = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(paged_unit(page.vs))));
           const float to = fmaxf(unit, need), rcp = paged_unit_rcp(to);
@@ -339,8 +346,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
           unit = to;
           __syncwarp();
           for (int s = 0; s < C::kKSlots && ok; ++s)
-            put_pages(&tm_k8, page.at, key0_of(i), kk0, kTtKeysPerCta >> box_k, box_k, C::kKCols << box_k, s * C::kKCols);
+            put_pages(&args.k8, page.at, key0_of(i), kk0, kTtKeysPerCta >> box_k, box_k, C::kKCols << box_k, s * C::kKCols);
         } else {
+          // A slot's barrier must be at most one phase behind the one that is waited for.  Pages leave the
+          // ring to the unpacking warps: once those have placed the last ones, it is.
+          for (uint32_t d = 1; d <= 2 && d <= st; ++d) {
+            ok = ok && wait_phase(unpacked_bar((st - d) % C::kStages), ((st - d) / C::kStages) & 1u, abort_flag, &g_tree_status);
+            ok = __all_sync(0xffffffffu, ok);
+          }
           for (int s = 0; s < C::kKSlots && ok; ++s)
             put(is_draft(i) ? &tm_kn : &tm_k, key0_of(i) + kk0, s * (C::kKCols / 64), false);
         }
@@ -350,8 +363,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
         tma_load_5d_pair(base, &tm_q, mapa_shared(q_full, 0), 0, c * a.group, row0 / a.group, 0, b);
       }
       __syncwarp();
-      Page page = page_of(entry_of(0)), next = page_of(entry_of(1));  // of this tile and the next
-      int entry = entry_of(2);
+      int entry = entry_of(0);
+      const int entry1 = entry_of(1);
+      const int entry2 = entry_of(2);
+      Page page = page_of(entry), next = page_of(entry1);  // of this tile and the next
+      entry = entry2;
       put_k(0, page);
       for (int i = 0; i < ntiles && ok; ++i) {
         const Page after = page_of(entry);
@@ -359,7 +375,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
         if (i + 1 < ntiles) put_k(i + 1, next);
         if (!ok) break;
         if (is_page(i))
-          put_pages(&tm_v8, page.at, key0_of(i), 0, kTtBN >> box_v, box_v, (C::kDV / 2) << box_v, vb0 * 64);
+          put_pages(&args.v8, page.at, key0_of(i), 0, kTtBN >> box_v, box_v, (C::kDV / 2) << box_v, vb0 * 64);
         else
           put(is_draft(i) ? &tm_vn : &tm_v, key0_of(i), vb0, careful(i));
         page = next, next = after;
@@ -497,35 +513,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
           return;
         }
         const uint32_t slot = g % C::kSlots, s = st % C::kStages;
+        // (in this order: what was put before this step, 16-bit rows among it, has waited for the ring)
         if (ok) ok = mbar_wait_bounded(staged_bar(s), (st / C::kStages) & 1u, abort_flag, &g_tree_status);
+        if (ok) ok = wait_phase(empty_bar(slot), ((g / C::kSlots) & 1u) ^ 1u, abort_flag, &g_tree_status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
         const uint32_t from = base + C::kOffStage + s * C::kStageBytes, to = ring + slot * C::kSlotBytes;
         // K: [64 keys x kKCols], V: [128 keys x kDV / 2], both of half a slot.
         constexpr int chunks = decltype(columns)::value / 16, keys = C::kStageBytes / 16 / chunks;
-        constexpr int kAll = C::kStageBytes / 16, kStep = 32 * kTtUnpackTeam, kBatch = 4;
+        constexpr int kStep = 32 * kTtUnpackTeam / chunks;  // a thread's chunk of every kStep-th row
+        static_assert(32 * kTtUnpackTeam % chunks == 0, "a thread stays in its columns");
+        const int ch = tid % chunks, r0 = tid / chunks;
+        const uint32_t dst = to + (ch >> 2) * (keys * 128);
+        // (Short code: several rows' loads ahead of their stores cost more, in instructions, than the waits.)
 #pragma unroll 1
-        for (int e0 = tid; e0 < kAll; e0 += kBatch * kStep) {
-          uint32_t x[kBatch][4];  // (all loads before the first store)
+        for (int row = r0; row < keys; row += kStep) {
+          uint32_t x[4], y[8];
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(from + (row * chunks + ch) * 16)
+                       : "memory");
 #pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            const int e = min(e0 + k * kStep, kAll - 1);
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(x[k][0]), "=r"(x[k][1]), "=r"(x[k][2]), "=r"(x[k][3])
-                         : "r"(from + e * 16)
-                         : "memory");
-          }
-#pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            const int e = e0 + k * kStep, row = e / chunks, ch = e % chunks;
-            if (e >= kAll) break;
-            uint32_t y[8];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) paged_unpack<T>(x[k][q], 0x4140u, 0x4342u, y[2 * q], y[2 * q + 1]);
-            const uint32_t line = to + (ch >> 2) * (keys * 128) + row * 128;
-            st_shared_v4(line + (((2 * ch & 7) ^ (row & 7)) << 4), y[0], y[1], y[2], y[3]);
-            st_shared_v4(line + (((2 * ch + 1 & 7) ^ (row & 7)) << 4), y[4], y[5], y[6], y[7]);
-          }
+          for (int q = 0; q < 4; ++q) paged_unpack<T>(x[q], 0x4140u, 0x4342u, y[2 * q], y[2 * q + 1]);
+          const uint32_t at = dst + row * 128 + (((2 * ch & 7) ^ (row & 7)) << 4);
+          st_shared_v4(at, y[0], y[1], y[2], y[3]);
+          st_shared_v4(at ^ 16u, y[4], y[5], y[6], y[7]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -556,6 +568,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
     volatile float* xch = reinterpret_cast<volatile float*>(smem + C::kOffXch);
     const volatile uint32_t* poison = reinterpret_cast<const volatile uint32_t*>(smem + C::kOffPoison);
     auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
+    auto pair_any = [&](bool on) {
+      uint32_t any;
+      __syncwarp();
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.u32 q, %1, 0;\n\t"
+          "bar.red.or.pred p, %2, 64, q;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(any)
+          : "r"(on ? 1u : 0u), "r"(1 + quarter)
+          : "memory");
+      return any != 0u;
+    };
     auto softmax_sync = [&]() { asm volatile("bar.sync 5, %0;" ::"n"(32 * kTtSoftWarps) : "memory"); };
 
     // Q rows that no TMA box describes (128 rows are whole tokens only for a group that divides
@@ -617,43 +642,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
         tmem_ld_32x32b_x32(tmem + lane_off + u * kTtBN + 64 * hv, sv[0]);
         tmem_ld_32x32b_x32(tmem + lane_off + u * kTtBN + 64 * hv + 32, sv[1]);
         tmem_wait_ld();
-        // What the row sees, one bit per key of each 32-key half.
-        uint32_t keep[2];
+        // Pages that every row sees whole need no masks (nor do rows behind the last: nobody reads theirs).
         const int k0 = key0 + 64 * hv;
-        if (draft) {
-          if (a.tree == nullptr && a.depth == nullptr) {  // a plain chunk: closed forms
+        bool plain = false;
+        if constexpr (kPaged) {
+          if (is_page(i)) plain = k0 + 64 <= full && (tok < 0 || first <= k0) && (scales[i % C::kScales].there >> (4 * hv) & 15u) == 15u;
+          plain = __all_sync(0xffffffffu, plain);
+        }
+        if (!plain) {
+          // What the row sees, one bit per key of each 32-key half.
+          uint32_t keep[2];
+          if (draft) {
+            if (a.tree == nullptr && a.depth == nullptr) {  // a plain chunk: closed forms
 #pragma unroll
-            for (int j = 0; j < 2; ++j) keep[j] = tok >= 0 ? tree_sees32(a, b, tok, k0 + 32 * j, dep, sink_left) : 0u;
-          } else {
-            tree_sees64_rows(a, b, tok, k0, dep, keep, sink_left);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if constexpr (kPaged) {
-              // Positions from p0 on, below the full pages' end or (the tail) the length.
-              const int p0 = (is_page(i) ? 0 : full) + k0 + 32 * j, hi = min((is_page(i) ? full : len) - 1 - p0, 31);
-              const int lo = max(first - p0, 0), sk = tok >= 0 ? min(a.sink - p0, 32) : 0;
-              uint32_t on = lo > 31 ? 0u : 0xFFFFFFFFu << lo;
-              if (a.window > 0 && sk > 0) on |= 0xFFFFFFFFu >> (32 - sk);
-              keep[j] = hi < 0 ? 0u : (0xFFFFFFFFu >> (31 - hi)) & on;
-              if (is_page(i)) {
-                const uint32_t on16 = scales[i % C::kScales].there >> (4 * hv + 2 * j);
-                if (!(on16 & 1u)) keep[j] &= 0xFFFF0000u;
-                if (!(on16 & 2u)) keep[j] &= 0x0000FFFFu;
-              }
+              for (int j = 0; j < 2; ++j) keep[j] = tok >= 0 ? tree_sees32(a, b, tok, k0 + 32 * j, dep, sink_left) : 0u;
             } else {
-              const int lo = max(first - k0 - 32 * j, 0), hi = min(len - 1 - k0 - 32 * j, 31);
-              keep[j] = hi < lo ? 0u : (0xFFFFFFFFu >> (31 - hi)) & (0xFFFFFFFFu << lo);
+              tree_sees64_rows(a, b, tok, k0, dep, keep, sink_left);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if constexpr (kPaged) {
+                // Positions from p0 on, below the full pages' end or (the tail) the length.
+                const int p0 = (is_page(i) ? 0 : full) + k0 + 32 * j, hi = min((is_page(i) ? full : len) - 1 - p0, 31);
+                const int lo = max(first - p0, 0), sk = tok >= 0 ? min(a.sink - p0, 32) : 0;
+                uint32_t on = lo > 31 ? 0u : 0xFFFFFFFFu << lo;
+                if (a.window > 0 && sk > 0) on |= 0xFFFFFFFFu >> (32 - sk);
+                keep[j] = hi < 0 ? 0u : (0xFFFFFFFFu >> (31 - hi)) & on;
+                if (is_page(i)) {
+                  const uint32_t on16 = scales[i % C::kScales].there >> (4 * hv + 2 * j);
+                  if (!(on16 & 1u)) keep[j] &= 0xFFFF0000u;
+                  if (!(on16 & 2u)) keep[j] &= 0x0000FFFFu;
+                }
+              } else {
+                const int lo = max(first - k0 - 32 * j, 0), hi = min(len - 1 - k0 - 32 * j, 31);
+                keep[j] = hi < lo ? 0u : (0xFFFFFFFFu >> (31 - hi)) & (0xFFFFFFFFu << lo);
+              }
             }
           }
-        }
-        if (!__all_sync(0xffffffffu, (keep[0] & keep[1]) == 0xFFFFFFFFu)) {
+          if (!__all_sync(0xffffffffu, (keep[0] & keep[1]) == 0xFFFFFFFFu)) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((keep[j] >> e) & 1u)) sv[j][e] = __float_as_uint(-INFINITY);
+              for (int e = 0; e < 32; ++e)
+                if (!((keep[j] >> e) & 1u)) sv[j][e] = __float_as_uint(-INFINITY);
+          }
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         if constexpr (kPaged) {  // 16 keys have one scale; in log2 units
@@ -670,7 +703,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
           for (int e = 0; e < 64; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(sv[e >> 5][e & 31]));
         }
         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        if (a.scores != nullptr && half == 0 && tok >= 0) {
+        if (!kPaged && a.scores != nullptr && half == 0 && tok >= 0) {
           float* dst = a.scores + (static_cast<int64_t>(bc) * rows + rr) * a.score_pitch + (draft ? a.draft_at : 0) + k0;
           const int left = (draft ? a.n : len) - k0;
           // (16 bytes at a time: the row's two parts begin and end on multiples of 4 slots, so the last
@@ -684,16 +717,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
                               __uint_as_float(sv[e >> 5][(e + 3) & 31]) * scale);
         }
       }
-      __syncwarp();
-      xch[hv * kTtBM + r] = mx;
       tc_fence_before();
-      pair_sync();  // both halves of S are in registers and both maxima are posted
+      // Both halves of S are in registers; the maxima are exchanged only if a row's m is to move.
+      const float limit = m + TreeRef<T>::kSlack;
+      const bool moves = pair_any((kPaged ? mx : mx * scale) > limit);
       tc_fence_after();
-      mx = fmaxf(mx, xch[(hv ^ 1) * kTtBM + r]);
-      pair_sync();  // the partner's maximum is read before either posts the next one
+      if (moves) {
+        xch[hv * kTtBM + r] = mx;
+        pair_sync();
+        mx = fmaxf(mx, xch[(hv ^ 1) * kTtBM + r]);
+        pair_sync();  // the partner's maximum is read before either posts the next one
+      }
       if (!ok) continue;
       const float mt = kPaged ? mx : mx * scale;
-      const bool move = mt > m + TreeRef<T>::kSlack;
+      const bool move = mt > limit;
       // O's unit: not below any scale of V so far, 1 from the first 16-bit rows on (the same in all
       // threads of the pair).
       float change = unit;
@@ -791,7 +828,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
             uint4* w = reinterpret_cast<uint4*>(vs) + e;
             if (!draft) {
               const int p = full + key0 + row;
-              if (p >= len || (p < span.low && p >= a.sink)) *w = make_uint4(0, 0, 0, 0);
+              if (p >= len || (p < span.low && (!kPaged || p >= a.sink))) *w = make_uint4(0, 0, 0, 0);
             } else {
               uint4 x = *w;
               if (nonfinite_bits<T>(x.x) | nonfinite_bits<T>(x.y) | nonfinite_bits<T>(x.z) | nonfinite_bits<T>(x.w)) {
@@ -1000,8 +1037,7 @@ static int encode_q(CUtensorMap* map, const w8::TreeArgs& a, bool half, int64_t 
 
 template <typename T, int D, int DR, bool kPaged, typename Args>
 static int launch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn, const CUtensorMap& tvn,
-                     const CUtensorMap& tk8, const CUtensorMap& tv8, const w8::TreeArgs& a, const Args& args,
-                     int64_t items, int device, cudaStream_t stream) {
+                     const w8::TreeArgs& a, const Args& args, int64_t items, int device, cudaStream_t stream) {
   using C = w8::TtCfg<D, kPaged>;
   CUtensorMap tq = tkn;
   if (a.q_tma) {
@@ -1027,7 +1063,7 @@ static int launch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const CUtenso
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cuda_status(
-      cudaLaunchKernelEx(&cfg, w8::attn_tree_tc_kernel<T, D, DR, kPaged, Args>, tq, tk, tv, tkn, tvn, tk8, tv8, args));
+      cudaLaunchKernelEx(&cfg, w8::attn_tree_tc_kernel<T, D, DR, kPaged, Args>, tq, tk, tv, tkn, tvn, args));
 }
 
 template <typename T, int D, int DR = D>
@@ -1047,7 +1083,7 @@ static int tree_tc_go(const w8::TreeArgs& a, int64_t items, int device, cudaStre
     st = tree_encode_rows(&tv, a.v, kHalf, DR, a.slots, a.kv_heads, a.batch, a.v_b, a.v_h, a.v_s, w8::kTtBN, vb);
     if (st != W8_OK) return st;
   }
-  return launch_tc<T, D, DR, false>(tk, tv, tkn, tvn, tkn, tvn, a, a, items, device, stream);
+  return launch_tc<T, D, DR, false>(tk, tv, tkn, tvn, a, a, items, device, stream);
 }
 
 // The tcgen05 schedule of w8_attention_tree (arguments checked by the caller; rows in tiles of
@@ -1081,7 +1117,9 @@ static int paged_tc_go(const w8_attention_paged_args& x, const w8::PagedArgs& pa
   using C = w8::TtCfg<D, true>;
   constexpr bool kHalf = __is_same(T, __half);
   const w8::TreeArgs& a = pa.t;
-  CUtensorMap tkn, tvn, tkt, tvt, tk8, tv8;
+  CUtensorMap tkn, tvn, tkt, tvt;
+  w8::TtPagedArgs args;
+  static_cast<w8::PagedArgs&>(args) = pa;
   auto rows = [&](CUtensorMap* map, const void* p, int64_t n, const int64_t* s, bool v) {
     return tree_encode_rows(map, p, kHalf, DR, n, a.kv_heads, a.batch, s[0], s[1], s[2], v ? w8::kTtBN : w8::kTtKeysPerCta,
                             v ? C::kDV / 128 : C::kKCols / 64);
@@ -1090,15 +1128,15 @@ static int paged_tc_go(const w8_attention_paged_args& x, const w8::PagedArgs& pa
   if (st == W8_OK) st = rows(&tvn, x.v_new, a.n, x.v_new_stride, true);
   if (st == W8_OK) st = rows(&tkt, x.k_tail, x.page, x.k_tail_stride, false);
   if (st == W8_OK) st = rows(&tvt, x.v_tail, x.page, x.v_tail_stride, true);
-  tk8 = tkn, tv8 = tvn;  // an empty pool: never read
+  args.k8 = tkn, args.v8 = tvn;  // an empty pool: never read
   const uint32_t box_k = static_cast<uint32_t>(std::min<int64_t>(x.page, w8::kTtKeysPerCta));
   const uint32_t box_v = static_cast<uint32_t>(std::min<int64_t>(x.page, w8::kTtBN));
   if (st == W8_OK && x.pages > 0)
-    st = encode_pages(&tk8, x.k, DR, x.page, x.kv_heads, x.pages, x.k_stride, C::kKCols, box_k);
+    st = encode_pages(&args.k8, x.k, DR, x.page, x.kv_heads, x.pages, x.k_stride, C::kKCols, box_k);
   if (st == W8_OK && x.pages > 0)
-    st = encode_pages(&tv8, x.v, DR, x.page, x.kv_heads, x.pages, x.v_stride, C::kDV / 2, box_v);
+    st = encode_pages(&args.v8, x.v, DR, x.page, x.kv_heads, x.pages, x.v_stride, C::kDV / 2, box_v);
   if (st != W8_OK) return st;
-  return launch_tc<T, D, DR, true>(tkt, tvt, tkn, tvn, tk8, tv8, a, pa, items, device, stream);
+  return launch_tc<T, D, DR, true>(tkt, tvt, tkn, tvn, a, args, items, device, stream);
 }
 
 // The same of w8_attention_paged.
