@@ -127,7 +127,8 @@ __device__ __forceinline__ int tree_depth(const TreeArgs& a, int b, int i) {
 
 // Whether token i sees new token j (both < n).
 // `sink_left`: a.sink less the committed length; new tokens of a smaller depth are sinks.
-__device__ __forceinline__ bool tree_sees(const TreeArgs& a, int b, int i, int j, int depth_i, int sink_left = 0) {
+constexpr int kNoSinks = INT32_MIN;
+__device__ __forceinline__ bool tree_sees(const TreeArgs& a, int b, int i, int j, int depth_i, int sink_left = kNoSinks) {
   const bool on = a.tree != nullptr ? a.tree[b * a.tree_b + i * a.tree_i + j] != 0 : j <= i;
   if (!on || a.window <= 0) return on;
   const int dj = tree_depth(a, b, j);
@@ -153,7 +154,7 @@ __device__ __forceinline__ uint32_t nonzero_bytes(uint32_t w) {
 // loads would wait for each in turn: the row is read with 16-byte loads where it is aligned
 // and with 32 independent ones where it is not.
 __device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i, int j0, int depth_i,
-                                                int sink_left = 0) {
+                                                int sink_left = kNoSinks) {
   const int left = a.n - j0;
   if (left <= 0) return 0u;
   uint32_t bits = 0;
@@ -196,7 +197,7 @@ __device__ __forceinline__ uint32_t tree_sees32(const TreeArgs& a, int b, int i,
 // token (ascending over the lanes, -1 for none) and its depth.  The rows of a token share its
 // line of the tree, which the warp reads once, a byte a lane (any alignment).  All lanes.
 __device__ __forceinline__ void tree_sees64_rows(const TreeArgs& a, int b, int tok, int j0, int depth_i,
-                                                 uint32_t (&keep)[2], int sink_left = 0) {
+                                                 uint32_t (&keep)[2], int sink_left = kNoSinks) {
   const int lane = threadIdx.x & 31;
   keep[0] = keep[1] = 0u;
   const int j[2] = {j0 + lane, j0 + 32 + lane};
@@ -228,7 +229,7 @@ __device__ __forceinline__ void tree_sees64_rows(const TreeArgs& a, int b, int t
 // The same for one row's new tokens j0 .. j0 + 15, in little code (it stands beside the common
 // tiles, which have none of it).  All lanes, of the same j0.
 __device__ __forceinline__ uint32_t tree_sees16(const TreeArgs& a, int b, int i, int j0, int depth_i,
-                                                int sink_left = 0) {
+                                                int sink_left = kNoSinks) {
   const int left = min(a.n - j0, 16);
   uint32_t bits = left <= 0 || i < 0 ? 0u : (1u << left) - 1u;
   if (a.tree == nullptr) {

@@ -223,7 +223,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
     }
     return (t0 + i >= nc ? t0 + i - nc : span.c0 + t0 + i) * kTtBN;
   };
-  const int sink_left = kPaged ? a.sink - len : 0;  // (negative or 0 without sinks: len >= 0)
+  const int sink_left = kPaged ? a.sink - len : kNoSinks;
   // Of a causal chunk's tiles of new tokens, those that every row of the pair sees whole are as
   // plain as committed ones.
   const int tok_lo = rt * (2 * kTtBM) / a.group, tok_hi = (min((rt + 1) * (2 * kTtBM), rows) - 1) / a.group;
@@ -568,19 +568,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
     volatile float* xch = reinterpret_cast<volatile float*>(smem + C::kOffXch);
     const volatile uint32_t* poison = reinterpret_cast<const volatile uint32_t*>(smem + C::kOffPoison);
     auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
-    auto pair_any = [&](bool on) {
-      uint32_t any;
-      __syncwarp();
-      asm volatile(
-          "{\n\t.reg .pred p, q;\n\t"
-          "setp.ne.u32 q, %1, 0;\n\t"
-          "bar.red.or.pred p, %2, 64, q;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(any)
-          : "r"(on ? 1u : 0u), "r"(1 + quarter)
-          : "memory");
-      return any != 0u;
-    };
     auto softmax_sync = [&]() { asm volatile("bar.sync 5, %0;" ::"n"(32 * kTtSoftWarps) : "memory"); };
 
     // Q rows that no TMA box describes (128 rows are whole tokens only for a group that divides
@@ -717,20 +704,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TtCfg<D, kPaged>::kT
                               __uint_as_float(sv[e >> 5][(e + 3) & 31]) * scale);
         }
       }
+      __syncwarp();
+      xch[hv * kTtBM + r] = mx;
       tc_fence_before();
-      // Both halves of S are in registers; the maxima are exchanged only if a row's m is to move.
-      const float limit = m + TreeRef<T>::kSlack;
-      const bool moves = pair_any((kPaged ? mx : mx * scale) > limit);
+      pair_sync();  // both halves of S are in registers and both maxima are posted
       tc_fence_after();
-      if (moves) {
-        xch[hv * kTtBM + r] = mx;
-        pair_sync();
-        mx = fmaxf(mx, xch[(hv ^ 1) * kTtBM + r]);
-        pair_sync();  // the partner's maximum is read before either posts the next one
-      }
+      mx = fmaxf(mx, xch[(hv ^ 1) * kTtBM + r]);
+      pair_sync();  // the partner's maximum is read before either posts the next one
       if (!ok) continue;
       const float mt = kPaged ? mx : mx * scale;
-      const bool move = mt > limit;
+      const bool move = mt > m + TreeRef<T>::kSlack;
       // O's unit: not below any scale of V so far, 1 from the first 16-bit rows on (the same in all
       // threads of the pair).
       float change = unit;
