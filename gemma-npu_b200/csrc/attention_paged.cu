@@ -933,8 +933,12 @@ static PagedPlan paged_plan(int64_t batch, int64_t kv_heads, int64_t group, int6
                             int64_t window, int64_t sink, int sms) {
   PagedPlan p;
   const int64_t rows = group * n;
-  p.tc = rows > (d == 512 ? 8 : 16);
-  p.bm = p.tc ? 256 : rows <= 8 ? 8 : 16;
+  // Up to so many rows a cache head in tiles of 16 (D = 512: 8), more in tiles of 256 on the tensor cores'
+  // schedule, whose cost hardly depends on how many of the 256 there are (40 sequences of 1000, 8 heads
+  // of 128: 32 rows 90 us against 155, 48 rows 127 against 156, 64 rows 165 against 156; D = 64, 64
+  // rows: 118 against 153; D = 256, 24 rows: 234 against 178; D = 512, 24 rows: 394 against 451).
+  p.tc = rows > (d == 64 ? 64 : d == 128 ? 48 : d == 256 ? 16 : 24);
+  p.bm = p.tc ? 256 : d == 512 || rows <= 8 ? 8 : 16;
   p.row_tiles = static_cast<int>((rows + p.bm - 1) / p.bm);
   p.items = batch * kv_heads * p.row_tiles;
   // Keys of one row tile: with a window, those its tokens see.

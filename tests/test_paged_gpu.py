@@ -172,6 +172,15 @@ SHAPES = [
     (16, 2, 64, 32, 40, [300, 0, 1, 127, 128, 129, 255, 256, 257], 50, 200),
     (33, 1, 64, 128, 1, [650], 0, 0),
     (17, 1, 128, 128, 1, [650, 127, 128], 300, 129),
+    # the same sizes' neighbours: several tiles of 16 (or 8) rows, and one row more than those take
+    (8, 1, 512, 128, 3, [700, 0, 129], 0, 0),
+    (4, 1, 512, 16, 5, [300, 64], 40, 17),
+    (25, 1, 512, 32, 1, [333, 1], 0, 0),
+    (12, 2, 128, 32, 8, [700, 33, 0], 0, 0),
+    (7, 1, 128, 64, 7, [500, 64], 130, 70),
+    (16, 2, 64, 16, 8, [600, 15, 17], 60, 33),
+    (13, 1, 64, 128, 5, [520], 0, 0),
+    (16, 8, 64, 32, 20, [3000, 1, 700, 2999, 256, 257, 0, 2000, 64, 1500], 900, 40),
 ]
 
 
@@ -189,8 +198,10 @@ def test_attention_chain(cuda, shape, dt):
 @DTYPES
 @pytest.mark.parametrize("shape", [(4, 2, 128, 32, 5, [100, 0, 33], 0, 0), (2, 1, 256, 64, 7, [300, 64], 50, 4),
                                    (8, 2, 256, 32, 24, [700, 0, 95], 0, 0), (8, 1, 512, 16, 30, [300, 17], 40, 10),
-                                   (4, 1, 64, 128, 60, [500], 100, 600), (4, 4, 64, 16, 13, [100, 5], 9, 104)],
-                         ids=[str(i) for i in range(6)])
+                                   (4, 1, 64, 128, 60, [500], 100, 600), (4, 4, 64, 16, 13, [100, 5], 9, 104),
+                                   (4, 1, 64, 16, 13, [300, 5, 0], 9, 104), (8, 2, 128, 64, 11, [700, 64], 0, 0),
+                                   (4, 2, 512, 32, 9, [200, 31], 20, 210)],
+                         ids=[str(i) for i in range(9)])
 def test_attention_tree(cuda, shape, dt):
     """Drafted trees: ancestors' masks, depths, sinks among the new tokens, padding drafts of NaN."""
     H, KV, D, P, N, lens, window, sink = shape
@@ -220,7 +231,7 @@ def test_attention_strides(cuda, H, N, D, P):
     assert got.data_ptr() == out.data_ptr() and bool((out[..., D:] == 7).all())
 
 
-@pytest.mark.parametrize("H,N", [(4, 1), (8, 5)])
+@pytest.mark.parametrize("H,N", [(4, 1), (8, 5), (8, 20)])
 @DTYPES
 def test_attention_scales_far_apart(cuda, H, N, dt):
     """Pages whose scales of V differ by orders of magnitude (O's unit moves), pages of zeros, and a zero
@@ -241,7 +252,7 @@ def test_attention_scales_far_apart(cuda, H, N, dt):
     check_out(attend(c, *a, scale=0.05), want, dt)
 
 
-@pytest.mark.parametrize("H,N", [(4, 1), (8, 5)])
+@pytest.mark.parametrize("H,N", [(4, 1), (8, 5), (8, 20)])
 def test_attention_of_a_page_with_nan_scales(cuda, H, N):
     """A NaN scale is for the rows that see the page: a window keeps it from others."""
     c = cache(5, 1, 64, 16, [100, 100])
@@ -256,7 +267,7 @@ def test_attention_of_a_page_with_nan_scales(cuda, H, N):
         check_out(attend(d, *a, **kw), want_attention(c, *a, **kw), torch.bfloat16)
 
 
-@pytest.mark.parametrize("H,N", [(4, 1), (8, 5)])
+@pytest.mark.parametrize("H,N", [(4, 1), (8, 5), (8, 20)])
 def test_attention_new_values_that_some_rows_see(cuda, H, N):
     """Infinite and NaN values of a new token reach the rows that see it and no others."""
     c = cache(7, 1, 128, 32, [70])
@@ -270,7 +281,7 @@ def test_attention_new_values_that_some_rows_see(cuda, H, N):
     assert bool(got[..., rest].eq(clean[..., rest]).all())
 
 
-@pytest.mark.parametrize("H,N", [(4, 1), (8, 5)])
+@pytest.mark.parametrize("H,N", [(4, 1), (8, 5), (8, 20)])
 def test_attention_pages_before_the_window_may_be_gone(cuda, H, N):
     c = cache(9, 1, 64, 16, [500, 37])
     a = new(10, 2, H, 1, 64, N, torch.bfloat16)
@@ -282,7 +293,7 @@ def test_attention_pages_before_the_window_may_be_gone(cuda, H, N):
     assert w8.device_status() == 0
 
 
-@pytest.mark.parametrize("H,N", [(4, 1), (8, 5)])
+@pytest.mark.parametrize("H,N", [(4, 1), (8, 5), (8, 20)])
 @pytest.mark.parametrize("entry", [-1, 10 ** 6])
 def test_attention_reports_a_missing_page(cuda, H, N, entry):
     c = cache(11, 1, 64, 16, [200])
