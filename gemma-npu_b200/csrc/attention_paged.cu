@@ -31,7 +31,7 @@
 // that no row sees are not read (nor their table entries followed), so a window's old pages may
 // be gone.
 //
-// 32 sequences of 2000 to 8191 tokens, 8 cache heads of 128, 4 query heads each: 69 us, 74% of what a
+// 32 sequences of 2000 to 8191 tokens, 8 cache heads of 128, 4 query heads each: 70 us, 74% of what a
 // copy moves, of which reading alone takes 62; what is left is the unpacking (some 9 instructions
 // for 4 values and both products) that no longer hides behind the loads.  One sequence of one
 // token is a chain (table, page, join, combine): 15 us for 3658 keys of 512.
