@@ -22,12 +22,14 @@
 // to 2^-48, and sums in double.
 //
 // After k rejections w is max(p - c q, 0) / Z with one c: of max(p - c q, 0) / Z less q, what is
-// positive is max(p - (c + Z) q, 0).  So nothing is stored: a rejection costs one pass over both rows,
-// which gives Z, and by warps' chunks what the draw then needs to find its token.
+// positive is max(p - (c + Z) q, 0).  So nothing is stored: a node's first rejection costs one pass over
+// both rows, which gives Z, and by warps' chunks what the draw then needs to find its token; a further
+// one takes off what the larger c drops, in 64 bits only for the values that may be (24 trees 197 ->
+// 164 us; one chain, which never gets there, 25 -> 26).
 //
 // What bounds it: the 64-bit operations of the passes (an SM has 62 a clock) and, for short walks, the
 // chain of a node (its children, a pass, two meetings of the cluster: some 4 us).  One chain of 5 drafts
-// over 262144 values takes 25 us; 24 trees take 195, as long as their longest walk.
+// over 262144 values takes 26 us; 24 trees take 164, as long as their longest walk.
 #include "common.cuh"
 
 #include <cuda_fp16.h>
@@ -316,6 +318,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
   __shared__ double shared[2][4][kVerifyCluster];        // a CTA's, by turns
   __shared__ double chunk_p[kVerifyChunks], chunk_q[kDraft ? kVerifyChunks : 1];  // of a warp's parts of the last pass
   __shared__ int gone[kDraft ? 1 : kVerifyNodes];        // without draft logits: tokens whose weight is taken
+  __shared__ uint8_t queue[kDraft ? kVerifyWarps : 1][256];  // of a warp's 256 values those that a rejection may drop
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const VerifyPlace at = verify_place(a);
   const int b = at.b, rank = at.rank, ranks = at.ranks, lo = at.lo, hi = at.hi;
@@ -569,6 +572,50 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
         }
       }
     };
+    // A further rejection's pass: c has grown, so values that stayed may be dropped and none comes back.
+    // fp32 tells which cannot have been (what it may be off by is 2^-18 of the levels); the others,
+    // 32 at a time, are looked at in 64 bits, and those dropped taken off the chunk's and the CTA's sums.
+    auto drop = [&](double (&sums)[4], double rp0, double rq0, double rp, double rq) {
+      const float tops = p.top - q.top, slack = 0x1p-18f * (fabsf(p.top) + fabsf(q.top) + (kCapped ? target.cap_slope : 0.f));
+      const float at0 = tops + static_cast<float>(log2(rq0 / rp0)) - slack, at1 = tops + static_cast<float>(log2(rq / rp)) + slack;
+      if (tid == 0) sums[2] = shared[turn][2][rank], sums[3] = shared[turn][3][rank];
+      uint8_t* mine = queue[kDraft ? warp : 0];
+#pragma unroll 1
+      for (int k = warp; k < chunks; k += kVerifyWarps) {
+        double part[2] = {0.0, 0.0};
+#pragma unroll 1
+        for (int j = 0; j < turns; ++j) {
+          const int v0 = lo + (k * turns + j) * 256;
+          float x[kVerifyVec], y[kVerifyVec];
+          load8<E>(xr, v0 + lane * kVerifyVec, hi, wx, x);
+          load8<E>(dr, v0 + lane * kVerifyVec, hi, wd, y);
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < kVerifyVec; ++i) {
+            const float lp = level_32<kCapped>(x[i], target), lq = level_32<false>(y[i], drafted), d = lp - lq;
+            const float off = 0x1p-18f * (fabsf(lp) + fabsf(lq));
+            // (p = 0 < q was dropped before; q = 0 is never)
+            const bool near = lp != -INFINITY && lq != -INFINITY && !(d > at1 + off) && !(d < at0 - off);
+            const uint32_t lanes = __ballot_sync(0xffffffffu, near);
+            if (near) mine[n + __popc(lanes & ((1u << lane) - 1u))] = static_cast<uint8_t>(lane * kVerifyVec + i);
+            n += __popc(lanes);
+          }
+          __syncwarp();
+#pragma unroll 1
+          for (int e = lane; e < n; e += 32) {
+            const int v = v0 + mine[e];
+            const double pv = p_of(logit_f32<E>(xr[v])), qv = q_of(logit_f32<E>(dr[v]));
+            if (__double2hiint(fma(-rq0, qv, pv * rp0)) >= 0 && __double2hiint(fma(-rq, qv, pv * rp)) < 0)
+              part[0] += pv, part[1] += qv;
+          }
+          __syncwarp();
+        }
+        sums[2] -= part[0], sums[3] -= part[1];
+        part[0] = warp_sum(part[0]), part[1] = warp_sum(part[1]);
+        if (lane == 0) chunk_p[k] -= part[0], chunk_q[kDraft ? k : 0] -= part[1];
+      }
+    };
+    double last_rp = 0.0, last_rq = 0.0;  // of the last pass
     if (q.fine)
       for (; c < a.n; c = child_after(a, at, tree, cur, c)) {
         const int t = tree.tokens[c];
@@ -598,7 +645,11 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
           // need them so exactly (where p and q are equal to 2^-23, what is left is 2^-23 of them).
           const double to_c = c_q + (rejected == 0 ? 1.0 : left);
           double sums[4] = {0.0, 0.0, 0.0, 0.0};
-          pass(std::true_type(), sums, 1.0 / p.sum, to_c / q.sum);
+          if (rejected == 0)
+            pass(std::true_type(), sums, 1.0 / p.sum, to_c / q.sum);
+          else
+            drop(sums, last_rp, last_rq, 1.0 / p.sum, to_c / q.sum);
+          last_rp = 1.0 / p.sum, last_rq = to_c / q.sum;
           exchange_sums(sums);
           if (!sharp) p.sum = shared_sum(0), q.sum = shared_sum(1);
           sharp = true;

@@ -775,6 +775,22 @@ def test_verify_many_rejections(cuda):
         check_verify(logits, tokens, uniform, parent, d)
 
 
+@pytest.mark.parametrize("V,dt,cap,temperature", [(70001, torch.float32, 0.0, 1.0), (70000, torch.bfloat16, 5.0, 0.7),
+                                                  (9000, torch.float16, 0.0, 2.0), (262144, torch.bfloat16, 30.0, 1.3)])
+def test_verify_many_rejections_of_wide_rows(cuda, V, dt, cap, temperature):
+    """Children that fall one after the other over vocabularies of many parts, with impossible tokens in
+    either model: each rejection drops some of what the one before left."""
+    B, N = 6, 12
+    logits, tokens, uniform, _, d = verify_case(7, B, N, V, dt, False, True, temperature)
+    logits[:, :, 5::97] = -math.inf
+    d[:, :, 11::89] = -math.inf
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    tokens = torch.multinomial(torch.softmax(d[:, 0].float() / temperature, 1), N, replacement=True, generator=gen)
+    parent = torch.tensor([-1] + [0] * (N - 1), dtype=torch.int32, device="cuda")
+    uniform[:, 1:] = 0.6 + 0.4 * uniform[:, 1:]
+    check_verify(logits, tokens, uniform, parent, d, temperature, cap)
+
+
 def test_verify_uniform_ends(cuda):
     """Numbers at the ends of [0, 1): the first possible token, the last one."""
     logits, tokens, _, parent, d = verify_case(8, 6, 4, 3000, torch.float32, False, True, 1.0)
