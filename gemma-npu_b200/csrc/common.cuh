@@ -267,16 +267,6 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
-// The same in two halves, of which the first orders nothing: every CTA of the cluster has started, and
-// its shared memory may be written, once the second has passed.
-__device__ __forceinline__ void cluster_started() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_all_started() {
-  __syncwarp();
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-}
 // Arrive on an mbarrier in this CTA or the peer CTA of the pair when what the waiter needs
 // is TMEM that this thread's tcgen05 loads or stores touched: tcgen05.wait has completed
 // them and tcgen05.fence::before_thread_sync orders them before the arrive, and the waiter

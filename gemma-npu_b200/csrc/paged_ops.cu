@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
   const int b1 = static_cast<int>(static_cast<int64_t>(a.batch) * (rank + 1) / ranks);
   const int count = b1 - b0;
   if (tid == 0) given = 0;
-  cluster_started();
   pdl_launch_dependents();
+  cluster_sync();  // every CTA has started: its shared memory may be written
   pdl_wait();
   const int top0 = *a.top;
   const bool bad_top = top0 < 0 || top0 > a.free_size;
@@ -392,7 +392,6 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
     if (w < warp) xb += scan[0][w], xm += scan[1][w];
     tb += scan[0][w], tm += scan[1][w];
   }
-  cluster_all_started();
   if (tid < static_cast<int>(ranks))
     st_cluster_u64(mapa_shared(smem_u32(&sums[0][rank]), tid),
                    static_cast<unsigned long long>(static_cast<uint32_t>(tb)) << 32 | static_cast<uint32_t>(tm));
