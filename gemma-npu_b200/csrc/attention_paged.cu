@@ -471,13 +471,12 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
           }
         }
     };
-    float unit = __uint_as_float(0x00800000u);  // of O (2^-126: nothing added yet)
-    bool permuted = true;
+    float unit = __uint_as_float(0x00800000u);  // of O: the smallest, which the smallest scales have too
+    bool permuted = false;                      // O holds pages' products: in `unit` and their columns' order
     // O in order and in units of 1: of each 16 columns a thread holds 2 gl and 2 gl + 1 (the even and
     // odd bytes of V's rows) and gets gl and gl + 8.
     auto natural = [&]() {
       permuted = false;
-      if (unit == __uint_as_float(0x00800000u)) return;  // (O is 0 as yet)
       const int s0 = ((gl >> 1) << 2) | tl, s1 = s0 + 16;
       const bool odd = gl & 1;
 #pragma unroll
@@ -515,6 +514,7 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
       const int kind = kind_of(t), tile0 = key0_of(t);
       const uint32_t sk = base + slot_k * C::kSlotBytes, sv = base + slot_v * C::kSlotBytes;
       if (kind == kPages) {
+        permuted = true;
         const int kr = grp * (C::kKT * 16), key0 = tile0 + kr;  // this step's keys
         // Rows of 16 bytes that a lane names for ldmatrix: 8 keys, the next 8, and the next 16 columns of
         // both.  A row's chunks are swizzled, a matter of one XOR as a row begins on 128 (64) bytes.

@@ -252,6 +252,21 @@ def test_attention_scales_far_apart(cuda, H, N, dt):
     check_out(attend(c, *a, scale=0.05), want, dt)
 
 
+@pytest.mark.parametrize("D,KV,H,N,lens", [(64, 2, 4, 1, [100, 40, 3]), (128, 1, 8, 2, [1000, 40, 3]), (256, 2, 4, 3, [300, 48, 0]),
+                                           (512, 1, 8, 1, [700, 64, 3]), (128, 8, 64, 1, [3000, 700, 2999, 128]),
+                                           (128, 1, 8, 20, [1000, 40, 3])])
+@pytest.mark.parametrize("size", [1e-37, 2.0 ** -125, 2.0 ** -126, 2.0 ** -127, 1e-39, 0.0])
+def test_attention_of_tiny_scales(cuda, size, D, KV, H, N, lens):
+    """Pages of values so small that their scales are at or below fp32's smallest normal number (what
+    `paged_append` makes of bf16 rows below 1.5e-36): next to nothing is added to the other rows."""
+    c = cache(4, KV, D, 16, lens)
+    a = new(5, len(lens), H, KV, D, N, torch.bfloat16)
+    c["v_scale"][torch.isfinite(c["v_scale"])] = size
+    check_out(attend(c, *a, scale=0.05), want_attention(c, *a, scale=0.05), torch.bfloat16)
+    c["v_scale"][c["table"][0, 0].long()] = 0.02  # (one page that is not)
+    check_out(attend(c, *a, scale=0.05), want_attention(c, *a, scale=0.05), torch.bfloat16)
+
+
 @pytest.mark.parametrize("H,N", [(4, 1), (8, 5), (8, 20)])
 def test_attention_of_a_page_with_nan_scales(cuda, H, N):
     """A NaN scale is for the rows that see the page: a window keeps it from others."""
