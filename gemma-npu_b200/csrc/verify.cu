@@ -55,6 +55,7 @@ struct VerifyArgs {
   int n, vocab, per;       // per: values of a CTA's part (a multiple of 8)
   int greedy;
   double cap, slope;       // slope: log2(e) / temperature, of y or (without a cap) the logit
+  double range;            // logits of 1000 levels
 };
 
 constexpr int kVerifyThreads = 512;
@@ -113,16 +114,19 @@ __device__ __forceinline__ double exp2_64(double t, const double* table) {
   const double u = table[k & 31], s = fma(u * g, p, u);
   return __hiloint2double(__double2hiint(s) + ((k >> 5) << 20), __double2loint(s));
 }
-// Weights of a row's logits: 2^(level - top), the level a logit in log2 units of its probability.
+// Weights of a row's logits: 2^(level - ref), the level a logit in log2 units of its probability.
 struct VerifyScale {
   bool deep;                // a capped row's levels may differ by more than 900
   float most;               // 20 caps: tanh is 1 to 2^-57 from there on
   float slope, two_over_cap, cap_slope;  // for fp32
   double in, out, twice;    // log2(e) 2 / cap, cap slope (slope without a cap), 2 cap slope
 };
-// One row's probabilities: 2^(level - top) / sum.
+// One row's probabilities: 2^(level - ref) / sum.  Without a cap ref is the largest logit's level and levels
+// are differences of logits, scaled: a level by itself, rounded to fp32, would be off by 2^-24 of it, 1e-3
+// at a temperature of 1e-3.  The largest logit's weight is 1 in fp32 and (to 2^-52 of ref) in 64 bits.
 struct VerifyRow {
-  float top, least;  // the largest level; the logit 1000 below it, less than which counts as 0
+  float top, least;  // the largest logit (level, with a cap); the logit 1000 levels below it, less than which counts as 0
+  double ref, out;   // levels a logit (no cap)
   double sum;
   bool fine;  // the row has a finite largest logit and no NaN
 };
@@ -133,7 +137,7 @@ __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, const
   bool none;
   if constexpr (!kCapped) {
     none = x < row.least;
-    w = exp2_64(fma(static_cast<double>(fmaxf(x, row.least)), c.out, -static_cast<double>(row.top)), table);
+    w = exp2_64(fma(static_cast<double>(fmaxf(x, row.least)), row.out, -row.ref), table);
   } else {
     // tanh(z) = 1 - 2 / (1 + e^2z); the reciprocal by one step of Newton's iteration from 22 bits
     const float xc = fminf(fmaxf(x, -c.most), c.most);
@@ -141,7 +145,7 @@ __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, const
     float r32;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r32) : "f"(static_cast<float>(d)));
     const double r0 = static_cast<double>(r32), r = fma(r0, fma(-d, r0, 1.0), r0);
-    double t = fma(-c.twice, r, c.out - static_cast<double>(row.top));
+    double t = fma(-c.twice, r, c.out - row.ref);
     none = x == -INFINITY;
     if (c.deep) {
       none = none || t < -1000.0;
@@ -151,9 +155,8 @@ __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, const
   }
   return __hiloint2double(none ? 0 : __double2hiint(w), none ? 0 : __double2loint(w));
 }
-template <bool kCapped>
+// A capped logit's level.
 __device__ __forceinline__ float level_32(float x, const VerifyScale& c) {
-  if constexpr (!kCapped) return x * c.slope;
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * c.two_over_cap));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
@@ -163,6 +166,12 @@ __device__ __forceinline__ float ex2_32(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// A logit's level less the row's largest one's.
+template <bool kCapped>
+__device__ __forceinline__ float below_32(float x, const VerifyScale& c, const VerifyRow& row) {
+  if constexpr (kCapped) return level_32(x, c) - row.top;
+  return (x - row.top) * c.slope;
 }
 
 // What both kernels know of their sequence: a cluster of CTAs, each with a part of the vocabulary.
@@ -380,17 +389,18 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
   // The largest levels and the sums of a target row and (if asked for) a draft row in fp32.
   auto stats = [&](const E* xr, const E* dr, bool two, VerifyRow& p, VerifyRow& q) {
     const bool wx = verify_on16(xr), wd = verify_on16(dr);
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // in log2 units
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // of levels (a capped row) or logits
     bool bad[2] = {false, false};
+    auto slope = [&](int r) { return kCapped && r == 0 ? 1.f : drafted.slope; };
     auto add = [&](const float (&y)[kVerifyVec], int r) {
       float most = y[0];
 #pragma unroll
       for (int i = 1; i < kVerifyVec; ++i) most = fmaxf(most, y[i]);
       // (without a branch: the sum is rescaled by 1 where the maximum stays)
       const float to = fmaxf(top[r], most), ref = to == -INFINITY ? 0.f : to;
-      float s = sum[r] * ex2_32(top[r] - ref);
+      float s = sum[r] * ex2_32((top[r] - ref) * slope(r));
 #pragma unroll
-      for (int i = 0; i < kVerifyVec; ++i) s += ex2_32(y[i] - ref);
+      for (int i = 0; i < kVerifyVec; ++i) s += ex2_32((y[i] - ref) * slope(r));
       sum[r] = s;
       top[r] = to;
     };
@@ -399,7 +409,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
 #pragma unroll
       for (int i = 0; i < kVerifyVec; ++i) {
         bad[r] |= !(x[i] < INFINITY);
-        y[i] = r == 0 ? level_32<kCapped>(x[i], target) : level_32<false>(x[i], drafted);
+        y[i] = kCapped && r == 0 ? level_32(x[i], target) : x[i];
       }
       add(y, r);
     };
@@ -439,9 +449,9 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       }
     }
     // A warp's, the CTA's, then the cluster's: sums relative to the largest level so far.
-    auto join = [&](float2 t) {
+    auto join = [&](float2 t, float slope) {
       const float to = warp_max(t.x);
-      float s = t.x == -INFINITY ? t.y : t.y * ex2_32(t.x - to);  // (a NaN stays)
+      float s = t.x == -INFINITY ? t.y : t.y * ex2_32((t.x - to) * slope);  // (a NaN stays)
 #pragma unroll
       for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
       return make_float2(to, s);
@@ -450,25 +460,34 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
     float2 t[2];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      t[r] = join(make_float2(top[r], bad[r] ? __uint_as_float(0x7FC00000u) : sum[r]));
+      t[r] = join(make_float2(top[r], bad[r] ? __uint_as_float(0x7FC00000u) : sum[r]), slope(r));
       if (lane == 0) tops[r][warp] = t[r];
     }
     __syncthreads();
     top_turn ^= 1;
     if (warp < kRows) {
-      const float2 c = join(lane < kVerifyWarps ? tops[warp][lane] : make_float2(-INFINITY, 0.f));
+      const float2 c = join(lane < kVerifyWarps ? tops[warp][lane] : make_float2(-INFINITY, 0.f), slope(warp));
       if (lane < ranks)
         st_cluster_f64(reinterpret_cast<const double*>(&all_tops[top_turn][warp][rank]), lane,
                        __hiloint2double(__float_as_int(c.y), __float_as_int(c.x)));
     }
     cluster_sync();
     auto row = [&](int r, const VerifyScale& scale) {
-      const float2 c = join(lane < ranks ? all_tops[top_turn][r][lane] : make_float2(-INFINITY, 0.f));
+      const float2 c = join(lane < ranks ? all_tops[top_turn][r][lane] : make_float2(-INFINITY, 0.f), slope(r));
       VerifyRow out;
       out.top = c.x;
       out.sum = static_cast<double>(c.y);
       out.fine = c.y > 0.f && c.y < INFINITY && c.x > -INFINITY && c.x < INFINITY;
-      out.least = fmaxf((out.top - 1000.f) / scale.slope, -3e38f);
+      out.ref = out.top, out.out = 0.0, out.least = out.top;
+      if (!kCapped || r != 0) {
+        // (From 2^40 levels on the next lower fp32 number is 2^16 below: the largest logit's weight is 1,
+        // every other one's 0.)
+        const double ref = static_cast<double>(out.top) * scale.out;
+        const bool far = !(fabs(ref) < 0x1p40);
+        out.ref = far ? 0.0 : ref;
+        out.out = far ? 0.0 : scale.out;
+        if (!far) out.least = __double2float_ru(static_cast<double>(out.top) - a.range);
+      }
       return out;
     };
     p = row(0, target);
@@ -491,7 +510,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       if (kDraft) d0 = logit_f32<E>(dr[tree.tokens[c0]]);
       u_c0 = u[c0];
     }
-    VerifyRow p, q = {0.f, 0.f, 1.0, true};
+    VerifyRow p, q = {0.f, 0.f, 0.0, 0.0, 1.0, true};
     stats(xr, dr, c < a.n, p, q);
     if (!p.fine) break;
     // After rejections w is max(p - c q, 0) / left: c = 0 and left = 1 at first, and of that less q what
@@ -576,8 +595,8 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
     // fp32 tells which cannot have been (what it may be off by is 2^-18 of the levels); the others,
     // 32 at a time, are looked at in 64 bits, and those dropped taken off the chunk's and the CTA's sums.
     auto drop = [&](double (&sums)[4], double rp0, double rq0, double rp, double rq) {
-      const float tops = p.top - q.top, slack = 0x1p-18f * (fabsf(p.top) + fabsf(q.top) + (kCapped ? target.cap_slope : 0.f));
-      const float at0 = tops + static_cast<float>(log2(rq0 / rp0)) - slack, at1 = tops + static_cast<float>(log2(rq / rp)) + slack;
+      const float slack = 0x1p-18f * (kCapped ? fabsf(p.top) + target.cap_slope : 0.f) + 0x1p-22f;
+      const float at0 = static_cast<float>(log2(rq0 / rp0)) - slack, at1 = static_cast<float>(log2(rq / rp)) + slack;
       if (tid == 0) sums[2] = shared[turn][2][rank], sums[3] = shared[turn][3][rank];
       uint8_t* mine = queue[kDraft ? warp : 0];
 #pragma unroll 1
@@ -592,7 +611,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
           int n = 0;
 #pragma unroll
           for (int i = 0; i < kVerifyVec; ++i) {
-            const float lp = level_32<kCapped>(x[i], target), lq = level_32<false>(y[i], drafted), d = lp - lq;
+            const float lp = below_32<kCapped>(x[i], target, p), lq = below_32<false>(y[i], drafted, q), d = lp - lq;
             const float off = 0x1p-18f * (fabsf(lp) + fabsf(lq));
             // (p = 0 < q was dropped before; q = 0 is never)
             const bool near = lp != -INFINITY && lq != -INFINITY && !(d > at1 + off) && !(d < at0 - off);
@@ -886,6 +905,7 @@ extern "C" int w8_draft_verify(const w8_draft_verify_args* in, w8_stream_t strea
   a.greedy = greedy;
   a.cap = greedy ? 0.0 : x.cap;
   a.slope = greedy ? 1.0 : 1.4426950408889634 / x.temperature;
+  a.range = 1000.0 / a.slope;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (x.dtype == W8_FP32) return verify_go<float>(a, x.batch, device, s);
   if (x.dtype == W8_BF16) return verify_go<__nv_bfloat16>(a, x.batch, device, s);
