@@ -517,7 +517,6 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
     // is positive is max(p - (c + left) q, 0).
     double c_q = 0.0, left = 1.0;
     int rejected = 0;     // without draft logits: their tokens' weights are taken, `left` stays
-    bool sharp = false;   // the sums are in 64 bits
     bool summed = false;  // shared[turn][2, 3] and the chunks have the last pass's parts of p and q
     const bool wx = verify_on16(xr), wd = kDraft && verify_on16(dr);
     auto p_of = [&](float x) { return weight_64<kCapped>(x, target, p, table); };
@@ -660,19 +659,31 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
             break;
           }
           // Rejected: what is left, in 64 bits.  With the sums of p and q by themselves over the values that
-          // stay positive, the first pass gives the sums over all besides: which values stay does not
-          // need them so exactly (where p and q are equal to 2^-23, what is left is 2^-23 of them).
+          // stay positive, the first pass gives the sums over all besides.  Which values stay it takes from the
+          // fp32 sums.  Those move the border p = q by some 10^-7 of it: what lies between (10^-7 of the
+          // probability, where p / q is spread) is miscounted by 10^-7 of itself, which shifts no draw.
+          // But where little is left, because p and q are nearly equal, a second pass counts again.
           const double to_c = c_q + (rejected == 0 ? 1.0 : left);
-          double sums[4] = {0.0, 0.0, 0.0, 0.0};
-          if (rejected == 0)
-            pass(std::true_type(), sums, 1.0 / p.sum, to_c / q.sum);
-          else
+          double z;
+          if (rejected == 0) {
+#pragma unroll 1
+            for (bool again = false;; again = true) {
+              double sums[4] = {0.0, 0.0, 0.0, 0.0};
+              const double p0 = p.sum, q0 = q.sum;
+              last_rp = 1.0 / p0, last_rq = 1.0 / q0;
+              pass(std::true_type(), sums, last_rp, last_rq);
+              exchange_sums(sums);
+              if (!again) p.sum = shared_sum(0), q.sum = shared_sum(1);
+              z = shared_sum(2) / p.sum - shared_sum(3) / q.sum;
+              if (again || !(fabs(q0 * p.sum - p0 * q.sum) > 0x1p-16 * z * (p0 * q.sum))) break;
+            }
+          } else {
+            double sums[4] = {0.0, 0.0, 0.0, 0.0};
             drop(sums, last_rp, last_rq, 1.0 / p.sum, to_c / q.sum);
-          last_rp = 1.0 / p.sum, last_rq = to_c / q.sum;
-          exchange_sums(sums);
-          if (!sharp) p.sum = shared_sum(0), q.sum = shared_sum(1);
-          sharp = true;
-          const double z = shared_sum(2) / p.sum - to_c * (shared_sum(3) / q.sum);
+            last_rp = 1.0 / p.sum, last_rq = to_c / q.sum;
+            exchange_sums(sums);
+            z = shared_sum(2) / p.sum - to_c * (shared_sum(3) / q.sum);
+          }
           // (Nothing but rounding is left where p and q are equal: w stays.)
           summed = z > 1e-13;
           if (summed) c_q = to_c, left = z;

@@ -1,5 +1,5 @@
 """Draft verification where the outcome hangs on a sum's last bits: certain tokens, rows at the ends of
-their type.
+their type, and what rejections leave.
 
 No tolerances: a path, its length and the token are those of the definition in 64 bits, whose own
 rounding moves a border by some 1e-15, or 1e-15 over what is left, where a number of the inputs lies
@@ -68,3 +68,23 @@ def test_rows_at_the_ends_of_the_type(cuda, draft):
             check_verify(logits, tokens, uniform, None, d, temperature)
     bf = logits.clamp(torch.finfo(torch.bfloat16).min, torch.finfo(torch.bfloat16).max).bfloat16()
     check_verify(bf, tokens, uniform, None, bf.roll(1, 0) if draft else None)
+
+
+# ---------------------------------------------------------------- what rejections leave
+@pytest.mark.parametrize("near", [1e-2, 1e-4, 1e-6])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_rows_that_are_nearly_equal(cuda, near, cap):
+    """A draft model that is nearly the target and a draft that falls all the same: the token is drawn from
+    the little that is left."""
+    B, V = 60, 5000
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    logits = torch.randn((B, 2, V), generator=gen, device="cuda") * 2
+    d = logits if not cap else cap * torch.tanh(logits / cap)
+    d = d + near * torch.randn((B, 2, V), generator=gen, device="cuda")
+    p, q = shares(logits[:, 0], 1.0, cap), shares(d[:, 0], 1.0)
+    tokens = ((q - p) / q).argmax(1, keepdim=True)
+    tokens = torch.cat([torch.zeros_like(tokens), tokens], 1)
+    uniform = torch.rand((B, 2), generator=gen, device="cuda")
+    uniform[:, 1] = 1 - 2.0 ** -24
+    path, taken, _ = check_verify(logits, tokens, uniform, None, d, 1.0, cap)
+    assert int((taken == 1).sum()) > (B // 2 if near > 1e-6 else 0)
