@@ -14,6 +14,8 @@
 // a node's row only when the walk is there.  Per node a pass for the maximum and the sum in fp32
 // (bound by the row's latency and bytes), then numbers that every CTA derives alike.
 //
+// A number that lies within the fp32 sums' error of the border where its token stands or falls is measured
+// again by sums in 64 bits (one in some ten thousand; every one where a range of levels is too wide for fp32).
 // What is drawn must not depend on how a sum is rounded: a boundary of the 262144 moves the token
 // when it crosses u_0, and the boundaries' errors add up.  In fp32 (about 1e-8 each) one draw in
 // a thousand would differ, so what is drawn from is computed in 64 bits: 2^x from a table of 32
@@ -42,6 +44,13 @@ namespace w8 {
 
 static __device__ int g_verify_status = 0;
 
+// Weights of a row's logits: 2^(level - ref), the level a logit in log2 units of its probability.
+struct VerifyScale {
+  float most;               // 20 caps: tanh is 1 to 2^-57 from there on
+  float slope, two_over_cap, cap_slope;  // for fp32
+  double in, out, twice;    // log2(e) 2 / cap, cap slope (slope without a cap), 2 cap slope
+};
+
 struct VerifyArgs {
   const void *x, *d;       // target's and draft model's logits [B, N, V]; d may be null
   int64_t x_b, x_n, d_b, d_n;
@@ -55,7 +64,9 @@ struct VerifyArgs {
   int n, vocab, per;       // per: values of a CTA's part (a multiple of 8)
   int greedy;
   double cap, slope;       // slope: log2(e) / temperature, of y or (without a cap) the logit
-  double range;            // logits of 1000 levels
+  float range;             // logits of 1000 levels
+  VerifyScale target, drafted;  // (here, so that they take no registers)
+  float err;               // what a fp32 sum may be off by, relative to it; 1 and more: anything
 };
 
 constexpr int kVerifyThreads = 512;
@@ -114,13 +125,6 @@ __device__ __forceinline__ double exp2_64(double t, const double* table) {
   const double u = table[k & 31], s = fma(u * g, p, u);
   return __hiloint2double(__double2hiint(s) + ((k >> 5) << 20), __double2loint(s));
 }
-// Weights of a row's logits: 2^(level - ref), the level a logit in log2 units of its probability.
-struct VerifyScale {
-  bool deep;                // a capped row's levels may differ by more than 900
-  float most;               // 20 caps: tanh is 1 to 2^-57 from there on
-  float slope, two_over_cap, cap_slope;  // for fp32
-  double in, out, twice;    // log2(e) 2 / cap, cap slope (slope without a cap), 2 cap slope
-};
 // One row's probabilities: 2^(level - ref) / sum.  Without a cap ref is the largest logit's level and levels
 // are differences of logits, scaled: a level by itself, rounded to fp32, would be off by 2^-24 of it, 1e-3
 // at a temperature of 1e-3.  The largest logit's weight is 1 in fp32 and (to 2^-52 of ref) in 64 bits.
@@ -130,12 +134,15 @@ struct VerifyRow {
   double sum;
   bool fine;  // the row has a finite largest logit and no NaN
 };
+// The softcap of the target's rows: none, one whose levels differ by 900 at most, or a wider one (above
+// 312 temperatures), whose weights may pass what a double holds.
+enum : int { kNoCap = 0, kCap = 1, kWideCap = 2 };
 // In 64 bits, without branches: the values of a thread are to be under way together.
-template <bool kCapped>
+template <int kCapped>
 __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, const VerifyRow& row, const double* table) {
   double w;
   bool none;
-  if constexpr (!kCapped) {
+  if constexpr (kCapped == kNoCap) {
     none = x < row.least;
     w = exp2_64(fma(static_cast<double>(fmaxf(x, row.least)), row.out, -row.ref), table);
   } else {
@@ -144,10 +151,11 @@ __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, const
     const double d = 1.0 + exp2_64(static_cast<double>(xc) * c.in, table);
     float r32;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r32) : "f"(static_cast<float>(d)));
-    const double r0 = static_cast<double>(r32), r = fma(r0, fma(-d, r0, 1.0), r0);
+    const double r0 = static_cast<double>(r32);
+    const double r = fma(r0, fma(-d, r0, 1.0), r0);
     double t = fma(-c.twice, r, c.out - row.ref);
     none = x == -INFINITY;
-    if (c.deep) {
+    if constexpr (kCapped == kWideCap) {
       none = none || t < -1000.0;
       t = fmax(t, -1000.0);
     }
@@ -168,9 +176,9 @@ __device__ __forceinline__ float ex2_32(float x) {
   return y;
 }
 // A logit's level less the row's largest one's.
-template <bool kCapped>
+template <int kCapped>
 __device__ __forceinline__ float below_32(float x, const VerifyScale& c, const VerifyRow& row) {
-  if constexpr (kCapped) return level_32(x, c) - row.top;
+  if constexpr (kCapped != kNoCap) return level_32(x, c) - row.top;
   return (x - row.top) * c.slope;
 }
 
@@ -317,8 +325,10 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_greedy_kernel(con
 }
 
 // ---------------------------------------------------------------- sampling
-template <typename E, bool kCapped, bool kDraft>
-__global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const VerifyArgs a) {
+// (Without draft logits two CTAs fit an SM, so that clusters may be larger: 16 chains of 6 in 39 us where one
+// CTA an SM, without the spills, takes 53.)
+template <typename E, int kCapped, bool kDraft>
+__global__ void __launch_bounds__(kVerifyThreads, kDraft || kCapped == kWideCap ? 1 : 2) draft_verify_kernel(const VerifyArgs a) {
   __shared__ VerifyTree tree;
   __shared__ double table[32];
   __shared__ float2 tops[2][kVerifyWarps];               // (largest level, sum) of a warp's part of p and q
@@ -332,19 +342,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
   const VerifyPlace at = verify_place(a);
   const int b = at.b, rank = at.rank, ranks = at.ranks, lo = at.lo, hi = at.hi;
   if (tid < 32) table[tid] = exp2(tid / 32.0);
-  VerifyScale drafted = {};
-  drafted.slope = static_cast<float>(a.slope);
-  drafted.out = a.slope;
-  VerifyScale target = drafted;
-  if constexpr (kCapped) {
-    target.most = static_cast<float>(20.0 * a.cap);
-    target.two_over_cap = static_cast<float>(2.0 * 1.4426950408889634 / a.cap);
-    target.cap_slope = static_cast<float>(a.cap * a.slope);
-    target.in = 2.0 * 1.4426950408889634 / a.cap;
-    target.out = a.cap * a.slope;
-    target.twice = 2.0 * target.out;
-    target.deep = target.twice > 900.0;
-  }
+  const VerifyScale &target = a.target, &drafted = a.drafted;
   // Chunks of `turns` times 256 values, a warp each.
   const int turns = max(1, (a.per + 256 * kVerifyChunks - 1) / (256 * kVerifyChunks));
   const int chunks = hi > lo ? (hi - lo + 256 * turns - 1) / (256 * turns) : 0;
@@ -386,12 +384,14 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
   };
   auto shared_sum = [&](int i) { return warp_sum(lane < ranks ? shared[turn][i][lane] : 0.0); };
 
-  // The largest levels and the sums of a target row and (if asked for) a draft row in fp32.
-  auto stats = [&](const E* xr, const E* dr, bool two, VerifyRow& p, VerifyRow& q) {
+  // The largest levels and the sums of a target row and (if asked for, which the compiler is to know: one
+  // loop for both cases took 1 us a node more) a draft row in fp32.
+  auto stats = [&](const E* xr, const E* dr, auto both, VerifyRow& p, VerifyRow& q) {
+    constexpr bool two = decltype(both)::value;
     const bool wx = verify_on16(xr), wd = verify_on16(dr);
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // of levels (a capped row) or logits
     bool bad[2] = {false, false};
-    auto slope = [&](int r) { return kCapped && r == 0 ? 1.f : drafted.slope; };
+    auto slope = [&](int r) { return kCapped != kNoCap && r == 0 ? 1.f : drafted.slope; };
     auto add = [&](const float (&y)[kVerifyVec], int r) {
       float most = y[0];
 #pragma unroll
@@ -409,18 +409,18 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
 #pragma unroll
       for (int i = 0; i < kVerifyVec; ++i) {
         bad[r] |= !(x[i] < INFINITY);
-        y[i] = kCapped && r == 0 ? level_32(x[i], target) : x[i];
+        y[i] = kCapped != kNoCap && r == 0 ? level_32(x[i], target) : x[i];
       }
       add(y, r);
     };
     constexpr int kBatch = 2;  // loads of a thread and row under way
     int v = lo + tid * kVerifyVec;
-    if (wx && (!kDraft || !two || wd))
+    if (wx && (!two || wd))
       for (; v + (kBatch - 1) * kVerifyStep + kVerifyVec <= hi; v += kBatch * kVerifyStep) {
         Raw8<E> rx[kBatch], ry[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) rx[k].load(xr + v + k * kVerifyStep);
-        if (kDraft && two) {
+        if constexpr (two) {
 #pragma unroll
           for (int k = 0; k < kBatch; ++k) ry[k].load(dr + v + k * kVerifyStep);
         }
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
           rx[k].get(x);
           take(x, 0);
         }
-        if (kDraft && two) {
+        if constexpr (two) {
 #pragma unroll
           for (int k = 0; k < kBatch; ++k) {
             ry[k].get(x);
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       float x[kVerifyVec];
       load8<E>(xr, v, hi, wx, x);
       take(x, 0);
-      if (kDraft && two) {
+      if constexpr (two) {
         load8<E>(dr, v, hi, wd, x);
         take(x, 1);
       }
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
       return make_float2(to, s);
     };
-    constexpr int kRows = kDraft ? 2 : 1;
+    constexpr int kRows = two ? 2 : 1;
     float2 t[2];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -479,19 +479,23 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       out.sum = static_cast<double>(c.y);
       out.fine = c.y > 0.f && c.y < INFINITY && c.x > -INFINITY && c.x < INFINITY;
       out.ref = out.top, out.out = 0.0, out.least = out.top;
-      if (!kCapped || r != 0) {
+      if (kCapped == kNoCap || r != 0) {
         // (From 2^40 levels on the next lower fp32 number is 2^16 below: the largest logit's weight is 1,
         // every other one's 0.)
-        const double ref = static_cast<double>(out.top) * scale.out;
-        const bool far = !(fabs(ref) < 0x1p40);
-        out.ref = far ? 0.0 : ref;
-        out.out = far ? 0.0 : scale.out;
-        if (!far) out.least = __double2float_ru(static_cast<double>(out.top) - a.range);
+        const float levels = fabsf(out.top) * scale.slope;
+        if (levels < 0x1p40f) {
+          out.ref = static_cast<double>(out.top) * scale.out, out.out = scale.out;
+          out.least = __fsub_ru(out.top, a.range);
+          if (levels > 0x1p28f)  // (ref is rounded to 2^-53 of it)
+            out.sum *= fma(fma(static_cast<double>(out.top), out.out, -out.ref), 0.6931471805599453, 1.0);
+        } else {
+          out.ref = 0.0;
+        }
       }
       return out;
     };
     p = row(0, target);
-    if (kDraft && two) q = row(1, drafted);
+    if constexpr (two) q = row(1, drafted);
   };
 
   int cur = 0, taken = 1;
@@ -511,16 +515,22 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       u_c0 = u[c0];
     }
     VerifyRow p, q = {0.f, 0.f, 0.0, 0.0, 1.0, true};
-    stats(xr, dr, c < a.n, p, q);
+    if (kDraft && c < a.n)
+      stats(xr, dr, std::bool_constant<kDraft>(), p, q);
+    else
+      stats(xr, dr, std::false_type(), p, q);
     if (!p.fine) break;
     // After rejections w is max(p - c q, 0) / left: c = 0 and left = 1 at first, and of that less q what
-    // is positive is max(p - (c + left) q, 0).
-    double c_q = 0.0, left = 1.0;
-    int rejected = 0;     // without draft logits: their tokens' weights are taken, `left` stays
+    // is positive is max(p - (c + left) q, 0).  Without draft logits the rejected tokens' weights are taken
+    // away and left is the others' sum, which may be off by `slack`.
+    double c_q = 0.0, left = kDraft ? 1.0 : p.sum;
+    double slack = kDraft ? 0.0 : a.err < 1.f ? a.err * p.sum : INFINITY;
+    int rejected = 0;
+    bool sharp = false;   // the sums are in 64 bits (with draft logits)
     bool summed = false;  // shared[turn][2, 3] and the chunks have the last pass's parts of p and q
     const bool wx = verify_on16(xr), wd = kDraft && verify_on16(dr);
     auto p_of = [&](float x) { return weight_64<kCapped>(x, target, p, table); };
-    auto q_of = [&](float x) { return weight_64<false>(x, drafted, q, table); };
+    auto q_of = [&](float x) { return weight_64<kNoCap>(x, drafted, q, table); };
     auto taken_away = [&](int v) {  // (without draft logits)
       bool was = false;
       for (int i = 0; i < rejected; ++i) was |= gone[i] == v;
@@ -594,7 +604,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
     // fp32 tells which cannot have been (what it may be off by is 2^-18 of the levels); the others,
     // 32 at a time, are looked at in 64 bits, and those dropped taken off the chunk's and the CTA's sums.
     auto drop = [&](double (&sums)[4], double rp0, double rq0, double rp, double rq) {
-      const float slack = 0x1p-18f * (kCapped ? fabsf(p.top) + target.cap_slope : 0.f) + 0x1p-22f;
+      const float slack = 0x1p-18f * (kCapped != kNoCap ? fabsf(p.top) + target.cap_slope : 0.f) + 0x1p-22f;
       const float at0 = static_cast<float>(log2(rq0 / rp0)) - slack, at1 = static_cast<float>(log2(rq / rp)) + slack;
       if (tid == 0) sums[2] = shared[turn][2][rank], sums[3] = shared[turn][3][rank];
       uint8_t* mine = queue[kDraft ? warp : 0];
@@ -610,7 +620,7 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
           int n = 0;
 #pragma unroll
           for (int i = 0; i < kVerifyVec; ++i) {
-            const float lp = below_32<kCapped>(x[i], target, p), lq = below_32<false>(y[i], drafted, q), d = lp - lq;
+            const float lp = below_32<kCapped>(x[i], target, p), lq = below_32<kNoCap>(y[i], drafted, q), d = lp - lq;
             const float off = 0x1p-18f * (fabsf(lp) + fabsf(lq));
             // (p = 0 < q was dropped before; q = 0 is never)
             const bool near = lp != -INFINITY && lq != -INFINITY && !(d > at1 + off) && !(d < at0 - off);
@@ -638,10 +648,22 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
       for (; c < a.n; c = child_after(a, at, tree, cur, c)) {
         const int t = tree.tokens[c];
         const double uc = static_cast<double>(c == c0 ? u_c0 : u[c]);
-        const double pt = p_of(c == c0 ? x0 : logit_f32<E>(xr[t])) / p.sum;
+        double pw = p_of(c == c0 ? x0 : logit_f32<E>(xr[t]));
         if constexpr (!kDraft) {
           const bool was = taken_away(t);
-          if (uc < (was ? 0.0 : left > 0.0 ? pt / left : pt)) {
+          if (was) pw = 0.0;
+          bool stands = uc * left < pw;
+          if (pw > 0.0 && !(fabs(uc * left - pw) > uc * slack)) {
+            // The number lies so near the border that the sum in 64 bits decides (of what is left: where that
+            // is little, a difference of sums would not do).
+            double sums[4] = {0.0, 0.0, 0.0, 0.0};
+            pass(std::false_type(), sums, 0.0, 0.0);
+            exchange_sums(sums);
+            left = shared_sum(2), slack = 0x1p-44 * left;
+            summed = left > 0.0;
+            stands = uc * left < pw;
+          }
+          if (stands) {
             went = c;
             break;
           }
@@ -649,35 +671,51 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_kernel(const Veri
           if (!was) {
             if (tid == 0) gone[rejected] = t;
             ++rejected;
-            left -= pt;
+            left -= pw;
+            summed = false;
           }
           __syncthreads();
         } else {
-          const double qt = q_of(c == c0 ? d0 : logit_f32<E>(dr[t])) / q.sum;
-          if (uc * qt < fmax(pt - c_q * qt, 0.0) / left) {
+          const double qw = q_of(c == c0 ? d0 : logit_f32<E>(dr[t]));
+          // u q < max(p - c q, 0) / left, without divisions
+          auto decide = [&]() { return uc * left * (qw * p.sum) < fmax(fma(-c_q, qw * p.sum, pw * q.sum), 0.0); };
+          const double to_c = c_q + (rejected == 0 ? 1.0 : left);
+          bool stands;
+          double z = 0.0;
+          if (sharp) {
+            stands = decide();
+          } else {
+            // The first child.  It stands by more than the fp32 sums may be off by; or a pass in 64 bits, which
+            // its rejection needs anyway: with the sums of p and q by themselves over the values that stay
+            // positive after it, which the fp32 sums tell, one pass gives the sums over all besides.  Those
+            // sums move the border p = q by some 10^-7 of it: what lies between (10^-7 of the probability,
+            // where p / q is spread) is miscounted by 10^-7 of itself, which shifts no draw.  But where little
+            // is left, because p and q are nearly equal, a second pass counts again.
+            const double l = uc * (qw * p.sum), r = pw * q.sum;
+            stands = r - l > a.err * (l + r);
+            if (!stands) {
+#pragma unroll 1
+              for (bool again = false;; again = true) {
+                double sums[4] = {0.0, 0.0, 0.0, 0.0};
+                last_rp = 1.0 / p.sum, last_rq = 1.0 / q.sum;
+                pass(std::true_type(), sums, last_rp, last_rq);
+                exchange_sums(sums);
+                if (!again) {
+                  p.sum = shared_sum(0), q.sum = shared_sum(1);
+                  sharp = true;
+                  stands = decide();
+                }
+                z = shared_sum(2) / p.sum - shared_sum(3) / q.sum;
+                if (again || stands || !(fabs(p.sum * last_rp - q.sum * last_rq) > 0x1p-16 * z)) break;
+              }
+            }
+          }
+          if (stands) {
             went = c;
             break;
           }
-          // Rejected: what is left, in 64 bits.  With the sums of p and q by themselves over the values that
-          // stay positive, the first pass gives the sums over all besides.  Which values stay it takes from the
-          // fp32 sums.  Those move the border p = q by some 10^-7 of it: what lies between (10^-7 of the
-          // probability, where p / q is spread) is miscounted by 10^-7 of itself, which shifts no draw.
-          // But where little is left, because p and q are nearly equal, a second pass counts again.
-          const double to_c = c_q + (rejected == 0 ? 1.0 : left);
-          double z;
-          if (rejected == 0) {
-#pragma unroll 1
-            for (bool again = false;; again = true) {
-              double sums[4] = {0.0, 0.0, 0.0, 0.0};
-              const double p0 = p.sum, q0 = q.sum;
-              last_rp = 1.0 / p0, last_rq = 1.0 / q0;
-              pass(std::true_type(), sums, last_rp, last_rq);
-              exchange_sums(sums);
-              if (!again) p.sum = shared_sum(0), q.sum = shared_sum(1);
-              z = shared_sum(2) / p.sum - shared_sum(3) / q.sum;
-              if (again || !(fabs(q0 * p.sum - p0 * q.sum) > 0x1p-16 * z * (p0 * q.sum))) break;
-            }
-          } else {
+          // Rejected: what is left.
+          if (rejected > 0) {
             double sums[4] = {0.0, 0.0, 0.0, 0.0};
             drop(sums, last_rp, last_rq, 1.0 / p.sum, to_c / q.sum);
             last_rp = 1.0 / p.sum, last_rq = to_c / q.sum;
@@ -859,13 +897,21 @@ static int verify_launch(Kern kern, int (&held)[64][w8::kVerifyCluster + 1], w8:
   for (int c = 2; c <= w8::kVerifyCluster && c * 2048ll <= a.vocab; ++c)
     if (held[device][c] >= batch) cluster = c;
   a.per = static_cast<int>(((a.vocab + cluster - 1) / cluster + 7) / 8 * 8);
+  // A thread's fp32 sum is of `values` numbers, which it scales at every eighth at most, by an exponential
+  // (2^-22); the warps' and CTAs' sums, the exponentials and the roundings of their arguments (3 2^-24 of
+  // each; their mean over the weights is below the logarithm of the vocabulary) are 158 2^-24 more.  A
+  // capped level is off by some 2^-21 of its range.  4 / 3 of that below 1 / 4, where a quotient is
+  // off by so much more.
+  const double values = static_cast<double>((a.per + w8::kVerifyStep - 1) / w8::kVerifyStep * w8::kVerifyVec);
+  const double err = 0x1p-24 * (2.0 * values + 160.0) + 0x1p-20 * a.cap * a.slope;
+  a.err = err < 0.25 ? static_cast<float>(1.5 * err) : 1.f;
   cfg.gridDim = dim3(static_cast<unsigned>(batch * cluster), 1, 1);
   attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   cfg.numAttrs = 2;
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
-template <typename E, bool kCapped, bool kDraft>
+template <typename E, int kCapped, bool kDraft>
 static int verify_sample(const w8::VerifyArgs& a, int64_t batch, int device, cudaStream_t stream) {
   static int held[64][w8::kVerifyCluster + 1] = {};
   return verify_launch(w8::draft_verify_kernel<E, kCapped, kDraft>, held, a, batch, device, stream);
@@ -877,11 +923,15 @@ static int verify_go(const w8::VerifyArgs& a, int64_t batch, int device, cudaStr
     static int held[64][w8::kVerifyCluster + 1] = {};
     return verify_launch(w8::draft_verify_greedy_kernel<E>, held, a, batch, device, stream);
   }
+  using namespace w8;
+  if (2.0 * a.cap * a.slope > 900.0)
+    return a.d != nullptr ? verify_sample<E, kWideCap, true>(a, batch, device, stream)
+                          : verify_sample<E, kWideCap, false>(a, batch, device, stream);
   if (a.cap > 0.0)
-    return a.d != nullptr ? verify_sample<E, true, true>(a, batch, device, stream)
-                          : verify_sample<E, true, false>(a, batch, device, stream);
-  return a.d != nullptr ? verify_sample<E, false, true>(a, batch, device, stream)
-                        : verify_sample<E, false, false>(a, batch, device, stream);
+    return a.d != nullptr ? verify_sample<E, kCap, true>(a, batch, device, stream)
+                          : verify_sample<E, kCap, false>(a, batch, device, stream);
+  return a.d != nullptr ? verify_sample<E, kNoCap, true>(a, batch, device, stream)
+                        : verify_sample<E, kNoCap, false>(a, batch, device, stream);
 }
 
 }  // namespace w8host
@@ -916,7 +966,19 @@ extern "C" int w8_draft_verify(const w8_draft_verify_args* in, w8_stream_t strea
   a.greedy = greedy;
   a.cap = greedy ? 0.0 : x.cap;
   a.slope = greedy ? 1.0 : 1.4426950408889634 / x.temperature;
-  a.range = 1000.0 / a.slope;
+  a.range = static_cast<float>(1000.0 / a.slope);
+  a.drafted.slope = static_cast<float>(a.slope);
+  a.drafted.out = a.slope;
+  a.target = a.drafted;
+  if (a.cap > 0.0) {
+    constexpr double kLog2e = 1.4426950408889634;
+    a.target.most = static_cast<float>(20.0 * a.cap);
+    a.target.two_over_cap = static_cast<float>(2.0 * kLog2e / a.cap);
+    a.target.cap_slope = static_cast<float>(a.cap * a.slope);
+    a.target.in = 2.0 * kLog2e / a.cap;
+    a.target.out = a.cap * a.slope;
+    a.target.twice = 2.0 * a.target.out;
+  }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (x.dtype == W8_FP32) return verify_go<float>(a, x.batch, device, s);
   if (x.dtype == W8_BF16) return verify_go<__nv_bfloat16>(a, x.batch, device, s);

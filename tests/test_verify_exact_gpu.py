@@ -1,5 +1,6 @@
-"""Draft verification where the outcome hangs on a sum's last bits: certain tokens, rows at the ends of
-their type, and what rejections leave.
+"""Draft verification where the outcome hangs on a sum's last bits: certain tokens, numbers beside the
+border of standing and falling, the ends of the accepted temperatures and caps, and what rejections
+leave.
 
 No tolerances: a path, its length and the token are those of the definition in 64 bits, whose own
 rounding moves a border by some 1e-15, or 1e-15 over what is left, where a number of the inputs lies
@@ -10,6 +11,7 @@ import math
 import pytest
 import torch
 
+import gemma_npu_b200 as w8
 from test_paged_gpu import check_verify
 
 pytestmark = pytest.mark.gpu
@@ -70,6 +72,114 @@ def test_rows_at_the_ends_of_the_type(cuda, draft):
     check_verify(bf, tokens, uniform, None, bf.roll(1, 0) if draft else None)
 
 
+@DRAFTS
+@pytest.mark.parametrize("cap", [30.0, 1e4, 1e6])
+@pytest.mark.parametrize("temperature", [1e-3, 0.1, 1.0])
+def test_certain_tokens_stand_under_a_cap(cuda, temperature, cap, draft):
+    """The same under a softcap, whose levels fp32 has to 2^-21 of their range."""
+    B, N, V = 160, 3, 2000
+    logits = torch.zeros((B, N, V), device="cuda")
+    tokens = (torch.arange(B, device="cuda")[:, None] * 37 + torch.arange(N, device="cuda")) % V
+    high = 63.625 - torch.arange(B, device="cuda") / 16.0
+    logits.scatter_(2, tokens.roll(-1, 1)[:, :, None], high[:, None, None].expand(B, N, 1))
+    uniform = torch.full((B, N), 1 - 2.0 ** -24, device="cuda")
+    uniform[1::3] = 1 - 2.0 ** -20
+    uniform[2::3] = 0.5
+    path, taken, token = check_verify(logits, tokens, uniform, None, logits if draft else None, temperature, cap)
+    assert taken.tolist() == [N] * B and bool((token == tokens[:, 0]).all())
+
+
+# ---------------------------------------------------------------- the accepted range
+# (cap, temperature, the logits' middle, their spread): rows of a few hundred probable tokens each.
+RANGE = [(0.0, 1e-3, 60.0, 4e-3), (0.0, 0.05, 60.0, 0.2), (0.0, 1.0, 20.0, 4.0), (0.0, 1e3, 0.0, 3e3), (0.0, 1.0, 6e4, 4.0),
+         (30.0, 1e-3, 10.0, 4e-3), (30.0, 0.01, 25.0, 0.1), (30.0, 1.0, 20.0, 8.0), (100.0, 1.0, 0.0, 5.0),
+         (1e4, 1.0, 20.0, 4.0), (1e5, 0.05, 20.0, 0.2), (1e6, 1.0, 20.0, 4.0), (1e6, 1.0, 1e6, 8.0),
+         (1e-3, 1e-3, 0.0, 1e-3), (0.5, 0.02, 0.0, 0.5)]
+
+
+def case_of(seed, B, N, V, middle, spread, near=0.3):
+    """Target rows, rows of a draft model beside them, drafts drawn from those (of node 0's rows)."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    logits = middle + spread * torch.randn((B, N, V), generator=gen, device="cuda")
+    d = logits + near * spread * torch.randn((B, N, V), generator=gen, device="cuda")
+    return logits, d, gen
+
+
+@pytest.mark.parametrize("cap,temperature,middle,spread", RANGE)
+def test_draws_over_the_whole_range(cuda, cap, temperature, middle, spread):
+    """Tokens drawn from rows without drafts."""
+    logits, _, gen = case_of(7, 400, 1, 6000, middle, spread)
+    uniform = torch.rand((400, 1), generator=gen, device="cuda")
+    check_verify(logits, torch.zeros((400, 1), dtype=torch.int64, device="cuda"), uniform, None, None, temperature, cap)
+
+
+@DRAFTS
+@pytest.mark.parametrize("cap,temperature,middle,spread", RANGE)
+def test_the_whole_range(cuda, cap, temperature, middle, spread, draft):
+    B, N, V = 40, 5, 6000
+    logits, d, gen = case_of(1, B, N, V, middle, spread)
+    parent = torch.tensor([-1, 0, 0, 1, 0], dtype=torch.int32, device="cuda")
+    up = torch.tensor([0, 0, 0, 1, 0], device="cuda")
+    q = shares(d, temperature)[:, up]
+    tokens = torch.multinomial(q.flatten(0, 1).float(), 1, generator=gen).view(B, N)
+    uniform = torch.rand((B, N), generator=gen, device="cuda")
+    check_verify(logits, tokens, uniform, parent, d if draft else None, temperature, cap)
+
+
+def check_border(cap, temperature, middle, spread, draft):
+    """A draft's number is the next one below, at or above w / q in fp32, at up to 8 steps from it."""
+    B, V = 68, 6000
+    logits, d, gen = case_of(2, B, 2, V, middle, spread)
+    p, q = shares(logits[:, 0], temperature, cap), shares(d[:, 0], temperature)
+    if draft:
+        tokens = torch.multinomial(torch.where(q > p, q, 0.0).float() + 1e-30, 1, generator=gen)
+        border = (p.gather(1, tokens) / q.gather(1, tokens))[:, 0]
+    else:
+        tokens = torch.multinomial(p.float(), 1, generator=gen)
+        border = p.gather(1, tokens)[:, 0]
+    steps = (torch.arange(B, device="cuda") % 17 - 8).int()
+    u = (border.float().view(torch.int32) + steps).view(torch.float32).clamp(0, 1 - 2.0 ** -24)
+    uniform = torch.stack([torch.rand(B, generator=gen, device="cuda"), u], 1)
+    tokens = torch.cat([torch.zeros_like(tokens), tokens], 1)
+    path, taken, _ = check_verify(logits, tokens, uniform, None, d if draft else None, temperature, cap)
+    assert 10 < int((taken == 2).sum()) < 58
+
+
+@DRAFTS
+@pytest.mark.parametrize("cap,temperature,middle,spread", RANGE)
+def test_numbers_beside_the_border(cuda, cap, temperature, middle, spread, draft):
+    check_border(cap, temperature, middle, spread, draft)
+
+
+@pytest.mark.parametrize("temperature", [0.25, 0.7, 1.0])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_what_a_dominant_rejected_token_leaves(cuda, cap, temperature):
+    """The first chosen draft has all but 2^-21 of the probability and falls: the drafts after it are
+    measured by what is left."""
+    B, V = 60, 32000
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    logits = torch.randn((B, 4, V), generator=gen, device="cuda").clamp(-4, 4) * 0.3
+    first = torch.randint(0, V, (B,), generator=gen, device="cuda")
+    low, up = 0.0, 100.0  # of the first draft's logit
+    for _ in range(60):
+        high = (low + up) / 2
+        logits[:, 0].scatter_(1, first[:, None], high)
+        left = 1 - float(shares(logits[0, 0], temperature, cap)[first[0]])
+        low, up = (high, up) if left > 2.0 ** -21 else (low, high)
+    logits[torch.arange(B), 0, (first + 1) % V] = 3.0
+    w = shares(logits[:, 0], temperature, cap)
+    w.scatter_(1, first[:, None], 0.0)
+    w /= w.sum(1, keepdim=True)
+    second = (first + 1) % V
+    border = w.gather(1, second[:, None])[:, 0]
+    uniform = torch.rand((B, 4), generator=gen, device="cuda")
+    uniform[:, 1] = 1 - 2.0 ** -24
+    uniform[:, 2] = (border * (1 + (torch.arange(B, device="cuda") % 11 - 5.5) * 1e-5)).float()
+    tokens = torch.stack([torch.zeros_like(first), first, second, (first + 5) % V], 1)
+    parent = torch.tensor([-1, 0, 0, 0], dtype=torch.int32, device="cuda")
+    check_verify(logits, tokens, uniform, parent, None, temperature, cap)
+
+
 # ---------------------------------------------------------------- what rejections leave
 @pytest.mark.parametrize("near", [1e-2, 1e-4, 1e-6])
 @pytest.mark.parametrize("cap", [0.0, 30.0])
@@ -88,3 +198,22 @@ def test_rows_that_are_nearly_equal(cuda, near, cap):
     uniform[:, 1] = 1 - 2.0 ** -24
     path, taken, _ = check_verify(logits, tokens, uniform, None, d, 1.0, cap)
     assert int((taken == 1).sum()) > (B // 2 if near > 1e-6 else 0)
+
+
+def test_the_targets_distribution_with_chosen_drafts(cuda):
+    """Chosen drafts, however they were chosen without the numbers: the first token after node 0 has the
+    target's frequencies (6 deviations of a count)."""
+    B, V = 60000, 6
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    row = torch.randn(V, generator=gen, device="cuda")
+    logits = row.expand(B, 4, V).contiguous()
+    parent = torch.tensor([-1, 0, 0, 0], dtype=torch.int32, device="cuda")
+    p = shares(row, 1.0)
+    uniform = torch.rand((B, 4), generator=gen, device="cuda")
+    drawn = torch.multinomial(torch.full((B, V), 1.0, device="cuda"), 4, replacement=True, generator=gen)
+    best = row.argsort(descending=True)[:4].roll(1).expand(B, 4).contiguous()
+    for tokens in (drawn, best):
+        path, taken, token = w8.draft_verify(logits, tokens, uniform, parent=parent)
+        first = torch.where(taken > 1, tokens.gather(1, path[:, 1:2].long().clamp(min=0))[:, 0], token)
+        count = torch.bincount(first, minlength=V).double()
+        assert bool(((count - B * p).abs() < 6 * (B * p * (1 - p)).sqrt()).all())
