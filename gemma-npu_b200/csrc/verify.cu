@@ -49,6 +49,7 @@ struct VerifyScale {
   float most;               // 20 caps: tanh is 1 to 2^-57 from there on
   float slope, two_over_cap, cap_slope;  // for fp32
   double in, out, twice;    // log2(e) 2 / cap, cap slope (slope without a cap), 2 cap slope
+  double per_cap;           // 1 / cap
 };
 
 struct VerifyArgs {
@@ -135,8 +136,10 @@ struct VerifyRow {
   bool fine;  // the row has a finite largest logit and no NaN
 };
 // The softcap of the target's rows: none, one whose levels differ by 900 at most, or a wider one (above
-// 312 temperatures), whose weights may pass what a double holds.
+// 312 temperatures), whose levels need more care (a kernel of its own: beside the common caps that care cost
+// registers, and with them an SM's second CTA).
 enum : int { kNoCap = 0, kCap = 1, kWideCap = 2 };
+__device__ __noinline__ double tanh_64(double z) { return tanh(z); }
 // In 64 bits, without branches: the values of a thread are to be under way together.
 template <int kCapped>
 __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, const VerifyRow& row, const double* table) {
@@ -152,10 +155,13 @@ __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, const
     float r32;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r32) : "f"(static_cast<float>(d)));
     const double r0 = static_cast<double>(r32);
-    const double r = fma(r0, fma(-d, r0, 1.0), r0);
+    double r = fma(r0, fma(-d, r0, 1.0), r0);
+    if constexpr (kCapped == kWideCap) r = fma(r, fma(-d, r, 1.0), r);
     double t = fma(-c.twice, r, c.out - row.ref);
     none = x == -INFINITY;
     if constexpr (kCapped == kWideCap) {
+      // The exponential's 2^-48 moves a level by up to 2^-49 of their range: of 2^31 levels that is 4e-6.
+      if (c.out > 65536.0) t = fma(c.out, tanh_64(static_cast<double>(xc) * c.per_cap), -row.ref);
       none = none || t < -1000.0;
       t = fmax(t, -1000.0);
     }
@@ -978,6 +984,7 @@ extern "C" int w8_draft_verify(const w8_draft_verify_args* in, w8_stream_t strea
     a.target.in = 2.0 * kLog2e / a.cap;
     a.target.out = a.cap * a.slope;
     a.target.twice = 2.0 * a.target.out;
+    a.target.per_cap = 1.0 / a.cap;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (x.dtype == W8_FP32) return verify_go<float>(a, x.batch, device, s);

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import gemma_npu_b200 as w8
-from test_paged_gpu import check_verify
+from test_paged_gpu import check_verify, want_verify
 
 pytestmark = pytest.mark.gpu
 DRAFTS = pytest.mark.parametrize("draft", [False, True], ids=["chosen", "sampled"])
@@ -126,7 +126,7 @@ def test_the_whole_range(cuda, cap, temperature, middle, spread, draft):
     check_verify(logits, tokens, uniform, parent, d if draft else None, temperature, cap)
 
 
-def check_border(cap, temperature, middle, spread, draft):
+def border_case(cap, temperature, middle, spread, draft):
     """A draft's number is the next one below, at or above w / q in fp32, at up to 8 steps from it."""
     B, V = 68, 6000
     logits, d, gen = case_of(2, B, 2, V, middle, spread)
@@ -141,14 +141,34 @@ def check_border(cap, temperature, middle, spread, draft):
     u = (border.float().view(torch.int32) + steps).view(torch.float32).clamp(0, 1 - 2.0 ** -24)
     uniform = torch.stack([torch.rand(B, generator=gen, device="cuda"), u], 1)
     tokens = torch.cat([torch.zeros_like(tokens), tokens], 1)
-    path, taken, _ = check_verify(logits, tokens, uniform, None, d if draft else None, temperature, cap)
-    assert 10 < int((taken == 2).sum()) < 58
+    return logits, tokens, uniform, d if draft else None, u.double() / border - 1
 
 
 @DRAFTS
 @pytest.mark.parametrize("cap,temperature,middle,spread", RANGE)
 def test_numbers_beside_the_border(cuda, cap, temperature, middle, spread, draft):
-    check_border(cap, temperature, middle, spread, draft)
+    logits, tokens, uniform, d, _ = border_case(cap, temperature, middle, spread, draft)
+    path, taken, _ = check_verify(logits, tokens, uniform, None, d, temperature, cap)
+    assert 10 < int((taken == 2).sum()) < 58
+
+
+@DRAFTS
+@pytest.mark.parametrize("cap,temperature,middle,spread", [(1e6, 0.1, -20.0, 0.4), (1e6, 1e-3, 20.0, 4e-3), (1e6, 1e-3, -3e3, 4e-3),
+                                                           (1e6, 2e-3, 8e4, 0.05), (3e5, 1e-3, 1.5e4, 0.02)])
+def test_numbers_beside_the_border_under_the_widest_caps(cuda, cap, temperature, middle, spread, draft):
+    """Caps of up to 2^30 levels, far above the logits.  Levels (exponents of 2) of size L, up to 6e7 here, are
+    rounded to 64 bits some 4 times, by 2^-53 L, on either side (the softcap's tanh, its product, the
+    quotient by the temperature): each side's w is off by at most 2^-51 L ln 2, and one within 2^-50 L of its
+    border may stand or fall."""
+    logits, tokens, uniform, d, off = border_case(cap, temperature, middle, spread, draft)
+    level = float((cap * torch.tanh(logits[:, 0].double() / cap)).abs().max()) * 1.4427 / temperature
+    clear = (off.abs() > 2.0 ** -50 * level).tolist()
+    path, taken, token = w8.draft_verify(logits, tokens, uniform, draft=d, temperature=temperature, cap=cap)
+    want = want_verify(logits, tokens, uniform, None, d, temperature, cap)
+    got = (path.tolist(), taken.tolist(), token.tolist())
+    for i, on in enumerate(clear):
+        assert not on or [x[i] for x in got] == [x[i] for x in want], i
+    assert 10 < int((taken == 2).sum()) < 58 and sum(clear) > 50
 
 
 @pytest.mark.parametrize("temperature", [0.25, 0.7, 1.0])
