@@ -787,23 +787,27 @@ __global__ void __launch_bounds__(kVerifyThreads, kDraft || kCapped == kWideCap 
           int k = place(k1 - k0, [&](int i) { return of(k0 + i); }, sum_at) + k0;
           k = max(__shfl_sync(0xffffffffu, k, l), 0);  // (a CTA with weight has such a chunk, but for rounding)
           sum_at = __shfl_sync(0xffffffffu, sum_at, l);
-          // The chunk's values, 256 at a time.
-          int last = -1, token = -1;
+          // The chunk's values, 256 at a time.  What further rejections took off a chunk's sums may have left it
+          // some 2^-53 of them and no value: the number then meant the next value that has weight, or
+          // (it may lie at the end of the sums) the last one.
+          const int begin = lo + k * turns * 256, end_own = min(begin + turns * 256, hi);
+          int last = -1, token = -1, v0 = begin;
+          bool own = true, back = false;
 #pragma unroll 1
-          for (int j = 0; j < turns && token < 0; ++j) {
-            const int v = lo + (k * turns + j) * 256 + lane * kVerifyVec;
+          while (true) {
+            const int v = v0 + lane * kVerifyVec, stop = own ? hi : a.vocab;
             float x[kVerifyVec], y[kVerifyVec];
             double f[kVerifyVec], sum = 0.0;
-            load8<E>(xr, v, hi, wx, x);
-            if (kDraft && c_q > 0.0) load8<E>(dr, v, hi, wd, y);
-            int end = -1;
+            load8<E>(xr, v, stop, wx, x);
+            if (kDraft && c_q > 0.0) load8<E>(dr, v, stop, wd, y);
+            int start = 0x7FFFFFFF, end = -1;
 #pragma unroll
             for (int i = 0; i < kVerifyVec; ++i) {
               f[i] = p_of(x[i]) * rp;
               if (kDraft && c_q > 0.0) f[i] = fmax(fma(-rq, q_of(y[i]), f[i]), 0.0);
               if (!kDraft && rejected > 0 && taken_away(v + i)) f[i] = 0.0;
               sum += f[i];
-              if (f[i] > 0.0) end = v + i;
+              if (f[i] > 0.0) start = min(start, v + i), end = v + i;
             }
             double incl = sum;
 #pragma unroll
@@ -812,7 +816,7 @@ __global__ void __launch_bounds__(kVerifyThreads, kDraft || kCapped == kWideCap 
               if (lane >= s) incl += o;
             }
             last = max(last, __reduce_max_sync(0xffffffffu, end));
-            over = __ballot_sync(0xffffffffu, end >= 0 && sum_at + incl > aim);
+            over = __ballot_sync(0xffffffffu, own && end >= 0 && sum_at + incl > aim);
             if (over) {
               double s = sum_at + incl - sum;
               int mine_token = -1;
@@ -823,10 +827,24 @@ __global__ void __launch_bounds__(kVerifyThreads, kDraft || kCapped == kWideCap 
               }
               if (mine_token < 0) mine_token = end;  // (rounding may leave the sum at the aim: the last)
               token = __shfl_sync(0xffffffffu, mine_token, __ffs(over) - 1);
+              break;
             }
             sum_at += __shfl_sync(0xffffffffu, incl, 31);
+            const bool more = own && v0 + 256 < end_own;
+            if (!more && last >= 0) {
+              token = own || back ? last : __reduce_min_sync(0xffffffffu, start);
+              break;
+            }
+            if (back) {
+              if (v0 == 0) break;
+              v0 = max(v0 - 256, 0);
+            } else {
+              v0 = own && !more ? end_own : v0 + 256;
+              own = more;
+              if (!own && v0 >= a.vocab) back = true, v0 = max(begin - 256, 0);
+            }
           }
-          if (lane == 0) a.token[b] = token >= 0 ? token : last >= 0 ? last : lo + k * turns * 256;
+          if (lane == 0) a.token[b] = token;
         } else if (owner < 0 && rank == 0 && lane == 0) {
           a.token[b] = -1;
         }

@@ -220,6 +220,29 @@ def test_rows_that_are_nearly_equal(cuda, near, cap):
     assert int((taken == 1).sum()) > (B // 2 if near > 1e-6 else 0)
 
 
+@pytest.mark.parametrize("u", [0.0, 2.0 ** -24, 1 - 2.0 ** -24])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_the_ends_of_what_several_rejections_leave(cuda, u, cap):
+    """Most of what the first rejection leaves, the front of the vocabulary among it, falls to the second
+    one: the numbers at the ends find the first and last token that is left, and no other."""
+    B, N, V = 96, 4, 70000
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    logits = torch.randn((B, N, V), generator=gen, device="cuda") * 2
+    flat = logits if not cap else cap * torch.tanh(logits / cap)
+    d = flat - 0.05 + 0.002 * torch.rand((B, N, V), generator=gen, device="cuda")  # p / q some 1.07
+    d[:, :, 30000:34000] -= 3.0
+    d[:, :, 34000:60000] += 0.2
+    logits[:, :, 11::97] = -math.inf
+    d[:, :, 30029:34000:89] = -math.inf
+    fall = torch.where(logits[:, 0, 34000:60000] == -math.inf, -math.inf, d[:, 0, 34000:60000])
+    tokens = 34000 + torch.multinomial(torch.softmax(fall, 1), N, generator=gen)
+    parent = torch.tensor([-1, 0, 0, 0], dtype=torch.int32, device="cuda")
+    uniform = torch.full((B, N), 1 - 2.0 ** -24, device="cuda")
+    uniform[:, 0] = u
+    path, taken, token = check_verify(logits, tokens, uniform, parent, d, 1.0, cap)
+    assert taken.tolist() == [1] * B and bool(((token >= 30000) & (token < 34000)).all())
+
+
 def test_the_targets_distribution_with_chosen_drafts(cuda):
     """Chosen drafts, however they were chosen without the numbers: the first token after node 0 has the
     target's frequencies (6 deviations of a count)."""
