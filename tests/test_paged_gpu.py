@@ -252,6 +252,22 @@ def test_attention_scales_far_apart(cuda, H, N, dt):
     check_out(attend(c, *a, scale=0.05), want, dt)
 
 
+@pytest.mark.parametrize("D,KV,H,N", [(64, 1, 8, 1), (128, 2, 8, 1), (256, 1, 8, 1), (512, 1, 8, 1), (512, 1, 16, 2), (256, 1, 16, 16)])
+@DTYPES
+def test_attention_of_queries_off_zero(cuda, D, KV, H, N, dt):
+    """Queries whose elements have a common offset, up to one sign: what pages' keys are raised by, times
+    the queries' sums, has to cancel.  Scores lose more there than about 0, within the bound above; calls
+    repeat to the bit."""
+    c = cache(1, KV, D, 64, [1500, 700], dt)
+    q, kn, vn = new(2, 2, H, KV, D, N, dt)
+    for off in (1.0, 4.0, -30.0):
+        x = (q.float() / 2 + off).to(dt)
+        scale = D ** -0.5 / (1 + abs(off) / 8)
+        got = attend(c, x, kn, vn, scale=scale)
+        check_out(got, want_attention(c, x, kn, vn, scale=scale), dt)
+        assert torch.equal(got, attend(c, x, kn, vn, scale=scale))
+
+
 @pytest.mark.parametrize("D,KV,H,N,lens", [(64, 2, 4, 1, [100, 40, 3]), (128, 1, 8, 2, [1000, 40, 3]), (256, 2, 4, 3, [300, 48, 0]),
                                            (512, 1, 8, 1, [700, 64, 3]), (128, 8, 64, 1, [3000, 700, 2999, 128]),
                                            (128, 1, 8, 20, [1000, 40, 3])])
@@ -548,6 +564,19 @@ def test_append_strides(cuda):
                            vn[:, :, :1].expand(-1, -1, 70, -1) if False else vn)
     for name in want:
         assert same(lens if name == "lens" else got[name], want[name]), name
+
+
+@pytest.mark.parametrize("dims", [(2,), (1,), (0,), (0, 1, 2)])
+def test_append_of_expanded_rows(cuda, dims):
+    """New rows that stand for several tokens, heads or sequences."""
+    c = give_pages(cache(1, 3, 128, 32, [40, 0, 31], spare=12, M=5), 70)
+    _, kn, vn = new(2, 3, 3, 3, 128, 70, torch.bfloat16)
+    for d in dims:
+        kn, vn = kn.narrow(d, 0, 1).expand_as(kn), vn.narrow(d, 1, 1).expand_as(vn)
+    check_append(c, kn, vn)
+    path = torch.tensor([[3, 0, 69], [5, -1, 0], [1, 2, 2]], dtype=torch.int32, device="cuda")
+    check_append(c, kn, vn, path=path)
+    assert w8.device_status() == 0
 
 
 def test_append_reports_what_is_lost(cuda):
