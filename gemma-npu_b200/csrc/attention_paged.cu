@@ -532,8 +532,9 @@ __global__ void __launch_bounds__(PagedCfg<D, NT>::kThreads, 1)
         // ---- S^T = K Q^T.  The 8-bit values go in as 1024 + 128 + k8, exact in fp16, and the sums start
         // from -1152 times Q's: the products cancel to S with what fp32 sums lose at their size, about
         // 2^-23 of 1152 |sum q| against a score's 30 |q| sqrt(D): 10^-5 of it where q's elements cancel in their
-        // sum, sqrt(D) times that where they are of one sign (fp16, D 256 and 512, q 8 to 60 deviations
-        // off 0: outputs are off by up to 0.8 and 1.7 half steps, 0.4 around 0, by the norm a third more or as ever).
+        // sum, sqrt(D) times that where they are of one sign (fp16, q 4 and 30 deviations
+        // off 0: outputs are off by up to 0.8 half steps at D 256 and 1.7 at 512, by 0.4 for q around 0; their
+        // errors' norm grows by a third at D 256 and hardly at 512).
         float s[C::kKT][NT][4];
 #pragma unroll
         for (int kt = 0; kt < C::kKT; ++kt)

@@ -7,7 +7,8 @@
 // A page becomes 8 bits when its last position is appended, all of it at once and from the
 // 16-bit rows themselves: one rounding a value, whatever the order in which the rows came.  Until
 // then they wait in the sequence's tail, which the attention reads as it is.  Indexes come from
-// device memory; one outside its range is skipped and recorded in the device status.
+// device memory; one outside its range is recorded in the device status: a length's or a page's is
+// skipped, a path's puts a row of zeros into the cache, which counts.
 #include "common.cuh"
 
 #include <cuda_fp16.h>
@@ -101,7 +102,7 @@ __device__ __forceinline__ uint2 paged_round8(const float (&x)[8], float m, floa
 // magnitude found and its values rounded from the registers, if the call fills it.  CTA 0 then
 // writes the rows that stay in the tail, which are all new: the tail's old rows, if the page was
 // filled, are read before.  Bound by the issue of its arithmetic for prompts (some 20 instructions a value of 2
-// bytes read and 1 written: 4 prompts of 400 to 4000 tokens, 8 heads of 128, take 31 us where the
+// bytes read and 1 written: 4 prompts of 2500 to 4000 tokens, 8 heads of 128, take 31 us where the
 // bytes alone would take 12) and by the chain length, table, row for a token (3.1 us for 8 sequences).
 template <typename T, int kVecs>
 __global__ void __launch_bounds__(kPageThreads) paged_append_kernel(const PagedAppendArgs a) {

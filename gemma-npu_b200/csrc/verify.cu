@@ -26,12 +26,13 @@
 // After k rejections w is max(p - c q, 0) / Z with one c: of max(p - c q, 0) / Z less q, what is
 // positive is max(p - (c + Z) q, 0).  So nothing is stored: a node's first rejection costs one pass over
 // both rows, which gives Z, and by warps' chunks what the draw then needs to find its token; a further
-// one takes off what the larger c drops, in 64 bits only for the values that may be (24 trees 197 ->
-// 164 us; one chain, which never gets there, 25 -> 26).
+// one takes off what the larger c drops, in 64 bits only for the values that may be (looking at all of them
+// again took 24 trees 33 us longer).
 //
 // What bounds it: the 64-bit operations of the passes (an SM has 62 a clock) and, for short walks, the
-// chain of a node (its children, a pass, two meetings of the cluster: some 4 us).  One chain of 5 drafts
-// over 262144 values takes 26 us; 24 trees take 164, as long as their longest walk.
+// chain of a node (its children, a pass, two meetings of the cluster: some 5 us).  One chain of 5 drafts
+// over 262144 values takes 22 to 46 us by the draw, 24 trees 135 to 169, as long as their longest walk.  A
+// node's statistics do not depend on the walk: a pass over all nodes at once, on all SMs, is not built.
 #include "common.cuh"
 
 #include <cuda_fp16.h>

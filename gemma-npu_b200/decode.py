@@ -219,7 +219,8 @@ def paged_append(k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_n
     They wait in the tail as they are; a page that becomes full is rounded to 8 bits at once, per
     head: scale = m / 127 for its largest magnitude m, values round(127 x / m), halves to even.  A
     page with an infinity or a NaN gets a scale of NaN.  The page must be in the table
-    (`page_assign`), and there only once: one that is not is lost and reported by `device_status`.
+    (`page_assign`), and there only once: one that is not is lost and reported by `device_status`.  A
+    path's entry of N or more puts a row of zeros, which counts, and is reported too.
     Returns lens_out int32 [B] (a tensor apart from lens, path, count and table).  k_new and v_new must not overlap the
     cache."""
     return (_binding or _c()).paged_append(k, v, k_scale, v_scale, k_tail, v_tail, table, lens, k_new, v_new, path,
@@ -239,8 +240,10 @@ def draft_verify(logits, tokens, uniform, parent=None, draft=None, temperature=1
     c stands if uniform[b, c] * q(its token) < w(its token), w = p at first, and if not w becomes
     max(w - q, 0) over its sum.  draft=None: the drafts were chosen, not sampled, q is 1 at the
     child's token.  From the last node that stands the token is drawn from w, the first whose
-    running sum exceeds uniform[b, 0] of the whole.  uniform fp32 [B, N] in [0, 1).  The tokens then
-    have the target's distribution, whatever the drafts.
+    running sum exceeds uniform[b, 0] of the whole.  uniform fp32 [B, N] in [0, 1).  Without `draft` the
+    tokens then have the target's distribution, whatever the drafts; with it, where a node's children
+    are independent draws from its q (the same token may be drawn twice), not its likeliest tokens or draws
+    without replacement: those are chosen drafts.
 
     temperature=0 (else 1e-3 to 1e3): a child stands if it is the largest logit (equal ones: the
     lowest token), which is also the token after the last; uniform may be None.  A logit of -inf

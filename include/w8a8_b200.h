@@ -465,7 +465,8 @@ typedef struct w8_paged_append_args {
  * becomes full gets scale = m / 127 (m its head's largest magnitude) and round(127 x / m),
  * halves to even, from the 16-bit rows; the rows behind the last full page go into the tail.  A
  * page with an infinity or a NaN gets a scale of NaN.  A page that the table does not have is lost
- * and reported by w8_device_status, and so are positions behind the table.  The new rows must not
+ * and reported by w8_device_status, and so are positions behind the table; for a path's index of n_new
+ * or more a row of zeros is put, and reported.  The new rows must not
  * overlap the pages and tails, and a page that the call fills may stand in the table only once. */
 int w8_paged_append(const w8_paged_append_args* args, w8_stream_t stream);
 
@@ -511,7 +512,7 @@ typedef struct w8_draft_verify_args {
  *   c stands if uniform[c] q_i(t_c) < w(t_c);  else w = max(w - q_i, 0) over its sum
  * (unchanged if nothing is left), and the walk goes on from the child that stands.  Where none
  * does, token is the first t with sum_{v <= t} w(v) > uniform[0] sum_v w(v).  Probabilities and
- * sums that decide a token are held in 64 bits.  At temperature 0 a child stands if its token is
+ * sums that decide a token are held in 64 bits; fp32 ones decide where their error cannot matter.  At temperature 0 a child stands if its token is
  * the largest logit's, the lowest of equal ones, and token is the last node's largest.  A logit of
  * -inf is an impossible token.  A node whose target row has a NaN or no finite largest logit ends
  * the walk with token -1; one whose draft row has none keeps no child.  At most 1024 nodes; a
