@@ -132,7 +132,7 @@ __device__ __forceinline__ double exp2_64(double t, const double* table) {
 // at a temperature of 1e-3.  The largest logit's weight is 1 in fp32 and (to 2^-52 of ref) in 64 bits.
 struct VerifyRow {
   float top, least;  // the largest logit (level, with a cap); the logit 1000 levels below it, less than which counts as 0
-  double ref, out;   // levels a logit (no cap)
+  double ref, out;   // its level in 64 bits; levels a logit (no cap)
   double sum;
   bool fine;  // the row has a finite largest logit and no NaN
 };
@@ -161,7 +161,7 @@ __device__ __forceinline__ double weight_64(float x, const VerifyScale& c, const
     double t = fma(-c.twice, r, c.out - row.ref);
     none = x == -INFINITY;
     if constexpr (kCapped == kWideCap) {
-      // The exponential's 2^-48 moves a level by up to 2^-49 of their range: of 2^31 levels that is 4e-6.
+      // The exponential's 2^-48 moves a level by up to 2^-49 of their range: of 2^31 levels that is 4e-6 of one.
       if (c.out > 65536.0) t = fma(c.out, tanh_64(static_cast<double>(xc) * c.per_cap), -row.ref);
       none = none || t < -1000.0;
       t = fmax(t, -1000.0);
@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(kVerifyThreads) draft_verify_greedy_kernel(con
 }
 
 // ---------------------------------------------------------------- sampling
-// (Without draft logits two CTAs fit an SM, so that clusters may be larger: 16 chains of 6 in 39 us where one
-// CTA an SM, without the spills, takes 53.)
+// (Without draft logits two CTAs fit an SM, so that clusters may be larger: 16 chains of 6 in 35 us where one
+// CTA an SM, without the spills, takes 44.)
 template <typename E, int kCapped, bool kDraft>
 __global__ void __launch_bounds__(kVerifyThreads, kDraft || kCapped == kWideCap ? 1 : 2) draft_verify_kernel(const VerifyArgs a) {
   __shared__ VerifyTree tree;
