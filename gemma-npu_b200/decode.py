@@ -240,10 +240,13 @@ def draft_verify(logits, tokens, uniform, parent=None, draft=None, temperature=1
     c stands if uniform[b, c] * q(its token) < w(its token), w = p at first, and if not w becomes
     max(w - q, 0) over its sum.  draft=None: the drafts were chosen, not sampled, q is 1 at the
     child's token.  From the last node that stands the token is drawn from w, the first whose
-    running sum exceeds uniform[b, 0] of the whole.  uniform fp32 [B, N] in [0, 1).  Without `draft` the
-    tokens then have the target's distribution, whatever the drafts; with it, where a node's children
-    are independent draws from its q (the same token may be drawn twice), not its likeliest tokens or draws
-    without replacement: those are chosen drafts.
+    running sum exceeds uniform[b, 0] of the whole.  uniform fp32 [B, N] in [0, 1).  All this in 64
+    bits: w stays as it is where rejections would leave less than 1e-13 of p, and weights below
+    2^-1000 of a row's largest count as 0.
+
+    The tokens then have the target's distribution: without `draft` whatever the drafts, with it if
+    a node's children are independent draws from its q (the same token may be drawn twice).  The
+    draft model's likeliest tokens, or draws without replacement, are chosen drafts.
 
     temperature=0 (else 1e-3 to 1e3): a child stands if it is the largest logit (equal ones: the
     lowest token), which is also the token after the last; uniform may be None.  A logit of -inf

@@ -506,17 +506,21 @@ typedef struct w8_draft_verify_args {
   double temperature, cap;            /* 0: greedy, the largest logit; cap 0: none */
 } w8_draft_verify_args;
 
-/* Speculative sampling over a drafted tree.  With p_i = softmax(y / temperature) of node i's
- * logits, y = cap tanh(logit / cap), and q_i = softmax(draft logits / temperature) (without draft
- * logits 1 at the child's token), from node 0: node i's children c in order, w = p_i,
+/* Speculative sampling over a drafted tree.  With p_i = softmax(y / temperature) of node
+ * i's logits, y = cap tanh(logit / cap), and q_i = softmax(draft logits / temperature)
+ * (without draft logits 1 at the child's token), from node 0: node i's children c in order,
+ * w = p_i,
  *   c stands if uniform[c] q_i(t_c) < w(t_c);  else w = max(w - q_i, 0) over its sum
- * (unchanged if nothing is left), and the walk goes on from the child that stands.  Where none
- * does, token is the first t with sum_{v <= t} w(v) > uniform[0] sum_v w(v).  Probabilities and
- * sums that decide a token are held in 64 bits; fp32 ones decide where their error cannot matter.  At temperature 0 a child stands if its token is
- * the largest logit's, the lowest of equal ones, and token is the last node's largest.  A logit of
- * -inf is an impossible token.  A node whose target row has a NaN or no finite largest logit ends
- * the walk with token -1; one whose draft row has none keeps no child.  At most 1024 nodes; a
- * token out of range does not stand and is reported by w8_device_status. */
+ * (unchanged if what rejections leave of p_i is below 1e-13 of it, which 64 bits cannot
+ * tell from nothing; a weight 2^-1000 of a row's largest counts as 0), and the walk goes on
+ * from the child that stands.  Where none does, token is the first t with sum_{v <= t} w(v)
+ * > uniform[0] sum_v w(v).  Probabilities and sums that decide a token are held in 64 bits;
+ * fp32 ones decide where their error cannot matter.  At temperature 0 a child stands if its
+ * token is the largest logit's, the lowest of equal ones, and token is the last node's
+ * largest.  A logit of -inf is an impossible token.  A node whose target row has a NaN or
+ * no finite largest logit ends the walk with token -1; one whose draft row has none keeps
+ * no child.  At most 1024 nodes; a token out of range does not stand and is reported by
+ * w8_device_status. */
 int w8_draft_verify(const w8_draft_verify_args* args, w8_stream_t stream);
 
 /* ---- quantisation ------------------------------------------------------ */
